@@ -39,6 +39,10 @@ extern "C" {
 #define LLMOPS_CACHE_F32 0
 #define LLMOPS_CACHE_F16 1
 
+#define LLMOPS_F32 0
+#define LLMOPS_F16 1
+#define LLMOPS_BF16 2
+
 typedef void* llmops_stream_t;
 
 const char* llmops_last_error(void);
@@ -269,6 +273,66 @@ int llmops_attention_rope_decode_records(float* q, float* k, const float* v, int
                                          int64_t planes, int64_t maxlen, const int32_t* slot, int position_id,
                                          const int32_t* position_id_dev, int layer_id, float* rec_stats, float* rec_outs,
                                          void* workspace, size_t workspace_bytes, llmops_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Several requests in step.  No counterparts in the reference, which answers one chat at a time.  Their workspaces need no
+ * zeroes and hold nothing between calls; calls that can overlap need one each.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Attention of B sequences that share a prefix: its keys and values are held once, and read once for all of them.
+ * Sequence b has n[b] = lengths[b] rows of its own in kv_cache [planes,B,Hkv,maxlen,S] and brings t[b] new tokens, t[b] = qL or,
+ * with q_lens, q_lens[b] of the qL; token l < t[b] has position prefix_len + n[b] + l.  Its k (rotated) and v go to row n[b] + l, and
+ *   out[b,l] = softmax(rot(q).K^T / sqrt(S)) . V over rows 0 .. prefix_len-1 of prefix_cache [prefix_planes,1,Hkv,prefix_maxlen,S] and
+ * rows 0 .. n[b]+l of its own; head h reads kv head h / (H / Hkv).  Planes 2*layer_id and 2*layer_id+1 of both caches; both have the
+ * type cache_dtype (halves: k and v are rounded to them, the arithmetic is fp32).  The caller adds t[b] to lengths[b] when all layers
+ * are done, or less: rows past lengths[b] are not looked at, and the next call's tokens overwrite them.
+ *   lengths, q_lens are int32 [B] on the device (q_lens may be NULL: qL each), read by the kernels: a captured call serves every
+ * following step.  A length outside 0 .. maxlen counts as the nearer of the two, and new tokens that do not fit the cache count as
+ * padding.  Padding (l >= t[b]) is not cached, and its out is 0.
+ *   q [B,qL,H*S], k and v [B,qL,Hkv*S] fp32, token l of sequence b at + b*stride_b + l*stride_l elements (multiples of 4: columns of a
+ * projection's output will do), unchanged; out [B,qL,H*S] dense.  inv_freq [half], 2*half <= S: as llmops_rope_embed, but the angle
+ * inv_freq * position keeps the product's rounding error, which fp32 loses (1e-4 at position 4000).  S == 128; 16-byte aligned
+ * pointers, 256-byte aligned workspace; prefix_len + maxlen <= 2^24.  prefix_len may be 0 (prefix_cache may then be NULL).
+ * prefix_cache and kv_cache must not overlap.
+ * Results agree with fp32 evaluation to about 1e-6 of the largest output, and are the same bits in every call. */
+size_t llmops_attention_prefix_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t prefix_len, int64_t maxlen);
+int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b,
+                                 int64_t k_stride_l, const float* v, int64_t v_stride_b, int64_t v_stride_l, int64_t B, int64_t qL,
+                                 int64_t H, int64_t Hkv, int64_t S, const float* inv_freq, int64_t half, const void* prefix_cache,
+                                 int64_t prefix_planes, int64_t prefix_maxlen, int64_t prefix_len, void* kv_cache, int cache_dtype,
+                                 int64_t planes, int64_t maxlen, const int32_t* lengths, const int32_t* q_lens, int layer_id, float* out,
+                                 void* workspace, size_t workspace_bytes, llmops_stream_t stream);
+
+/* Low-rank adapters beside a projection K -> N (llmops_fc_Q4A): out[b,l] = y[b,l] + scales[a] * (x[b,l] A_a^T) B_a^T, a = ids[b].
+ * lora_A [adapters,R,K] and lora_B [adapters,N,R], dense, of weight_dtype (LLMOPS_F32, _F16, _BF16); scales fp32 [adapters] and ids
+ * int32 [batch] on the device.  An id outside 0 .. adapters-1 (-1) is none: out = y.  Adapters of a lower rank than R are padded with
+ * zeros.  x [batch,tokens,K], y and out [batch,tokens,N] fp32, token l of sequence b at + b*stride_b + l*stride_l elements; out may be y
+ * (the same pointer and strides) and must not overlap x or y otherwise.  Up to 1048560 tokens in all, R up to 4096.  Sizes and
+ * strides are free; 16-byte aligned rows (K, R multiples of 8, strides of 4) are read 16 bytes at a time.
+ * fp32 arithmetic, except that products are formed of exact bf16 pieces: what is dropped is below 2^-22 of a product. */
+size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R);
+int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, const float* x, int64_t x_stride_b, int64_t x_stride_l,
+                    int64_t batch, int64_t tokens, int64_t N, int64_t K, const void* lora_A, const void* lora_B, int weight_dtype, int64_t R,
+                    int64_t adapters, const int32_t* ids, const float* scales, float* out, int64_t out_stride_b, int64_t out_stride_l,
+                    void* workspace, size_t workspace_bytes, llmops_stream_t stream);
+
+/* Up to K drafted tokens of each of B sequences against the model's logits fp32 [B,K+1,V] (dense; row i: behind i drafts), and the
+ * token behind those accepted.  p_i = softmax(logits[b,i] / T), T = temperature[b] (fp32 [B]; NULL: one_temperature).
+ *   draft x_i = drafts[b,i] (int64 [B,K]) is accepted while  uniforms[b,i] * q_i(x_i) < p_i(x_i),  q_i = draft_probs[b,i] (fp32 [B,K,V],
+ *   what it was drawn from), or 1 for all with draft_probs NULL (drafts that come from no distribution);
+ *   the next token is the smallest j whose running sum of r is above uniforms[b,K] * (sum of r): r = max(p_i - q_i, 0) where draft i was
+ *   refused (draft_probs NULL: p_i without x_i), r = p_i behind the last draft.  A sum of r that is 0 stands for r = p_i.
+ * T not above 0: the likeliest token (the lowest of equals), and drafts are accepted while they are it.  draft_lens int32 [B] (NULL: K
+ * each; held to 0 .. K): the sequence's drafts.  K may be 0: the next token is drawn.  Drafts outside 0 .. V-1 are refused.
+ * uniforms fp32 [B,K+1], in [0, 1): [b,K] draws the next token.
+ * tokens int64 [B,K+1]: the accepted drafts, the next token, -1 behind; accepted int32 [B]: how many drafts.
+ * Logits that are NaN or minus infinity weigh nothing, equal plus infinities share the row; a row without any other logit gives -1.
+ * Exponentials and sums are in 64 bits: the answer is the definition's but for numbers within about 1e-14 of a border.
+ * B*(K+1) < 2^24, V <= 2^27. */
+size_t llmops_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
+int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, int64_t V, const int64_t* drafts, const float* draft_probs,
+                         const float* uniforms, const float* temperature, float one_temperature, const int32_t* draft_lens, int64_t* tokens,
+                         int32_t* accepted, void* workspace, size_t workspace_bytes, llmops_stream_t stream);
 
 /* softmax (ops/op_misc.hpp:183-194, ops/utils.hpp:484-490): in place over rows of length K */
 int llmops_softmax(float* x, int64_t rows, int64_t K, llmops_stream_t stream);

@@ -1,0 +1,793 @@
+// Attention of a batch whose sequences share a long prefix: the prefix's keys and values are held once and read once for all
+// of the batch's queries; behind it every sequence has rows of its own.  (Beside attention_rope2 of attn.hip, whose cache
+// belongs to one batch row from the first token on.)
+//
+// For sequence b with len[b] own rows and n[b] new tokens, token l < n[b], head h on kv head h / G, G = H / Hkv:
+//   pos = P + len[b] + l,  q' = rot(q, pos),  own row len[b] + l = (rot(k, pos), v) in the cache's type,
+//   out = sum_r e_r V_r / sum_r e_r,  e_r = exp(q' . K_r / sqrt(S) - max),  r over the P prefix rows and own rows 0 .. len[b] + l.
+//
+//   1. prefix_prep_kernel   rotates, writes the new cache rows and leaves q' as operands of the matrix instructions
+//   2. prefix_attn_kernel   softmax(q'K^T)V of a piece of the rows for a tile of queries: running maximum and sum, one pass
+//   3. prefix_merge_kernel  joins the pieces of a query
+//
+// Queries of a kv head are numbered m = (b*qL + l)*G + g, so that the queries that see the prefix, those of all sequences, and
+// those of one sequence are both runs of m.  Rows are numbered through: r < P is the prefix's, P + i is the sequence's own row i.
+//
+// Arithmetic.  Products run on the fp16 matrix cores (v_mfma_f32_16x16x32_f16, fp32 sums) with fp32 values carried as two halves:
+//   q'  scaled by a power of two of its row so that its largest value is in [2^13, 2^14): hi + lo, 22 bits of that
+//   K,V hi + lo / 2048, hi truncated and lo = (x - hi) * 2048 in a half: 21 bits of x from 2^-14 on, 2^-36 below (a cache of
+//       halves is hi alone)
+//   e   times 2^14: hi + lo, so that weights down to 2^-28 of the largest keep their bits
+// A product is hi*hi + lo*hi + hi*lo/2048; what is dropped is below 2^-21 of it.  Values outside the halves' range, infinities
+// and NaN are seen while a tile is cut up; such a tile is multiplied on the vector ALU in full width instead, row by row of those
+// that a query sees, so that what a mask hides has no effect whatever it holds.
+#include <float.h>
+
+#include "common.h"
+#include "gemv_device.h"
+
+namespace llmops {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+
+constexpr int kS = 128;
+constexpr float kLift = 14.0f;  // weights are exp2(.. + kLift)
+
+struct PrefixArgs {
+    _Float16 *qh, *ql;                  // [Hkv][M][128]
+    float* cq;                          // [Hkv][M]: score = cq * (q' . k), in units of log2
+    const void *pk, *pv, *ok, *ov;      // [Hkv][pmax][128], [B][Hkv][maxlen][128]
+    const int32_t *lengths, *q_lens;    // [B]; q_lens may be null
+    float* rec_out;                     // [Hkv*M][nrec][128]
+    float2* rec_stat;                   // [Hkv*M][nrec]: max (log2), sum
+    float* out;                         // [B][qL][H*128]
+    int64_t pmax, maxlen;
+    int B, qL, G, Hkv, P, M, Mq;        // M = B*qL*G, Mq = qL*G
+    int ptiles, ppieces, prows;         // prefix: tiles of queries, pieces of rows, rows of a piece
+    int otiles, opieces;                // own rows (or all rows): tiles of a sequence's queries, pieces
+    int nrec;
+    unsigned pitems;
+};
+
+// rows that sequence b has and new tokens that it brings; what does not fit the cache counts as padding
+__device__ __forceinline__ void own_extent(const int32_t* __restrict__ lengths, const int32_t* __restrict__ q_lens, int b, int qL, int64_t maxlen,
+                                           int& len, int& n) {
+    len = (int)max((int64_t)0, min((int64_t)lengths[b], maxlen));
+    const int want = q_lens != nullptr ? min(q_lens[b], qL) : qL;
+    n = (int)max((int64_t)0, min((int64_t)want, maxlen - len));
+}
+
+// ---- 1. rotation, cache rows, operands ----
+// cos and sin of inv_freq * pos with the product's rounding put back (at position 4000 it is 1.2e-4 of an angle)
+__device__ __forceinline__ void turn_of(float f, int pos, float& c, float& s) {
+    const float p = (float)pos, hi = f * p, lo = fmaf(f, p, -hi);
+    float s0, c0;
+    sincosf(hi, &s0, &c0);
+    c = fmaf(-lo, s0, c0);
+    s = fmaf(lo, c0, s0);
+}
+
+__device__ __forceinline__ void store_row4(float* dst, const float* v) { *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store_row4(__half* dst, const float* v) {
+    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+    uint2 u;
+    u.x = *reinterpret_cast<const uint32_t*>(&a);
+    u.y = *reinterpret_cast<const uint32_t*>(&b);
+    *reinterpret_cast<uint2*>(dst) = u;
+}
+
+struct PrepArgs {
+    const float *q, *k, *v, *inv_freq;
+    int64_t qsb, qsl, ksb, ksl, vsb, vsl;
+    int half, groups;
+};
+
+// A workgroup per token and 16 of its H + 2*Hkv rows of 128, 16 lanes to a row, dims 4i .. +3 and 64 + 4i .. +3 to lane i.
+// Bound by latency at few tokens and by memory at many.
+template <typename T>
+__global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a, PrepArgs p) {
+    __shared__ float turn[2][64];
+    const int bl = blockIdx.x / p.groups, group = blockIdx.x - bl * p.groups, b = bl / a.qL, l = bl - b * a.qL;
+    int len, n;
+    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    const bool live = l < n;
+    if (live && (int)threadIdx.x < p.half) turn_of(p.inv_freq[threadIdx.x], a.P + len + l, turn[0][threadIdx.x], turn[1][threadIdx.x]);
+    __syncthreads();
+    const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), i4 = 4 * (threadIdx.x & 15);
+    if (row >= H + 2 * a.Hkv) return;
+    const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv;
+    if (!live && !is_q) return;
+    const float* src = is_q ? p.q + b * p.qsb + l * p.qsl + (int64_t)row * kS
+                            : is_k ? p.k + b * p.ksb + l * p.ksl + (int64_t)(row - H) * kS : p.v + b * p.vsb + l * p.vsl + (int64_t)(row - H - a.Hkv) * kS;
+    float x[8];
+    {
+        const float4 lo = *reinterpret_cast<const float4*>(src + i4), hi = *reinterpret_cast<const float4*>(src + 64 + i4);
+        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+    }
+    if (is_q || is_k) {
+        if (live && p.half == 64) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float c = turn[0][i4 + e], s = turn[1][i4 + e], x0 = x[e], x1 = x[4 + e];
+                x[e] = c * x0 - s * x1;
+                x[4 + e] = s * x0 + c * x1;
+            }
+        } else if (live) {  // pairs (d, d + half), the other dims as they are
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int d = (e < 4 ? i4 : 60 + i4) + e;
+                if (d < p.half) x[e] = turn[0][d] * x[e] - turn[1][d] * src[d + p.half];
+                else if (d < 2 * p.half) x[e] = turn[1][d - p.half] * src[d - p.half] + turn[0][d - p.half] * x[e];
+            }
+        }
+    }
+    if (!is_q) {
+        const int hk = is_k ? row - H : row - H - a.Hkv;
+        T* dst = reinterpret_cast<T*>(const_cast<void*>(is_k ? a.ok : a.ov)) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kS;
+        store_row4(dst + i4, x);
+        store_row4(dst + 64 + i4, x + 4);
+        return;
+    }
+    const int64_t m = (int64_t)(row / a.G) * a.M + (int64_t)bl * a.G + row % a.G;
+    float top = 0.0f;
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e])), fine &= fabsf(x[e]) <= FLT_MAX;
+    float bad = fine ? 0.0f : 1.0f;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64)), bad = fmaxf(bad, __shfl_xor(bad, o, 64));
+    const bool use = live && bad == 0.0f && top > 0.0f;
+    const int e2 = use ? 13 - ilogbf(top) : 0;
+    v8h hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float y = use ? ldexpf(x[e], e2) : 0.0f;
+        hi[e] = (_Float16)y;
+        lo[e] = (_Float16)(y - (float)hi[e]);
+    }
+    const uint4 h = *reinterpret_cast<const uint4*>(&hi), w = *reinterpret_cast<const uint4*>(&lo);
+    *reinterpret_cast<uint2*>(a.qh + m * kS + i4) = make_uint2(h.x, h.y);
+    *reinterpret_cast<uint2*>(a.qh + m * kS + 64 + i4) = make_uint2(h.z, h.w);
+    *reinterpret_cast<uint2*>(a.ql + m * kS + i4) = make_uint2(w.x, w.y);
+    *reinterpret_cast<uint2*>(a.ql + m * kS + 64 + i4) = make_uint2(w.z, w.w);
+    // (a query that holds an infinity or NaN has no score that is a number)
+    if ((threadIdx.x & 15) == 0) a.cq[m] = live && bad != 0.0f ? NAN : ldexpf(1.44269504f * 0.08838834764831845f, -e2);
+}
+
+// ---- 2. a piece of the rows for a tile of queries ----
+// Lanes of v_mfma_f32_16x16x32_f16: operand A row lane % 16, B column lane % 16, eight k-values 8 * (lane / 16) .. +7 of either;
+// result column lane % 16, rows 4 * (lane / 16) + v.  With g = lane / 16 and i = lane % 16, 32 cache rows from t on:
+//   S^T = K Q^T   A: rows t + 16*tt + i, dims 32*step + 8*g .. +7.  B: query i.  Result: query i, rows t + 16*tt + 4*g + v.
+//   O^T = V^T e^T k-value j of lane group g stands for row t + 16*(j/4) + 4*g + j%4, so that B is the scores as they lie.
+//                 A: column 64*(c/4) + 4*i + c%4 of product c, so that a lane's rows are loaded 16 bytes at a time.
+//                 Result of product c: query i, dim 64*(c/4) + 16*g + 4*v + c%4.
+// K or V of one head, rows 0 .. end: a run of the prefix or of a sequence's own
+template <typename T>
+struct Rows {
+    const T* p;
+    int end;
+    // 32 rows from t on (the same t in the whole wave) as a descriptor that ends with the run: rows behind read as zero
+    __device__ __forceinline__ buffer_rsrc from(int t) const {
+        return make_rsrc(p + (int64_t)t * kS, (uint32_t)__builtin_amdgcn_readfirstlane(max(0, min(32, end - t))) * (uint32_t)(kS * sizeof(T)));
+    }
+    __device__ __forceinline__ const T* at(int r) const { return p + (int64_t)min(r, end - 1) * kS; }
+};
+
+struct Halves {
+    v8h hi, lo;
+};
+__device__ __forceinline__ uint32_t cut2(float x, float y, uint32_t& lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+    const v2h hv = *reinterpret_cast<const v2h*>(&h);
+    v2h l;
+    l[0] = (_Float16)fmaf((float)hv[0], -2048.0f, x * 2048.0f);
+    l[1] = (_Float16)fmaf((float)hv[1], -2048.0f, y * 2048.0f);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// largest magnitude of the halves seen so far, as bits (NaN above infinity above all else)
+__device__ __forceinline__ void note(v2us& top, uint32_t halves) {
+    const uint32_t u = halves & 0x7fff7fffu;
+    top = __builtin_elementwise_max(top, *reinterpret_cast<const v2us*>(&u));
+}
+__device__ __forceinline__ void note4(v2us& top, uint4 h) {
+    note(top, h.x), note(top, h.y), note(top, h.z), note(top, h.w);
+    asm volatile("" : "+v"(top));  // here and now: put off to the loop's end, a tile's 64 operands stay in registers till then
+}
+// What was seen of K or V: 2 if there are values outside the halves' range (fp32 values that truncate to the largest half, infinities,
+// NaN), 1 if there are some in their normal range; 0 if all are below 2^-14, where the low halves no longer hold 21 bits of the largest
+template <typename T>
+__device__ __forceinline__ int range_of(v2us top) {
+    const unsigned short most = top[0] > top[1] ? top[0] : top[1];
+    return sizeof(T) == 4 ? (most >= 0x7bff ? 2 : most >= 0x0400 ? 1 : 0) : most >= 0x7c00 ? 2 : 1;
+}
+
+__device__ __forceinline__ v8h as_v8h(uint4 u) { return *reinterpret_cast<const v8h*>(&u); }
+__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ float value(const float* p) { return *p; }
+__device__ __forceinline__ float value(const __half* p) { return __half2float(*p); }
+
+// queries 16*rt + lane % 16 of a wave: factor, running maximum (log2), this lane's part of the sum, O^T
+template <int RT>
+struct Queries {
+    float c[RT], m[RT], l[RT];
+    int see[RT];  // rows below this one are seen
+    v4f o[RT][8];
+    __device__ __forceinline__ void start(const PrefixArgs& a, int hk, int m0, int m_end, int i) {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            c[rt] = a.cq[(int64_t)hk * a.M + min(m0 + 16 * rt + i, m_end - 1)];
+            m[rt] = -INFINITY;
+            l[rt] = 0.0f;
+#pragma unroll
+            for (int c8 = 0; c8 < 8; c8++) o[rt][c8] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+};
+// their operands: in registers for sixteen queries, in LDS for more (the four waves share them)
+template <int RT>
+struct QueryOps;
+template <>
+struct QueryOps<1> {
+    v8h h[4], l[4];
+    __device__ __forceinline__ void load(const PrefixArgs& a, uint4*, int hk, int m0, int m_end, int lane) {
+        const int64_t at = ((int64_t)hk * a.M + min(m0 + (lane & 15), m_end - 1)) * kS + 8 * (lane >> 4);
+#pragma unroll
+        for (int step = 0; step < 4; step++) {
+            h[step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + at + 32 * step));
+            l[step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + at + 32 * step));
+        }
+    }
+    __device__ __forceinline__ v8h hi(int, int step) const { return h[step]; }
+    __device__ __forceinline__ v8h lo(int, int step) const { return l[step]; }
+};
+template <>
+struct QueryOps<2> {
+    const uint4* mine;
+    __device__ __forceinline__ void load(const PrefixArgs& a, uint4* lds, int hk, int m0, int m_end, int lane) {
+        const int wave = threadIdx.x >> 6;  // a step to a wave
+#pragma unroll
+        for (int rt = 0; rt < 2; rt++) {
+            const int64_t at = ((int64_t)hk * a.M + min(m0 + 16 * rt + (lane & 15), m_end - 1)) * kS + 8 * (lane >> 4) + 32 * wave;
+            lds[(rt * 8 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.qh + at);
+            lds[(rt * 8 + 4 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.ql + at);
+        }
+        mine = lds + lane;
+        __syncthreads();
+    }
+    __device__ __forceinline__ v8h hi(int rt, int step) const { return as_v8h(mine[(rt * 8 + step) * 64]); }
+    __device__ __forceinline__ v8h lo(int rt, int step) const { return as_v8h(mine[(rt * 8 + 4 + step) * 64]); }
+};
+
+// S^T of 16 rows, one step; `low` collects what the low halves of K add, times 2048
+template <typename T>
+__device__ __forceinline__ void score_step(v4f& acc, v4f& low, const Halves& k, v8h qh, v8h ql) {
+    acc = mfma(k.hi, qh, acc);
+    if constexpr (sizeof(T) == 4) low = mfma(k.lo, qh, low);
+    acc = mfma(k.hi, ql, acc);
+}
+
+// scores to weights: the running maximum, the sum, and what the sums so far shrink by.  sc[tt]: rows t + 16*tt + 4*g + v
+template <int RT>
+__device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[2], int t, int g, bool masked) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            float x = sc[tt][v] * s.c[rt];
+            if (masked) x = t + 16 * tt + 4 * g + v < s.see[rt] ? x : -INFINITY;
+            sc[tt][v] = x;
+            top = fmaxf(top, x);
+        }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any(top > s.m[rt])) {
+        const float m = fmaxf(s.m[rt], top), shrink = s.m[rt] == m ? 1.0f : __builtin_amdgcn_exp2f(s.m[rt] - m);
+        s.m[rt] = m;
+        s.l[rt] *= shrink;
+#pragma unroll
+        for (int c = 0; c < 8; c++) s.o[rt][c] *= shrink;
+    }
+    const float base = s.m[rt] == -INFINITY ? 0.0f : s.m[rt] - kLift;  // (nothing seen yet: every weight is exp2(-inf) = 0)
+#pragma unroll
+    for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            sc[tt][v] = __builtin_amdgcn_exp2f(sc[tt][v] - base);
+            s.l[rt] += sc[tt][v];
+        }
+}
+
+// the weights of 32 rows as operands: hi, lo, hi / 2048
+struct Weights {
+    v8h hi, lo, low;
+};
+template <typename T>
+__device__ __forceinline__ Weights weights_of(const v4f (&sc)[2]) {
+    Weights w;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        w.hi[j] = (_Float16)sc[j >> 2][j & 3];
+        w.lo[j] = (_Float16)(sc[j >> 2][j & 3] - (float)w.hi[j]);
+    }
+    if constexpr (sizeof(T) == 4) w.low = w.hi * (_Float16)(1.0f / 2048.0f);
+    return w;
+}
+template <typename T>
+__device__ __forceinline__ v4f add_rows(v4f o, const Halves& v, const Weights& w) {
+    o = mfma(v.hi, w.hi, o);
+    o = mfma(v.hi, w.lo, o);
+    if constexpr (sizeof(T) == 4) o = mfma(v.lo, w.low, o);
+    return o;
+}
+
+// the row below which query m of sequence b sees its own rows
+__device__ __forceinline__ int rows_seen(const PrefixArgs& a, int m, int b, int len, int n) {
+    const int l = (m - b * a.Mq) / a.G;
+    return l < n ? len + l + 1 : 0;
+}
+
+// The same in full width, for rows that hold values outside the halves' range: the workgroup starts again, a wave to a query and
+// two dims to a lane, only the rows that the query sees, in up to two runs (prefix, own).  Slow, and not met in a model's caches.
+template <typename T>
+__device__ __forceinline__ void full_width(const PrefixArgs& a, int hk, int m0, int m_end, Rows<T> K0, Rows<T> V0, int from0, Rows<T> K1, Rows<T> V1, int from1,
+                                           bool own, int b, int len, int n, int piece) {
+    const int lane = threadIdx.x & 63, d = 2 * lane;
+#pragma unroll 1
+    for (int m = m0 + (threadIdx.x >> 6); m < m_end; m += 4) {
+        const int64_t at = ((int64_t)hk * a.M + m) * kS + d;
+        const double q0 = (double)(float)a.qh[at] + (double)(float)a.ql[at], q1 = (double)(float)a.qh[at + 1] + (double)(float)a.ql[at + 1];
+        const double c = (double)a.cq[(int64_t)hk * a.M + m];
+        const int see = own ? rows_seen(a, m, b, len, n) : 0;
+        float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll 1
+        for (int run = 0; run < 2; run++) {
+            const T* k = run ? K1.p : K0.p;
+            const T* v = run ? V1.p : V0.p;
+            const int end = run ? min(K1.end, see) : see > 0 || !own ? K0.end : 0;
+#pragma unroll 1
+            for (int r = run ? from1 : from0; r < end; r++) {
+                double x = q0 * (double)value(k + (int64_t)r * kS + d) + q1 * (double)value(k + (int64_t)r * kS + d + 1);
+#pragma unroll
+                for (int w = 32; w > 0; w >>= 1) x += __shfl_xor(x, w, 64);
+                const float s = (float)(x * c), up = fmaxf(top, s), shrink = top == up ? 1.0f : __builtin_amdgcn_exp2f(top - up);
+                const float e = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - up + kLift);
+                top = up;
+                sum = fmaf(sum, shrink, e);
+                o0 = fmaf(e, value(v + (int64_t)r * kS + d), o0 * shrink);
+                o1 = fmaf(e, value(v + (int64_t)r * kS + d + 1), o1 * shrink);
+            }
+        }
+        const int64_t rec = ((int64_t)hk * a.M + m) * a.nrec + piece;
+        if (lane == 0) a.rec_stat[rec] = make_float2(top, sum);
+        *reinterpret_cast<float2*>(a.rec_out + rec * kS + d) = make_float2(o0, o1);
+    }
+}
+
+// a wave's say, and the workgroup's decision
+template <typename T>
+__device__ __forceinline__ void note_range(v2us ktop, v2us vtop, int (&range)[2], int lane) {
+    const int k = range_of<T>(ktop), v = range_of<T>(vtop);
+    const int ks = __any(k == 2) ? 2 : __any(k == 1) ? 1 : 0, vs = __any(v == 2) ? 2 : __any(v == 1) ? 1 : 0;
+    if (lane == 0) range[0] = ks, range[1] = vs;
+}
+template <typename T>
+__device__ __forceinline__ bool all_zero(Rows<T> x, int from) {
+    int some = 0;
+    for (int64_t e = (int64_t)from * kS + threadIdx.x; e < (int64_t)x.end * kS; e += 256) some |= value(x.p + e) != 0.0f;
+    return !__syncthreads_or(some);
+}
+template <typename T>
+__device__ __forceinline__ bool needs_full_width(const int (&range)[4][2], Rows<T> K, Rows<T> V, int from) {
+    const int k = max(max(range[0][0], range[1][0]), max(range[2][0], range[3][0])), v = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    return k == 2 || v == 2 || (k == 0 && !all_zero(K, from)) || (v == 0 && !all_zero(V, from));
+}
+
+// Few queries to a workgroup (16 * RT): bound by reading the rows.  The four waves take 32 rows each of every 128; operands come
+// straight from memory, K of the next rows asked for when K of these is used up, and so V; the waves' sums meet in LDS.
+constexpr int kMeetRow = 132;  // floats (16 queries' rows on different banks)
+struct MeetSmem {
+    float m[4][32], l[4][32];
+    int range[4][2];
+    union {
+        float o[4][16][kMeetRow];
+        uint4 q[16 * 64];
+    };
+};
+
+// `lane_at` is hidden from the compiler here so that it adds `at` where it loads, up to 4095 in the instruction, and does not keep
+// sixteen sums in registers
+__device__ __forceinline__ uint32_t unseen(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+__device__ __forceinline__ uint4 ask16(buffer_rsrc r, uint32_t lane_at, uint32_t at) {
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_at + at, 0, 0));
+}
+__device__ __forceinline__ uint2 ask8(buffer_rsrc r, uint32_t lane_at, uint32_t at) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_at + at, 0, 0));
+}
+
+template <typename T>
+struct RowRegs;
+template <>
+struct RowRegs<float> {
+    float4 k[2][4][2], v[8][2];
+    __device__ __forceinline__ void load_k(Rows<float> K, int t, int i, int g) {
+        const buffer_rsrc r = K.from(t);
+        const uint32_t mine = unseen((uint32_t)(i * kS + 8 * g) * 4);
+#pragma unroll
+        for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+            for (int step = 0; step < 4; step++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) k[tt][step][h] = __builtin_bit_cast(float4, ask16(r, mine, (16 * tt * kS + 32 * step + 4 * h) * 4));
+    }
+    __device__ __forceinline__ void load_v(Rows<float> V, int t, int i, int g) {
+        const buffer_rsrc r = V.from(t);
+        const uint32_t mine = unseen((uint32_t)(4 * g * kS + 4 * i) * 4);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) v[j][h] = __builtin_bit_cast(float4, ask16(r, mine, ((16 * (j >> 2) + (j & 3)) * kS + 64 * h) * 4));
+    }
+    __device__ __forceinline__ Halves k_op(int tt, int step, v2us& top) const {
+        const float4 x = k[tt][step][0], y = k[tt][step][1];
+        uint4 h, l;
+        h.x = cut2(x.x, x.y, l.x), h.y = cut2(x.z, x.w, l.y), h.z = cut2(y.x, y.y, l.z), h.w = cut2(y.z, y.w, l.w);
+        note4(top, h);
+        return {as_v8h(h), as_v8h(l)};
+    }
+    __device__ __forceinline__ Halves v_op(int c, v2us& top) const {
+        auto f = [&](int j) { return reinterpret_cast<const float*>(&v[j][c >> 2])[c & 3]; };
+        uint4 h, l;
+        h.x = cut2(f(0), f(1), l.x), h.y = cut2(f(2), f(3), l.y), h.z = cut2(f(4), f(5), l.z), h.w = cut2(f(6), f(7), l.w);
+        note4(top, h);
+        return {as_v8h(h), as_v8h(l)};
+    }
+};
+template <>
+struct RowRegs<__half> {
+    uint4 k[2][4];
+    uint2 v[8][2];
+    __device__ __forceinline__ void load_k(Rows<__half> K, int t, int i, int g) {
+        const buffer_rsrc r = K.from(t);
+        const uint32_t mine = unseen((uint32_t)(i * kS + 8 * g) * 2);
+#pragma unroll
+        for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+            for (int step = 0; step < 4; step++) k[tt][step] = ask16(r, mine, (16 * tt * kS + 32 * step) * 2);
+    }
+    __device__ __forceinline__ void load_v(Rows<__half> V, int t, int i, int g) {
+        const buffer_rsrc r = V.from(t);
+        const uint32_t mine = unseen((uint32_t)(4 * g * kS + 4 * i) * 2);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) v[j][h] = ask8(r, mine, ((16 * (j >> 2) + (j & 3)) * kS + 64 * h) * 2);
+    }
+    __device__ __forceinline__ Halves k_op(int tt, int step, v2us& top) const {
+        const uint4 h = k[tt][step];
+        note4(top, h);
+        return {as_v8h(h), v8h{}};
+    }
+    __device__ __forceinline__ Halves v_op(int c, v2us& top) const {
+        uint32_t h[4];
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const uint2 x = v[2 * p][c >> 2], y = v[2 * p + 1][c >> 2];
+            const uint32_t a = (c & 2) ? x.y : x.x, b = (c & 2) ? y.y : y.x;
+            h[p] = __builtin_amdgcn_perm(b, a, (c & 1) ? 0x07060302u : 0x05040100u);
+        }
+        const uint4 all = make_uint4(h[0], h[1], h[2], h[3]);
+        note4(top, all);
+        return {as_v8h(all), v8h{}};
+    }
+};
+
+template <typename T, int RT>
+__device__ __forceinline__ void few_queries(const PrefixArgs& a, Rows<T> K, Rows<T> V, int hk, int m0, int m_end, int r0, bool own, int b, int len,
+                                            int n, int piece, MeetSmem& sm) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    const int r1 = K.end;
+    if (r0 >= r1) {  // nothing here: say so
+        if ((int)threadIdx.x < 16 * RT && m0 + (int)threadIdx.x < m_end)
+            a.rec_stat[((int64_t)hk * a.M + m0 + threadIdx.x) * a.nrec + piece] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+    RowRegs<T> x;
+    int t = r0 + 32 * wave;
+    const bool any = t < r1;
+    if (any) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
+    QueryOps<RT> q;
+    q.load(a, sm.q, hk, m0, m_end, lane);
+    Queries<RT> s;
+    s.start(a, hk, m0, m_end, i);
+    int see_min = INT_MAX;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int m = min(m0 + 16 * rt + i, m_end - 1);
+        s.see[rt] = own ? min(r1, rows_seen(a, m, b, len, n)) : r1;
+        see_min = min(see_min, s.see[rt]);
+    }
+    v2us ktop = {0, 0}, vtop = {0, 0};
+    for (; t < r1; t += 128) {
+        const bool masked = __any(t + 32 > see_min);
+        v4f sc[RT][2], low[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = low[rt][0] = low[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int step = 0; step < 4; step++) {
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++) {
+                const Halves h = x.k_op(tt, step, ktop);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) score_step<T>(sc[rt][tt], low[rt][tt], h, q.hi(rt, step), q.lo(rt, step));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (sizeof(T) == 4)
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) sc[rt][tt][v] = fmaf(low[rt][tt][v], 1.0f / 2048.0f, sc[rt][tt][v]);
+        if (t + 128 < r1) x.load_k(K, t + 128, i, g);
+        Weights w[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            weigh(s, rt, sc[rt], t, g, masked);
+            w[rt] = weights_of<T>(sc[rt]);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const Halves h = x.v_op(c, vtop);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) s.o[rt][c] = add_rows<T>(s.o[rt][c], h, w[rt]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (t + 128 < r1) x.load_v(V, t + 128, i, g);
+    }
+    // the four waves' sums
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        s.l[rt] += __shfl_xor(s.l[rt], 16, 64);
+        s.l[rt] += __shfl_xor(s.l[rt], 32, 64);
+        if (g == 0) sm.m[wave][16 * rt + i] = s.m[rt], sm.l[wave][16 * rt + i] = s.l[rt];
+    }
+    note_range<T>(ktop, vtop, sm.range[wave], lane);
+    __syncthreads();
+    if (needs_full_width(sm.range, K, V, r0)) {
+        const Rows<T> none{K.p, 0};
+        full_width<T>(a, hk, m0, min(m_end, m0 + 16 * RT), own ? none : K, own ? none : V, r0, own ? K : none, own ? V : none, r0, own, b, len, n, piece);
+        return;
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        float M = sm.m[0][16 * rt + i];
+#pragma unroll
+        for (int w = 1; w < 4; w++) M = fmaxf(M, sm.m[w][16 * rt + i]);
+        const float f = s.m[rt] == M ? 1.0f : __builtin_amdgcn_exp2f(s.m[rt] - M);  // (equal: also both -inf)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+                *reinterpret_cast<float4*>(&sm.o[wave][i][64 * h + 16 * g + 4 * v]) =
+                    make_float4(s.o[rt][4 * h][v] * f, s.o[rt][4 * h + 1][v] * f, s.o[rt][4 * h + 2][v] * f, s.o[rt][4 * h + 3][v] * f);
+        if (wave == 0 && g == 0 && m0 + 16 * rt + i < m_end) {
+            float L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float mw = sm.m[w][16 * rt + i];
+                L += sm.l[w][16 * rt + i] * (mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
+            }
+            a.rec_stat[((int64_t)hk * a.M + m0 + 16 * rt + i) * a.nrec + piece] = make_float2(M, L);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int at = threadIdx.x + 256 * u, q = at >> 5, d = 4 * (at & 31);
+            if (m0 + 16 * rt + q < m_end) {
+                float4 r = *reinterpret_cast<const float4*>(&sm.o[0][q][d]);
+#pragma unroll
+                for (int w = 1; w < 4; w++) {
+                    const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][q][d]);
+                    r.x += y.x, r.y += y.y, r.z += y.z, r.w += y.w;
+                }
+                *reinterpret_cast<float4*>(a.rec_out + (((int64_t)hk * a.M + m0 + 16 * rt + q) * a.nrec + piece) * kS + d) = r;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int RTP, int RTO>
+__global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PrefixArgs a) {
+    __shared__ MeetSmem sm;
+    if (blockIdx.x < a.pitems) {
+        unsigned item = blockIdx.x;
+        const int tile = item % a.ptiles;
+        item /= a.ptiles;
+        const int piece = item % a.ppieces, hk = item / a.ppieces;
+        const int64_t plane = (int64_t)hk * a.pmax * kS;
+        const int end = min(a.P, (piece + 1) * a.prows);
+        const Rows<T> K{(const T*)a.pk + plane, end}, V{(const T*)a.pv + plane, end};
+        few_queries<T, RTP>(a, K, V, hk, tile * 16 * RTP, a.M, piece * a.prows, false, 0, 0, 0, piece, sm);
+    } else {
+        unsigned item = blockIdx.x - a.pitems;
+        const int tile = item % a.otiles;
+        item /= a.otiles;
+        const int piece = item % a.opieces;
+        item /= a.opieces;
+        const int hk = item % a.Hkv, b = item / a.Hkv;
+        int len, n;
+        own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+        const int m0 = b * a.Mq + tile * 16 * RTO, m_end = (b + 1) * a.Mq;
+        // rows that the tile's last live query sees, in pieces of whole 128
+        const int last = min(n, (tile * 16 * RTO + 16 * RTO - 1) / a.G + 1), rows = last > 0 && tile * 16 * RTO < n * a.G ? len + last : 0;
+        const int step = max(128, (rows + 128 * a.opieces - 1) / (128 * a.opieces) * 128);
+        const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kS;
+        const int end = min(rows, (piece + 1) * step);
+        const Rows<T> K{(const T*)a.ok + plane, end}, V{(const T*)a.ov + plane, end};
+        few_queries<T, RTO>(a, K, V, hk, m0, m_end, piece * step, true, b, len, n, a.ppieces + piece, sm);
+    }
+}
+
+// ---- 3. the pieces of a query ----
+// half a wave to a query, 16 bytes to a lane
+__global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int d = 4 * (threadIdx.x & 31);
+    if (r >= (int64_t)a.Hkv * a.M) return;
+    const int hk = (int)(r / a.M), m = (int)(r - (int64_t)hk * a.M), bl = m / a.G, b = bl / a.qL, l = bl - b * a.qL;
+    int len, n;
+    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    float* out = a.out + ((int64_t)bl * a.G * a.Hkv + (int64_t)hk * a.G + (m - bl * a.G)) * kS + d;
+    if (l >= n) {
+        *reinterpret_cast<float4*>(out) = make_float4(0.f, 0.f, 0.f, 0.f);
+        return;
+    }
+    const float2* stat = a.rec_stat + r * a.nrec;
+    const float* rec = a.rec_out + r * a.nrec * kS + d;
+    float M = -INFINITY;
+    for (int c = 0; c < a.nrec; c++) M = fmaxf(M, stat[c].x);
+    float L = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < a.nrec; c++) {
+        const float2 st = stat[c];
+        if (st.y == 0.0f) continue;  // (a piece that the query sees nothing of; its record may not have been written)
+        const float w = st.x == M ? 1.0f : __builtin_amdgcn_exp2f(st.x - M);
+        const float4 x = *reinterpret_cast<const float4*>(rec + (int64_t)c * kS);
+        L = fmaf(w, st.y, L);
+        o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    }
+    const float inv = 1.0f / L;
+    *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+struct PrefixPlan {
+    int rtp, rto, ptiles, ppieces, prows, otiles, opieces;
+};
+static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t P, int64_t maxlen) {
+    PrefixPlan p{};
+    const int64_t Mq = qL * (H / Hkv), M = B * Mq;
+    p.rtp = M > 16 ? 2 : 1;
+    p.rto = Mq > 16 ? 2 : 1;
+    p.ptiles = (int)((M + 16 * p.rtp - 1) / (16 * p.rtp));
+    p.otiles = (int)((Mq + 16 * p.rto - 1) / (16 * p.rto));
+    auto pieces = [](int64_t others, int64_t rows) {
+        int64_t n = others > 0 ? (512 + others - 1) / others : 1;
+        const int64_t most = (rows + 127) / 128;
+        n = n < most ? n : most;
+        return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    };
+    if (P > 0) {
+        const int64_t n = pieces(Hkv * p.ptiles, P);
+        p.prows = (int)((P + 128 * n - 1) / (128 * n) * 128);
+        p.ppieces = (int)((P + p.prows - 1) / p.prows);
+    }
+    p.opieces = pieces(B * Hkv * p.otiles, maxlen);
+    return p;
+}
+
+static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+struct PrefixLayout {
+    size_t qh, ql, cq, stat, rec, total;
+};
+static PrefixLayout layout_prefix(int64_t rows, int nrec) {
+    PrefixLayout w{};
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align_up(bytes, 256);
+        return here;
+    };
+    w.qh = take((size_t)rows * kS * 2);
+    w.ql = take((size_t)rows * kS * 2);
+    w.cq = take((size_t)rows * 4);
+    w.stat = take((size_t)rows * nrec * 8);
+    w.rec = take((size_t)rows * nrec * kS * 4);
+    w.total = at;
+    return w;
+}
+
+template <typename T>
+static int prefix_launch(PrefixArgs a, PrepArgs p, const PrefixPlan& plan, hipStream_t st) {
+    const int64_t prep = (int64_t)a.B * a.qL * p.groups, items = (int64_t)a.pitems + (int64_t)a.B * a.Hkv * a.otiles * a.opieces,
+                  merge = ((int64_t)a.Hkv * a.M + 7) / 8;
+    LLMOPS_REQUIRE(prep < ((int64_t)1 << 31) && items < ((int64_t)1 << 31) && merge < ((int64_t)1 << 31));
+    prefix_prep_kernel<T><<<(unsigned)prep, 256, 0, st>>>(a, p);
+    LLMOPS_LAUNCH_CHECK();
+    if (plan.rtp == 1 && plan.rto == 1) prefix_attn_kernel<T, 1, 1><<<(unsigned)items, 256, 0, st>>>(a);
+    else if (plan.rto == 1) prefix_attn_kernel<T, 2, 1><<<(unsigned)items, 256, 0, st>>>(a);
+    else prefix_attn_kernel<T, 2, 2><<<(unsigned)items, 256, 0, st>>>(a);
+    LLMOPS_LAUNCH_CHECK();
+    prefix_merge_kernel<<<(unsigned)merge, 256, 0, st>>>(a);
+    LLMOPS_LAUNCH_CHECK();
+    return LLMOPS_OK;
+}
+
+}  // namespace llmops
+
+using namespace llmops;
+
+static bool prefix_sizes_fit(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t prefix_len, int64_t maxlen) {
+    const int64_t most = (int64_t)1 << 24;  // positions are exact in fp32
+    return B > 0 && qL > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && prefix_len >= 0 && maxlen > 0 && B < most && qL < most && H < most && prefix_len < most &&
+           maxlen < most && prefix_len + maxlen <= most && B * qL < ((int64_t)1 << 31) / H;
+}
+
+extern "C" size_t llmops_attention_prefix_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t prefix_len, int64_t maxlen) {
+    if (S != kS || !prefix_sizes_fit(B, qL, H, Hkv, prefix_len, maxlen)) return 0;
+    const PrefixPlan p = plan_prefix(B, qL, H, Hkv, prefix_len, maxlen);
+    return layout_prefix(B * qL * H, p.ppieces + p.opieces).total;
+}
+
+extern "C" int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b, int64_t k_stride_l,
+                                            const float* v, int64_t v_stride_b, int64_t v_stride_l, int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S,
+                                            const float* inv_freq, int64_t half, const void* prefix_cache, int64_t prefix_planes, int64_t prefix_maxlen,
+                                            int64_t prefix_len, void* kv_cache, int cache_dtype, int64_t planes, int64_t maxlen, const int32_t* lengths,
+                                            const int32_t* q_lens, int layer_id, float* out, void* workspace, size_t workspace_bytes,
+                                            llmops_stream_t stream) {
+    LLMOPS_REQUIRE(q != nullptr && k != nullptr && v != nullptr && inv_freq != nullptr && kv_cache != nullptr && lengths != nullptr);
+    LLMOPS_REQUIRE(out != nullptr && workspace != nullptr && (prefix_cache != nullptr || prefix_len == 0));
+    LLMOPS_REQUIRE(S == 128);  // head size of every supported model shape
+    LLMOPS_REQUIRE(prefix_sizes_fit(B, qL, H, Hkv, prefix_len, maxlen));
+    LLMOPS_REQUIRE(half > 0 && 2 * half <= S);
+    LLMOPS_REQUIRE(prefix_len == 0 || prefix_len <= prefix_maxlen);
+    LLMOPS_REQUIRE(layer_id >= 0 && 2 * (int64_t)layer_id + 1 < planes && (prefix_len == 0 || 2 * (int64_t)layer_id + 1 < prefix_planes));
+    LLMOPS_REQUIRE(cache_dtype == LLMOPS_CACHE_F32 || cache_dtype == LLMOPS_CACHE_F16);
+    LLMOPS_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(prefix_cache, 16) && aligned(kv_cache, 16) &&
+                   aligned(workspace, 256));
+    LLMOPS_REQUIRE(q_stride_b % 4 == 0 && q_stride_l % 4 == 0 && k_stride_b % 4 == 0 && k_stride_l % 4 == 0 && v_stride_b % 4 == 0 && v_stride_l % 4 == 0);
+    const size_t e = cache_dtype == LLMOPS_CACHE_F32 ? 4 : 2, row = (size_t)Hkv * kS * e;
+    const uintptr_t p0 = reinterpret_cast<uintptr_t>(prefix_cache), p1 = p0 + (size_t)prefix_planes * prefix_maxlen * row,
+                    o0 = reinterpret_cast<uintptr_t>(kv_cache), o1 = o0 + (size_t)planes * B * maxlen * row;
+    LLMOPS_REQUIRE(prefix_len == 0 || p1 <= o0 || o1 <= p0);  // the caches do not overlap
+    const PrefixPlan plan = plan_prefix(B, qL, H, Hkv, prefix_len, maxlen);
+    const PrefixLayout w = layout_prefix(B * qL * H, plan.ppieces + plan.opieces);
+    if (workspace_bytes < w.total)
+        return fail(LLMOPS_EWORKSPACE, "attention_rope_prefix needs %zu workspace bytes, got %zu", w.total, workspace_bytes);
+    char* ws = reinterpret_cast<char*>(workspace);
+    PrefixArgs a{};
+    a.qh = reinterpret_cast<_Float16*>(ws + w.qh), a.ql = reinterpret_cast<_Float16*>(ws + w.ql), a.cq = reinterpret_cast<float*>(ws + w.cq);
+    a.rec_out = reinterpret_cast<float*>(ws + w.rec), a.rec_stat = reinterpret_cast<float2*>(ws + w.stat);
+    const size_t pplane = (size_t)prefix_maxlen * row, oplane = (size_t)B * maxlen * row;
+    a.pk = reinterpret_cast<const char*>(prefix_cache) + 2 * layer_id * pplane, a.pv = reinterpret_cast<const char*>(a.pk) + pplane;
+    a.ok = reinterpret_cast<const char*>(kv_cache) + 2 * layer_id * oplane, a.ov = reinterpret_cast<const char*>(a.ok) + oplane;
+    a.lengths = lengths, a.q_lens = q_lens, a.out = out;
+    a.pmax = prefix_maxlen, a.maxlen = maxlen;
+    a.B = (int)B, a.qL = (int)qL, a.G = (int)(H / Hkv), a.Hkv = (int)Hkv, a.P = (int)prefix_len, a.Mq = (int)(qL * a.G), a.M = (int)(B * a.Mq);
+    a.ptiles = plan.ptiles, a.ppieces = plan.ppieces, a.prows = plan.prows, a.otiles = plan.otiles, a.opieces = plan.opieces;
+    a.nrec = plan.ppieces + plan.opieces;
+    a.pitems = (unsigned)(Hkv * plan.ptiles * plan.ppieces);
+    const PrepArgs p{q, k, v, inv_freq, q_stride_b, q_stride_l, k_stride_b, k_stride_l, v_stride_b, v_stride_l, (int)half, (int)((H + 2 * Hkv + 15) / 16)};
+    hipStream_t st = as_stream(stream);
+    return cache_dtype == LLMOPS_CACHE_F32 ? prefix_launch<float>(a, p, plan, st) : prefix_launch<__half>(a, p, plan, st);
+}

@@ -24,7 +24,7 @@ __all__ = [
     "offline_FC_quant_Q4A", "offline_FC_dequant_Q4A", "fc_Q4A", "fc_Q4A_noalloc", "fc_Q4A_decode", "interleave_gate_up", "FC_dynamic_quantize_x", "fc_Q4A_partials",
     "attention_rope", "attention_rope2", "attention_rope2_records", "attention_records_supported", "AttentionRecords", "rope_embed", "softmax", "rmsnorm", "iadd", "imul", "itrans", "clone",
     "rmsnorm_out", "silu_mul", "empty", "ones", "embedding", "embedding_q8c_quant_w", "embedding_q8c", "tensor_pool", "set_default_group_k", "reserve_workspace", "reset_workspaces",
-    "group_k_of",
+    "group_k_of", "attention_rope_prefix", "lora_add", "verify_drafts",
 ]
 
 # Callers of the reference read ``tensor.item_size`` (chatllama/main.py:171-173, ops/perf_ops.py:242; bound at
@@ -516,6 +516,153 @@ def mm_qk24(q, kcache):
 def mm_qk42(q, kcache, attn_w):
     """q [B,H,qL,S], kcache [B,H,max-kv-len,S]; fills attn_w [B,H,qL,kvLen] (ops/op_attn.hpp:195-298)."""
     _mm_qk(q, kcache, attn_w, True)
+
+
+# ---- several requests in step -----------------------------------------------------------------
+# Extensions: the reference answers one chat at a time.  Their scratch memory comes from torch's allocator call by call: it holds nothing
+# between calls, and a graph that captures one keeps its own.
+def _here(first, **others):
+    """all on first's device"""
+    for name, t in others.items():
+        if t is not None:
+            _require(isinstance(t, torch.Tensor) and t.device == first.device, f"{name} is on the same HIP device")
+
+
+def _rows(t, name):
+    """fp32 [B, L, C] whose innermost dimension is dense: pointer and strides of the other two"""
+    _require(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} is on the HIP device (llmops has no CPU path)")
+    _require(t.dtype == torch.float32 and t.dim() == 3, f"{name}.is<float>(3)")
+    _require(t.stride(2) == 1 or t.shape[2] == 1, f"{name} inner dimension is contiguous")
+    return _ptr(t), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+
+
+def _on_device(device, call, *args):
+    """the call with `device` current (a launch goes to the current device) and its current stream"""
+    if device.index == torch.cuda.current_device():
+        return _lib.check(call(*args, ctypes.c_void_p(_raw_stream(device))))
+    with torch.cuda.device(device):
+        return _lib.check(call(*args, ctypes.c_void_p(_raw_stream(device))))
+
+
+def attention_rope_prefix(q, k, v, inv_freq, prefix_cache, prefix_len, kv_cache, lengths, layer_id, q_lens=None):
+    """Rotary, cache update and attention of a batch whose sequences share a prefix that is held, and read, once.
+
+    q fp32 [B,qL,H*S], k and v fp32 [B,qL,Hkv*S] (H a multiple of Hkv; columns of a projection's output will do), left as they are.
+    prefix_cache [2*layers,1,Hkv,rows,S]: the first ``prefix_len`` rows are what every sequence has seen (what ``attention_rope2`` left in
+    a cache of batch 1); None with prefix_len 0.  kv_cache [2*layers,B,Hkv,maxlen,S]: each sequence's own rows behind it, as many as
+    ``lengths`` (int32 [B], device) says; both fp32 or both fp16.  Token l of sequence b is at position prefix_len + lengths[b] + l; its
+    rotated k and its v are written to row lengths[b] + l, and it sees the prefix and its own rows up to that one.  ``lengths`` is not
+    changed: add to it what is to be kept, and the next call overwrites the rest.
+    q_lens (int32 [B], device): a sequence brings that many of the qL tokens; the rest, and tokens that no longer fit the cache, are
+    padding: not cached, and 0 in the result.  Returns fp32 [B,qL,H*S]."""
+    (qp, qb, ql), (kp, kb, kl), (vp, vb, vl) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    for t, n in ((kv_cache, "kv_cache"),) + (((prefix_cache, "prefix_cache"),) if prefix_cache is not None else ()):
+        _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 5 and t.is_contiguous(), f"{n}.is<float>(5)")
+        _require(t.dtype in (torch.float32, torch.float16), f"{n}.is<float>(5)")
+    _dev(inv_freq, torch.float32, 1, "inv_freq")
+    _dev(lengths, torch.int32, 1, "lengths")
+    if q_lens is not None:
+        _dev(q_lens, torch.int32, 1, "q_lens")
+        _require(q_lens.shape[0] == q.shape[0], "q_lens.is({B})")
+    _here(q, k=k, v=v, inv_freq=inv_freq, prefix_cache=prefix_cache, kv_cache=kv_cache, lengths=lengths, q_lens=q_lens)
+    B, qL, width = q.shape
+    planes, Bc, Hkv, maxlen, S = kv_cache.shape
+    prefix_len = int(prefix_len)
+    _require(Bc == B and lengths.shape[0] == B, "kv_cache.size(1) == B, lengths.is({B})")
+    _require(S > 0 and width % S == 0, "q.size(2) % S == 0")
+    for t, n in ((k, "k"), (v, "v")):
+        _require(tuple(t.shape) == (B, qL, Hkv * S), f"{n}.is({{B, qL, Hkv * S}})")
+    pp, pplanes, pmax = None, 0, 0
+    if prefix_cache is not None:
+        pplanes, pb, ph, pmax, ps = prefix_cache.shape
+        _require(pb == 1 and ph == Hkv and ps == S and prefix_cache.dtype == kv_cache.dtype, "prefix_cache.is({planes, 1, Hkv, rows, S})")
+        pp = _ptr(prefix_cache)
+    _require(0 <= prefix_len <= pmax, "0 <= prefix_len <= prefix_cache.size(3)")
+    lib = _lib.load()
+    H = width // S
+    need = lib.llmops_attention_prefix_workspace_bytes(B, qL, H, Hkv, S, prefix_len, maxlen)
+    out = torch.empty((B, qL, width), dtype=torch.float32, device=q.device)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+    _on_device(q.device, lib.llmops_attention_rope_prefix, qp, qb, ql, kp, kb, kl, vp, vb, vl, B, qL, H, Hkv, S, _ptr(inv_freq),
+               inv_freq.shape[0], pp, pplanes, pmax, prefix_len, _ptr(kv_cache), 0 if kv_cache.dtype == torch.float32 else 1, planes, maxlen,
+               _ptr(lengths), _ptr(q_lens) if q_lens is not None else None, int(layer_id), _ptr(out), _ptr(ws), ws.numel())
+    return out
+
+
+_LORA_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def lora_add(y, x, lora_A, lora_B, adapters, scales, out=None):
+    """y + scales[a] * (x A_a^T) B_a^T with a = adapters[b] for every token of sequence b: low-rank adapters of several requests
+    beside the projection that made y of x.
+
+    y fp32 [B,M,N], x fp32 [B,M,K] (inner dimension dense, any strides: columns of a fused projection's output will do); lora_A [n,R,K]
+    and lora_B [n,N,R] (fp32, fp16 or bf16) hold n adapters, those of a lower rank padded with zeros; adapters int32 [B] and scales fp32
+    [n] on the device.  An adapter outside 0 .. n-1 (-1) is none: the sequence keeps its y.  Returns a new tensor, or ``out`` [B,M,N],
+    which may be y itself and must not overlap x or y otherwise."""
+    (yp, yb, yl), (xp, xb, xl) = _rows(y, "y"), _rows(x, "x")
+    for t, n in ((lora_A, "lora_A"), (lora_B, "lora_B")):
+        _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 3 and t.is_contiguous() and t.dtype in _LORA_TYPES, f"{n}.is_dense(3)")
+    _dev(adapters, torch.int32, 1, "adapters")
+    _dev(scales, torch.float32, 1, "scales")
+    B, M, N = y.shape
+    K, (n, R, _) = x.shape[2], lora_A.shape
+    _require(tuple(x.shape[:2]) == (B, M), "x.is({B, M, K})")
+    _require(tuple(lora_A.shape) == (n, R, K) and tuple(lora_B.shape) == (n, N, R) and lora_A.dtype == lora_B.dtype, "lora_A.is({n, R, K}), lora_B.is({n, N, R})")
+    _require(adapters.shape[0] == B and scales.shape[0] == n, "adapters.is({B}), scales.is({n})")
+    if out is None:
+        out = torch.empty((B, M, N), dtype=torch.float32, device=y.device)
+    op, ob, ol = _rows(out, "out")
+    _require(tuple(out.shape) == (B, M, N) and (B == 1 or abs(ob) >= N) and (M == 1 or abs(ol) >= N), "out.is({B, M, N}), rows apart")
+    _here(y, x=x, lora_A=lora_A, lora_B=lora_B, adapters=adapters, scales=scales, out=out)
+    lib = _lib.load()
+    ws = torch.empty(max(lib.llmops_lora_workspace_bytes(B, M, N, K, R), 1), dtype=torch.uint8, device=y.device)
+    _on_device(y.device, lib.llmops_lora_add, yp, yb, yl, xp, xb, xl, B, M, N, K, _ptr(lora_A), _ptr(lora_B), _LORA_TYPES[lora_A.dtype], R, n,
+               _ptr(adapters), _ptr(scales), op, ob, ol, _ptr(ws), ws.numel())
+    return out
+
+
+def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature=None, draft_lens=None):
+    """Checks K drafted tokens of each sequence against the model's logits and gives the token behind those accepted.
+
+    logits fp32 [B,K+1,V] (row i: behind i drafts), drafts int64 or int32 [B,K], uniforms fp32 [B,K+1] in [0, 1).  With p_i =
+    softmax(logits[:, i] / temperature): draft i is accepted while uniforms[:, i] * q_i(draft) < p_i(draft), q_i = draft_probs[:, i] (fp32
+    [B,K,V], what the drafts were drawn from; None: drafts that come from no distribution, q_i = 1).  The next token is drawn, with
+    uniforms[:, K], from max(p_i - q_i, 0) where draft i was refused (without draft_probs: from p_i without the draft), and from the row
+    behind the last draft where none was: the answers are distributed as the model's own.  temperature: None (1), a number, or fp32 [B]
+    on the device; 0 takes the likeliest token, and drafts while they are it.  draft_lens (int32 [B], device): a sequence has that many
+    drafts.  K may be 0: the next token is drawn from the logits.
+
+    Returns (tokens int64 [B,K+1]: the accepted drafts, the next token, -1 behind it; accepted int32 [B]: how many drafts)."""
+    _dev(logits, torch.float32, 3, "logits")
+    _require(isinstance(drafts, torch.Tensor) and drafts.is_cuda and drafts.dtype in (torch.int64, torch.int32), "drafts.is<int64_t>(2)")
+    _require(drafts.dim() == 2 and drafts.is_contiguous(), "drafts.is<int64_t>(2)")
+    _dev(uniforms, torch.float32, 2, "uniforms")
+    B, rows, V = logits.shape
+    K = rows - 1
+    _require(tuple(drafts.shape) == (B, K) and tuple(uniforms.shape) == (B, K + 1), "drafts.is({B, K}), uniforms.is({B, K + 1})")
+    if draft_probs is not None:
+        _dev(draft_probs, torch.float32, 3, "draft_probs")
+        _require(tuple(draft_probs.shape) == (B, K, V), "draft_probs.is({B, K, V})")
+    if draft_lens is not None:
+        _dev(draft_lens, torch.int32, 1, "draft_lens")
+        _require(draft_lens.shape[0] == B, "draft_lens.is({B})")
+    per_row = isinstance(temperature, torch.Tensor)
+    if per_row:
+        _dev(temperature, torch.float32, 1, "temperature")
+        _require(temperature.shape[0] == B, "temperature.is({B})")
+    _here(logits, drafts=drafts, uniforms=uniforms, draft_probs=draft_probs, draft_lens=draft_lens, temperature=temperature if per_row else None)
+    if drafts.dtype != torch.int64:
+        drafts = drafts.to(torch.int64)
+    lib = _lib.load()
+    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=logits.device)
+    accepted = torch.empty((B,), dtype=torch.int32, device=logits.device)
+    ws = torch.empty(max(lib.llmops_verify_drafts_workspace_bytes(B, K, V), 1), dtype=torch.uint8, device=logits.device)
+    _on_device(logits.device, lib.llmops_verify_drafts, _ptr(logits), B, K, V, _ptr(drafts) if K else None,
+               _ptr(draft_probs) if draft_probs is not None and K else None, _ptr(uniforms), _ptr(temperature) if per_row else None,
+               1.0 if temperature is None or per_row else float(temperature), _ptr(draft_lens) if draft_lens is not None else None, _ptr(tokens),
+               _ptr(accepted), _ptr(ws), ws.numel())
+    return tokens, accepted
 
 
 # ---- neighbours -------------------------------------------------------------------------------

@@ -49,6 +49,14 @@ SIGNATURES = {
     "llmops_attention_records_chunk_rows": (c_i64, [c_i64, c_int]),
     "llmops_attention_rope_decode_records": (c_int, [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_int, c_i64,
                                                      c_i64, c_ptr, c_int, c_ptr, c_int, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
+    "llmops_attention_prefix_workspace_bytes": (c_size, [c_i64] * 7),
+    "llmops_attention_rope_prefix": (c_int, [c_ptr, c_i64, c_i64] * 3 + [c_i64] * 5 + [c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_int,
+                                             c_i64, c_i64, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_size, c_ptr]),
+    "llmops_lora_workspace_bytes": (c_size, [c_i64] * 5),
+    "llmops_lora_add": (c_int, [c_ptr, c_i64, c_i64] * 2 + [c_i64] * 4 + [c_ptr, c_ptr, c_int, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_i64,
+                                c_ptr, c_size, c_ptr]),
+    "llmops_verify_drafts_workspace_bytes": (c_size, [c_i64] * 3),
+    "llmops_verify_drafts": (c_int, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_f32, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
     "llmops_softmax": (c_int, [c_ptr, c_i64, c_i64, c_ptr]),
     "llmops_mm_qk": (c_int, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_ptr]),
     "llmops_rmsnorm": (c_int, [c_ptr, c_i64, c_i64, c_ptr, c_f32, c_ptr]),

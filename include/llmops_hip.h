@@ -308,9 +308,9 @@ int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_s
  * int32 [batch] on the device.  An id outside 0 .. adapters-1 (-1) is none: out = y.  Adapters of a lower rank than R are padded with
  * zeros.  x [batch,tokens,K], y and out [batch,tokens,N] fp32, token l of sequence b at + b*stride_b + l*stride_l elements; out may be y
  * (the same pointer and strides) and must not overlap x or y otherwise.  Up to 1048560 tokens in all, R up to 4096.  Sizes and
- * strides are free; 16-byte aligned rows (K, R multiples of 8, strides of 4) are read 16 bytes at a time.
+ * strides are free.
  * fp32 arithmetic, except that products are formed of exact bf16 pieces: what is dropped is below 2^-22 of a product. */
-size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R);
+size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R, int64_t adapters);
 int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, const float* x, int64_t x_stride_b, int64_t x_stride_l,
                     int64_t batch, int64_t tokens, int64_t N, int64_t K, const void* lora_A, const void* lora_B, int weight_dtype, int64_t R,
                     int64_t adapters, const int32_t* ids, const float* scales, float* out, int64_t out_stride_b, int64_t out_stride_l,
@@ -327,7 +327,7 @@ int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, cons
  * uniforms fp32 [B,K+1], in [0, 1): [b,K] draws the next token.
  * tokens int64 [B,K+1]: the accepted drafts, the next token, -1 behind; accepted int32 [B]: how many drafts.
  * Logits that are NaN or minus infinity weigh nothing, equal plus infinities share the row; a row without any other logit gives -1.
- * Exponentials and sums are in 64 bits: the answer is the definition's but for numbers within about 1e-14 of a border.
+ * Exponentials and sums are in 64 bits: the answer is the definition's but for numbers within about 1e-13 of a border.
  * B*(K+1) < 2^24, V <= 2^27. */
 size_t llmops_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
 int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, int64_t V, const int64_t* drafts, const float* draft_probs,

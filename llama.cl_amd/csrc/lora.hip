@@ -34,7 +34,7 @@ struct Pieces {
 __device__ __forceinline__ v8bf as_v8bf(uint4 u) { return __builtin_bit_cast(v8bf, u); }
 __device__ __forceinline__ uint32_t upper(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// eight fp32 values as N bf16 pieces each (infinities and NaN in the first)
+// eight fp32 values as N bf16 pieces each (an infinity leaves NaN behind it)
 template <int N>
 __device__ __forceinline__ Pieces<N> cut8(const float (&x)[8]) {
     Pieces<N> r;
@@ -43,75 +43,89 @@ __device__ __forceinline__ Pieces<N> cut8(const float (&x)[8]) {
     for (int e = 0; e < 8; e++) rest[e] = x[e];
 #pragma unroll
     for (int n = 0; n < N; n++) {
-        uint32_t u[8], w[4];
+        uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            u[e] = __float_as_uint(rest[e]);
-            const float left = rest[e] - __uint_as_float(u[e] & 0xffff0000u);
-            rest[e] = (u[e] << 1) == 0xff000000u ? 0.0f : left;
-        }
+        for (int e = 0; e < 4; e++) w[e] = upper(__float_as_uint(rest[2 * e]), __float_as_uint(rest[2 * e + 1]));
 #pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = upper(u[2 * e], u[2 * e + 1]);
+        for (int e = 0; e < 8; e++) rest[e] -= __uint_as_float(__float_as_uint(rest[e]) & 0xffff0000u);
         r.p[n] = as_v8bf(make_uint4(w[0], w[1], w[2], w[3]));
     }
     return r;
 }
 
-// a weight's type: its pieces, and eight of a row from `at` on, zeros from `end` on
-template <typename W>
-struct Weight;
-template <>
-struct Weight<float> {
-    static constexpr int kPieces = 3;
-    template <bool VEC>
-    static __device__ __forceinline__ Pieces<3> load(const float* row, int at, int end) {
-        float x[8];
-        if (VEC && at + 8 <= end) {
-            const float4 a = *reinterpret_cast<const float4*>(row + at), b = *reinterpret_cast<const float4*>(row + at + 4);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = at + e < end ? row[at + e] : 0.0f;
-        }
-        return cut8<3>(x);
-    }
+// Eight neighbours of a row, wherever it starts (global loads need no alignment)
+struct __attribute__((packed, aligned(4))) Eight32 {
+    float x[8];
 };
+struct __attribute__((packed, aligned(2))) Eight16 {
+    uint16_t x[8];
+};
+// The eight that a lane takes at the end of a row: where fewer are left, those that end with it, and the other operand's are zero where they
+// are before `at` (another lane's, or nobody's)
+__device__ __forceinline__ int eight_from(int at, int end) { return max(0, min(at, end - 8)); }
+
+// a weight's type: eight of a row as they are in memory, and their pieces
 struct Half16 {
     uint16_t u;
 };
 struct Bf16 {
     uint16_t u;
 };
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const uint16_t* row, int at, int end) {
-    if (VEC && at + 8 <= end) return *reinterpret_cast<const uint4*>(row + at);
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-        w[e] = (at + 2 * e < end ? row[at + 2 * e] : 0u) | (at + 2 * e + 1 < end ? (uint32_t)row[at + 2 * e + 1] << 16 : 0u);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
+template <typename W>
+struct Weight;
 template <>
-struct Weight<Half16> {
-    static constexpr int kPieces = 2;
-    template <bool VEC>
-    static __device__ __forceinline__ Pieces<2> load(const Half16* row, int at, int end) {
-        const uint4 u = load8<VEC>(reinterpret_cast<const uint16_t*>(row), at, end);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Weight<float> {
+    typedef Eight32 Raw;
+    typedef float Bits;
+    static __device__ __forceinline__ Pieces<3> cut(const Raw& r) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = f16_bits_to_f32((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+        for (int e = 0; e < 8; e++) x[e] = r.x[e];
+        return cut8<3>(x);
+    }
+};
+template <>
+struct Weight<Half16> {
+    typedef Eight16 Raw;
+    typedef uint16_t Bits;
+    static __device__ __forceinline__ Pieces<2> cut(const Raw& r) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = f16_bits_to_f32(r.x[e]);
         return cut8<2>(x);
     }
 };
 template <>
 struct Weight<Bf16> {
-    static constexpr int kPieces = 1;
-    template <bool VEC>
-    static __device__ __forceinline__ Pieces<1> load(const Bf16* row, int at, int end) {
-        return {{as_v8bf(load8<VEC>(reinterpret_cast<const uint16_t*>(row), at, end))}};
-    }
+    typedef Eight16 Raw;
+    typedef uint16_t Bits;
+    static __device__ __forceinline__ Pieces<1> cut(const Raw& r) { return {{__builtin_bit_cast(v8bf, r)}}; }
 };
+template <typename W>
+__device__ __forceinline__ typename Weight<W>::Raw load8(const W* row, int at) {
+    return *reinterpret_cast<const typename Weight<W>::Raw*>(row + at);
+}
+// the same at a row's end; SHORT: the whole row is fewer than eight
+template <bool SHORT, typename W>
+__device__ __forceinline__ typename Weight<W>::Raw load8_end(const W* row, int at, int end) {
+    if constexpr (!SHORT) {
+        return load8(row, eight_from(at, end));
+    } else {
+        typename Weight<W>::Raw r{};
+        const auto* from = reinterpret_cast<const typename Weight<W>::Bits*>(row);
+#pragma unroll
+        for (int e = 0; e < 7; e++)
+            if (e < end) r.x[e] = from[e];
+        return r;
+    }
+}
+__device__ __forceinline__ Pieces<3> cut_end(const Eight32& r, int at, int end) {
+    const int from = eight_from(at, end);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = from + e < at ? 0.0f : r.x[e];
+    return cut8<3>(x);
+}
 
 template <int NW>
 __device__ __forceinline__ v4f times(const Pieces<NW>& w, const Pieces<3>& x, v4f acc) {
@@ -121,159 +135,325 @@ __device__ __forceinline__ v4f times(const Pieces<NW>& w, const Pieces<3>& x, v4
         for (int m = 0; m < 3 && n + m < 3; m++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.p[n], x.p[m], acc, 0, 0, 0);
     return acc;
 }
+__device__ __forceinline__ v4f keep(bool match, v4f sum, v4f acc) {
+#pragma unroll
+    for (int v = 0; v < 4; v++) acc[v] = match ? sum[v] : acc[v];
+    return acc;
+}
 
+constexpr int kDownWaves = 8;
+
+// The adapters that occur among a workgroup's tokens, in the order of their first token
+struct Adapters {
+    int count;
+    int id[32];
+};
 // token `row`'s adapter, -1 for none
 __device__ __forceinline__ int adapter_of(const LoraArgs& a, int row) {
     if (row >= a.rows) return -1;
     const int id = a.ids[row / a.tokens];
     return id >= 0 && id < a.adapters ? id : -1;
 }
-// calls f(adapter, whether this lane's token is one of its) for every adapter among the sixteen tokens (token lane % 16)
-template <typename F>
-__device__ __forceinline__ void each_adapter(int mine, F f) {
-    uint32_t todo = (uint32_t)__ballot(mine >= 0) & 0xffffu;
-    while (todo != 0) {
-        const int id = __builtin_amdgcn_readlane(mine, __builtin_ctz(todo));
-        f(id, mine == id);
-        todo &= ~(uint32_t)__ballot(mine == id);
+template <int TT>
+__device__ __forceinline__ void list_adapters(const LoraArgs& a, Adapters& list, int row0) {
+    if (threadIdx.x < 64) {
+        const int mine = (int)threadIdx.x < 16 * TT ? adapter_of(a, row0 + threadIdx.x) : -1;
+        uint64_t todo = __ballot(mine >= 0);
+        int n = 0;
+        while (todo != 0) {
+            const int id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+            if (threadIdx.x == 0) list.id[n] = id;
+            n++;
+            todo &= ~__ballot(mine == id);
+        }
+        if (threadIdx.x == 0) list.count = n;
     }
+    __syncthreads();
 }
 
-// A workgroup: sixteen tokens, a run of K (its four waves a quarter of every 128 each), 16 * NR rows of A.
+// A workgroup: 16 * TT tokens, a run of K (its eight waves an eighth of every 256 each), 16 * NR rows of A.  Bound by latency with few
+// tokens, by reading x with many; so the operands of U steps, or of U adapters, are asked for before the first is used.
 // A operand: row of A lane % 16, eight k; B operand: token lane % 16, the same k; result: token lane % 16, rows 4 * (lane / 16) + v.
-template <typename W, int NR, bool VEC>
-__global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
-    __shared__ v4f meet[4][NR][64];
+template <typename W, int NR, int TT, bool SHORT>
+__global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) {
+    constexpr int kStep = 32 * kDownWaves;
+    constexpr int U = sizeof(W) == 4 && NR * TT > 2 ? 2 : 4;
+    typedef typename Weight<W>::Raw Raw;
+    __shared__ Adapters list;
+    __shared__ v4f meet[kDownWaves][NR * TT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.x * 16, r0 = blockIdx.z * 16 * NR, row = row0 + i;
+    const int row0 = blockIdx.x * 16 * TT, r0 = blockIdx.z * 16 * NR;
     const int k0 = blockIdx.y * a.chunk, k1 = min(a.K, k0 + a.chunk);
-    const int mine = adapter_of(a, row);
-    const int safe = min(row, a.rows - 1), b = safe / a.tokens;
-    const float* x = a.x + b * a.xsb + (safe - b * a.tokens) * a.xsl;
-    v4f acc[NR];
+    list_adapters<TT>(a, list, row0);
+    const int count = __builtin_amdgcn_readfirstlane(list.count);
+    if (count == 0) return;  // (nobody reads these sums)
+    const float* x[TT];
 #pragma unroll
-    for (int n = 0; n < NR; n++) acc[n] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int k = k0 + 32 * wave; k < k1; k += 128) {
-        const Pieces<3> xp = Weight<float>::load<VEC>(x, k + 8 * g, k1);
-        each_adapter(mine, [&](int id, bool match) {
-            const W* A = reinterpret_cast<const W*>(a.A) + (int64_t)id * a.R * a.K;
+    for (int tt = 0; tt < TT; tt++) {
+        const int row = min(row0 + 16 * tt + i, a.rows - 1), b = row / a.tokens;
+        x[tt] = a.x + b * a.xsb + (row - b * a.tokens) * a.xsl;
+    }
+    const W* A[NR];  // rows of the adapter with number 0; past the last rank that rank again (not stored)
+#pragma unroll
+    for (int n = 0; n < NR; n++) A[n] = reinterpret_cast<const W*>(a.A) + (int64_t)min(r0 + 16 * n + i, a.R - 1) * a.K;
+    const int64_t adapter = (int64_t)a.R * a.K;
+    v4f acc[NR][TT];
+#pragma unroll
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++) acc[n][tt] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (count == 1) {
+        const int64_t at = __builtin_amdgcn_readfirstlane(list.id[0]) * adapter;
+        int k = k0 + 32 * wave;
+        for (; k + kStep * (U - 1) + 32 <= k1; k += kStep * U) {
+            Raw w[U][NR];
+            Eight32 xr[U][TT];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++) xr[u][tt] = load8(x[tt], k + kStep * u + 8 * g);
+#pragma unroll
+                for (int n = 0; n < NR; n++) w[u][n] = load8(A[n] + at, k + kStep * u + 8 * g);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                Pieces<3> xp[TT];
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++) xp[tt] = Weight<float>::cut(xr[u][tt]);
+#pragma unroll
+                for (int n = 0; n < NR; n++) {
+                    const auto wp = Weight<W>::cut(w[u][n]);
+#pragma unroll
+                    for (int tt = 0; tt < TT; tt++) acc[n][tt] = times(wp, xp[tt], acc[n][tt]);
+                }
+            }
+        }
+        for (; k < k1; k += kStep) {
+            Pieces<3> xp[TT];
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) xp[tt] = cut_end(load8_end<SHORT>(x[tt], k + 8 * g, k1), k + 8 * g, k1);
 #pragma unroll
             for (int n = 0; n < NR; n++) {
-                const int r = r0 + 16 * n + i;
-                const auto w = Weight<W>::template load<VEC>(A + (int64_t)min(r, a.R - 1) * a.K, k + 8 * g, k1);
-                const v4f sum = times(w, xp, acc[n]);
+                const auto wp = Weight<W>::cut(load8_end<SHORT>(A[n] + at, k + 8 * g, k1));
 #pragma unroll
-                for (int v = 0; v < 4; v++) acc[n][v] = match ? sum[v] : acc[n][v];
+                for (int tt = 0; tt < TT; tt++) acc[n][tt] = times(wp, xp[tt], acc[n][tt]);
             }
-        });
+        }
+    } else {
+        int mine[TT];
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++) mine[tt] = adapter_of(a, row0 + 16 * tt + i);
+        for (int k = k0 + 32 * wave; k < k1; k += kStep) {
+            Pieces<3> xp[TT];
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) xp[tt] = cut_end(load8_end<SHORT>(x[tt], k + 8 * g, k1), k + 8 * g, k1);
+            for (int c = 0; c < count; c += U) {
+                int id[U];
+                Raw w[U][NR];
+#pragma unroll
+                for (int u = 0; u < U; u++) {  // (past the last adapter that one again, whose sum is not taken over)
+                    id[u] = __builtin_amdgcn_readfirstlane(list.id[min(c + u, count - 1)]);
+#pragma unroll
+                    for (int n = 0; n < NR; n++) w[u][n] = load8_end<SHORT>(A[n] + id[u] * adapter, k + 8 * g, k1);
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (c + u >= count) break;
+#pragma unroll
+                    for (int n = 0; n < NR; n++) {
+                        const auto wp = Weight<W>::cut(w[u][n]);
+#pragma unroll
+                        for (int tt = 0; tt < TT; tt++) acc[n][tt] = keep(mine[tt] == id[u], times(wp, xp[tt], acc[n][tt]), acc[n][tt]);
+                    }
+                }
+            }
+        }
     }
 #pragma unroll
-    for (int n = 0; n < NR; n++) meet[wave][n][lane] = acc[n];
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++) meet[wave][n * TT + tt][lane] = acc[n][tt];
     __syncthreads();
-    for (int n = wave; n < NR; n += 4) {
-        const v4f s = (meet[0][n][lane] + meet[1][n][lane]) + (meet[2][n][lane] + meet[3][n][lane]);
+    for (int m = wave; m < NR * TT; m += kDownWaves) {
+        const int n = m / TT, row = row0 + 16 * (m - n * TT) + i, r = r0 + 16 * n + 4 * g;
+        v4f s = meet[0][m][lane];
+#pragma unroll
+        for (int w = 1; w < kDownWaves; w++) s += meet[w][m][lane];
         if (row >= a.rows) continue;
-        float* to = a.part + ((int64_t)blockIdx.y * a.rows + row) * a.R;
+        float* to = a.part + ((int64_t)blockIdx.y * a.rows + row) * a.R + r;
 #pragma unroll
         for (int v = 0; v < 4; v++)
-            if (r0 + 16 * n + 4 * g + v < a.R) to[r0 + 16 * n + 4 * g + v] = s[v];
+            if (r + v < a.R) to[v] = s[v];
     }
 }
 
-// A workgroup: sixteen tokens, 256 columns (64 to a wave), ranks 128 at a time.
+// A workgroup: 16 * TT tokens, 64 * CT columns (16 * CT to a wave), ranks 128 at a time; y is asked for first, as it is used last.
 // A operand: column lane % 16 of B, eight ranks; B operand: token lane % 16, the same ranks; result: token lane % 16, columns 4 * (lane / 16) + v.
-template <typename W, bool VEC>
+template <typename W, int CT, int TT, bool SHORT>
 __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) {
-    constexpr int kRanks = 128, kStride = kRanks + 4;
-    __shared__ __align__(16) float t[16][kStride];
+    constexpr int kRanks = 128, kStride = kRanks + 4, U = CT == 1 ? 8 : 1;
+    typedef typename Weight<W>::Raw Raw;
+    __shared__ Adapters list;
+    __shared__ __align__(16) float t[16 * TT][kStride];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.y * 16, n0 = blockIdx.x * 256 + 64 * wave, row = row0 + i;
-    const int mine = adapter_of(a, row);
-    v4f acc[4];
+    const int row0 = blockIdx.y * 16 * TT, n0 = (blockIdx.x * 4 + wave) * 16 * CT;
+    const float* y[TT];
+    float* out[TT];
+    float4 yv[CT][TT];
 #pragma unroll
-    for (int n = 0; n < 4; n++) acc[n] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int r0 = 0; r0 < a.R; r0 += kRanks) {
-        const int ranks = min(kRanks, a.R - r0), padded = (ranks + 31) & ~31;
-        __syncthreads();
-        for (int e = threadIdx.x; e < 16 * padded; e += 256) {
-            const int token = e / padded, r = e - token * padded;
-            float s = 0.0f;
-            if (r < ranks && row0 + token < a.rows) {
-                const float* from = a.part + (int64_t)(row0 + token) * a.R + r0 + r;
-                for (int c = 0; c < a.splits; c++) s += from[(int64_t)c * a.rows * a.R];
+    for (int tt = 0; tt < TT; tt++) {
+        const int row = min(row0 + 16 * tt + i, a.rows - 1), b = row / a.tokens, l = row - b * a.tokens;
+        y[tt] = a.y + b * a.ysb + l * a.ysl;
+        out[tt] = a.out + b * a.osb + l * a.osl;
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            const int col = n0 + 16 * c + 4 * g;
+            yv[c][tt] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (vec_out && col + 4 <= a.N) {
+                yv[c][tt] = *reinterpret_cast<const float4*>(y[tt] + col);
+            } else {
+                float* to = reinterpret_cast<float*>(&yv[c][tt]);
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    if (col + v < a.N) to[v] = y[tt][col + v];
             }
-            t[token][r] = s;
+        }
+    }
+    int mine[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; tt++) mine[tt] = adapter_of(a, row0 + 16 * tt + i);
+    list_adapters<TT>(a, list, row0);
+    const int count = __builtin_amdgcn_readfirstlane(list.count);
+    const W* B[CT];
+#pragma unroll
+    for (int c = 0; c < CT; c++) B[c] = reinterpret_cast<const W*>(a.B) + (int64_t)min(n0 + 16 * c + i, a.N - 1) * a.R;
+    const int64_t adapter = (int64_t)a.N * a.R;
+    v4f acc[CT][TT];
+#pragma unroll
+    for (int c = 0; c < CT; c++)
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++) acc[c][tt] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int r0 = 0; r0 < a.R && count > 0; r0 += kRanks) {
+        const int ranks = min(kRanks, a.R - r0), padded = (ranks + 31) & ~31;
+        if (r0 > 0) __syncthreads();
+        // (two values and eight runs at a time: sixteen loads on their way; one by one they were two thirds of a prompt's launch)
+        for (int e0 = threadIdx.x; e0 < 16 * TT * padded; e0 += 512) {
+            float sum[2];
+            const float* from[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int e = e0 + 256 * h, token = e / padded, r = e - token * padded;
+                from[h] = e < 16 * TT * padded && r < ranks && row0 + token < a.rows ? a.part + (int64_t)(row0 + token) * a.R + r0 + r : nullptr;
+                sum[h] = 0.0f;
+            }
+            const int64_t run = (int64_t)a.rows * a.R;
+            for (int c = 0; c < a.splits; c += 8) {
+                float x[2][8];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int u = 0; u < 8; u++) x[h][u] = (from[h] != nullptr ? from[h] : a.part)[min(c + u, a.splits - 1) * run];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int u = 0; u < 8; u++) sum[h] += c + u < a.splits ? x[h][u] : 0.0f;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int e = e0 + 256 * h, token = e / padded;
+                if (e < 16 * TT * padded) t[token][e - token * padded] = from[h] != nullptr ? sum[h] : 0.0f;
+            }
         }
         __syncthreads();
         for (int step = 0; step < padded; step += 32) {
-            float x[8];
+            Pieces<3> tp[TT];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float4 u = *reinterpret_cast<const float4*>(&t[i][step + 8 * g + 4 * h]);
-                x[4 * h] = u.x, x[4 * h + 1] = u.y, x[4 * h + 2] = u.z, x[4 * h + 3] = u.w;
+            for (int tt = 0; tt < TT; tt++) {
+                // (t holds zeros behind the last rank, so that the operand may start anywhere)
+                const int at = r0 + step + 8 * g, from = eight_from(at, a.R) - r0;
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = r0 + from + e < at || from + e < 0 ? 0.0f : t[16 * tt + i][max(from + e, 0)];
+                tp[tt] = cut8<3>(x);
             }
-            const Pieces<3> tp = cut8<3>(x);
-            each_adapter(mine, [&](int id, bool match) {
-                const W* B = reinterpret_cast<const W*>(a.B) + (int64_t)id * a.N * a.R;
+            for (int c0 = 0; c0 < count; c0 += U) {
+                int id[U];
+                Raw w[U][CT];
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const int col = min(n0 + 16 * n + i, a.N - 1);
-                    const auto w = Weight<W>::template load<VEC>(B + (int64_t)col * a.R, r0 + step + 8 * g, a.R);
-                    const v4f sum = times(w, tp, acc[n]);
+                for (int u = 0; u < U; u++) {
+                    id[u] = __builtin_amdgcn_readfirstlane(list.id[min(c0 + u, count - 1)]);
 #pragma unroll
-                    for (int v = 0; v < 4; v++) acc[n][v] = match ? sum[v] : acc[n][v];
+                    for (int c = 0; c < CT; c++) w[u][c] = load8_end<SHORT>(B[c] + id[u] * adapter, r0 + step + 8 * g, a.R);
                 }
-            });
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (c0 + u >= count) break;
+#pragma unroll
+                    for (int c = 0; c < CT; c++) {
+                        const auto wp = Weight<W>::cut(w[u][c]);
+#pragma unroll
+                        for (int tt = 0; tt < TT; tt++) acc[c][tt] = keep(mine[tt] == id[u], times(wp, tp[tt], acc[c][tt]), acc[c][tt]);
+                    }
+                }
+            }
         }
     }
-    if (row >= a.rows) return;
-    const int b = row / a.tokens, l = row - b * a.tokens;
-    const float* y = a.y + b * a.ysb + l * a.ysl;
-    float* out = a.out + b * a.osb + l * a.osl;
-    const float scale = mine >= 0 ? a.scales[mine] : 0.0f;
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-        const int col = n0 + 16 * n + 4 * g;
-        if (vec_out && col + 4 <= a.N) {
-            float4 u = *reinterpret_cast<const float4*>(y + col);
-            if (mine >= 0) u = make_float4(fmaf(scale, acc[n][0], u.x), fmaf(scale, acc[n][1], u.y), fmaf(scale, acc[n][2], u.z), fmaf(scale, acc[n][3], u.w));
-            *reinterpret_cast<float4*>(out + col) = u;
-        } else {
+    for (int tt = 0; tt < TT; tt++) {
+        if (row0 + 16 * tt + i >= a.rows) continue;
+        const float scale = mine[tt] >= 0 ? a.scales[mine[tt]] : 0.0f;
 #pragma unroll
-            for (int v = 0; v < 4; v++)
-                if (col + v < a.N) out[col + v] = mine >= 0 ? fmaf(scale, acc[n][v], y[col + v]) : y[col + v];
+        for (int c = 0; c < CT; c++) {
+            const int col = n0 + 16 * c + 4 * g;
+            float4 u = yv[c][tt];
+            if (mine[tt] >= 0)
+                u = make_float4(fmaf(scale, acc[c][tt][0], u.x), fmaf(scale, acc[c][tt][1], u.y), fmaf(scale, acc[c][tt][2], u.z), fmaf(scale, acc[c][tt][3], u.w));
+            if (vec_out && col + 4 <= a.N) {
+                *reinterpret_cast<float4*>(out[tt] + col) = u;
+            } else {
+                const float* from = reinterpret_cast<const float*>(&u);
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    if (col + v < a.N) out[tt][col + v] = from[v];
+            }
         }
     }
 }
 
-// K in runs: until there are some 512 workgroups, a run at least 128
-static int lora_splits(int64_t rows, int64_t K, int64_t R) {
-    const int64_t groups = (rows + 15) / 16 * ((R + 63) / 64), most = (K + 127) / 128;
-    int64_t n = (512 + groups - 1) / groups;
-    n = n < most ? n : most;
-    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+// Tokens to a workgroup: 32 where there are enough of them to fill the chip so
+static int lora_tiles(int64_t rows) { return rows > 256 ? 2 : 1; }
+// K in runs, until there are some 256 workgroups.  A run is at least 1024 (four steps to a wave, asked for at once) where a tile has one
+// adapter or two; the weights of several fill the wait of one step.
+static int lora_chunk(int64_t batch, int64_t tokens, int64_t K, int64_t R, int64_t adapters) {
+    const int64_t rows = batch * tokens, tile = 16 * lora_tiles(rows), groups = (rows + tile - 1) / tile * ((R + 63) / 64);
+    const int64_t sequences = (tile + tokens - 1) / tokens + 1, several = sequences < batch ? sequences : batch;
+    const int64_t least = (several < adapters ? several : adapters) > 2 ? 256 : 1024;
+    const int64_t n = (256 + groups - 1) / groups;
+    return (int)((K + least * n - 1) / (least * n) * least);
 }
 
 template <typename W>
-static int lora_launch(LoraArgs a, bool vec_down, bool vec_up, bool vec_out, hipStream_t st) {
-    const unsigned tiles = (unsigned)((a.rows + 15) / 16);
-    const int nr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
+static int lora_launch(LoraArgs a, bool vec_out, hipStream_t st) {
+    const int tt = lora_tiles(a.rows), nr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
+    const unsigned tiles = (unsigned)((a.rows + 16 * tt - 1) / (16 * tt));
     const dim3 down(tiles, (unsigned)a.splits, (unsigned)((a.R + 16 * nr - 1) / (16 * nr)));
-#define LLMOPS_DOWN(NR)                                                          \
-    if (vec_down) lora_down_kernel<W, NR, true><<<down, 256, 0, st>>>(a);        \
-    else lora_down_kernel<W, NR, false><<<down, 256, 0, st>>>(a)
-    if (nr == 1) {
-        LLMOPS_DOWN(1);
-    } else if (nr == 2) {
-        LLMOPS_DOWN(2);
-    } else {
-        LLMOPS_DOWN(4);
-    }
+#define LLMOPS_DOWN(NR, TT) lora_down_kernel<W, NR, TT, false><<<down, 64 * kDownWaves, 0, st>>>(a)
+    if (a.K < 8) lora_down_kernel<W, 4, 1, true><<<dim3((unsigned)((a.rows + 15) / 16), 1, (unsigned)((a.R + 63) / 64)), 64 * kDownWaves, 0, st>>>(a);
+    else if (tt == 1 && nr == 1) LLMOPS_DOWN(1, 1);
+    else if (tt == 1 && nr == 2) LLMOPS_DOWN(2, 1);
+    else if (tt == 1) LLMOPS_DOWN(4, 1);
+    else if (nr == 1) LLMOPS_DOWN(1, 2);
+    else if (nr == 2) LLMOPS_DOWN(2, 2);
+    else LLMOPS_DOWN(4, 2);
 #undef LLMOPS_DOWN
     LLMOPS_LAUNCH_CHECK();
-    const dim3 up((unsigned)((a.N + 255) / 256), tiles);
-    if (vec_up) lora_up_kernel<W, true><<<up, 256, 0, st>>>(a, vec_out);
-    else lora_up_kernel<W, false><<<up, 256, 0, st>>>(a, vec_out);
+    // few tokens: 64 columns to a workgroup, so that there are enough of them, and the weights of eight adapters on their way
+    const int ct = tt == 1 ? 1 : 4;
+    const dim3 up((unsigned)((a.N + 64 * ct - 1) / (64 * ct)), tiles);
+    if (tt == 1 && a.R < 8) lora_up_kernel<W, 1, 1, true><<<up, 256, 0, st>>>(a, vec_out);
+    else if (tt == 1) lora_up_kernel<W, 1, 1, false><<<up, 256, 0, st>>>(a, vec_out);
+    else if (a.R < 8) lora_up_kernel<W, 4, 2, true><<<up, 256, 0, st>>>(a, vec_out);
+    else lora_up_kernel<W, 4, 2, false><<<up, 256, 0, st>>>(a, vec_out);
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }
@@ -288,9 +468,10 @@ static bool lora_sizes_fit(int64_t batch, int64_t tokens, int64_t N, int64_t K, 
            batch * tokens <= 65535 * 16;
 }
 
-extern "C" size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R) {
-    if (!lora_sizes_fit(batch, tokens, N, K, R)) return 0;
-    return (size_t)lora_splits(batch * tokens, K, R) * (size_t)(batch * tokens) * (size_t)R * sizeof(float);
+extern "C" size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R, int64_t adapters) {
+    if (!lora_sizes_fit(batch, tokens, N, K, R) || adapters <= 0) return 0;
+    const int64_t chunk = lora_chunk(batch, tokens, K, R, adapters);
+    return (size_t)((K + chunk - 1) / chunk) * (size_t)(batch * tokens) * (size_t)R * sizeof(float);
 }
 
 extern "C" int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, const float* x, int64_t x_stride_b, int64_t x_stride_l, int64_t batch,
@@ -303,7 +484,7 @@ extern "C" int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_str
     LLMOPS_REQUIRE(weight_dtype == LLMOPS_F32 || weight_dtype == LLMOPS_F16 || weight_dtype == LLMOPS_BF16);
     const size_t e = weight_dtype == LLMOPS_F32 ? 4 : 2;
     LLMOPS_REQUIRE(aligned(y, 4) && aligned(x, 4) && aligned(out, 4) && aligned(lora_A, e) && aligned(lora_B, e));
-    const size_t need = llmops_lora_workspace_bytes(batch, tokens, N, K, R);
+    const size_t need = llmops_lora_workspace_bytes(batch, tokens, N, K, R, adapters);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(LLMOPS_EWORKSPACE, "lora_add needs %zu workspace bytes, got %zu", need, workspace == nullptr ? (size_t)0 : workspace_bytes);
     LLMOPS_REQUIRE(aligned(workspace, 4));
@@ -311,14 +492,11 @@ extern "C" int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_str
     a.x = x, a.y = y, a.scales = scales, a.A = lora_A, a.B = lora_B, a.ids = ids, a.out = out, a.part = reinterpret_cast<float*>(workspace);
     a.xsb = x_stride_b, a.xsl = x_stride_l, a.ysb = y_stride_b, a.ysl = y_stride_l, a.osb = out_stride_b, a.osl = out_stride_l;
     a.rows = (int)(batch * tokens), a.tokens = (int)tokens, a.K = (int)K, a.N = (int)N, a.R = (int)R, a.adapters = (int)adapters;
-    a.splits = lora_splits(a.rows, K, R);
-    a.chunk = (int)((K + 128 * a.splits - 1) / (128 * a.splits) * 128);
+    a.chunk = lora_chunk(batch, tokens, K, R, adapters);
     a.splits = (int)((K + a.chunk - 1) / a.chunk);
-    const bool vec_down = K % 8 == 0 && aligned(x, 16) && x_stride_b % 4 == 0 && x_stride_l % 4 == 0 && aligned(lora_A, 16),
-               vec_up = R % 8 == 0 && aligned(lora_B, 16),
-               vec_out = aligned(y, 16) && aligned(out, 16) && y_stride_b % 4 == 0 && y_stride_l % 4 == 0 && out_stride_b % 4 == 0 && out_stride_l % 4 == 0;
+    const bool vec_out = aligned(y, 16) && aligned(out, 16) && y_stride_b % 4 == 0 && y_stride_l % 4 == 0 && out_stride_b % 4 == 0 && out_stride_l % 4 == 0;
     hipStream_t st = as_stream(stream);
-    if (weight_dtype == LLMOPS_F32) return lora_launch<float>(a, vec_down, vec_up, vec_out, st);
-    if (weight_dtype == LLMOPS_F16) return lora_launch<Half16>(a, vec_down, vec_up, vec_out, st);
-    return lora_launch<Bf16>(a, vec_down, vec_up, vec_out, st);
+    if (weight_dtype == LLMOPS_F32) return lora_launch<float>(a, vec_out, st);
+    if (weight_dtype == LLMOPS_F16) return lora_launch<Half16>(a, vec_out, st);
+    return lora_launch<Bf16>(a, vec_out, st);
 }

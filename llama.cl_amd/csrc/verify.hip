@@ -7,18 +7,19 @@
 // running sum is above u * total.  T not above 0: the likeliest token, the lowest of equals, and drafts that equal it.
 //
 //   1. verify_rows_kernel   per row and run of the vocabulary: maximum, its place, sum of exponentials
-//   2. verify_rest_kernel   how many drafts are accepted; per run, the sum of the distribution that the next token is drawn from
-//   3. verify_pick_kernel   the run, then the token, where the running sum passes
+//   2. verify_next_kernel   how many drafts are accepted; per run, the sum of what the next token is drawn from; the workgroup of a
+//                           sequence that is done last takes the run, then the token, where the running sum passes
 //
 // Answers are whole numbers that a rounding can change: a running sum over V tokens passes a border wrongly once in about
-// 1 / (V * error) draws, so that exponentials and sums are in 64 bits.  A row is read once by 1; 2 and 3 read the one row per sequence
-// that the next token comes from.  Logits that are NaN, and minus infinity, weigh nothing; plus infinities share the row.
+// 1 / (V * error) draws, so that exponentials (to 2e-14) and sums are in 64 bits.  A row is read once by 1; 2 reads the one row per
+// sequence that the next token comes from.  Logits that are NaN, and minus infinity, weigh nothing; plus infinities share the row.
 #include <math.h>
 
 #include "common.h"
 
 namespace llmops {
 
+constexpr double kLog2e = 1.4426950408889634;
 constexpr int kRun = 4096;  // logits to a workgroup: 16 to a thread, in registers between maximum and sum
 
 struct VerifyArgs {
@@ -30,219 +31,317 @@ struct VerifyArgs {
     int64_t *tokens;
     int32_t* accepted;
     double *sum, *rest;  // [B*(K+1)][runs], [B][runs]
+    int32_t* arrived;    // [B]
     float* top;          // [B*(K+1)][runs]
     int32_t* place;      // [B*(K+1)][runs]
 };
 
 __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int b) { return a.draft_lens != nullptr ? max(0, min(a.draft_lens[b], a.K)) : a.K; }
 __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int b) { return a.temperature != nullptr ? a.temperature[b] : a.one_temperature; }
-// exp((z - top) / T); a row without a value above minus infinity has no weight anywhere
-__device__ __forceinline__ double weight(float z, float top, double inv_t) {
+
+// 2^y for y <= 0: a whole power and a polynomial over [-1/2, 1/2] (degree 9, interpolated at Chebyshev's points: off by 1.9e-14 at
+// most, half the instructions of exp(), which is as exact as the type)
+__device__ __forceinline__ double power_of_two(double y) {
+    const double whole = rint(y), f = y - whole;
+    double p = 0x1.b6571de2f2351p-24;
+    p = fma(p, f, 0x1.63ef969a64d3cp-20);
+    p = fma(p, f, 0x1.ffcb76789860fp-17);
+    p = fma(p, f, 0x1.43088e257f341p-13);
+    p = fma(p, f, 0x1.5d87fe908f88ap-10);
+    p = fma(p, f, 0x1.3b2ab72b175eep-7);
+    p = fma(p, f, 0x1.c6b08d7044119p-5);
+    p = fma(p, f, 0x1.ebfbdff8149f2p-3);
+    p = fma(p, f, 0x1.62e42fefa39f7p-1);
+    p = fma(p, f, 0x1.000000000003dp+0);
+    return ldexp(p, (int)fmax(whole, -2000.0));
+}
+// exp((z - top) / T), per_t = log2(e) / T; a row without a value above minus infinity has no weight anywhere
+__device__ __forceinline__ double weight(float z, float top, double per_t) {
     if (!(z > -INFINITY)) return 0.0;
-    return z == top ? 1.0 : top == INFINITY ? 0.0 : exp(((double)z - (double)top) * inv_t);
+    return z == top ? 1.0 : top == INFINITY ? 0.0 : power_of_two(((double)z - (double)top) * per_t);
 }
 // what a run's sum counts for beside the row's maximum
-__device__ __forceinline__ double share(float run_top, float top, double inv_t) {
-    return run_top == top ? 1.0 : run_top == -INFINITY || top == INFINITY ? 0.0 : exp(((double)run_top - (double)top) * inv_t);
-}
+__device__ __forceinline__ double share(float run_top, float top, double per_t) { return weight(run_top, top, per_t); }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+// Reductions over a wave whose steps stay in the vector ALU (a step through LDS waits some 100 cycles, and there are eight reductions one
+// behind the other in a call): neighbours at 1, 2, 4, 8 lanes below within rows of 16, then the rows' ends.  `other`: what lanes without
+// a neighbour take, the operation's zero.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t below(uint32_t x, uint32_t other) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)other, (int)x, CTRL, ROWS, 0xf, false);
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float below(float x, float other) {
+    return __uint_as_float(below<CTRL, ROWS>(__float_as_uint(x), __float_as_uint(other)));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double below(double x, double) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)below<CTRL, ROWS>((uint32_t)(u >> 32), 0u) << 32 | below<CTRL, ROWS>((uint32_t)u, 0u));
+}
+// every lane: the lanes up to it and itself
+template <typename V, typename F>
+__device__ __forceinline__ V wave_scan(V v, V zero, F f) {
+    v = f(v, below<0x111, 0xf>(v, zero));
+    v = f(v, below<0x112, 0xf>(v, zero));
+    v = f(v, below<0x114, 0xf>(v, zero));
+    v = f(v, below<0x118, 0xf>(v, zero));
+    v = f(v, below<0x142, 0xa>(v, zero));  // lane 15 to row 1, lane 47 to row 3
+    return f(v, below<0x143, 0xc>(v, zero));  // lane 31 to rows 2 and 3
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ float lane_of(float v, int lane) { return __uint_as_float(lane_of(__float_as_uint(v), lane)); }
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)lane_of((uint32_t)(u >> 32), lane) << 32 | lane_of((uint32_t)u, lane));
+}
+__device__ __forceinline__ double scan64(double v) { return wave_scan(v, 0.0, [](double x, double y) { return x + y; }); }
+__device__ __forceinline__ double wave_sum64(double v) { return lane_of(scan64(v), 63); }
+__device__ __forceinline__ float wave_top(float v) {
+    return lane_of(wave_scan(v, -INFINITY, [](float x, float y) { return fmaxf(x, y); }), 63);
+}
+__device__ __forceinline__ uint32_t wave_least(uint32_t v) {
+    return lane_of(wave_scan(v, 0xffffffffu, [](uint32_t x, uint32_t y) { return x < y ? x : y; }), 63);
+}
+constexpr uint32_t kNowhere = 0x7fffffff;
 
 __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     __shared__ float tops[4];
-    __shared__ int places[4];
+    __shared__ uint32_t places[4];
     __shared__ double sums[4];
     const int row = blockIdx.x, run = blockIdx.y, b = row / (a.K + 1), i = row - b * (a.K + 1);
     if (i > drafts_of(a, b)) return;  // (a row behind the last draft's is not looked at)
-    const float t = temperature_of(a, b);
+    if (i == 0 && run == 0 && threadIdx.x == 0) a.arrived[b] = 0;  // (for the launch behind this one)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j0 = run * kRun;
     const float* z = a.logits + (int64_t)row * a.V + j0;
     const int n = min(kRun, a.V - j0);
     float x[16];
-    float top = -INFINITY;
-    int place = 0x7fffffff;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
         const int j = threadIdx.x + 256 * e;
         x[e] = j < n ? z[j] : -INFINITY;
-        if (x[e] > top) top = x[e], place = j0 + j;
     }
+    const float t = temperature_of(a, b);
+    float top = -INFINITY;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float y = __shfl_xor(top, o, 64);
-        const int p = __shfl_xor(place, o, 64);
-        if (y > top || (y == top && p < place)) top = y, place = p;
-    }
-    if (lane == 0) tops[wave] = top, places[wave] = place;
-    __syncthreads();
-    top = tops[0], place = places[0];
+    for (int e = 0; e < 16; e++) top = fmaxf(top, x[e]);
+    top = wave_top(top);
+    if (t > 0.0f) {  // sums beside a wave's own maximum: the waves meet once
+        const double per_t = kLog2e / (double)t;
+        double sum = 0.0;
 #pragma unroll
-    for (int w = 1; w < 4; w++)
-        if (tops[w] > top || (tops[w] == top && places[w] < place)) top = tops[w], place = places[w];
-    double sum = 0.0;
-    if (t > 0.0f) {
-        const double inv_t = 1.0 / (double)t;
-#pragma unroll
-        for (int e = 0; e < 16; e++) sum += weight(x[e], top, inv_t);
+        for (int e = 0; e < 16; e++) sum += weight(x[e], top, per_t);
         sum = wave_sum64(sum);
-        if (lane == 0) sums[wave] = sum;
+        if (lane == 0) tops[wave] = top, sums[wave] = sum;
         __syncthreads();
-        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    }
-    if (threadIdx.x == 0) {
-        const int64_t at = (int64_t)row * a.runs + run;
-        a.top[at] = top;
-        a.place[at] = place;
-        a.sum[at] = sum;
+        if (wave != 0) return;
+        const float mine = tops[lane & 3], all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        sum = wave_sum64(lane < 4 ? sums[lane] * share(mine, all, per_t) : 0.0);
+        if (lane == 0) a.top[(int64_t)row * a.runs + run] = all, a.sum[(int64_t)row * a.runs + run] = sum;
+    } else {
+        uint32_t place = kNowhere;
+#pragma unroll
+        for (int e = 15; e >= 0; e--)
+            if (x[e] == top && top > -INFINITY) place = j0 + threadIdx.x + 256 * e;
+        place = wave_least(place);
+        if (lane == 0) tops[wave] = top, places[wave] = place;
+        __syncthreads();
+        if (wave != 0) return;
+        const float mine = tops[lane & 3], all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        place = wave_least(mine == all ? places[lane & 3] : kNowhere);
+        if (lane == 0) a.top[(int64_t)row * a.runs + run] = all, a.place[(int64_t)row * a.runs + run] = (int)place;
     }
 }
 
-// a row's maximum, its place, its sum, by one thread
+// a row's maximum; the maximum's place (-1: there is none) or, where tokens are drawn, the sum and its inverse: by one wave, a run to a lane
 struct Row {
     float top;
     int place;
-    double sum;
+    double sum, inv;
 };
-__device__ __forceinline__ Row row_of(const VerifyArgs& a, int row, double inv_t) {
-    Row r{-INFINITY, -1, 0.0};
+__device__ __forceinline__ Row row_of(const VerifyArgs& a, int row, bool draws, double per_t, int lane) {
+    Row r{-INFINITY, -1, 0.0, 0.0};
     const int64_t at = (int64_t)row * a.runs;
-    for (int c = 0; c < a.runs; c++)
-        if (a.top[at + c] > r.top) r.top = a.top[at + c], r.place = a.place[at + c];
-    for (int c = 0; c < a.runs; c++) r.sum += a.sum[at + c] * share(a.top[at + c], r.top, inv_t);
-    return r;
-}
-__device__ __forceinline__ bool draft_fits(const VerifyArgs& a, int b, int i, float t, double inv_t) {
-    const int64_t x = a.drafts[(int64_t)b * a.K + i];
-    if (x < 0 || x >= a.V) return false;
-    const int row = b * (a.K + 1) + i;
-    const Row r = row_of(a, row, inv_t);
-    if (!(t > 0.0f)) return x == r.place;
-    const double q = a.probs != nullptr ? (double)a.probs[((int64_t)b * a.K + i) * a.V + x] : 1.0;
-    return (double)a.uniforms[(int64_t)b * (a.K + 1) + i] * q * r.sum < weight(a.logits[(int64_t)row * a.V + x], r.top, inv_t);
-}
-// how many drafts are accepted, by the whole workgroup
-__device__ __forceinline__ int accepted_of(const VerifyArgs& a, int b, int n, float t, double inv_t, int* shared) {
-    if (threadIdx.x == 0) *shared = n;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += blockDim.x)
-        if (!draft_fits(a, b, i, t, inv_t)) atomicMin(shared, i);
-    __syncthreads();
-    return *shared;
-}
-
-// what token j of a row weighs for the next token; q: the draft's distribution (or null), x: a draft without one (or -1)
-__device__ __forceinline__ double rest_weight(const Row& r, float z, double inv_t, const float* q, int64_t x, int j) {
-    const double p = weight(z, r.top, inv_t) / r.sum;
-    if (q != nullptr) {
-        const double d = p - (double)q[j];
-        return d > 0.0 ? d : 0.0;
-    }
-    return j == x ? 0.0 : p;
-}
-
-__device__ __forceinline__ double block_sum64(double v, double* red) {
-    v = wave_sum64(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    const double s = (red[0] + red[1]) + (red[2] + red[3]);
-    __syncthreads();
-    return s;
-}
-
-// threads take 16 neighbours each, so that sums run in the tokens' order
-__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs a) {
-    __shared__ int shared;
-    __shared__ Row shared_row;
-    __shared__ double red[4];
-    const int b = blockIdx.x, run = blockIdx.y, n = drafts_of(a, b);
-    const float t = temperature_of(a, b);
-    const double inv_t = 1.0 / (double)t;
-    const int done = accepted_of(a, b, n, t, inv_t, &shared);
-    if (run == 0 && threadIdx.x == 0) a.accepted[b] = done;
-    if (!(t > 0.0f)) return;
-    const int row = b * (a.K + 1) + done;
-    if (threadIdx.x == 0) shared_row = row_of(a, row, inv_t);
-    __syncthreads();
-    const Row r = shared_row;
-    const bool refused = done < n;
-    const float* q = refused && a.probs != nullptr ? a.probs + ((int64_t)b * a.K + done) * a.V : nullptr;
-    const int64_t x = refused && a.probs == nullptr ? a.drafts[(int64_t)b * a.K + done] : -1;
-    const int j0 = run * kRun + 16 * threadIdx.x, j1 = min(a.V, j0 + 16);
-    double sum = 0.0;
-    for (int j = j0; j < j1; j++) sum += rest_weight(r, a.logits[(int64_t)row * a.V + j], inv_t, q, x, j);
-    sum = block_sum64(sum, red);
-    if (threadIdx.x == 0) a.rest[(int64_t)b * a.runs + run] = sum;
-}
-
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a) {
-    __shared__ Row shared_row;
-    __shared__ double sums[256];
-    __shared__ int found, last;
-    const int b = blockIdx.x, n = drafts_of(a, b), done = a.accepted[b], row = b * (a.K + 1) + done;
-    const float t = temperature_of(a, b);
-    const double inv_t = 1.0 / (double)t;
-    if (threadIdx.x == 0) shared_row = row_of(a, row, inv_t), found = 0x7fffffff, last = -1;
-    __syncthreads();
-    const Row r = shared_row;
-    int64_t* tokens = a.tokens + (int64_t)b * (a.K + 1);
-    for (int i = threadIdx.x; i <= a.K; i += 256)
-        if (i != done) tokens[i] = i < done ? a.drafts[(int64_t)b * a.K + i] : -1;
-    if (!(t > 0.0f) || r.top == -INFINITY) {  // the likeliest; nothing to take: none
-        if (threadIdx.x == 0) tokens[done] = r.place;
-        return;
-    }
-    const bool refused = done < n;
-    const float* q = refused && a.probs != nullptr ? a.probs + ((int64_t)b * a.K + done) * a.V : nullptr;
-    int64_t x = refused && a.probs == nullptr ? a.drafts[(int64_t)b * a.K + done] : -1;
-    const double* rest = a.rest + (int64_t)b * a.runs;
-    double total = 0.0;
-    for (int c = 0; c < a.runs; c++) total += rest[c];
-    const bool none = !(total > 0.0);  // nothing above the draft's distribution: the target's own
-    if (none) q = nullptr, x = -1;
-    const int64_t at = (int64_t)row * a.runs;
-    auto run_sum = [&](int c) { return none ? a.sum[at + c] * share(a.top[at + c], r.top, inv_t) / r.sum : rest[c]; };
-    if (none) {
-        total = 0.0;
-        for (int c = 0; c < a.runs; c++) total += run_sum(c);
-    }
-    const double goal = (double)a.uniforms[(int64_t)b * (a.K + 1) + a.K] * total;
-    double before = 0.0;
-    int run = 0, heavy = 0;
-    double heavy_before = 0.0;
-    for (; run < a.runs; run++) {
-        const double s = run_sum(run);
-        if (s > 0.0) heavy = run, heavy_before = before;
-        if (before + s > goal) break;
-        before += s;
-    }
-    if (run == a.runs) run = heavy, before = heavy_before;  // (rounding, or a random number of 1: the last token with a weight)
-    const int j0 = run * kRun + 16 * threadIdx.x, j1 = min(a.V, j0 + 16);
-    double sum = 0.0;
-    for (int j = j0; j < j1; j++) sum += rest_weight(r, a.logits[(int64_t)row * a.V + j], inv_t, q, x, j);
-    sums[threadIdx.x] = sum;
-    __syncthreads();
-    for (unsigned u = 0; u < threadIdx.x; u++) before += sums[u];
-    for (int j = j0; j < j1; j++) {
-        const double w = rest_weight(r, a.logits[(int64_t)row * a.V + j], inv_t, q, x, j);
-        before += w;
-        if (w > 0.0) {
-            atomicMax(&last, j);
-            if (before > goal) {
-                atomicMin(&found, j);
-                break;
-            }
+    for (int c0 = 0; c0 < a.runs; c0 += 64) {
+        const bool has = c0 + lane < a.runs;
+        const float mine = has ? a.top[at + c0 + lane] : -INFINITY;
+        if (draws) {
+            const double sum = has ? a.sum[at + c0 + lane] : 0.0;
+            const float up = fmaxf(r.top, wave_top(mine));
+            r.sum = r.sum * share(r.top, up, per_t) + wave_sum64(sum * share(mine, up, per_t));
+            r.top = up;
+        } else {
+            const uint32_t place = has ? (uint32_t)a.place[at + c0 + lane] : kNowhere;
+            const float top = wave_top(mine);
+            const uint32_t least = wave_least(mine == top ? place : kNowhere);
+            if (top > r.top) r.top = top, r.place = (int)least;
         }
     }
+    r.inv = 1.0 / r.sum;
+    return r;
+}
+
+// what token j of a row weighs for the next token; q: its weight in the draft's distribution (behind a refused draft that has one)
+__device__ __forceinline__ double rest_weight(const Row& r, float z, double per_t, bool less, float q, bool out) {
+    const double p = weight(z, r.top, per_t) * r.inv;
+    if (less) return fmax(p - (double)q, 0.0);
+    return out ? 0.0 : p;
+}
+
+__global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
+    __shared__ int first, arrivals, found, last;
+    __shared__ Row shared_row;
+    __shared__ double red[4];
+    __shared__ float neighbours[2][kRun + kRun / 16];  // (16 in a row and a gap: a thread's on banks of their own)
+    const int b = blockIdx.x / (unsigned)a.runs, run = blockIdx.x - b * a.runs, n = drafts_of(a, b), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float t = temperature_of(a, b);
+    const bool draws = t > 0.0f;
+    const double per_t = draws ? kLog2e / (double)t : 0.0;
+    if (!draws && run > 0) return;  // (the likeliest token needs no sums)
+    if (threadIdx.x == 0) first = n;
     __syncthreads();
-    if (threadIdx.x == 0) tokens[done] = found != 0x7fffffff ? found : last;
+    // drafts, four at a time, until one is refused
+    const int row0 = b * (a.K + 1);
+    const float* probs = a.probs != nullptr ? a.probs + (int64_t)b * a.K * a.V : nullptr;
+    for (int i0 = 0; i0 <= n; i0 += 4) {
+        const int i = i0 + wave;
+        Row r{};
+        if (i <= n) {
+            const int64_t x = i < n ? a.drafts[(int64_t)b * a.K + i] : -1;
+            const bool inside = x >= 0 && x < a.V;
+            const float z = inside ? a.logits[(int64_t)(row0 + i) * a.V + x] : -INFINITY;
+            const double q = inside && probs != nullptr ? (double)probs[(int64_t)i * a.V + x] : 1.0;
+            const double u = (double)a.uniforms[row0 + i];
+            r = row_of(a, row0 + i, draws, per_t, lane);
+            const bool fits = inside && (draws ? u * q * r.sum < weight(z, r.top, per_t) : x == r.place);
+            if (lane == 0 && i < n && !fits) atomicMin(&first, i);
+        }
+        __syncthreads();
+        const int done = first;
+        if (done == i && lane == 0) shared_row = r;
+        __syncthreads();
+        if (done < i0 + 4) break;
+    }
+    const int done = first, row = row0 + done;
+    const Row r = shared_row;
+    const bool refused = done < n;
+    const float *zrow = a.logits + (int64_t)row * a.V, *qrow = refused && probs != nullptr ? probs + (int64_t)done * a.V : nullptr;
+    bool less = qrow != nullptr;
+    int64_t x = refused && qrow == nullptr ? a.drafts[(int64_t)b * a.K + done] : -1;
+    int64_t* tokens = a.tokens + row0;
+    if (run == 0) {
+        if (threadIdx.x == 0) a.accepted[b] = done;
+        for (int i = threadIdx.x; i <= a.K; i += 256)
+            if (i != done) tokens[i] = i < done ? a.drafts[(int64_t)b * a.K + i] : -1;
+    }
+    if (!draws || r.top == -INFINITY) {  // the likeliest; nothing to take: none
+        if (run == 0 && threadIdx.x == 0) tokens[done] = r.place;
+        return;
+    }
+    double* rest = a.rest + (int64_t)b * a.runs;
+    // j of a thread's value e; what lies behind the row weighs nothing
+    auto z_at = [&](int at_run, int e) {
+        const int j = at_run * kRun + threadIdx.x + 256 * e;
+        return j < a.V ? zrow[j] : -INFINITY;
+    };
+    auto q_at = [&](int at_run, int e) {
+        const int j = at_run * kRun + threadIdx.x + 256 * e;
+        return qrow != nullptr && j < a.V ? qrow[j] : 0.0f;
+    };
+    float z[16], q[16];
+#pragma unroll
+    for (int e = 0; e < 16; e++) z[e] = z_at(run, e), q[e] = q_at(run, e);
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < 16; e++) sum += rest_weight(r, z[e], per_t, less, q[e], run * kRun + (int)threadIdx.x + 256 * e == x);
+    sum = wave_sum64(sum);
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        // the exchange has come back before the arrival is counted: whoever counts the last one finds every sum.  (Nothing else is handed
+        // over; a release and an acquire of the device's scope would write back and empty the L2 in every workgroup.)
+        double before = __hip_atomic_exchange(&rest[run], (red[0] + red[1]) + (red[2] + red[3]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("" : "+v"(before) : : "memory");
+        arrivals = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        found = (int)kNowhere, last = -1;
+    }
+    __syncthreads();
+    if (arrivals != a.runs - 1) return;
+
+    // the last one: every wave finds the run, a run to a lane
+    const int64_t at = (int64_t)row * a.runs;
+    auto run_sum = [&](int c, bool own) {
+        if (c >= a.runs) return 0.0;
+        return own ? a.sum[at + c] * share(a.top[at + c], r.top, per_t) * r.inv : __hip_atomic_load(&rest[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    double total = 0.0;
+    for (int c0 = 0; c0 < a.runs; c0 += 64) total += wave_sum64(run_sum(c0 + lane, false));
+    const bool none = !(total > 0.0);  // nothing above the draft's distribution: the target's own
+    if (none) {
+        less = false, x = -1, total = 0.0;
+        for (int c0 = 0; c0 < a.runs; c0 += 64) total += wave_sum64(run_sum(c0 + lane, true));
+    }
+    const double goal = (double)a.uniforms[row0 + a.K] * total;
+    double before = 0.0, heavy_before = 0.0;  // sums of the runs before the one, and before the last with a weight
+    int at_run = -1, heavy = 0;
+    for (int c0 = 0; c0 < a.runs && at_run < 0; c0 += 64) {
+        const double mine = run_sum(c0 + lane, none);
+        const double to = before + scan64(mine);  // up to and with this lane's run
+        const uint64_t past = __ballot(to > goal && mine > 0.0), some = __ballot(mine > 0.0);
+        if (some != 0) {
+            const int h = 63 - __builtin_clzll(some);
+            heavy = c0 + h;
+            heavy_before = h > 0 ? lane_of(to, h - 1) : before;
+        }
+        if (past != 0) {
+            const int f = __builtin_ctzll(past);
+            at_run = c0 + f;
+            before = f > 0 ? lane_of(to, f - 1) : before;
+        } else {
+            before = lane_of(to, 63);
+        }
+    }
+    if (at_run < 0) at_run = heavy, before = heavy_before;  // (rounding, or a random number of 1: the last token with a weight)
+    // its tokens in their order, 16 to a thread
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const int at = threadIdx.x + 256 * e + (threadIdx.x >> 4) + 16 * e;
+        neighbours[0][at] = z_at(at_run, e);
+        neighbours[1][at] = q_at(at_run, e);
+    }
+    __syncthreads();
+    const int j0 = at_run * kRun + 16 * threadIdx.x;
+    double w[16];
+    sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        w[e] = rest_weight(r, neighbours[0][17 * threadIdx.x + e], per_t, less, neighbours[1][17 * threadIdx.x + e], j0 + e == x);
+        sum += w[e];
+    }
+    const double to = scan64(sum);
+    if (lane == 63) red[wave] = to;
+    __syncthreads();
+    for (int u = 0; u < wave; u++) before += red[u];
+    before += to - sum;
+    int mine = (int)kNowhere, some = -1;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        before += w[e];
+        if (w[e] > 0.0) {
+            some = j0 + e;
+            if (before > goal) mine = min(mine, j0 + e);
+        }
+    }
+    mine = (int)wave_least((uint32_t)mine);
+    const uint64_t with = __ballot(some >= 0);
+    some = with != 0 ? (int)lane_of((uint32_t)some, 63 - __builtin_clzll(with)) : -1;  // (the highest lane has the highest tokens)
+    if (lane == 0) atomicMin(&found, mine), atomicMax(&last, some);
+    __syncthreads();
+    if (threadIdx.x == 0) tokens[done] = found != (int)kNowhere ? found : last;
 }
 
 struct VerifyLayout {
-    size_t sum, rest, top, place, total;
+    size_t sum, rest, top, place, arrived, total;
 };
 static VerifyLayout layout_verify(int64_t B, int64_t K, int64_t runs) {
     VerifyLayout w{};
@@ -251,7 +350,8 @@ static VerifyLayout layout_verify(int64_t B, int64_t K, int64_t runs) {
     w.rest = w.sum + rows * 8;
     w.top = w.rest + (size_t)(B * runs) * 8;
     w.place = w.top + rows * 4;
-    w.total = w.place + rows * 4;
+    w.arrived = w.place + rows * 4;
+    w.total = w.arrived + (size_t)B * 4;
     return w;
 }
 
@@ -277,6 +377,7 @@ extern "C" int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, i
     LLMOPS_REQUIRE(aligned(logits, 4) && aligned(draft_probs, 4) && aligned(uniforms, 4) && aligned(drafts, 8) && aligned(tokens, 8));
     VerifyArgs a{};
     a.runs = (int)((V + kRun - 1) / kRun);
+    LLMOPS_REQUIRE(B * a.runs < ((int64_t)1 << 31));
     const VerifyLayout w = layout_verify(B, K, a.runs);
     if (workspace == nullptr || workspace_bytes < w.total)
         return fail(LLMOPS_EWORKSPACE, "verify_drafts needs %zu workspace bytes, got %zu", w.total, workspace == nullptr ? (size_t)0 : workspace_bytes);
@@ -286,13 +387,11 @@ extern "C" int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, i
     a.one_temperature = one_temperature;
     a.B = (int)B, a.K = (int)K, a.V = (int)V, a.tokens = tokens, a.accepted = accepted;
     a.sum = reinterpret_cast<double*>(ws + w.sum), a.rest = reinterpret_cast<double*>(ws + w.rest), a.top = reinterpret_cast<float*>(ws + w.top);
-    a.place = reinterpret_cast<int32_t*>(ws + w.place);
+    a.place = reinterpret_cast<int32_t*>(ws + w.place), a.arrived = reinterpret_cast<int32_t*>(ws + w.arrived);
     hipStream_t st = as_stream(stream);
     verify_rows_kernel<<<dim3((unsigned)(B * (K + 1)), (unsigned)a.runs), 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
-    verify_rest_kernel<<<dim3((unsigned)B, (unsigned)a.runs), 256, 0, st>>>(a);
-    LLMOPS_LAUNCH_CHECK();
-    verify_pick_kernel<<<(unsigned)B, 256, 0, st>>>(a);
+    verify_next_kernel<<<(unsigned)(B * a.runs), 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }

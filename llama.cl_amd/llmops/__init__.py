@@ -616,7 +616,7 @@ def lora_add(y, x, lora_A, lora_B, adapters, scales, out=None):
     _require(tuple(out.shape) == (B, M, N) and (B == 1 or abs(ob) >= N) and (M == 1 or abs(ol) >= N), "out.is({B, M, N}), rows apart")
     _here(y, x=x, lora_A=lora_A, lora_B=lora_B, adapters=adapters, scales=scales, out=out)
     lib = _lib.load()
-    ws = torch.empty(max(lib.llmops_lora_workspace_bytes(B, M, N, K, R), 1), dtype=torch.uint8, device=y.device)
+    ws = torch.empty(max(lib.llmops_lora_workspace_bytes(B, M, N, K, R, n), 1), dtype=torch.uint8, device=y.device)
     _on_device(y.device, lib.llmops_lora_add, yp, yb, yl, xp, xb, xl, B, M, N, K, _ptr(lora_A), _ptr(lora_B), _LORA_TYPES[lora_A.dtype], R, n,
                _ptr(adapters), _ptr(scales), op, ob, ol, _ptr(ws), ws.numel())
     return out

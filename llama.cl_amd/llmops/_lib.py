@@ -52,7 +52,7 @@ SIGNATURES = {
     "llmops_attention_prefix_workspace_bytes": (c_size, [c_i64] * 7),
     "llmops_attention_rope_prefix": (c_int, [c_ptr, c_i64, c_i64] * 3 + [c_i64] * 5 + [c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_int,
                                              c_i64, c_i64, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_size, c_ptr]),
-    "llmops_lora_workspace_bytes": (c_size, [c_i64] * 5),
+    "llmops_lora_workspace_bytes": (c_size, [c_i64] * 6),
     "llmops_lora_add": (c_int, [c_ptr, c_i64, c_i64] * 2 + [c_i64] * 4 + [c_ptr, c_ptr, c_int, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_i64,
                                 c_ptr, c_size, c_ptr]),
     "llmops_verify_drafts_workspace_bytes": (c_size, [c_i64] * 3),

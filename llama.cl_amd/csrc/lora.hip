@@ -25,6 +25,23 @@ struct LoraArgs {
     float *out, *part;   // part [splits][rows][R]
     int64_t xsb, xsl, ysb, ysl, osb, osl;
     int rows, tokens, K, N, R, adapters, splits, chunk;
+    int tiles;  // of a sequence; 0: tiles go on over the sequences' ends
+};
+
+// The tokens of a tile: numbers first .. end - 1.  Sequences of a tile's tokens or more have tiles of their own, so that a tile has one
+// adapter; of shorter ones several share a tile
+struct Tile {
+    int first, end;
+    __device__ __forceinline__ Tile(const LoraArgs& a, int tile, int size) {
+        if (a.tiles > 0) {
+            const int b = tile / a.tiles;
+            first = b * a.tokens + (tile - b * a.tiles) * size;
+            end = min(first + size, (b + 1) * a.tokens);
+        } else {
+            first = tile * size;
+            end = min(first + size, a.rows);
+        }
+    }
 };
 
 template <int N>
@@ -143,54 +160,53 @@ __device__ __forceinline__ v4f keep(bool match, v4f sum, v4f acc) {
 
 constexpr int kDownWaves = 8;
 
-// The adapters that occur among a workgroup's tokens, in the order of their first token
-struct Adapters {
-    int count;
-    int id[32];
-};
 // token `row`'s adapter, -1 for none
-__device__ __forceinline__ int adapter_of(const LoraArgs& a, int row) {
-    if (row >= a.rows) return -1;
-    const int id = a.ids[row / a.tokens];
-    return id >= 0 && id < a.adapters ? id : -1;
+__device__ __forceinline__ int adapter_of(const LoraArgs& a, int row, int end) {
+    const int id = a.ids[min(row, end - 1) / a.tokens];
+    return row < end && id >= 0 && id < a.adapters ? id : -1;
 }
-template <int TT>
-__device__ __forceinline__ void list_adapters(const LoraArgs& a, Adapters& list, int row0) {
-    if (threadIdx.x < 64) {
-        const int mine = (int)threadIdx.x < 16 * TT ? adapter_of(a, row0 + threadIdx.x) : -1;
-        uint64_t todo = __ballot(mine >= 0);
-        int n = 0;
-        while (todo != 0) {
-            const int id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
-            if (threadIdx.x == 0) list.id[n] = id;
-            n++;
-            todo &= ~__ballot(mine == id);
-        }
-        if (threadIdx.x == 0) list.count = n;
+// The adapters that occur among a wave's tokens (token t's in lane t), each once, in the order of their first token
+struct Adapters {
+    int of_lane;
+    uint64_t todo;
+    __device__ __forceinline__ explicit Adapters(int ids) : of_lane(ids), todo(__ballot(ids >= 0)) {}
+    __device__ __forceinline__ int next() {
+        const int id = __builtin_amdgcn_readlane(of_lane, __builtin_ctzll(todo));
+        todo &= ~__ballot(of_lane == id);
+        return id;
     }
-    __syncthreads();
-}
+    // up to U of them; past the last, that one again.  Returns how many
+    template <int U>
+    __device__ __forceinline__ int next(int (&id)[U]) {
+        int n = 1;
+        id[0] = next();
+#pragma unroll
+        for (int u = 1; u < U; u++) {
+            id[u] = id[u - 1];
+            if (todo != 0) id[u] = next(), n = u + 1;
+        }
+        return n;
+    }
+};
 
 // A workgroup: 16 * TT tokens, a run of K (its eight waves an eighth of every 256 each), 16 * NR rows of A.  Bound by latency with few
-// tokens, by reading x with many; so the operands of U steps, or of U adapters, are asked for before the first is used.
+// tokens, by reading x with many; so the operands of two steps are asked for before those of the two before them are used, or those
+// of four adapters at a time.
 // A operand: row of A lane % 16, eight k; B operand: token lane % 16, the same k; result: token lane % 16, rows 4 * (lane / 16) + v.
 template <typename W, int NR, int TT, bool SHORT>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) {
-    constexpr int kStep = 32 * kDownWaves;
-    constexpr int U = sizeof(W) == 4 && NR * TT > 2 ? 2 : 4;
+    constexpr int kStep = 32 * kDownWaves, U = 2, UA = sizeof(W) == 4 && NR * TT > 2 ? 2 : 4;
     typedef typename Weight<W>::Raw Raw;
-    __shared__ Adapters list;
     __shared__ v4f meet[kDownWaves][NR * TT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.x * 16 * TT, r0 = blockIdx.z * 16 * NR;
+    const Tile tile(a, blockIdx.x, 16 * TT);
+    const int row0 = tile.first, r0 = blockIdx.z * 16 * NR;
     const int k0 = blockIdx.y * a.chunk, k1 = min(a.K, k0 + a.chunk);
-    list_adapters<TT>(a, list, row0);
-    const int count = __builtin_amdgcn_readfirstlane(list.count);
-    if (count == 0) return;  // (nobody reads these sums)
+    const int of_lane = adapter_of(a, row0 + (lane & (16 * TT - 1)), tile.end);
     const float* x[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; tt++) {
-        const int row = min(row0 + 16 * tt + i, a.rows - 1), b = row / a.tokens;
+        const int row = min(row0 + 16 * tt + i, tile.end - 1), b = row / a.tokens;
         x[tt] = a.x + b * a.xsb + (row - b * a.tokens) * a.xsl;
     }
     const W* A[NR];  // rows of the adapter with number 0; past the last rank that rank again (not stored)
@@ -202,31 +218,52 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) 
     for (int n = 0; n < NR; n++)
 #pragma unroll
         for (int tt = 0; tt < TT; tt++) acc[n][tt] = v4f{0.f, 0.f, 0.f, 0.f};
-    if (count == 1) {
-        const int64_t at = __builtin_amdgcn_readfirstlane(list.id[0]) * adapter;
-        int k = k0 + 32 * wave;
-        for (; k + kStep * (U - 1) + 32 <= k1; k += kStep * U) {
+    Adapters all(lane < 16 * TT ? of_lane : -1);
+    if (all.todo == 0) return;  // (nobody reads these sums)
+    const int only = all.next();
+    int k = k0 + 32 * wave;
+    if (all.todo == 0) {
+        const int64_t at = only * adapter;
+        struct Stage {
             Raw w[U][NR];
-            Eight32 xr[U][TT];
+            Eight32 x[U][TT];
+        } s0, s1;
+        auto ask = [&](Stage& s, int from) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
 #pragma unroll
-                for (int tt = 0; tt < TT; tt++) xr[u][tt] = load8(x[tt], k + kStep * u + 8 * g);
+                for (int tt = 0; tt < TT; tt++) s.x[u][tt] = load8(x[tt], from + kStep * u + 8 * g);
 #pragma unroll
-                for (int n = 0; n < NR; n++) w[u][n] = load8(A[n] + at, k + kStep * u + 8 * g);
+                for (int n = 0; n < NR; n++) s.w[u][n] = load8(A[n] + at, from + kStep * u + 8 * g);
             }
+        };
+        auto use = [&](const Stage& s) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 Pieces<3> xp[TT];
 #pragma unroll
-                for (int tt = 0; tt < TT; tt++) xp[tt] = Weight<float>::cut(xr[u][tt]);
+                for (int tt = 0; tt < TT; tt++) xp[tt] = Weight<float>::cut(s.x[u][tt]);
 #pragma unroll
                 for (int n = 0; n < NR; n++) {
-                    const auto wp = Weight<W>::cut(w[u][n]);
+                    const auto wp = Weight<W>::cut(s.w[u][n]);
 #pragma unroll
                     for (int tt = 0; tt < TT; tt++) acc[n][tt] = times(wp, xp[tt], acc[n][tt]);
                 }
             }
+        };
+        // (past the last stage that one is asked for again: a wave that may or may not have asked waits for everything)
+        const int reach = kStep * (U - 1) + 32, stages = k1 - k >= reach ? (k1 - k - reach) / (kStep * U) + 1 : 0;
+        const int last = k + (stages - 1) * kStep * U;
+        if (stages > 0) {
+            ask(s0, k);
+            for (int n = 0; n < stages; n += 2) {
+                ask(s1, min(k + kStep * U, last));
+                use(s0);
+                ask(s0, min(k + 2 * kStep * U, last));
+                if (n + 1 < stages) use(s1);
+                k += 2 * kStep * U;
+            }
+            k = last + kStep * U;
         }
         for (; k < k1; k += kStep) {
             Pieces<3> xp[TT];
@@ -242,30 +279,50 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) 
     } else {
         int mine[TT];
 #pragma unroll
-        for (int tt = 0; tt < TT; tt++) mine[tt] = adapter_of(a, row0 + 16 * tt + i);
-        for (int k = k0 + 32 * wave; k < k1; k += kStep) {
+        for (int tt = 0; tt < TT; tt++) mine[tt] = __shfl(of_lane, 16 * tt + i, 64);
+        Adapters some(lane < 16 * TT ? of_lane : -1);
+        struct Stage {
+            int k, n, id[UA];
+            Raw w[UA][NR];
+            Eight32 x[TT];
+        } s0, s1;
+        // the next adapters of this step, or the first of the next; past the last step its first again (not used)
+        auto ask = [&](Stage& s) {
+            if (some.todo == 0) some = Adapters(lane < 16 * TT ? of_lane : -1), k += kStep;
+            s.n = some.next(s.id);
+            s.k = k;
+            const int at = (k < k1 ? k : k - kStep) + 8 * g;
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) s.x[tt] = load8_end<SHORT>(x[tt], at, k1);
+#pragma unroll
+            for (int u = 0; u < UA; u++)
+#pragma unroll
+                for (int n = 0; n < NR; n++) s.w[u][n] = load8_end<SHORT>(A[n] + s.id[u] * adapter, at, k1);
+        };
+        auto use = [&](const Stage& s) {
             Pieces<3> xp[TT];
 #pragma unroll
-            for (int tt = 0; tt < TT; tt++) xp[tt] = cut_end(load8_end<SHORT>(x[tt], k + 8 * g, k1), k + 8 * g, k1);
-            for (int c = 0; c < count; c += U) {
-                int id[U];
-                Raw w[U][NR];
+            for (int tt = 0; tt < TT; tt++) xp[tt] = cut_end(s.x[tt], s.k + 8 * g, k1);
 #pragma unroll
-                for (int u = 0; u < U; u++) {  // (past the last adapter that one again, whose sum is not taken over)
-                    id[u] = __builtin_amdgcn_readfirstlane(list.id[min(c + u, count - 1)]);
+            for (int u = 0; u < UA; u++) {
+                if (u >= s.n) break;
 #pragma unroll
-                    for (int n = 0; n < NR; n++) w[u][n] = load8_end<SHORT>(A[n] + id[u] * adapter, k + 8 * g, k1);
+                for (int n = 0; n < NR; n++) {
+                    const auto wp = Weight<W>::cut(s.w[u][n]);
+#pragma unroll
+                    for (int tt = 0; tt < TT; tt++) acc[n][tt] = keep(mine[tt] == s.id[u], times(wp, xp[tt], acc[n][tt]), acc[n][tt]);
                 }
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (c + u >= count) break;
-#pragma unroll
-                    for (int n = 0; n < NR; n++) {
-                        const auto wp = Weight<W>::cut(w[u][n]);
-#pragma unroll
-                        for (int tt = 0; tt < TT; tt++) acc[n][tt] = keep(mine[tt] == id[u], times(wp, xp[tt], acc[n][tt]), acc[n][tt]);
-                    }
-                }
+            }
+        };
+        if (k < k1) {
+            ask(s0);
+            while (true) {
+                ask(s1);
+                use(s0);
+                if (s1.k >= k1) break;
+                ask(s0);
+                use(s1);
+                if (s0.k >= k1) break;
             }
         }
     }
@@ -279,7 +336,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) 
         v4f s = meet[0][m][lane];
 #pragma unroll
         for (int w = 1; w < kDownWaves; w++) s += meet[w][m][lane];
-        if (row >= a.rows) continue;
+        if (row >= tile.end) continue;
         float* to = a.part + ((int64_t)blockIdx.y * a.rows + row) * a.R + r;
 #pragma unroll
         for (int v = 0; v < 4; v++)
@@ -287,43 +344,40 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) 
     }
 }
 
-// A workgroup: 16 * TT tokens, 64 * CT columns (16 * CT to a wave), ranks 128 at a time; y is asked for first, as it is used last.
+// A workgroup: 16 * TT tokens, 64 * CT columns (16 * CT to a wave), ranks 128 at a time.  Bound by latency: what does not depend on
+// anything (adapters, y, the first partial sums) is asked for at once, and the first weights before the sums are used.
 // A operand: column lane % 16 of B, eight ranks; B operand: token lane % 16, the same ranks; result: token lane % 16, columns 4 * (lane / 16) + v.
 template <typename W, int CT, int TT, bool SHORT>
 __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) {
-    constexpr int kRanks = 128, kStride = kRanks + 4, U = CT == 1 ? 8 : 1;
+    constexpr int kRanks = 128, kStride = kRanks + 4, U = CT == 1 ? 4 : 1;
     typedef typename Weight<W>::Raw Raw;
-    __shared__ Adapters list;
     __shared__ __align__(16) float t[16 * TT][kStride];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.y * 16 * TT, n0 = (blockIdx.x * 4 + wave) * 16 * CT;
+    const Tile tile(a, blockIdx.y, 16 * TT);
+    const int row0 = tile.first, n0 = (blockIdx.x * 4 + wave) * 16 * CT;
+    const int of_lane = adapter_of(a, row0 + (lane & (16 * TT - 1)), tile.end);
     const float* y[TT];
     float* out[TT];
     float4 yv[CT][TT];
 #pragma unroll
     for (int tt = 0; tt < TT; tt++) {
-        const int row = min(row0 + 16 * tt + i, a.rows - 1), b = row / a.tokens, l = row - b * a.tokens;
+        const int row = min(row0 + 16 * tt + i, tile.end - 1), b = row / a.tokens, l = row - b * a.tokens;
         y[tt] = a.y + b * a.ysb + l * a.ysl;
         out[tt] = a.out + b * a.osb + l * a.osl;
-#pragma unroll
-        for (int c = 0; c < CT; c++) {
-            const int col = n0 + 16 * c + 4 * g;
-            yv[c][tt] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (vec_out && col + 4 <= a.N) {
-                yv[c][tt] = *reinterpret_cast<const float4*>(y[tt] + col);
-            } else {
-                float* to = reinterpret_cast<float*>(&yv[c][tt]);
-#pragma unroll
-                for (int v = 0; v < 4; v++)
-                    if (col + v < a.N) to[v] = y[tt][col + v];
-            }
-        }
     }
-    int mine[TT];
+    if (vec_out) {  // (a lane past the last column reads the last four again, and stores nothing)
 #pragma unroll
-    for (int tt = 0; tt < TT; tt++) mine[tt] = adapter_of(a, row0 + 16 * tt + i);
-    list_adapters<TT>(a, list, row0);
-    const int count = __builtin_amdgcn_readfirstlane(list.count);
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) yv[c][tt] = *reinterpret_cast<const float4*>(y[tt] + min(n0 + 16 * c + 4 * g, a.N - 4));
+    } else {
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) reinterpret_cast<float*>(&yv[c][tt])[v] = y[tt][min(n0 + 16 * c + 4 * g + v, a.N - 1)];
+    }
     const W* B[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) B[c] = reinterpret_cast<const W*>(a.B) + (int64_t)min(n0 + 16 * c + i, a.N - 1) * a.R;
@@ -333,7 +387,11 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
     for (int c = 0; c < CT; c++)
 #pragma unroll
         for (int tt = 0; tt < TT; tt++) acc[c][tt] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int r0 = 0; r0 < a.R && count > 0; r0 += kRanks) {
+    const bool any = __ballot(lane < 16 * TT && of_lane >= 0) != 0;  // (the same in the four waves)
+    int mine[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; tt++) mine[tt] = __shfl(of_lane, 16 * tt + i, 64);
+    for (int r0 = 0; r0 < a.R && any; r0 += kRanks) {
         const int ranks = min(kRanks, a.R - r0), padded = (ranks + 31) & ~31;
         if (r0 > 0) __syncthreads();
         // (two values and eight runs at a time: sixteen loads on their way; one by one they were two thirds of a prompt's launch)
@@ -343,7 +401,7 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int e = e0 + 256 * h, token = e / padded, r = e - token * padded;
-                from[h] = e < 16 * TT * padded && r < ranks && row0 + token < a.rows ? a.part + (int64_t)(row0 + token) * a.R + r0 + r : nullptr;
+                from[h] = e < 16 * TT * padded && r < ranks && row0 + token < tile.end ? a.part + (int64_t)(row0 + token) * a.R + r0 + r : nullptr;
                 sum[h] = 0.0f;
             }
             const int64_t run = (int64_t)a.rows * a.R;
@@ -364,43 +422,68 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
                 if (e < 16 * TT * padded) t[token][e - token * padded] = from[h] != nullptr ? sum[h] : 0.0f;
             }
         }
-        __syncthreads();
-        for (int step = 0; step < padded; step += 32) {
-            Pieces<3> tp[TT];
+        Adapters some(lane < 16 * TT ? of_lane : -1);
+        struct Stage {
+            int step, n, id[U];
+            Raw w[U][CT];
+        } s0, s1;
+        int step = 0;
+        auto ask = [&](Stage& s) {  // as above
+            if (some.todo == 0) some = Adapters(lane < 16 * TT ? of_lane : -1), step += 32;
+            s.n = some.next(s.id);
+            s.step = step;
+            const int at = r0 + (step < padded ? step : step - 32) + 8 * g;
 #pragma unroll
-            for (int tt = 0; tt < TT; tt++) {
-                // (t holds zeros behind the last rank, so that the operand may start anywhere)
-                const int at = r0 + step + 8 * g, from = eight_from(at, a.R) - r0;
-                float x[8];
+            for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = r0 + from + e < at || from + e < 0 ? 0.0f : t[16 * tt + i][max(from + e, 0)];
-                tp[tt] = cut8<3>(x);
-            }
-            for (int c0 = 0; c0 < count; c0 += U) {
-                int id[U];
-                Raw w[U][CT];
+                for (int c = 0; c < CT; c++) s.w[u][c] = load8_end<SHORT>(B[c] + s.id[u] * adapter, at, a.R);
+        };
+        int cut = -1;
+        Pieces<3> tp[TT];
+        auto use = [&](const Stage& s) {
+            if (s.step != cut) {
+                cut = s.step;
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    id[u] = __builtin_amdgcn_readfirstlane(list.id[min(c0 + u, count - 1)]);
+                for (int tt = 0; tt < TT; tt++) {
+                    // (t holds zeros behind the last rank, so that the operand may start anywhere)
+                    float x[8];
+                    const int at = r0 + s.step + 8 * g, from = eight_from(at, a.R) - r0;
+                    if (a.R % 8 == 0) {
+                        const float* here = &t[16 * tt + i][s.step + 8 * g];
+                        const float4 lo = *reinterpret_cast<const float4*>(here), hi = *reinterpret_cast<const float4*>(here + 4);
+                        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+                    } else {
 #pragma unroll
-                    for (int c = 0; c < CT; c++) w[u][c] = load8_end<SHORT>(B[c] + id[u] * adapter, r0 + step + 8 * g, a.R);
-                }
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (c0 + u >= count) break;
-#pragma unroll
-                    for (int c = 0; c < CT; c++) {
-                        const auto wp = Weight<W>::cut(w[u][c]);
-#pragma unroll
-                        for (int tt = 0; tt < TT; tt++) acc[c][tt] = keep(mine[tt] == id[u], times(wp, tp[tt], acc[c][tt]), acc[c][tt]);
+                        for (int e = 0; e < 8; e++) x[e] = r0 + from + e < at || from + e < 0 ? 0.0f : t[16 * tt + i][max(from + e, 0)];
                     }
+                    tp[tt] = cut8<3>(x);
                 }
             }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (u >= s.n) break;
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    const auto wp = Weight<W>::cut(s.w[u][c]);
+#pragma unroll
+                    for (int tt = 0; tt < TT; tt++) acc[c][tt] = keep(mine[tt] == s.id[u], times(wp, tp[tt], acc[c][tt]), acc[c][tt]);
+                }
+            }
+        };
+        ask(s0);
+        __syncthreads();
+        while (true) {
+            ask(s1);
+            use(s0);
+            if (s1.step >= padded) break;
+            ask(s0);
+            use(s1);
+            if (s0.step >= padded) break;
         }
     }
 #pragma unroll
     for (int tt = 0; tt < TT; tt++) {
-        if (row0 + 16 * tt + i >= a.rows) continue;
+        if (row0 + 16 * tt + i >= tile.end) continue;
         const float scale = mine[tt] >= 0 ? a.scales[mine[tt]] : 0.0f;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
@@ -408,8 +491,8 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
             float4 u = yv[c][tt];
             if (mine[tt] >= 0)
                 u = make_float4(fmaf(scale, acc[c][tt][0], u.x), fmaf(scale, acc[c][tt][1], u.y), fmaf(scale, acc[c][tt][2], u.z), fmaf(scale, acc[c][tt][3], u.w));
-            if (vec_out && col + 4 <= a.N) {
-                *reinterpret_cast<float4*>(out[tt] + col) = u;
+            if (vec_out) {
+                if (col < a.N) *reinterpret_cast<float4*>(out[tt] + col) = u;
             } else {
                 const float* from = reinterpret_cast<const float*>(&u);
 #pragma unroll
@@ -420,25 +503,30 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
     }
 }
 
-// Tokens to a workgroup: 32 where there are enough of them to fill the chip so
-static int lora_tiles(int64_t rows) { return rows > 256 ? 2 : 1; }
-// K in runs, until there are some 256 workgroups.  A run is at least 1024 (four steps to a wave, asked for at once) where a tile has one
-// adapter or two; the weights of several fill the wait of one step.
+// Tokens to a tile: 32 where there are enough of them to fill the chip so
+static int lora_tile(int64_t rows) { return rows > 256 ? 32 : 16; }
+static int64_t lora_tiles(int64_t batch, int64_t tokens) {
+    const int64_t tile = lora_tile(batch * tokens);
+    return tokens >= tile ? batch * ((tokens + tile - 1) / tile) : (batch * tokens + tile - 1) / tile;
+}
+// K in runs, until there are some 256 workgroups.  A run is at least 1024 (two stages of two steps to a wave) where tiles have one
+// adapter; the weights of several fill the wait of one step.
 static int lora_chunk(int64_t batch, int64_t tokens, int64_t K, int64_t R, int64_t adapters) {
-    const int64_t rows = batch * tokens, tile = 16 * lora_tiles(rows), groups = (rows + tile - 1) / tile * ((R + 63) / 64);
-    const int64_t sequences = (tile + tokens - 1) / tokens + 1, several = sequences < batch ? sequences : batch;
-    const int64_t least = (several < adapters ? several : adapters) > 2 ? 256 : 1024;
-    const int64_t n = (256 + groups - 1) / groups;
+    const int64_t tile = lora_tile(batch * tokens), groups = lora_tiles(batch, tokens) * ((R + 63) / 64);
+    const int64_t least = tokens >= tile || batch == 1 || adapters == 1 ? 1024 : 256, n = (256 + groups - 1) / groups;
     return (int)((K + least * n - 1) / (least * n) * least);
 }
 
 template <typename W>
 static int lora_launch(LoraArgs a, bool vec_out, hipStream_t st) {
-    const int tt = lora_tiles(a.rows), nr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
-    const unsigned tiles = (unsigned)((a.rows + 16 * tt - 1) / (16 * tt));
+    const int tile = lora_tile(a.rows), tt = tile / 16, nr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
+    const unsigned tiles = (unsigned)lora_tiles(a.rows / a.tokens, a.tokens);
+    a.tiles = a.tokens >= tile ? (a.tokens + tile - 1) / tile : 0;
     const dim3 down(tiles, (unsigned)a.splits, (unsigned)((a.R + 16 * nr - 1) / (16 * nr)));
 #define LLMOPS_DOWN(NR, TT) lora_down_kernel<W, NR, TT, false><<<down, 64 * kDownWaves, 0, st>>>(a)
-    if (a.K < 8) lora_down_kernel<W, 4, 1, true><<<dim3((unsigned)((a.rows + 15) / 16), 1, (unsigned)((a.R + 63) / 64)), 64 * kDownWaves, 0, st>>>(a);
+    const dim3 narrow(tiles, 1, (unsigned)((a.R + 15) / 16));
+    if (a.K < 8 && tt == 1) lora_down_kernel<W, 1, 1, true><<<narrow, 64 * kDownWaves, 0, st>>>(a);
+    else if (a.K < 8) lora_down_kernel<W, 1, 2, true><<<narrow, 64 * kDownWaves, 0, st>>>(a);
     else if (tt == 1 && nr == 1) LLMOPS_DOWN(1, 1);
     else if (tt == 1 && nr == 2) LLMOPS_DOWN(2, 1);
     else if (tt == 1) LLMOPS_DOWN(4, 1);
@@ -465,7 +553,7 @@ using namespace llmops;
 static bool lora_sizes_fit(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R) {
     const int64_t most = (int64_t)1 << 30;
     return batch > 0 && tokens > 0 && N > 0 && K > 0 && R > 0 && batch < most && tokens < most && N < most && K < most && R <= 4096 &&
-           batch * tokens <= 65535 * 16;
+           batch * tokens <= ((int64_t)1 << 20) && lora_tiles(batch, tokens) <= 65535;
 }
 
 extern "C" size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R, int64_t adapters) {
@@ -494,7 +582,7 @@ extern "C" int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_str
     a.rows = (int)(batch * tokens), a.tokens = (int)tokens, a.K = (int)K, a.N = (int)N, a.R = (int)R, a.adapters = (int)adapters;
     a.chunk = lora_chunk(batch, tokens, K, R, adapters);
     a.splits = (int)((K + a.chunk - 1) / a.chunk);
-    const bool vec_out = aligned(y, 16) && aligned(out, 16) && y_stride_b % 4 == 0 && y_stride_l % 4 == 0 && out_stride_b % 4 == 0 && out_stride_l % 4 == 0;
+    const bool vec_out = N % 4 == 0 && aligned(y, 16) && aligned(out, 16) && y_stride_b % 4 == 0 && y_stride_l % 4 == 0 && out_stride_b % 4 == 0 && out_stride_l % 4 == 0;
     hipStream_t st = as_stream(stream);
     if (weight_dtype == LLMOPS_F32) return lora_launch<float>(a, vec_out, st);
     if (weight_dtype == LLMOPS_F16) return lora_launch<Half16>(a, vec_out, st);

@@ -22,6 +22,12 @@ namespace llmops {
 constexpr double kLog2e = 1.4426950408889634;
 constexpr int kRun = 4096;  // logits to a workgroup: 16 to a thread, in registers between maximum and sum
 
+// a draft and what it is judged by, beside its row's sums, so that the second launch finds it without following the draft
+struct Draft {
+    float z, q, u;  // its logit (-inf: not a token), its probability where it was drawn, its random number
+    int x;
+};
+
 struct VerifyArgs {
     const float *logits, *probs, *uniforms, *temperature;
     const int64_t* drafts;
@@ -32,6 +38,7 @@ struct VerifyArgs {
     int32_t* accepted;
     double *sum, *rest;  // [B*(K+1)][runs], [B][runs]
     int32_t* arrived;    // [B]
+    Draft* draft;        // [B*(K+1)]
     float* top;          // [B*(K+1)][runs]
     int32_t* place;      // [B*(K+1)][runs]
 };
@@ -122,6 +129,16 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
         x[e] = j < n ? z[j] : -INFINITY;
     }
     const float t = temperature_of(a, b);
+    if (run == 0 && threadIdx.x == 255 && i < a.K) {
+        const int64_t x = a.drafts[(int64_t)b * a.K + i];
+        const bool inside = x >= 0 && x < a.V;
+        Draft d;
+        d.z = inside ? a.logits[(int64_t)row * a.V + x] : -INFINITY;
+        d.q = inside && a.probs != nullptr ? a.probs[((int64_t)b * a.K + i) * a.V + x] : 1.0f;
+        d.u = a.uniforms[row];
+        d.x = inside ? (int)x : -1;
+        a.draft[row] = d;
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; e++) top = fmaxf(top, x[e]);
@@ -191,6 +208,8 @@ __device__ __forceinline__ double rest_weight(const Row& r, float z, double per_
 __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     __shared__ int first, arrivals, found, last;
     __shared__ Row shared_row;
+    __shared__ Draft shared_draft[4];
+    __shared__ int refused_token;
     __shared__ double red[4];
     __shared__ float neighbours[2][kRun + kRun / 16];  // (16 in a row and a gap: a thread's on banks of their own)
     const int b = blockIdx.x / (unsigned)a.runs, run = blockIdx.x - b * a.runs, n = drafts_of(a, b), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -207,18 +226,15 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
         const int i = i0 + wave;
         Row r{};
         if (i <= n) {
-            const int64_t x = i < n ? a.drafts[(int64_t)b * a.K + i] : -1;
-            const bool inside = x >= 0 && x < a.V;
-            const float z = inside ? a.logits[(int64_t)(row0 + i) * a.V + x] : -INFINITY;
-            const double q = inside && probs != nullptr ? (double)probs[(int64_t)i * a.V + x] : 1.0;
-            const double u = (double)a.uniforms[row0 + i];
+            const Draft d = a.draft[row0 + i];  // (behind the last draft: whatever is there, and not looked at)
             r = row_of(a, row0 + i, draws, per_t, lane);
-            const bool fits = inside && (draws ? u * q * r.sum < weight(z, r.top, per_t) : x == r.place);
+            const bool fits = d.x >= 0 && (draws ? (double)d.u * (double)d.q * r.sum < weight(d.z, r.top, per_t) : d.x == r.place);
+            if (lane == 0) shared_draft[wave] = d;
             if (lane == 0 && i < n && !fits) atomicMin(&first, i);
         }
         __syncthreads();
         const int done = first;
-        if (done == i && lane == 0) shared_row = r;
+        if (done == i && lane == 0) shared_row = r, refused_token = shared_draft[wave].x;
         __syncthreads();
         if (done < i0 + 4) break;
     }
@@ -227,7 +243,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     const bool refused = done < n;
     const float *zrow = a.logits + (int64_t)row * a.V, *qrow = refused && probs != nullptr ? probs + (int64_t)done * a.V : nullptr;
     bool less = qrow != nullptr;
-    int64_t x = refused && qrow == nullptr ? a.drafts[(int64_t)b * a.K + done] : -1;
+    int x = refused && qrow == nullptr ? refused_token : -1;
     int64_t* tokens = a.tokens + row0;
     if (run == 0) {
         if (threadIdx.x == 0) a.accepted[b] = done;
@@ -238,6 +254,10 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
         if (run == 0 && threadIdx.x == 0) tokens[done] = r.place;
         return;
     }
+    // Where a draft with a distribution was refused, every run has a sum to form; else the sums are those of the first launch, but for the
+    // run of a refused draft without one
+    const bool spread = less;
+    if (!spread && run > 0) return;
     double* rest = a.rest + (int64_t)b * a.runs;
     // j of a thread's value e; what lies behind the row weighs nothing
     auto z_at = [&](int at_run, int e) {
@@ -248,34 +268,42 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
         const int j = at_run * kRun + threadIdx.x + 256 * e;
         return qrow != nullptr && j < a.V ? qrow[j] : 0.0f;
     };
-    float z[16], q[16];
-#pragma unroll
-    for (int e = 0; e < 16; e++) z[e] = z_at(run, e), q[e] = q_at(run, e);
+    const int sum_run = spread ? run : x >= 0 ? x / kRun : -1;
     double sum = 0.0;
+    if (sum_run >= 0) {
+        float z[16], q[16];
 #pragma unroll
-    for (int e = 0; e < 16; e++) sum += rest_weight(r, z[e], per_t, less, q[e], run * kRun + (int)threadIdx.x + 256 * e == x);
-    sum = wave_sum64(sum);
-    if (lane == 0) red[wave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        // the exchange has come back before the arrival is counted: whoever counts the last one finds every sum.  (Nothing else is handed
-        // over; a release and an acquire of the device's scope would write back and empty the L2 in every workgroup.)
-        double before = __hip_atomic_exchange(&rest[run], (red[0] + red[1]) + (red[2] + red[3]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("" : "+v"(before) : : "memory");
-        arrivals = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        found = (int)kNowhere, last = -1;
+        for (int e = 0; e < 16; e++) z[e] = z_at(sum_run, e), q[e] = q_at(sum_run, e);
+#pragma unroll
+        for (int e = 0; e < 16; e++) sum += rest_weight(r, z[e], per_t, less, q[e], sum_run * kRun + (int)threadIdx.x + 256 * e == x);
+        sum = wave_sum64(sum);
+        if (lane == 0) red[wave] = sum;
+        __syncthreads();
+        sum = (red[0] + red[1]) + (red[2] + red[3]);
     }
-    __syncthreads();
-    if (arrivals != a.runs - 1) return;
+    if (threadIdx.x == 0) found = (int)kNowhere, last = -1;
+    if (spread) {
+        if (threadIdx.x == 0) {
+            // the exchange has come back before the arrival is counted: whoever counts the last one finds every sum.  (Nothing else is
+            // handed over; a release and an acquire of the device's scope would write back and empty the L2 in every workgroup.)
+            double before = __hip_atomic_exchange(&rest[run], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("" : "+v"(before) : : "memory");
+            arrivals = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (arrivals != a.runs - 1) return;
+    }
 
-    // the last one: every wave finds the run, a run to a lane
+    // the last one (or the only one): every wave finds the run, a run to a lane
+    const double sum_left = sum;
     const int64_t at = (int64_t)row * a.runs;
     auto run_sum = [&](int c, bool own) {
         if (c >= a.runs) return 0.0;
+        if (own && x >= 0 && c == sum_run) return sum_left;
         return own ? a.sum[at + c] * share(a.top[at + c], r.top, per_t) * r.inv : __hip_atomic_load(&rest[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
     double total = 0.0;
-    for (int c0 = 0; c0 < a.runs; c0 += 64) total += wave_sum64(run_sum(c0 + lane, false));
+    for (int c0 = 0; c0 < a.runs; c0 += 64) total += wave_sum64(run_sum(c0 + lane, !spread));
     const bool none = !(total > 0.0);  // nothing above the draft's distribution: the target's own
     if (none) {
         less = false, x = -1, total = 0.0;
@@ -285,7 +313,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     double before = 0.0, heavy_before = 0.0;  // sums of the runs before the one, and before the last with a weight
     int at_run = -1, heavy = 0;
     for (int c0 = 0; c0 < a.runs && at_run < 0; c0 += 64) {
-        const double mine = run_sum(c0 + lane, none);
+        const double mine = run_sum(c0 + lane, none || !spread);
         const double to = before + scan64(mine);  // up to and with this lane's run
         const uint64_t past = __ballot(to > goal && mine > 0.0), some = __ballot(mine > 0.0);
         if (some != 0) {
@@ -341,12 +369,13 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
 }
 
 struct VerifyLayout {
-    size_t sum, rest, top, place, arrived, total;
+    size_t draft, sum, rest, top, place, arrived, total;
 };
 static VerifyLayout layout_verify(int64_t B, int64_t K, int64_t runs) {
     VerifyLayout w{};
     const size_t rows = (size_t)(B * (K + 1) * runs);
-    w.sum = 0;
+    w.draft = 0;
+    w.sum = w.draft + (size_t)(B * (K + 1)) * sizeof(Draft);
     w.rest = w.sum + rows * 8;
     w.top = w.rest + (size_t)(B * runs) * 8;
     w.place = w.top + rows * 4;
@@ -381,12 +410,12 @@ extern "C" int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, i
     const VerifyLayout w = layout_verify(B, K, a.runs);
     if (workspace == nullptr || workspace_bytes < w.total)
         return fail(LLMOPS_EWORKSPACE, "verify_drafts needs %zu workspace bytes, got %zu", w.total, workspace == nullptr ? (size_t)0 : workspace_bytes);
-    LLMOPS_REQUIRE(aligned(workspace, 8));
+    LLMOPS_REQUIRE(aligned(workspace, 16));
     char* ws = reinterpret_cast<char*>(workspace);
     a.logits = logits, a.probs = draft_probs, a.uniforms = uniforms, a.temperature = temperature, a.drafts = drafts, a.draft_lens = draft_lens;
     a.one_temperature = one_temperature;
     a.B = (int)B, a.K = (int)K, a.V = (int)V, a.tokens = tokens, a.accepted = accepted;
-    a.sum = reinterpret_cast<double*>(ws + w.sum), a.rest = reinterpret_cast<double*>(ws + w.rest), a.top = reinterpret_cast<float*>(ws + w.top);
+    a.draft = reinterpret_cast<Draft*>(ws + w.draft), a.sum = reinterpret_cast<double*>(ws + w.sum), a.rest = reinterpret_cast<double*>(ws + w.rest), a.top = reinterpret_cast<float*>(ws + w.top);
     a.place = reinterpret_cast<int32_t*>(ws + w.place), a.arrived = reinterpret_cast<int32_t*>(ws + w.arrived);
     hipStream_t st = as_stream(stream);
     verify_rows_kernel<<<dim3((unsigned)(B * (K + 1)), (unsigned)a.runs), 256, 0, st>>>(a);

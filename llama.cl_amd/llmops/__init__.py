@@ -555,6 +555,9 @@ def attention_rope_prefix(q, k, v, inv_freq, prefix_cache, prefix_len, kv_cache,
     changed: add to it what is to be kept, and the next call overwrites the rest.
     q_lens (int32 [B], device): a sequence brings that many of the qL tokens; the rest, and tokens that no longer fit the cache, are
     padding: not cached, and 0 in the result.  Returns fp32 [B,qL,H*S]."""
+    out = (_lib._host or _lib.host()).attention_rope_prefix(q, k, v, inv_freq, prefix_cache, prefix_len, kv_cache, lengths, layer_id, q_lens)
+    if out is not NotImplemented:  # (the ordinary call, in native code)
+        return out
     (qp, qb, ql), (kp, kb, kl), (vp, vb, vl) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
     for t, n in ((kv_cache, "kv_cache"),) + (((prefix_cache, "prefix_cache"),) if prefix_cache is not None else ()):
         _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 5 and t.is_contiguous(), f"{n}.is<float>(5)")
@@ -600,6 +603,10 @@ def lora_add(y, x, lora_A, lora_B, adapters, scales, out=None):
     and lora_B [n,N,R] (fp32, fp16 or bf16) hold n adapters, those of a lower rank padded with zeros; adapters int32 [B] and scales fp32
     [n] on the device.  An adapter outside 0 .. n-1 (-1) is none: the sequence keeps its y.  Returns a new tensor, or ``out`` [B,M,N],
     which may be y itself and must not overlap x or y otherwise."""
+    if out is None:
+        done = (_lib._host or _lib.host()).lora_add(y, x, lora_A, lora_B, adapters, scales)
+        if done is not NotImplemented:  # (as above)
+            return done
     (yp, yb, yl), (xp, xb, xl) = _rows(y, "y"), _rows(x, "x")
     for t, n in ((lora_A, "lora_A"), (lora_B, "lora_B")):
         _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 3 and t.is_contiguous() and t.dtype in _LORA_TYPES, f"{n}.is_dense(3)")
@@ -634,6 +641,9 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature=None, 
     drafts.  K may be 0: the next token is drawn from the logits.
 
     Returns (tokens int64 [B,K+1]: the accepted drafts, the next token, -1 behind it; accepted int32 [B]: how many drafts)."""
+    done = (_lib._host or _lib.host()).verify_drafts(logits, drafts, uniforms, draft_probs, temperature, draft_lens)
+    if done is not NotImplemented:  # (as above)
+        return done
     _dev(logits, torch.float32, 3, "logits")
     _require(isinstance(drafts, torch.Tensor) and drafts.is_cuda and drafts.dtype in (torch.int64, torch.int32), "drafts.is<int64_t>(2)")
     _require(drafts.dim() == 2 and drafts.is_contiguous(), "drafts.is<int64_t>(2)")

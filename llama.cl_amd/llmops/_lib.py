@@ -121,7 +121,7 @@ class _PythonCalls:
     def fc_Q4A(*args):
         return NotImplemented
 
-    attention_rope2 = fc_Q4A
+    attention_rope2 = attention_rope_prefix = lora_add = verify_drafts = fc_Q4A
 
 
 def host():
@@ -143,7 +143,8 @@ def host():
             return _host
         native.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "llmops_fc_Q4A_workspace_bytes", "llmops_fc_Q4A", "llmops_attention_workspace_bytes", "llmops_attention_rope",
-            "llmops_last_error")))
+            "llmops_last_error", "llmops_attention_prefix_workspace_bytes", "llmops_attention_rope_prefix", "llmops_lora_workspace_bytes",
+            "llmops_lora_add", "llmops_verify_drafts_workspace_bytes", "llmops_verify_drafts")))
         _host = native
     return _host
 

@@ -7,8 +7,9 @@
 //   out = sum_r e_r V_r / sum_r e_r,  e_r = exp(q' . K_r / sqrt(S) - max),  r over the P prefix rows and own rows 0 .. len[b] + l.
 //
 //   1. prefix_prep_kernel   rotates, writes the new cache rows and leaves q' as operands of the matrix instructions
-//   2. prefix_attn_kernel   softmax(q'K^T)V of a piece of the rows for a tile of queries: running maximum and sum, one pass
-//   3. prefix_merge_kernel  joins the pieces of a query
+//   2. prefix_apart_kernel  softmax(q'K^T)V of a piece of the rows for a tile of queries: running maximum and sum, one pass; the prefix
+//      prefix_sweep_kernel  and the own rows apart, or in one sweep where a sequence has queries to fill tiles of its own
+//   3. prefix_merge_kernel  joins the pieces of a query, where there are several
 //
 // Queries of a kv head are numbered m = (b*qL + l)*G + g, so that the queries that see the prefix, those of all sequences, and
 // those of one sequence are both runs of m.  Rows are numbered through: r < P is the prefix's, P + i is the sequence's own row i.
@@ -326,25 +327,43 @@ __device__ __forceinline__ v4f add_rows(v4f o, const Halves& v, const Weights& w
     return o;
 }
 
+// Four dims from d on of what piece `piece` has for query m: a record, or the answer where there is one piece (live: the query is no padding)
+__device__ __forceinline__ void leave(const PrefixArgs& a, int hk, int m, int piece, int d, float4 o, float sum, bool live) {
+    if (a.nrec > 1) {
+        *reinterpret_cast<float4*>(a.rec_out + (((int64_t)hk * a.M + m) * a.nrec + piece) * kS + d) = o;
+        return;
+    }
+    const float f = live ? 1.0f / sum : 0.0f;
+    const int bl = m / a.G;
+    *reinterpret_cast<float4*>(a.out + ((int64_t)bl * a.G * a.Hkv + (int64_t)hk * a.G + (m - bl * a.G)) * kS + d) =
+        live ? make_float4(o.x * f, o.y * f, o.z * f, o.w * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ void leave_stat(const PrefixArgs& a, int hk, int m, int piece, float top, float sum) {
+    if (a.nrec > 1) a.rec_stat[((int64_t)hk * a.M + m) * a.nrec + piece] = make_float2(top, sum);
+}
+
 // the row below which query m of sequence b sees its own rows
 __device__ __forceinline__ int rows_seen(const PrefixArgs& a, int m, int b, int len, int n) {
     const int l = (m - b * a.Mq) / a.G;
     return l < n ? len + l + 1 : 0;
 }
 
-// The same in full width, for rows that hold values outside the halves' range: the workgroup starts again, a wave to a query and
-// two dims to a lane, only the rows that the query sees, in up to two runs (prefix, own).  Slow, and not met in a model's caches.
+// The same in full width, for rows that hold values outside the halves' range: the workgroup starts again, half a wave to a query and
+// four dims to a lane, only the rows that the query sees, in up to two runs (prefix, own).  Slow, and not met in a model's caches.
 template <typename T>
 __device__ __forceinline__ void full_width(const PrefixArgs& a, int hk, int m0, int m_end, Rows<T> K0, Rows<T> V0, int from0, Rows<T> K1, Rows<T> V1, int from1,
                                            bool own, int b, int len, int n, int piece) {
-    const int lane = threadIdx.x & 63, d = 2 * lane;
+    const int d = 4 * (threadIdx.x & 31);
 #pragma unroll 1
-    for (int m = m0 + (threadIdx.x >> 6); m < m_end; m += 4) {
+    for (int m = m0 + (threadIdx.x >> 5); m < m_end; m += 8) {
         const int64_t at = ((int64_t)hk * a.M + m) * kS + d;
-        const double q0 = (double)(float)a.qh[at] + (double)(float)a.ql[at], q1 = (double)(float)a.qh[at + 1] + (double)(float)a.ql[at + 1];
+        double q[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[e] = (double)(float)a.qh[at + e] + (double)(float)a.ql[at + e];
         const double c = (double)a.cq[(int64_t)hk * a.M + m];
         const int see = own ? rows_seen(a, m, b, len, n) : 0;
-        float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+        float top = -INFINITY, sum = 0.0f;
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int run = 0; run < 2; run++) {
             const T* k = run ? K1.p : K0.p;
@@ -352,21 +371,29 @@ __device__ __forceinline__ void full_width(const PrefixArgs& a, int hk, int m0, 
             const int end = run ? min(K1.end, see) : see > 0 || !own ? K0.end : 0;
 #pragma unroll 1
             for (int r = run ? from1 : from0; r < end; r++) {
-                double x = q0 * (double)value(k + (int64_t)r * kS + d) + q1 * (double)value(k + (int64_t)r * kS + d + 1);
+                double x = 0.0;
 #pragma unroll
-                for (int w = 32; w > 0; w >>= 1) x += __shfl_xor(x, w, 64);
+                for (int e = 0; e < 4; e++) x += q[e] * (double)value(k + (int64_t)r * kS + d + e);
+#pragma unroll
+                for (int w = 16; w > 0; w >>= 1) x += __shfl_xor(x, w, 64);
                 const float s = (float)(x * c), up = fmaxf(top, s), shrink = top == up ? 1.0f : __builtin_amdgcn_exp2f(top - up);
-                const float e = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - up + kLift);
+                const float w = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - up + kLift);
                 top = up;
-                sum = fmaf(sum, shrink, e);
-                o0 = fmaf(e, value(v + (int64_t)r * kS + d), o0 * shrink);
-                o1 = fmaf(e, value(v + (int64_t)r * kS + d + 1), o1 * shrink);
+                sum = fmaf(sum, shrink, w);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = fmaf(w, value(v + (int64_t)r * kS + d + e), o[e] * shrink);
             }
         }
-        const int64_t rec = ((int64_t)hk * a.M + m) * a.nrec + piece;
-        if (lane == 0) a.rec_stat[rec] = make_float2(top, sum);
-        *reinterpret_cast<float2*>(a.rec_out + rec * kS + d) = make_float2(o0, o1);
+        if (d == 0) leave_stat(a, hk, m, piece, top, sum);
+        leave(a, hk, m, piece, d, make_float4(o[0], o[1], o[2], o[3]), sum, see > 0);
     }
+}
+
+// a piece without rows
+__device__ __forceinline__ void nothing(const PrefixArgs& a, int hk, int m0, int m_end, int piece) {
+    for (int m = m0 + threadIdx.x; m < m_end; m += 256) leave_stat(a, hk, m, piece, -INFINITY, 0.0f);
+    if (a.nrec == 1)  // (then the queries are padding)
+        for (int e = threadIdx.x; e < (m_end - m0) * 32; e += 256) leave(a, hk, m0 + (e >> 5), piece, 4 * (e & 31), make_float4(0.f, 0.f, 0.f, 0.f), 1.0f, false);
 }
 
 // a wave's say, and the workgroup's decision
@@ -383,16 +410,16 @@ __device__ __forceinline__ bool all_zero(Rows<T> x, int from) {
     return !__syncthreads_or(some);
 }
 template <typename T>
-__device__ __forceinline__ bool needs_full_width(const int (&range)[4][2], Rows<T> K, Rows<T> V, int from) {
+__device__ __forceinline__ bool needs_full_width(const int (&range)[4][2], Rows<T> K, Rows<T> V, int from, Rows<T> K1, Rows<T> V1, int from1) {
     const int k = max(max(range[0][0], range[1][0]), max(range[2][0], range[3][0])), v = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
-    return k == 2 || v == 2 || (k == 0 && !all_zero(K, from)) || (v == 0 && !all_zero(V, from));
+    return k == 2 || v == 2 || (k == 0 && !(all_zero(K, from) && all_zero(K1, from1))) || (v == 0 && !(all_zero(V, from) && all_zero(V1, from1)));
 }
 
 // Few queries to a workgroup (16 * RT): bound by reading the rows.  The four waves take 32 rows each of every 128; operands come
 // straight from memory, K of the next rows asked for when K of these is used up, and so V; the waves' sums meet in LDS.
 constexpr int kMeetRow = 132;  // floats (16 queries' rows on different banks)
 struct MeetSmem {
-    float m[4][32], l[4][32];
+    float m[4][32], l[4][32], sum[16];
     int range[4][2];
     union {
         float o[4][16][kMeetRow];
@@ -495,9 +522,8 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, Rows<T> K, Rows
                                             int n, int piece, MeetSmem& sm) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const int r1 = K.end;
-    if (r0 >= r1) {  // nothing here: say so
-        if ((int)threadIdx.x < 16 * RT && m0 + (int)threadIdx.x < m_end)
-            a.rec_stat[((int64_t)hk * a.M + m0 + threadIdx.x) * a.nrec + piece] = make_float2(-INFINITY, 0.0f);
+    if (r0 >= r1) {
+        nothing(a, hk, m0, min(m_end, m0 + 16 * RT), piece);
         return;
     }
     RowRegs<T> x;
@@ -563,8 +589,8 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, Rows<T> K, Rows
     }
     note_range<T>(ktop, vtop, sm.range[wave], lane);
     __syncthreads();
-    if (needs_full_width(sm.range, K, V, r0)) {
-        const Rows<T> none{K.p, 0};
+    const Rows<T> none{K.p, 0};
+    if (needs_full_width(sm.range, K, V, r0, none, none, 0)) {
         full_width<T>(a, hk, m0, min(m_end, m0 + 16 * RT), own ? none : K, own ? none : V, r0, own ? K : none, own ? V : none, r0, own, b, len, n, piece);
         return;
     }
@@ -580,14 +606,15 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, Rows<T> K, Rows
             for (int v = 0; v < 4; v++)
                 *reinterpret_cast<float4*>(&sm.o[wave][i][64 * h + 16 * g + 4 * v]) =
                     make_float4(s.o[rt][4 * h][v] * f, s.o[rt][4 * h + 1][v] * f, s.o[rt][4 * h + 2][v] * f, s.o[rt][4 * h + 3][v] * f);
-        if (wave == 0 && g == 0 && m0 + 16 * rt + i < m_end) {
+        if (wave == 0 && g == 0) {
             float L = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 const float mw = sm.m[w][16 * rt + i];
                 L += sm.l[w][16 * rt + i] * (mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
             }
-            a.rec_stat[((int64_t)hk * a.M + m0 + 16 * rt + i) * a.nrec + piece] = make_float2(M, L);
+            sm.sum[i] = s.see[rt] > 0 ? L : -1.0f;
+            if (m0 + 16 * rt + i < m_end) leave_stat(a, hk, m0 + 16 * rt + i, piece, M, L);
         }
         __syncthreads();
 #pragma unroll
@@ -600,43 +627,262 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, Rows<T> K, Rows
                     const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][q][d]);
                     r.x += y.x, r.y += y.y, r.z += y.z, r.w += y.w;
                 }
-                *reinterpret_cast<float4*>(a.rec_out + (((int64_t)hk * a.M + m0 + 16 * rt + q) * a.nrec + piece) * kS + d) = r;
+                leave(a, hk, m0 + 16 * rt + q, piece, d, r, sm.sum[q], sm.sum[q] != -1.0f);
             }
         }
         __syncthreads();
     }
 }
 
-template <typename T, int RTP, int RTO>
-__global__ __launch_bounds__(256, 2) void prefix_attn_kernel(PrefixArgs a) {
-    __shared__ MeetSmem sm;
-    if (blockIdx.x < a.pitems) {
-        unsigned item = blockIdx.x;
-        const int tile = item % a.ptiles;
-        item /= a.ptiles;
-        const int piece = item % a.ppieces, hk = item / a.ppieces;
-        const int64_t plane = (int64_t)hk * a.pmax * kS;
-        const int end = min(a.P, (piece + 1) * a.prows);
-        const Rows<T> K{(const T*)a.pk + plane, end}, V{(const T*)a.pv + plane, end};
-        few_queries<T, RTP>(a, K, V, hk, tile * 16 * RTP, a.M, piece * a.prows, false, 0, 0, 0, piece, sm);
+// Many queries (64 * RT to a workgroup, 16 * RT to a wave): bound by the matrix cores and, beside them, the vector ALU that cuts rows up
+// and weighs scores.  All waves multiply the same 32 rows, which the workgroup cuts up once and leaves in LDS in the order of the
+// operands (a read is 16 bytes to a lane, in lane order); two buffers: while a tile is multiplied the next is cut up and the one behind
+// it is on its way from memory.  Tiles 0 .. np-1 are the prefix's, those from np on the sequence's own.
+template <typename T>
+struct TileSmem {
+    static constexpr int kPieces = sizeof(T) == 4 ? 2 : 1;
+    uint4 k[2][kPieces][8][64], v[2][kPieces][8][64];
+    int range[4][2];
+};
+template <typename T>
+struct TileRegs;
+template <>
+struct TileRegs<float> {
+    float4 k[2][2], v[4];
+    // K: rows 16*tt + i, dims 32*step + 8*g .. of the wave's two (tt, step).  V: rows 16*(wave/2) + 4*g + 0..3, dims 64*(wave%2) + 4*i ..
+    __device__ __forceinline__ void load(buffer_rsrc K, buffer_rsrc V, int wave, int i, int g) {
+        const uint32_t k_at = unseen((uint32_t)((16 * (wave >> 1) + i) * kS + 64 * (wave & 1) + 8 * g) * 4),
+                       v_at = unseen((uint32_t)((16 * (wave >> 1) + 4 * g) * kS + 64 * (wave & 1) + 4 * i) * 4);
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) k[c][h] = __builtin_bit_cast(float4, ask16(K, k_at, (32 * c + 4 * h) * 4));
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = __builtin_bit_cast(float4, ask16(V, v_at, r * kS * 4));
+    }
+    __device__ __forceinline__ void write(TileSmem<float>& sm, int buf, int wave, int lane, v2us& ktop, v2us& vtop) const {
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const float4 x = k[c][0], y = k[c][1];
+            uint4 h, l;
+            h.x = cut2(x.x, x.y, l.x), h.y = cut2(x.z, x.w, l.y), h.z = cut2(y.x, y.y, l.z), h.w = cut2(y.z, y.w, l.w);
+            note4(ktop, h);
+            sm.k[buf][0][2 * wave + c][lane] = h;
+            sm.k[buf][1][2 * wave + c][lane] = l;
+        }
+        const int tt = wave >> 1;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            auto f = [&](int r) { return reinterpret_cast<const float*>(&v[r])[c]; };
+            uint2 h, l;
+            h.x = cut2(f(0), f(1), l.x), h.y = cut2(f(2), f(3), l.y);
+            note4(vtop, make_uint4(h.x, h.y, 0u, 0u));
+            reinterpret_cast<uint2*>(&sm.v[buf][0][4 * (wave & 1) + c][lane])[tt] = h;
+            reinterpret_cast<uint2*>(&sm.v[buf][1][4 * (wave & 1) + c][lane])[tt] = l;
+        }
+    }
+};
+template <>
+struct TileRegs<__half> {
+    uint4 k[2];
+    uint2 v[4];
+    __device__ __forceinline__ void load(buffer_rsrc K, buffer_rsrc V, int wave, int i, int g) {
+        const uint32_t k_at = unseen((uint32_t)((16 * (wave >> 1) + i) * kS + 64 * (wave & 1) + 8 * g) * 2),
+                       v_at = unseen((uint32_t)((16 * (wave >> 1) + 4 * g) * kS + 64 * (wave & 1) + 4 * i) * 2);
+#pragma unroll
+        for (int c = 0; c < 2; c++) k[c] = ask16(K, k_at, 32 * c * 2);
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = ask8(V, v_at, r * kS * 2);
+    }
+    __device__ __forceinline__ void write(TileSmem<__half>& sm, int buf, int wave, int lane, v2us& ktop, v2us& vtop) const {
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            note4(ktop, k[c]);
+            sm.k[buf][0][2 * wave + c][lane] = k[c];
+        }
+        const int tt = wave >> 1;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            auto f = [&](int r) { return (c & 2) ? v[r].y : v[r].x; };
+            const uint32_t pick = (c & 1) ? 0x07060302u : 0x05040100u;
+            const uint2 h = make_uint2(__builtin_amdgcn_perm(f(1), f(0), pick), __builtin_amdgcn_perm(f(3), f(2), pick));
+            note4(vtop, make_uint4(h.x, h.y, 0u, 0u));
+            reinterpret_cast<uint2*>(&sm.v[buf][0][4 * (wave & 1) + c][lane])[tt] = h;
+        }
+    }
+};
+
+template <typename T, int RT>
+__device__ __forceinline__ void many_queries(const PrefixArgs& a, int hk, int m0, int m_end, Rows<T> K0, Rows<T> V0, Rows<T> K1, Rows<T> V1, int np, int j0,
+                                             int j1, bool own, int b, int len, int n, int piece, TileSmem<T>& sm) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    m_end = min(m_end, m0 + 64 * RT);
+    if (j0 >= j1) {
+        nothing(a, hk, m0, m_end, piece);
+        return;
+    }
+    TileRegs<T> x;
+    auto load = [&](int j) {
+        const bool mine = j >= np;
+        const int t = 32 * (mine ? j - np : j);
+        x.load((mine ? K1 : K0).from(t), (mine ? V1 : V0).from(t), wave, i, g);
+    };
+    load(j0);
+    v8h qh[RT][4], ql[RT][4];
+    Queries<RT> s;
+    const int mw = m0 + 16 * RT * wave;
+    s.start(a, hk, mw, m_end, i);
+    int see[RT], see_min = INT_MAX;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int m = min(mw + 16 * rt + i, m_end - 1);
+        const int64_t at = ((int64_t)hk * a.M + m) * kS + 8 * g;
+#pragma unroll
+        for (int step = 0; step < 4; step++) {
+            qh[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + at + 32 * step));
+            ql[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + at + 32 * step));
+        }
+        see[rt] = own ? min(K1.end, rows_seen(a, m, b, len, n)) : 0;
+        see_min = min(see_min, see[rt]);
+    }
+    v2us ktop = {0, 0}, vtop = {0, 0};
+    x.write(sm, 0, wave, lane, ktop, vtop);
+    load(min(j0 + 1, j1 - 1));
+    __syncthreads();
+#pragma unroll 1
+    for (int j = j0; j < j1; j++) {
+        const int buf = (j - j0) & 1;
+        x.write(sm, buf ^ 1, wave, lane, ktop, vtop);  // (behind the last tile that one again: nobody reads it)
+        load(min(j + 2, j1 - 1));
+        const bool mine = j >= np;
+        const int t = 32 * (mine ? j - np : j);
+        const bool masked = __any(t + 32 > (mine ? see_min : K0.end));
+        v4f sc[RT][2], low[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            sc[rt][0] = sc[rt][1] = low[rt][0] = low[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+            s.see[rt] = mine ? see[rt] : K0.end;
+        }
+#pragma unroll
+        for (int step = 0; step < 4; step++)
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++) {
+                Halves h{as_v8h(sm.k[buf][0][4 * tt + step][lane]), v8h{}};
+                if constexpr (sizeof(T) == 4) h.lo = as_v8h(sm.k[buf][TileSmem<T>::kPieces - 1][4 * tt + step][lane]);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) score_step<T>(sc[rt][tt], low[rt][tt], h, qh[rt][step], ql[rt][step]);
+            }
+        Weights w[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            if constexpr (sizeof(T) == 4)
+#pragma unroll
+                for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) sc[rt][tt][v] = fmaf(low[rt][tt][v], 1.0f / 2048.0f, sc[rt][tt][v]);
+            weigh(s, rt, sc[rt], t, g, masked);
+            w[rt] = weights_of<T>(sc[rt]);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            Halves h{as_v8h(sm.v[buf][0][c][lane]), v8h{}};
+            if constexpr (sizeof(T) == 4) h.lo = as_v8h(sm.v[buf][TileSmem<T>::kPieces - 1][c][lane]);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) s.o[rt][c] = add_rows<T>(s.o[rt][c], h, w[rt]);
+        }
+        __syncthreads();
+    }
+    note_range<T>(ktop, vtop, sm.range[wave], lane);
+    __syncthreads();
+    const Rows<T> k0{K0.p, min(K0.end, 32 * min(j1, np))}, v0{V0.p, k0.end}, k1{K1.p, min(K1.end, 32 * (j1 - np))}, v1{V1.p, k1.end};
+    const int from0 = 32 * j0, from1 = 32 * max(0, j0 - np);
+    if (needs_full_width(sm.range, k0, v0, from0, k1, v1, from1)) {
+        full_width<T>(a, hk, m0, m_end, k0, v0, from0, k1, v1, from1, own, b, len, n, piece);
+        return;
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        s.l[rt] += __shfl_xor(s.l[rt], 16, 64);
+        s.l[rt] += __shfl_xor(s.l[rt], 32, 64);
+        const int m = mw + 16 * rt + i;
+        if (m >= m_end) continue;
+        if (g == 0) leave_stat(a, hk, m, piece, s.m[rt], s.l[rt]);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+                leave(a, hk, m, piece, 64 * h + 16 * g + 4 * v, make_float4(s.o[rt][4 * h][v], s.o[rt][4 * h + 1][v], s.o[rt][4 * h + 2][v], s.o[rt][4 * h + 3][v]),
+                      s.l[rt], see[rt] > 0);
+    }
+}
+
+// Item `at` of groups * each: the items of a group, which read the same rows, follow each other on one XCD (consecutive workgroups go to
+// the eight in turn), so that its L2 serves all but the first
+__device__ __forceinline__ void item_of(unsigned at, unsigned groups, unsigned each, int& group, int& sub) {
+    const unsigned whole = groups & ~7u;
+    if (at < whole * each) {
+        const unsigned eight = at / (8 * each), in = at - eight * 8 * each;
+        group = (int)(eight * 8 + (in & 7)), sub = (int)(in >> 3);
     } else {
-        unsigned item = blockIdx.x - a.pitems;
-        const int tile = item % a.otiles;
-        item /= a.otiles;
-        const int piece = item % a.opieces;
-        item /= a.opieces;
-        const int hk = item % a.Hkv, b = item / a.Hkv;
+        const unsigned in = at - whole * each;
+        group = (int)(whole + in / each), sub = (int)(in % each);
+    }
+}
+
+// The prefix for the queries of all sequences, RTP times 16 of them (MANY: 64) to a workgroup, then every sequence's own rows for its
+// queries, RTO times 16
+template <typename T, int RTP, bool MANY, int RTO>
+__global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a) {
+    __shared__ union {
+        MeetSmem few;
+        TileSmem<T> many;
+    } sm;
+    if (blockIdx.x < a.pitems) {
+        int group, tile;  // (a group: a head's piece of the prefix)
+        item_of(blockIdx.x, a.Hkv * a.ppieces, a.ptiles, group, tile);
+        const int piece = group % a.ppieces, hk = group / a.ppieces;
+        const int64_t plane = (int64_t)hk * a.pmax * kS;
+        if constexpr (MANY) {
+            const Rows<T> K{(const T*)a.pk + plane, a.P}, V{(const T*)a.pv + plane, a.P}, none{(const T*)a.pk, 0};
+            const int tiles = (a.P + 31) / 32;
+            many_queries<T, RTP>(a, hk, tile * 64 * RTP, a.M, K, V, none, none, tiles, piece * (a.prows / 32), min(tiles, (piece + 1) * (a.prows / 32)), false, 0,
+                                 0, 0, piece, sm.many);
+        } else {
+            const int end = min(a.P, (piece + 1) * a.prows);
+            const Rows<T> K{(const T*)a.pk + plane, end}, V{(const T*)a.pv + plane, end};
+            few_queries<T, RTP>(a, K, V, hk, tile * 16 * RTP, a.M, piece * a.prows, false, 0, 0, 0, piece, sm.few);
+        }
+    } else {
+        int group, sub;  // (a group: a sequence's head)
+        item_of(blockIdx.x - a.pitems, a.B * a.Hkv, a.otiles * a.opieces, group, sub);
+        const int hk = group % a.Hkv, b = group / a.Hkv, tile = sub % a.otiles, piece = sub / a.otiles;
         int len, n;
         own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-        const int m0 = b * a.Mq + tile * 16 * RTO, m_end = (b + 1) * a.Mq;
+        const int first = tile * 16 * RTO, m0 = b * a.Mq + first, m_end = (b + 1) * a.Mq;
         // rows that the tile's last live query sees, in pieces of whole 128
-        const int last = min(n, (tile * 16 * RTO + 16 * RTO - 1) / a.G + 1), rows = last > 0 && tile * 16 * RTO < n * a.G ? len + last : 0;
+        const int last = min(n, (first + 16 * RTO - 1) / a.G + 1), rows = first < n * a.G ? len + last : 0;
         const int step = max(128, (rows + 128 * a.opieces - 1) / (128 * a.opieces) * 128);
         const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kS;
         const int end = min(rows, (piece + 1) * step);
         const Rows<T> K{(const T*)a.ok + plane, end}, V{(const T*)a.ov + plane, end};
-        few_queries<T, RTO>(a, K, V, hk, m0, m_end, piece * step, true, b, len, n, a.ppieces + piece, sm);
+        few_queries<T, RTO>(a, K, V, hk, m0, m_end, piece * step, true, b, len, n, a.ppieces + piece, sm.few);
     }
+}
+
+// The prefix and the sequence's own rows in one sweep, or in pieces of it, for 64 * RT of a sequence's queries to a workgroup
+template <typename T, int RT>
+__global__ __launch_bounds__(256, 2) void prefix_sweep_kernel(PrefixArgs a) {
+    __shared__ TileSmem<T> sm;
+    int group, sub;
+    item_of(blockIdx.x, a.B * a.Hkv, a.otiles * a.opieces, group, sub);
+    const int hk = group % a.Hkv, b = group / a.Hkv, tile = a.otiles - 1 - sub / a.opieces, piece = sub % a.opieces;
+    int len, n;
+    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    const int first = tile * 64 * RT, last = min(n, (first + 64 * RT - 1) / a.G + 1), rows = first < n * a.G ? len + last : 0;
+    const int np = (a.P + 31) / 32, tiles = rows > 0 ? np + (rows + 31) / 32 : 0, step = (tiles + a.opieces - 1) / a.opieces;
+    const int64_t pplane = (int64_t)hk * a.pmax * kS, oplane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kS;
+    const Rows<T> K0{(const T*)a.pk + pplane, a.P}, V0{(const T*)a.pv + pplane, a.P}, K1{(const T*)a.ok + oplane, rows}, V1{(const T*)a.ov + oplane, rows};
+    many_queries<T, RT>(a, hk, b * a.Mq + first, (b + 1) * a.Mq, K0, V0, K1, V1, np, piece * step, min(tiles, (piece + 1) * step), true, b, len, n, piece, sm);
 }
 
 // ---- 3. the pieces of a query ----
@@ -653,46 +899,74 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
         *reinterpret_cast<float4*>(out) = make_float4(0.f, 0.f, 0.f, 0.f);
         return;
     }
+    // eight records at a time, asked for together; a piece that the query sees nothing of has sum 0 and may have written nothing else
     const float2* stat = a.rec_stat + r * a.nrec;
     const float* rec = a.rec_out + r * a.nrec * kS + d;
-    float M = -INFINITY;
-    for (int c = 0; c < a.nrec; c++) M = fmaxf(M, stat[c].x);
-    float L = 0.0f;
+    float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < a.nrec; c++) {
-        const float2 st = stat[c];
-        if (st.y == 0.0f) continue;  // (a piece that the query sees nothing of; its record may not have been written)
-        const float w = st.x == M ? 1.0f : __builtin_amdgcn_exp2f(st.x - M);
-        const float4 x = *reinterpret_cast<const float4*>(rec + (int64_t)c * kS);
-        L = fmaf(w, st.y, L);
-        o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    for (int c0 = 0; c0 < a.nrec; c0 += 8) {
+        float2 st[8];
+        float4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const int c = min(c0 + u, a.nrec - 1);
+            st[u] = stat[c];
+            x[u] = *reinterpret_cast<const float4*>(rec + (int64_t)c * kS);
+        }
+        float up = M;
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            if (c0 + u >= a.nrec) st[u] = make_float2(-INFINITY, 0.0f);
+            up = fmaxf(up, st[u].x);
+        }
+        const float shrink = M == up ? 1.0f : __builtin_amdgcn_exp2f(M - up);
+        M = up;
+        L *= shrink, o.x *= shrink, o.y *= shrink, o.z *= shrink, o.w *= shrink;
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const bool none = st[u].y == 0.0f;
+            const float w = none ? 0.0f : st[u].x == M ? 1.0f : __builtin_amdgcn_exp2f(st[u].x - M);
+            if (none) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            L = fmaf(w, st[u].y, L);
+            o.x = fmaf(w, x[u].x, o.x), o.y = fmaf(w, x[u].y, o.y), o.z = fmaf(w, x[u].z, o.z), o.w = fmaf(w, x[u].w, o.w);
+        }
     }
     const float inv = 1.0f / L;
     *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 struct PrefixPlan {
+    bool sweep, many;  // one sweep for a sequence's tiles; the prefix by many_queries
     int rtp, rto, ptiles, ppieces, prows, otiles, opieces;
 };
+static int pieces_of(int64_t others, int64_t rows, int64_t least, int64_t workgroups) {
+    int64_t n = others > 0 ? (workgroups + others / 2) / others : 1;
+    const int64_t most = (rows + least - 1) / least;
+    n = n < most ? n : most;
+    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
 static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t P, int64_t maxlen) {
     PrefixPlan p{};
     const int64_t Mq = qL * (H / Hkv), M = B * Mq;
-    p.rtp = M > 16 ? 2 : 1;
+    p.sweep = Mq >= 64;
+    if (p.sweep) {
+        p.rto = Mq > 64 ? 2 : 1;
+        p.otiles = (int)((Mq + 64 * p.rto - 1) / (64 * p.rto));
+        p.opieces = pieces_of(B * Hkv * p.otiles, P + maxlen, 256, 512);
+        return p;
+    }
+    p.many = M > 32;
+    p.rtp = p.many ? (M > 64 ? 2 : 1) : M > 16 ? 2 : 1;
     p.rto = Mq > 16 ? 2 : 1;
-    p.ptiles = (int)((M + 16 * p.rtp - 1) / (16 * p.rtp));
+    const int64_t tile = (p.many ? 64 : 16) * p.rtp;
+    p.ptiles = (int)((M + tile - 1) / tile);
     p.otiles = (int)((Mq + 16 * p.rto - 1) / (16 * p.rto));
-    auto pieces = [](int64_t others, int64_t rows) {
-        int64_t n = others > 0 ? (512 + others - 1) / others : 1;
-        const int64_t most = (rows + 127) / 128;
-        n = n < most ? n : most;
-        return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-    };
     if (P > 0) {
-        const int64_t n = pieces(Hkv * p.ptiles, P);
+        const int64_t n = pieces_of(Hkv * p.ptiles, P, 128, 512);
         p.prows = (int)((P + 128 * n - 1) / (128 * n) * 128);
         p.ppieces = (int)((P + p.prows - 1) / p.prows);
     }
-    p.opieces = pieces(B * Hkv * p.otiles, maxlen);
+    p.opieces = pieces_of(B * Hkv * p.otiles, maxlen, 128, 512);
     return p;
 }
 
@@ -724,11 +998,18 @@ static int prefix_launch(PrefixArgs a, PrepArgs p, const PrefixPlan& plan, hipSt
     LLMOPS_REQUIRE(prep < ((int64_t)1 << 31) && items < ((int64_t)1 << 31) && merge < ((int64_t)1 << 31));
     prefix_prep_kernel<T><<<(unsigned)prep, 256, 0, st>>>(a, p);
     LLMOPS_LAUNCH_CHECK();
-    if (plan.rtp == 1 && plan.rto == 1) prefix_attn_kernel<T, 1, 1><<<(unsigned)items, 256, 0, st>>>(a);
-    else if (plan.rto == 1) prefix_attn_kernel<T, 2, 1><<<(unsigned)items, 256, 0, st>>>(a);
-    else prefix_attn_kernel<T, 2, 2><<<(unsigned)items, 256, 0, st>>>(a);
+    const unsigned grid = (unsigned)items;
+    if (plan.sweep && plan.rto == 1) prefix_sweep_kernel<T, 1><<<grid, 256, 0, st>>>(a);
+    else if (plan.sweep) prefix_sweep_kernel<T, 2><<<grid, 256, 0, st>>>(a);
+    else if (plan.many && plan.rtp == 1 && plan.rto == 1) prefix_apart_kernel<T, 1, true, 1><<<grid, 256, 0, st>>>(a);
+    else if (plan.many && plan.rtp == 1) prefix_apart_kernel<T, 1, true, 2><<<grid, 256, 0, st>>>(a);
+    else if (plan.many && plan.rto == 1) prefix_apart_kernel<T, 2, true, 1><<<grid, 256, 0, st>>>(a);
+    else if (plan.many) prefix_apart_kernel<T, 2, true, 2><<<grid, 256, 0, st>>>(a);
+    else if (plan.rtp == 1) prefix_apart_kernel<T, 1, false, 1><<<grid, 256, 0, st>>>(a);
+    else if (plan.rto == 1) prefix_apart_kernel<T, 2, false, 1><<<grid, 256, 0, st>>>(a);
+    else prefix_apart_kernel<T, 2, false, 2><<<grid, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
-    prefix_merge_kernel<<<(unsigned)merge, 256, 0, st>>>(a);
+    if (a.nrec > 1) prefix_merge_kernel<<<(unsigned)merge, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }

@@ -48,7 +48,7 @@ struct PrefixArgs {
     int64_t pmax, maxlen;
     int B, qL, G, Hkv, P, M, Mq;        // M = B*qL*G, Mq = qL*G
     int ptiles, ppieces, prows;         // prefix: tiles of queries, pieces of rows, rows of a piece
-    int otiles, opieces;                // own rows (or all rows): tiles of a sequence's queries, pieces
+    int otiles, opieces, ostep;         // own rows (or all rows): tiles of a sequence's queries, pieces, least rows of one
     int nrec;
     unsigned pitems;
 };
@@ -272,21 +272,27 @@ __device__ __forceinline__ void score_step(v4f& acc, v4f& low, const Halves& k, 
     acc = mfma(k.hi, ql, acc);
 }
 
-// scores to weights: the running maximum, the sum, and what the sums so far shrink by.  sc[tt]: rows t + 16*tt + 4*g + v
+// the larger of this lane's value and those of the lanes 16, 32 and 48 away
+__device__ __forceinline__ float over_groups(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t w = __float_as_uint(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+    const auto y = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+
+// scores (before the factor, which is positive) to weights: the running maximum, the sum, and what the sums so far shrink by.
+// sc[tt]: rows t + 16*tt + 4*g + v
 template <int RT>
 __device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[2], int t, int g, bool masked) {
-    float top = -INFINITY;
+    if (masked) {
 #pragma unroll
-    for (int tt = 0; tt < 2; tt++)
+        for (int tt = 0; tt < 2; tt++)
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
-            float x = sc[tt][v] * s.c[rt];
-            if (masked) x = t + 16 * tt + 4 * g + v < s.see[rt] ? x : -INFINITY;
-            sc[tt][v] = x;
-            top = fmaxf(top, x);
-        }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+            for (int v = 0; v < 4; v++) sc[tt][v] = t + 16 * tt + 4 * g + v < s.see[rt] ? sc[tt][v] : -INFINITY;
+    }
+    float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    top = over_groups(top) * s.c[rt];
     if (__any(top > s.m[rt])) {
         const float m = fmaxf(s.m[rt], top), shrink = s.m[rt] == m ? 1.0f : __builtin_amdgcn_exp2f(s.m[rt] - m);
         s.m[rt] = m;
@@ -294,12 +300,12 @@ __device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[2], int 
 #pragma unroll
         for (int c = 0; c < 8; c++) s.o[rt][c] *= shrink;
     }
-    const float base = s.m[rt] == -INFINITY ? 0.0f : s.m[rt] - kLift;  // (nothing seen yet: every weight is exp2(-inf) = 0)
+    const float base = s.m[rt] == -INFINITY ? 0.0f : kLift - s.m[rt];  // (nothing seen yet: every weight is exp2(-inf) = 0)
 #pragma unroll
     for (int tt = 0; tt < 2; tt++)
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            sc[tt][v] = __builtin_amdgcn_exp2f(sc[tt][v] - base);
+            sc[tt][v] = __builtin_amdgcn_exp2f(fmaf(sc[tt][v], s.c[rt], base));
             s.l[rt] += sc[tt][v];
         }
 }
@@ -312,9 +318,12 @@ template <typename T>
 __device__ __forceinline__ Weights weights_of(const v4f (&sc)[2]) {
     Weights w;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        w.hi[j] = (_Float16)sc[j >> 2][j & 3];
-        w.lo[j] = (_Float16)(sc[j >> 2][j & 3] - (float)w.hi[j]);
+    for (int j = 0; j < 8; j += 2) {
+        const float x = sc[j >> 2][j & 3], y = sc[j >> 2][(j & 3) + 1];
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+        const v2h hv = __builtin_bit_cast(v2h, h);
+        w.hi[j] = hv[0], w.hi[j + 1] = hv[1];
+        w.lo[j] = (_Float16)fmaf((float)hv[0], -1.0f, x), w.lo[j + 1] = (_Float16)fmaf((float)hv[1], -1.0f, y);
     }
     if constexpr (sizeof(T) == 4) w.low = w.hi * (_Float16)(1.0f / 2048.0f);
     return w;
@@ -754,6 +763,7 @@ __device__ __forceinline__ void many_queries(const PrefixArgs& a, int hk, int m0
         const int buf = (j - j0) & 1;
         x.write(sm, buf ^ 1, wave, lane, ktop, vtop);  // (behind the last tile that one again: nobody reads it)
         load(min(j + 2, j1 - 1));
+        __builtin_amdgcn_sched_barrier(0);  // (asked for now: behind the scores' products they come late)
         const bool mine = j >= np;
         const int t = 32 * (mine ? j - np : j);
         const bool masked = __any(t + 32 > (mine ? see_min : K0.end));
@@ -784,11 +794,23 @@ __device__ __forceinline__ void many_queries(const PrefixArgs& a, int hk, int m0
             w[rt] = weights_of<T>(sc[rt]);
         }
 #pragma unroll
-        for (int c = 0; c < 8; c++) {
-            Halves h{as_v8h(sm.v[buf][0][c][lane]), v8h{}};
-            if constexpr (sizeof(T) == 4) h.lo = as_v8h(sm.v[buf][TileSmem<T>::kPieces - 1][c][lane]);
+        for (int c0 = 0; c0 < 8; c0 += 4) {
+            Halves h[4];
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) s.o[rt][c] = add_rows<T>(s.o[rt][c], h, w[rt]);
+            for (int c = 0; c < 4; c++) {
+                h[c].hi = as_v8h(sm.v[buf][0][c0 + c][lane]);
+                if constexpr (sizeof(T) == 4) h[c].lo = as_v8h(sm.v[buf][TileSmem<T>::kPieces - 1][c0 + c][lane]);
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) s.o[rt][c0 + c] = mfma(h[c].hi, w[rt].hi, s.o[rt][c0 + c]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) s.o[rt][c0 + c] = mfma(h[c].hi, w[rt].lo, s.o[rt][c0 + c]);
+                if constexpr (sizeof(T) == 4)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s.o[rt][c0 + c] = mfma(h[c].lo, w[rt].low, s.o[rt][c0 + c]);
+            }
         }
         __syncthreads();
     }
@@ -861,7 +883,7 @@ __global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a) {
         const int first = tile * 16 * RTO, m0 = b * a.Mq + first, m_end = (b + 1) * a.Mq;
         // rows that the tile's last live query sees, in pieces of whole 128
         const int last = min(n, (first + 16 * RTO - 1) / a.G + 1), rows = first < n * a.G ? len + last : 0;
-        const int step = max(128, (rows + 128 * a.opieces - 1) / (128 * a.opieces) * 128);
+        const int step = max(a.ostep, (rows + 128 * a.opieces - 1) / (128 * a.opieces) * 128);
         const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kS;
         const int end = min(rows, (piece + 1) * step);
         const Rows<T> K{(const T*)a.ok + plane, end}, V{(const T*)a.ov + plane, end};
@@ -937,12 +959,11 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
 
 struct PrefixPlan {
     bool sweep, many;  // one sweep for a sequence's tiles; the prefix by many_queries
-    int rtp, rto, ptiles, ppieces, prows, otiles, opieces;
+    int rtp, rto, ptiles, ppieces, prows, otiles, opieces, ostep;
 };
-static int pieces_of(int64_t others, int64_t rows, int64_t least, int64_t workgroups) {
-    int64_t n = others > 0 ? (workgroups + others / 2) / others : 1;
-    const int64_t most = (rows + least - 1) / least;
-    n = n < most ? n : most;
+// pieces of `rows`: some `wanted` of them, none below `least` rows
+static int pieces_of(int64_t wanted, int64_t rows, int64_t least) {
+    const int64_t most = (rows + least - 1) / least, n = wanted < most ? wanted : most;
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t P, int64_t maxlen) {
@@ -950,9 +971,13 @@ static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int
     const int64_t Mq = qL * (H / Hkv), M = B * Mq;
     p.sweep = Mq >= 64;
     if (p.sweep) {
-        p.rto = Mq > 64 ? 2 : 1;
+        // 64 queries to a workgroup until there are twice the workgroups that the chip holds of the other kind, 128 then (half the reading of
+        // cut rows per product); pieces where even that leaves the chip empty
+        p.rto = B * Hkv * ((Mq + 127) / 128) >= 1024 ? 2 : 1;
         p.otiles = (int)((Mq + 64 * p.rto - 1) / (64 * p.rto));
-        p.opieces = pieces_of(B * Hkv * p.otiles, P + maxlen, 256, 512);
+        const int64_t items = B * Hkv * p.otiles;
+        p.opieces = pieces_of((512 + items / 2) / items, P + maxlen, 256);
+        p.ostep = 1;
         return p;
     }
     p.many = M > 32;
@@ -961,12 +986,18 @@ static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int
     const int64_t tile = (p.many ? 64 : 16) * p.rtp;
     p.ptiles = (int)((M + tile - 1) / tile);
     p.otiles = (int)((Mq + 16 * p.rto - 1) / (16 * p.rto));
+    // Pieces of 512 rows of the prefix and 1024 of the own rows, so that none is the last at work; smaller ones, down to 128, until there are
+    // the 512 workgroups that the chip holds.  (us, prefix in pieces of 2048 / 1024 / 512 / 256 / 128: 32 tokens behind 2048 halves - / 45.1 / 46.2 /
+    // 49.0 / 53.2; 64 grouped behind 4001 112 / 68.7 / 52.5 / 63.0 / 73.4; 80 behind 1500 - / 78.0 / 65.4 / 66.8 / 75.9.)
+    const int64_t pitems = Hkv * p.ptiles, oitems = B * Hkv * p.otiles, all = (P > 0 ? pitems : 0) + oitems;
+    const int64_t fill = (512 + all - 1) / all;
     if (P > 0) {
-        const int64_t n = pieces_of(Hkv * p.ptiles, P, 128, 512);
+        const int64_t large = (P + 511) / 512, n = pieces_of(fill > large ? fill : large, P, 128);
         p.prows = (int)((P + 128 * n - 1) / (128 * n) * 128);
         p.ppieces = (int)((P + p.prows - 1) / p.prows);
     }
-    p.opieces = pieces_of(B * Hkv * p.otiles, maxlen, 128, 512);
+    p.ostep = fill > 1 ? 128 : 1024;
+    p.opieces = pieces_of(fill > 1 ? fill : (maxlen + 1023) / 1024, maxlen, p.ostep);
     return p;
 }
 
@@ -1065,7 +1096,7 @@ extern "C" int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, 
     a.lengths = lengths, a.q_lens = q_lens, a.out = out;
     a.pmax = prefix_maxlen, a.maxlen = maxlen;
     a.B = (int)B, a.qL = (int)qL, a.G = (int)(H / Hkv), a.Hkv = (int)Hkv, a.P = (int)prefix_len, a.Mq = (int)(qL * a.G), a.M = (int)(B * a.Mq);
-    a.ptiles = plan.ptiles, a.ppieces = plan.ppieces, a.prows = plan.prows, a.otiles = plan.otiles, a.opieces = plan.opieces;
+    a.ptiles = plan.ptiles, a.ppieces = plan.ppieces, a.prows = plan.prows, a.otiles = plan.otiles, a.opieces = plan.opieces, a.ostep = plan.ostep;
     a.nrec = plan.ppieces + plan.opieces;
     a.pitems = (unsigned)(Hkv * plan.ptiles * plan.ppieces);
     const PrepArgs p{q, k, v, inv_freq, q_stride_b, q_stride_l, k_stride_b, k_stride_l, v_stride_b, v_stride_l, (int)half, (int)((H + 2 * Hkv + 15) / 16)};

@@ -122,12 +122,9 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j0 = run * kRun;
     const float* z = a.logits + (int64_t)row * a.V + j0;
     const int n = min(kRun, a.V - j0);
-    float x[16];
+    float x[16];  // (unconditional loads: behind a branch each, they would be waited for one by one)
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-        const int j = threadIdx.x + 256 * e;
-        x[e] = j < n ? z[j] : -INFINITY;
-    }
+    for (int e = 0; e < 16; e++) x[e] = z[min((int)threadIdx.x + 256 * e, n - 1)];
     const float t = temperature_of(a, b);
     if (run == 0 && threadIdx.x == 255 && i < a.K) {
         const int64_t x = a.drafts[(int64_t)b * a.K + i];
@@ -141,7 +138,10 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     }
     float top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 16; e++) top = fmaxf(top, x[e]);
+    for (int e = 0; e < 16; e++) {
+        if ((int)threadIdx.x + 256 * e >= n) x[e] = -INFINITY;
+        top = fmaxf(top, x[e]);
+    }
     top = wave_top(top);
     if (t > 0.0f) {  // sums beside a wave's own maximum: the waves meet once
         const double per_t = kLog2e / (double)t;
@@ -259,21 +259,27 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     const bool spread = less;
     if (!spread && run > 0) return;
     double* rest = a.rest + (int64_t)b * a.runs;
-    // j of a thread's value e; what lies behind the row weighs nothing
-    auto z_at = [&](int at_run, int e) {
-        const int j = at_run * kRun + threadIdx.x + 256 * e;
-        return j < a.V ? zrow[j] : -INFINITY;
-    };
-    auto q_at = [&](int at_run, int e) {
-        const int j = at_run * kRun + threadIdx.x + 256 * e;
-        return qrow != nullptr && j < a.V ? qrow[j] : 0.0f;
+    // a thread's sixteen of a run, 256 apart; what lies behind the row weighs nothing
+    auto load = [&](int at_run, float (&z)[16], float (&q)[16]) {
+        const int j0 = at_run * kRun + threadIdx.x;
+#pragma unroll
+        for (int e = 0; e < 16; e++) z[e] = zrow[min(j0 + 256 * e, a.V - 1)];
+        if (qrow != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) q[e] = qrow[min(j0 + 256 * e, a.V - 1)];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) q[e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            if (j0 + 256 * e >= a.V) z[e] = -INFINITY;
     };
     const int sum_run = spread ? run : x >= 0 ? x / kRun : -1;
     double sum = 0.0;
     if (sum_run >= 0) {
         float z[16], q[16];
-#pragma unroll
-        for (int e = 0; e < 16; e++) z[e] = z_at(sum_run, e), q[e] = q_at(sum_run, e);
+        load(sum_run, z, q);
 #pragma unroll
         for (int e = 0; e < 16; e++) sum += rest_weight(r, z[e], per_t, less, q[e], sum_run * kRun + (int)threadIdx.x + 256 * e == x);
         sum = wave_sum64(sum);
@@ -331,11 +337,15 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     }
     if (at_run < 0) at_run = heavy, before = heavy_before;  // (rounding, or a random number of 1: the last token with a weight)
     // its tokens in their order, 16 to a thread
+    {
+        float z[16], q[16];
+        load(at_run, z, q);
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-        const int at = threadIdx.x + 256 * e + (threadIdx.x >> 4) + 16 * e;
-        neighbours[0][at] = z_at(at_run, e);
-        neighbours[1][at] = q_at(at_run, e);
+        for (int e = 0; e < 16; e++) {
+            const int at = threadIdx.x + 256 * e + (threadIdx.x >> 4) + 16 * e;
+            neighbours[0][at] = z[e];
+            neighbours[1][at] = q[e];
+        }
     }
     __syncthreads();
     const int j0 = at_run * kRun + 16 * threadIdx.x;

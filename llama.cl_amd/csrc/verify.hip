@@ -47,8 +47,9 @@ __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int b) { return a.
 __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int b) { return a.temperature != nullptr ? a.temperature[b] : a.one_temperature; }
 
 // 2^y for y <= 0: a whole power and a polynomial over [-1/2, 1/2] (degree 9, interpolated at Chebyshev's points: off by 1.9e-14 at
-// most, half the instructions of exp(), which is as exact as the type)
+// most, half the instructions of exp(), which is as exact as the type).  What is not above -1100, NaN too, gives 0
 __device__ __forceinline__ double power_of_two(double y) {
+    y = fmax(y, -1100.0);
     const double whole = rint(y), f = y - whole;
     double p = 0x1.b6571de2f2351p-24;
     p = fma(p, f, 0x1.63ef969a64d3cp-20);
@@ -60,15 +61,22 @@ __device__ __forceinline__ double power_of_two(double y) {
     p = fma(p, f, 0x1.ebfbdff8149f2p-3);
     p = fma(p, f, 0x1.62e42fefa39f7p-1);
     p = fma(p, f, 0x1.000000000003dp+0);
-    return ldexp(p, (int)fmax(whole, -2000.0));
+    return ldexp(p, (int)whole);
 }
-// exp((z - top) / T), per_t = log2(e) / T; a row without a value above minus infinity has no weight anywhere
-__device__ __forceinline__ double weight(float z, float top, double per_t) {
-    if (!(z > -INFINITY)) return 0.0;
-    return z == top ? 1.0 : top == INFINITY ? 0.0 : power_of_two(((double)z - (double)top) * per_t);
-}
+// exp((z - top) / T), per_t = log2(e) / T: 1 at the maximum, infinite or not; 0 for minus infinity and NaN, and everywhere in a row without
+// a value above minus infinity.  (Twenty instructions an element, the least that were found: they are most of the first launch.  The
+// rounding of `shift` is the same in all of a row's weights.)
+struct Weigher {
+    float one;  // the logit that weighs 1; NaN: none
+    double per_t, shift;
+    __device__ __forceinline__ Weigher(float top, double per) : one(top > -INFINITY ? top : NAN), per_t(per), shift(-(double)top * per) {}
+    __device__ __forceinline__ double operator()(float z) const {
+        const double p = power_of_two(fma((double)z, per_t, shift));
+        return z == one ? 1.0 : p;
+    }
+};
 // what a run's sum counts for beside the row's maximum
-__device__ __forceinline__ double share(float run_top, float top, double per_t) { return weight(run_top, top, per_t); }
+__device__ __forceinline__ double share(float run_top, float top, double per_t) { return Weigher(top, per_t)(run_top); }
 
 // Reductions over a wave whose steps stay in the vector ALU (a step through LDS waits some 100 cycles, and there are eight reductions one
 // behind the other in a call): neighbours at 1, 2, 4, 8 lanes below within rows of 16, then the rows' ends.  `other`: what lanes without
@@ -146,8 +154,9 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     if (t > 0.0f) {  // sums beside a wave's own maximum: the waves meet once
         const double per_t = kLog2e / (double)t;
         double sum = 0.0;
+        const Weigher weigh(top, per_t);
 #pragma unroll
-        for (int e = 0; e < 16; e++) sum += weight(x[e], top, per_t);
+        for (int e = 0; e < 16; e++) sum += weigh(x[e]);
         sum = wave_sum64(sum);
         if (lane == 0) tops[wave] = top, sums[wave] = sum;
         __syncthreads();
@@ -199,10 +208,10 @@ __device__ __forceinline__ Row row_of(const VerifyArgs& a, int row, bool draws, 
 }
 
 // what token j of a row weighs for the next token; q: its weight in the draft's distribution (behind a refused draft that has one)
-__device__ __forceinline__ double rest_weight(const Row& r, float z, double per_t, bool less, float q, bool out) {
-    const double p = weight(z, r.top, per_t) * r.inv;
-    if (less) return fmax(p - (double)q, 0.0);
-    return out ? 0.0 : p;
+__device__ __forceinline__ double rest_weight(const Weigher& weigh, double inv, float z, bool less, float q, bool out) {
+    const double p = weigh(z) * inv;
+    const double d = less ? fmax(p - (double)q, 0.0) : p;
+    return out ? 0.0 : d;
 }
 
 __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
@@ -228,7 +237,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
         if (i <= n) {
             const Draft d = a.draft[row0 + i];  // (behind the last draft: whatever is there, and not looked at)
             r = row_of(a, row0 + i, draws, per_t, lane);
-            const bool fits = d.x >= 0 && (draws ? (double)d.u * (double)d.q * r.sum < weight(d.z, r.top, per_t) : d.x == r.place);
+            const bool fits = d.x >= 0 && (draws ? (double)d.u * (double)d.q * r.sum < Weigher(r.top, per_t)(d.z) : d.x == r.place);
             if (lane == 0) shared_draft[wave] = d;
             if (lane == 0 && i < n && !fits) atomicMin(&first, i);
         }
@@ -240,6 +249,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     }
     const int done = first, row = row0 + done;
     const Row r = shared_row;
+    const Weigher weigh(r.top, per_t);
     const bool refused = done < n;
     const float *zrow = a.logits + (int64_t)row * a.V, *qrow = refused && probs != nullptr ? probs + (int64_t)done * a.V : nullptr;
     bool less = qrow != nullptr;
@@ -281,7 +291,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
         float z[16], q[16];
         load(sum_run, z, q);
 #pragma unroll
-        for (int e = 0; e < 16; e++) sum += rest_weight(r, z[e], per_t, less, q[e], sum_run * kRun + (int)threadIdx.x + 256 * e == x);
+        for (int e = 0; e < 16; e++) sum += rest_weight(weigh, r.inv, z[e], less, q[e], sum_run * kRun + (int)threadIdx.x + 256 * e == x);
         sum = wave_sum64(sum);
         if (lane == 0) red[wave] = sum;
         __syncthreads();
@@ -353,7 +363,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     sum = 0.0;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        w[e] = rest_weight(r, neighbours[0][17 * threadIdx.x + e], per_t, less, neighbours[1][17 * threadIdx.x + e], j0 + e == x);
+        w[e] = rest_weight(weigh, r.inv, neighbours[0][17 * threadIdx.x + e], less, neighbours[1][17 * threadIdx.x + e], j0 + e == x);
         sum += w[e];
     }
     const double to = scan64(sum);

@@ -12,12 +12,15 @@ This is the caller of the hot path, kept as thin as the reference's: every arith
 
 A decode step (one token, batch 1) has fixed shapes and no host-side decisions, so it can be
 captured once as a HIP graph and replayed (``capture_decode``).
+
+Several requests in step (``forward_requests``, ``step_requests``; no counterpart in the reference): sequences that share a prefix and
+differ in length, with low-rank adapters of their own, each bringing drafted tokens that the step checks.
 """
 import numpy as np
 import torch
 
 import llmops
-from llmops.opset import KVCache, llmop_embedding_q8c, llmop_fc_q4a, llmop_rmsnorm
+from llmops.opset import KVCache, LoraAdapters, PrefixCache, llmop_embedding_q8c, llmop_fc_q4a, llmop_rmsnorm
 
 LLAMA_7B = dict(layer_num=32, head_num=32, head_size=128, hidden_size=4096, intermediate_size=11008,
                 vocab_size=55296, rms_norm_eps=1e-5, rope_base=10000.0)
@@ -233,6 +236,111 @@ class LlamaDecoder:
     @staticmethod
     def _decode_fc(sums, *args, **kw):
         return llmops.fc_Q4A_decode(*args, want_sumsq=True, **kw) if sums else (llmops.fc_Q4A_decode(*args, **kw), None)
+
+    # ---- several requests in step ----
+    #: what a low-rank adapter may change in a layer
+    PROJECTIONS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
+
+    def read_prefix(self, input_ids, dtype=torch.float32):
+        """Runs the tokens int64 [1, P] that requests will have in common; returns their cache for ``PrefixCache``."""
+        kv = KVCache(self.configs, 1, input_ids.shape[1], device=self.device, dtype=dtype)
+        kv.prepare(input_ids.shape[1], 1, 0)
+        self.forward(input_ids, kv.cache, kv.slots, kv.position_id)
+        return kv.cache
+
+    def request_cache(self, batch_size, max_kv_len, prefix=None, dtype=None):
+        """A ``PrefixCache`` for this model behind a prefix that ``read_prefix`` has made (all of its rows)."""
+        return PrefixCache(self.configs, batch_size, max_kv_len, prefix, 0 if prefix is None else prefix.shape[3], self.device, dtype)
+
+    def set_adapters(self, layers, dtype=torch.float16):
+        """Low-rank adapters, by number: ``layers`` holds for each layer a dict from the names in ``PROJECTIONS`` to lists of
+        (A [r, K], B [N, r], scale) or None, all lists of one length; projections that are not named have none.  None takes them off."""
+        if layers is not None:
+            if len(layers) != len(self.layers):
+                raise ValueError("one dict of adapters for each layer")
+            counts = {len(a) for layer in layers for a in layer.values()}
+            unknown = {n for layer in layers for n in layer} - set(self.PROJECTIONS)
+            if unknown or len(counts) > 1:
+                raise ValueError(f"adapters of unknown projections {sorted(unknown)} or of different number {sorted(counts)}")
+            layers = [{n: LoraAdapters(a, self.device, dtype) for n, a in layer.items() if any(x is not None for x in a)} for layer in layers]
+            if any(n in layer for layer in layers for n in ("gate_proj", "up_proj")) and self.plan == "fused" and not self.stacked_gate_up:
+                raise ValueError("adapters of gate_proj and up_proj need their columns side by side (an intermediate size of whole strips)")
+        self.adapters = layers
+
+    def forward_requests(self, input_ids, cache, q_lens=None, adapters=None):
+        """Like ``forward`` for sequences that share ``cache``'s prefix: input_ids int64 [B, qL], the tokens behind those that each
+        sequence has kept (``cache.keep``).  q_lens int32 [B]: how many of the qL each brings; logits of the others mean nothing.
+        adapters int32 [B]: each sequence's number for ``set_adapters``, -1 for none.  All of it is read on the device: a captured call
+        serves following steps.  A sequence must have room for its tokens in the cache.  Returns logits fp32 [B, qL, vocab]."""
+        hidden_states = self.embed_tokens(input_ids)
+        own = getattr(self, "adapters", None)
+        if adapters is not None and own is None:
+            raise RuntimeError("no adapters are set (set_adapters)")
+        for i, ops in enumerate(self.layers):
+            hidden_states = self._layer_requests(i, ops, hidden_states, cache, q_lens, own[i] if adapters is not None else {}, adapters)
+        return llmops.fc_Q4A(self.norm.out_of_place(hidden_states), self.lm_head.weight, self.lm_head.N)
+
+    def _layer_requests(self, i, ops, hidden_states, cache, q_lens, lora, numbers):
+        H, F = self.configs["hidden_size"], self.configs["intermediate_size"]
+        fused = self.plan == "fused"
+
+        def add(name, y, x):
+            if name in lora:
+                lora[name](y, x, numbers)
+
+        def project(names, norm, stacked, width):
+            # the projections of one normalised input, as columns of one product or products of their own
+            changed = any(n in lora for n in names)
+            if fused and not changed:  # the norm rides in the product's launch
+                y = llmops.fc_Q4A_decode(hidden, ops[stacked].weight, width * len(names), norm=(norm.weight, norm.eps))
+                return [y[..., j * width:(j + 1) * width] for j in range(len(names))], y
+            x = norm.out_of_place(hidden)
+            if fused:
+                y = llmops.fc_Q4A(x, ops[stacked].weight, width * len(names))
+                parts = [y[..., j * width:(j + 1) * width] for j in range(len(names))]
+            else:
+                y, parts = None, [ops[n](x) for n in names]
+            for n, part in zip(names, parts):
+                add(n, part, x)
+            return parts, y
+
+        hidden = hidden_states
+        (q, k, v), _ = project(("q_proj", "k_proj", "v_proj"), ops["input_layernorm"], "qkv_proj", H)
+        attn = llmops.attention_rope_prefix(q, k, v, self.inv_freq, cache.prefix, cache.prefix_len, cache.cache, cache.lengths, i, q_lens=q_lens)
+        hidden = llmops.fc_Q4A(attn, ops["o_proj"].weight, H, residual=hidden_states)
+        add("o_proj", hidden, attn)
+        norm = ops["post_attention_layernorm"]
+        if fused and not self.stacked_gate_up:
+            act = llmops.fc_Q4A_decode(hidden, ops["gate_up_proj"].weight, F, norm=(norm.weight, norm.eps), glu=True)
+        else:
+            (gate, up), gate_up = project(("gate_proj", "up_proj"), norm, "gate_up_proj", F)
+            if fused and "down_proj" not in lora:
+                return llmops.fc_Q4A_decode(gate_up, ops["down_proj"].weight, H, residual=hidden, glu_in=True)
+            if fused:
+                act = llmops.silu_mul(gate_up)
+            else:
+                llmops.itrans(gate, "silu")
+                llmops.imul(up, gate)
+                act = up
+        out = llmops.fc_Q4A(act, ops["down_proj"].weight, H, residual=hidden)
+        add("down_proj", out, act)
+        return out
+
+    def step_requests(self, tokens, cache, uniforms, drafts=None, draft_probs=None, draft_lens=None, temperature=None, adapters=None):
+        """One step of several requests: each sequence's last token (``tokens`` int64 [B], not yet in the cache) and its K drafted ones
+        (``drafts`` int64 [B, K]; None: none) go through the model, the drafts are checked and the token behind those accepted is drawn
+        (``llmops.verify_drafts`` for the other arguments), and the rows of what was accepted are kept in the cache.  Returns its (tokens
+        [B, K+1], accepted [B]): ``tokens`` of the next step is ``result.gather(1, accepted[:, None].long())[:, 0]``."""
+        B = tokens.shape[0]
+        if drafts is None:
+            drafts = torch.empty((B, 0), dtype=torch.int64, device=tokens.device)
+        # (a draft that is no token, padding among them, is refused by the check: any row of the table will do for it)
+        ids = torch.cat((tokens[:, None], drafts), dim=1).clamp(0, self.embed_tokens.weight.shape[0] - 1)
+        q_lens = None if draft_lens is None else draft_lens.clamp(0, drafts.shape[1]) + 1
+        logits = self.forward_requests(ids, cache, q_lens, adapters)
+        result, accepted = llmops.verify_drafts(logits, drafts, uniforms, draft_probs=draft_probs, temperature=temperature, draft_lens=draft_lens)
+        cache.keep(accepted + 1)
+        return result, accepted
 
     def capture_decode(self, kv_cache, slot, position_id, stream=None):
         """Capture one decode step (batch 1, one token) as a HIP graph that serves every position: the token id,

@@ -124,3 +124,71 @@ class llmop_embedding_q8c:
 
     def __repr__(self):
         return f"llmop_embedding_q8c(weight: {list(self.weight.shape)})"
+
+
+class PrefixCache:
+    """KV cache of a batch whose sequences share a prefix (a system prompt, a document): the prefix's rows once, behind them
+    ``max_kv_len`` rows for each sequence (``llmops.attention_rope_prefix``).  The reference keeps the system prompt's rows in the one
+    cache of its one chat (mask -1 of chatllama/main.py:60-134); here many chats have them in common.
+
+    ``prefix`` is a cache [2*layers, 1, heads, rows, head_size] whose first ``prefix_len`` rows are filled (``LlamaDecoder.read_prefix``
+    makes one; several PrefixCaches may share it).  ``lengths`` (int32 [batch], on the device) counts each sequence's own rows: what a
+    model has been given with this cache counts from ``keep`` on; rows that are not kept are overwritten by the next call."""
+
+    def __init__(self, configs, batch_size, max_kv_len, prefix=None, prefix_len=0, device="cuda", dtype=None):
+        if dtype is None:
+            dtype = torch.float32 if prefix is None else prefix.dtype
+        if prefix is not None and (prefix.dtype != dtype or not 0 <= prefix_len <= prefix.shape[3]):
+            raise ValueError("the prefix has the cache's type and at least prefix_len rows")
+        self.prefix, self.prefix_len = prefix, int(prefix_len)
+        self.cache = torch.zeros(configs["layer_num"] * 2, batch_size, configs["head_num"], max_kv_len, configs["head_size"],
+                                 dtype=dtype, device=device)
+        self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        self.max_kv_len = max_kv_len
+
+    def size(self):
+        shared = self.prefix.numel() if self.prefix is not None else 0
+        return (self.cache.numel() + shared) * self.cache.element_size()
+
+    def keep(self, tokens):
+        """``tokens`` (an int, or int32 [batch] on the device) more rows of each sequence are its own from now on"""
+        self.lengths.add_(tokens).clamp_(0, self.max_kv_len)
+
+    def forget(self, sequence, length=0):
+        """a sequence ends (or goes back to its first ``length`` rows): a new one may begin behind the prefix"""
+        if not 0 <= length <= self.max_kv_len:
+            raise ValueError("length outside the cache")
+        self.lengths[sequence] = length
+
+
+class LoraAdapters:
+    """Low-rank adapters of one projection, by number: y + scale * (x A^T) B^T (``llmops.lora_add``).  ``adapters``: a list of
+    (A [r, K], B [N, r], scale) whose ranks may differ (they are padded to the largest), or None where an adapter leaves this
+    projection alone."""
+
+    def __init__(self, adapters, device="cuda", dtype=torch.float16):
+        some = [a for a in adapters if a is not None]
+        if not some:
+            raise ValueError("no adapter for this projection")
+        K, N = some[0][0].shape[1], some[0][1].shape[0]
+        for A, B, _ in some:
+            if A.dim() != 2 or B.dim() != 2 or A.shape[1] != K or B.shape[0] != N or B.shape[1] != A.shape[0]:
+                raise ValueError("adapters of one projection are A [r, K] and B [N, r] with the same K and N")
+        rank = max(A.shape[0] for A, _, _ in some)
+        rank += -rank % 8  # (rows of 16 bytes)
+        self.A = torch.zeros(len(adapters), rank, K, dtype=dtype, device=device)
+        self.B = torch.zeros(len(adapters), N, rank, dtype=dtype, device=device)
+        scales = [0.0] * len(adapters)
+        for i, a in enumerate(adapters):
+            if a is not None:
+                self.A[i, :a[0].shape[0]] = a[0].detach().to(self.A)
+                self.B[i, :, :a[1].shape[1]] = a[1].detach().to(self.B)
+                scales[i] = float(a[2])
+        self.scales = torch.tensor(scales, dtype=torch.float32, device=device)
+
+    def __call__(self, y, x, numbers):
+        """adds to y in place; numbers int32 [B]: each sequence's adapter, -1 for none"""
+        return llmops.lora_add(y, x, self.A, self.B, numbers, self.scales, out=y)
+
+    def __repr__(self):
+        return f"LoraAdapters({self.A.shape[0]} of rank {self.A.shape[1]}, {self.A.shape[2]} -> {self.B.shape[1]})"

@@ -1,0 +1,126 @@
+"""No-GPU checks of the entry points for several requests: bad arguments are refused before anything touches the device, workspaces
+are sized by host arithmetic, and the Python functions refuse host tensors."""
+import ctypes
+
+import pytest
+import torch
+
+import llmops
+from llmops import _lib
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+P = ctypes.c_void_p(4096)  # (an aligned address that is never followed: there is no device here, a launch would be a HIP error)
+NONE = ctypes.c_void_p(0)
+
+
+def _refused(lib, rc, what, code=1):
+    assert rc == code and what in lib.llmops_last_error(), (rc, lib.llmops_last_error())
+
+
+def _prefix(lib, **kw):
+    a = dict(q=P, qb=4096, ql=4096, k=P, kb=4096, kl=4096, v=P, vb=4096, vl=4096, B=2, qL=3, H=32, Hkv=8, S=128, f=P, half=64, pc=P, pplanes=2, pmax=100, plen=50,
+             kv=ctypes.c_void_p(1 << 40), dt=0, planes=2, maxlen=64, lengths=P, q_lens=NONE, layer=0, out=P, ws=P, bytes=1 << 40, stream=NONE)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.llmops_attention_rope_prefix(*a.values())
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(q=NONE), b"q != nullptr"), (dict(out=NONE), b"out != nullptr"), (dict(lengths=NONE), b"lengths != nullptr"), (dict(pc=NONE), b"prefix_cache != nullptr"),
+    (dict(S=64), b"S == 128"), (dict(H=30), b"prefix_sizes_fit"), (dict(Hkv=0), b"prefix_sizes_fit"), (dict(B=0), b"prefix_sizes_fit"), (dict(qL=0), b"prefix_sizes_fit"),
+    (dict(B=1 << 20, qL=1 << 10), b"prefix_sizes_fit"), (dict(plen=1 << 24, pmax=1 << 24), b"prefix_sizes_fit"), (dict(plen=-1), b"prefix_sizes_fit"),
+    (dict(plen=101), b"prefix_len <= prefix_maxlen"), (dict(half=65), b"2 * half <= S"), (dict(half=0), b"half > 0"), (dict(layer=1), b"layer_id"), (dict(layer=-1), b"layer_id"),
+    (dict(layer=1, planes=4), b"prefix_planes"), (dict(dt=2), b"cache_dtype"), (dict(q=ctypes.c_void_p(4104)), b"aligned(q, 16)"), (dict(ws=ctypes.c_void_p(4112)), b"aligned(workspace, 256)"),
+    (dict(kl=1026), b"k_stride_l % 4 == 0"), (dict(kv=P), b"p1 <= o0"), (dict(kv=ctypes.c_void_p(4096 + 4 * 1024 * 8)), b"p1 <= o0"),
+])
+def test_attention_rope_prefix_refuses(lib, kw, what):
+    _refused(lib, _prefix(lib, **kw), what)
+
+
+def test_attention_rope_prefix_workspace(lib):
+    need = lib.llmops_attention_prefix_workspace_bytes(2, 3, 32, 8, 128, 50, 64)
+    assert need > 2 * 3 * 32 * 128 * 4  # at least the rotated queries
+    _refused(lib, _prefix(lib, bytes=need - 1), b"workspace bytes", 2)
+    _refused(lib, _prefix(lib, ws=NONE), b"workspace != nullptr")
+    assert lib.llmops_attention_prefix_workspace_bytes(2, 3, 32, 8, 64, 50, 64) == 0
+    assert lib.llmops_attention_prefix_workspace_bytes(2, 3, 32, 5, 128, 50, 64) == 0
+
+
+def _lora(lib, **kw):
+    a = dict(y=P, yb=100, yl=100, x=P, xb=100, xl=100, B=4, M=2, N=64, K=96, A=P, W=P, dt=1, R=16, n=3, ids=P, scales=P, out=P, ob=100, ol=100, ws=P, bytes=1 << 40,
+             stream=NONE)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.llmops_lora_add(*a.values())
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(y=NONE), b"y != nullptr"), (dict(ids=NONE), b"ids != nullptr"), (dict(out=NONE), b"out != nullptr"), (dict(B=0), b"lora_sizes_fit"), (dict(M=-1), b"lora_sizes_fit"),
+    (dict(N=0), b"lora_sizes_fit"), (dict(K=0), b"lora_sizes_fit"), (dict(R=0), b"lora_sizes_fit"), (dict(R=4097), b"lora_sizes_fit"), (dict(B=1 << 12, M=1 << 9), b"lora_sizes_fit"),
+    (dict(n=0), b"adapters > 0"), (dict(dt=3), b"weight_dtype"), (dict(A=ctypes.c_void_p(4097)), b"aligned(lora_A, e)"), (dict(x=ctypes.c_void_p(4098)), b"aligned(x, 4)"),
+    (dict(W=ctypes.c_void_p(4098), dt=0), b"aligned(lora_B, e)"),
+])
+def test_lora_add_refuses(lib, kw, what):
+    _refused(lib, _lora(lib, **kw), what)
+
+
+def test_lora_add_workspace(lib):
+    for B, M, K, R, n in ((4, 2, 96, 16, 3), (1, 1, 4096, 8, 1), (1, 2048, 11008, 64, 1), (64, 1, 4096, 100, 64), (300, 20, 5000, 7, 9)):
+        need = lib.llmops_lora_workspace_bytes(B, M, 64, K, R, n)
+        assert need >= B * M * R * 4 and need % (B * M * R * 4) == 0  # (whole runs of K)
+        _refused(lib, _lora(lib, B=B, M=M, K=K, R=R, n=n, bytes=need - 1), b"workspace bytes", 2)
+    _refused(lib, _lora(lib, ws=NONE), b"workspace bytes", 2)
+    assert lib.llmops_lora_workspace_bytes(0, 1, 1, 1, 1, 1) == 0 and lib.llmops_lora_workspace_bytes(1, 1, 1, 1, 1, 0) == 0
+
+
+def _verify(lib, **kw):
+    a = dict(z=P, B=2, K=3, V=100, d=P, q=P, u=P, t=NONE, one=ctypes.c_float(1.0), n=NONE, tokens=P, accepted=P, ws=P, bytes=1 << 40, stream=NONE)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.llmops_verify_drafts(*a.values())
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(z=NONE), b"logits != nullptr"), (dict(u=NONE), b"uniforms != nullptr"), (dict(tokens=NONE), b"tokens != nullptr"), (dict(d=NONE), b"drafts != nullptr"),
+    (dict(B=0), b"verify_sizes_fit"), (dict(K=-1), b"verify_sizes_fit"), (dict(V=0), b"verify_sizes_fit"), (dict(V=(1 << 27) + 1), b"verify_sizes_fit"),
+    (dict(B=1 << 20, K=15), b"verify_sizes_fit"), (dict(d=ctypes.c_void_p(4100)), b"aligned(drafts, 8)"), (dict(ws=ctypes.c_void_p(4104)), b"aligned(workspace, 16)"),
+])
+def test_verify_drafts_refuses(lib, kw, what):
+    _refused(lib, _verify(lib, **kw), what)
+
+
+def test_verify_drafts_workspace(lib):
+    need = lib.llmops_verify_drafts_workspace_bytes(2, 3, 100)
+    assert need > 0
+    _refused(lib, _verify(lib, bytes=need - 1), b"workspace bytes", 2)
+    _refused(lib, _verify(lib, ws=NONE), b"workspace bytes", 2)
+    assert lib.llmops_verify_drafts_workspace_bytes(2, 3, 0) == 0
+
+
+def test_host_tensors_are_refused():
+    z = torch.zeros
+    with pytest.raises(RuntimeError, match="HIP device"):
+        llmops.attention_rope_prefix(z(1, 1, 128), z(1, 1, 128), z(1, 1, 128), z(64), None, 0, z(2, 1, 1, 4, 128), z(1, dtype=torch.int32), 0)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        llmops.lora_add(z(1, 1, 8), z(1, 1, 8), z(1, 8, 8), z(1, 8, 8), z(1, dtype=torch.int32), z(1))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        llmops.verify_drafts(z(1, 1, 8), z(1, 0, dtype=torch.int64), z(1, 1))
+
+
+def test_request_cache_bookkeeping_on_the_host():
+    from llmops.opset import PrefixCache
+    cfg = dict(layer_num=1, head_num=2, head_size=128)
+    c = PrefixCache(cfg, 3, 10, device="cpu")
+    c.keep(4)
+    c.keep(torch.tensor([1, 7, 0], dtype=torch.int32))
+    assert c.lengths.tolist() == [5, 10, 4] and c.size() == c.cache.numel() * 4 and c.prefix_len == 0
+    c.forget(1)
+    c.forget(0, 2)
+    assert c.lengths.tolist() == [2, 0, 4]
+    with pytest.raises(ValueError):
+        c.forget(0, 11)

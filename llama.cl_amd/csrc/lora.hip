@@ -22,10 +22,16 @@ struct LoraArgs {
     const float *x, *y, *scales;
     const void *A, *B;   // [adapters][R][K], [adapters][N][R]
     const int32_t* ids;  // [batch]
-    float *out, *part;   // part [splits][rows][R]
+    float *out, *part;   // part [splits][rows][rank_stride(R)]
     int64_t xsb, xsl, ysb, ysl, osb, osl;
     int rows, tokens, K, N, R, adapters, splits, chunk;
     int tiles;  // of a sequence; 0: tiles go on over the sequences' ends
+};
+
+// A row of partial sums takes up whole fours
+__host__ __device__ __forceinline__ int rank_stride(int R) { return (R + 3) & ~3; }
+struct __attribute__((packed, aligned(4))) Four32 {
+    float x[4];
 };
 
 // The tokens of a tile: numbers first .. end - 1.  Sequences of a tile's tokens or more have tiles of their own, so that a tile has one
@@ -337,10 +343,8 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) 
 #pragma unroll
         for (int w = 1; w < kDownWaves; w++) s += meet[w][m][lane];
         if (row >= tile.end) continue;
-        float* to = a.part + ((int64_t)blockIdx.y * a.rows + row) * a.R + r;
-#pragma unroll
-        for (int v = 0; v < 4; v++)
-            if (r + v < a.R) to[v] = s[v];
+        const int stride = rank_stride(a.R);  // (behind the last rank stands that one again, which nobody takes)
+        if (r < stride) *reinterpret_cast<Four32*>(a.part + ((int64_t)blockIdx.y * a.rows + row) * stride + r) = Four32{{s[0], s[1], s[2], s[3]}};
     }
 }
 
@@ -394,33 +398,26 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
     for (int r0 = 0; r0 < a.R && any; r0 += kRanks) {
         const int ranks = min(kRanks, a.R - r0), padded = (ranks + 31) & ~31;
         if (r0 > 0) __syncthreads();
-        // (two values and eight runs at a time: sixteen loads on their way; one by one they were two thirds of a prompt's launch)
-        for (int e0 = threadIdx.x; e0 < 16 * TT * padded; e0 += 512) {
-            float sum[2];
-            const float* from[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int e = e0 + 256 * h, token = e / padded, r = e - token * padded;
-                from[h] = e < 16 * TT * padded && r < ranks && row0 + token < tile.end ? a.part + (int64_t)(row0 + token) * a.R + r0 + r : nullptr;
-                sum[h] = 0.0f;
-            }
-            const int64_t run = (int64_t)a.rows * a.R;
+        // (four neighbours and eight runs at a time, all on their way together; value by value they were two thirds of a prompt's launch)
+        const int fours = padded / 4;
+        for (int e = threadIdx.x; e < 16 * TT * fours; e += 256) {
+            const int token = e / fours, r = 4 * (e - token * fours), stride = rank_stride(a.R);
+            const bool there = r < ranks && row0 + token < tile.end;
+            const float* from = a.part + (there ? (int64_t)(row0 + token) * stride + r0 + r : 0);
+            const int64_t run = (int64_t)a.rows * stride;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
             for (int c = 0; c < a.splits; c += 8) {
-                float x[2][8];
+                Four32 x[8];
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int u = 0; u < 8; u++) x[u] = *reinterpret_cast<const Four32*>(from + min(c + u, a.splits - 1) * run);
 #pragma unroll
-                    for (int u = 0; u < 8; u++) x[h][u] = (from[h] != nullptr ? from[h] : a.part)[min(c + u, a.splits - 1) * run];
+                for (int u = 0; u < 8; u++)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int u = 0; u < 8; u++) sum[h] += c + u < a.splits ? x[h][u] : 0.0f;
+                    for (int v = 0; v < 4; v++) sum[v] += c + u < a.splits ? x[u].x[v] : 0.0f;
             }
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int e = e0 + 256 * h, token = e / padded;
-                if (e < 16 * TT * padded) t[token][e - token * padded] = from[h] != nullptr ? sum[h] : 0.0f;
-            }
+            for (int v = 0; v < 4; v++) sum[v] = there && r + v < ranks ? sum[v] : 0.0f;
+            *reinterpret_cast<float4*>(&t[token][r]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
         }
         Adapters some(lane < 16 * TT ? of_lane : -1);
         struct Stage {
@@ -559,7 +556,7 @@ static bool lora_sizes_fit(int64_t batch, int64_t tokens, int64_t N, int64_t K, 
 extern "C" size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R, int64_t adapters) {
     if (!lora_sizes_fit(batch, tokens, N, K, R) || adapters <= 0) return 0;
     const int64_t chunk = lora_chunk(batch, tokens, K, R, adapters);
-    return (size_t)((K + chunk - 1) / chunk) * (size_t)(batch * tokens) * (size_t)R * sizeof(float);
+    return (size_t)((K + chunk - 1) / chunk) * (size_t)(batch * tokens) * (size_t)rank_stride((int)R) * sizeof(float);
 }
 
 extern "C" int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, const float* x, int64_t x_stride_b, int64_t x_stride_l, int64_t batch,

@@ -292,7 +292,8 @@ int llmops_attention_rope_decode_records(float* q, float* k, const float* v, int
  *   q [B,qL,H*S], k and v [B,qL,Hkv*S] fp32, token l of sequence b at + b*stride_b + l*stride_l elements (multiples of 4: columns of a
  * projection's output will do), unchanged; out [B,qL,H*S] dense.  inv_freq [half], 2*half <= S: as llmops_rope_embed, but the angle
  * inv_freq * position keeps the product's rounding error, which fp32 loses (1e-4 at position 4000).  S == 128; 16-byte aligned
- * pointers, 256-byte aligned workspace; prefix_len + maxlen <= 2^24.  prefix_len may be 0 (prefix_cache may then be NULL).
+ * pointers, 256-byte aligned workspace; prefix_len + maxlen <= 2^24, and each launch
+ * below 2^24 workgroups, as it is while B*qL*H * (2 + maxlen/1024) is.  prefix_len may be 0 (prefix_cache may then be NULL).
  * prefix_cache and kv_cache must not overlap.
  * Results agree with fp32 evaluation to about 1e-6 of the largest output, and are the same bits in every call. */
 size_t llmops_attention_prefix_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t prefix_len, int64_t maxlen);
@@ -307,9 +308,10 @@ int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_s
  * lora_A [adapters,R,K] and lora_B [adapters,N,R], dense, of weight_dtype (LLMOPS_F32, _F16, _BF16); scales fp32 [adapters] and ids
  * int32 [batch] on the device.  An id outside 0 .. adapters-1 (-1) is none: out = y.  Adapters of a lower rank than R are padded with
  * zeros.  x [batch,tokens,K], y and out [batch,tokens,N] fp32, token l of sequence b at + b*stride_b + l*stride_l elements; out may be y
- * (the same pointer and strides) and must not overlap x or y otherwise.  Up to 2^20 tokens in all, R up to 4096.  Sizes and
- * strides are free.
- * fp32 arithmetic, except that products are formed of exact bf16 pieces: what is dropped is below 2^-22 of a product. */
+ * (the same pointer and strides) and must not overlap x or y otherwise.  Up to 2^20 tokens in all, R up to 4096, N and K
+ * below 2^29; other sizes and the strides are free.
+ * fp32 arithmetic, except that products are formed of exact bf16 pieces: what is dropped is below 2^-22 of a product, and an infinity
+ * among a sequence's x or its adapter's weights leaves NaN in what depends on it. */
 size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R, int64_t adapters);
 int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, const float* x, int64_t x_stride_b, int64_t x_stride_l,
                     int64_t batch, int64_t tokens, int64_t N, int64_t K, const void* lora_A, const void* lora_B, int weight_dtype, int64_t R,
@@ -327,8 +329,9 @@ int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, cons
  * uniforms fp32 [B,K+1], in [0, 1): [b,K] draws the next token.
  * tokens int64 [B,K+1]: the accepted drafts, the next token, -1 behind; accepted int32 [B]: how many drafts.
  * Logits that are NaN or minus infinity weigh nothing, equal plus infinities share the row; a row without any other logit gives -1.
- * Exponentials and sums are in 64 bits: the answer is the definition's but for numbers within about 1e-13 of a border.
- * B*(K+1) < 2^24, V <= 2^27. */
+ * Exponentials and sums are in 64 bits: the answer is the definition's but for numbers within about 1e-13 (at a temperature below 1e-3 of
+ * the largest logit: 2e-16 of their ratio) of a border.
+ * B*(K+1) < 2^24, V <= 2^27, B*V < 2^36. */
 size_t llmops_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
 int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, int64_t V, const int64_t* drafts, const float* draft_probs,
                          const float* uniforms, const float* temperature, float one_temperature, const int32_t* draft_lens, int64_t* tokens,

@@ -1025,8 +1025,8 @@ static PrefixLayout layout_prefix(int64_t rows, int nrec) {
 template <typename T>
 static int prefix_launch(PrefixArgs a, PrepArgs p, const PrefixPlan& plan, hipStream_t st) {
     const int64_t prep = (int64_t)a.B * a.qL * p.groups, items = (int64_t)a.pitems + (int64_t)a.B * a.Hkv * a.otiles * a.opieces,
-                  merge = ((int64_t)a.Hkv * a.M + 7) / 8;
-    LLMOPS_REQUIRE(prep < ((int64_t)1 << 31) && items < ((int64_t)1 << 31) && merge < ((int64_t)1 << 31));
+                  merge = ((int64_t)a.Hkv * a.M + 7) / 8, most = (int64_t)1 << 24;  // (a launch has fewer than 2^32 threads)
+    LLMOPS_REQUIRE(prep < most && items < most && merge < most);
     prefix_prep_kernel<T><<<(unsigned)prep, 256, 0, st>>>(a, p);
     LLMOPS_LAUNCH_CHECK();
     const unsigned grid = (unsigned)items;
@@ -1098,7 +1098,9 @@ extern "C" int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, 
     a.B = (int)B, a.qL = (int)qL, a.G = (int)(H / Hkv), a.Hkv = (int)Hkv, a.P = (int)prefix_len, a.Mq = (int)(qL * a.G), a.M = (int)(B * a.Mq);
     a.ptiles = plan.ptiles, a.ppieces = plan.ppieces, a.prows = plan.prows, a.otiles = plan.otiles, a.opieces = plan.opieces, a.ostep = plan.ostep;
     a.nrec = plan.ppieces + plan.opieces;
-    a.pitems = (unsigned)(Hkv * plan.ptiles * plan.ppieces);
+    const int64_t pitems = Hkv * plan.ptiles * plan.ppieces;
+    LLMOPS_REQUIRE(pitems < ((int64_t)1 << 24));
+    a.pitems = (unsigned)pitems;
     const PrepArgs p{q, k, v, inv_freq, q_stride_b, q_stride_l, k_stride_b, k_stride_l, v_stride_b, v_stride_l, (int)half, (int)((H + 2 * Hkv + 15) / 16)};
     hipStream_t st = as_stream(stream);
     return cache_dtype == LLMOPS_CACHE_F32 ? prefix_launch<float>(a, p, plan, st) : prefix_launch<__half>(a, p, plan, st);

@@ -548,7 +548,7 @@ static int lora_launch(LoraArgs a, bool vec_out, hipStream_t st) {
 using namespace llmops;
 
 static bool lora_sizes_fit(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R) {
-    const int64_t most = (int64_t)1 << 30;
+    const int64_t most = (int64_t)1 << 29;  // (a launch has fewer than 2^32 threads, four to a column; K + what a step reaches fits 31 bits)
     return batch > 0 && tokens > 0 && N > 0 && K > 0 && R > 0 && batch < most && tokens < most && N < most && K < most && R <= 4096 &&
            batch * tokens <= ((int64_t)1 << 20) && lora_tiles(batch, tokens) <= 65535;
 }

@@ -620,7 +620,8 @@ def lora_add(y, x, lora_A, lora_B, adapters, scales, out=None):
     if out is None:
         out = torch.empty((B, M, N), dtype=torch.float32, device=y.device)
     op, ob, ol = _rows(out, "out")
-    _require(tuple(out.shape) == (B, M, N) and (B == 1 or abs(ob) >= N) and (M == 1 or abs(ol) >= N), "out.is({B, M, N}), rows apart")
+    _require(tuple(out.shape) == (B, M, N), "out.is({B, M, N})")
+    _require((M == 1 or ol >= N) and (B == 1 or ob >= (M - 1) * ol + N) or (B == 1 or ob >= N) and (M == 1 or ol >= (B - 1) * ob + N), "out's rows apart")
     _here(y, x=x, lora_A=lora_A, lora_B=lora_B, adapters=adapters, scales=scales, out=out)
     lib = _lib.load()
     ws = torch.empty(max(lib.llmops_lora_workspace_bytes(B, M, N, K, R, n), 1), dtype=torch.uint8, device=y.device)

@@ -329,7 +329,8 @@ class LlamaDecoder:
     def step_requests(self, tokens, cache, uniforms, drafts=None, draft_probs=None, draft_lens=None, temperature=None, adapters=None):
         """One step of several requests: each sequence's last token (``tokens`` int64 [B], not yet in the cache) and its K drafted ones
         (``drafts`` int64 [B, K]; None: none) go through the model, the drafts are checked and the token behind those accepted is drawn
-        (``llmops.verify_drafts`` for the other arguments), and the rows of what was accepted are kept in the cache.  Returns its (tokens
+        (``llmops.verify_drafts`` for the other arguments), and the rows of what was accepted are kept in the cache, which must have room for
+        1 + K (or 1 + draft_lens) of them in each sequence whose answer is used.  Returns its (tokens
         [B, K+1], accepted [B]): ``tokens`` of the next step is ``result.gather(1, accepted[:, None].long())[:, 0]``."""
         B = tokens.shape[0]
         if drafts is None:

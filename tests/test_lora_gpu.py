@@ -140,3 +140,9 @@ def test_refusals():
         llmops.lora_add(y, x, A, W, ids, scales, out=y[:1].expand(2, -1, -1))
     with pytest.raises(RuntimeError):
         llmops.lora_add(y, x, A, W, ids, scales, out=y[:, :1])
+    for strides in ((32, 32, 1), (48, 32, 1), (32, 48, 1), (64, 31, 1), (31, 64, 1)):  # rows one in the other
+        with pytest.raises(RuntimeError, match="rows apart"):
+            llmops.lora_add(y, x, A, W, ids, scales, out=torch.empty(200, device="cuda").as_strided((2, 2, 32), strides))
+    for strides in ((64, 32, 1), (32, 64, 1), (100, 40, 1)):
+        out = torch.empty(200, device="cuda").as_strided((2, 2, 32), strides)
+        assert torch.equal(llmops.lora_add(y, x, A, W, ids, scales, out=out), llmops.lora_add(y, x, A, W, ids, scales))

@@ -35,6 +35,7 @@ def _prefix(lib, **kw):
     (dict(S=64), b"S == 128"), (dict(H=30), b"prefix_sizes_fit"), (dict(Hkv=0), b"prefix_sizes_fit"), (dict(B=0), b"prefix_sizes_fit"), (dict(qL=0), b"prefix_sizes_fit"),
     (dict(B=1 << 20, qL=1 << 10), b"prefix_sizes_fit"), (dict(plen=1 << 24, pmax=1 << 24), b"prefix_sizes_fit"), (dict(plen=-1), b"prefix_sizes_fit"),
     (dict(plen=101), b"prefix_len <= prefix_maxlen"), (dict(half=65), b"2 * half <= S"), (dict(half=0), b"half > 0"), (dict(layer=1), b"layer_id"), (dict(layer=-1), b"layer_id"),
+    (dict(B=1 << 22, qL=2, H=16, Hkv=1, maxlen=1, kv=ctypes.c_void_p(1 << 56)), b"merge < most"), (dict(B=(1 << 24) - 1, qL=2, H=1, Hkv=1, maxlen=1, pc=NONE, plen=0), b"prep < most"),
     (dict(layer=1, planes=4), b"prefix_planes"), (dict(dt=2), b"cache_dtype"), (dict(q=ctypes.c_void_p(4104)), b"aligned(q, 16)"), (dict(ws=ctypes.c_void_p(4112)), b"aligned(workspace, 256)"),
     (dict(kl=1026), b"k_stride_l % 4 == 0"), (dict(kv=P), b"p1 <= o0"), (dict(kv=ctypes.c_void_p(4096 + 4 * 1024 * 8)), b"p1 <= o0"),
 ])
@@ -63,7 +64,7 @@ def _lora(lib, **kw):
     (dict(y=NONE), b"y != nullptr"), (dict(ids=NONE), b"ids != nullptr"), (dict(out=NONE), b"out != nullptr"), (dict(B=0), b"lora_sizes_fit"), (dict(M=-1), b"lora_sizes_fit"),
     (dict(N=0), b"lora_sizes_fit"), (dict(K=0), b"lora_sizes_fit"), (dict(R=0), b"lora_sizes_fit"), (dict(R=4097), b"lora_sizes_fit"), (dict(B=1 << 12, M=1 << 9), b"lora_sizes_fit"),
     (dict(n=0), b"adapters > 0"), (dict(dt=3), b"weight_dtype"), (dict(A=ctypes.c_void_p(4097)), b"aligned(lora_A, e)"), (dict(x=ctypes.c_void_p(4098)), b"aligned(x, 4)"),
-    (dict(W=ctypes.c_void_p(4098), dt=0), b"aligned(lora_B, e)"),
+    (dict(W=ctypes.c_void_p(4098), dt=0), b"aligned(lora_B, e)"), (dict(N=1 << 29), b"lora_sizes_fit"), (dict(K=1 << 29), b"lora_sizes_fit"),
 ])
 def test_lora_add_refuses(lib, kw, what):
     _refused(lib, _lora(lib, **kw), what)
@@ -72,7 +73,8 @@ def test_lora_add_refuses(lib, kw, what):
 def test_lora_add_workspace(lib):
     for B, M, K, R, n in ((4, 2, 96, 16, 3), (1, 1, 4096, 8, 1), (1, 2048, 11008, 64, 1), (64, 1, 4096, 100, 64), (300, 20, 5000, 7, 9)):
         need = lib.llmops_lora_workspace_bytes(B, M, 64, K, R, n)
-        assert need >= B * M * R * 4 and need % (B * M * R * 4) == 0  # (whole runs of K)
+        row = (R + 3) // 4 * 16
+        assert need >= B * M * row and need % (B * M * row) == 0  # (whole runs of K, a row of sums in whole fours)
         _refused(lib, _lora(lib, B=B, M=M, K=K, R=R, n=n, bytes=need - 1), b"workspace bytes", 2)
     _refused(lib, _lora(lib, ws=NONE), b"workspace bytes", 2)
     assert lib.llmops_lora_workspace_bytes(0, 1, 1, 1, 1, 1) == 0 and lib.llmops_lora_workspace_bytes(1, 1, 1, 1, 1, 0) == 0
@@ -88,7 +90,7 @@ def _verify(lib, **kw):
 @pytest.mark.parametrize("kw,what", [
     (dict(z=NONE), b"logits != nullptr"), (dict(u=NONE), b"uniforms != nullptr"), (dict(tokens=NONE), b"tokens != nullptr"), (dict(d=NONE), b"drafts != nullptr"),
     (dict(B=0), b"verify_sizes_fit"), (dict(K=-1), b"verify_sizes_fit"), (dict(V=0), b"verify_sizes_fit"), (dict(V=(1 << 27) + 1), b"verify_sizes_fit"),
-    (dict(B=1 << 20, K=15), b"verify_sizes_fit"), (dict(d=ctypes.c_void_p(4100)), b"aligned(drafts, 8)"), (dict(ws=ctypes.c_void_p(4104)), b"aligned(workspace, 16)"),
+    (dict(B=1 << 20, K=15), b"verify_sizes_fit"), (dict(B=1 << 20, V=1 << 16), b"a.runs < "), (dict(d=ctypes.c_void_p(4100)), b"aligned(drafts, 8)"), (dict(ws=ctypes.c_void_p(4104)), b"aligned(workspace, 16)"),
 ])
 def test_verify_drafts_refuses(lib, kw, what):
     _refused(lib, _verify(lib, **kw), what)

@@ -311,3 +311,23 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="p1 <= o0"):  # the prefix inside the batch's own cache
         llmops.attention_rope_prefix(q[:1], k[:1], v[:1], f, one, 4, one, n[:1], 0)
     assert torch.equal(cache, before)
+
+
+def test_offsets_past_32_bits():
+    """the last of many sequences in a cache whose planes hold more than 2^31 values, beside the same sequence alone"""
+    B, H, maxlen, n, P = 40, 8, 65536, 65534, 70
+    g = torch.Generator(device="cuda").manual_seed(11)
+    q, k, v = (torch.randn(B, 2, H * S, generator=g, device="cuda") for _ in range(3))
+    prefix = torch.randn(2, 1, H, P, S, generator=g, device="cuda").half()
+    alone = torch.randn(2, 1, H, maxlen, S, generator=g, device="cuda").half()
+    kv = torch.empty(2, B, H, maxlen, S, dtype=torch.float16, device="cuda")
+    kv[:, B - 1] = alone[:, 0]
+    lengths = torch.zeros(B, dtype=torch.int32, device="cuda")
+    lengths[B - 1] = n
+    f = _inv_freq().cuda()
+    out = llmops.attention_rope_prefix(q, k, v, f, prefix, P, kv, lengths, 0)
+    one = llmops.attention_rope_prefix(q[B - 1:], k[B - 1:], v[B - 1:], f, prefix, P, alone, lengths[B - 1:], 0)
+    assert torch.equal(kv[:, B - 1], alone[:, 0])
+    err = (out[B - 1] - one[0]).double()  # (each is off by REL at most)
+    assert err.norm() <= 2 * REL * one.double().norm() and err.abs().max() <= 2 * MAX * one.abs().max()
+    assert out.isfinite().all()

@@ -146,3 +146,15 @@ def test_refusals():
     for strides in ((64, 32, 1), (32, 64, 1), (100, 40, 1)):
         out = torch.empty(200, device="cuda").as_strided((2, 2, 32), strides)
         assert torch.equal(llmops.lora_add(y, x, A, W, ids, scales, out=out), llmops.lora_add(y, x, A, W, ids, scales))
+
+
+def test_offsets_past_32_bits():
+    """the last of many sequences whose x is more than 2^32 values"""
+    B, M, K, N = 1 << 10, 1 << 10, 4100, 32
+    y, x1, A, W, _, scales = _case(1, M, N, K, 8, 1, "fp16", seed=13)
+    x = torch.zeros(B, M, K, device="cuda")
+    x[B - 1] = x1[0].cuda()
+    ids = torch.zeros(B, dtype=torch.int32)
+    out = llmops.lora_add(y.cuda().expand(B, M, N), x, A.cuda(), W.cuda(), ids.cuda(), scales.cuda())
+    _check(out[B - 1:], y, _delta(x1, A, W, ids[:1], scales))
+    assert torch.equal(out[:B - 1], y.cuda().expand(B - 1, M, N))

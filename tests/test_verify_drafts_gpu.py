@@ -239,3 +239,33 @@ def test_refusals():
                      ((logits, drafts, uniforms), dict(draft_lens=n[:1])), ((logits, drafts.cpu(), uniforms), {}), ((logits, drafts[:, ::2], uniforms), {})):
         with pytest.raises(RuntimeError):
             llmops.verify_drafts(*args, **kw)
+
+
+def test_numbers_that_are_none_of_the_definitions():
+    """random numbers and temperatures outside their ranges: still a token that weighs something"""
+    logits, drafts, uniforms, q = _case(8, 3, 4200, True, seed=6)
+    logits[:, :, :50] = -math.inf
+    for bad in (math.nan, math.inf, -math.inf, -1.0, 2.0):
+        for t in (None, math.inf, 1e-40, math.nan):
+            for probs in (q.cuda(), None):
+                u = uniforms.clone()
+                u[::2], u[1, 3], u[3, 0] = bad, bad, bad
+                tokens, n = llmops.verify_drafts(logits.cuda(), drafts.cuda(), u.cuda(), draft_probs=probs, temperature=t)
+                tokens, n = tokens.cpu(), n.cpu()
+                assert ((n >= 0) & (n <= 3)).all()
+                last = tokens.gather(1, n[:, None].long())[:, 0]
+                assert ((last >= 50) & (last < 4200)).all() and (tokens[torch.arange(4)[None] > n[:, None]] == -1).all()
+
+
+def test_offsets_past_32_bits():
+    """the last of many sequences whose logits are more than 2^31 values, beside the same sequence alone"""
+    B, K, V = 64, 3, (1 << 23) + 5
+    g = torch.Generator(device="cuda").manual_seed(12)
+    logits, q = torch.zeros(B, K + 1, V, device="cuda"), torch.zeros(B, K, V, device="cuda")
+    logits[B - 1] = torch.randn(K + 1, V, generator=g, device="cuda")
+    q[B - 1] = torch.softmax(logits[B - 1, :K] + torch.randn(K, V, generator=g, device="cuda"), -1)
+    drafts, uniforms = torch.randint(0, V, (B, K), generator=g, device="cuda"), torch.rand(B, K + 1, generator=g, device="cuda")
+    for probs in (q, None):
+        tokens, n = llmops.verify_drafts(logits, drafts, uniforms, draft_probs=probs)
+        one, m = llmops.verify_drafts(logits[B - 1:], drafts[B - 1:], uniforms[B - 1:], draft_probs=None if probs is None else probs[B - 1:])
+        assert torch.equal(tokens[B - 1:], one) and torch.equal(n[B - 1:], m)

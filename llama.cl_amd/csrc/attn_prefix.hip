@@ -6,7 +6,7 @@
 //   pos = P + len[b] + l,  q' = rot(q, pos),  own row len[b] + l = (rot(k, pos), v) in the cache's type,
 //   out = sum_r e_r V_r / sum_r e_r,  e_r = exp(q' . K_r / sqrt(S) - max),  r over the P prefix rows and own rows 0 .. len[b] + l.
 //
-//   1. prefix_prep_kernel   rotates, writes the new cache rows and leaves q' as operands of the matrix instructions
+//   1. prefix_prep_kernel   rotates, writes the new cache rows and leaves q' as operands of the matrix instructions (part of 2 where that is one round)
 //   2. prefix_apart_kernel  softmax(q'K^T)V of a piece of the rows for a tile of queries: running maximum and sum, one pass; the prefix
 //      prefix_sweep_kernel  and the own rows apart, or in one sweep where a sequence has queries to fill tiles of its own
 //   3. prefix_merge_kernel  joins the pieces of a query, where there are several
@@ -86,53 +86,34 @@ struct PrepArgs {
     int half, groups;
 };
 
-// A workgroup per token and 16 of its H + 2*Hkv rows of 128, 16 lanes to a row, dims 4i .. +3 and 64 + 4i .. +3 to lane i.
-// Bound by latency at few tokens and by memory at many.
-template <typename T>
-__global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a, PrepArgs p) {
-    __shared__ float turn[2][64];
-    const int bl = blockIdx.x / p.groups, group = blockIdx.x - bl * p.groups, b = bl / a.qL, l = bl - b * a.qL;
-    int len, n;
-    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-    const bool live = l < n;
-    if (live && (int)threadIdx.x < p.half) turn_of(p.inv_freq[threadIdx.x], a.P + len + l, turn[0][threadIdx.x], turn[1][threadIdx.x]);
-    __syncthreads();
-    const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), i4 = 4 * (threadIdx.x & 15);
-    if (row >= H + 2 * a.Hkv) return;
-    const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv;
-    if (!live && !is_q) return;
-    const float* src = is_q ? p.q + b * p.qsb + l * p.qsl + (int64_t)row * kS
-                            : is_k ? p.k + b * p.ksb + l * p.ksl + (int64_t)(row - H) * kS : p.v + b * p.vsb + l * p.vsl + (int64_t)(row - H - a.Hkv) * kS;
-    float x[8];
-    {
-        const float4 lo = *reinterpret_cast<const float4*>(src + i4), hi = *reinterpret_cast<const float4*>(src + 64 + i4);
-        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-    }
-    if (is_q || is_k) {
-        if (live && p.half == 64) {
+// Sixteen lanes to a row of 128: dims d .. d+3 and 64+d .. +3 to a lane, d = 4 * (lane % 16)
+__device__ __forceinline__ void load_row(const float* __restrict__ src, int d, float (&x)[8]) {
+    const float4 lo = *reinterpret_cast<const float4*>(src + d), hi = *reinterpret_cast<const float4*>(src + 64 + d);
+    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+}
+__device__ __forceinline__ void turn_row(const float* __restrict__ src, int d, const float2* turn, int half, float (&x)[8]) {
+    if (half == 64) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float c = turn[0][i4 + e], s = turn[1][i4 + e], x0 = x[e], x1 = x[4 + e];
-                x[e] = c * x0 - s * x1;
-                x[4 + e] = s * x0 + c * x1;
-            }
-        } else if (live) {  // pairs (d, d + half), the other dims as they are
+        for (int e = 0; e < 4; e++) {
+            const float c = turn[d + e].x, s = turn[d + e].y, x0 = x[e], x1 = x[4 + e];
+            x[e] = c * x0 - s * x1;
+            x[4 + e] = s * x0 + c * x1;
+        }
+    } else {  // pairs (at, at + half), the other dims as they are
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int d = (e < 4 ? i4 : 60 + i4) + e;
-                if (d < p.half) x[e] = turn[0][d] * x[e] - turn[1][d] * src[d + p.half];
-                else if (d < 2 * p.half) x[e] = turn[1][d - p.half] * src[d - p.half] + turn[0][d - p.half] * x[e];
-            }
+        for (int e = 0; e < 8; e++) {
+            const int at = (e < 4 ? d : 60 + d) + e;
+            if (at < half) x[e] = turn[at].x * x[e] - turn[at].y * src[at + half];
+            else if (at < 2 * half) x[e] = turn[at - half].y * src[at - half] + turn[at - half].x * x[e];
         }
     }
-    if (!is_q) {
-        const int hk = is_k ? row - H : row - H - a.Hkv;
-        T* dst = reinterpret_cast<T*>(const_cast<void*>(is_k ? a.ok : a.ov)) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kS;
-        store_row4(dst + i4, x);
-        store_row4(dst + 64 + i4, x + 4);
-        return;
-    }
-    const int64_t m = (int64_t)(row / a.G) * a.M + (int64_t)bl * a.G + row % a.G;
+}
+// a rotated query as halves, dims in x's order, and its factor
+struct QueryRow {
+    uint4 hi, lo;
+    float c;
+};
+__device__ __forceinline__ QueryRow query_row(const float (&x)[8], bool live) {
     float top = 0.0f;
     bool fine = true;
 #pragma unroll
@@ -149,13 +130,47 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a, PrepArgs
         hi[e] = (_Float16)y;
         lo[e] = (_Float16)(y - (float)hi[e]);
     }
-    const uint4 h = *reinterpret_cast<const uint4*>(&hi), w = *reinterpret_cast<const uint4*>(&lo);
-    *reinterpret_cast<uint2*>(a.qh + m * kS + i4) = make_uint2(h.x, h.y);
-    *reinterpret_cast<uint2*>(a.qh + m * kS + 64 + i4) = make_uint2(h.z, h.w);
-    *reinterpret_cast<uint2*>(a.ql + m * kS + i4) = make_uint2(w.x, w.y);
-    *reinterpret_cast<uint2*>(a.ql + m * kS + 64 + i4) = make_uint2(w.z, w.w);
     // (a query that holds an infinity or NaN has no score that is a number)
-    if ((threadIdx.x & 15) == 0) a.cq[m] = live && bad != 0.0f ? NAN : ldexpf(1.44269504f * 0.08838834764831845f, -e2);
+    return {__builtin_bit_cast(uint4, hi), __builtin_bit_cast(uint4, lo), live && bad != 0.0f ? NAN : ldexpf(1.44269504f * 0.08838834764831845f, -e2)};
+}
+template <typename T>
+__device__ __forceinline__ void store_row(T* dst, int d, const float (&x)[8]) {
+    store_row4(dst + d, x);
+    store_row4(dst + 64 + d, x + 4);
+}
+
+// Where queries fill tiles of 64 or 128.  A workgroup per token and 16 of its H + 2*Hkv rows of 128.  Bound by latency at few tokens and by
+// memory at many.
+template <typename T>
+__global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a, PrepArgs p) {
+    __shared__ float2 turn[64];
+    const int bl = blockIdx.x / p.groups, group = blockIdx.x - bl * p.groups, b = bl / a.qL, l = bl - b * a.qL;
+    int len, n;
+    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    const bool live = l < n;
+    if (live && (int)threadIdx.x < p.half) turn_of(p.inv_freq[threadIdx.x], a.P + len + l, turn[threadIdx.x].x, turn[threadIdx.x].y);
+    __syncthreads();
+    const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), d = 4 * (threadIdx.x & 15);
+    if (row >= H + 2 * a.Hkv) return;
+    const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv;
+    if (!live && !is_q) return;
+    const float* src = is_q ? p.q + b * p.qsb + l * p.qsl + (int64_t)row * kS
+                            : is_k ? p.k + b * p.ksb + l * p.ksl + (int64_t)(row - H) * kS : p.v + b * p.vsb + l * p.vsl + (int64_t)(row - H - a.Hkv) * kS;
+    float x[8];
+    load_row(src, d, x);
+    if (live && (is_q || is_k)) turn_row(src, d, turn, p.half, x);
+    if (!is_q) {
+        const int hk = is_k ? row - H : row - H - a.Hkv;
+        store_row(reinterpret_cast<T*>(const_cast<void*>(is_k ? a.ok : a.ov)) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kS, d, x);
+        return;
+    }
+    const int64_t m = (int64_t)(row / a.G) * a.M + (int64_t)bl * a.G + row % a.G;
+    const QueryRow r = query_row(x, live);
+    *reinterpret_cast<uint2*>(a.qh + m * kS + d) = make_uint2(r.hi.x, r.hi.y);
+    *reinterpret_cast<uint2*>(a.qh + m * kS + 64 + d) = make_uint2(r.hi.z, r.hi.w);
+    *reinterpret_cast<uint2*>(a.ql + m * kS + d) = make_uint2(r.lo.x, r.lo.y);
+    *reinterpret_cast<uint2*>(a.ql + m * kS + 64 + d) = make_uint2(r.lo.z, r.lo.w);
+    if ((threadIdx.x & 15) == 0) a.cq[m] = r.c;
 }
 
 // ---- 2. a piece of the rows for a tile of queries ----
@@ -218,10 +233,11 @@ struct Queries {
     float c[RT], m[RT], l[RT];
     int see[RT];  // rows below this one are seen
     v4f o[RT][8];
-    __device__ __forceinline__ void start(const PrefixArgs& a, int hk, int m0, int m_end, int i) {
+    // cq: the factor of query m0
+    __device__ __forceinline__ void start(const float* cq, int m0, int m_end, int i) {
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            c[rt] = a.cq[(int64_t)hk * a.M + min(m0 + 16 * rt + i, m_end - 1)];
+            c[rt] = cq[min(16 * rt + i, m_end - 1 - m0)];
             m[rt] = -INFINITY;
             l[rt] = 0.0f;
 #pragma unroll
@@ -235,6 +251,10 @@ struct QueryOps;
 template <>
 struct QueryOps<1> {
     v8h h[4], l[4];
+    __device__ __forceinline__ void take(const uint4* lds, int lane) {
+#pragma unroll
+        for (int step = 0; step < 4; step++) h[step] = as_v8h(lds[step * 64 + lane]), l[step] = as_v8h(lds[(4 + step) * 64 + lane]);
+    }
     __device__ __forceinline__ void load(const PrefixArgs& a, uint4*, int hk, int m0, int m_end, int lane) {
         const int64_t at = ((int64_t)hk * a.M + min(m0 + (lane & 15), m_end - 1)) * kS + 8 * (lane >> 4);
 #pragma unroll
@@ -249,6 +269,7 @@ struct QueryOps<1> {
 template <>
 struct QueryOps<2> {
     const uint4* mine;
+    __device__ __forceinline__ void take(const uint4* lds, int lane) { mine = lds + lane; }
     __device__ __forceinline__ void load(const PrefixArgs& a, uint4* lds, int hk, int m0, int m_end, int lane) {
         const int wave = threadIdx.x >> 6;  // a step to a wave
 #pragma unroll
@@ -359,17 +380,26 @@ __device__ __forceinline__ int rows_seen(const PrefixArgs& a, int m, int b, int 
 
 // The same in full width, for rows that hold values outside the halves' range: the workgroup starts again, half a wave to a query and
 // four dims to a lane, only the rows that the query sees, in up to two runs (prefix, own).  Slow, and not met in a model's caches.
+// queries in LDS: hi of step 0..3, lo of step 0..3, of sixteen queries, 16 bytes to a lane; where (in halves) the hi of dims d .. of query 16*rt + i is
+__device__ __forceinline__ int held_at(int rt, int i, int d) { return ((rt * 8 + (d >> 5)) * 64 + ((d >> 3) & 3) * 16 + i) * 8 + (d & 7); }
+struct HeldQueries {  // in LDS: (16-byte pieces as the operands lie, factors), or null: in memory
+    const uint4* q;
+    const float* c;
+};
 template <typename T>
-__device__ __forceinline__ void full_width(const PrefixArgs& a, int hk, int m0, int m_end, Rows<T> K0, Rows<T> V0, int from0, Rows<T> K1, Rows<T> V1, int from1,
+__device__ __forceinline__ void full_width(const PrefixArgs& a, HeldQueries held, int hk, int m0, int m_end, Rows<T> K0, Rows<T> V0, int from0, Rows<T> K1, Rows<T> V1, int from1,
                                            bool own, int b, int len, int n, int piece) {
     const int d = 4 * (threadIdx.x & 31);
 #pragma unroll 1
     for (int m = m0 + (threadIdx.x >> 5); m < m_end; m += 8) {
-        const int64_t at = ((int64_t)hk * a.M + m) * kS + d;
+        const int64_t at = (int64_t)hk * a.M + m;
+        const int in = held_at((m - m0) >> 4, (m - m0) & 15, d);
+        const _Float16 *hi = held.q != nullptr ? reinterpret_cast<const _Float16*>(held.q) + in : a.qh + at * kS + d,
+                       *lo = held.q != nullptr ? reinterpret_cast<const _Float16*>(held.q + 4 * 64) + in : a.ql + at * kS + d;
         double q[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) q[e] = (double)(float)a.qh[at + e] + (double)(float)a.ql[at + e];
-        const double c = (double)a.cq[(int64_t)hk * a.M + m];
+        for (int e = 0; e < 4; e++) q[e] = (double)(float)hi[e] + (double)(float)lo[e];
+        const double c = (double)(held.q != nullptr ? held.c[m - m0] : a.cq[at]);
         const int see = own ? rows_seen(a, m, b, len, n) : 0;
         float top = -INFINITY, sum = 0.0f;
         float o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -432,7 +462,11 @@ struct MeetSmem {
     int range[4][2];
     union {
         float o[4][16][kMeetRow];
-        uint4 q[16 * 64];
+        struct {
+            uint4 q[16 * 64];
+            float c[32];
+            float2 turn[32][64];
+        } in;
     };
 };
 
@@ -526,9 +560,74 @@ struct RowRegs<__half> {
     }
 };
 
-template <typename T, int RT>
-__device__ __forceinline__ void few_queries(const PrefixArgs& a, Rows<T> K, Rows<T> V, int hk, int m0, int m_end, int r0, bool own, int b, int len,
-                                            int n, int piece, MeetSmem& sm) {
+// SELF: there is no launch before this one (prefix_prep_kernel).  A workgroup rotates its queries itself, and the rows that are new among a
+// sequence's own (they are in one workgroup's piece).  It pays where all workgroups are at work at once: two chats behind 130 rows 13.8 ->
+// 11.8 us a call; 32 sequences of 32 heads, whose 1152 workgroups take turns and rotate in each, 46.7 -> 48.7.
+// The queries of a workgroup, asked for; their tokens' angles
+template <int RT>
+struct OwnQueries {
+    float x[RT][8];
+    const float* src[RT];
+    bool live[RT];
+    int token[RT], first;
+    __device__ __forceinline__ void load(const PrefixArgs& a, const PrepArgs& p, int hk, int m0, int m_end, MeetSmem& sm) {
+        first = m0 / a.G;
+        const int last = (m_end - 1) / a.G;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const int m = min(m0 + 16 * rt + (int)(threadIdx.x >> 4), m_end - 1), bl = m / a.G, b = bl / a.qL, l = bl - b * a.qL;
+            int len, n;
+            own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+            live[rt] = l < n;
+            token[rt] = bl - first;
+            src[rt] = p.q + b * p.qsb + l * p.qsl + ((int64_t)hk * a.G + (m - bl * a.G)) * kS;
+            load_row(src[rt], 4 * (threadIdx.x & 15), x[rt]);
+        }
+        const int f = threadIdx.x & 63;
+        for (int bl = first + (int)(threadIdx.x >> 6); bl <= last; bl += 4) {
+            const int b = bl / a.qL, l = bl - b * a.qL;
+            int len, n;
+            own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+            if (l < n && f < p.half) turn_of(p.inv_freq[f], a.P + len + l, sm.in.turn[bl - first][f].x, sm.in.turn[bl - first][f].y);
+        }
+        __syncthreads();
+    }
+    // rotated, as operands
+    __device__ __forceinline__ void put(const PrepArgs& p, MeetSmem& sm) {
+        const int i = threadIdx.x >> 4, d = 4 * (threadIdx.x & 15);
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            if (live[rt]) turn_row(src[rt], d, sm.in.turn[token[rt]], p.half, x[rt]);
+            const QueryRow r = query_row(x[rt], live[rt]);
+            _Float16* hi = reinterpret_cast<_Float16*>(sm.in.q);
+            _Float16* lo = hi + 4 * 64 * 8;
+            *reinterpret_cast<uint2*>(hi + held_at(rt, i, d)) = make_uint2(r.hi.x, r.hi.y);
+            *reinterpret_cast<uint2*>(hi + held_at(rt, i, 64 + d)) = make_uint2(r.hi.z, r.hi.w);
+            *reinterpret_cast<uint2*>(lo + held_at(rt, i, d)) = make_uint2(r.lo.x, r.lo.y);
+            *reinterpret_cast<uint2*>(lo + held_at(rt, i, 64 + d)) = make_uint2(r.lo.z, r.lo.w);
+            if (d == 0) sm.in.c[16 * rt + i] = r.c;
+        }
+    }
+};
+// the new rows among a sequence's own from r0 on (K.end: their end), whose first new token is token `first` of the workgroup's
+template <typename T>
+__device__ __forceinline__ void new_rows(const PrefixArgs& a, const PrepArgs& p, Rows<T> K, Rows<T> V, int hk, int b, int len, int r0, const MeetSmem& sm) {
+    const int d = 4 * (threadIdx.x & 15);
+    for (int r = max(r0, len) + (int)(threadIdx.x >> 4); r < K.end; r += 16) {
+        const int l = r - len;
+        const float *k = p.k + b * p.ksb + l * p.ksl + (int64_t)hk * kS, *v = p.v + b * p.vsb + l * p.vsl + (int64_t)hk * kS;
+        float x[8], y[8];
+        load_row(k, d, x);
+        load_row(v, d, y);
+        turn_row(k, d, sm.in.turn[l], p.half, x);
+        store_row(const_cast<T*>(K.p) + (int64_t)r * kS, d, x);
+        store_row(const_cast<T*>(V.p) + (int64_t)r * kS, d, y);
+    }
+}
+
+template <typename T, int RT, bool SELF>
+__device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs& p, Rows<T> K, Rows<T> V, int hk, int m0, int m_end, int r0, bool own, int b,
+                                            int len, int n, int piece, MeetSmem& sm) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const int r1 = K.end;
     if (r0 >= r1) {
@@ -537,12 +636,25 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, Rows<T> K, Rows
     }
     RowRegs<T> x;
     int t = r0 + 32 * wave;
-    const bool any = t < r1;
-    if (any) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
     QueryOps<RT> q;
-    q.load(a, sm.q, hk, m0, m_end, lane);
     Queries<RT> s;
-    s.start(a, hk, m0, m_end, i);
+    if constexpr (SELF) {
+        m_end = min(m_end, m0 + 16 * RT);
+        OwnQueries<RT> mine;
+        mine.load(a, p, hk, m0, m_end, sm);
+        const bool late = own && t + 32 > len;  // (rows that are about to be written among them)
+        if (t < r1 && !late) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
+        mine.put(p, sm);
+        if (own) new_rows<T>(a, p, K, V, hk, b, len, r0, sm);
+        __syncthreads();
+        if (t < r1 && late) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
+        q.take(sm.in.q, lane);
+        s.start(sm.in.c, m0, m_end, i);
+    } else {
+        if (t < r1) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
+        q.load(a, sm.in.q, hk, m0, m_end, lane);
+        s.start(a.cq + (int64_t)hk * a.M + m0, m0, m_end, i);
+    }
     int see_min = INT_MAX;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
@@ -600,7 +712,7 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, Rows<T> K, Rows
     __syncthreads();
     const Rows<T> none{K.p, 0};
     if (needs_full_width(sm.range, K, V, r0, none, none, 0)) {
-        full_width<T>(a, hk, m0, min(m_end, m0 + 16 * RT), own ? none : K, own ? none : V, r0, own ? K : none, own ? V : none, r0, own, b, len, n, piece);
+        full_width<T>(a, SELF ? HeldQueries{sm.in.q, sm.in.c} : HeldQueries{nullptr, nullptr}, hk, m0, min(m_end, m0 + 16 * RT), own ? none : K, own ? none : V, r0, own ? K : none, own ? V : none, r0, own, b, len, n, piece);
         return;
     }
 #pragma unroll
@@ -740,7 +852,7 @@ __device__ __forceinline__ void many_queries(const PrefixArgs& a, int hk, int m0
     v8h qh[RT][4], ql[RT][4];
     Queries<RT> s;
     const int mw = m0 + 16 * RT * wave;
-    s.start(a, hk, mw, m_end, i);
+    s.start(a.cq + (int64_t)hk * a.M + mw, mw, m_end, i);
     int see[RT], see_min = INT_MAX;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
@@ -819,7 +931,7 @@ __device__ __forceinline__ void many_queries(const PrefixArgs& a, int hk, int m0
     const Rows<T> k0{K0.p, min(K0.end, 32 * min(j1, np))}, v0{V0.p, k0.end}, k1{K1.p, min(K1.end, 32 * (j1 - np))}, v1{V1.p, k1.end};
     const int from0 = 32 * j0, from1 = 32 * max(0, j0 - np);
     if (needs_full_width(sm.range, k0, v0, from0, k1, v1, from1)) {
-        full_width<T>(a, hk, m0, m_end, k0, v0, from0, k1, v1, from1, own, b, len, n, piece);
+        full_width<T>(a, HeldQueries{nullptr, nullptr}, hk, m0, m_end, k0, v0, from0, k1, v1, from1, own, b, len, n, piece);
         return;
     }
 #pragma unroll
@@ -853,8 +965,8 @@ __device__ __forceinline__ void item_of(unsigned at, unsigned groups, unsigned e
 
 // The prefix for the queries of all sequences, RTP times 16 of them (MANY: 64) to a workgroup, then every sequence's own rows for its
 // queries, RTO times 16
-template <typename T, int RTP, bool MANY, int RTO>
-__global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a) {
+template <typename T, int RTP, bool MANY, int RTO, bool SELF>
+__global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a, PrepArgs p) {
     __shared__ union {
         MeetSmem few;
         TileSmem<T> many;
@@ -872,7 +984,7 @@ __global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a) {
         } else {
             const int end = min(a.P, (piece + 1) * a.prows);
             const Rows<T> K{(const T*)a.pk + plane, end}, V{(const T*)a.pv + plane, end};
-            few_queries<T, RTP>(a, K, V, hk, tile * 16 * RTP, a.M, piece * a.prows, false, 0, 0, 0, piece, sm.few);
+            few_queries<T, RTP, SELF>(a, p, K, V, hk, tile * 16 * RTP, a.M, piece * a.prows, false, 0, 0, 0, piece, sm.few);
         }
     } else {
         int group, sub;  // (a group: a sequence's head)
@@ -887,7 +999,7 @@ __global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a) {
         const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kS;
         const int end = min(rows, (piece + 1) * step);
         const Rows<T> K{(const T*)a.ok + plane, end}, V{(const T*)a.ov + plane, end};
-        few_queries<T, RTO>(a, K, V, hk, m0, m_end, piece * step, true, b, len, n, a.ppieces + piece, sm.few);
+        few_queries<T, RTO, SELF>(a, p, K, V, hk, m0, m_end, piece * step, true, b, len, n, a.ppieces + piece, sm.few);
     }
 }
 
@@ -958,7 +1070,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
 }
 
 struct PrefixPlan {
-    bool sweep, many;  // one sweep for a sequence's tiles; the prefix by many_queries
+    bool sweep, many, self;  // one sweep for a sequence's tiles; the prefix by many_queries; workgroups rotate their queries themselves
     int rtp, rto, ptiles, ppieces, prows, otiles, opieces, ostep;
 };
 // pieces of `rows`: some `wanted` of them, none below `least` rows
@@ -998,6 +1110,7 @@ static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int
     }
     p.ostep = fill > 1 ? 128 : 1024;
     p.opieces = pieces_of(fill > 1 ? fill : (maxlen + 1023) / 1024, maxlen, p.ostep);
+    p.self = !p.many && pitems * p.ppieces + oitems * p.opieces <= 512;
     return p;
 }
 
@@ -1005,17 +1118,18 @@ static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 struct PrefixLayout {
     size_t qh, ql, cq, stat, rec, total;
 };
-static PrefixLayout layout_prefix(int64_t rows, int nrec) {
+static PrefixLayout layout_prefix(const PrefixPlan& plan, int64_t rows) {
     PrefixLayout w{};
+    const size_t nrec = plan.ppieces + plan.opieces, held = plan.self ? 0 : rows;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += align_up(bytes, 256);
         return here;
     };
-    w.qh = take((size_t)rows * kS * 2);
-    w.ql = take((size_t)rows * kS * 2);
-    w.cq = take((size_t)rows * 4);
+    w.qh = take(held * kS * 2);
+    w.ql = take(held * kS * 2);
+    w.cq = take(held * 4);
     w.stat = take((size_t)rows * nrec * 8);
     w.rec = take((size_t)rows * nrec * kS * 4);
     w.total = at;
@@ -1027,18 +1141,23 @@ static int prefix_launch(PrefixArgs a, PrepArgs p, const PrefixPlan& plan, hipSt
     const int64_t prep = (int64_t)a.B * a.qL * p.groups, items = (int64_t)a.pitems + (int64_t)a.B * a.Hkv * a.otiles * a.opieces,
                   merge = ((int64_t)a.Hkv * a.M + 7) / 8, most = (int64_t)1 << 24;  // (a launch has fewer than 2^32 threads)
     LLMOPS_REQUIRE(prep < most && items < most && merge < most);
-    prefix_prep_kernel<T><<<(unsigned)prep, 256, 0, st>>>(a, p);
+    if (!plan.self) prefix_prep_kernel<T><<<(unsigned)prep, 256, 0, st>>>(a, p);
     LLMOPS_LAUNCH_CHECK();
     const unsigned grid = (unsigned)items;
+#define LLMOPS_APART(RTP, MANY, RTO, SELF) prefix_apart_kernel<T, RTP, MANY, RTO, SELF><<<grid, 256, 0, st>>>(a, p)
     if (plan.sweep && plan.rto == 1) prefix_sweep_kernel<T, 1><<<grid, 256, 0, st>>>(a);
     else if (plan.sweep) prefix_sweep_kernel<T, 2><<<grid, 256, 0, st>>>(a);
-    else if (plan.many && plan.rtp == 1 && plan.rto == 1) prefix_apart_kernel<T, 1, true, 1><<<grid, 256, 0, st>>>(a);
-    else if (plan.many && plan.rtp == 1) prefix_apart_kernel<T, 1, true, 2><<<grid, 256, 0, st>>>(a);
-    else if (plan.many && plan.rto == 1) prefix_apart_kernel<T, 2, true, 1><<<grid, 256, 0, st>>>(a);
-    else if (plan.many) prefix_apart_kernel<T, 2, true, 2><<<grid, 256, 0, st>>>(a);
-    else if (plan.rtp == 1) prefix_apart_kernel<T, 1, false, 1><<<grid, 256, 0, st>>>(a);
-    else if (plan.rto == 1) prefix_apart_kernel<T, 2, false, 1><<<grid, 256, 0, st>>>(a);
-    else prefix_apart_kernel<T, 2, false, 2><<<grid, 256, 0, st>>>(a);
+    else if (plan.many && plan.rtp == 1 && plan.rto == 1) LLMOPS_APART(1, true, 1, false);
+    else if (plan.many && plan.rtp == 1) LLMOPS_APART(1, true, 2, false);
+    else if (plan.many && plan.rto == 1) LLMOPS_APART(2, true, 1, false);
+    else if (plan.many) LLMOPS_APART(2, true, 2, false);
+    else if (plan.rtp == 1 && plan.self) LLMOPS_APART(1, false, 1, true);
+    else if (plan.rtp == 1) LLMOPS_APART(1, false, 1, false);
+    else if (plan.rto == 1 && plan.self) LLMOPS_APART(2, false, 1, true);
+    else if (plan.rto == 1) LLMOPS_APART(2, false, 1, false);
+    else if (plan.self) LLMOPS_APART(2, false, 2, true);
+    else LLMOPS_APART(2, false, 2, false);
+#undef LLMOPS_APART
     LLMOPS_LAUNCH_CHECK();
     if (a.nrec > 1) prefix_merge_kernel<<<(unsigned)merge, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
@@ -1058,7 +1177,7 @@ static bool prefix_sizes_fit(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int6
 extern "C" size_t llmops_attention_prefix_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t prefix_len, int64_t maxlen) {
     if (S != kS || !prefix_sizes_fit(B, qL, H, Hkv, prefix_len, maxlen)) return 0;
     const PrefixPlan p = plan_prefix(B, qL, H, Hkv, prefix_len, maxlen);
-    return layout_prefix(B * qL * H, p.ppieces + p.opieces).total;
+    return layout_prefix(p, B * qL * H).total;
 }
 
 extern "C" int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b, int64_t k_stride_l,
@@ -1083,7 +1202,7 @@ extern "C" int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, 
                     o0 = reinterpret_cast<uintptr_t>(kv_cache), o1 = o0 + (size_t)planes * B * maxlen * row;
     LLMOPS_REQUIRE(prefix_len == 0 || p1 <= o0 || o1 <= p0);  // the caches do not overlap
     const PrefixPlan plan = plan_prefix(B, qL, H, Hkv, prefix_len, maxlen);
-    const PrefixLayout w = layout_prefix(B * qL * H, plan.ppieces + plan.opieces);
+    const PrefixLayout w = layout_prefix(plan, B * qL * H);
     if (workspace_bytes < w.total)
         return fail(LLMOPS_EWORKSPACE, "attention_rope_prefix needs %zu workspace bytes, got %zu", w.total, workspace_bytes);
     char* ws = reinterpret_cast<char*>(workspace);

@@ -269,7 +269,6 @@ struct QueryOps<1> {
 template <>
 struct QueryOps<2> {
     const uint4* mine;
-    __device__ __forceinline__ void take(const uint4* lds, int lane) { mine = lds + lane; }
     __device__ __forceinline__ void load(const PrefixArgs& a, uint4* lds, int hk, int m0, int m_end, int lane) {
         const int wave = threadIdx.x >> 6;  // a step to a wave
 #pragma unroll
@@ -380,8 +379,8 @@ __device__ __forceinline__ int rows_seen(const PrefixArgs& a, int m, int b, int 
 
 // The same in full width, for rows that hold values outside the halves' range: the workgroup starts again, half a wave to a query and
 // four dims to a lane, only the rows that the query sees, in up to two runs (prefix, own).  Slow, and not met in a model's caches.
-// queries in LDS: hi of step 0..3, lo of step 0..3, of sixteen queries, 16 bytes to a lane; where (in halves) the hi of dims d .. of query 16*rt + i is
-__device__ __forceinline__ int held_at(int rt, int i, int d) { return ((rt * 8 + (d >> 5)) * 64 + ((d >> 3) & 3) * 16 + i) * 8 + (d & 7); }
+// sixteen queries in LDS: hi of step 0..3, lo of step 0..3, 16 bytes to a lane; where (in halves) the hi of dims d .. of query i is
+__device__ __forceinline__ int held_at(int i, int d) { return ((d >> 5) * 64 + ((d >> 3) & 3) * 16 + i) * 8 + (d & 7); }
 struct HeldQueries {  // in LDS: (16-byte pieces as the operands lie, factors), or null: in memory
     const uint4* q;
     const float* c;
@@ -393,7 +392,7 @@ __device__ __forceinline__ void full_width(const PrefixArgs& a, HeldQueries held
 #pragma unroll 1
     for (int m = m0 + (threadIdx.x >> 5); m < m_end; m += 8) {
         const int64_t at = (int64_t)hk * a.M + m;
-        const int in = held_at((m - m0) >> 4, (m - m0) & 15, d);
+        const int in = held_at(m - m0, d);
         const _Float16 *hi = held.q != nullptr ? reinterpret_cast<const _Float16*>(held.q) + in : a.qh + at * kS + d,
                        *lo = held.q != nullptr ? reinterpret_cast<const _Float16*>(held.q + 4 * 64) + in : a.ql + at * kS + d;
         double q[4];
@@ -464,8 +463,8 @@ struct MeetSmem {
         float o[4][16][kMeetRow];
         struct {
             uint4 q[16 * 64];
-            float c[32];
-            float2 turn[32][64];
+            float c[16];
+            float2 turn[16][64];
         } in;
     };
 };
@@ -561,52 +560,42 @@ struct RowRegs<__half> {
 };
 
 // SELF: there is no launch before this one (prefix_prep_kernel).  A workgroup rotates its queries itself, and the rows that are new among a
-// sequence's own (they are in one workgroup's piece).  It pays where all workgroups are at work at once: two chats behind 130 rows 13.8 ->
-// 11.8 us a call; 32 sequences of 32 heads, whose 1152 workgroups take turns and rotate in each, 46.7 -> 48.7.
-// The queries of a workgroup, asked for; their tokens' angles
-template <int RT>
+// sequence's own (they are in one workgroup's piece).
+// The queries of a workgroup, sixteen at most, asked for; their tokens' angles
 struct OwnQueries {
-    float x[RT][8];
-    const float* src[RT];
-    bool live[RT];
-    int token[RT], first;
+    float x[8];
+    const float* src;
+    bool live;
+    int token;
     __device__ __forceinline__ void load(const PrefixArgs& a, const PrepArgs& p, int hk, int m0, int m_end, MeetSmem& sm) {
-        first = m0 / a.G;
-        const int last = (m_end - 1) / a.G;
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            const int m = min(m0 + 16 * rt + (int)(threadIdx.x >> 4), m_end - 1), bl = m / a.G, b = bl / a.qL, l = bl - b * a.qL;
-            int len, n;
-            own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-            live[rt] = l < n;
-            token[rt] = bl - first;
-            src[rt] = p.q + b * p.qsb + l * p.qsl + ((int64_t)hk * a.G + (m - bl * a.G)) * kS;
-            load_row(src[rt], 4 * (threadIdx.x & 15), x[rt]);
-        }
+        const int first = m0 / a.G, last = (m_end - 1) / a.G, m = min(m0 + (int)(threadIdx.x >> 4), m_end - 1), mine = m / a.G, b = mine / a.qL,
+                  l = mine - b * a.qL;
+        int len, n;
+        own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+        live = l < n;
+        token = mine - first;
+        src = p.q + b * p.qsb + l * p.qsl + ((int64_t)hk * a.G + (m - mine * a.G)) * kS;
+        load_row(src, 4 * (threadIdx.x & 15), x);
         const int f = threadIdx.x & 63;
         for (int bl = first + (int)(threadIdx.x >> 6); bl <= last; bl += 4) {
-            const int b = bl / a.qL, l = bl - b * a.qL;
-            int len, n;
-            own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-            if (l < n && f < p.half) turn_of(p.inv_freq[f], a.P + len + l, sm.in.turn[bl - first][f].x, sm.in.turn[bl - first][f].y);
+            const int c = bl / a.qL, lc = bl - c * a.qL;
+            own_extent(a.lengths, a.q_lens, c, a.qL, a.maxlen, len, n);
+            if (lc < n && f < p.half) turn_of(p.inv_freq[f], a.P + len + lc, sm.in.turn[bl - first][f].x, sm.in.turn[bl - first][f].y);
         }
         __syncthreads();
     }
     // rotated, as operands
     __device__ __forceinline__ void put(const PrepArgs& p, MeetSmem& sm) {
         const int i = threadIdx.x >> 4, d = 4 * (threadIdx.x & 15);
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            if (live[rt]) turn_row(src[rt], d, sm.in.turn[token[rt]], p.half, x[rt]);
-            const QueryRow r = query_row(x[rt], live[rt]);
-            _Float16* hi = reinterpret_cast<_Float16*>(sm.in.q);
-            _Float16* lo = hi + 4 * 64 * 8;
-            *reinterpret_cast<uint2*>(hi + held_at(rt, i, d)) = make_uint2(r.hi.x, r.hi.y);
-            *reinterpret_cast<uint2*>(hi + held_at(rt, i, 64 + d)) = make_uint2(r.hi.z, r.hi.w);
-            *reinterpret_cast<uint2*>(lo + held_at(rt, i, d)) = make_uint2(r.lo.x, r.lo.y);
-            *reinterpret_cast<uint2*>(lo + held_at(rt, i, 64 + d)) = make_uint2(r.lo.z, r.lo.w);
-            if (d == 0) sm.in.c[16 * rt + i] = r.c;
-        }
+        if (live) turn_row(src, d, sm.in.turn[token], p.half, x);
+        const QueryRow r = query_row(x, live);
+        _Float16* hi = reinterpret_cast<_Float16*>(sm.in.q);
+        _Float16* lo = hi + 4 * 64 * 8;
+        *reinterpret_cast<uint2*>(hi + held_at(i, d)) = make_uint2(r.hi.x, r.hi.y);
+        *reinterpret_cast<uint2*>(hi + held_at(i, 64 + d)) = make_uint2(r.hi.z, r.hi.w);
+        *reinterpret_cast<uint2*>(lo + held_at(i, d)) = make_uint2(r.lo.x, r.lo.y);
+        *reinterpret_cast<uint2*>(lo + held_at(i, 64 + d)) = make_uint2(r.lo.z, r.lo.w);
+        if (d == 0) sm.in.c[i] = r.c;
     }
 };
 // the new rows among a sequence's own from r0 on (K.end: their end), whose first new token is token `first` of the workgroup's
@@ -640,7 +629,8 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs&
     Queries<RT> s;
     if constexpr (SELF) {
         m_end = min(m_end, m0 + 16 * RT);
-        OwnQueries<RT> mine;
+        static_assert(RT == 1, "");
+        OwnQueries mine;
         mine.load(a, p, hk, m0, m_end, sm);
         const bool late = own && t + 32 > len;  // (rows that are about to be written among them)
         if (t < r1 && !late) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
@@ -964,8 +954,8 @@ __device__ __forceinline__ void item_of(unsigned at, unsigned groups, unsigned e
 }
 
 // The prefix for the queries of all sequences, RTP times 16 of them (MANY: 64) to a workgroup, then every sequence's own rows for its
-// queries, RTO times 16
-template <typename T, int RTP, bool MANY, int RTO, bool SELF>
+// queries, 16 to a workgroup
+template <typename T, int RTP, bool MANY, bool SELF>
 __global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a, PrepArgs p) {
     __shared__ union {
         MeetSmem few;
@@ -992,14 +982,14 @@ __global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a, Prep
         const int hk = group % a.Hkv, b = group / a.Hkv, tile = sub % a.otiles, piece = sub / a.otiles;
         int len, n;
         own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-        const int first = tile * 16 * RTO, m0 = b * a.Mq + first, m_end = (b + 1) * a.Mq;
+        const int first = tile * 16, m0 = b * a.Mq + first, m_end = (b + 1) * a.Mq;
         // rows that the tile's last live query sees, in pieces of whole 128
-        const int last = min(n, (first + 16 * RTO - 1) / a.G + 1), rows = first < n * a.G ? len + last : 0;
+        const int last = min(n, (first + 15) / a.G + 1), rows = first < n * a.G ? len + last : 0;
         const int step = max(a.ostep, (rows + 128 * a.opieces - 1) / (128 * a.opieces) * 128);
         const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kS;
         const int end = min(rows, (piece + 1) * step);
         const Rows<T> K{(const T*)a.ok + plane, end}, V{(const T*)a.ov + plane, end};
-        few_queries<T, RTO, SELF>(a, p, K, V, hk, m0, m_end, piece * step, true, b, len, n, a.ppieces + piece, sm.few);
+        few_queries<T, 1, SELF>(a, p, K, V, hk, m0, m_end, piece * step, true, b, len, n, a.ppieces + piece, sm.few);
     }
 }
 
@@ -1071,37 +1061,51 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
 
 struct PrefixPlan {
     bool sweep, many, self;  // one sweep for a sequence's tiles; the prefix by many_queries; workgroups rotate their queries themselves
-    int rtp, rto, ptiles, ppieces, prows, otiles, opieces, ostep;
+    int rt, ptiles, ppieces, prows, otiles, opieces, ostep;
 };
 // pieces of `rows`: some `wanted` of them, none below `least` rows
 static int pieces_of(int64_t wanted, int64_t rows, int64_t least) {
     const int64_t most = (rows + least - 1) / least, n = wanted < most ? wanted : most;
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
-static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t P, int64_t maxlen) {
+static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t P, int64_t maxlen, bool half, bool ragged) {
     PrefixPlan p{};
     const int64_t Mq = qL * (H / Hkv), M = B * Mq;
-    p.sweep = Mq >= 64;
+    // (All us a call, fp32 caches and then halves; 16 sequences of 32 heads behind 1500 rows, apart / sweep: 32 tokens 106 / 144, 77 / 92; 48 tokens
+    // 155 / 142, 110 / 93; 64 tokens 181 / 154, 131 / 102.)
+    p.sweep = Mq >= 48;
     if (p.sweep) {
-        // 64 queries to a workgroup until there are twice the workgroups that the chip holds of the other kind, 128 then (half the reading of
-        // cut rows per product); pieces where even that leaves the chip empty
-        p.rto = B * Hkv * ((Mq + 127) / 128) >= 1024 ? 2 : 1;
-        p.otiles = (int)((Mq + 64 * p.rto - 1) / (64 * p.rto));
+        // 64 queries to a workgroup, or 128, which read the cut rows half as often: where the tiles are as full and there are workgroups enough, which
+        // matters more for halves (nothing to cut).  64 / 128: 8 sequences of 256 tokens 222 / 187, 143 / 136; 4 of 300 170 / 160, 102 / 117; 4 of 160
+        // 100 / 100, 66 / 75; 2 of 128 with 4 heads to a kv head 44 / 48, 39 / 43.  4 of 150 to 300, the rest padding: 129 / 169, so 64 where lengths differ.
+        const int64_t t64 = (Mq + 63) / 64, t128 = (Mq + 127) / 128, items2 = B * Hkv * t128;
+        const bool two = !ragged && (half ? 20 * t64 >= 38 * t128 && items2 >= 512 : 100 * t64 > 164 * t128 && items2 >= 128);
+        p.rt = two ? 2 : 1;
+        p.otiles = (int)(two ? t128 : t64);
         const int64_t items = B * Hkv * p.otiles;
+        // (Pieces where that leaves the chip empty, until there are some 512 workgroups; until 256 / 512 / 1024: one sequence of 300 tokens 64 / 51 / 59.)
         p.opieces = pieces_of((512 + items / 2) / items, P + maxlen, 256);
         p.ostep = 1;
         return p;
     }
-    p.many = M > 32;
-    p.rtp = p.many ? (M > 64 ? 2 : 1) : M > 16 ? 2 : 1;
-    p.rto = Mq > 16 ? 2 : 1;
-    const int64_t tile = (p.many ? 64 : 16) * p.rtp;
+    const int64_t oitems = B * Hkv * ((Mq + 15) / 16);
+    // many_queries cuts a row up once for 64 queries, few_queries goes through a piece four times as fast.  (Few / many behind 2000 rows: 128 queries of
+    // each of 8 kv heads 30 / 37, 23 / 29; 256 of 8 45 / 41, 29 / 31; 48 of 32 39 / 42, 25 / 30; 128 of 32 64 / 53, 40 / 35.)
+    p.many = M > 32 && M * Hkv > 1536;
+    // many_queries with 128 queries as above, for fp32 rows and where they leave workgroups enough (64 / 128, 80 queries of 32 heads behind 2000 rows 107 / 102,
+    // halves 63 / 65; 256 of 8 41 / 52).
+    const bool wide = !half && 100 * ((M + 63) / 64) > 164 * ((M + 127) / 128) && Hkv * ((M + 127) / 128) * ((P + 511) / 512) >= 96;
+    // few_queries with 32 queries reads rows half as often, with 16 there are more workgroups.  (16 / 32 behind 2000 rows: 128 of 8 27 / 30, 23 / 24; 40 of 32
+    // 37 / 33, 26 / 24.)  Own rows always by 16: for 20 tokens of 8 sequences 32 took 67 instead of 67, 46 instead of 41.
+    p.rt = (p.many ? wide : M > 16 && Hkv * ((M + 31) / 32) * ((P + 511) / 512) + oitems >= 320) ? 2 : 1;
+    const int64_t tile = (p.many ? 64 : 16) * p.rt;
     p.ptiles = (int)((M + tile - 1) / tile);
-    p.otiles = (int)((Mq + 16 * p.rto - 1) / (16 * p.rto));
+    p.otiles = (int)((Mq + 15) / 16);
     // Pieces of 512 rows of the prefix and 1024 of the own rows, so that none is the last at work; smaller ones, down to 128, until there are
-    // the 512 workgroups that the chip holds.  (us, prefix in pieces of 2048 / 1024 / 512 / 256 / 128: 32 tokens behind 2048 halves - / 45.1 / 46.2 /
-    // 49.0 / 53.2; 64 grouped behind 4001 112 / 68.7 / 52.5 / 63.0 / 73.4; 80 behind 1500 - / 78.0 / 65.4 / 66.8 / 75.9.)
-    const int64_t pitems = Hkv * p.ptiles, oitems = B * Hkv * p.otiles, all = (P > 0 ? pitems : 0) + oitems;
+    // the 512 workgroups that the chip holds.  (Prefix in pieces of 256 / 512 / 1024 / 2048 rows: 64 sequences with 4 heads to a kv head behind 4001 rows
+    // 77 / 68 / 71 / 115, 49 / 39 / 50 / 78; 16 of 5 tokens behind 1500 70 / 62 / 64 / 94.  Own rows, some 3000, in pieces of 512 / 1024 / 2048: 32 sequences
+    // 289 / 296 / 344.)
+    const int64_t pitems = Hkv * p.ptiles, all = (P > 0 ? pitems : 0) + oitems;
     const int64_t fill = (512 + all - 1) / all;
     if (P > 0) {
         const int64_t large = (P + 511) / 512, n = pieces_of(fill > large ? fill : large, P, 128);
@@ -1110,7 +1114,10 @@ static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int
     }
     p.ostep = fill > 1 ? 128 : 1024;
     p.opieces = pieces_of(fill > 1 ? fill : (maxlen + 1023) / 1024, maxlen, p.ostep);
-    p.self = !p.many && pitems * p.ppieces + oitems * p.opieces <= 512;
+    // A launch less where the workgroups are at work at once and have sixteen queries.  (Two / one launch before the pieces are joined: 2 sequences behind
+    // 130 rows 13.2 / 11.8, 10.9 / 9.9; 8 behind 500 19.8 / 18.9, 15.5 / 14.3; 32 behind 2048, whose 1152 workgroups take turns and rotate in each,
+    // 46.7 / 48.7 for halves; 8 with 32 queries to a workgroup 24.3 / 26.1, 19.3 / 18.6.)
+    p.self = M <= 16 && pitems * p.ppieces + oitems * p.opieces <= 512;
     return p;
 }
 
@@ -1144,19 +1151,14 @@ static int prefix_launch(PrefixArgs a, PrepArgs p, const PrefixPlan& plan, hipSt
     if (!plan.self) prefix_prep_kernel<T><<<(unsigned)prep, 256, 0, st>>>(a, p);
     LLMOPS_LAUNCH_CHECK();
     const unsigned grid = (unsigned)items;
-#define LLMOPS_APART(RTP, MANY, RTO, SELF) prefix_apart_kernel<T, RTP, MANY, RTO, SELF><<<grid, 256, 0, st>>>(a, p)
-    if (plan.sweep && plan.rto == 1) prefix_sweep_kernel<T, 1><<<grid, 256, 0, st>>>(a);
+#define LLMOPS_APART(RTP, MANY, SELF) prefix_apart_kernel<T, RTP, MANY, SELF><<<grid, 256, 0, st>>>(a, p)
+    if (plan.sweep && plan.rt == 1) prefix_sweep_kernel<T, 1><<<grid, 256, 0, st>>>(a);
     else if (plan.sweep) prefix_sweep_kernel<T, 2><<<grid, 256, 0, st>>>(a);
-    else if (plan.many && plan.rtp == 1 && plan.rto == 1) LLMOPS_APART(1, true, 1, false);
-    else if (plan.many && plan.rtp == 1) LLMOPS_APART(1, true, 2, false);
-    else if (plan.many && plan.rto == 1) LLMOPS_APART(2, true, 1, false);
-    else if (plan.many) LLMOPS_APART(2, true, 2, false);
-    else if (plan.rtp == 1 && plan.self) LLMOPS_APART(1, false, 1, true);
-    else if (plan.rtp == 1) LLMOPS_APART(1, false, 1, false);
-    else if (plan.rto == 1 && plan.self) LLMOPS_APART(2, false, 1, true);
-    else if (plan.rto == 1) LLMOPS_APART(2, false, 1, false);
-    else if (plan.self) LLMOPS_APART(2, false, 2, true);
-    else LLMOPS_APART(2, false, 2, false);
+    else if (plan.many && plan.rt == 2) LLMOPS_APART(sizeof(T) == 4 ? 2 : 1, true, false);
+    else if (plan.many) LLMOPS_APART(1, true, false);
+    else if (plan.self) LLMOPS_APART(1, false, true);
+    else if (plan.rt == 1) LLMOPS_APART(1, false, false);
+    else LLMOPS_APART(2, false, false);
 #undef LLMOPS_APART
     LLMOPS_LAUNCH_CHECK();
     if (a.nrec > 1) prefix_merge_kernel<<<(unsigned)merge, 256, 0, st>>>(a);
@@ -1176,8 +1178,12 @@ static bool prefix_sizes_fit(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int6
 
 extern "C" size_t llmops_attention_prefix_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t prefix_len, int64_t maxlen) {
     if (S != kS || !prefix_sizes_fit(B, qL, H, Hkv, prefix_len, maxlen)) return 0;
-    const PrefixPlan p = plan_prefix(B, qL, H, Hkv, prefix_len, maxlen);
-    return layout_prefix(p, B * qL * H).total;
+    size_t most = 0;
+    for (int kind = 0; kind < 4; kind++) {
+        const size_t need = layout_prefix(plan_prefix(B, qL, H, Hkv, prefix_len, maxlen, kind & 1, kind & 2), B * qL * H).total;
+        most = need > most ? need : most;
+    }
+    return most;
 }
 
 extern "C" int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b, int64_t k_stride_l,
@@ -1201,10 +1207,10 @@ extern "C" int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, 
     const uintptr_t p0 = reinterpret_cast<uintptr_t>(prefix_cache), p1 = p0 + (size_t)prefix_planes * prefix_maxlen * row,
                     o0 = reinterpret_cast<uintptr_t>(kv_cache), o1 = o0 + (size_t)planes * B * maxlen * row;
     LLMOPS_REQUIRE(prefix_len == 0 || p1 <= o0 || o1 <= p0);  // the caches do not overlap
-    const PrefixPlan plan = plan_prefix(B, qL, H, Hkv, prefix_len, maxlen);
+    const PrefixPlan plan = plan_prefix(B, qL, H, Hkv, prefix_len, maxlen, cache_dtype == LLMOPS_CACHE_F16, q_lens != nullptr);
     const PrefixLayout w = layout_prefix(plan, B * qL * H);
-    if (workspace_bytes < w.total)
-        return fail(LLMOPS_EWORKSPACE, "attention_rope_prefix needs %zu workspace bytes, got %zu", w.total, workspace_bytes);
+    const size_t need = llmops_attention_prefix_workspace_bytes(B, qL, H, Hkv, S, prefix_len, maxlen);
+    if (workspace_bytes < need) return fail(LLMOPS_EWORKSPACE, "attention_rope_prefix needs %zu workspace bytes, got %zu", need, workspace_bytes);
     char* ws = reinterpret_cast<char*>(workspace);
     PrefixArgs a{};
     a.qh = reinterpret_cast<_Float16*>(ws + w.qh), a.ql = reinterpret_cast<_Float16*>(ws + w.ql), a.cq = reinterpret_cast<float*>(ws + w.cq);

@@ -500,18 +500,18 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
     }
 }
 
-// Tokens to a tile: 32 where there are enough of them to fill the chip so
-static int lora_tile(int64_t rows) { return rows > 256 ? 32 : 16; }
+// Tokens to a tile: 32 where there are enough of them to fill the chip so.  (us a call, 16 / 32, fp16 and then fp32 weights: 320 tokens 15.4 / 19.2, 22.0 / 21.0;
+// 384 16.0 / 15.6, 20.3 / 16.2; 512 of rank 64 31 / 23, 42 / 24.)
+static int lora_tile(int64_t rows) { return rows > 320 ? 32 : 16; }
 static int64_t lora_tiles(int64_t batch, int64_t tokens) {
     const int64_t tile = lora_tile(batch * tokens);
     return tokens >= tile ? batch * ((tokens + tile - 1) / tile) : (batch * tokens + tile - 1) / tile;
 }
-// K in runs, until there are some 256 workgroups.  A run is at least 1024 (two stages of two steps to a wave) where tiles have one
-// adapter; the weights of several fill the wait of one step.
-static int lora_chunk(int64_t batch, int64_t tokens, int64_t K, int64_t R, int64_t adapters) {
-    const int64_t tile = lora_tile(batch * tokens), groups = lora_tiles(batch, tokens) * ((R + 63) / 64);
-    const int64_t least = tokens >= tile || batch == 1 || adapters == 1 ? 1024 : 256, n = (256 + groups - 1) / groups;
-    return (int)((K + least * n - 1) / (least * n) * least);
+// K in runs of whole steps, until there are some 256 workgroups.  (128 / 256 / 512 of them: 4 x 300 tokens, 11008 -> 4096, rank 64 58 / 52 / 56; runs of at
+// least 256 / 1024, 4 x 16 tokens, 4096 -> 4096, rank 16 7.8 / 10.5: a step waits once, however few there are.)
+static int lora_chunk(int64_t batch, int64_t tokens, int64_t K, int64_t R) {
+    const int64_t groups = lora_tiles(batch, tokens) * ((R + 63) / 64), step = 32 * kDownWaves, n = step * ((256 + groups - 1) / groups);
+    return (int)((K + n - 1) / n * step);
 }
 
 template <typename W>
@@ -532,7 +532,8 @@ static int lora_launch(LoraArgs a, bool vec_out, hipStream_t st) {
     else LLMOPS_DOWN(4, 2);
 #undef LLMOPS_DOWN
     LLMOPS_LAUNCH_CHECK();
-    // few tokens: 64 columns to a workgroup, so that there are enough of them, and the weights of eight adapters on their way
+    // few tokens: 64 columns to a workgroup, so that there are enough of them, and the weights of eight adapters on their way; many: 256, so that a
+    // token's sums are read by fewer
     const int ct = tt == 1 ? 1 : 4;
     const dim3 up((unsigned)((a.N + 64 * ct - 1) / (64 * ct)), tiles);
     if (tt == 1 && a.R < 8) lora_up_kernel<W, 1, 1, true><<<up, 256, 0, st>>>(a, vec_out);
@@ -555,7 +556,7 @@ static bool lora_sizes_fit(int64_t batch, int64_t tokens, int64_t N, int64_t K, 
 
 extern "C" size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R, int64_t adapters) {
     if (!lora_sizes_fit(batch, tokens, N, K, R) || adapters <= 0) return 0;
-    const int64_t chunk = lora_chunk(batch, tokens, K, R, adapters);
+    const int64_t chunk = lora_chunk(batch, tokens, K, R);
     return (size_t)((K + chunk - 1) / chunk) * (size_t)(batch * tokens) * (size_t)rank_stride((int)R) * sizeof(float);
 }
 
@@ -577,7 +578,7 @@ extern "C" int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_str
     a.x = x, a.y = y, a.scales = scales, a.A = lora_A, a.B = lora_B, a.ids = ids, a.out = out, a.part = reinterpret_cast<float*>(workspace);
     a.xsb = x_stride_b, a.xsl = x_stride_l, a.ysb = y_stride_b, a.ysl = y_stride_l, a.osb = out_stride_b, a.osl = out_stride_l;
     a.rows = (int)(batch * tokens), a.tokens = (int)tokens, a.K = (int)K, a.N = (int)N, a.R = (int)R, a.adapters = (int)adapters;
-    a.chunk = lora_chunk(batch, tokens, K, R, adapters);
+    a.chunk = lora_chunk(batch, tokens, K, R);
     a.splits = (int)((K + a.chunk - 1) / a.chunk);
     const bool vec_out = N % 4 == 0 && aligned(y, 16) && aligned(out, 16) && y_stride_b % 4 == 0 && y_stride_l % 4 == 0 && out_stride_b % 4 == 0 && out_stride_l % 4 == 0;
     hipStream_t st = as_stream(stream);

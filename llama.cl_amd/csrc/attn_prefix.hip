@@ -8,7 +8,8 @@
 //
 //   1. prefix_prep_kernel   rotates, writes the new cache rows and leaves q' as operands of the matrix instructions (part of 2 where that is one round)
 //   2. prefix_apart_kernel  softmax(q'K^T)V of a piece of the rows for a tile of queries: running maximum and sum, one pass; the prefix
-//      prefix_sweep_kernel  and the own rows apart, or in one sweep where a sequence has queries to fill tiles of its own
+//      prefix_sweep_kernel  and the own rows apart, or in one sweep where a sequence has queries to fill tiles of its own, or where
+//      prefix_brief_kernel  there are few rows
 //   3. prefix_merge_kernel  joins the pieces of a query, where there are several
 //
 // Queries of a kv head are numbered m = (b*qL + l)*G + g, so that the queries that see the prefix, those of all sequences, and
@@ -614,47 +615,52 @@ __device__ __forceinline__ void new_rows(const PrefixArgs& a, const PrepArgs& p,
     }
 }
 
+// Tiles of 32 rows j0 .. j1-1: those below np are the prefix's (K0, V0), the others the sequence's own.
 template <typename T, int RT, bool SELF>
-__device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs& p, Rows<T> K, Rows<T> V, int hk, int m0, int m_end, int r0, bool own, int b,
-                                            int len, int n, int piece, MeetSmem& sm) {
+__device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs& p, int hk, int m0, int m_end, Rows<T> K0, Rows<T> V0, Rows<T> K1, Rows<T> V1,
+                                            int np, int j0, int j1, bool own, int b, int len, int n, int piece, MeetSmem& sm) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-    const int r1 = K.end;
-    if (r0 >= r1) {
-        nothing(a, hk, m0, min(m_end, m0 + 16 * RT), piece);
+    m_end = min(m_end, m0 + 16 * RT);
+    if (j0 >= j1) {
+        nothing(a, hk, m0, m_end, piece);
         return;
     }
     RowRegs<T> x;
-    int t = r0 + 32 * wave;
+    auto load_k = [&](int j) { x.load_k(j >= np ? K1 : K0, 32 * (j >= np ? j - np : j), i, g); };
+    auto load_v = [&](int j) { x.load_v(j >= np ? V1 : V0, 32 * (j >= np ? j - np : j), i, g); };
+    int j = j0 + wave;
     QueryOps<RT> q;
     Queries<RT> s;
     if constexpr (SELF) {
-        m_end = min(m_end, m0 + 16 * RT);
         static_assert(RT == 1, "");
         OwnQueries mine;
         mine.load(a, p, hk, m0, m_end, sm);
-        const bool late = own && t + 32 > len;  // (rows that are about to be written among them)
-        if (t < r1 && !late) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
+        const bool late = own && 32 * (j - np + 1) > len;  // (rows that are about to be written among them)
+        if (j < j1 && !late) load_k(j), load_v(j);
         mine.put(p, sm);
-        if (own) new_rows<T>(a, p, K, V, hk, b, len, r0, sm);
+        if (own) new_rows<T>(a, p, K1, V1, hk, b, len, 32 * max(0, j0 - np), sm);
         __syncthreads();
-        if (t < r1 && late) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
+        if (j < j1 && late) load_k(j), load_v(j);
         q.take(sm.in.q, lane);
         s.start(sm.in.c, m0, m_end, i);
     } else {
-        if (t < r1) x.load_k(K, t, i, g), x.load_v(V, t, i, g);
+        if (j < j1) load_k(j), load_v(j);
         q.load(a, sm.in.q, hk, m0, m_end, lane);
         s.start(a.cq + (int64_t)hk * a.M + m0, m0, m_end, i);
     }
-    int see_min = INT_MAX;
+    int see[RT], see_min = INT_MAX;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const int m = min(m0 + 16 * rt + i, m_end - 1);
-        s.see[rt] = own ? min(r1, rows_seen(a, m, b, len, n)) : r1;
-        see_min = min(see_min, s.see[rt]);
+        see[rt] = own ? min(K1.end, rows_seen(a, min(m0 + 16 * rt + i, m_end - 1), b, len, n)) : 0;
+        see_min = min(see_min, see[rt]);
     }
     v2us ktop = {0, 0}, vtop = {0, 0};
-    for (; t < r1; t += 128) {
-        const bool masked = __any(t + 32 > see_min);
+    for (; j < j1; j += 4) {
+        const bool mine = j >= np;
+        const int t = 32 * (mine ? j - np : j);
+        const bool masked = __any(t + 32 > (mine ? see_min : K0.end));
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) s.see[rt] = mine ? see[rt] : K0.end;
         v4f sc[RT][2], low[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = low[rt][0] = low[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -675,7 +681,7 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs&
                 for (int tt = 0; tt < 2; tt++)
 #pragma unroll
                     for (int v = 0; v < 4; v++) sc[rt][tt][v] = fmaf(low[rt][tt][v], 1.0f / 2048.0f, sc[rt][tt][v]);
-        if (t + 128 < r1) x.load_k(K, t + 128, i, g);
+        if (j + 4 < j1) load_k(j + 4);
         Weights w[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
@@ -689,7 +695,7 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs&
             for (int rt = 0; rt < RT; rt++) s.o[rt][c] = add_rows<T>(s.o[rt][c], h, w[rt]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (t + 128 < r1) x.load_v(V, t + 128, i, g);
+        if (j + 4 < j1) load_v(j + 4);
     }
     // the four waves' sums
 #pragma unroll
@@ -700,9 +706,10 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs&
     }
     note_range<T>(ktop, vtop, sm.range[wave], lane);
     __syncthreads();
-    const Rows<T> none{K.p, 0};
-    if (needs_full_width(sm.range, K, V, r0, none, none, 0)) {
-        full_width<T>(a, SELF ? HeldQueries{sm.in.q, sm.in.c} : HeldQueries{nullptr, nullptr}, hk, m0, min(m_end, m0 + 16 * RT), own ? none : K, own ? none : V, r0, own ? K : none, own ? V : none, r0, own, b, len, n, piece);
+    const Rows<T> k0{K0.p, min(K0.end, 32 * min(j1, np))}, v0{V0.p, k0.end}, k1{K1.p, K1.end}, v1{V1.p, K1.end};
+    const int from0 = 32 * j0, from1 = 32 * max(0, j0 - np);
+    if (needs_full_width(sm.range, k0, v0, from0, k1, v1, from1)) {
+        full_width<T>(a, SELF ? HeldQueries{sm.in.q, sm.in.c} : HeldQueries{nullptr, nullptr}, hk, m0, m_end, k0, v0, from0, k1, v1, from1, own, b, len, n, piece);
         return;
     }
 #pragma unroll
@@ -724,7 +731,7 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs&
                 const float mw = sm.m[w][16 * rt + i];
                 L += sm.l[w][16 * rt + i] * (mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
             }
-            sm.sum[i] = s.see[rt] > 0 ? L : -1.0f;
+            sm.sum[i] = !own || see[rt] > 0 ? L : -1.0f;
             if (m0 + 16 * rt + i < m_end) leave_stat(a, hk, m0 + 16 * rt + i, piece, M, L);
         }
         __syncthreads();
@@ -972,9 +979,10 @@ __global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a, Prep
             many_queries<T, RTP>(a, hk, tile * 64 * RTP, a.M, K, V, none, none, tiles, piece * (a.prows / 32), min(tiles, (piece + 1) * (a.prows / 32)), false, 0,
                                  0, 0, piece, sm.many);
         } else {
-            const int end = min(a.P, (piece + 1) * a.prows);
-            const Rows<T> K{(const T*)a.pk + plane, end}, V{(const T*)a.pv + plane, end};
-            few_queries<T, RTP, SELF>(a, p, K, V, hk, tile * 16 * RTP, a.M, piece * a.prows, false, 0, 0, 0, piece, sm.few);
+            const Rows<T> K{(const T*)a.pk + plane, a.P}, V{(const T*)a.pv + plane, a.P}, none{(const T*)a.pk, 0};
+            const int tiles = (a.P + 31) / 32;
+            few_queries<T, RTP, SELF>(a, p, hk, tile * 16 * RTP, a.M, K, V, none, none, tiles, piece * (a.prows / 32), min(tiles, (piece + 1) * (a.prows / 32)), false,
+                                      0, 0, 0, piece, sm.few);
         }
     } else {
         int group, sub;  // (a group: a sequence's head)
@@ -988,9 +996,22 @@ __global__ __launch_bounds__(256, 2) void prefix_apart_kernel(PrefixArgs a, Prep
         const int step = max(a.ostep, (rows + 128 * a.opieces - 1) / (128 * a.opieces) * 128);
         const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kS;
         const int end = min(rows, (piece + 1) * step);
-        const Rows<T> K{(const T*)a.ok + plane, end}, V{(const T*)a.ov + plane, end};
-        few_queries<T, 1, SELF>(a, p, K, V, hk, m0, m_end, piece * step, true, b, len, n, a.ppieces + piece, sm.few);
+        const Rows<T> none{(const T*)a.ok, 0}, K{(const T*)a.ok + plane, end}, V{(const T*)a.ov + plane, end};
+        few_queries<T, 1, SELF>(a, p, hk, m0, m_end, none, none, K, V, 0, piece * (step / 32), (end + 31) / 32, true, b, len, n, a.ppieces + piece, sm.few);
     }
+}
+
+// Few rows: the prefix and the sequence's own in one go, sixteen queries of a sequence to a workgroup
+template <typename T>
+__global__ __launch_bounds__(256, 2) void prefix_brief_kernel(PrefixArgs a, PrepArgs p) {
+    __shared__ MeetSmem sm;
+    const int hk = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv;
+    int len, n;
+    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    const int rows = n > 0 ? len + n : 0, np = (a.P + 31) / 32, tiles = rows > 0 ? np + (rows + 31) / 32 : 0;
+    const int64_t pplane = (int64_t)hk * a.pmax * kS, oplane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kS;
+    const Rows<T> K0{(const T*)a.pk + pplane, a.P}, V0{(const T*)a.pv + pplane, a.P}, K1{(const T*)a.ok + oplane, rows}, V1{(const T*)a.ov + oplane, rows};
+    few_queries<T, 1, true>(a, p, hk, b * a.Mq, (b + 1) * a.Mq, K0, V0, K1, V1, np, 0, tiles, true, b, len, n, 0, sm);
 }
 
 // The prefix and the sequence's own rows in one sweep, or in pieces of it, for 64 * RT of a sequence's queries to a workgroup
@@ -1060,7 +1081,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
 }
 
 struct PrefixPlan {
-    bool sweep, many, self;  // one sweep for a sequence's tiles; the prefix by many_queries; workgroups rotate their queries themselves
+    bool brief, sweep, many, self;  // one sweep for a sequence's tiles; the prefix by many_queries; workgroups rotate their queries themselves
     int rt, ptiles, ppieces, prows, otiles, opieces, ostep;
 };
 // pieces of `rows`: some `wanted` of them, none below `least` rows
@@ -1071,8 +1092,17 @@ static int pieces_of(int64_t wanted, int64_t rows, int64_t least) {
 static PrefixPlan plan_prefix(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t P, int64_t maxlen, bool half, bool ragged) {
     PrefixPlan p{};
     const int64_t Mq = qL * (H / Hkv), M = B * Mq;
-    // (All us a call, fp32 caches and then halves; 16 sequences of 32 heads behind 1500 rows, apart / sweep: 32 tokens 106 / 144, 77 / 92; 48 tokens
+    // (16 sequences of 32 heads behind 1500 rows, apart / sweep: 32 tokens 106 / 144, 77 / 92; 48 tokens
     // 155 / 142, 110 / 93; 64 tokens 181 / 154, 131 / 102.)
+    // (All figures: us a call, fp32 caches and then halves.)  Few rows: one workgroup goes through all of a sequence's, 128 at a time, 2 us each time of
+    // fp32 and 1 of halves, and nothing is to be joined.  In pieces / in one go, 32 heads: 1 sequence behind 20 rows, 30 of its own 10.4 / 7.5, 9.6 / 6.7;
+    // 8 behind 130, 64 14.8 / 12.8, 11.8 / 8.8; 16 behind 200, 64 18.3 / 20.5, 15.6 / 13.4; 1 behind 400, 100 12.4 / 18.6, 10.3 / 11.3.
+    p.brief = Mq <= 16 && P + maxlen <= (half ? 384 : 128) && B * Hkv <= 512;
+    if (p.brief) {
+        p.self = true;
+        p.otiles = p.opieces = p.ostep = 1;
+        return p;
+    }
     p.sweep = Mq >= 48;
     if (p.sweep) {
         // 64 queries to a workgroup, or 128, which read the cut rows half as often: where the tiles are as full and there are workgroups enough, which
@@ -1152,7 +1182,8 @@ static int prefix_launch(PrefixArgs a, PrepArgs p, const PrefixPlan& plan, hipSt
     LLMOPS_LAUNCH_CHECK();
     const unsigned grid = (unsigned)items;
 #define LLMOPS_APART(RTP, MANY, SELF) prefix_apart_kernel<T, RTP, MANY, SELF><<<grid, 256, 0, st>>>(a, p)
-    if (plan.sweep && plan.rt == 1) prefix_sweep_kernel<T, 1><<<grid, 256, 0, st>>>(a);
+    if (plan.brief) prefix_brief_kernel<T><<<grid, 256, 0, st>>>(a, p);
+    else if (plan.sweep && plan.rt == 1) prefix_sweep_kernel<T, 1><<<grid, 256, 0, st>>>(a);
     else if (plan.sweep) prefix_sweep_kernel<T, 2><<<grid, 256, 0, st>>>(a);
     else if (plan.many && plan.rt == 2) LLMOPS_APART(sizeof(T) == 4 ? 2 : 1, true, false);
     else if (plan.many) LLMOPS_APART(1, true, false);

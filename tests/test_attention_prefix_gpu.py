@@ -331,3 +331,29 @@ def test_offsets_past_32_bits():
     err = (out[B - 1] - one[0]).double()  # (each is off by REL at most)
     assert err.norm() <= 2 * REL * one.double().norm() and err.abs().max() <= 2 * MAX * one.abs().max()
     assert out.isfinite().all()
+
+
+# one for each way that the work is cut up: all rows in one go; pieces, in one launch and in two; 32 queries to a workgroup; rows cut up for 64 and
+# for 128 queries; a sequence's 64 and 128 queries in one sweep
+KINDS = [(9, 2, 4, 2, 60, 40), (3, 2, 4, 2, 600, 40), (16, 1, 32, 32, 600, 9), (20, 1, 16, 16, 400, 9), (50, 2, 32, 8, 300, 9), (70, 1, 32, 32, 1100, 9),
+         (3, 50, 2, 2, 100, 60), (64, 70, 8, 8, 70, 80)]
+
+
+@pytest.mark.parametrize("half_cache", [False, True])
+@pytest.mark.parametrize("B,L,H,Hkv,P,maxlen", KINDS)
+def test_every_way_of_cutting_up(B, L, H, Hkv, P, maxlen, half_cache):
+    qkv, prefix, cache, lengths, _ = _case(B, L, H, Hkv, P, maxlen, half_cache, seed=21)
+    out, _ = _check(qkv, H, Hkv, prefix, P, cache, lengths, None)
+    # what is behind the prefix and behind a sequence's rows has no effect, bit for bit
+    pre, own = prefix.clone(), cache.clone()
+    pre[:, :, :, P:] = math.nan
+    for b in range(B):
+        own[:, b, :, int(lengths[b]) + L:] = math.nan
+    got, _ = _call(qkv, H, Hkv, _inv_freq(), pre, P, own, lengths, None)
+    assert torch.equal(got.cpu(), out)
+    # values that the halves do not hold, and then padding
+    big = qkv.clone()
+    big[..., H * S:] *= 1e5 if not half_cache else 1.0
+    big[..., (H + Hkv) * S:] *= 1e2
+    big[..., :H * S] *= 1e-5 if not half_cache else 1.0
+    _check(big, H, Hkv, prefix, P, cache, lengths, (torch.arange(B) % (L + 1)).to(torch.int32))

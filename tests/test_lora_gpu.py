@@ -56,6 +56,15 @@ def test_against_64_bits(B, M, N, K, R, n, dtype):
     _check(_run(case), case[0], _delta(*case[1:]))
 
 
+# 32 tokens to a tile: tiles of one sequence and of several, ranks past 128, rows and ranks shorter than eight, sizes that fill nothing
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("B,M,N,K,R,n", [(4, 100, 260, 520, 16, 3), (350, 1, 130, 264, 16, 5), (2, 200, 1030, 96, 64, 2), (5, 70, 77, 4, 3, 2), (1, 330, 100, 2049, 140, 1),
+                                         (66, 5, 640, 1000, 40, 7), (11, 33, 65, 31, 5, 4)])
+def test_many_tokens(B, M, N, K, R, n, dtype):
+    case = _case(B, M, N, K, R, n, dtype, seed=B + 10 * M)
+    _check(_run(case), case[0], _delta(*case[1:]))
+
+
 @pytest.mark.parametrize("ids", [[-1] * 6, [0] * 6, [2, 1, 0, 2, 1, 0], [-1, 3, 2, 99, -7, 0]])
 def test_which_adapter(ids):
     case = _case(6, 5, 200, 320, 16, 3, "fp16", seed=1, ids=ids)

@@ -11,6 +11,8 @@
 // Products run on the bf16 matrix cores (v_mfma_f32_16x16x32_bf16, fp32 sums) on exact pieces: an fp32 value is three bf16 values
 // (8 bits each, cut off), an fp16 weight two, a bf16 weight itself.  Products of pieces whose places sum to three or less are
 // formed; what is dropped is below 2^-22 of a product.
+#include <algorithm>
+
 #include "common.h"
 
 namespace llmops {
@@ -25,6 +27,7 @@ struct LoraArgs {
     float *out, *part;   // part [splits][rows][rank_stride(R)]
     int64_t xsb, xsl, ysb, ysl, osb, osl;
     int rows, tokens, K, N, R, adapters, splits, chunk;
+    int share;  // workgroups among which the adapters of a tile are dealt out, by number
     int tiles;  // of a sequence; 0: tiles go on over the sequences' ends
 };
 
@@ -195,8 +198,9 @@ struct Adapters {
     }
 };
 
-// A workgroup: 16 * TT tokens, a run of K (its eight waves an eighth of every 256 each), 16 * NR rows of A.  Bound by latency with few
-// tokens, by reading x with many; so the operands of two steps are asked for before those of the two before them are used, or those
+// A workgroup: 16 * TT tokens (of several adapters: those whose number is its own among `share`), a run of K (its eight waves an eighth of
+// every 256 each), 16 * NR rows of A.  Bound by latency with few tokens (1 x 4096, rank 8: 2.8 us) and by issuing instructions with many, those
+// that cut x and A up most of all (4 x 300 x 11008, rank 64, of which three quarters have an adapter: 29 us, 1.9 TB/s); so the operands of two steps are asked for before those of the two before them are used, or those
 // of four adapters at a time.
 // A operand: row of A lane % 16, eight k; B operand: token lane % 16, the same k; result: token lane % 16, rows 4 * (lane / 16) + v.
 template <typename W, int NR, int TT, bool SHORT>
@@ -206,9 +210,10 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) 
     __shared__ v4f meet[kDownWaves][NR * TT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const Tile tile(a, blockIdx.x, 16 * TT);
-    const int row0 = tile.first, r0 = blockIdx.z * 16 * NR;
+    const int row0 = tile.first, r0 = blockIdx.z / a.share * 16 * NR, part = blockIdx.z % a.share;
     const int k0 = blockIdx.y * a.chunk, k1 = min(a.K, k0 + a.chunk);
-    const int of_lane = adapter_of(a, row0 + (lane & (16 * TT - 1)), tile.end);
+    int of_lane = adapter_of(a, row0 + (lane & (16 * TT - 1)), tile.end);
+    if (of_lane % a.share != part) of_lane = -1;
     const float* x[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; tt++) {
@@ -342,13 +347,15 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) 
         v4f s = meet[0][m][lane];
 #pragma unroll
         for (int w = 1; w < kDownWaves; w++) s += meet[w][m][lane];
-        if (row >= tile.end) continue;
+        const bool mine = __shfl(of_lane, row - row0, 64) >= 0;
+        if (!mine) continue;
         const int stride = rank_stride(a.R);  // (behind the last rank stands that one again, which nobody takes)
         if (r < stride) *reinterpret_cast<Four32*>(a.part + ((int64_t)blockIdx.y * a.rows + row) * stride + r) = Four32{{s[0], s[1], s[2], s[3]}};
     }
 }
 
-// A workgroup: 16 * TT tokens, 64 * CT columns (16 * CT to a wave), ranks 128 at a time.  Bound by latency: what does not depend on
+// A workgroup: 16 * TT tokens (as above; those without an adapter with part 0), 64 * CT columns (16 * CT to a wave), ranks 128 at a time.  Bound by
+// latency (one token, 4096 columns: 4.5 us; 4 x 300, rank 64: 25 us, 1.6 TB/s, 12 of it until the sums are there): what does not depend on
 // anything (adapters, y, the first partial sums) is asked for at once, and the first weights before the sums are used.
 // A operand: column lane % 16 of B, eight ranks; B operand: token lane % 16, the same ranks; result: token lane % 16, columns 4 * (lane / 16) + v.
 template <typename W, int CT, int TT, bool SHORT>
@@ -359,7 +366,9 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const Tile tile(a, blockIdx.y, 16 * TT);
     const int row0 = tile.first, n0 = (blockIdx.x * 4 + wave) * 16 * CT;
-    const int of_lane = adapter_of(a, row0 + (lane & (16 * TT - 1)), tile.end);
+    int of_lane = adapter_of(a, row0 + (lane & (16 * TT - 1)), tile.end);
+    const uint64_t here = __ballot((of_lane < 0 ? 0 : of_lane % a.share) == (int)blockIdx.z);  // its tokens, and part 0 those without an adapter
+    if (!(here >> lane & 1)) of_lane = -1;
     const float* y[TT];
     float* out[TT];
     float4 yv[CT][TT];
@@ -480,7 +489,7 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a, bool vec_out) 
     }
 #pragma unroll
     for (int tt = 0; tt < TT; tt++) {
-        if (row0 + 16 * tt + i >= tile.end) continue;
+        if (row0 + 16 * tt + i >= tile.end || !(here >> (16 * tt + i) & 1)) continue;
         const float scale = mine[tt] >= 0 ? a.scales[mine[tt]] : 0.0f;
 #pragma unroll
         for (int c = 0; c < CT; c++) {
@@ -519,9 +528,15 @@ static int lora_launch(LoraArgs a, bool vec_out, hipStream_t st) {
     const int tile = lora_tile(a.rows), tt = tile / 16, nr = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
     const unsigned tiles = (unsigned)lora_tiles(a.rows / a.tokens, a.tokens);
     a.tiles = a.tokens >= tile ? (a.tokens + tile - 1) / tile : 0;
-    const dim3 down(tiles, (unsigned)a.splits, (unsigned)((a.R + 16 * nr - 1) / (16 * nr)));
+    // Tiles with several adapters: dealt out while there are fewer than 256 workgroups.  (us a call, the first launch with 1 / 2 / 4 / 8 for each, fp16: 32
+    // tokens, 20 adapters 4096 -> 11008, rank 16 16.4 / 14.9 / 14.0 / 13.6; 3 tokens, 3 adapters 4096 -> 4096 8.8 / 7.4; 32 x 5 tokens, which have 160 workgroups,
+    // 12.4 / 14.9 / 13.7 / 13.1.  The second, until there are 128 / 256 / 1024: 32 tokens, 32 adapters 4096 -> 4096 11.7 / 10.9 / 12.0.)
+    auto shares = [&](unsigned groups) { return a.tokens < tile && a.rows > a.tokens ? std::max(1, std::min(a.adapters, (int)(256 / groups))) : 1; };
+    const unsigned nz = (unsigned)((a.R + 16 * nr - 1) / (16 * nr));
+    a.share = shares(tiles * (unsigned)a.splits * nz);
+    const dim3 down(tiles, (unsigned)a.splits, nz * (unsigned)a.share);
 #define LLMOPS_DOWN(NR, TT) lora_down_kernel<W, NR, TT, false><<<down, 64 * kDownWaves, 0, st>>>(a)
-    const dim3 narrow(tiles, 1, (unsigned)((a.R + 15) / 16));
+    const dim3 narrow(tiles, 1, (unsigned)((a.R + 15) / 16) * (unsigned)a.share);
     if (a.K < 8 && tt == 1) lora_down_kernel<W, 1, 1, true><<<narrow, 64 * kDownWaves, 0, st>>>(a);
     else if (a.K < 8) lora_down_kernel<W, 1, 2, true><<<narrow, 64 * kDownWaves, 0, st>>>(a);
     else if (tt == 1 && nr == 1) LLMOPS_DOWN(1, 1);
@@ -535,7 +550,9 @@ static int lora_launch(LoraArgs a, bool vec_out, hipStream_t st) {
     // few tokens: 64 columns to a workgroup, so that there are enough of them, and the weights of eight adapters on their way; many: 256, so that a
     // token's sums are read by fewer
     const int ct = tt == 1 ? 1 : 4;
-    const dim3 up((unsigned)((a.N + 64 * ct - 1) / (64 * ct)), tiles);
+    const unsigned columns = (unsigned)((a.N + 64 * ct - 1) / (64 * ct));
+    a.share = shares(columns * tiles);
+    const dim3 up(columns, tiles, (unsigned)a.share);
     if (tt == 1 && a.R < 8) lora_up_kernel<W, 1, 1, true><<<up, 256, 0, st>>>(a, vec_out);
     else if (tt == 1) lora_up_kernel<W, 1, 1, false><<<up, 256, 0, st>>>(a, vec_out);
     else if (a.R < 8) lora_up_kernel<W, 4, 2, true><<<up, 256, 0, st>>>(a, vec_out);

@@ -140,8 +140,8 @@ __device__ __forceinline__ void store_row(T* dst, int d, const float (&x)[8]) {
     store_row4(dst + 64 + d, x + 4);
 }
 
-// Where queries fill tiles of 64 or 128.  A workgroup per token and 16 of its H + 2*Hkv rows of 128.  Bound by latency at few tokens and by
-// memory at many.
+// Before the launches whose workgroups do not rotate for themselves.  A workgroup per token and 16 of its H + 2*Hkv rows of 128.  Bound by latency
+// at few tokens (64 of 48 rows: 5 us) and by memory at many (4 x 300 of 96 rows, a quarter padding: 20 us, 71 MB to and from HBM).
 template <typename T>
 __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a, PrepArgs p) {
     __shared__ float2 turn[64];
@@ -454,7 +454,8 @@ __device__ __forceinline__ bool needs_full_width(const int (&range)[4][2], Rows<
     return k == 2 || v == 2 || (k == 0 && !(all_zero(K, from) && all_zero(K1, from1))) || (v == 0 && !(all_zero(V, from) && all_zero(V1, from1)));
 }
 
-// Few queries to a workgroup (16 * RT): bound by reading the rows.  The four waves take 32 rows each of every 128; operands come
+// Few queries to a workgroup (16 * RT): bound by reading rows of halves (32 sequences of 32 heads behind 2048 rows, 512 of their own at most: 170 MB in
+// 38 us, 4.4 TB/s) and by cutting up those of fp32 (2 us for a wave's 32).  The four waves take 32 rows each of every 128; operands come
 // straight from memory, K of the next rows asked for when K of these is used up, and so V; the waves' sums meet in LDS.
 constexpr int kMeetRow = 132;  // floats (16 queries' rows on different banks)
 struct MeetSmem {
@@ -752,8 +753,10 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs&
     }
 }
 
-// Many queries (64 * RT to a workgroup, 16 * RT to a wave): bound by the matrix cores and, beside them, the vector ALU that cuts rows up
-// and weighs scores.  All waves multiply the same 32 rows, which the workgroup cuts up once and leaves in LDS in the order of the
+// Many queries (64 * RT to a workgroup, 16 * RT to a wave): bound by issuing instructions to three units that overlap in part.  (4 x 300 tokens of 32
+// heads behind 1000 rows, a quarter padding, fp32, RT 1: 115 to 130 us, of which the vector ALU, weighing and cutting, would take 43 at 2.4 GHz, LDS
+// reads 47, the matrix cores 28; waves wait for memory a quarter of the time.  RT 2 halves the reads.  A single buffer and three workgroups to a compute unit
+// instead of two buffers and two: 151 us a call for 144.)  All waves multiply the same 32 rows, which the workgroup cuts up once and leaves in LDS in the order of the
 // operands (a read is 16 bytes to a lane, in lane order); two buffers: while a tile is multiplied the next is cut up and the one behind
 // it is on its way from memory.  Tiles 0 .. np-1 are the prefix's, those from np on the sequence's own.
 template <typename T>
@@ -1031,7 +1034,7 @@ __global__ __launch_bounds__(256, 2) void prefix_sweep_kernel(PrefixArgs a) {
 }
 
 // ---- 3. the pieces of a query ----
-// half a wave to a query, 16 bytes to a lane
+// half a wave to a query, 16 bytes to a lane.  Bound by latency: 4 us for two chats, 5 for 64 sequences of 32 heads (8 MB)
 __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int d = 4 * (threadIdx.x & 31);

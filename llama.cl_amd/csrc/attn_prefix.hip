@@ -205,22 +205,34 @@ __device__ __forceinline__ uint32_t cut2(float x, float y, uint32_t& lo) {
     lo = *reinterpret_cast<const uint32_t*>(&l);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// largest magnitude of the halves seen so far, as bits (NaN above infinity above all else)
-__device__ __forceinline__ void note(v2us& top, uint32_t halves) {
-    const uint32_t u = halves & 0x7fff7fffu;
-    top = __builtin_elementwise_max(top, *reinterpret_cast<const v2us*>(&u));
-}
-__device__ __forceinline__ void note4(v2us& top, uint4 h) {
-    note(top, h.x), note(top, h.y), note(top, h.z), note(top, h.w);
-    asm volatile("" : "+v"(top));  // here and now: put off to the loop's end, a tile's 64 operands stay in registers till then
-}
-// What was seen of K or V: 2 if there are values outside the halves' range (fp32 values that truncate to the largest half, infinities,
-// NaN), 1 if there are some in their normal range; 0 if all are below 2^-14, where the low halves no longer hold 21 bits of the largest
+// The largest magnitude seen of K or V so far, NaN above all else: of fp32 values (an instruction for two), of halves as bits
 template <typename T>
-__device__ __forceinline__ int range_of(v2us top) {
-    const unsigned short most = top[0] > top[1] ? top[0] : top[1];
-    return sizeof(T) == 4 ? (most >= 0x7bff ? 2 : most >= 0x0400 ? 1 : 0) : most >= 0x7c00 ? 2 : 1;
-}
+struct Seen;
+template <>
+struct Seen<float> {
+    float top = 0.0f;
+    __device__ __forceinline__ void note(float x, float y) { top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, fabsf(x)), fabsf(y)); }
+    __device__ __forceinline__ void note(float4 x) {
+        note(x.x, x.y), note(x.z, x.w);
+        asm volatile("" : "+v"(top));  // here and now: put off to the loop's end, a tile's 64 operands stay in registers till then
+    }
+    // 2 if there are values outside the halves' range (those that truncate to the largest half, infinities, NaN), 1 if there are some in their
+    // normal range; 0 if all are below 2^-14, where the low halves no longer hold 21 bits of the largest
+    __device__ __forceinline__ int range() const { return !(top < 65504.0f) ? 2 : top >= 0x1p-14f ? 1 : 0; }
+};
+template <>
+struct Seen<__half> {
+    v2us top = {0, 0};
+    __device__ __forceinline__ void note(uint32_t halves) {
+        const uint32_t u = halves & 0x7fff7fffu;
+        top = __builtin_elementwise_max(top, *reinterpret_cast<const v2us*>(&u));
+    }
+    __device__ __forceinline__ void note(uint4 h) {
+        note(h.x), note(h.y), note(h.z), note(h.w);
+        asm volatile("" : "+v"(top));  // (as above)
+    }
+    __device__ __forceinline__ int range() const { return (top[0] > top[1] ? top[0] : top[1]) >= 0x7c00 ? 2 : 1; }
+};
 
 __device__ __forceinline__ v8h as_v8h(uint4 u) { return *reinterpret_cast<const v8h*>(&u); }
 __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -437,8 +449,8 @@ __device__ __forceinline__ void nothing(const PrefixArgs& a, int hk, int m0, int
 
 // a wave's say, and the workgroup's decision
 template <typename T>
-__device__ __forceinline__ void note_range(v2us ktop, v2us vtop, int (&range)[2], int lane) {
-    const int k = range_of<T>(ktop), v = range_of<T>(vtop);
+__device__ __forceinline__ void note_range(const Seen<T>& ktop, const Seen<T>& vtop, int (&range)[2], int lane) {
+    const int k = ktop.range(), v = vtop.range();
     const int ks = __any(k == 2) ? 2 : __any(k == 1) ? 1 : 0, vs = __any(v == 2) ? 2 : __any(v == 1) ? 1 : 0;
     if (lane == 0) range[0] = ks, range[1] = vs;
 }
@@ -507,18 +519,18 @@ struct RowRegs<float> {
 #pragma unroll
             for (int h = 0; h < 2; h++) v[j][h] = __builtin_bit_cast(float4, ask16(r, mine, ((16 * (j >> 2) + (j & 3)) * kS + 64 * h) * 4));
     }
-    __device__ __forceinline__ Halves k_op(int tt, int step, v2us& top) const {
+    __device__ __forceinline__ Halves k_op(int tt, int step, Seen<float>& top) const {
         const float4 x = k[tt][step][0], y = k[tt][step][1];
+        top.note(x), top.note(y);
         uint4 h, l;
         h.x = cut2(x.x, x.y, l.x), h.y = cut2(x.z, x.w, l.y), h.z = cut2(y.x, y.y, l.z), h.w = cut2(y.z, y.w, l.w);
-        note4(top, h);
         return {as_v8h(h), as_v8h(l)};
     }
-    __device__ __forceinline__ Halves v_op(int c, v2us& top) const {
+    __device__ __forceinline__ Halves v_op(int c, Seen<float>& top) const {
         auto f = [&](int j) { return reinterpret_cast<const float*>(&v[j][c >> 2])[c & 3]; };
         uint4 h, l;
         h.x = cut2(f(0), f(1), l.x), h.y = cut2(f(2), f(3), l.y), h.z = cut2(f(4), f(5), l.z), h.w = cut2(f(6), f(7), l.w);
-        note4(top, h);
+        top.note(make_float4(f(0), f(1), f(2), f(3))), top.note(make_float4(f(4), f(5), f(6), f(7)));
         return {as_v8h(h), as_v8h(l)};
     }
 };
@@ -542,12 +554,12 @@ struct RowRegs<__half> {
 #pragma unroll
             for (int h = 0; h < 2; h++) v[j][h] = ask8(r, mine, ((16 * (j >> 2) + (j & 3)) * kS + 64 * h) * 2);
     }
-    __device__ __forceinline__ Halves k_op(int tt, int step, v2us& top) const {
+    __device__ __forceinline__ Halves k_op(int tt, int step, Seen<__half>& top) const {
         const uint4 h = k[tt][step];
-        note4(top, h);
+        top.note(h);
         return {as_v8h(h), v8h{}};
     }
-    __device__ __forceinline__ Halves v_op(int c, v2us& top) const {
+    __device__ __forceinline__ Halves v_op(int c, Seen<__half>& top) const {
         uint32_t h[4];
 #pragma unroll
         for (int p = 0; p < 4; p++) {
@@ -556,7 +568,7 @@ struct RowRegs<__half> {
             h[p] = __builtin_amdgcn_perm(b, a, (c & 1) ? 0x07060302u : 0x05040100u);
         }
         const uint4 all = make_uint4(h[0], h[1], h[2], h[3]);
-        note4(top, all);
+        top.note(all);
         return {as_v8h(all), v8h{}};
     }
 };
@@ -655,7 +667,7 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs&
         see[rt] = own ? min(K1.end, rows_seen(a, min(m0 + 16 * rt + i, m_end - 1), b, len, n)) : 0;
         see_min = min(see_min, see[rt]);
     }
-    v2us ktop = {0, 0}, vtop = {0, 0};
+    Seen<T> ktop, vtop;
     for (; j < j1; j += 4) {
         const bool mine = j >= np;
         const int t = 32 * (mine ? j - np : j);
@@ -781,13 +793,13 @@ struct TileRegs<float> {
 #pragma unroll
         for (int r = 0; r < 4; r++) v[r] = __builtin_bit_cast(float4, ask16(V, v_at, r * kS * 4));
     }
-    __device__ __forceinline__ void write(TileSmem<float>& sm, int buf, int wave, int lane, v2us& ktop, v2us& vtop) const {
+    __device__ __forceinline__ void write(TileSmem<float>& sm, int buf, int wave, int lane, Seen<float>& ktop, Seen<float>& vtop) const {
 #pragma unroll
         for (int c = 0; c < 2; c++) {
             const float4 x = k[c][0], y = k[c][1];
             uint4 h, l;
             h.x = cut2(x.x, x.y, l.x), h.y = cut2(x.z, x.w, l.y), h.z = cut2(y.x, y.y, l.z), h.w = cut2(y.z, y.w, l.w);
-            note4(ktop, h);
+            ktop.note(x), ktop.note(y);
             sm.k[buf][0][2 * wave + c][lane] = h;
             sm.k[buf][1][2 * wave + c][lane] = l;
         }
@@ -797,7 +809,7 @@ struct TileRegs<float> {
             auto f = [&](int r) { return reinterpret_cast<const float*>(&v[r])[c]; };
             uint2 h, l;
             h.x = cut2(f(0), f(1), l.x), h.y = cut2(f(2), f(3), l.y);
-            note4(vtop, make_uint4(h.x, h.y, 0u, 0u));
+            vtop.note(make_float4(f(0), f(1), f(2), f(3)));
             reinterpret_cast<uint2*>(&sm.v[buf][0][4 * (wave & 1) + c][lane])[tt] = h;
             reinterpret_cast<uint2*>(&sm.v[buf][1][4 * (wave & 1) + c][lane])[tt] = l;
         }
@@ -815,10 +827,10 @@ struct TileRegs<__half> {
 #pragma unroll
         for (int r = 0; r < 4; r++) v[r] = ask8(V, v_at, r * kS * 2);
     }
-    __device__ __forceinline__ void write(TileSmem<__half>& sm, int buf, int wave, int lane, v2us& ktop, v2us& vtop) const {
+    __device__ __forceinline__ void write(TileSmem<__half>& sm, int buf, int wave, int lane, Seen<__half>& ktop, Seen<__half>& vtop) const {
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-            note4(ktop, k[c]);
+            ktop.note(k[c]);
             sm.k[buf][0][2 * wave + c][lane] = k[c];
         }
         const int tt = wave >> 1;
@@ -827,7 +839,7 @@ struct TileRegs<__half> {
             auto f = [&](int r) { return (c & 2) ? v[r].y : v[r].x; };
             const uint32_t pick = (c & 1) ? 0x07060302u : 0x05040100u;
             const uint2 h = make_uint2(__builtin_amdgcn_perm(f(1), f(0), pick), __builtin_amdgcn_perm(f(3), f(2), pick));
-            note4(vtop, make_uint4(h.x, h.y, 0u, 0u));
+            vtop.note(make_uint4(h.x, h.y, 0u, 0u));
             reinterpret_cast<uint2*>(&sm.v[buf][0][4 * (wave & 1) + c][lane])[tt] = h;
         }
     }
@@ -866,7 +878,7 @@ __device__ __forceinline__ void many_queries(const PrefixArgs& a, int hk, int m0
         see[rt] = own ? min(K1.end, rows_seen(a, m, b, len, n)) : 0;
         see_min = min(see_min, see[rt]);
     }
-    v2us ktop = {0, 0}, vtop = {0, 0};
+    Seen<T> ktop, vtop;
     x.write(sm, 0, wave, lane, ktop, vtop);
     load(min(j0 + 1, j1 - 1));
     __syncthreads();

@@ -322,18 +322,24 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
         if (own && x >= 0 && c == sum_run) return sum_left;
         return own ? a.sum[at + c] * share(a.top[at + c], r.top, per_t) * r.inv : __hip_atomic_load(&rest[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
-    double total = 0.0;
-    for (int c0 = 0; c0 < a.runs; c0 += 64) total += wave_sum64(run_sum(c0 + lane, !spread));
+    double held = run_sum(lane, !spread);  // (of the first 64 runs, mostly all there are: asked for once)
+    auto sum_of = [&](bool own) {
+        double t = wave_sum64(held);
+        for (int c0 = 64; c0 < a.runs; c0 += 64) t += wave_sum64(run_sum(c0 + lane, own));
+        return t;
+    };
+    double total = sum_of(!spread);
     const bool none = !(total > 0.0);  // nothing above the draft's distribution: the target's own
     if (none) {
-        less = false, x = -1, total = 0.0;
-        for (int c0 = 0; c0 < a.runs; c0 += 64) total += wave_sum64(run_sum(c0 + lane, true));
+        less = false, x = -1;
+        held = run_sum(lane, true);
+        total = sum_of(true);
     }
     const double goal = (double)a.uniforms[row0 + a.K] * total;
     double before = 0.0, heavy_before = 0.0;  // sums of the runs before the one, and before the last with a weight
     int at_run = -1, heavy = 0;
     for (int c0 = 0; c0 < a.runs && at_run < 0; c0 += 64) {
-        const double mine = run_sum(c0 + lane, none || !spread);
+        const double mine = c0 == 0 ? held : run_sum(c0 + lane, none || !spread);
         const double to = before + scan64(mine);  // up to and with this lane's run
         const uint64_t past = __ballot(to > goal && mine > 0.0), some = __ballot(mine > 0.0);
         if (some != 0) {

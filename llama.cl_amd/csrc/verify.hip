@@ -218,13 +218,14 @@ __device__ __forceinline__ double rest_weight(const Weigher& weigh, double inv, 
 
 // A workgroup: a run of the row that the next token of a sequence comes from (all but the first end at once where the first launch's sums do).  Bound by
 // latency, a chain of dependent steps: rows' sums, the accepted drafts, the run's sum, the arrival, the run, the token (12.6 us for 32 sequences, 55296).
-__global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
+constexpr int kNextWaves = 8, kNext = 64 * kNextWaves, kEach = kRun / kNext;
+__global__ __launch_bounds__(kNext) void verify_next_kernel(VerifyArgs a) {
     __shared__ int first, arrivals, found, last;
     __shared__ Row shared_row;
-    __shared__ Draft shared_draft[4];
+    __shared__ Draft shared_draft[kNextWaves];
     __shared__ int refused_token;
-    __shared__ double red[4];
-    __shared__ float neighbours[2][kRun + kRun / 16];  // (16 in a row and a gap: a thread's on banks of their own)
+    __shared__ double red[kNextWaves];
+    __shared__ float neighbours[2][kRun + kNext];  // (a thread's in a row and a gap: on banks of their own)
     const int b = blockIdx.x / (unsigned)a.runs, run = blockIdx.x - b * a.runs, n = drafts_of(a, b), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float t = temperature_of(a, b);
     const bool draws = t > 0.0f;
@@ -232,10 +233,10 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     if (!draws && run > 0) return;  // (the likeliest token needs no sums)
     if (threadIdx.x == 0) first = n;
     __syncthreads();
-    // drafts, four at a time, until one is refused
+    // drafts, a wave to each, until one is refused
     const int row0 = b * (a.K + 1);
     const float* probs = a.probs != nullptr ? a.probs + (int64_t)b * a.K * a.V : nullptr;
-    for (int i0 = 0; i0 <= n; i0 += 4) {
+    for (int i0 = 0; i0 <= n; i0 += kNextWaves) {
         const int i = i0 + wave;
         Row r{};
         if (i <= n) {
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
         const int done = first;
         if (done == i && lane == 0) shared_row = r, refused_token = shared_draft[wave].x;
         __syncthreads();
-        if (done < i0 + 4) break;
+        if (done < i0 + kNextWaves) break;
     }
     const int done = first, row = row0 + done;
     const Row r = shared_row;
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     int64_t* tokens = a.tokens + row0;
     if (run == 0) {
         if (threadIdx.x == 0) a.accepted[b] = done;
-        for (int i = threadIdx.x; i <= a.K; i += 256)
+        for (int i = threadIdx.x; i <= a.K; i += kNext)
             if (i != done) tokens[i] = i < done ? a.drafts[(int64_t)b * a.K + i] : -1;
     }
     if (!draws || r.top == -INFINITY) {  // the likeliest; nothing to take: none
@@ -273,33 +274,35 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     const bool spread = less;
     if (!spread && run > 0) return;
     double* rest = a.rest + (int64_t)b * a.runs;
-    // a thread's sixteen of a run, 256 apart; what lies behind the row weighs nothing
-    auto load = [&](int at_run, float (&z)[16], float (&q)[16]) {
+    // a thread's part of a run, kNext apart; what lies behind the row weighs nothing
+    auto load = [&](int at_run, float (&z)[kEach], float (&q)[kEach]) {
         const int j0 = at_run * kRun + threadIdx.x;
 #pragma unroll
-        for (int e = 0; e < 16; e++) z[e] = zrow[min(j0 + 256 * e, a.V - 1)];
+        for (int e = 0; e < kEach; e++) z[e] = zrow[min(j0 + kNext * e, a.V - 1)];
         if (qrow != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) q[e] = qrow[min(j0 + 256 * e, a.V - 1)];
+            for (int e = 0; e < kEach; e++) q[e] = qrow[min(j0 + kNext * e, a.V - 1)];
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; e++) q[e] = 0.0f;
+            for (int e = 0; e < kEach; e++) q[e] = 0.0f;
         }
 #pragma unroll
-        for (int e = 0; e < 16; e++)
-            if (j0 + 256 * e >= a.V) z[e] = -INFINITY;
+        for (int e = 0; e < kEach; e++)
+            if (j0 + kNext * e >= a.V) z[e] = -INFINITY;
     };
     const int sum_run = spread ? run : x >= 0 ? x / kRun : -1;
     double sum = 0.0;
     if (sum_run >= 0) {
-        float z[16], q[16];
+        float z[kEach], q[kEach];
         load(sum_run, z, q);
 #pragma unroll
-        for (int e = 0; e < 16; e++) sum += rest_weight(weigh, r.inv, z[e], less, q[e], sum_run * kRun + (int)threadIdx.x + 256 * e == x);
+        for (int e = 0; e < kEach; e++) sum += rest_weight(weigh, r.inv, z[e], less, q[e], sum_run * kRun + (int)threadIdx.x + kNext * e == x);
         sum = wave_sum64(sum);
         if (lane == 0) red[wave] = sum;
         __syncthreads();
-        sum = (red[0] + red[1]) + (red[2] + red[3]);
+        sum = 0.0;
+#pragma unroll
+        for (int u = 0; u < kNextWaves; u++) sum += red[u];
     }
     if (threadIdx.x == 0) found = (int)kNowhere, last = -1;
     if (spread) {
@@ -356,24 +359,24 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
         }
     }
     if (at_run < 0) at_run = heavy, before = heavy_before;  // (rounding, or a random number of 1: the last token with a weight)
-    // its tokens in their order, 16 to a thread
+    // its tokens in their order, kEach to a thread
     {
-        float z[16], q[16];
+        float z[kEach], q[kEach];
         load(at_run, z, q);
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int at = threadIdx.x + 256 * e + (threadIdx.x >> 4) + 16 * e;
+        for (int e = 0; e < kEach; e++) {
+            const int p = threadIdx.x + kNext * e, at = p + p / kEach;
             neighbours[0][at] = z[e];
             neighbours[1][at] = q[e];
         }
     }
     __syncthreads();
-    const int j0 = at_run * kRun + 16 * threadIdx.x;
-    double w[16];
+    const int j0 = at_run * kRun + kEach * threadIdx.x;
+    double w[kEach];
     sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-        w[e] = rest_weight(weigh, r.inv, neighbours[0][17 * threadIdx.x + e], less, neighbours[1][17 * threadIdx.x + e], j0 + e == x);
+    for (int e = 0; e < kEach; e++) {
+        w[e] = rest_weight(weigh, r.inv, neighbours[0][(kEach + 1) * threadIdx.x + e], less, neighbours[1][(kEach + 1) * threadIdx.x + e], j0 + e == x);
         sum += w[e];
     }
     const double to = scan64(sum);
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
     before += to - sum;
     int mine = (int)kNowhere, some = -1;
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
+    for (int e = 0; e < kEach; e++) {
         before += w[e];
         if (w[e] > 0.0) {
             some = j0 + e;
@@ -436,7 +439,7 @@ extern "C" int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, i
     LLMOPS_REQUIRE(aligned(logits, 4) && aligned(draft_probs, 4) && aligned(uniforms, 4) && aligned(drafts, 8) && aligned(tokens, 8));
     VerifyArgs a{};
     a.runs = (int)((V + kRun - 1) / kRun);
-    LLMOPS_REQUIRE(B * a.runs < ((int64_t)1 << 24));  // (a launch has fewer than 2^32 threads)
+    LLMOPS_REQUIRE(B * a.runs * kNext < ((int64_t)1 << 32));  // (a launch has fewer than 2^32 threads)
     const VerifyLayout w = layout_verify(B, K, a.runs);
     if (workspace == nullptr || workspace_bytes < w.total)
         return fail(LLMOPS_EWORKSPACE, "verify_drafts needs %zu workspace bytes, got %zu", w.total, workspace == nullptr ? (size_t)0 : workspace_bytes);
@@ -450,7 +453,7 @@ extern "C" int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, i
     hipStream_t st = as_stream(stream);
     verify_rows_kernel<<<dim3((unsigned)(B * (K + 1)), (unsigned)a.runs), 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
-    verify_next_kernel<<<(unsigned)(B * a.runs), 256, 0, st>>>(a);
+    verify_next_kernel<<<(unsigned)(B * a.runs), kNext, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }

@@ -766,8 +766,8 @@ __device__ __forceinline__ void few_queries(const PrefixArgs& a, const PrepArgs&
 }
 
 // Many queries (64 * RT to a workgroup, 16 * RT to a wave): bound by issuing instructions to three units that overlap in part.  (4 x 300 tokens of 32
-// heads behind 1000 rows, a quarter padding, fp32, RT 1: 115 to 130 us, of which the vector ALU, weighing and cutting, would take 43 at 2.4 GHz, LDS
-// reads 47, the matrix cores 28; waves wait for memory a quarter of the time.  RT 2 halves the reads.  A single buffer and three workgroups to a compute unit
+// heads behind 1000 rows, a quarter padding, fp32, RT 1: 110 to 126 us, of which the vector ALU, weighing and cutting, would take 50 at 2.3 GHz, LDS
+// reads 35, the matrix cores 29; waves wait for memory a quarter of the time.  RT 2 halves the reads.  A single buffer and three workgroups to a compute unit
 // instead of two buffers and two: 151 us a call for 144.)  All waves multiply the same 32 rows, which the workgroup cuts up once and leaves in LDS in the order of the
 // operands (a read is 16 bytes to a lane, in lane order); two buffers: while a tile is multiplied the next is cut up and the one behind
 // it is on its way from memory.  Tiles 0 .. np-1 are the prefix's, those from np on the sequence's own.

@@ -440,7 +440,7 @@ extern "C" int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, i
     LLMOPS_REQUIRE(aligned(logits, 4) && aligned(draft_probs, 4) && aligned(uniforms, 4) && aligned(drafts, 8) && aligned(tokens, 8));
     VerifyArgs a{};
     a.runs = (int)((V + kRun - 1) / kRun);
-    LLMOPS_REQUIRE(B * a.runs * kNext < ((int64_t)1 << 32));  // (a launch has fewer than 2^32 threads)
+    LLMOPS_REQUIRE(B * a.runs < ((int64_t)1 << 32) / kNext);  // (a launch has fewer than 2^32 threads)
     const VerifyLayout w = layout_verify(B, K, a.runs);
     if (workspace == nullptr || workspace_bytes < w.total)
         return fail(LLMOPS_EWORKSPACE, "verify_drafts needs %zu workspace bytes, got %zu", w.total, workspace == nullptr ? (size_t)0 : workspace_bytes);

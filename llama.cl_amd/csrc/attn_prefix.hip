@@ -146,19 +146,19 @@ template <typename T>
 __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a, PrepArgs p) {
     __shared__ float2 turn[64];
     const int bl = blockIdx.x / p.groups, group = blockIdx.x - bl * p.groups, b = bl / a.qL, l = bl - b * a.qL;
+    const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), d = 4 * (threadIdx.x & 15);
+    const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv, none = row >= H + 2 * a.Hkv;
+    const float* src = is_q ? p.q + b * p.qsb + l * p.qsl + (int64_t)row * kS
+                            : is_k ? p.k + b * p.ksb + l * p.ksl + (int64_t)(row - H) * kS : p.v + b * p.vsb + l * p.vsl + (int64_t)(row - H - a.Hkv) * kS;
+    // (the row is on its way while the length is fetched and the angles are formed, also where the token turns out to be padding)
+    float x[8] = {};
+    if (!none) load_row(src, d, x);
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
     const bool live = l < n;
     if (live && (int)threadIdx.x < p.half) turn_of(p.inv_freq[threadIdx.x], a.P + len + l, turn[threadIdx.x].x, turn[threadIdx.x].y);
     __syncthreads();
-    const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), d = 4 * (threadIdx.x & 15);
-    if (row >= H + 2 * a.Hkv) return;
-    const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv;
-    if (!live && !is_q) return;
-    const float* src = is_q ? p.q + b * p.qsb + l * p.qsl + (int64_t)row * kS
-                            : is_k ? p.k + b * p.ksb + l * p.ksl + (int64_t)(row - H) * kS : p.v + b * p.vsb + l * p.vsl + (int64_t)(row - H - a.Hkv) * kS;
-    float x[8];
-    load_row(src, d, x);
+    if (none || (!live && !is_q)) return;
     if (live && (is_q || is_k)) turn_row(src, d, turn, p.half, x);
     if (!is_q) {
         const int hk = is_k ? row - H : row - H - a.Hkv;

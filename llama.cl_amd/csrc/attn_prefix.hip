@@ -1055,11 +1055,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
     float* out = a.out + ((int64_t)bl * a.G * a.Hkv + (int64_t)hk * a.G + (m - bl * a.G)) * kS + d;
-    if (l >= n) {
-        *reinterpret_cast<float4*>(out) = make_float4(0.f, 0.f, 0.f, 0.f);
-        return;
-    }
-    // eight records at a time, asked for together; a piece that the query sees nothing of has sum 0 and may have written nothing else
+    // eight records at a time, asked for together, with the length that tells whether the query is padding; a piece that the query sees nothing of has sum 0 and may have written nothing else
     const float2* stat = a.rec_stat + r * a.nrec;
     const float* rec = a.rec_out + r * a.nrec * kS + d;
     float M = -INFINITY, L = 0.0f;
@@ -1092,7 +1088,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
         }
     }
     const float inv = 1.0f / L;
-    *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    *reinterpret_cast<float4*>(out) = l < n ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 struct PrefixPlan {

@@ -16,7 +16,8 @@
 // those of one sequence are both runs of m.  Rows are numbered through: r < P is the prefix's, P + i is the sequence's own row i.
 //
 // Arithmetic.  Products run on the fp16 matrix cores (v_mfma_f32_16x16x32_f16, fp32 sums) with fp32 values carried as two halves:
-//   q'  scaled by a power of two of its row so that its largest value is in [2^13, 2^14): hi + lo, 22 bits of that
+//   q'  scaled by a power of two of its row so that its largest value is in [2^13, 2^14): hi + lo, 22 bits of that (rows below 2^-110 scaled
+//       by 2^123: 2^-148 at least)
 //   K,V hi + lo / 2048, hi truncated and lo = (x - hi) * 2048 in a half: 21 bits of x from 2^-14 on, 2^-36 below (a cache of
 //       halves is hi alone)
 //   e   times 2^14: hi + lo, so that weights down to 2^-28 of the largest keep their bits
@@ -123,7 +124,8 @@ __device__ __forceinline__ QueryRow query_row(const float (&x)[8], bool live) {
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64)), bad = fmaxf(bad, __shfl_xor(bad, o, 64));
     const bool use = live && bad == 0.0f && top > 0.0f;
-    const int e2 = use ? 13 - ilogbf(top) : 0;
+    // (2^123 at most: the factor stays a normal number.  It would lose its bits below 2^-126, and at 0 make NaN of a masked score's -inf)
+    const int e2 = use ? min(123, 13 - ilogbf(top)) : 0;
     v8h hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; e++) {

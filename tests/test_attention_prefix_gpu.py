@@ -357,3 +357,28 @@ def test_every_way_of_cutting_up(B, L, H, Hkv, P, maxlen, half_cache):
     big[..., (H + Hkv) * S:] *= 1e2
     big[..., :H * S] *= 1e-5 if not half_cache else 1.0
     _check(big, H, Hkv, prefix, P, cache, lengths, (torch.arange(B) % (L + 1)).to(torch.int32))
+
+
+@pytest.mark.parametrize("half_cache", [False, True])
+@pytest.mark.parametrize("B,L,H,Hkv,P,maxlen", KINDS)
+def test_queries_down_to_the_least_number(B, L, H, Hkv, P, maxlen, half_cache):
+    """queries of 1e-36 down to the least denormal, tokens and heads of each beside each other and beside ordinary ones, in front of tiles that a
+    mask ends in: their scores are 0 to 64 bits' eyes and an output is the mean of the rows seen"""
+    qkv, prefix, cache, lengths, _ = _case(B, L, H, Hkv, P, maxlen, half_cache, seed=22)
+    sizes = torch.tensor([1.0, 1e-36, 1e-38, 1e-39, 3e-41, 5e-42, 1e-43, 5e-45, 1.5e-45, 0.0])
+    size = sizes[torch.arange(B * L * H) % len(sizes)].reshape(B, L, H, 1)
+    qkv[..., :H * S] = (qkv[..., :H * S].reshape(B, L, H, S) * size).reshape(B, L, H * S)
+    _check(qkv, H, Hkv, prefix, P, cache, lengths, None)
+
+
+@pytest.mark.parametrize("L,P", [(1, 20), (1, 300), (3, 90), (70, 90)])
+@pytest.mark.parametrize("q_size", [1e-37, 1e-39, 1e-41])
+def test_least_queries_and_largest_keys(L, P, q_size):
+    """A query's denormal is a multiple of 2^-149, and so are the rounding errors of its rotation and of its operands, 2^-148 at most: beside keys of
+    3e37 = 2^124.5 a score is off by 2^-148 * 2^124.5 * sqrt(128) / sqrt(128) = 2^-23.5, within REL"""
+    qkv, prefix, cache, lengths, _ = _case(2, L, 4, 2, P, L + 60, False, seed=23)
+    qkv[..., :4 * S] *= q_size
+    qkv[..., 4 * S:6 * S] *= 3e37
+    prefix[0] *= 3e37
+    cache[0] *= 3e37
+    _check(qkv, 4, 2, prefix, P, cache, lengths, None)

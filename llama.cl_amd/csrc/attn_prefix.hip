@@ -1216,8 +1216,8 @@ using namespace llmops;
 
 static bool prefix_sizes_fit(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t prefix_len, int64_t maxlen) {
     const int64_t most = (int64_t)1 << 24;  // positions are exact in fp32
-    return B > 0 && qL > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && prefix_len >= 0 && maxlen > 0 && B < most && qL < most && H < most && prefix_len < most &&
-           maxlen < most && prefix_len + maxlen <= most && B * qL < ((int64_t)1 << 31) / H;
+    return B > 0 && qL > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && prefix_len >= 0 && maxlen > 0 && B < most && qL < most && H < most && prefix_len <= most &&
+           maxlen <= most && prefix_len + maxlen <= most && B * qL < ((int64_t)1 << 31) / H;
 }
 
 extern "C" size_t llmops_attention_prefix_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t prefix_len, int64_t maxlen) {

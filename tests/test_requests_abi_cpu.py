@@ -126,3 +126,14 @@ def test_request_cache_bookkeeping_on_the_host():
     assert c.lengths.tolist() == [2, 0, 4]
     with pytest.raises(ValueError):
         c.forget(0, 11)
+
+
+@pytest.mark.parametrize("prefix,maxlen", [(0, 1 << 24), (1 << 23, 1 << 23), ((1 << 24) - 1, 1)])
+def test_attention_rope_prefix_up_to_the_last_position(lib, prefix, maxlen):
+    """prefix and own rows together up to 2^24, as documented: the sizes are taken (refused is the workspace), and one row more is not"""
+    need = lib.llmops_attention_prefix_workspace_bytes(2, 3, 32, 8, 128, prefix, maxlen)
+    assert need > 0 and lib.llmops_attention_prefix_workspace_bytes(2, 3, 32, 8, 128, prefix, maxlen + 1) == 0
+    kw = dict(plen=prefix, pmax=1 << 24, maxlen=maxlen, kv=ctypes.c_void_p(1 << 50), bytes=need - 1)
+    _refused(lib, _prefix(lib, **kw), b"workspace bytes", 2)
+    kw["maxlen"] += 1
+    _refused(lib, _prefix(lib, **kw), b"prefix_sizes_fit")

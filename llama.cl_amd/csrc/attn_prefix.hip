@@ -64,9 +64,12 @@ __device__ __forceinline__ void own_extent(const int32_t* __restrict__ lengths, 
 }
 
 // ---- 1. rotation, cache rows, operands ----
-// cos and sin of inv_freq * pos with the product's rounding put back (at position 4000 it is 1.2e-4 of an angle)
+// cos and sin of inv_freq * pos: the product is exact in 64 bits, and so reduced to [-pi, pi] there (in fp32 it is off by 1.2e-4 at position
+// 4000, by up to 0.5 at 2^23); what its rounding to fp32 leaves out is put back to first order, 2^-24 being all that it can be
 __device__ __forceinline__ void turn_of(float f, int pos, float& c, float& s) {
-    const float p = (float)pos, hi = f * p, lo = fmaf(f, p, -hi);
+    const double angle = (double)f * (double)pos, whole = rint(angle * 0.15915494309189535);
+    const double rest = fma(-whole, 2.4492935982947064e-16, fma(-whole, 6.283185307179586, angle));  // 2 pi in two parts
+    const float hi = (float)rest, lo = (float)(rest - (double)hi);
     float s0, c0;
     sincosf(hi, &s0, &c0);
     c = fmaf(-lo, s0, c0);

@@ -382,3 +382,38 @@ def test_least_queries_and_largest_keys(L, P, q_size):
     prefix[0] *= 3e37
     cache[0] *= 3e37
     _check(qkv, 4, 2, prefix, P, cache, lengths, None)
+
+
+# (tokens, prefix, rows of its own): odd positions, for which a product with a frequency is rounded in fp32
+@pytest.mark.parametrize("L,P,n", [(1, 40001, 3), (1, 131071, 3), (20, 131071, 70), (70, 262139, 33), (2, 1000003, 5), (20, 70, 1000003), (3, 0, (1 << 24) - 3),
+                                   (17, (1 << 24) - 60, 40), (60, (1 << 24) - 70, 9)])
+def test_far_positions(L, P, n):
+    """Keys (1, 0) in every pair of dimensions leave the cosines and sines of their positions in the cache.  Each is off by sincosf's 2 ulp (2^-23) and
+    by the rounding of what is put back and of the product (2^-24 each): 2.4e-7.
+    Rows before them are all alike, so that the sums have a closed form.  A score, at most ln(2^24) = 17, is off by 2 * 2.4e-7 of itself (both sides'
+    rotation), 2^-21 + 2^-22 (operands) and 10 * 2^-24 (sums), 1.8e-6, that is 3e-5; a weight by a quarter of that, beside outputs near 1: 2e-5"""
+    H, maxlen, f = 2, n + L, _inv_freq()
+    N = P + n
+    g = torch.Generator().manual_seed(L)
+    a = math.log(N) * math.sqrt(S) / 64  # (a token's own row weighs as much as all before it)
+    pair = torch.cat((torch.ones(64), torch.zeros(64)))
+    q, k, v = (a * pair).repeat(H).expand(1, L, -1).contiguous(), pair.expand(1, L, -1).contiguous(), torch.randn(1, L, S, generator=g)
+    key, value = 2.0 ** -9, 0.25
+    prefix = torch.empty(2, 1, 1, P, S, device="cuda") if P else None
+    kv = torch.empty(2, 1, 1, maxlen, S, device="cuda")
+    for t in (prefix, kv):
+        if t is not None:
+            t[0], t[1] = key, value
+    out = llmops.attention_rope_prefix(q.cuda(), k.cuda(), v.cuda(), f.cuda(), prefix, P, kv, torch.tensor([n], dtype=torch.int32).cuda(), 0)
+    angle = torch.arange(N, N + L, dtype=torch.float64)[:, None] * f.double()
+    turned = torch.cat((angle.cos(), angle.sin()), dim=1)
+    rows = kv[0, 0, 0, n:].cpu().double()
+    assert (rows - turned).abs().max() <= 2.4e-7, (rows - turned).abs().max()
+    assert torch.equal(kv[1, 0, 0, n:].cpu(), v[0])
+    scores = (a * turned) @ turned.T / math.sqrt(S)
+    before = (a * turned).sum(1, keepdim=True) * key / math.sqrt(S)
+    weights = torch.cat((before + math.log(N), scores.masked_fill(torch.ones(L, L).triu(1) > 0, -math.inf)), dim=1).softmax(1)
+    want = weights[:, :1] * value + weights[:, 1:] @ v[0].double()
+    for h in range(H):
+        err = out[0, :, h * S:(h + 1) * S].cpu().double() - want
+        assert err.norm() <= 2e-5 * want.norm() and err.abs().max() <= 2e-4 * want.abs().max(), (err.norm() / want.norm(), err.abs().max())

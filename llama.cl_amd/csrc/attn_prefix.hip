@@ -19,11 +19,12 @@
 //   q'  scaled by a power of two of its row so that its largest value is in [2^13, 2^14): hi + lo, 22 bits of that (rows below 2^-110 scaled
 //       by 2^123: 2^-148 at least)
 //   K,V hi + lo / 2048, hi truncated and lo = (x - hi) * 2048 in a half: 21 bits of x from 2^-14 on, 2^-36 below (a cache of
-//       halves is hi alone)
+//       halves is hi alone: all of x from 2^-14 on, 2^-38 in the sums below)
 //   e   times 2^14: hi + lo, so that weights down to 2^-28 of the largest keep their bits
 // A product is hi*hi + lo*hi + hi*lo/2048; what is dropped is below 2^-21 of it.  Values outside the halves' range, infinities
-// and NaN are seen while a tile is cut up; such a tile is multiplied on the vector ALU in full width instead, row by row of those
-// that a query sees, so that what a mask hides has no effect whatever it holds.
+// and NaN are seen while a tile is cut up, and so is a piece whose K or whose V is below 2^-14 throughout; such a piece is multiplied on the
+// vector ALU in full width instead, row by row of those that a query sees, so that what a mask hides has no effect whatever it holds.  (Values
+// below 2^-14 beside larger ones of their piece are not seen: they are right to 2^-36, not to a part of themselves.)
 #include <float.h>
 
 #include "common.h"
@@ -236,7 +237,11 @@ struct Seen<__half> {
         note(h.x), note(h.y), note(h.z), note(h.w);
         asm volatile("" : "+v"(top));  // (as above)
     }
-    __device__ __forceinline__ int range() const { return (top[0] > top[1] ? top[0] : top[1]) >= 0x7c00 ? 2 : 1; }
+    // (0 as above: sums of halves below 2^-14 come out of the matrix cores right to 2^-38, 3e-5 of values near 1e-7)
+    __device__ __forceinline__ int range() const {
+        const unsigned short most = top[0] > top[1] ? top[0] : top[1];
+        return most >= 0x7c00 ? 2 : most >= 0x0400 ? 1 : 0;
+    }
 };
 
 __device__ __forceinline__ v8h as_v8h(uint4 u) { return *reinterpret_cast<const v8h*>(&u); }

@@ -417,3 +417,16 @@ def test_far_positions(L, P, n):
     for h in range(H):
         err = out[0, :, h * S:(h + 1) * S].cpu().double() - want
         assert err.norm() <= 2e-5 * want.norm() and err.abs().max() <= 2e-4 * want.abs().max(), (err.norm() / want.norm(), err.abs().max())
+
+
+@pytest.mark.parametrize("L,P", [(1, 20), (1, 300), (3, 90), (40, 90), (70, 90)])
+@pytest.mark.parametrize("kscale,vscale,qscale", [(1.0, 1e-6, 1.0), (1.0, 1e-7, 1.0), (1e-6, 1.0, 1e6), (1e-7, 1e-7, 1e7)])
+def test_halves_below_their_normal_range(L, P, kscale, vscale, qscale):
+    """caches of halves that hold denormals only: within REL of the largest output like all others"""
+    qkv, prefix, cache, lengths, _ = _case(2, L, 4, 2, P, L + 60, True, seed=24)
+    qkv[..., :4 * S] *= qscale
+    for t in (prefix, cache):
+        t[0], t[1] = (t[0].float() * kscale).half(), (t[1].float() * vscale).half()
+    qkv[..., 4 * S:6 * S] *= kscale
+    qkv[..., 6 * S:] *= vscale
+    _check(qkv, 4, 2, prefix, P, cache, lengths, None)

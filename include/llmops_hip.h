@@ -308,8 +308,9 @@ int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_s
  * lora_A [adapters,R,K] and lora_B [adapters,N,R], dense, of weight_dtype (LLMOPS_F32, _F16, _BF16); scales fp32 [adapters] and ids
  * int32 [batch] on the device.  An id outside 0 .. adapters-1 (-1) is none: out = y.  Adapters of a lower rank than R are padded with
  * zeros.  x [batch,tokens,K], y and out [batch,tokens,N] fp32, token l of sequence b at + b*stride_b + l*stride_l elements; out may be y
- * (the same pointer and strides) and must not overlap x or y otherwise.  Up to 2^20 tokens in all, R up to 4096, N and K
- * below 2^29; other sizes and the strides are free.
+ * (the same pointer and strides).  Refused: an out whose rows lie over each other, over x's or, otherwise, over y's (columns of one wider
+ * tensor do not; where spans meet, an out whose rows are not one behind the other counts as lying over).  Up to 2^20 tokens in all, R up to
+ * 4096, N and K below 2^29; other sizes and the strides are free.
  * fp32 arithmetic, except that products are formed of exact bf16 pieces: what is dropped is below 2^-22 of a product, and an infinity
  * among a sequence's x or its adapter's weights leaves NaN in what depends on it. */
 size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R, int64_t adapters);

@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "extents.h"
 
 namespace llmops {
 
@@ -591,6 +592,13 @@ extern "C" int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_str
     if (workspace == nullptr || workspace_bytes < need)
         return fail(LLMOPS_EWORKSPACE, "lora_add needs %zu workspace bytes, got %zu", need, workspace == nullptr ? (size_t)0 : workspace_bytes);
     LLMOPS_REQUIRE(aligned(workspace, 4));
+    // (a workgroup reads its x and y while others may have written their out)
+    const Extent out_rows(out, batch, (Wide)out_stride_b * 4, tokens, (Wide)out_stride_l * 4, (Wide)N * 4),
+        y_rows(y, batch, (Wide)y_stride_b * 4, tokens, (Wide)y_stride_l * 4, (Wide)N * 4), x_rows(x, batch, (Wide)x_stride_b * 4, tokens, (Wide)x_stride_l * 4, (Wide)K * 4);
+    const bool in_place = out == y && (batch == 1 || out_stride_b == y_stride_b) && (tokens == 1 || out_stride_l == y_stride_l);
+    LLMOPS_REQUIRE(rows_apart(out_rows));
+    LLMOPS_REQUIRE(apart(out_rows, x_rows));
+    LLMOPS_REQUIRE(in_place || apart(out_rows, y_rows));
     LoraArgs a{};
     a.x = x, a.y = y, a.scales = scales, a.A = lora_A, a.B = lora_B, a.ids = ids, a.out = out, a.part = reinterpret_cast<float*>(workspace);
     a.xsb = x_stride_b, a.xsl = x_stride_l, a.ysb = y_stride_b, a.ysl = y_stride_l, a.osb = out_stride_b, a.osl = out_stride_l;

@@ -602,7 +602,7 @@ def lora_add(y, x, lora_A, lora_B, adapters, scales, out=None):
     y fp32 [B,M,N], x fp32 [B,M,K] (inner dimension dense, any strides: columns of a fused projection's output will do); lora_A [n,R,K]
     and lora_B [n,N,R] (fp32, fp16 or bf16) hold n adapters, those of a lower rank padded with zeros; adapters int32 [B] and scales fp32
     [n] on the device.  An adapter outside 0 .. n-1 (-1) is none: the sequence keeps its y.  Returns a new tensor, or ``out`` [B,M,N],
-    which may be y itself and must not overlap x or y otherwise."""
+    which may be y itself; one that lies over x, or over y otherwise, is refused."""
     if out is None:
         done = (_lib._host or _lib.host()).lora_add(y, x, lora_A, lora_B, adapters, scales)
         if done is not NotImplemented:  # (as above)

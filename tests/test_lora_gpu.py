@@ -167,3 +167,33 @@ def test_offsets_past_32_bits():
     out = llmops.lora_add(y.cuda().expand(B, M, N), x, A.cuda(), W.cuda(), ids.cuda(), scales.cuda())
     _check(out[B - 1:], y, _delta(x1, A, W, ids[:1], scales))
     assert torch.equal(out[:B - 1], y.cuda().expand(B - 1, M, N))
+
+
+def test_x_y_and_out_beside_each_other_in_one_tensor():
+    """columns of one wide tensor, and sequences between each other's: nothing lies over anything"""
+    y, x, A, W, ids, scales = _case(4, 3, 96, 160, 16, 3, "fp16", seed=7)
+    d = _delta(x, A, W, ids, scales)
+    rest = [t.cuda() for t in (A, W, ids, scales)]
+    for at_y, at_x, at_out in ((0, 96, 256), (0, 96, 0), (160, 0, 256), (256, 0, 160), (160, 0, 160)):
+        wide = torch.randn(4, 3, 352).cuda()
+        wide[..., at_y:at_y + 96], wide[..., at_x:at_x + 160] = y.cuda(), x.cuda()
+        before = wide.clone()
+        out = wide[..., at_out:at_out + 96]
+        assert llmops.lora_add(wide[..., at_y:at_y + 96], wide[..., at_x:at_x + 160], *rest, out=out) is out
+        _check(out, y, d)
+        before[..., at_out:at_out + 96] = out
+        assert torch.equal(wide, before)
+    flat = torch.zeros(4, 3, 2, 160).cuda()  # out's rows between x's
+    flat[:, :, 0] = x.cuda()
+    _check(llmops.lora_add(y.cuda(), flat[:, :, 0], *rest, out=flat[:, :, 1, 64:]), y, d)
+
+
+def test_outputs_over_inputs_are_refused():
+    y, x, A, W, ids, scales = (t.cuda() for t in _case(2, 2, 32, 48, 8, 2, "fp16", seed=1))
+    some = torch.zeros(2, 2, 100, device="cuda")
+    for args in ((some[..., :32], x, some[..., 4:36]), (y, some[..., 10:58], some[..., 50:82]), (some[..., :32], x, some.flatten()[:128].view(2, 2, 32)),
+                 (y, some[..., :48], some.flatten()[96:224].view(2, 2, 32)), (some[:1, :, :32].expand(2, -1, -1), x, some[..., :32])):
+        before = some.clone()
+        with pytest.raises(RuntimeError, match="apart"):
+            llmops.lora_add(args[0], args[1], A, W, ids, scales, out=args[2])
+        assert torch.equal(some, before)

@@ -137,3 +137,19 @@ def test_attention_rope_prefix_up_to_the_last_position(lib, prefix, maxlen):
     _refused(lib, _prefix(lib, **kw), b"workspace bytes", 2)
     kw["maxlen"] += 1
     _refused(lib, _prefix(lib, **kw), b"prefix_sizes_fit")
+
+
+@pytest.mark.parametrize("kw,what", [
+    # (y, x and out: 4 sequences of 2 tokens, 100 fp32 values apart each way unless said; y and out 64 wide, x 96)
+    (dict(), b"rows_apart(out_rows)"), (dict(ob=200, ol=63), b"rows_apart(out_rows)"), (dict(ob=0, ol=64), b"rows_apart(out_rows)"), (dict(ob=64, ol=64), b"rows_apart(out_rows)"),
+    (dict(ob=200), b"apart(out_rows, x_rows)"), (dict(ob=200, yb=200), b"apart(out_rows, x_rows)"),
+    (dict(ob=400, ol=200, yb=400, yl=200, xb=400, xl=200, x=ctypes.c_void_p(4096 + 4 * 63)), b"apart(out_rows, x_rows)"),
+    (dict(ob=400, ol=200, yb=400, yl=200, xb=400, xl=200, x=ctypes.c_void_p(4096 + 4 * 110)), b"apart(out_rows, x_rows)"),
+    (dict(ob=400, ol=200, yb=400, yl=200, xb=0, xl=0, x=ctypes.c_void_p(4096 + 4 * 1390)), b"apart(out_rows, x_rows)"),
+    (dict(ob=200, yb=201, x=ctypes.c_void_p(1 << 20)), b"in_place || apart(out_rows, y_rows)"),
+    (dict(ob=200, yb=200, x=ctypes.c_void_p(1 << 20), y=ctypes.c_void_p(4100)), b"in_place || apart(out_rows, y_rows)"),
+    (dict(ob=200, yb=200, x=ctypes.c_void_p(1 << 20), y=ctypes.c_void_p(4096 + 4 * 363)), b"in_place || apart(out_rows, y_rows)"),
+    (dict(B=1, M=1, x=ctypes.c_void_p(1 << 20), y=ctypes.c_void_p(4096 - 4 * 63)), b"in_place || apart(out_rows, y_rows)"),
+])
+def test_lora_add_refuses_an_output_over_its_inputs(lib, kw, what):
+    _refused(lib, _lora(lib, **kw), what)

@@ -294,7 +294,7 @@ int llmops_attention_rope_decode_records(float* q, float* k, const float* v, int
  * inv_freq * position keeps the product's rounding error, which fp32 loses (1e-4 at position 4000).  S == 128; 16-byte aligned
  * pointers, 256-byte aligned workspace; prefix_len + maxlen <= 2^24, and each launch
  * below 2^24 workgroups, as it is while B*qL*H * (2 + maxlen/1024) is.  prefix_len may be 0 (prefix_cache may then be NULL).
- * prefix_cache and kv_cache must not overlap.
+ * Refused: caches that overlap, an out over q, k, v or the layer's planes, q, k or v over the planes that take the new rows.
  * Results agree with fp32 evaluation to about 1e-6 of the largest output, and are the same bits in every call. */
 size_t llmops_attention_prefix_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t prefix_len, int64_t maxlen);
 int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b,

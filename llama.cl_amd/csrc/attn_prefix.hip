@@ -28,6 +28,7 @@
 #include <float.h>
 
 #include "common.h"
+#include "extents.h"
 #include "gemv_device.h"
 
 namespace llmops {
@@ -1199,6 +1200,13 @@ static int prefix_launch(PrefixArgs a, PrepArgs p, const PrefixPlan& plan, hipSt
     const int64_t prep = (int64_t)a.B * a.qL * p.groups, items = (int64_t)a.pitems + (int64_t)a.B * a.Hkv * a.otiles * a.opieces,
                   merge = ((int64_t)a.Hkv * a.M + 7) / 8, most = (int64_t)1 << 24;  // (a launch has fewer than 2^32 threads)
     LLMOPS_REQUIRE(prep < most && items < most && merge < most);
+    // (a workgroup reads its q, k and v while others may have written their rows and results)
+    const Wide heads = (Wide)a.G * a.Hkv * kS * 4, kv_heads = (Wide)a.Hkv * kS * 4, plane = (Wide)a.Hkv * kS * sizeof(T);
+    const Extent q(p.q, a.B, (Wide)p.qsb * 4, a.qL, (Wide)p.qsl * 4, heads), k(p.k, a.B, (Wide)p.ksb * 4, a.qL, (Wide)p.ksl * 4, kv_heads),
+        v(p.v, a.B, (Wide)p.vsb * 4, a.qL, (Wide)p.vsl * 4, kv_heads), out(a.out, (Wide)a.B * a.qL * heads), own(a.ok, 2 * a.B * a.maxlen * plane),
+        prefix(a.pk, a.P > 0 ? 2 * a.pmax * plane : 0);
+    LLMOPS_REQUIRE(apart(own, q) && apart(own, k) && apart(own, v));
+    LLMOPS_REQUIRE(apart(out, q) && apart(out, k) && apart(out, v) && apart(out, own) && apart(out, prefix));
     if (!plan.self) prefix_prep_kernel<T><<<(unsigned)prep, 256, 0, st>>>(a, p);
     LLMOPS_LAUNCH_CHECK();
     const unsigned grid = (unsigned)items;

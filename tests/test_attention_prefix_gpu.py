@@ -430,3 +430,19 @@ def test_halves_below_their_normal_range(L, P, kscale, vscale, qscale):
     qkv[..., 4 * S:6 * S] *= kscale
     qkv[..., 6 * S:] *= vscale
     _check(qkv, 4, 2, prefix, P, cache, lengths, None)
+
+
+def test_inputs_over_the_new_rows_are_refused():
+    qkv, prefix, cache, lengths, _ = _case(2, 2, 4, 2, 10, 8, False, seed=1, layers=2)
+    q, k, v = (t.contiguous() for t in _split(qkv.cuda(), 4, 2))
+    f, prefix, cache, n = _inv_freq().cuda(), prefix.cuda(), cache.cuda(), lengths.cuda()
+    before = cache.clone()
+    inside = cache[0].flatten()[:2 * 2 * 2 * S].view(2, 2, 2 * S)
+    for kw in (dict(k=inside), dict(v=inside), dict(q=cache[1].flatten()[:2 * 2 * 4 * S].view(2, 2, 4 * S))):
+        with pytest.raises(RuntimeError, match="apart"):
+            llmops.attention_rope_prefix(**{**dict(q=q, k=k, v=v, inv_freq=f, prefix_cache=prefix, prefix_len=10, kv_cache=cache, lengths=n, layer_id=0), **kw})
+    assert torch.equal(cache, before)
+    # the other layer's planes are nobody's now
+    k2 = cache[2].flatten()[:2 * 2 * 2 * S].view(2, 2, 2 * S)
+    want = llmops.attention_rope_prefix(q, k2.clone(), v, f, prefix, 10, cache.clone(), n, 0)
+    assert torch.equal(llmops.attention_rope_prefix(q, k2, v, f, prefix, 10, cache, n, 0), want)

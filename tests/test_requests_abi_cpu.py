@@ -153,3 +153,17 @@ def test_attention_rope_prefix_up_to_the_last_position(lib, prefix, maxlen):
 ])
 def test_lora_add_refuses_an_output_over_its_inputs(lib, kw, what):
     _refused(lib, _lora(lib, **kw), what)
+
+
+@pytest.mark.parametrize("kw,what", [
+    # q [2, 3, 32 heads] and out dense, k and v [2, 3, 8 heads], cache [2, 2, 8, 64, 128]: 2 * 8 * 64 * 128 = 2^17 values a plane, 2^18 a layer
+    (dict(kv=ctypes.c_void_p((1 << 30) - 4 * (1 << 18) + 16)), b"apart(own, q)"), (dict(k=ctypes.c_void_p((1 << 40) + 4 * ((1 << 18) - 4))), b"apart(own, k)"),
+    (dict(v=ctypes.c_void_p((1 << 40) - 4 * (5 * 1024 + 1024 - 4)), vb=3072, vl=1024), b"apart(own, v)"), (dict(layer=1, planes=4, pplanes=4, v=ctypes.c_void_p((1 << 40) + 4 * (1 << 18))), b"apart(own, v)"),
+    (dict(out=ctypes.c_void_p(1 << 30)), b"apart(out, q)"), (dict(out=ctypes.c_void_p((1 << 30) + 4 * 4092), qb=12288), b"apart(out, q)"),
+    (dict(out=ctypes.c_void_p((1 << 31) + 4 * 1020)), b"apart(out, k)"), (dict(out=ctypes.c_void_p((1 << 32) - 16)), b"apart(out, v)"),
+    (dict(out=ctypes.c_void_p(1 << 40)), b"apart(out, own)"), (dict(out=ctypes.c_void_p(4096)), b"apart(out, prefix)"),
+])
+def test_attention_rope_prefix_refuses_outputs_over_inputs(lib, kw, what):
+    a = dict(q=ctypes.c_void_p(1 << 30), k=ctypes.c_void_p(1 << 31), v=ctypes.c_void_p(1 << 32), out=ctypes.c_void_p(1 << 33))
+    a.update(kw)
+    _refused(lib, _prefix(lib, **a), what)

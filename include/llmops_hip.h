@@ -332,7 +332,7 @@ int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, cons
  * Logits that are NaN or minus infinity weigh nothing, equal plus infinities share the row; a row without any other logit gives -1.
  * Exponentials and sums are in 64 bits: the answer is the definition's but for numbers within about 1e-13 (at a temperature below 1e-3 of
  * the largest logit: 2e-16 of their ratio) of a border.
- * B*(K+1) < 2^24, V <= 2^27, B * ceil(V / 4096) < 2^23. */
+ * B*(K+1) < 2^24, V <= 2^27, B * ceil(V / 4096) < 2^23.  Outputs that lie over each other or over inputs are refused. */
 size_t llmops_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
 int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, int64_t V, const int64_t* drafts, const float* draft_probs,
                          const float* uniforms, const float* temperature, float one_temperature, const int32_t* draft_lens, int64_t* tokens,

@@ -16,6 +16,7 @@
 #include <math.h>
 
 #include "common.h"
+#include "extents.h"
 
 namespace llmops {
 
@@ -445,6 +446,20 @@ extern "C" int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, i
     if (workspace == nullptr || workspace_bytes < w.total)
         return fail(LLMOPS_EWORKSPACE, "verify_drafts needs %zu workspace bytes, got %zu", w.total, workspace == nullptr ? (size_t)0 : workspace_bytes);
     LLMOPS_REQUIRE(aligned(workspace, 16));
+    // (a workgroup reads a sequence's drafts and lengths while another may have written its answer)
+    const Wide rows = (Wide)B * (K + 1);
+    const Extent first(tokens, rows * 8), second(accepted, B * 4), drafts_at(drafts, (Wide)B * K * 8), logits_at(logits, rows * V * 4),
+        random_at(uniforms, rows * 4), probs_at(draft_probs, draft_probs != nullptr ? (Wide)B * K * V * 4 : 0),
+        temperatures_at(temperature, temperature != nullptr ? B * 4 : 0), lens_at(draft_lens, draft_lens != nullptr ? B * 4 : 0);
+    LLMOPS_REQUIRE(apart(first, second));
+    for (const Extent& out : {first, second}) {
+        LLMOPS_REQUIRE(apart(out, drafts_at));
+        LLMOPS_REQUIRE(apart(out, logits_at));
+        LLMOPS_REQUIRE(apart(out, random_at));
+        LLMOPS_REQUIRE(apart(out, probs_at));
+        LLMOPS_REQUIRE(apart(out, temperatures_at));
+        LLMOPS_REQUIRE(apart(out, lens_at));
+    }
     char* ws = reinterpret_cast<char*>(workspace);
     a.logits = logits, a.probs = draft_probs, a.uniforms = uniforms, a.temperature = temperature, a.drafts = drafts, a.draft_lens = draft_lens;
     a.one_temperature = one_temperature;

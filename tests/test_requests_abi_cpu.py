@@ -167,3 +167,14 @@ def test_attention_rope_prefix_refuses_outputs_over_inputs(lib, kw, what):
     a = dict(q=ctypes.c_void_p(1 << 30), k=ctypes.c_void_p(1 << 31), v=ctypes.c_void_p(1 << 32), out=ctypes.c_void_p(1 << 33))
     a.update(kw)
     _refused(lib, _prefix(lib, **a), what)
+
+
+@pytest.mark.parametrize("kw,what", [
+    # 2 sequences, 3 drafts, 100 tokens: logits [2, 4, 100], probabilities [2, 3, 100], tokens [2, 4] int64
+    (dict(d=1 << 20), b"apart(out, drafts_at)"), (dict(d=(1 << 20) - 40), b"apart(out, drafts_at)"), (dict(z=(1 << 20) - 3196), b"apart(out, logits_at)"), (dict(u=(1 << 20) + 60), b"apart(out, random_at)"),
+    (dict(q=(1 << 20) - 2396), b"apart(out, probs_at)"), (dict(t=(1 << 21) + 4), b"apart(out, temperatures_at)"), (dict(n=1 << 21), b"apart(out, lens_at)"), (dict(accepted=(1 << 20) + 60), b"apart(first, second)"),
+])
+def test_verify_drafts_refuses_outputs_over_inputs(lib, kw, what):
+    at = dict(z=1 << 30, d=1 << 31, q=1 << 32, u=1 << 33, t=1 << 34, n=1 << 35, tokens=1 << 20, accepted=1 << 21)
+    at.update(kw)
+    _refused(lib, _verify(lib, **{name: ctypes.c_void_p(x) for name, x in at.items()}), what)

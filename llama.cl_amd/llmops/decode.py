@@ -329,17 +329,20 @@ class LlamaDecoder:
     def step_requests(self, tokens, cache, uniforms, drafts=None, draft_probs=None, draft_lens=None, temperature=None, adapters=None):
         """One step of several requests: each sequence's last token (``tokens`` int64 [B], not yet in the cache) and its K drafted ones
         (``drafts`` int64 [B, K]; None: none) go through the model, the drafts are checked and the token behind those accepted is drawn
-        (``llmops.verify_drafts`` for the other arguments), and the rows of what was accepted are kept in the cache, which must have room for
-        1 + K (or 1 + draft_lens) of them in each sequence whose answer is used.  Returns its (tokens
+        (``llmops.verify_drafts`` for the other arguments), and the rows of what was accepted are kept in the cache.  Drafts that no longer
+        fit the cache are not judged; a sequence without a row left for its token answers -1.  Returns its (tokens
         [B, K+1], accepted [B]): ``tokens`` of the next step is ``result.gather(1, accepted[:, None].long())[:, 0]``."""
         B = tokens.shape[0]
         if drafts is None:
             drafts = torch.empty((B, 0), dtype=torch.int64, device=tokens.device)
+        K = drafts.shape[1]
         # (a draft that is no token, padding among them, is refused by the check: any row of the table will do for it)
         ids = torch.cat((tokens[:, None], drafts), dim=1).clamp(0, self.embed_tokens.weight.shape[0] - 1)
-        q_lens = None if draft_lens is None else draft_lens.clamp(0, drafts.shape[1]) + 1
+        room = cache.max_kv_len - cache.lengths
+        q_lens = room.clamp(max=K + 1) if draft_lens is None else torch.minimum(draft_lens.clamp(0, K) + 1, room)
         logits = self.forward_requests(ids, cache, q_lens, adapters)
-        result, accepted = llmops.verify_drafts(logits, drafts, uniforms, draft_probs=draft_probs, temperature=temperature, draft_lens=draft_lens)
+        result, accepted = llmops.verify_drafts(logits, drafts, uniforms, draft_probs=draft_probs, temperature=temperature, draft_lens=q_lens - 1)
+        result.masked_fill_((room <= 0)[:, None], -1)
         cache.keep(accepted + 1)
         return result, accepted
 

@@ -221,3 +221,32 @@ def test_a_captured_step_serves_the_following_ones():
         drafts.copy_(_ids(20 + step, 4, 2))
         uniforms.copy_((uniforms * 3.7) % 1.0)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("given", [None, [2, 4, 4, 1]])
+def test_a_step_at_the_end_of_the_cache(given):
+    """drafts that no longer fit are not judged, and a sequence without room for its token gives none; the others are as they are"""
+    model = LlamaDecoder(CFG, seed=9)
+    cache, other = (model.request_cache(4, 9, model.read_prefix(_ids(1, 1, 11))) for _ in range(2))
+    said = torch.tensor([0, 5, 8, 9], dtype=torch.int32).cuda()
+    model.forward_requests(_ids(2, 4, 9), cache, said)
+    cache.keep(said)
+    other.cache.copy_(cache.cache), other.lengths.copy_(cache.lengths)
+    tokens, drafts = _ids(3, 4), _ids(4, 4, 4)
+    uniforms = torch.zeros(4, 5).cuda()  # (every draft that is judged is accepted)
+    uniforms[:, 4] = 0.4
+    lens = None if given is None else torch.tensor(given, dtype=torch.int32).cuda()
+    fit = [4, 3, 0, 0] if given is None else [2, 3, 0, 0]
+    result, accepted = model.step_requests(tokens, cache, uniforms, drafts, draft_lens=lens)
+    assert accepted.tolist() == fit and cache.lengths.tolist() == [fit[0] + 1, 9, 9, 9]
+    assert (result[3] == -1).all()
+    for b in range(3):
+        n = fit[b]
+        assert torch.equal(result[b, :n], drafts[b, :n]) and 0 <= int(result[b, n]) < CFG["vocab_size"] and (result[b, n + 1:] == -1).all()
+    want, _ = model.step_requests(tokens, other, uniforms, drafts, draft_lens=torch.tensor(fit, dtype=torch.int32).cuda())
+    assert torch.equal(result, want) and torch.equal(cache.cache, other.cache)
+    # a token that was not given goes nowhere
+    before = cache.cache.clone()
+    result, accepted = model.step_requests(result.gather(1, accepted[:, None].long())[:, 0], cache, uniforms[:, :1].contiguous())
+    assert (result[1:] == -1).all() and accepted.tolist() == [0] * 4 and int(result[0, 0]) >= 0 and cache.lengths.tolist() == [fit[0] + 2, 9, 9, 9]
+    assert torch.equal(cache.cache[:, 1:], before[:, 1:])

@@ -42,8 +42,11 @@ def sources():
 # Kernels that must compile without VGPR spills: the one-row group-128 decode kernels are written to fit
 # the 64 registers that two 16-wave workgroups per CU leave each wave, and scratch traffic in their loop
 # costs what the rewrite gained; the prompt attention kernel likewise (a reload in its loop waits for the
-# next tile's loads), and so the tiled GEMM (a reload waits for the next k-group's copies).
-NO_SPILL = ["fc_gemv_fused_kernelILi128ELi1E", "attn_prefill_kernel", "fc_gemm_tile_kernel"]
+# next tile's loads), and so the tiled GEMM (a reload waits for the next k-group's copies); likewise the kernels of several
+# requests in step, but for prefix_apart_kernel<float, 2, false, false> (9 registers, 40 bytes of scratch a lane).
+NO_SPILL = ["fc_gemv_fused_kernelILi128ELi1E", "attn_prefill_kernel", "fc_gemm_tile_kernel", "prefix_brief_kernel", "prefix_sweep_kernel",
+            "prefix_apart_kernelI6__half", "prefix_apart_kernelIfLi1E", "prefix_apart_kernelIfLi2ELb1E", "lora_down_kernel", "lora_up_kernel",
+            "verify_rows_kernel", "verify_next_kernel"]
 
 
 def check_spills(remarks):

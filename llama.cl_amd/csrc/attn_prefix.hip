@@ -197,7 +197,6 @@ struct Rows {
     __device__ __forceinline__ buffer_rsrc from(int t) const {
         return make_rsrc(p + (int64_t)t * kS, (uint32_t)__builtin_amdgcn_readfirstlane(max(0, min(32, end - t))) * (uint32_t)(kS * sizeof(T)));
     }
-    __device__ __forceinline__ const T* at(int r) const { return p + (int64_t)min(r, end - 1) * kS; }
 };
 
 struct Halves {

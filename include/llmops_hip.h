@@ -284,18 +284,23 @@ int llmops_attention_rope_decode_records(float* q, float* k, const float* v, int
  * with q_lens, q_lens[b] of the qL; token l < t[b] has position prefix_len + n[b] + l.  Its k (rotated) and v go to row n[b] + l, and
  *   out[b,l] = softmax(rot(q).K^T / sqrt(S)) . V over rows 0 .. prefix_len-1 of prefix_cache [prefix_planes,1,Hkv,prefix_maxlen,S] and
  * rows 0 .. n[b]+l of its own; head h reads kv head h / (H / Hkv).  Planes 2*layer_id and 2*layer_id+1 of both caches; both have the
- * type cache_dtype (halves: k and v are rounded to them, the arithmetic is fp32).  The caller adds t[b] to lengths[b] when all layers
+ * type cache_dtype (halves: k and v are rounded to them).  The caller adds t[b] to lengths[b] when all layers
  * are done, or less: rows past lengths[b] are not looked at, and the next call's tokens overwrite them.
  *   lengths, q_lens are int32 [B] on the device (q_lens may be NULL: qL each), read by the kernels: a captured call serves every
  * following step.  A length outside 0 .. maxlen counts as the nearer of the two, and new tokens that do not fit the cache count as
  * padding.  Padding (l >= t[b]) is not cached, and its out is 0.
  *   q [B,qL,H*S], k and v [B,qL,Hkv*S] fp32, token l of sequence b at + b*stride_b + l*stride_l elements (multiples of 4: columns of a
  * projection's output will do), unchanged; out [B,qL,H*S] dense.  inv_freq [half], 2*half <= S: as llmops_rope_embed, but the angle
- * inv_freq * position keeps the product's rounding error, which fp32 loses (1e-4 at position 4000).  S == 128; 16-byte aligned
+ * inv_freq * position is formed in 64 bits (in fp32 it is off by 1e-4 at position 4000): cosines and sines to 2.4e-7 everywhere.  S == 128; 16-byte aligned
  * pointers, 256-byte aligned workspace; prefix_len + maxlen <= 2^24, and each launch
  * below 2^24 workgroups, as it is while B*qL*H * (2 + maxlen/1024) is.  prefix_len may be 0 (prefix_cache may then be NULL).
  * Refused: caches that overlap, an out over q, k, v or the layer's planes, q, k or v over the planes that take the new rows.
- * Results agree with fp32 evaluation to about 1e-6 of the largest output, and are the same bits in every call. */
+ * Arithmetic: products of halves, two to an fp32 value, with fp32 sums.  That leaves 22 bits of a query beside its head's largest value, 21 of
+ * a K or V of 2^-14 and more, and 2^-36 of smaller ones, however few of their bits that is (a column of V near 1e-6 beside others near 1 is
+ * right to 1.5e-5 of itself; 2^-38 for halves): fewer than llmops_attention_rope keeps below 32 tokens.  Rows that hold values of 65504 and
+ * more, infinities or NaN, or whose K or V has nothing of 2^-14 and more, are multiplied in full width by the workgroups that meet them, up
+ * to 70 times slower.  Results agree with fp32 evaluation to about 1e-6 of the largest output, and 2^-36 beside it, and are the same bits in
+ * every call. */
 size_t llmops_attention_prefix_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t prefix_len, int64_t maxlen);
 int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b,
                                  int64_t k_stride_l, const float* v, int64_t v_stride_b, int64_t v_stride_l, int64_t B, int64_t qL,
@@ -311,7 +316,8 @@ int llmops_attention_rope_prefix(const float* q, int64_t q_stride_b, int64_t q_s
  * (the same pointer and strides).  Refused: an out whose rows lie over each other, over x's or, otherwise, over y's (columns of one wider
  * tensor do not; where spans meet, an out whose rows are not one behind the other counts as lying over).  Up to 2^20 tokens in all, R up to
  * 4096, N and K below 2^29; other sizes and the strides are free.
- * fp32 arithmetic, except that products are formed of exact bf16 pieces: what is dropped is below 2^-22 of a product, and an infinity
+ * fp32 arithmetic, except that products are formed of exact bf16 pieces: what is dropped is below 2^-21 of a product with fp32 weights, 2^-22
+ * with fp16 and nothing with bf16; pieces and products below 2^-126 count as 0 (a delta near 1e-36 is right to 1e-4 of itself); and an infinity
  * among a sequence's x or its adapter's weights leaves NaN in what depends on it. */
 size_t llmops_lora_workspace_bytes(int64_t batch, int64_t tokens, int64_t N, int64_t K, int64_t R, int64_t adapters);
 int llmops_lora_add(const float* y, int64_t y_stride_b, int64_t y_stride_l, const float* x, int64_t x_stride_b, int64_t x_stride_l,

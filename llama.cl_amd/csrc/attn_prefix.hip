@@ -148,7 +148,7 @@ __device__ __forceinline__ void store_row(T* dst, int d, const float (&x)[8]) {
 }
 
 // Before the launches whose workgroups do not rotate for themselves.  A workgroup per token and 16 of its H + 2*Hkv rows of 128.  Bound by latency
-// at few tokens (64 of 48 rows: 5 us) and by memory at many (4 x 300 of 96 rows, a quarter padding: 20 us, 71 MB to and from HBM).
+// at few tokens (64 of 48 rows: 5 us) and by memory at many (4 x 300 of 96 rows, a quarter padding: 20 us, 76 MB to and from HBM).
 template <typename T>
 __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a, PrepArgs p) {
     __shared__ float2 turn[64];
@@ -401,7 +401,9 @@ __device__ __forceinline__ int rows_seen(const PrefixArgs& a, int m, int b, int 
 }
 
 // The same in full width, for rows that hold values outside the halves' range: the workgroup starts again, half a wave to a query and
-// four dims to a lane, only the rows that the query sees, in up to two runs (prefix, own).  Slow, and not met in a model's caches.
+// four dims to a lane, only the rows that the query sees, in up to two runs (prefix, own).  Slow, and not met in a model's caches: with one value
+// outside in the prefix a call takes 56 us instead of 16 (2 sequences behind 130 rows), 1.9 ms instead of 59 us (16 of 5 tokens behind 1500), 0.9 ms
+// instead of 43 us (32 behind 2048, halves), 13 ms instead of 193 us (4 of 300 tokens behind 1000).
 // sixteen queries in LDS: hi of step 0..3, lo of step 0..3, 16 bytes to a lane; where (in halves) the hi of dims d .. of query i is
 __device__ __forceinline__ int held_at(int i, int d) { return ((d >> 5) * 64 + ((d >> 3) & 3) * 16 + i) * 8 + (d & 7); }
 struct HeldQueries {  // in LDS: (16-byte pieces as the operands lie, factors), or null: in memory

@@ -9,8 +9,9 @@
 // requests.  One adapter in a tile is read once for all; sixteen are read once each, which they must be anyway.
 //
 // Products run on the bf16 matrix cores (v_mfma_f32_16x16x32_bf16, fp32 sums) on exact pieces: an fp32 value is three bf16 values
-// (8 bits each, cut off), an fp16 weight two, a bf16 weight itself.  Products of pieces whose places sum to three or less are
-// formed; what is dropped is below 2^-22 of a product.
+// (8 bits each, cut off), an fp16 weight two, a bf16 weight itself.  Products of pieces whose places (0 to 2) sum to two or less are
+// formed.  A piece is below 2^-7 of the one before it, the third below 2^-15 of the first: what is dropped is below 2 * 2^-22 of a product with
+// fp32 weights, 2^-22 with fp16, nothing with bf16.
 #include <algorithm>
 
 #include "common.h"

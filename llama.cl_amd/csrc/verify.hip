@@ -65,7 +65,7 @@ __device__ __forceinline__ double power_of_two(double y) {
     return ldexp(p, (int)whole);
 }
 // exp((z - top) / T), per_t = log2(e) / T: 1 at the maximum, infinite or not; 0 for minus infinity and NaN, and everywhere in a row without
-// a value above minus infinity.  (Twenty instructions an element, the least that were found: they are most of the first launch.  The
+// a value above minus infinity.  (Twenty instructions an element, two thirds of what the first launch issues.  The
 // rounding of `shift` is the same in all of a row's weights.)
 struct Weigher {
     float one;  // the logit that weighs 1; NaN: none
@@ -121,8 +121,9 @@ __device__ __forceinline__ uint32_t wave_least(uint32_t v) {
 }
 constexpr uint32_t kNowhere = 0x7fffffff;
 
-// A workgroup: 4096 logits of a row.  Bound by the vector ALU in 64 bits (160 rows of 55296: 35 MB in 11.6 us, 3.0 TB/s; 24 instructions an element, most
-// of them at half rate), by latency with few rows (5 of 55296: 4.6 us).
+// A workgroup: 4096 logits of a row.  Bound by loads and then the vector ALU in 64 bits, one behind the other, since all workgroups start at
+// once (128 rows of 55296, a quarter at temperature 0: 28 MB in 11.3 us, 2.5 TB/s; 31 instructions a logit, most of them at half rate), by latency
+// with few rows (4 of 55296: 3.8 us).
 __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     __shared__ float tops[4];
     __shared__ uint32_t places[4];

@@ -330,7 +330,7 @@ class LlamaDecoder:
         """One step of several requests: each sequence's last token (``tokens`` int64 [B], not yet in the cache) and its K drafted ones
         (``drafts`` int64 [B, K]; None: none) go through the model, the drafts are checked and the token behind those accepted is drawn
         (``llmops.verify_drafts`` for the other arguments), and the rows of what was accepted are kept in the cache.  Drafts that no longer
-        fit the cache are not judged; a sequence without a row left for its token answers -1.  Returns its (tokens
+        fit the cache are not checked; a sequence without a row left for its token answers -1.  Returns its (tokens
         [B, K+1], accepted [B]): ``tokens`` of the next step is ``result.gather(1, accepted[:, None].long())[:, 0]``."""
         B = tokens.shape[0]
         if drafts is None:

@@ -225,7 +225,7 @@ def test_a_captured_step_serves_the_following_ones():
 
 @pytest.mark.parametrize("given", [None, [2, 4, 4, 1]])
 def test_a_step_at_the_end_of_the_cache(given):
-    """drafts that no longer fit are not judged, and a sequence without room for its token gives none; the others are as they are"""
+    """drafts that no longer fit are not checked, and a sequence without room for its token gives none; the others are as they are"""
     model = LlamaDecoder(CFG, seed=9)
     cache, other = (model.request_cache(4, 9, model.read_prefix(_ids(1, 1, 11))) for _ in range(2))
     said = torch.tensor([0, 5, 8, 9], dtype=torch.int32).cuda()
@@ -233,7 +233,7 @@ def test_a_step_at_the_end_of_the_cache(given):
     cache.keep(said)
     other.cache.copy_(cache.cache), other.lengths.copy_(cache.lengths)
     tokens, drafts = _ids(3, 4), _ids(4, 4, 4)
-    uniforms = torch.zeros(4, 5).cuda()  # (every draft that is judged is accepted)
+    uniforms = torch.zeros(4, 5).cuda()  # (every draft that is checked is accepted)
     uniforms[:, 4] = 0.4
     lens = None if given is None else torch.tensor(given, dtype=torch.int32).cuda()
     fit = [4, 3, 0, 0] if given is None else [2, 3, 0, 0]

@@ -344,6 +344,54 @@ int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, int64_t V, c
                          const float* uniforms, const float* temperature, float one_temperature, const int32_t* draft_lens, int64_t* tokens,
                          int32_t* accepted, void* workspace, size_t workspace_bytes, llmops_stream_t stream);
 
+/* A key/value cache in 4 bits: kv_cache int8 [planes,B,Hkv,maxlen,LLMOPS_Q4_ROW_BYTES], planes 2*layer and 2*layer+1 as in the other caches, a
+ * row the S = 128 values of a token and kv head as four groups of 32 values x one behind the other.  With u the smallest power of two from
+ * 2^-24 on for which max |x| <= 2032 u, lo = round(min x / u), hi = round(max x / u) and s = ceil((hi - lo) / 15), a group is the halves
+ * d = s u and m = lo u and for each value the code round((x / u - lo) / s), 0 to 15 (roundings to even); it stands for d code + m, which is a
+ * half, exactly.  Bytes 16 g .. of a row: group g's codes, eight in a word of 32 bits, code i at bit 4 (i / 2) + 16 (i % 2); bytes 64 + 4 g ..: d and
+ * m.  A row that is given NaN or a magnitude above 65024 stands for NaN throughout; 80 zero bytes stand for zeros. */
+#define LLMOPS_Q4_ROW_BYTES 80
+
+/* New rows of a cache in 4 bits: token l < t[b] of sequence b, t[b] = qL or q_lens[b] of the qL, goes to row lengths[b] + l of planes 2*layer_id (k) and
+ * 2*layer_id+1 (v).  k and v are of `dtype` (LLMOPS_F32, _F16), head h of token l of sequence b at + b*stride_b + l*stride_l + h*stride_h elements
+ * (multiples of 16 bytes; 0 where rows are the same), unchanged.  With inv_freq [half] k is rotated by its row's number first, as
+ * llmops_rope_embed with angles, rotation and codes in 64 bits; NULL: k comes rotated.  lengths, q_lens, and tokens that do not fit: as llmops_attention_rope_prefix.
+ * The caller adds to lengths[b] what is to be kept.  kv_cache 16-byte aligned; k or v over the two planes are refused. */
+int llmops_cache_write_q4(const void* k, int64_t k_stride_b, int64_t k_stride_l, int64_t k_stride_h, const void* v, int64_t v_stride_b,
+                          int64_t v_stride_l, int64_t v_stride_h, int dtype, int64_t B, int64_t qL, int64_t Hkv, int64_t S, const float* inv_freq,
+                          int64_t half, void* kv_cache, int64_t planes, int64_t maxlen, const int32_t* lengths, const int32_t* q_lens, int layer_id,
+                          llmops_stream_t stream);
+
+/* The values that rows starts[b] .. starts[b] + rows - 1 (starts int32 [B] on the device, NULL: from 0) of every plane, sequence and head of a cache in
+ * 4 bits stand for -> out [planes,B,Hkv,rows,S] of `dtype` (LLMOPS_F32, _F16: exact in both).  Rows outside the cache give 0.  An out over the cache or
+ * starts is refused.  planes*B*Hkv*rows below 2^28. */
+int llmops_cache_read_q4(const void* kv_cache, int64_t planes, int64_t B, int64_t Hkv, int64_t maxlen, int64_t S, const int32_t* starts, int64_t rows,
+                         void* out, int dtype, llmops_stream_t stream);
+
+/* llmops_attention_rope_prefix without a prefix, over a cache in 4 bits: the new tokens' k (rotated) and v go to the cache as llmops_cache_write_q4 writes them,
+ * and out is the softmax over what rows 0 .. lengths[b] + l of the cache stand for, the call's own among them.  Arguments, padding and refusals as there.
+ * Rows are shared out among workgroups by the lengths on the device: a cache's capacity costs nothing but its memory.
+ * Arithmetic: products of halves with fp32 sums, the cache's values exact, queries and weights in two halves (22 bits of a query beside its
+ * head's largest value): results agree with fp32 evaluation to about 1e-6 of the largest output, and 2^-36 beside it, and are the same bits in every call.
+ * B*qL*H < 2^24, and times ceil(maxlen/128) < 2^31. */
+size_t llmops_attention_q4_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t maxlen);
+int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b, int64_t k_stride_l,
+                             const float* v, int64_t v_stride_b, int64_t v_stride_l, int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S,
+                             const float* inv_freq, int64_t half, void* kv_cache, int64_t planes, int64_t maxlen, const int32_t* lengths,
+                             const int32_t* q_lens, int layer_id, float* out, void* workspace, size_t workspace_bytes, llmops_stream_t stream);
+
+/* Log probabilities of given tokens: logits fp32, row (b, l) of V at + b*stride_b + l*stride_l elements (dense rows, any strides: a text's logits without
+ * its last row will do), tokens int64, that of row (b, l) at + b*token_stride_b + l*token_stride_l; p = softmax(row).
+ *   logprobs [B,L] = log p(token), a token outside 0..V-1 (padding) 0;  entropy [B,L] = -sum p log p;  top_tokens int64 and top_logprobs [B,L,top]: the
+ *   `top` likeliest tokens in the order of their logits, equal ones in the order of their numbers (top 0 .. 64, at most V; 0: both may be NULL).
+ * Logits that are NaN or minus infinity weigh nothing (log p is minus infinity), equal plus infinities share the row; a row without any other
+ * logit gives NaN.  fp32 sums; right to about 1e-6.
+ * B*L < 2^24, V <= 2^27, B*L*ceil(V/8192) < 2^24.  Outputs that lie over each other or over inputs are refused. */
+size_t llmops_token_logprobs_workspace_bytes(int64_t B, int64_t L, int64_t V, int64_t top);
+int llmops_token_logprobs(const float* logits, int64_t stride_b, int64_t stride_l, int64_t B, int64_t L, int64_t V, const int64_t* tokens,
+                          int64_t token_stride_b, int64_t token_stride_l, int64_t top, float* logprobs, float* entropy, int64_t* top_tokens,
+                          float* top_logprobs, void* workspace, size_t workspace_bytes, llmops_stream_t stream);
+
 /* softmax (ops/op_misc.hpp:183-194, ops/utils.hpp:484-490): in place over rows of length K */
 int llmops_softmax(float* x, int64_t rows, int64_t K, llmops_stream_t stream);
 

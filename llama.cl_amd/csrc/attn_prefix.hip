@@ -25,21 +25,10 @@
 // and NaN are seen while a tile is cut up, and so is a piece whose K or whose V is below 2^-14 throughout; such a piece is multiplied on the
 // vector ALU in full width instead, row by row of those that a query sees, so that what a mask hides has no effect whatever it holds.  (Values
 // below 2^-14 beside larger ones of their piece are not seen: they are right to 2^-36, not to a part of themselves.)
-#include <float.h>
-
-#include "common.h"
+#include "attn_device.h"
 #include "extents.h"
-#include "gemv_device.h"
 
 namespace llmops {
-
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef unsigned short v2us __attribute__((ext_vector_type(2)));
-
-constexpr int kS = 128;
-constexpr float kLift = 14.0f;  // weights are exp2(.. + kLift)
 
 struct PrefixArgs {
     _Float16 *qh, *ql;                  // [Hkv][M][128]
@@ -57,27 +46,7 @@ struct PrefixArgs {
     unsigned pitems;
 };
 
-// rows that sequence b has and new tokens that it brings; what does not fit the cache counts as padding
-__device__ __forceinline__ void own_extent(const int32_t* __restrict__ lengths, const int32_t* __restrict__ q_lens, int b, int qL, int64_t maxlen,
-                                           int& len, int& n) {
-    len = (int)max((int64_t)0, min((int64_t)lengths[b], maxlen));
-    const int want = q_lens != nullptr ? min(q_lens[b], qL) : qL;
-    n = (int)max((int64_t)0, min((int64_t)want, maxlen - len));
-}
-
 // ---- 1. rotation, cache rows, operands ----
-// cos and sin of inv_freq * pos: the product is exact in 64 bits, and so reduced to [-pi, pi] there (in fp32 it is off by 1.2e-4 at position
-// 4000, by up to 0.5 at 2^23); what its rounding to fp32 leaves out is put back to first order, 2^-24 being all that it can be
-__device__ __forceinline__ void turn_of(float f, int pos, float& c, float& s) {
-    const double angle = (double)f * (double)pos, whole = rint(angle * 0.15915494309189535);
-    const double rest = fma(-whole, 2.4492935982947064e-16, fma(-whole, 6.283185307179586, angle));  // 2 pi in two parts
-    const float hi = (float)rest, lo = (float)(rest - (double)hi);
-    float s0, c0;
-    sincosf(hi, &s0, &c0);
-    c = fmaf(-lo, s0, c0);
-    s = fmaf(lo, c0, s0);
-}
-
 __device__ __forceinline__ void store_row4(float* dst, const float* v) { *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void store_row4(__half* dst, const float* v) {
     const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
@@ -114,32 +83,6 @@ __device__ __forceinline__ void turn_row(const float* __restrict__ src, int d, c
             else if (at < 2 * half) x[e] = turn[at - half].y * src[at - half] + turn[at - half].x * x[e];
         }
     }
-}
-// a rotated query as halves, dims in x's order, and its factor
-struct QueryRow {
-    uint4 hi, lo;
-    float c;
-};
-__device__ __forceinline__ QueryRow query_row(const float (&x)[8], bool live) {
-    float top = 0.0f;
-    bool fine = true;
-#pragma unroll
-    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e])), fine &= fabsf(x[e]) <= FLT_MAX;
-    float bad = fine ? 0.0f : 1.0f;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64)), bad = fmaxf(bad, __shfl_xor(bad, o, 64));
-    const bool use = live && bad == 0.0f && top > 0.0f;
-    // (2^123 at most: the factor stays a normal number.  It would lose its bits below 2^-126, and at 0 make NaN of a masked score's -inf)
-    const int e2 = use ? min(123, 13 - ilogbf(top)) : 0;
-    v8h hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float y = use ? ldexpf(x[e], e2) : 0.0f;
-        hi[e] = (_Float16)y;
-        lo[e] = (_Float16)(y - (float)hi[e]);
-    }
-    // (a query that holds an infinity or NaN has no score that is a number)
-    return {__builtin_bit_cast(uint4, hi), __builtin_bit_cast(uint4, lo), live && bad != 0.0f ? NAN : ldexpf(1.44269504f * 0.08838834764831845f, -e2)};
 }
 template <typename T>
 __device__ __forceinline__ void store_row(T* dst, int d, const float (&x)[8]) {
@@ -244,30 +187,9 @@ struct Seen<__half> {
     }
 };
 
-__device__ __forceinline__ v8h as_v8h(uint4 u) { return *reinterpret_cast<const v8h*>(&u); }
-__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-
 __device__ __forceinline__ float value(const float* p) { return *p; }
 __device__ __forceinline__ float value(const __half* p) { return __half2float(*p); }
 
-// queries 16*rt + lane % 16 of a wave: factor, running maximum (log2), this lane's part of the sum, O^T
-template <int RT>
-struct Queries {
-    float c[RT], m[RT], l[RT];
-    int see[RT];  // rows below this one are seen
-    v4f o[RT][8];
-    // cq: the factor of query m0
-    __device__ __forceinline__ void start(const float* cq, int m0, int m_end, int i) {
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            c[rt] = cq[min(16 * rt + i, m_end - 1 - m0)];
-            m[rt] = -INFINITY;
-            l[rt] = 0.0f;
-#pragma unroll
-            for (int c8 = 0; c8 < 8; c8++) o[rt][c8] = v4f{0.f, 0.f, 0.f, 0.f};
-        }
-    }
-};
 // their operands: in registers for sixteen queries, in LDS for more (the four waves share them)
 template <int RT>
 struct QueryOps;
@@ -315,62 +237,6 @@ __device__ __forceinline__ void score_step(v4f& acc, v4f& low, const Halves& k, 
     acc = mfma(k.hi, ql, acc);
 }
 
-// the larger of this lane's value and those of the lanes 16, 32 and 48 away
-__device__ __forceinline__ float over_groups(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t w = __float_as_uint(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
-    const auto y = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-}
-
-// scores (before the factor, which is positive) to weights: the running maximum, the sum, and what the sums so far shrink by.
-// sc[tt]: rows t + 16*tt + 4*g + v
-template <int RT>
-__device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[2], int t, int g, bool masked) {
-    if (masked) {
-#pragma unroll
-        for (int tt = 0; tt < 2; tt++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) sc[tt][v] = t + 16 * tt + 4 * g + v < s.see[rt] ? sc[tt][v] : -INFINITY;
-    }
-    float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-    top = over_groups(top) * s.c[rt];
-    if (__any(top > s.m[rt])) {
-        const float m = fmaxf(s.m[rt], top), shrink = s.m[rt] == m ? 1.0f : __builtin_amdgcn_exp2f(s.m[rt] - m);
-        s.m[rt] = m;
-        s.l[rt] *= shrink;
-#pragma unroll
-        for (int c = 0; c < 8; c++) s.o[rt][c] *= shrink;
-    }
-    const float base = s.m[rt] == -INFINITY ? 0.0f : kLift - s.m[rt];  // (nothing seen yet: every weight is exp2(-inf) = 0)
-#pragma unroll
-    for (int tt = 0; tt < 2; tt++)
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-            sc[tt][v] = __builtin_amdgcn_exp2f(fmaf(sc[tt][v], s.c[rt], base));
-            s.l[rt] += sc[tt][v];
-        }
-}
-
-// the weights of 32 rows as operands: hi, lo, hi / 2048
-struct Weights {
-    v8h hi, lo, low;
-};
-template <typename T>
-__device__ __forceinline__ Weights weights_of(const v4f (&sc)[2]) {
-    Weights w;
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        const float x = sc[j >> 2][j & 3], y = sc[j >> 2][(j & 3) + 1];
-        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
-        const v2h hv = __builtin_bit_cast(v2h, h);
-        w.hi[j] = hv[0], w.hi[j + 1] = hv[1];
-        w.lo[j] = (_Float16)fmaf((float)hv[0], -1.0f, x), w.lo[j + 1] = (_Float16)fmaf((float)hv[1], -1.0f, y);
-    }
-    if constexpr (sizeof(T) == 4) w.low = w.hi * (_Float16)(1.0f / 2048.0f);
-    return w;
-}
 template <typename T>
 __device__ __forceinline__ v4f add_rows(v4f o, const Halves& v, const Weights& w) {
     o = mfma(v.hi, w.hi, o);
@@ -494,19 +360,6 @@ struct MeetSmem {
         } in;
     };
 };
-
-// `lane_at` is hidden from the compiler here so that it adds `at` where it loads, up to 4095 in the instruction, and does not keep
-// sixteen sums in registers
-__device__ __forceinline__ uint32_t unseen(uint32_t x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-__device__ __forceinline__ uint4 ask16(buffer_rsrc r, uint32_t lane_at, uint32_t at) {
-    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_at + at, 0, 0));
-}
-__device__ __forceinline__ uint2 ask8(buffer_rsrc r, uint32_t lane_at, uint32_t at) {
-    return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_at + at, 0, 0));
-}
 
 template <typename T>
 struct RowRegs;
@@ -971,19 +824,6 @@ __device__ __forceinline__ void many_queries(const PrefixArgs& a, int hk, int m0
             for (int v = 0; v < 4; v++)
                 leave(a, hk, m, piece, 64 * h + 16 * g + 4 * v, make_float4(s.o[rt][4 * h][v], s.o[rt][4 * h + 1][v], s.o[rt][4 * h + 2][v], s.o[rt][4 * h + 3][v]),
                       s.l[rt], see[rt] > 0);
-    }
-}
-
-// Item `at` of groups * each: the items of a group, which read the same rows, follow each other on one XCD (consecutive workgroups go to
-// the eight in turn), so that its L2 serves all but the first
-__device__ __forceinline__ void item_of(unsigned at, unsigned groups, unsigned each, int& group, int& sub) {
-    const unsigned whole = groups & ~7u;
-    if (at < whole * each) {
-        const unsigned eight = at / (8 * each), in = at - eight * 8 * each;
-        group = (int)(eight * 8 + (in & 7)), sub = (int)(in >> 3);
-    } else {
-        const unsigned in = at - whole * each;
-        group = (int)(whole + in / each), sub = (int)(in % each);
     }
 }
 

@@ -1,0 +1,532 @@
+// Attention of a batch over a cache that is held in 4 bits (its rows: cache_q4_device.h).  For sequence b with len[b] rows and n[b] new tokens,
+// token l < n[b], head h on kv head h / G, G = H / Hkv:
+//   pos = len[b] + l,  q' = rot(q, pos),  row pos of the cache = the codes of (rot(k, pos), v),
+//   out = sum_r e_r V_r / sum_r e_r,  e_r = exp(q' . K_r / sqrt(S) - max),  r = 0 .. pos,  K and V as the cache holds them
+//
+//   1. q4_prep_kernel   rotates, writes the new rows and leaves q' as operands of the matrix instructions
+//   2. q4_few_kernel    softmax(q'K^T)V, running maximum and sum, one pass: rows shared out among workgroups by the lengths
+//   3. q4_join_kernel   joins what several workgroups have of a query
+//
+// Queries of a kv head are numbered m = (b*qL + l)*G + g.
+//
+// Arithmetic.  The cache's values are halves, so that they are operands of v_mfma_f32_16x16x32_f16 (fp32 sums) without any loss; q' and the weights
+// are two halves each: q' scaled by a power of two of its row so that its largest value is in [2^13, 2^14), 22 bits of that, the weights times
+// 2^14, so that those down to 2^-28 of the largest keep their bits.
+#include "cache_q4_device.h"
+#include "extents.h"
+
+namespace llmops {
+
+constexpr int kUnit = 128;  // rows that a workgroup's four waves read at a time
+
+struct Q4Args {
+    _Float16 *qh, *ql;                  // [Hkv][M][128]
+    float* cq;                          // [Hkv][M]: score = cq * (q' . k), in units of log2
+    uint8_t *k, *v;                     // the layer's planes [B][Hkv][maxlen][80]
+    const int32_t *lengths, *q_lens;    // [B]; q_lens may be null
+    float* rec_out;                     // [groups][2][queries of a tile][128]
+    float2* rec_stat;                   // [groups][2][queries of a tile]: max (log2), sum
+    float* out;                         // [B][qL][H*128]
+    int64_t maxlen;
+    int B, qL, G, Hkv, M, Mq;           // M = B*qL*G, Mq = qL*G
+    int tiles, groups;                  // tiles of a sequence's queries for a kv head; workgroups
+};
+struct Q4Prep {
+    const float *q, *k, *v, *inv_freq;
+    int64_t qsb, qsl, ksb, ksl, vsb, vsl;
+    int half, rows16;
+};
+
+// ---- 1. ----
+// A workgroup per token and 16 of its H + 2*Hkv rows of 128, sixteen lanes to a row
+__global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a, Q4Prep p) {
+    __shared__ double2 turn[64];
+    const int bl = blockIdx.x / p.rows16, group = blockIdx.x - bl * p.rows16, b = bl / a.qL, l = bl - b * a.qL;
+    const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), j = threadIdx.x & 15;
+    const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv, none = row >= H + 2 * a.Hkv;
+    const int hk = is_k ? row - H : row - H - a.Hkv;
+    const float* src = is_q ? p.q + b * p.qsb + l * p.qsl + (int64_t)row * kS : is_k ? p.k + b * p.ksb + l * p.ksl + (int64_t)hk * kS : p.v + b * p.vsb + l * p.vsl + (int64_t)hk * kS;
+    // (the row is on its way while the length is fetched and the angles are formed, also where the token turns out to be padding)
+    double x[8] = {};
+    if (!none) load8(src + 8 * j, x);
+    int len, n;
+    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    const bool live = l < n;
+    if (live && (int)threadIdx.x < p.half) turn[threadIdx.x] = turn64(p.inv_freq[threadIdx.x], len + l);
+    __syncthreads();
+    if (none || (!live && !is_q)) return;
+    if (live && (is_q || is_k)) turn_row64(src, j, turn, p.half, x);
+    if (!is_q) {
+        store_q4((is_k ? a.k : a.v) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kQ4Row, quantise8(x), j);
+        return;
+    }
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = (float)x[e];
+    const int64_t m = (int64_t)(row / a.G) * a.M + (int64_t)bl * a.G + row % a.G;
+    const QueryRow r = query_row(y, live);
+    *reinterpret_cast<uint4*>(a.qh + m * kS + 8 * j) = r.hi;
+    *reinterpret_cast<uint4*>(a.ql + m * kS + 8 * j) = r.lo;
+    if (j == 0) a.cq[m] = r.c;
+}
+
+// ---- 2. rows for a tile of queries ----
+// Lanes of v_mfma_f32_16x16x32_f16: operand A row lane % 16, B column lane % 16, eight k-values 8 * (lane / 16) .. +7 of either;
+// result column lane % 16, rows 4 * (lane / 16) + v.  With g = lane / 16 and i = lane % 16, 32 cache rows from t on:
+//   S^T = K Q^T   A: rows t + 16*tt + i, dims 32*g + 8*step .. +7: one group of the cache's to a lane, 16 bytes of codes.  B: query i.
+//                 Result: query i, rows t + 16*tt + 4*g + v.
+//   O^T = V^T e^T k-value j of lane group g stands for row t + 16*(j/4) + 4*g + j%4, so that B is the scores as they lie.
+//                 A: dim 8*i + c of product c: a lane loads word i of its eight rows, which holds the eight products' codes, and turns the
+//                 8 x 8 codes over in its registers.  Result of product c: query i, dim 8*(4*g + v) + c.
+__device__ __forceinline__ uint32_t ask4(buffer_rsrc r, uint32_t lane_at, uint32_t at) { return __builtin_amdgcn_raw_buffer_load_b32(r, lane_at + at, 0, 0); }
+
+// 32 rows from t on (the same t in the whole wave) as a descriptor that ends with the rows: those behind read as zero
+__device__ __forceinline__ buffer_rsrc q4_rows(const uint8_t* p, int t, int end) {
+    return make_rsrc(p + (int64_t)t * kQ4Row, (uint32_t)__builtin_amdgcn_readfirstlane(max(0, min(32, end - t))) * (uint32_t)kQ4Row);
+}
+struct Q4Regs {
+    uint4 k[2];
+    uint32_t kdm[2], v[8], vdm[8];
+    __device__ __forceinline__ void load_k(buffer_rsrc r, int i, int g) {
+        const uint32_t codes = unseen((uint32_t)(i * kQ4Row + 16 * g)), pairs = unseen((uint32_t)(i * kQ4Row + 64 + 4 * g));
+#pragma unroll
+        for (int tt = 0; tt < 2; tt++) k[tt] = ask16(r, codes, 16 * tt * kQ4Row), kdm[tt] = ask4(r, pairs, 16 * tt * kQ4Row);
+    }
+    __device__ __forceinline__ void load_v(buffer_rsrc r, int i, int g) {
+        const uint32_t codes = unseen((uint32_t)(4 * g * kQ4Row + 4 * i)), pairs = unseen((uint32_t)(4 * g * kQ4Row + 64 + (i & 12)));
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            v[j] = ask4(r, codes, (16 * (j >> 2) + (j & 3)) * kQ4Row);
+            vdm[j] = ask4(r, pairs, (16 * (j >> 2) + (j & 3)) * kQ4Row);
+        }
+    }
+    __device__ __forceinline__ v8h k_op(int tt, int step) const {
+        return values8(step == 0 ? k[tt].x : step == 1 ? k[tt].y : step == 2 ? k[tt].z : k[tt].w, kdm[tt]);
+    }
+    // the operands of two products from byte y of the eight words: codes 0 2, 4 6, 1 3, 5 7
+    __device__ __forceinline__ void v_ops(int y, v8h& low, v8h& high) const {
+        const uint32_t pick = 0x0c000c00u | (uint32_t)(4 + y) << 16 | (uint32_t)y;
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const uint32_t x = __builtin_amdgcn_perm(v[2 * p + 1], v[2 * p], pick);
+            const v2h d = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(vdm[2 * p + 1], vdm[2 * p], 0x05040100u)),
+                      m = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(vdm[2 * p + 1], vdm[2 * p], 0x07060302u));
+            const v2h lo = __builtin_elementwise_fma(pair_low(x), d, m), hi = __builtin_elementwise_fma(pair_high(x), d, m);
+            low[2 * p] = lo[0], low[2 * p + 1] = lo[1], high[2 * p] = hi[0], high[2 * p + 1] = hi[1];
+        }
+    }
+    // a V row that holds NaN (m tells, in every group) among rows that not every query sees: NaN in the scores of those that do, and nothing in
+    // the operand, where it would reach the others as 0 * NaN
+    __device__ __forceinline__ void hide_nan(uint32_t& hidden) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if ((vdm[j] & 0x7fff0000u) > 0x7c000000u) vdm[j] = 0, hidden |= 1u << j;
+    }
+};
+__device__ __forceinline__ constexpr int first_code(int y) { return y == 0 ? 0 : y == 1 ? 4 : y == 2 ? 1 : 5; }  // of byte y; the other is 2 more
+
+template <int RT>
+struct Q4QueryOps;
+template <>
+struct Q4QueryOps<1> {
+    v8h h[4], l[4];
+    __device__ __forceinline__ void load(const Q4Args& a, uint4*, int hk, int m0, int m_end, int lane) {
+        const int64_t at = ((int64_t)hk * a.M + min(m0 + (lane & 15), m_end - 1)) * kS + 32 * (lane >> 4);
+#pragma unroll
+        for (int step = 0; step < 4; step++) {
+            h[step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + at + 8 * step));
+            l[step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + at + 8 * step));
+        }
+    }
+    __device__ __forceinline__ v8h hi(int, int step) const { return h[step]; }
+    __device__ __forceinline__ v8h lo(int, int step) const { return l[step]; }
+};
+template <>
+struct Q4QueryOps<2> {
+    const uint4* mine;
+    __device__ __forceinline__ void load(const Q4Args& a, uint4* lds, int hk, int m0, int m_end, int lane) {
+        const int wave = threadIdx.x >> 6;  // a step to a wave
+#pragma unroll
+        for (int rt = 0; rt < 2; rt++) {
+            const int64_t at = ((int64_t)hk * a.M + min(m0 + 16 * rt + (lane & 15), m_end - 1)) * kS + 32 * (lane >> 4) + 8 * wave;
+            lds[(rt * 8 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.qh + at);
+            lds[(rt * 8 + 4 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.ql + at);
+        }
+        mine = lds + lane;
+        __syncthreads();
+    }
+    __device__ __forceinline__ v8h hi(int rt, int step) const { return as_v8h(mine[(rt * 8 + step) * 64]); }
+    __device__ __forceinline__ v8h lo(int rt, int step) const { return as_v8h(mine[(rt * 8 + 4 + step) * 64]); }
+};
+
+// Units of 128 rows are numbered through: sequence after sequence, in each kv head after kv head, in each tile after tile.  A sequence without
+// rows (padding) has one unit for each all the same, in which its zeros are written.
+__device__ __forceinline__ int units_of(const Q4Args& a, int b) {
+    int len, n;
+    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    return n > 0 ? (len + n + kUnit - 1) / kUnit : 1;
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        v += lane >= o ? u : 0;
+    }
+    return v;
+}
+// Every wave for itself: all units, and the sequence that has unit `wanted(all)`, or that is `wanted(all)` where by_unit is false; its units for a
+// tile, and the units before it.
+struct UnitPlace {
+    int all, b, units, before;
+};
+template <typename F>
+__device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane, bool by_unit, F wanted) {
+    const int each = a.Hkv * a.tiles;
+    int all = 0, units = 0, upto = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        units = b0 + lane < a.B ? units_of(a, b0 + lane) : 0;
+        upto = all + wave_scan(units * each, lane);
+        all = __builtin_amdgcn_readlane(upto, 63);
+    }
+    UnitPlace p{all, -1, 0, 0};
+    const int want = wanted(all);
+    if (by_unit && want >= all) return p;
+    int before = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        if (a.B > 64) {
+            units = b0 + lane < a.B ? units_of(a, b0 + lane) : 0;
+            upto = before + wave_scan(units * each, lane);
+        }
+        const uint64_t hit = by_unit ? __ballot(upto > want) : want >= b0 && want < b0 + 64 ? 1ull << (want - b0) : 0;
+        if (hit != 0) {
+            const int at = __builtin_ctzll(hit);
+            p.b = b0 + at;
+            p.units = __builtin_amdgcn_readlane(units, at);
+            p.before = __builtin_amdgcn_readlane(upto, at) - p.units * each;
+            break;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return p;
+}
+__device__ __forceinline__ int share_of(int all, int groups) { return (all + groups - 1) / groups; }
+
+__device__ __forceinline__ void q4_leave(const Q4Args& a, int hk, int m, int d, float4 o, float sum, bool live) {
+    const float f = live ? 1.0f / sum : 0.0f;
+    const int bl = m / a.G;
+    *reinterpret_cast<float4*>(a.out + ((int64_t)bl * a.G * a.Hkv + (int64_t)hk * a.G + (m - bl * a.G)) * kS + d) =
+        live ? make_float4(o.x * f, o.y * f, o.z * f, o.w * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+constexpr int kQ4MeetRow = 132;  // floats (16 queries' rows on different banks)
+struct Q4MeetSmem {
+    float m[4][32], l[4][32], sum[16];
+    union {
+        float o[4][16][kQ4MeetRow];
+        uint4 q[16 * 64];
+    };
+};
+
+// Few queries to a workgroup (16 * RT).  The four waves take 32 rows each of every 128; operands come straight from memory, the next rows asked
+// for when these are used up; the waves' sums meet in LDS.
+template <int RT>
+__global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void q4_few_kernel(Q4Args a) {
+    __shared__ Q4MeetSmem sm;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    int share = 0;
+    const UnitPlace start = place_of(a, lane, true, [&](int all) { share = share_of(all, a.groups); return (int)min((int64_t)blockIdx.x * share, (int64_t)INT_MAX); });
+    if (start.b < 0) return;
+    const int first = (int)blockIdx.x * share, last = min(start.all, first + share), each = a.Hkv * a.tiles;
+    int b = start.b, units = start.units, before = start.before;
+#pragma unroll 1
+    for (int at = first; at < last;) {
+        if (at >= before + units * each) {  // (the next sequence)
+            before += units * each;
+            units = units_of(a, ++b);
+        }
+        const int item = (at - before) / units, u0 = at - before - item * units, u1 = min(units, u0 + last - at), hk = item / a.tiles, tile = item - hk * a.tiles;
+        at += u1 - u0;
+        int len, n;
+        own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+        const int m0 = b * a.Mq + tile * 16 * RT, m_end = min((b + 1) * a.Mq, m0 + 16 * RT);
+        // rows that the tile's last live query sees
+        const int seen_by_last = min(n, (m_end - 1 - b * a.Mq) / a.G + 1), rows = tile * 16 * RT < n * a.G ? len + seen_by_last : 0;
+        const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kQ4Row;
+        const uint8_t *K = a.k + plane, *V = a.v + plane;
+        Q4Regs x;
+        const int j0 = 4 * u0 + wave, j1 = min(4 * u1, (rows + 31) / 32);
+        if (j0 < j1) x.load_k(q4_rows(K, 32 * j0, rows), i, g), x.load_v(q4_rows(V, 32 * j0, rows), i, g);
+        Q4QueryOps<RT> q;
+        q.load(a, sm.q, hk, m0, m_end, lane);
+        Queries<RT> s;
+        s.start(a.cq + (int64_t)hk * a.M + m0, m0, m_end, i);
+        bool live[RT];
+        int see_min = INT_MAX;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const int l = (min(m0 + 16 * rt + i, m_end - 1) - b * a.Mq) / a.G;
+            live[rt] = l < n;
+            s.see[rt] = live[rt] ? len + l + 1 : INT_MAX;  // (what padding sees is thrown away)
+            see_min = min(see_min, s.see[rt]);
+        }
+#pragma unroll 1
+        for (int j = j0; j < j1; j += 4) {
+            const int t = 32 * j;
+            const bool masked = __any(t + 32 > see_min);
+            v4f sc[RT][2];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int step = 0; step < 4; step++) {
+#pragma unroll
+                for (int tt = 0; tt < 2; tt++) {
+                    const v8h k = x.k_op(tt, step);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        sc[rt][tt] = mfma(k, q.hi(rt, step), sc[rt][tt]);
+                        sc[rt][tt] = mfma(k, q.lo(rt, step), sc[rt][tt]);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (j + 4 < j1) x.load_k(q4_rows(K, t + 128, rows), i, g);
+            uint32_t hidden = 0;
+            if (masked) x.hide_nan(hidden);
+            Weights w[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                if (hidden != 0)
+#pragma unroll
+                    for (int r = 0; r < 8; r++)
+                        if (hidden >> r & 1) sc[rt][r >> 2][r & 3] = NAN;
+                weigh<true>(s, rt, sc[rt], t, g, masked);
+                w[rt] = weights_of<__half>(sc[rt]);
+            }
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                v8h low, high;
+                x.v_ops(y, low, high);
+                const int c = first_code(y);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    s.o[rt][c] = mfma(low, w[rt].hi, s.o[rt][c]);
+                    s.o[rt][c + 2] = mfma(high, w[rt].hi, s.o[rt][c + 2]);
+                    s.o[rt][c] = mfma(low, w[rt].lo, s.o[rt][c]);
+                    s.o[rt][c + 2] = mfma(high, w[rt].lo, s.o[rt][c + 2]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (j + 4 < j1) x.load_v(q4_rows(V, t + 128, rows), i, g);
+        }
+        // the four waves' sums
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            s.l[rt] += __shfl_xor(s.l[rt], 16, 64);
+            s.l[rt] += __shfl_xor(s.l[rt], 32, 64);
+            if (g == 0) sm.m[wave][16 * rt + i] = s.m[rt], sm.l[wave][16 * rt + i] = s.l[rt];
+        }
+        __syncthreads();
+        const bool whole = u0 == 0 && u1 == units;
+        const int64_t record = ((int64_t)blockIdx.x * 2 + (u0 == 0)) * (16 * RT);
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            float M = sm.m[0][16 * rt + i];
+#pragma unroll
+            for (int w = 1; w < 4; w++) M = fmaxf(M, sm.m[w][16 * rt + i]);
+            const float f = s.m[rt] == M ? 1.0f : __builtin_amdgcn_exp2f(s.m[rt] - M);  // (equal: also both -inf)
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    *reinterpret_cast<float4*>(&sm.o[wave][i][8 * (4 * g + v) + 4 * h]) =
+                        make_float4(s.o[rt][4 * h][v] * f, s.o[rt][4 * h + 1][v] * f, s.o[rt][4 * h + 2][v] * f, s.o[rt][4 * h + 3][v] * f);
+            if (wave == 0 && g == 0) {
+                float L = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const float mw = sm.m[w][16 * rt + i];
+                    L += sm.l[w][16 * rt + i] * (mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
+                }
+                sm.sum[i] = live[rt] ? L : -1.0f;
+                if (!whole) a.rec_stat[record + 16 * rt + i] = make_float2(M, L);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int e = threadIdx.x + 256 * u, query = e >> 5, d = 4 * (e & 31), m = m0 + 16 * rt + query;
+                if (m < m_end) {
+                    float4 r = *reinterpret_cast<const float4*>(&sm.o[0][query][d]);
+#pragma unroll
+                    for (int w = 1; w < 4; w++) {
+                        const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][query][d]);
+                        r.x += y.x, r.y += y.y, r.z += y.z, r.w += y.w;
+                    }
+                    if (whole) q4_leave(a, hk, m, d, r, sm.sum[query], sm.sum[query] != -1.0f);
+                    else *reinterpret_cast<float4*>(a.rec_out + (record + 16 * rt + query) * kS + d) = r;
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// ---- 3. what several workgroups have of a query ----
+// a workgroup to a query, half a wave to every eighth record, 16 bytes to a lane
+template <int RT>
+__global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
+    __shared__ float stat[8][2];
+    __shared__ float4 part[8][32];
+    const int64_t r = blockIdx.x;
+    const int hk = (int)(r / a.M), m = (int)(r - (int64_t)hk * a.M), b = m / a.Mq, in = m - b * a.Mq, tile = in / (16 * RT), l = in / a.G;
+    const UnitPlace p = place_of(a, threadIdx.x & 63, false, [&](int) { return b; });
+    const int share = share_of(p.all, a.groups), at = p.before + (hk * a.tiles + tile) * p.units, w0 = at / share, w1 = (at + p.units - 1) / share;
+    if (w0 == w1) return;
+    int len, n;
+    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    const int half = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31), query = in - tile * 16 * RT;
+    float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int w = w0 + half; w <= w1; w += 32) {
+        float2 st[4];
+        float4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t wg = min(w + 8 * u, w1), record = (wg * 2 + (wg * share <= at)) * (16 * RT) + query;
+            st[u] = a.rec_stat[record];
+            x[u] = *reinterpret_cast<const float4*>(a.rec_out + record * kS + d);
+        }
+        float up = M;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (w + 8 * u > w1) st[u] = make_float2(-INFINITY, 0.0f);
+            up = fmaxf(up, st[u].x);
+        }
+        const float shrink = M == up ? 1.0f : __builtin_amdgcn_exp2f(M - up);
+        M = up;
+        L *= shrink, o.x *= shrink, o.y *= shrink, o.z *= shrink, o.w *= shrink;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const bool none = st[u].y == 0.0f;
+            const float f = none ? 0.0f : st[u].x == M ? 1.0f : __builtin_amdgcn_exp2f(st[u].x - M);
+            if (none) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            L = fmaf(f, st[u].y, L);
+            o.x = fmaf(f, x[u].x, o.x), o.y = fmaf(f, x[u].y, o.y), o.z = fmaf(f, x[u].z, o.z), o.w = fmaf(f, x[u].w, o.w);
+        }
+    }
+    if (d == 0) stat[half][0] = M, stat[half][1] = L;
+    part[half][threadIdx.x & 31] = o;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    M = stat[0][0];
+#pragma unroll
+    for (int h = 1; h < 8; h++) M = fmaxf(M, stat[h][0]);
+    L = 0.0f, o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int h = 0; h < 8; h++) {
+        const float f = stat[h][1] == 0.0f ? 0.0f : stat[h][0] == M ? 1.0f : __builtin_amdgcn_exp2f(stat[h][0] - M);
+        const float4 x = part[h][threadIdx.x];
+        L = fmaf(f, stat[h][1], L);
+        o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+    }
+    q4_leave(a, hk, m, d, o, L, l < n);
+}
+
+struct Q4Plan {
+    int rt, tiles, groups;
+};
+static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t maxlen) {
+    Q4Plan p{};
+    const int64_t Mq = qL * (H / Hkv);
+    p.rt = Mq > 16 ? 2 : 1;
+    p.tiles = (int)((Mq + 16 * p.rt - 1) / (16 * p.rt));
+    const int64_t most = B * Hkv * p.tiles * ((maxlen + kUnit - 1) / kUnit), held = p.rt == 1 ? 768 : 512;  // (workgroups that the chip holds)
+    p.groups = (int)(most < held ? most : held);
+    return p;
+}
+struct Q4Layout {
+    size_t qh, ql, cq, stat, rec, total;
+};
+static Q4Layout layout_q4(const Q4Plan& plan, int64_t rows) {
+    Q4Layout w{};
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const size_t records = (size_t)plan.groups * 2 * 16 * plan.rt;
+    w.qh = take((size_t)rows * kS * 2);
+    w.ql = take((size_t)rows * kS * 2);
+    w.cq = take((size_t)rows * 4);
+    w.stat = take(records * 8);
+    w.rec = take(records * kS * 4);
+    w.total = at;
+    return w;
+}
+
+template <int RT>
+static int q4_launch(const Q4Args& a, const Q4Prep& p, const Q4Plan& plan, hipStream_t st) {
+    q4_prep_kernel<<<(unsigned)((int64_t)a.B * a.qL * p.rows16), 256, 0, st>>>(a, p);
+    LLMOPS_LAUNCH_CHECK();
+    q4_few_kernel<RT><<<(unsigned)plan.groups, 256, 0, st>>>(a);
+    LLMOPS_LAUNCH_CHECK();
+    q4_join_kernel<RT><<<(unsigned)((int64_t)a.Hkv * a.M), 256, 0, st>>>(a);
+    LLMOPS_LAUNCH_CHECK();
+    return LLMOPS_OK;
+}
+
+}  // namespace llmops
+
+using namespace llmops;
+
+static bool q4_sizes_fit(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t maxlen) {
+    const int64_t most = (int64_t)1 << 24;  // (a launch has fewer than 2^32 threads)
+    return B > 0 && qL > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && maxlen > 0 && B < most && qL < most && H < most && maxlen <= most && B * qL < most &&
+           B * qL * H < most && (Wide)B * H * qL * ((maxlen + kUnit - 1) / kUnit) < ((Wide)1 << 31);
+}
+
+extern "C" size_t llmops_attention_q4_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t maxlen) {
+    if (S != kS || !q4_sizes_fit(B, qL, H, Hkv, maxlen)) return 0;
+    return layout_q4(plan_q4(B, qL, H, Hkv, maxlen), B * qL * H).total;
+}
+
+extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b, int64_t k_stride_l,
+                                        const float* v, int64_t v_stride_b, int64_t v_stride_l, int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S,
+                                        const float* inv_freq, int64_t half, void* kv_cache, int64_t planes, int64_t maxlen, const int32_t* lengths,
+                                        const int32_t* q_lens, int layer_id, float* out, void* workspace, size_t workspace_bytes, llmops_stream_t stream) {
+    LLMOPS_REQUIRE(q != nullptr && k != nullptr && v != nullptr && inv_freq != nullptr && kv_cache != nullptr && lengths != nullptr);
+    LLMOPS_REQUIRE(out != nullptr && workspace != nullptr);
+    LLMOPS_REQUIRE(S == 128);  // head size of every supported model shape
+    LLMOPS_REQUIRE(q4_sizes_fit(B, qL, H, Hkv, maxlen));
+    LLMOPS_REQUIRE(half > 0 && 2 * half <= S);
+    LLMOPS_REQUIRE(layer_id >= 0 && 2 * (int64_t)layer_id + 1 < planes);
+    LLMOPS_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(kv_cache, 16) && aligned(workspace, 256));
+    LLMOPS_REQUIRE(aligned(inv_freq, 4) && aligned(lengths, 4) && aligned(q_lens, 4));
+    LLMOPS_REQUIRE(q_stride_b % 4 == 0 && q_stride_l % 4 == 0 && k_stride_b % 4 == 0 && k_stride_l % 4 == 0 && v_stride_b % 4 == 0 && v_stride_l % 4 == 0);
+    const int64_t G = H / Hkv, rows16 = (H + 2 * Hkv + 15) / 16;
+    LLMOPS_REQUIRE((Wide)B * qL * rows16 < ((Wide)1 << 24));
+    const Wide heads = (Wide)H * kS * 4, kv_heads = (Wide)Hkv * kS * 4, plane = (Wide)B * Hkv * maxlen * kQ4Row;
+    LLMOPS_REQUIRE((Wide)planes * plane < ((Wide)1 << 62));
+    const Q4Plan plan = plan_q4(B, qL, H, Hkv, maxlen);
+    const Q4Layout w = layout_q4(plan, B * qL * H);
+    if (workspace_bytes < w.total) return fail(LLMOPS_EWORKSPACE, "attention_rope_q4 needs %zu workspace bytes, got %zu", w.total, workspace_bytes);
+    char* ws = reinterpret_cast<char*>(workspace);
+    Q4Args a{};
+    a.qh = reinterpret_cast<_Float16*>(ws + w.qh), a.ql = reinterpret_cast<_Float16*>(ws + w.ql), a.cq = reinterpret_cast<float*>(ws + w.cq);
+    a.rec_out = reinterpret_cast<float*>(ws + w.rec), a.rec_stat = reinterpret_cast<float2*>(ws + w.stat);
+    a.k = reinterpret_cast<uint8_t*>(kv_cache) + 2 * layer_id * (int64_t)plane, a.v = a.k + (int64_t)plane;
+    a.lengths = lengths, a.q_lens = q_lens, a.out = out, a.maxlen = maxlen;
+    a.B = (int)B, a.qL = (int)qL, a.G = (int)G, a.Hkv = (int)Hkv, a.Mq = (int)(qL * G), a.M = (int)(B * qL * G);
+    a.tiles = plan.tiles, a.groups = plan.groups;
+    // (a workgroup reads its q, k and v while others may have written their rows and results)
+    const Extent q_at(q, B, (Wide)q_stride_b * 4, qL, (Wide)q_stride_l * 4, heads), k_at(k, B, (Wide)k_stride_b * 4, qL, (Wide)k_stride_l * 4, kv_heads),
+        v_at(v, B, (Wide)v_stride_b * 4, qL, (Wide)v_stride_l * 4, kv_heads), out_at(out, (Wide)B * qL * heads), written(a.k, 2 * plane);
+    LLMOPS_REQUIRE(apart(written, q_at) && apart(written, k_at) && apart(written, v_at));
+    LLMOPS_REQUIRE(apart(out_at, q_at) && apart(out_at, k_at) && apart(out_at, v_at) && apart(out_at, written));
+    const Q4Prep p{q, k, v, inv_freq, q_stride_b, q_stride_l, k_stride_b, k_stride_l, v_stride_b, v_stride_l, (int)half, (int)rows16};
+    hipStream_t st = as_stream(stream);
+    return plan.rt == 1 ? q4_launch<1>(a, p, plan, st) : q4_launch<2>(a, p, plan, st);
+}

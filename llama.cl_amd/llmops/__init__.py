@@ -25,6 +25,7 @@ __all__ = [
     "attention_rope", "attention_rope2", "attention_rope2_records", "attention_records_supported", "AttentionRecords", "rope_embed", "softmax", "rmsnorm", "iadd", "imul", "itrans", "clone",
     "rmsnorm_out", "silu_mul", "empty", "ones", "embedding", "embedding_q8c_quant_w", "embedding_q8c", "tensor_pool", "set_default_group_k", "reserve_workspace", "reset_workspaces",
     "group_k_of", "attention_rope_prefix", "lora_add", "verify_drafts",
+    "cache_write_q4", "cache_read_q4", "attention_rope_q4", "token_logprobs",
 ]
 
 # Callers of the reference read ``tensor.item_size`` (chatllama/main.py:171-173, ops/perf_ops.py:242; bound at
@@ -674,6 +675,118 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature=None, 
                1.0 if temperature is None or per_row else float(temperature), _ptr(draft_lens) if draft_lens is not None else None, _ptr(tokens),
                _ptr(accepted), _ptr(ws), ws.numel())
     return tokens, accepted
+
+
+_Q4_ROW = 80  # bytes of a row of 128 values
+
+
+def _q4_cache(t):
+    _require(isinstance(t, torch.Tensor) and t.is_cuda, "kv_cache is on the HIP device (llmops has no CPU path)")
+    _require(t.dtype == torch.int8 and t.dim() == 5 and t.shape[4] == _Q4_ROW and t.is_contiguous(), "kv_cache.is<int8_t>({planes, B, Hkv, maxlen, 80})")
+    return t.shape[:4]
+
+
+def _q4_lengths(kv_cache, lengths, q_lens):
+    _dev(lengths, torch.int32, 1, "lengths")
+    _require(lengths.shape[0] == kv_cache.shape[1], "lengths.is({B})")
+    if q_lens is not None:
+        _dev(q_lens, torch.int32, 1, "q_lens")
+        _require(q_lens.shape[0] == kv_cache.shape[1], "q_lens.is({B})")
+
+
+def cache_write_q4(k, v, kv_cache, lengths, layer_id, inv_freq=None, q_lens=None):
+    """Writes rows into a cache that is held in 4 bits, 80 bytes for the 128 values of a token and head (``llmops_cache_write_q4`` has the format).
+
+    k and v [B,L,Hkv*128] (columns of a projection's output will do) or [B,L,Hkv,128], fp32 or fp16, any strides with a dense innermost dimension (a cache's
+    rows, ``cache[0].transpose(1, 2)``, will do, and ``expand`` over sequences: the rows are quantised once then), left as they are; kv_cache
+    int8 [2*layers,B,Hkv,maxlen,80].  Token l of sequence b goes to row lengths[b] + l (int32 [B], device, not changed); with ``inv_freq`` k is rotated by
+    that row's number, without it comes rotated.  q_lens (int32 [B], device): a sequence brings that many of the L tokens; the rest,
+    and tokens that do not fit the cache, are left out."""
+    planes, B, Hkv, maxlen = _q4_cache(kv_cache)
+    at = []
+    for t, n in ((k, "k"), (v, "v")):
+        _require(isinstance(t, torch.Tensor) and t.is_cuda, f"{n} is on the HIP device (llmops has no CPU path)")
+        _require(t.dtype in (torch.float32, torch.float16) and t.dtype == k.dtype and t.dim() in (3, 4), f"{n}.is<float>(3) || {n}.is<float>(4)")
+        _require(t.stride(-1) == 1, f"{n} inner dimension is contiguous")
+        _require(tuple(t.shape[2:]) == ((Hkv * 128,) if t.dim() == 3 else (Hkv, 128)) and t.shape[0] == B and t.shape[1] == k.shape[1], f"{n}.is({{B, L, Hkv * 128}})")
+        at += [_ptr(t), t.stride(0) if B > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0, 128 if t.dim() == 3 else t.stride(2) if Hkv > 1 else 0]
+    _q4_lengths(kv_cache, lengths, q_lens)
+    if inv_freq is not None:
+        _dev(inv_freq, torch.float32, 1, "inv_freq")
+    _here(kv_cache, k=k, v=v, lengths=lengths, inv_freq=inv_freq, q_lens=q_lens)
+    _on_device(kv_cache.device, _lib.load().llmops_cache_write_q4, *at, _LORA_TYPES[k.dtype], B, k.shape[1], Hkv, 128,
+               _ptr(inv_freq) if inv_freq is not None else None, inv_freq.shape[0] if inv_freq is not None else 0, _ptr(kv_cache), planes, maxlen, _ptr(lengths),
+               _ptr(q_lens) if q_lens is not None else None, int(layer_id))
+
+
+def cache_read_q4(kv_cache, rows, starts=None, dtype=torch.float16):
+    """What ``rows`` rows of a cache in 4 bits stand for, from row starts[b] (int32 [B], device; None: 0) of each sequence on: [2*layers,B,Hkv,rows,128]
+    in fp16 or fp32 (the values are halves: both are exact), the form of a cache in full width.  Rows outside the cache give 0."""
+    planes, B, Hkv, maxlen = _q4_cache(kv_cache)
+    _require(dtype in (torch.float32, torch.float16), "dtype is float32 or float16")
+    if starts is not None:
+        _dev(starts, torch.int32, 1, "starts")
+        _require(starts.shape[0] == B, "starts.is({B})")
+        _here(kv_cache, starts=starts)
+    rows = int(rows)
+    _require(rows >= 0, "rows >= 0")
+    out = torch.empty((planes, B, Hkv, rows, 128), dtype=dtype, device=kv_cache.device)
+    if out.numel():
+        _on_device(kv_cache.device, _lib.load().llmops_cache_read_q4, _ptr(kv_cache), planes, B, Hkv, maxlen, 128, _ptr(starts) if starts is not None else None, rows,
+                   _ptr(out), _LORA_TYPES[dtype])
+    return out
+
+
+def attention_rope_q4(q, k, v, inv_freq, kv_cache, lengths, layer_id, q_lens=None):
+    """Rotary, cache update and attention of a batch over a cache that is held in 4 bits (``cache_write_q4``), each sequence with as many rows as
+    ``lengths`` (int32 [B], device) says.
+
+    q fp32 [B,qL,H*128], k and v fp32 [B,qL,Hkv*128] (H a multiple of Hkv; columns of a projection's output will do), left as they are; kv_cache int8
+    [2*layers,B,Hkv,maxlen,80].  Token l of sequence b is at position lengths[b] + l; its rotated k and its v are quantised into that row, and it sees what the
+    rows up to that one stand for, its own among them.  ``lengths`` is not changed, and q_lens and padding are as in ``attention_rope_prefix``.
+    Returns fp32 [B,qL,H*128]."""
+    (qp, qb, ql), (kp, kb, kl), (vp, vb, vl) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    planes, B, Hkv, maxlen = _q4_cache(kv_cache)
+    _dev(inv_freq, torch.float32, 1, "inv_freq")
+    _q4_lengths(kv_cache, lengths, q_lens)
+    _here(q, k=k, v=v, inv_freq=inv_freq, kv_cache=kv_cache, lengths=lengths, q_lens=q_lens)
+    _require(q.shape[0] == B, "kv_cache.size(1) == B")
+    qL, width = q.shape[1:]
+    _require(width % 128 == 0, "q.size(2) % 128 == 0")
+    for t, n in ((k, "k"), (v, "v")):
+        _require(tuple(t.shape) == (B, qL, Hkv * 128), f"{n}.is({{B, qL, Hkv * 128}})")
+    lib = _lib.load()
+    H = width // 128
+    out = torch.empty((B, qL, width), dtype=torch.float32, device=q.device)
+    ws = torch.empty(max(lib.llmops_attention_q4_workspace_bytes(B, qL, H, Hkv, 128, maxlen), 1), dtype=torch.uint8, device=q.device)
+    _on_device(q.device, lib.llmops_attention_rope_q4, qp, qb, ql, kp, kb, kl, vp, vb, vl, B, qL, H, Hkv, 128, _ptr(inv_freq), inv_freq.shape[0],
+               _ptr(kv_cache), planes, maxlen, _ptr(lengths), _ptr(q_lens) if q_lens is not None else None, int(layer_id), _ptr(out), _ptr(ws), ws.numel())
+    return out
+
+
+def token_logprobs(logits, tokens, top=0):
+    """Log probabilities of given tokens, with the entropy of the distributions and the likeliest tokens beside them.
+
+    logits fp32 [B,L,V] (innermost dimension dense: a text's, without the last row, will do), tokens int64 or int32 [B,L] (any strides).  A token outside
+    0 .. V-1 is padding and has 0.  ``top``: how many of the likeliest tokens, 0 to 64 and at most V.  Logits that are NaN or minus infinity weigh nothing.
+
+    Returns (logprobs fp32 [B,L], entropy fp32 [B,L], top_tokens int64 [B,L,top], top_logprobs fp32 [B,L,top]), the likeliest first, equal
+    ones in the order of their numbers."""
+    zp, zb, zl = _rows(logits, "logits")
+    B, L, V = logits.shape
+    _require(isinstance(tokens, torch.Tensor) and tokens.is_cuda and tokens.dtype in (torch.int64, torch.int32), "tokens.is<int64_t>(2)")
+    _require(tuple(tokens.shape) == (B, L), "tokens.is({B, L})")
+    _here(logits, tokens=tokens)
+    top = int(top)
+    if tokens.dtype != torch.int64:
+        tokens = tokens.to(torch.int64)
+    lib = _lib.load()
+    logprobs, entropy, top_logprobs = (torch.empty(s, dtype=torch.float32, device=logits.device) for s in ((B, L), (B, L), (B, L, max(top, 0))))
+    top_tokens = torch.empty((B, L, max(top, 0)), dtype=torch.int64, device=logits.device)
+    ws = torch.empty(max(lib.llmops_token_logprobs_workspace_bytes(B, L, V, top), 1), dtype=torch.uint8, device=logits.device)
+    _on_device(logits.device, lib.llmops_token_logprobs, zp, zb, zl, B, L, V, _ptr(tokens), tokens.stride(0) if B > 1 else 0, tokens.stride(1) if L > 1 else 0,
+               top, _ptr(logprobs), _ptr(entropy), _ptr(top_tokens) if top > 0 else None, _ptr(top_logprobs) if top > 0 else None, _ptr(ws), ws.numel())
+    return logprobs, entropy, top_tokens, top_logprobs
 
 
 # ---- neighbours -------------------------------------------------------------------------------

@@ -57,6 +57,13 @@ SIGNATURES = {
                                 c_ptr, c_size, c_ptr]),
     "llmops_verify_drafts_workspace_bytes": (c_size, [c_i64] * 3),
     "llmops_verify_drafts": (c_int, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_f32, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
+    "llmops_cache_write_q4": (c_int, [c_ptr, c_i64, c_i64, c_i64] * 2 + [c_int] + [c_i64] * 4 + [c_ptr, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_int, c_ptr]),
+    "llmops_cache_read_q4": (c_int, [c_ptr] + [c_i64] * 5 + [c_ptr, c_i64, c_ptr, c_int, c_ptr]),
+    "llmops_attention_q4_workspace_bytes": (c_size, [c_i64] * 6),
+    "llmops_attention_rope_q4": (c_int, [c_ptr, c_i64, c_i64] * 3 + [c_i64] * 5 + [c_ptr, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_int, c_ptr, c_ptr,
+                                         c_size, c_ptr]),
+    "llmops_token_logprobs_workspace_bytes": (c_size, [c_i64] * 4),
+    "llmops_token_logprobs": (c_int, [c_ptr] + [c_i64] * 5 + [c_ptr] + [c_i64] * 3 + [c_ptr] * 5 + [c_size, c_ptr]),
     "llmops_softmax": (c_int, [c_ptr, c_i64, c_i64, c_ptr]),
     "llmops_mm_qk": (c_int, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_ptr]),
     "llmops_rmsnorm": (c_int, [c_ptr, c_i64, c_i64, c_ptr, c_f32, c_ptr]),

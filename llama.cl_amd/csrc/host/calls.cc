@@ -33,6 +33,12 @@ decltype(&llmops_lora_workspace_bytes) lora_workspace_bytes;
 decltype(&llmops_lora_add) lora;
 decltype(&llmops_verify_drafts_workspace_bytes) verify_workspace_bytes;
 decltype(&llmops_verify_drafts) verify;
+decltype(&llmops_cache_write_q4) write_q4;
+decltype(&llmops_cache_read_q4) read_q4;
+decltype(&llmops_attention_q4_workspace_bytes) q4_workspace_bytes;
+decltype(&llmops_attention_rope_q4) attention_q4;
+decltype(&llmops_token_logprobs_workspace_bytes) logprobs_workspace_bytes;
+decltype(&llmops_token_logprobs) logprobs;
 
 // a plain tensor with memory of its own on the HIP device
 bool plain_strided(PyObject* o, at::ScalarType type, int64_t dims) {
@@ -271,14 +277,147 @@ PyObject* call_verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// int8 [planes, B, Hkv, maxlen, LLMOPS_Q4_ROW_BYTES]
+bool q4_cache(PyObject* o) { return plain(o, at::kChar, 5) && THPVariable_Unpack(o).size(4) == LLMOPS_Q4_ROW_BYTES && THPVariable_Unpack(o).numel() > 0; }
+bool counts(PyObject* o, int64_t B) { return plain(o, at::kInt, 1) && THPVariable_Unpack(o).size(0) == B; }
+
+// cache_write_q4(k, v, kv_cache, lengths, layer_id, inv_freq, q_lens)
+PyObject* call_write_q4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t layer = 0;
+    if (n != 7 || !THPVariable_CheckExact(args[0]) || !THPVariable_CheckExact(args[1]) || !q4_cache(args[2]) || !whole(args[4], layer) ||
+        !(args[5] == Py_None || plain(args[5], at::kFloat, 1)) || !direct())
+        return not_ordinary();
+    const at::Tensor &c = THPVariable_Unpack(args[2]), &first = THPVariable_Unpack(args[0]);
+    const int64_t B = c.size(1), Hkv = c.size(2), S = 128;
+    const at::ScalarType type = first.scalar_type();
+    if ((type != at::kFloat && type != at::kHalf) || layer != (int)layer || !counts(args[3], B) || !(args[6] == Py_None || counts(args[6], B)) || first.dim() < 3)
+        return not_ordinary();
+    const int64_t L = first.size(1);
+    int64_t at[2][3];
+    for (int i = 0; i < 2; i++) {
+        const int64_t dims = THPVariable_Unpack(args[i]).dim();
+        if ((dims != 3 && dims != 4) || !plain_strided(args[i], type, dims)) return not_ordinary();
+        const at::Tensor& t = THPVariable_Unpack(args[i]);
+        if (t.size(0) != B || t.size(1) != L || L <= 0 || t.stride(-1) != 1 || (dims == 3 ? t.size(2) != Hkv * S : t.size(2) != Hkv || t.size(3) != S)) return not_ordinary();
+        at[i][0] = stride_of(t, 0), at[i][1] = stride_of(t, 1), at[i][2] = dims == 3 ? S : stride_of(t, 2);
+    }
+    if (!all_here({args[0], args[1], args[2], args[3], args[5], args[6]})) return not_ordinary();
+    const hipStream_t st = current_stream(c);
+    int rc = 0;
+    {
+        pybind11::gil_scoped_release others_run;
+        rc = write_q4(first.data_ptr(), at[0][0], at[0][1], at[0][2], THPVariable_Unpack(args[1]).data_ptr(), at[1][0], at[1][1], at[1][2],
+                      type == at::kFloat ? LLMOPS_F32 : LLMOPS_F16, B, L, Hkv, S, static_cast<const float*>(address(args[5])),
+                      args[5] == Py_None ? 0 : THPVariable_Unpack(args[5]).size(0), c.data_ptr(), c.size(0), c.size(3),
+                      static_cast<const int32_t*>(address(args[3])), static_cast<const int32_t*>(address(args[6])), (int)layer, st);
+    }
+    if (rc != 0) return refused();
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// cache_read_q4(kv_cache, rows, starts, whether to fp32)
+PyObject* call_read_q4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t rows = 0;
+    if (n != 4 || !q4_cache(args[0]) || !whole(args[1], rows) || rows <= 0 || !PyBool_Check(args[3]) || !direct()) return not_ordinary();
+    const at::Tensor& c = THPVariable_Unpack(args[0]);
+    if (!(args[2] == Py_None || counts(args[2], c.size(1))) || !all_here({args[0], args[2]})) return not_ordinary();
+    const bool full = args[3] == Py_True;
+    const hipStream_t st = current_stream(c);
+    at::Tensor out = at::empty({c.size(0), c.size(1), c.size(2), rows, 128}, c.options().dtype(full ? at::kFloat : at::kHalf).requires_grad(false));
+    int rc = 0;
+    {
+        pybind11::gil_scoped_release others_run;
+        rc = read_q4(c.data_ptr(), c.size(0), c.size(1), c.size(2), c.size(3), 128, static_cast<const int32_t*>(address(args[2])), rows, out.data_ptr(),
+                     full ? LLMOPS_F32 : LLMOPS_F16, st);
+    }
+    if (rc != 0) return refused();
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// attention_rope_q4(q, k, v, inv_freq, kv_cache, lengths, layer_id, q_lens)
+PyObject* call_attention_q4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t layer = 0;
+    if (n != 8 || !plain_rows(args[0]) || !plain_rows(args[1]) || !plain_rows(args[2]) || !plain(args[3], at::kFloat, 1) || !q4_cache(args[4]) ||
+        !whole(args[6], layer) || !direct())
+        return not_ordinary();
+    const at::Tensor &q = THPVariable_Unpack(args[0]), &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]), &f = THPVariable_Unpack(args[3]),
+                     &c = THPVariable_Unpack(args[4]);
+    const int64_t B = c.size(1), qL = q.size(1), planes = c.size(0), Hkv = c.size(2), maxlen = c.size(3), S = 128;
+    if (q.size(0) != B || q.size(2) % S != 0 || k.size(0) != B || k.size(1) != qL || k.size(2) != Hkv * S || k.sizes() != v.sizes() || layer != (int)layer ||
+        !counts(args[5], B) || !(args[7] == Py_None || counts(args[7], B)) || !all_here({args[0], args[1], args[2], args[3], args[4], args[5], args[7]}))
+        return not_ordinary();
+    const int64_t H = q.size(2) / S;
+    const hipStream_t st = current_stream(q);
+    at::Tensor out = at::empty({B, qL, H * S}, q.options().requires_grad(false));
+    const at::Tensor ws = scratch(q, q4_workspace_bytes(B, qL, H, Hkv, S, maxlen));
+    int rc = 0;
+    {
+        pybind11::gil_scoped_release others_run;
+        rc = attention_q4(static_cast<const float*>(q.data_ptr()), stride_of(q, 0), stride_of(q, 1), static_cast<const float*>(k.data_ptr()), stride_of(k, 0),
+                          stride_of(k, 1), static_cast<const float*>(v.data_ptr()), stride_of(v, 0), stride_of(v, 1), B, qL, H, Hkv, S,
+                          static_cast<const float*>(f.data_ptr()), f.size(0), c.data_ptr(), planes, maxlen, static_cast<const int32_t*>(address(args[5])),
+                          static_cast<const int32_t*>(address(args[7])), (int)layer, static_cast<float*>(out.data_ptr()), ws.data_ptr(), (size_t)ws.numel(), st);
+    }
+    if (rc != 0) return refused();
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// token_logprobs(logits, tokens, top) with tokens int64
+PyObject* call_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t top = 0;
+    if (n != 3 || !plain_rows(args[0]) || !plain_strided(args[1], at::kLong, 2) || !whole(args[2], top) || top < 0 || top > 64 || !direct()) return not_ordinary();
+    const at::Tensor &z = THPVariable_Unpack(args[0]), &t = THPVariable_Unpack(args[1]);
+    const int64_t B = z.size(0), L = z.size(1), V = z.size(2);
+    if (t.size(0) != B || t.size(1) != L || !all_here({args[0], args[1]})) return not_ordinary();
+    const hipStream_t st = current_stream(z);
+    const auto real = z.options().requires_grad(false);
+    at::Tensor out[4] = {at::empty({B, L}, real), at::empty({B, L}, real), at::empty({B, L, top}, real.dtype(at::kLong)), at::empty({B, L, top}, real)};
+    const at::Tensor ws = scratch(z, logprobs_workspace_bytes(B, L, V, top));
+    int rc = 0;
+    {
+        pybind11::gil_scoped_release others_run;
+        rc = logprobs(static_cast<const float*>(z.data_ptr()), stride_of(z, 0), stride_of(z, 1), B, L, V, static_cast<const int64_t*>(t.data_ptr()), stride_of(t, 0),
+                      stride_of(t, 1), top, static_cast<float*>(out[0].data_ptr()), static_cast<float*>(out[1].data_ptr()),
+                      top > 0 ? static_cast<int64_t*>(out[2].data_ptr()) : nullptr, top > 0 ? static_cast<float*>(out[3].data_ptr()) : nullptr, ws.data_ptr(),
+                      (size_t)ws.numel(), st);
+    }
+    if (rc != 0) return refused();
+    PyObject* all = PyTuple_New(4);
+    for (int i = 0; all != nullptr && i < 4; i++) {
+        PyObject* one = THPVariable_Wrap(std::move(out[i]));
+        if (one == nullptr) {
+            Py_DECREF(all);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(all, i, one);
+    }
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(addresses of the C entries, in the order of the variables above)
 PyObject* bind(PyObject*, PyObject* args) {
-    unsigned long long a[11];
-    if (!PyArg_ParseTuple(args, "KKKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10])) return nullptr;
+    unsigned long long a[17];
+    if (PyTuple_GET_SIZE(args) != 17) {
+        PyErr_SetString(PyExc_TypeError, "bind: the addresses of 17 entries");
+        return nullptr;
+    }
+    for (int j = 0; j < 17; j++) {
+        a[j] = PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(args, j));
+        if (PyErr_Occurred()) return nullptr;
+    }
     int i = 0;
     auto take = [&](auto& entry) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>((uintptr_t)a[i++]); };
     take(fc_workspace_bytes), take(fc), take(attention_workspace_bytes), take(attention), take(last_error);
     take(prefix_workspace_bytes), take(attention_prefix), take(lora_workspace_bytes), take(lora), take(verify_workspace_bytes), take(verify);
+    take(write_q4), take(read_q4), take(q4_workspace_bytes), take(attention_q4), take(logprobs_workspace_bytes), take(logprobs);
     Py_RETURN_NONE;
 }
 
@@ -288,6 +427,10 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          {"attention_rope_prefix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_attention_prefix)), METH_FASTCALL, nullptr},
                          {"lora_add", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_lora)), METH_FASTCALL, nullptr},
                          {"verify_drafts", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_verify)), METH_FASTCALL, nullptr},
+                         {"cache_write_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_write_q4)), METH_FASTCALL, nullptr},
+                         {"cache_read_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_read_q4)), METH_FASTCALL, nullptr},
+                         {"attention_rope_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_attention_q4)), METH_FASTCALL, nullptr},
+                         {"token_logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call_logprobs)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -702,6 +702,8 @@ def cache_write_q4(k, v, kv_cache, lengths, layer_id, inv_freq=None, q_lens=None
     int8 [2*layers,B,Hkv,maxlen,80].  Token l of sequence b goes to row lengths[b] + l (int32 [B], device, not changed); with ``inv_freq`` k is rotated by
     that row's number, without it comes rotated.  q_lens (int32 [B], device): a sequence brings that many of the L tokens; the rest,
     and tokens that do not fit the cache, are left out."""
+    if (_lib._host or _lib.host()).cache_write_q4(k, v, kv_cache, lengths, layer_id, inv_freq, q_lens) is not NotImplemented:  # (the ordinary call, in native code)
+        return
     planes, B, Hkv, maxlen = _q4_cache(kv_cache)
     at = []
     for t, n in ((k, "k"), (v, "v")):
@@ -722,6 +724,10 @@ def cache_write_q4(k, v, kv_cache, lengths, layer_id, inv_freq=None, q_lens=None
 def cache_read_q4(kv_cache, rows, starts=None, dtype=torch.float16):
     """What ``rows`` rows of a cache in 4 bits stand for, from row starts[b] (int32 [B], device; None: 0) of each sequence on: [2*layers,B,Hkv,rows,128]
     in fp16 or fp32 (the values are halves: both are exact), the form of a cache in full width.  Rows outside the cache give 0."""
+    if dtype is torch.float16 or dtype is torch.float32:
+        out = (_lib._host or _lib.host()).cache_read_q4(kv_cache, rows, starts, dtype is torch.float32)
+        if out is not NotImplemented:  # (as above)
+            return out
     planes, B, Hkv, maxlen = _q4_cache(kv_cache)
     _require(dtype in (torch.float32, torch.float16), "dtype is float32 or float16")
     if starts is not None:
@@ -745,6 +751,9 @@ def attention_rope_q4(q, k, v, inv_freq, kv_cache, lengths, layer_id, q_lens=Non
     [2*layers,B,Hkv,maxlen,80].  Token l of sequence b is at position lengths[b] + l; its rotated k and its v are quantised into that row, and it sees what the
     rows up to that one stand for, its own among them.  ``lengths`` is not changed, and q_lens and padding are as in ``attention_rope_prefix``.
     Returns fp32 [B,qL,H*128]."""
+    out = (_lib._host or _lib.host()).attention_rope_q4(q, k, v, inv_freq, kv_cache, lengths, layer_id, q_lens)
+    if out is not NotImplemented:  # (as above)
+        return out
     (qp, qb, ql), (kp, kb, kl), (vp, vb, vl) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
     planes, B, Hkv, maxlen = _q4_cache(kv_cache)
     _dev(inv_freq, torch.float32, 1, "inv_freq")
@@ -772,6 +781,9 @@ def token_logprobs(logits, tokens, top=0):
 
     Returns (logprobs fp32 [B,L], entropy fp32 [B,L], top_tokens int64 [B,L,top], top_logprobs fp32 [B,L,top]), the likeliest first, equal
     ones in the order of their numbers."""
+    done = (_lib._host or _lib.host()).token_logprobs(logits, tokens, top)
+    if done is not NotImplemented:  # (as above)
+        return done
     zp, zb, zl = _rows(logits, "logits")
     B, L, V = logits.shape
     _require(isinstance(tokens, torch.Tensor) and tokens.is_cuda and tokens.dtype in (torch.int64, torch.int32), "tokens.is<int64_t>(2)")

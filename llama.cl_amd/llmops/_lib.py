@@ -129,6 +129,7 @@ class _PythonCalls:
         return NotImplemented
 
     attention_rope2 = attention_rope_prefix = lora_add = verify_drafts = fc_Q4A
+    cache_write_q4 = cache_read_q4 = attention_rope_q4 = token_logprobs = fc_Q4A
 
 
 def host():
@@ -151,7 +152,8 @@ def host():
         native.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "llmops_fc_Q4A_workspace_bytes", "llmops_fc_Q4A", "llmops_attention_workspace_bytes", "llmops_attention_rope",
             "llmops_last_error", "llmops_attention_prefix_workspace_bytes", "llmops_attention_rope_prefix", "llmops_lora_workspace_bytes",
-            "llmops_lora_add", "llmops_verify_drafts_workspace_bytes", "llmops_verify_drafts")))
+            "llmops_lora_add", "llmops_verify_drafts_workspace_bytes", "llmops_verify_drafts", "llmops_cache_write_q4", "llmops_cache_read_q4",
+            "llmops_attention_q4_workspace_bytes", "llmops_attention_rope_q4", "llmops_token_logprobs_workspace_bytes", "llmops_token_logprobs")))
         _host = native
     return _host
 

@@ -7,40 +7,76 @@
 //   1. logprob_runs_kernel   a run of a row to a workgroup, whose logits stay in registers: maximum, both sums, its likeliest tokens
 //   2. logprob_rows_kernel   joins a row's runs
 //
-// The likeliest of a run: the `top` largest of the threads' own maxima bound what can be among them, which leaves little more than `top`
-// logits (and top * E at most, all from those threads); each of these counts how many others are before it.
+// The likeliest of a run: the `top`-th largest of the 64 lanes' own maxima is found in each wave bit by bit (a comparison and a count of lanes for each
+// bit, most of it on the scalar unit), and no logit below the largest of the four waves' can be among them; that leaves some 3 * top logits, of which each
+// counts how many others are before it.  Rows of equal logits leave more; where that is more than there is room for, the same search goes over all
+// logits and then over the numbers of those that are equal to the last.
 // fp32 sums over a thread's logits and a workgroup's threads; runs are joined, and logarithms taken, in 64 bits.
+#include <limits.h>
+
 #include "common.h"
 #include "extents.h"
 #include "gemv_device.h"
 
 namespace llmops {
 
-constexpr int kMostTop = 64;
+constexpr int kMostTop = 64, kHeld = 1024;  // (logits that there is room for)
 
 struct LogprobArgs {
     const float* logits;
     const int64_t* tokens;
     int64_t lsb, lsl, tsb, tsl;  // strides, elements
     int L, V, runs, top;
-    float4* stat;      // [rows][runs]: M, S, sum exp(z - M) (z - M)
-    float* best;       // [rows][runs][top]
-    int32_t* best_at;  // [rows][runs][top]
+    float4* stat;       // [rows][runs]: M, S, sum exp(z - M) (z - M)
+    struct Held* best;  // [rows][runs][top]
     float *logprobs, *entropy, *top_logprobs;
     int64_t* top_tokens;
 };
 
-// NaN and minus infinity are one and the same: nothing
+// Logits as whole numbers in their order; NaN and minus infinity are one and the same (nothing), and so are zeros of either sign
 __device__ __forceinline__ float something(float z) { return fmaxf(z, -INFINITY); }
-__device__ __forceinline__ bool ahead(float v, int at, float w, int wat) { return v > w || (v == w && at < wat); }
+__device__ __forceinline__ uint32_t rank_key(float z) {
+    const uint32_t u = __float_as_uint(something(z) + 0.0f);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+// a logit and its token, of which (key, -token) counts
+struct Held {
+    uint32_t key;
+    int32_t at;
+};
+__device__ __forceinline__ int is_ahead(Held a, Held b) { return a.key > b.key || (a.key == b.key && a.at < b.at) ? 1 : 0; }
+// how many of `held` (n, and up to three that are nothing behind them) are before one of them
+__device__ __forceinline__ int how_many_ahead(const Held* held, int n, Held one) {
+    int before = 0;
+    for (int t = 0; t < n; t += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(held + t), y = *reinterpret_cast<const uint4*>(held + t + 2);
+        before += is_ahead({x.x, (int)x.y}, one) + is_ahead({x.z, (int)x.w}, one) + is_ahead({y.x, (int)y.y}, one) + is_ahead({y.z, (int)y.w}, one);
+    }
+    return before;
+}
+__device__ __forceinline__ Held nothing_held() { return {0u, INT_MAX}; }
+
+// the workgroup's count of what its threads' E values hold true
+template <int E, typename F>
+__device__ __forceinline__ int count_all(int* sums, F is) {
+    int mine = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) mine += (int)__builtin_popcountll(__ballot(is(e)));
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    const int all = sums[0] + sums[1] + sums[2] + sums[3];
+    __syncthreads();
+    return all;
+}
 
 template <int E>
 __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
-    __shared__ float red[3][4], most[256];
-    __shared__ int most_at[256];
-    __shared__ float held[E * kMostTop];
-    __shared__ int held_at[E * kMostTop], count, bound_at;
-    __shared__ float bound;
+    __shared__ float red[3][4];
+    __shared__ int sums[4], count;
+    __shared__ uint32_t bounds[4];
+    __shared__ __align__(16) Held held[kHeld + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = blockIdx.x / a.runs, run = blockIdx.x - row * a.runs, b = row / a.L, l = row - b * a.L;
     const float* z = a.logits + b * a.lsb + l * a.lsl;
@@ -61,6 +97,17 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
     for (int e = 0; e < E; e++) own = fmaxf(own, x[e]);
     const float wave_top = wave_max(own);
     if (lane == 0) red[0][wave] = wave_top;
+    if (a.top > 0) {
+        const uint32_t key = rank_key(own);
+        uint32_t bound = 0;
+#pragma unroll 1
+        for (int bit = 31; bit >= 0; bit--) {
+            const uint32_t more = bound | 1u << bit;
+            if ((int)__builtin_popcountll(__ballot(key >= more)) >= a.top) bound = more;
+        }
+        if (lane == 0) bounds[wave] = bound;
+    }
+    if (threadIdx.x == 0) count = 0;
     __syncthreads();
     const float M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
     float S = 0.0f, T = 0.0f;
@@ -77,109 +124,144 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
     }
     S = wave_sum(S), T = wave_sum(T);
     if (lane == 0) red[1][wave] = S, red[2][wave] = T;
+    auto at = [&](int e) { return base + 1024 * (e >> 2) + (e & 3); };
     if (a.top > 0) {
-        int at = 0;
+        const uint32_t bound = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
+        if (rank_key(own) >= bound) {
 #pragma unroll
-        for (int e = E - 1; e >= 0; e--) at = something(x[e]) == own ? e : at;
-        most[threadIdx.x] = own, most_at[threadIdx.x] = base + 1024 * (at >> 2) + (at & 3);
-    }
-    if (threadIdx.x == 0) count = 0;
-    __syncthreads();
-    if (threadIdx.x == 0) a.stat[(int64_t)row * a.runs + run] = make_float4(M, red[1][0] + red[1][1] + red[1][2] + red[1][3], red[2][0] + red[2][1] + red[2][2] + red[2][3], 0.0f);
-    if (a.top == 0) return;
-    {
-        int before = 0;
-        const int mine = most_at[threadIdx.x];
-        for (int t = 0; t < 256; t++) before += ahead(most[t], most_at[t], own, mine) ? 1 : 0;
-        if (before == a.top - 1) bound = own, bound_at = mine;
-    }
-    __syncthreads();
-    const float least = bound;
-    const int least_at = bound_at;
-    if (!ahead(least, least_at, own, most_at[threadIdx.x])) {
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int at = base + 1024 * (e >> 2) + (e & 3);
-            const float v = something(x[e]);
-            if (!ahead(least, least_at, v, at)) {
-                const int slot = atomicAdd(&count, 1);
-                held[slot] = v, held_at[slot] = at;
+            for (int e = 0; e < E; e++) {
+                const uint32_t key = rank_key(x[e]);
+                if (key >= bound) {
+                    const int slot = atomicAdd(&count, 1);
+                    if (slot < kHeld) held[slot] = {key, at(e)};
+                }
             }
         }
     }
     __syncthreads();
+    if (threadIdx.x == 0) a.stat[(int64_t)row * a.runs + run] = make_float4(M, red[1][0] + red[1][1] + red[1][2] + red[1][3], red[2][0] + red[2][1] + red[2][2] + red[2][3], 0.0f);
+    if (a.top == 0) return;
+    if (count > kHeld) {  // (the same in all threads)
+        uint32_t last = 0;
+#pragma unroll 1
+        for (int bit = 31; bit >= 0; bit--) {
+            const uint32_t more = last | 1u << bit;
+            if (count_all<E>(sums, [&](int e) { return rank_key(x[e]) >= more; }) >= a.top) last = more;
+        }
+        const int equals = a.top - count_all<E>(sums, [&](int e) { return rank_key(x[e]) > last; });
+        int upto = 0;  // the largest number below which there are too few of them
+#pragma unroll 1
+        for (int bit = 27; bit >= 0; bit--) {
+            const int more = upto | 1 << bit;
+            if (count_all<E>(sums, [&](int e) { return rank_key(x[e]) == last && at(e) < more; }) < equals) upto = more;
+        }
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const uint32_t key = rank_key(x[e]);
+            if (key > last || (key == last && at(e) <= upto)) held[atomicAdd(&count, 1)] = {key, at(e)};
+        }
+        __syncthreads();
+    }
     const int n = count;
+    if (threadIdx.x < 4) held[n + threadIdx.x] = nothing_held();
+    __syncthreads();
     const int64_t to = ((int64_t)row * a.runs + run) * a.top;
     for (int c = threadIdx.x; c < n; c += 256) {
-        const float v = held[c];
-        const int at = held_at[c];
-        int before = 0;
-        for (int t = 0; t < n; t++) before += ahead(held[t], held_at[t], v, at) ? 1 : 0;
-        if (before < a.top) a.best[to + before] = v, a.best_at[to + before] = at;
+        const int before = how_many_ahead(held, n, held[c]);
+        if (before < a.top) a.best[to + before] = held[c];
     }
 }
 
-// a workgroup to a row
-__global__ __launch_bounds__(256) void logprob_rows_kernel(LogprobArgs a) {
-    __shared__ double red[3][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x, b = row / a.L, l = row - b * a.L;
-    const float* z = a.logits + b * a.lsb + l * a.lsl;
-    const int64_t token = a.tokens[b * a.tsb + l * a.tsl];
-    const bool real = token >= 0 && token < a.V;
-    const float its = real ? something(z[token]) : 0.0f;
+// A row's runs, in one wave: its top, its logarithm of the sum and its entropy
+struct RowSums {
+    float M;
+    double log_s, entropy;
+};
+__device__ __forceinline__ RowSums row_sums(const LogprobArgs& a, int row, int lane) {
     const float4* stat = a.stat + (int64_t)row * a.runs;
-    float top = -INFINITY;
-    for (int r = threadIdx.x; r < a.runs; r += 256) top = fmaxf(top, stat[r].x);
-    top = wave_max(top);
-    if (lane == 0) red[0][wave] = top;
-    __syncthreads();
-    const float M = (float)fmax(fmax(red[0][0], red[0][1]), fmax(red[0][2], red[0][3]));
+    float4 s = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    if (lane < a.runs) s = stat[lane];
+    float M = s.x;
+    for (int r = lane + 64; r < a.runs; r += 64) M = fmaxf(M, stat[r].x);
+    M = wave_max(M);
     double S = 0.0, T = 0.0;
-    for (int r = threadIdx.x; r < a.runs; r += 256) {
-        const float4 s = stat[r];
+    for (int r = lane; r < a.runs; r += 64) {
+        if (r >= 64) s = stat[r];
         if (s.x == -INFINITY) continue;
-        const double lower = s.x == M ? 0.0 : (double)s.x - (double)M, w = exp(lower);  // (a run below one with plus infinity: 0 * -inf)
+        const double lower = s.x == M ? 0.0 : (double)s.x - (double)M, w = s.x == M ? 1.0 : exp(lower);  // (a run below one with plus infinity: 0 * -inf)
         S += w * s.y;
         if (w > 0.0) T += w * ((double)s.z + lower * s.y);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) S += __shfl_xor(S, o, 64), T += __shfl_xor(T, o, 64);
-    if (lane == 0) red[1][wave] = S, red[2][wave] = T;
-    __syncthreads();
-    S = red[1][0] + red[1][1] + red[1][2] + red[1][3], T = red[2][0] + red[2][1] + red[2][2] + red[2][3];
     const double log_s = M == -INFINITY ? NAN : log(S);
-    auto logprob = [&](float v) { return (float)((v == M ? 0.0 : (double)v - (double)M) - log_s); };
-    if (threadIdx.x == 0) {
-        a.logprobs[row] = real ? logprob(its) : 0.0f;
-        a.entropy[row] = (float)(log_s - T / S);
+    return {M, log_s, log_s - T / S};
+}
+__device__ __forceinline__ float logprob_of(const RowSums& s, float v) { return (float)((v == s.M ? 0.0 : (double)v - (double)s.M) - s.log_s); }
+__device__ __forceinline__ void row_answers(const LogprobArgs& a, int row, int lane, RowSums& s) {
+    const int b = row / a.L, l = row - b * a.L;
+    const int64_t token = a.tokens[b * a.tsb + l * a.tsl];
+    const bool real = token >= 0 && token < a.V;
+    const float its = real ? something(a.logits[b * a.lsb + l * a.lsl + token]) : 0.0f;
+    s = row_sums(a, row, lane);
+    if (lane == 0) a.logprobs[row] = real ? logprob_of(s, its) : 0.0f, a.entropy[row] = (float)s.entropy;
+}
+
+// without likeliest tokens: a wave to a row
+__global__ __launch_bounds__(256) void logprob_sums_kernel(LogprobArgs a, int rows) {
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    RowSums s;
+    if (row < rows) row_answers(a, row, threadIdx.x & 63, s);
+}
+
+// a workgroup to a row: one wave its sums, all its likeliest tokens, those of 512 / top runs after the other
+__global__ __launch_bounds__(256) void logprob_rows_kernel(LogprobArgs a) {
+    __shared__ __align__(16) Held held[512 + kMostTop + 4], best[kMostTop];
+    __shared__ RowSums sums;
+    const int row = blockIdx.x;
+    const int64_t n = (int64_t)a.runs * a.top;
+    const Held* from = a.best + (int64_t)row * n;
+    int kept = 0;
+    for (int64_t c0 = 0; c0 < n; c0 += 512) {
+        const int more = (int)min((int64_t)512, n - c0), m = more + kept;
+        for (int c = threadIdx.x; c < more + 4; c += 256) held[kept + c] = c < more ? from[c0 + c] : nothing_held();
+        if ((int)threadIdx.x < kept) held[threadIdx.x] = best[threadIdx.x];
+        __syncthreads();
+        for (int c = threadIdx.x; c < m; c += 256) {
+            const int before = how_many_ahead(held, m, held[c]);
+            if (before < a.top) best[before] = held[c];
+        }
+        kept = min(m, a.top);
+        __syncthreads();
     }
-    const int n = a.runs * a.top;
-    const float* best = a.best + (int64_t)row * n;
-    const int32_t* best_at = a.best_at + (int64_t)row * n;
-    for (int c = threadIdx.x; c < n; c += 256) {
-        const float v = best[c];
-        const int at = best_at[c];
-        int before = 0;
-        for (int t = 0; t < n; t++) before += ahead(best[t], best_at[t], v, at) ? 1 : 0;
-        if (before < a.top) a.top_tokens[(int64_t)row * a.top + before] = at, a.top_logprobs[(int64_t)row * a.top + before] = logprob(v);
+    if (threadIdx.x < 64) {
+        RowSums s;
+        row_answers(a, row, threadIdx.x, s);
+        if (threadIdx.x == 0) sums = s;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < a.top) {
+        a.top_tokens[(int64_t)row * a.top + threadIdx.x] = best[threadIdx.x].at;
+        a.top_logprobs[(int64_t)row * a.top + threadIdx.x] = logprob_of(sums, of_key(best[threadIdx.x].key));
     }
 }
 
-// logits to a thread: eight where that leaves workgroups for the whole chip
-static int logprob_each(int64_t rows, int64_t V) { return rows * ((V + 2047) / 2048) <= 1024 ? 8 : 32; }
+// logits to a thread: eight where that is the whole row
+static int logprob_each(int64_t V) { return V <= 2048 ? 8 : 32; }
 
 struct LogprobLayout {
-    size_t stat, best, best_at, total;
+    size_t stat, best, total;
     int64_t runs;
 };
 static LogprobLayout layout_logprobs(int64_t rows, int64_t V, int64_t top) {
     LogprobLayout w{};
-    const int64_t run = 256 * logprob_each(rows, V);
+    const int64_t run = 256 * logprob_each(V);
     w.runs = (V + run - 1) / run;
     w.stat = 0;
     w.best = w.stat + (size_t)(rows * w.runs) * 16;
-    w.best_at = w.best + (size_t)(rows * w.runs * top) * 4;
-    w.total = w.best_at + (size_t)(rows * w.runs * top) * 4;
+    w.total = w.best + (size_t)(rows * w.runs * top) * 8;
     return w;
 }
 
@@ -219,14 +301,15 @@ extern "C" int llmops_token_logprobs(const float* logits, int64_t stride_b, int6
     }
     char* ws = reinterpret_cast<char*>(workspace);
     LogprobArgs a{logits, tokens, stride_b, stride_l, token_stride_b, token_stride_l, (int)L, (int)V, (int)w.runs, (int)top};
-    a.stat = reinterpret_cast<float4*>(ws + w.stat), a.best = reinterpret_cast<float*>(ws + w.best), a.best_at = reinterpret_cast<int32_t*>(ws + w.best_at);
+    a.stat = reinterpret_cast<float4*>(ws + w.stat), a.best = reinterpret_cast<Held*>(ws + w.best);
     a.logprobs = logprobs, a.entropy = entropy, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
     hipStream_t st = as_stream(stream);
     const unsigned grid = (unsigned)(B * L * w.runs);
-    if (logprob_each(B * L, V) == 8) logprob_runs_kernel<8><<<grid, 256, 0, st>>>(a);
+    if (logprob_each(V) == 8) logprob_runs_kernel<8><<<grid, 256, 0, st>>>(a);
     else logprob_runs_kernel<32><<<grid, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
-    logprob_rows_kernel<<<(unsigned)(B * L), 256, 0, st>>>(a);
+    if (top > 0) logprob_rows_kernel<<<(unsigned)(B * L), 256, 0, st>>>(a);
+    else logprob_sums_kernel<<<(unsigned)((B * L + 3) / 4), 256, 0, st>>>(a, (int)(B * L));
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }

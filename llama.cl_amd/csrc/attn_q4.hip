@@ -100,18 +100,18 @@ struct Q4Regs {
             vdm[j] = ask4(r, pairs, (16 * (j >> 2) + (j & 3)) * kQ4Row);
         }
     }
-    __device__ __forceinline__ v8h k_op(int tt, int step) const {
-        return values8(step == 0 ? k[tt].x : step == 1 ? k[tt].y : step == 2 ? k[tt].z : k[tt].w, kdm[tt]);
+    __device__ __forceinline__ v8h k_op(const Codes& codes, int tt, int step) const {
+        return codes.values(step == 0 ? k[tt].x : step == 1 ? k[tt].y : step == 2 ? k[tt].z : k[tt].w, kdm[tt]);
     }
     // the operands of two products from byte y of the eight words: codes 0 2, 4 6, 1 3, 5 7
-    __device__ __forceinline__ void v_ops(int y, v8h& low, v8h& high) const {
+    __device__ __forceinline__ void v_ops(const Codes& codes, int y, v8h& low, v8h& high) const {
         const uint32_t pick = 0x0c000c00u | (uint32_t)(4 + y) << 16 | (uint32_t)y;
 #pragma unroll
         for (int p = 0; p < 4; p++) {
             const uint32_t x = __builtin_amdgcn_perm(v[2 * p + 1], v[2 * p], pick);
             const v2h d = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(vdm[2 * p + 1], vdm[2 * p], 0x05040100u)),
                       m = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(vdm[2 * p + 1], vdm[2 * p], 0x07060302u));
-            const v2h lo = __builtin_elementwise_fma(pair_low(x), d, m), hi = __builtin_elementwise_fma(pair_high(x), d, m);
+            const v2h lo = __builtin_elementwise_fma(codes.low(x), d, m), hi = __builtin_elementwise_fma(codes.high(x), d, m);
             low[2 * p] = lo[0], low[2 * p + 1] = lo[1], high[2 * p] = hi[0], high[2 * p + 1] = hi[1];
         }
     }
@@ -125,29 +125,14 @@ struct Q4Regs {
 };
 __device__ __forceinline__ constexpr int first_code(int y) { return y == 0 ? 0 : y == 1 ? 4 : y == 2 ? 1 : 5; }  // of byte y; the other is 2 more
 
+// the queries' operands, in LDS: the four waves share them, and leave registers for a fourth wave on a SIMD
 template <int RT>
-struct Q4QueryOps;
-template <>
-struct Q4QueryOps<1> {
-    v8h h[4], l[4];
-    __device__ __forceinline__ void load(const Q4Args& a, uint4*, int hk, int m0, int m_end, int lane) {
-        const int64_t at = ((int64_t)hk * a.M + min(m0 + (lane & 15), m_end - 1)) * kS + 32 * (lane >> 4);
-#pragma unroll
-        for (int step = 0; step < 4; step++) {
-            h[step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + at + 8 * step));
-            l[step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + at + 8 * step));
-        }
-    }
-    __device__ __forceinline__ v8h hi(int, int step) const { return h[step]; }
-    __device__ __forceinline__ v8h lo(int, int step) const { return l[step]; }
-};
-template <>
-struct Q4QueryOps<2> {
+struct Q4QueryOps {
     const uint4* mine;
     __device__ __forceinline__ void load(const Q4Args& a, uint4* lds, int hk, int m0, int m_end, int lane) {
         const int wave = threadIdx.x >> 6;  // a step to a wave
 #pragma unroll
-        for (int rt = 0; rt < 2; rt++) {
+        for (int rt = 0; rt < RT; rt++) {
             const int64_t at = ((int64_t)hk * a.M + min(m0 + 16 * rt + (lane & 15), m_end - 1)) * kS + 32 * (lane >> 4) + 8 * wave;
             lds[(rt * 8 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.qh + at);
             lds[(rt * 8 + 4 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.ql + at);
@@ -160,11 +145,13 @@ struct Q4QueryOps<2> {
 };
 
 // Units of 128 rows are numbered through: sequence after sequence, in each kv head after kv head, in each tile after tile.  A sequence without
-// rows (padding) has one unit for each all the same, in which its zeros are written.
+// rows (padding) has one unit for each all the same, in which its zeros are written.  Behind the units of a tile there are kStart more
+// without rows, for what it costs to begin with queries and to bring the waves' sums together, so that workgroups with short sequences have no more to do.
+constexpr int kStart = 1;
 __device__ __forceinline__ int units_of(const Q4Args& a, int b) {
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-    return n > 0 ? (len + n + kUnit - 1) / kUnit : 1;
+    return (n > 0 ? (len + n + kUnit - 1) / kUnit : 1) + kStart;
 }
 __device__ __forceinline__ int wave_scan(int v, int lane) {
 #pragma unroll
@@ -232,9 +219,10 @@ struct Q4MeetSmem {
 // Few queries to a workgroup (16 * RT).  The four waves take 32 rows each of every 128; operands come straight from memory, the next rows asked
 // for when these are used up; the waves' sums meet in LDS.
 template <int RT>
-__global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void q4_few_kernel(Q4Args a) {
+__global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) {
     __shared__ Q4MeetSmem sm;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    const Codes codes;
     int share = 0;
     const UnitPlace start = place_of(a, lane, true, [&](int all) { share = share_of(all, a.groups); return (int)min((int64_t)blockIdx.x * share, (int64_t)INT_MAX); });
     if (start.b < 0) return;
@@ -248,6 +236,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void q4_few_kernel(Q4Args a) 
         }
         const int item = (at - before) / units, u0 = at - before - item * units, u1 = min(units, u0 + last - at), hk = item / a.tiles, tile = item - hk * a.tiles;
         at += u1 - u0;
+        if (u0 >= units - kStart) continue;
         int len, n;
         own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
         const int m0 = b * a.Mq + tile * 16 * RT, m_end = min((b + 1) * a.Mq, m0 + 16 * RT);
@@ -280,14 +269,14 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void q4_few_kernel(Q4Args a) 
             for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int step = 0; step < 4; step++) {
+                const v8h k0 = x.k_op(codes, 0, step), k1 = x.k_op(codes, 1, step);
 #pragma unroll
-                for (int tt = 0; tt < 2; tt++) {
-                    const v8h k = x.k_op(tt, step);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        sc[rt][tt] = mfma(k, q.hi(rt, step), sc[rt][tt]);
-                        sc[rt][tt] = mfma(k, q.lo(rt, step), sc[rt][tt]);
-                    }
+                for (int rt = 0; rt < RT; rt++) {
+                    const v8h hi = q.hi(rt, step), lo = q.lo(rt, step);
+                    sc[rt][0] = mfma(k0, hi, sc[rt][0]);
+                    sc[rt][1] = mfma(k1, hi, sc[rt][1]);
+                    sc[rt][0] = mfma(k0, lo, sc[rt][0]);
+                    sc[rt][1] = mfma(k1, lo, sc[rt][1]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -307,7 +296,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void q4_few_kernel(Q4Args a) 
 #pragma unroll
             for (int y = 0; y < 4; y++) {
                 v8h low, high;
-                x.v_ops(y, low, high);
+                x.v_ops(codes, y, low, high);
                 const int c = first_code(y);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
@@ -328,7 +317,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 3 : 2) void q4_few_kernel(Q4Args a) 
             if (g == 0) sm.m[wave][16 * rt + i] = s.m[rt], sm.l[wave][16 * rt + i] = s.l[rt];
         }
         __syncthreads();
-        const bool whole = u0 == 0 && u1 == units;
+        const bool whole = u0 == 0 && u1 >= units - kStart;
         const int64_t record = ((int64_t)blockIdx.x * 2 + (u0 == 0)) * (16 * RT);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
@@ -381,7 +370,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
     const int64_t r = blockIdx.x;
     const int hk = (int)(r / a.M), m = (int)(r - (int64_t)hk * a.M), b = m / a.Mq, in = m - b * a.Mq, tile = in / (16 * RT), l = in / a.G;
     const UnitPlace p = place_of(a, threadIdx.x & 63, false, [&](int) { return b; });
-    const int share = share_of(p.all, a.groups), at = p.before + (hk * a.tiles + tile) * p.units, w0 = at / share, w1 = (at + p.units - 1) / share;
+    const int share = share_of(p.all, a.groups), at = p.before + (hk * a.tiles + tile) * p.units, w0 = at / share, w1 = (at + p.units - kStart - 1) / share;
     if (w0 == w1) return;
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
@@ -442,7 +431,7 @@ static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t max
     const int64_t Mq = qL * (H / Hkv);
     p.rt = Mq > 16 ? 2 : 1;
     p.tiles = (int)((Mq + 16 * p.rt - 1) / (16 * p.rt));
-    const int64_t most = B * Hkv * p.tiles * ((maxlen + kUnit - 1) / kUnit), held = p.rt == 1 ? 768 : 512;  // (workgroups that the chip holds)
+    const int64_t most = B * Hkv * p.tiles * ((maxlen + kUnit - 1) / kUnit + kStart), held = p.rt == 1 ? 1024 : 512;  // (workgroups that the chip holds)
     p.groups = (int)(most < held ? most : held);
     return p;
 }
@@ -485,7 +474,7 @@ using namespace llmops;
 static bool q4_sizes_fit(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t maxlen) {
     const int64_t most = (int64_t)1 << 24;  // (a launch has fewer than 2^32 threads)
     return B > 0 && qL > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && maxlen > 0 && B < most && qL < most && H < most && maxlen <= most && B * qL < most &&
-           B * qL * H < most && (Wide)B * H * qL * ((maxlen + kUnit - 1) / kUnit) < ((Wide)1 << 31);
+           B * qL * H < most && (Wide)B * H * qL * ((maxlen + kUnit - 1) / kUnit + kStart) < ((Wide)1 << 31);
 }
 
 extern "C" size_t llmops_attention_q4_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t maxlen) {

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void q4_read_kernel(const uint8_t* __restrict_
     v8h x = {};
     if (row >= 0 && row < maxlen) {
         const uint32_t* src = reinterpret_cast<const uint32_t*>(cache + (head * maxlen + row) * kQ4Row);
-        x = values8(src[j], src[16 + (j >> 2)]);
+        x = Codes().values(src[j], src[16 + (j >> 2)]);
     }
     T* dst = out + at * kS + 8 * j;
     if constexpr (sizeof(T) == 4) {

@@ -124,14 +124,19 @@ __device__ __forceinline__ void store_q4(uint8_t* row, uint2 q, int j) {
 }
 
 // eight codes as halves: two and two, codes 0 1, 2 3, 4 5, 6 7 of a word.  (The bits of a code below those of 1024, or four places up below
-// those of 64, are a half that is 1024 or 64 more.)
-__device__ __forceinline__ v2h pair_low(uint32_t x) { return __builtin_bit_cast(v2h, (x & 0x000f000fu) | 0x64006400u) - (_Float16)1024.0f; }
-__device__ __forceinline__ v2h pair_high(uint32_t x) { return __builtin_bit_cast(v2h, (x & 0x00f000f0u) | 0x54005400u) - (_Float16)64.0f; }
-__device__ __forceinline__ v8h values8(uint32_t word, uint32_t dm) {
-    const v2h p = __builtin_bit_cast(v2h, dm), d = {p[0], p[0]}, m = {p[1], p[1]};
-    const v2h a = __builtin_elementwise_fma(pair_low(word), d, m), b = __builtin_elementwise_fma(pair_high(word), d, m),
-              c = __builtin_elementwise_fma(pair_low(word >> 8), d, m), e = __builtin_elementwise_fma(pair_high(word >> 8), d, m);
-    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
-}
+// those of 64, are a half that is 1024 or 64 more.)  The masks and what goes above them in registers of their own, one scalar: an instruction can
+// have one scalar operand and no constants beside it, and with constants the compiler takes two (v_and, v_or).
+struct Codes {
+    uint32_t low_mask = 0x000f000fu, high_mask = 0x00f000f0u, of_1024 = 0x64006400u, of_64 = 0x54005400u;
+    __device__ __forceinline__ Codes() { asm volatile("" : "+s"(low_mask), "+s"(high_mask), "+v"(of_1024), "+v"(of_64)); }
+    __device__ __forceinline__ v2h low(uint32_t x) const { return __builtin_bit_cast(v2h, (x & low_mask) | of_1024) - (_Float16)1024.0f; }
+    __device__ __forceinline__ v2h high(uint32_t x) const { return __builtin_bit_cast(v2h, (x & high_mask) | of_64) - (_Float16)64.0f; }
+    __device__ __forceinline__ v8h values(uint32_t word, uint32_t dm) const {
+        const v2h p = __builtin_bit_cast(v2h, dm), d = {p[0], p[0]}, m = {p[1], p[1]};
+        const v2h a = __builtin_elementwise_fma(low(word), d, m), b = __builtin_elementwise_fma(high(word), d, m), c = __builtin_elementwise_fma(low(word >> 8), d, m),
+                  e = __builtin_elementwise_fma(high(word >> 8), d, m);
+        return v8h{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
+    }
+};
 
 }  // namespace llmops

@@ -97,15 +97,17 @@ __device__ __forceinline__ float over_groups(float v) {
 // scores (before the factor, which is positive) to weights: the running maximum, the sum, and what the sums so far shrink by.
 // sc[tt]: rows t + 16*tt + 4*g + v.  FAR: also scores so far from 0 that their products with the factor may not be left unrounded beside the
 // rounded maximum (from 2^31 on the weight of the maximum itself would be infinite)
-template <bool FAR = false, int RT>
-__device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[2], int t, int g, bool masked) {
+template <bool FAR = false, int RT, int N>
+__device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[N], int t, int g, bool masked) {
     if (masked) {
 #pragma unroll
-        for (int tt = 0; tt < 2; tt++)
+        for (int tt = 0; tt < N; tt++)
 #pragma unroll
             for (int v = 0; v < 4; v++) sc[tt][v] = t + 16 * tt + 4 * g + v < s.see[rt] ? sc[tt][v] : -INFINITY;
     }
-    float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+#pragma unroll
+    for (int tt = 1; tt < N; tt++) top = fmaxf(top, fmaxf(fmaxf(sc[tt][0], sc[tt][1]), fmaxf(sc[tt][2], sc[tt][3])));
     top = over_groups(top) * s.c[rt];
     if (__any(top > s.m[rt])) {
         const float m = fmaxf(s.m[rt], top), shrink = s.m[rt] == m ? 1.0f : __builtin_amdgcn_exp2f(s.m[rt] - m);
@@ -116,7 +118,7 @@ __device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[2], int 
     }
     if (FAR && __any(fabsf(s.m[rt]) > 0x1p20f && s.m[rt] != -INFINITY)) {
 #pragma unroll
-        for (int tt = 0; tt < 2; tt++)
+        for (int tt = 0; tt < N; tt++)
 #pragma unroll
             for (int v = 0; v < 4; v++) {
                 const float x = sc[tt][v] * s.c[rt];
@@ -127,7 +129,7 @@ __device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[2], int 
     }
     const float base = s.m[rt] == -INFINITY ? 0.0f : kLift - s.m[rt];  // (nothing seen yet: every weight is exp2(-inf) = 0)
 #pragma unroll
-    for (int tt = 0; tt < 2; tt++)
+    for (int tt = 0; tt < N; tt++)
 #pragma unroll
         for (int v = 0; v < 4; v++) {
             sc[tt][v] = __builtin_amdgcn_exp2f(fmaf(sc[tt][v], s.c[rt], base));

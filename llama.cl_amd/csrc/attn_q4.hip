@@ -4,7 +4,7 @@
 //   out = sum_r e_r V_r / sum_r e_r,  e_r = exp(q' . K_r / sqrt(S) - max),  r = 0 .. pos,  K and V as the cache holds them
 //
 //   1. q4_prep_kernel   rotates, writes the new rows and leaves q' as operands of the matrix instructions
-//   2. q4_few_kernel    softmax(q'K^T)V, running maximum and sum, one pass: rows shared out among workgroups by the lengths
+//   2. q4_few_kernel or q4_many_kernel   softmax(q'K^T)V, running maximum and sum, one pass: rows shared out among workgroups by the lengths
 //   3. q4_join_kernel   joins what several workgroups have of a query
 //
 // Queries of a kv head are numbered m = (b*qL + l)*G + g.
@@ -29,7 +29,7 @@ struct Q4Args {
     float* out;                         // [B][qL][H*128]
     int64_t maxlen;
     int B, qL, G, Hkv, M, Mq;           // M = B*qL*G, Mq = qL*G
-    int tiles, groups;                  // tiles of a sequence's queries for a kv head; workgroups
+    int tile, tiles, groups, join;      // queries of a tile, tiles of a sequence's queries for a kv head; workgroups; queries that one joins
 };
 struct Q4Prep {
     const float *q, *k, *v, *inv_freq;
@@ -80,9 +80,10 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a, Q4Prep p) {
 //                 8 x 8 codes over in its registers.  Result of product c: query i, dim 8*(4*g + v) + c.
 __device__ __forceinline__ uint32_t ask4(buffer_rsrc r, uint32_t lane_at, uint32_t at) { return __builtin_amdgcn_raw_buffer_load_b32(r, lane_at + at, 0, 0); }
 
-// 32 rows from t on (the same t in the whole wave) as a descriptor that ends with the rows: those behind read as zero
+// N rows from t on (the same t in the whole wave) as a descriptor that ends with the rows: those behind read as zero
+template <int N = 32>
 __device__ __forceinline__ buffer_rsrc q4_rows(const uint8_t* p, int t, int end) {
-    return make_rsrc(p + (int64_t)t * kQ4Row, (uint32_t)__builtin_amdgcn_readfirstlane(max(0, min(32, end - t))) * (uint32_t)kQ4Row);
+    return make_rsrc(p + (int64_t)t * kQ4Row, (uint32_t)__builtin_amdgcn_readfirstlane(max(0, min(N, end - t))) * (uint32_t)kQ4Row);
 }
 struct Q4Regs {
     uint4 k[2];
@@ -144,14 +145,28 @@ struct Q4QueryOps {
     __device__ __forceinline__ v8h lo(int rt, int step) const { return as_v8h(mine[(rt * 8 + 4 + step) * 64]); }
 };
 
-// Units of 128 rows are numbered through: sequence after sequence, in each kv head after kv head, in each tile after tile.  A sequence without
-// rows (padding) has one unit for each all the same, in which its zeros are written.  Behind the units of a tile there are kStart more
-// without rows, for what it costs to begin with queries and to bring the waves' sums together, so that workgroups with short sequences have no more to do.
+// Units of 128 rows are numbered through: sequence after sequence, in each kv head after kv head, in each tile after tile.  Behind the units of a tile
+// there are kStart more without rows, for what it costs to begin with queries and to bring the waves' sums together, so that workgroups with short
+// sequences have no more to do.  A tile that is all padding has one unit, in which its zeros are written.
 constexpr int kStart = 1;
-__device__ __forceinline__ int units_of(const Q4Args& a, int b) {
+struct UnitsOf {
+    int tile, live, head;  // units of a tile that is not all padding, such tiles, units of a kv head
+};
+__device__ __forceinline__ UnitsOf units_of(const Q4Args& a, int b) {
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-    return (n > 0 ? (len + n + kUnit - 1) / kUnit : 1) + kStart;
+    UnitsOf u;
+    u.live = (n * a.G + a.tile - 1) / a.tile;
+    u.tile = n > 0 ? (len + n + kUnit - 1) / kUnit + kStart : 1;
+    u.head = u.live * u.tile + a.tiles - u.live;
+    return u;
+}
+// the tile of unit `in` of a kv head, its units, and how many are before this one
+__device__ __forceinline__ void tile_of(const UnitsOf& u, int in, int& tile, int& units, int& at) {
+    const bool live = in < u.live * u.tile;
+    tile = live ? in / u.tile : u.live + in - u.live * u.tile;
+    units = live ? u.tile : 1;
+    at = live ? in - tile * u.tile : 0;
 }
 __device__ __forceinline__ int wave_scan(int v, int lane) {
 #pragma unroll
@@ -161,37 +176,34 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
     }
     return v;
 }
-// Every wave for itself: all units, and the sequence that has unit `wanted(all)`, or that is `wanted(all)` where by_unit is false; its units for a
-// tile, and the units before it.
+// Every wave for itself: all units, and the sequence that has unit `wanted(all)`, or that is `wanted(all)` where by_unit is false; the units before it.
 struct UnitPlace {
-    int all, b, units, before;
+    int all, b, before;
 };
 template <typename F>
 __device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane, bool by_unit, F wanted) {
-    const int each = a.Hkv * a.tiles;
-    int all = 0, units = 0, upto = 0;
+    int all = 0, its = 0, upto = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        units = b0 + lane < a.B ? units_of(a, b0 + lane) : 0;
-        upto = all + wave_scan(units * each, lane);
+        its = b0 + lane < a.B ? units_of(a, b0 + lane).head * a.Hkv : 0;
+        upto = all + wave_scan(its, lane);
         all = __builtin_amdgcn_readlane(upto, 63);
     }
-    UnitPlace p{all, -1, 0, 0};
+    UnitPlace p{all, -1, 0};
     const int want = wanted(all);
     if (by_unit && want >= all) return p;
     int before = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         if (a.B > 64) {
-            units = b0 + lane < a.B ? units_of(a, b0 + lane) : 0;
-            upto = before + wave_scan(units * each, lane);
+            its = b0 + lane < a.B ? units_of(a, b0 + lane).head * a.Hkv : 0;
+            upto = before + wave_scan(its, lane);
         }
         const uint64_t hit = by_unit ? __ballot(upto > want) : want >= b0 && want < b0 + 64 ? 1ull << (want - b0) : 0;
         if (hit != 0) {
             const int at = __builtin_ctzll(hit);
             p.b = b0 + at;
-            p.units = __builtin_amdgcn_readlane(units, at);
-            p.before = __builtin_amdgcn_readlane(upto, at) - p.units * each;
+            p.before = __builtin_amdgcn_readlane(upto - its, at);
             break;
         }
         before = __builtin_amdgcn_readlane(upto, 63);
@@ -226,17 +238,21 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
     int share = 0;
     const UnitPlace start = place_of(a, lane, true, [&](int all) { share = share_of(all, a.groups); return (int)min((int64_t)blockIdx.x * share, (int64_t)INT_MAX); });
     if (start.b < 0) return;
-    const int first = (int)blockIdx.x * share, last = min(start.all, first + share), each = a.Hkv * a.tiles;
-    int b = start.b, units = start.units, before = start.before;
+    const int first = (int)blockIdx.x * share, last = min(start.all, first + share);
+    int b = start.b, before = start.before;
+    UnitsOf its = units_of(a, b);
 #pragma unroll 1
     for (int at = first; at < last;) {
-        if (at >= before + units * each) {  // (the next sequence)
-            before += units * each;
-            units = units_of(a, ++b);
+        if (at >= before + its.head * a.Hkv) {  // (the next sequence)
+            before += its.head * a.Hkv;
+            its = units_of(a, ++b);
         }
-        const int item = (at - before) / units, u0 = at - before - item * units, u1 = min(units, u0 + last - at), hk = item / a.tiles, tile = item - hk * a.tiles;
+        const int hk = (at - before) / its.head;
+        int tile, units, u0;
+        tile_of(its, at - before - hk * its.head, tile, units, u0);
+        const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
         at += u1 - u0;
-        if (u0 >= units - kStart) continue;
+        if (u0 >= real) continue;
         int len, n;
         own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
         const int m0 = b * a.Mq + tile * 16 * RT, m_end = min((b + 1) * a.Mq, m0 + 16 * RT);
@@ -317,7 +333,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
             if (g == 0) sm.m[wave][16 * rt + i] = s.m[rt], sm.l[wave][16 * rt + i] = s.l[rt];
         }
         __syncthreads();
-        const bool whole = u0 == 0 && u1 >= units - kStart;
+        const bool whole = u0 == 0 && u1 >= real;
         const int64_t record = ((int64_t)blockIdx.x * 2 + (u0 == 0)) * (16 * RT);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
@@ -361,78 +377,283 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
     }
 }
 
-// ---- 3. what several workgroups have of a query ----
-// a workgroup to a query, half a wave to every eighth record, 16 bytes to a lane
+// Many queries (64 * RT to a workgroup, 16 * RT to a wave).  All waves multiply the same 64 rows, whose values the workgroup forms once and leaves in LDS in the
+// order of the operands (a read is 16 bytes to a lane, in lane order); two buffers: while a tile is multiplied the next one's values are formed and the one
+// behind it is on its way from memory.
+struct Q4TileSmem {
+    uint4 k[2][16][64], v[2][16][64];
+    uint32_t bad[2][4];  // of 16 rows each: V rows that hold NaN, among those that are new
+};
+struct Q4TileRegs {
+    uint4 k;
+    uint32_t kdm, v[4], vdm[4];
+    // rows 16*wave .. of 64 to a wave.  K: row i, group g.  V: word i of rows 4*g + 0..3
+    __device__ __forceinline__ void load(buffer_rsrc K, buffer_rsrc V, int wave, int i, int g) {
+        const uint32_t k_at = (uint32_t)((16 * wave + i) * kQ4Row), v_at = (uint32_t)((16 * wave + 4 * g) * kQ4Row);
+        k = ask16(K, k_at + 16 * g, 0);
+        kdm = ask4(K, k_at + 64 + 4 * g, 0);
+        const uint32_t codes = unseen(v_at + 4 * i), pairs = unseen(v_at + 64 + (i & 12));
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = ask4(V, codes, r * kQ4Row), vdm[r] = ask4(V, pairs, r * kQ4Row);
+    }
+    __device__ __forceinline__ void write(const Codes& codes, Q4TileSmem& sm, int buf, int wave, int lane, bool fresh) {
+        sm.k[buf][4 * wave][lane] = __builtin_bit_cast(uint4, codes.values(k.x, kdm));
+        sm.k[buf][4 * wave + 1][lane] = __builtin_bit_cast(uint4, codes.values(k.y, kdm));
+        sm.k[buf][4 * wave + 2][lane] = __builtin_bit_cast(uint4, codes.values(k.z, kdm));
+        sm.k[buf][4 * wave + 3][lane] = __builtin_bit_cast(uint4, codes.values(k.w, kdm));
+        if (fresh) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const bool nan = (vdm[r] & 0x7fff0000u) > 0x7c000000u;
+                const uint64_t rows = __ballot(nan);
+                if (nan) vdm[r] = 0;
+#pragma unroll
+                for (int g = 0; g < 4; g++) bad |= (uint32_t)(rows >> (16 * g) & 1) << (4 * g + r);
+            }
+            if (lane == 0) sm.bad[buf][wave] = bad;
+        }
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+            const uint32_t pick = 0x0c000c00u | (uint32_t)(4 + y) << 16 | (uint32_t)y;
+            uint2 low, high;
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const uint32_t x = __builtin_amdgcn_perm(v[2 * p + 1], v[2 * p], pick);
+                const v2h d = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(vdm[2 * p + 1], vdm[2 * p], 0x05040100u)),
+                          m = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(vdm[2 * p + 1], vdm[2 * p], 0x07060302u));
+                (p ? low.y : low.x) = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(codes.low(x), d, m));
+                (p ? high.y : high.x) = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(codes.high(x), d, m));
+            }
+            // (rows 0 .. 31 are the first eight operands' first and second halves, rows 32 .. 63 the others')
+            const int c = 8 * (wave >> 1) + first_code(y);
+            reinterpret_cast<uint2*>(&sm.v[buf][c][lane])[wave & 1] = low;
+            reinterpret_cast<uint2*>(&sm.v[buf][c + 2][lane])[wave & 1] = high;
+        }
+    }
+};
+
 template <int RT>
+__global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
+    __shared__ Q4TileSmem sm;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    const Codes codes;
+    int share = 0;
+    const UnitPlace start = place_of(a, lane, true, [&](int all) { share = share_of(all, a.groups); return (int)min((int64_t)blockIdx.x * share, (int64_t)INT_MAX); });
+    if (start.b < 0) return;
+    const int first = (int)blockIdx.x * share, last = min(start.all, first + share);
+    int b = start.b, before = start.before;
+    UnitsOf its = units_of(a, b);
+#pragma unroll 1
+    for (int at = first; at < last;) {
+        if (at >= before + its.head * a.Hkv) {  // (the next sequence)
+            before += its.head * a.Hkv;
+            its = units_of(a, ++b);
+        }
+        const int hk = (at - before) / its.head;
+        int tile, units, u0;
+        tile_of(its, at - before - hk * its.head, tile, units, u0);
+        const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
+        at += u1 - u0;
+        if (u0 >= real) continue;
+        int len, n;
+        own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+        const int m0 = b * a.Mq + tile * 64 * RT, m_end = min((b + 1) * a.Mq, m0 + 64 * RT);
+        const int seen_by_last = min(n, (m_end - 1 - b * a.Mq) / a.G + 1), rows = tile * 64 * RT < n * a.G ? len + seen_by_last : 0;
+        const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kQ4Row;
+        const uint8_t *K = a.k + plane, *V = a.v + plane;
+        const int j0 = 2 * u0, j1 = min(2 * u1, (rows + 63) / 64);
+        Q4TileRegs x;
+        auto load = [&](int j) { x.load(q4_rows<64>(K, 64 * j, rows), q4_rows<64>(V, 64 * j, rows), wave, i, g); };
+        if (j0 < j1) load(j0);
+        v8h qh[RT][4], ql[RT][4];
+        Queries<RT> s;
+        const int mw = m0 + 16 * RT * wave;
+        bool live[RT];
+        int see_min = INT_MAX;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const int m = min(mw + 16 * rt + i, m_end - 1), l = (m - b * a.Mq) / a.G;
+            const int64_t from = ((int64_t)hk * a.M + m) * kS + 32 * g;
+#pragma unroll
+            for (int step = 0; step < 4; step++) {
+                qh[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + from + 8 * step));
+                ql[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + from + 8 * step));
+            }
+            s.c[rt] = a.cq[(int64_t)hk * a.M + m];
+            s.m[rt] = -INFINITY, s.l[rt] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 8; c++) s.o[rt][c] = v4f{0.f, 0.f, 0.f, 0.f};
+            live[rt] = l < n;
+            s.see[rt] = live[rt] ? len + l + 1 : INT_MAX;  // (what padding sees is thrown away)
+            see_min = min(see_min, s.see[rt]);
+        }
+        if (j0 < j1) {
+            x.write(codes, sm, 0, wave, lane, 64 * j0 + 64 > len);
+            load(min(j0 + 1, j1 - 1));
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int j = j0; j < j1; j++) {
+            const int buf = (j - j0) & 1, t = 64 * j;
+            x.write(codes, sm, buf ^ 1, wave, lane, t + 128 > len);  // (behind the last tile that one again: nobody reads it)
+            load(min(j + 2, j1 - 1));
+            __builtin_amdgcn_sched_barrier(0);  // (asked for now: behind the scores' products they come late)
+            const bool masked = __any(t + 64 > see_min);
+            v4f sc[RT][4];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = sc[rt][2] = sc[rt][3] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int step = 0; step < 4; step++) {
+                v8h k[4];
+#pragma unroll
+                for (int tt = 0; tt < 4; tt++) k[tt] = as_v8h(sm.k[buf][4 * tt + step][lane]);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++) sc[rt][tt] = mfma(k[tt], qh[rt][step], sc[rt][tt]);
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++) sc[rt][tt] = mfma(k[tt], ql[rt][step], sc[rt][tt]);
+                }
+            }
+            Weights w[RT][2];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                if (t + 64 > len) {
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++) {
+                        const uint32_t bad = __builtin_amdgcn_readfirstlane(sm.bad[buf][tt]);
+                        if (bad != 0)
+#pragma unroll
+                            for (int v = 0; v < 4; v++)
+                                if (bad >> (4 * g + v) & 1) sc[rt][tt][v] = NAN;
+                    }
+                }
+                weigh<true>(s, rt, sc[rt], t, g, masked);
+                w[rt][0] = weights_of<__half>({sc[rt][0], sc[rt][1]});
+                w[rt][1] = weights_of<__half>({sc[rt][2], sc[rt][3]});
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < 16; c0 += 4) {
+                v8h h[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) h[c] = as_v8h(sm.v[buf][c0 + c][lane]);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    const Weights& x2 = w[rt][c0 >> 3];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s.o[rt][(c0 & 7) + c] = mfma(h[c], x2.hi, s.o[rt][(c0 & 7) + c]);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s.o[rt][(c0 & 7) + c] = mfma(h[c], x2.lo, s.o[rt][(c0 & 7) + c]);
+                }
+            }
+            __syncthreads();
+        }
+        const bool whole = u0 == 0 && u1 >= real;
+        const int64_t record = ((int64_t)blockIdx.x * 2 + (u0 == 0)) * (64 * RT);
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            s.l[rt] += __shfl_xor(s.l[rt], 16, 64);
+            s.l[rt] += __shfl_xor(s.l[rt], 32, 64);
+            const int in = 16 * RT * wave + 16 * rt + i, m = m0 + in;
+            if (m >= m_end) continue;
+            if (!whole && g == 0) a.rec_stat[record + in] = make_float2(s.m[rt], s.l[rt]);
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float4 o = make_float4(s.o[rt][4 * h][v], s.o[rt][4 * h + 1][v], s.o[rt][4 * h + 2][v], s.o[rt][4 * h + 3][v]);
+                    const int d = 8 * (4 * g + v) + 4 * h;
+                    if (whole) q4_leave(a, hk, m, d, o, s.l[rt], live[rt]);
+                    else *reinterpret_cast<float4*>(a.rec_out + (record + in) * kS + d) = o;
+                }
+        }
+    }
+}
+
+// ---- 3. what several workgroups have of a query ----
+// A workgroup to a.join (1, 2, 4, 8) queries of a tile, 8 / a.join half waves to a query, each to as many records from the other, 16 bytes to a lane
 __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
     __shared__ float stat[8][2];
     __shared__ float4 part[8][32];
-    const int64_t r = blockIdx.x;
-    const int hk = (int)(r / a.M), m = (int)(r - (int64_t)hk * a.M), b = m / a.Mq, in = m - b * a.Mq, tile = in / (16 * RT), l = in / a.G;
+    const int parts = (min(a.tile, a.Mq) + a.join - 1) / a.join, item = blockIdx.x / parts, in0 = a.join * (blockIdx.x - item * parts);
+    const int each = a.Hkv * a.tiles, b = item / each, hk = (item - b * each) / a.tiles, tile = item % a.tiles;
     const UnitPlace p = place_of(a, threadIdx.x & 63, false, [&](int) { return b; });
-    const int share = share_of(p.all, a.groups), at = p.before + (hk * a.tiles + tile) * p.units, w0 = at / share, w1 = (at + p.units - kStart - 1) / share;
-    if (w0 == w1) return;
+    const UnitsOf its = units_of(a, b);
+    if (tile >= its.live) return;  // (zeros, which one workgroup has written)
+    const int share = share_of(p.all, a.groups), at = p.before + hk * its.head + tile * its.tile, w0 = at / share, w1 = (at + its.tile - kStart - 1) / share;
+    const int queries = min(a.join, min(a.tile, a.Mq - tile * a.tile) - in0);
+    if (w0 == w1 || queries <= 0) return;
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-    const int half = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31), query = in - tile * 16 * RT;
+    const int halves = 8 / a.join;
+    const int half = threadIdx.x >> 5, turn = half & (halves - 1), query = in0 + half / halves, d = 4 * (threadIdx.x & 31);
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (query < in0 + queries) {
 #pragma unroll 1
-    for (int w = w0 + half; w <= w1; w += 32) {
-        float2 st[4];
-        float4 x[4];
+        for (int w = w0 + turn; w <= w1; w += 4 * halves) {
+            float2 st[4];
+            float4 x[4];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int64_t wg = min(w + 8 * u, w1), record = (wg * 2 + (wg * share <= at)) * (16 * RT) + query;
-            st[u] = a.rec_stat[record];
-            x[u] = *reinterpret_cast<const float4*>(a.rec_out + record * kS + d);
-        }
-        float up = M;
+            for (int u = 0; u < 4; u++) {
+                const int64_t wg = min(w + halves * u, w1), record = (wg * 2 + (wg * share <= at)) * a.tile + query;
+                st[u] = a.rec_stat[record];
+                x[u] = *reinterpret_cast<const float4*>(a.rec_out + record * kS + d);
+            }
+            float up = M;
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            if (w + 8 * u > w1) st[u] = make_float2(-INFINITY, 0.0f);
-            up = fmaxf(up, st[u].x);
-        }
-        const float shrink = M == up ? 1.0f : __builtin_amdgcn_exp2f(M - up);
-        M = up;
-        L *= shrink, o.x *= shrink, o.y *= shrink, o.z *= shrink, o.w *= shrink;
+            for (int u = 0; u < 4; u++) {
+                if (w + halves * u > w1) st[u] = make_float2(-INFINITY, 0.0f);
+                up = fmaxf(up, st[u].x);
+            }
+            const float shrink = M == up ? 1.0f : __builtin_amdgcn_exp2f(M - up);
+            M = up;
+            L *= shrink, o.x *= shrink, o.y *= shrink, o.z *= shrink, o.w *= shrink;
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const bool none = st[u].y == 0.0f;
-            const float f = none ? 0.0f : st[u].x == M ? 1.0f : __builtin_amdgcn_exp2f(st[u].x - M);
-            if (none) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            L = fmaf(f, st[u].y, L);
-            o.x = fmaf(f, x[u].x, o.x), o.y = fmaf(f, x[u].y, o.y), o.z = fmaf(f, x[u].z, o.z), o.w = fmaf(f, x[u].w, o.w);
+            for (int u = 0; u < 4; u++) {
+                const bool none = st[u].y == 0.0f;
+                const float f = none ? 0.0f : st[u].x == M ? 1.0f : __builtin_amdgcn_exp2f(st[u].x - M);
+                if (none) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                L = fmaf(f, st[u].y, L);
+                o.x = fmaf(f, x[u].x, o.x), o.y = fmaf(f, x[u].y, o.y), o.z = fmaf(f, x[u].z, o.z), o.w = fmaf(f, x[u].w, o.w);
+            }
         }
     }
-    if (d == 0) stat[half][0] = M, stat[half][1] = L;
-    part[half][threadIdx.x & 31] = o;
-    __syncthreads();
-    if (threadIdx.x >= 32) return;
-    M = stat[0][0];
-#pragma unroll
-    for (int h = 1; h < 8; h++) M = fmaxf(M, stat[h][0]);
-    L = 0.0f, o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int h = 0; h < 8; h++) {
-        const float f = stat[h][1] == 0.0f ? 0.0f : stat[h][0] == M ? 1.0f : __builtin_amdgcn_exp2f(stat[h][0] - M);
-        const float4 x = part[h][threadIdx.x];
-        L = fmaf(f, stat[h][1], L);
-        o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+    if (halves > 1) {
+        if (d == 0) stat[half][0] = M, stat[half][1] = L;
+        part[half][threadIdx.x & 31] = o;
+        __syncthreads();
+        if (turn != 0 || query >= in0 + queries) return;
+        M = stat[half][0];
+        for (int h = 1; h < halves; h++) M = fmaxf(M, stat[half + h][0]);
+        L = 0.0f, o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int h = 0; h < halves; h++) {
+            const float sum = stat[half + h][1], f = sum == 0.0f ? 0.0f : stat[half + h][0] == M ? 1.0f : __builtin_amdgcn_exp2f(stat[half + h][0] - M);
+            const float4 x = part[half + h][threadIdx.x & 31];
+            L = fmaf(f, sum, L);
+            o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+        }
     }
-    q4_leave(a, hk, m, d, o, L, l < n);
+    const int in = tile * a.tile + query;
+    if (query < in0 + queries) q4_leave(a, hk, b * a.Mq + in, d, o, L, in / a.G < n);
 }
 
 struct Q4Plan {
-    int rt, tiles, groups;
+    bool many;
+    int rt, tile, tiles, groups, join;
 };
 static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t maxlen) {
     Q4Plan p{};
     const int64_t Mq = qL * (H / Hkv);
-    p.rt = Mq > 16 ? 2 : 1;
-    p.tiles = (int)((Mq + 16 * p.rt - 1) / (16 * p.rt));
-    const int64_t most = B * Hkv * p.tiles * ((maxlen + kUnit - 1) / kUnit + kStart), held = p.rt == 1 ? 1024 : 512;  // (workgroups that the chip holds)
+    p.many = Mq > 32;
+    p.rt = !p.many && Mq > 16 ? 2 : 1;
+    p.tile = (p.many ? 64 : 16) * p.rt;
+    p.tiles = (int)((Mq + p.tile - 1) / p.tile);
+    const int64_t most = B * Hkv * p.tiles * ((maxlen + kUnit - 1) / kUnit + kStart), held = p.many || p.rt == 2 ? 512 : 1024;  // (workgroups that the chip holds)
     p.groups = (int)(most < held ? most : held);
+    const int64_t queries = B * Hkv * Mq;  // (workgroups enough to fill the chip, then queries to each)
+    p.join = queries >= 8192 ? 8 : queries >= 4096 ? 4 : queries >= 2048 ? 2 : 1;
     return p;
 }
 struct Q4Layout {
@@ -446,7 +667,7 @@ static Q4Layout layout_q4(const Q4Plan& plan, int64_t rows) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    const size_t records = (size_t)plan.groups * 2 * 16 * plan.rt;
+    const size_t records = (size_t)plan.groups * 2 * plan.tile;
     w.qh = take((size_t)rows * kS * 2);
     w.ql = take((size_t)rows * kS * 2);
     w.cq = take((size_t)rows * 4);
@@ -456,13 +677,16 @@ static Q4Layout layout_q4(const Q4Plan& plan, int64_t rows) {
     return w;
 }
 
-template <int RT>
 static int q4_launch(const Q4Args& a, const Q4Prep& p, const Q4Plan& plan, hipStream_t st) {
     q4_prep_kernel<<<(unsigned)((int64_t)a.B * a.qL * p.rows16), 256, 0, st>>>(a, p);
     LLMOPS_LAUNCH_CHECK();
-    q4_few_kernel<RT><<<(unsigned)plan.groups, 256, 0, st>>>(a);
+    const unsigned groups = (unsigned)plan.groups;
+    if (plan.many) q4_many_kernel<1><<<groups, 256, 0, st>>>(a);
+    else if (plan.rt == 2) q4_few_kernel<2><<<groups, 256, 0, st>>>(a);
+    else q4_few_kernel<1><<<groups, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
-    q4_join_kernel<RT><<<(unsigned)((int64_t)a.Hkv * a.M), 256, 0, st>>>(a);
+    const int64_t parts = ((plan.tile < a.Mq ? plan.tile : a.Mq) + plan.join - 1) / plan.join;
+    q4_join_kernel<<<(unsigned)((int64_t)a.B * a.Hkv * plan.tiles * parts), 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }
@@ -509,7 +733,7 @@ extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int6
     a.k = reinterpret_cast<uint8_t*>(kv_cache) + 2 * layer_id * (int64_t)plane, a.v = a.k + (int64_t)plane;
     a.lengths = lengths, a.q_lens = q_lens, a.out = out, a.maxlen = maxlen;
     a.B = (int)B, a.qL = (int)qL, a.G = (int)G, a.Hkv = (int)Hkv, a.Mq = (int)(qL * G), a.M = (int)(B * qL * G);
-    a.tiles = plan.tiles, a.groups = plan.groups;
+    a.tile = plan.tile, a.tiles = plan.tiles, a.groups = plan.groups, a.join = plan.join;
     // (a workgroup reads its q, k and v while others may have written their rows and results)
     const Extent q_at(q, B, (Wide)q_stride_b * 4, qL, (Wide)q_stride_l * 4, heads), k_at(k, B, (Wide)k_stride_b * 4, qL, (Wide)k_stride_l * 4, kv_heads),
         v_at(v, B, (Wide)v_stride_b * 4, qL, (Wide)v_stride_l * 4, kv_heads), out_at(out, (Wide)B * qL * heads), written(a.k, 2 * plane);
@@ -517,5 +741,5 @@ extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int6
     LLMOPS_REQUIRE(apart(out_at, q_at) && apart(out_at, k_at) && apart(out_at, v_at) && apart(out_at, written));
     const Q4Prep p{q, k, v, inv_freq, q_stride_b, q_stride_l, k_stride_b, k_stride_l, v_stride_b, v_stride_l, (int)half, (int)rows16};
     hipStream_t st = as_stream(stream);
-    return plan.rt == 1 ? q4_launch<1>(a, p, plan, st) : q4_launch<2>(a, p, plan, st);
+    return q4_launch(a, p, plan, st);
 }

@@ -37,7 +37,22 @@ __device__ __forceinline__ void turn_of(float f, int pos, float& c, float& s) {
     s = fmaf(lo, c0, s0);
 }
 
-// a rotated query as halves, dims in x's order, and its factor
+// 8 * N values of a rotated query as halves, in their order, and its factor.  top: the largest magnitude of all of the query's; bad: it holds an infinity or NaN
+template <int N>
+__device__ __forceinline__ float halves_of(const float (&x)[8 * N], float top, bool bad, bool live, v8h (&hi)[N], v8h (&lo)[N]) {
+    const bool use = live && !bad && top > 0.0f;
+    // (2^123 at most: the factor stays a normal number.  It would lose its bits below 2^-126, and at 0 make NaN of a masked score's -inf)
+    const int e2 = use ? min(123, 13 - ilogbf(top)) : 0;
+#pragma unroll
+    for (int e = 0; e < 8 * N; e++) {
+        const float y = use ? ldexpf(x[e], e2) : 0.0f;
+        const _Float16 h = (_Float16)y;
+        hi[e >> 3][e & 7] = h;
+        lo[e >> 3][e & 7] = (_Float16)(y - (float)h);
+    }
+    // (a query that holds an infinity or NaN has no score that is a number)
+    return live && bad ? NAN : ldexpf(1.44269504f * 0.08838834764831845f, -e2);
+}
 struct QueryRow {
     uint4 hi, lo;
     float c;
@@ -50,18 +65,9 @@ __device__ __forceinline__ QueryRow query_row(const float (&x)[8], bool live) {
     float bad = fine ? 0.0f : 1.0f;
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64)), bad = fmaxf(bad, __shfl_xor(bad, o, 64));
-    const bool use = live && bad == 0.0f && top > 0.0f;
-    // (2^123 at most: the factor stays a normal number.  It would lose its bits below 2^-126, and at 0 make NaN of a masked score's -inf)
-    const int e2 = use ? min(123, 13 - ilogbf(top)) : 0;
-    v8h hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float y = use ? ldexpf(x[e], e2) : 0.0f;
-        hi[e] = (_Float16)y;
-        lo[e] = (_Float16)(y - (float)hi[e]);
-    }
-    // (a query that holds an infinity or NaN has no score that is a number)
-    return {__builtin_bit_cast(uint4, hi), __builtin_bit_cast(uint4, lo), live && bad != 0.0f ? NAN : ldexpf(1.44269504f * 0.08838834764831845f, -e2)};
+    v8h h[1], l[1];
+    const float c = halves_of(x, top, bad != 0.0f, live, h, l);
+    return {__builtin_bit_cast(uint4, h[0]), __builtin_bit_cast(uint4, l[0]), c};
 }
 
 __device__ __forceinline__ v8h as_v8h(uint4 u) { return *reinterpret_cast<const v8h*>(&u); }

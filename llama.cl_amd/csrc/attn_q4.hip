@@ -3,11 +3,11 @@
 //   pos = len[b] + l,  q' = rot(q, pos),  row pos of the cache = the codes of (rot(k, pos), v),
 //   out = sum_r e_r V_r / sum_r e_r,  e_r = exp(q' . K_r / sqrt(S) - max),  r = 0 .. pos,  K and V as the cache holds them
 //
-//   1. q4_prep_kernel   rotates, writes the new rows and leaves q' as operands of the matrix instructions
+//   1. q4_prep_kernel   rotates, writes the new rows and leaves q' as operands of the matrix instructions (part of 2 where caches are short)
 //   2. q4_few_kernel or q4_many_kernel   softmax(q'K^T)V, running maximum and sum, one pass: rows shared out among workgroups by the lengths
-//   3. q4_join_kernel   joins what several workgroups have of a query
+//   3. q4_join_kernel   joins what several workgroups have of a query, unless each has all rows of its queries
 //
-// Queries of a kv head are numbered m = (b*qL + l)*G + g.
+// A sequence's queries of a kv head are numbered l*G + g.
 //
 // Arithmetic.  The cache's values are halves, so that they are operands of v_mfma_f32_16x16x32_f16 (fp32 sums) without any loss; q' and the weights
 // are two halves each: q' scaled by a power of two of its row so that its largest value is in [2^13, 2^14), 22 bits of that, the weights times
@@ -20,54 +20,69 @@ namespace llmops {
 constexpr int kUnit = 128;  // rows that a workgroup's four waves read at a time
 
 struct Q4Args {
-    _Float16 *qh, *ql;                  // [Hkv][M][128]
+    const float *q, *k, *v, *inv_freq;
+    int64_t qsb, qsl, ksb, ksl, vsb, vsl;
+    _Float16 *qh, *ql;                  // [Hkv][M][128]: rotated queries (M = B*Mq)
     float* cq;                          // [Hkv][M]: score = cq * (q' . k), in units of log2
-    uint8_t *k, *v;                     // the layer's planes [B][Hkv][maxlen][80]
+    uint8_t *ck, *cv;                   // the layer's planes [B][Hkv][maxlen][80]
     const int32_t *lengths, *q_lens;    // [B]; q_lens may be null
     float* rec_out;                     // [groups][2][queries of a tile][128]
     float2* rec_stat;                   // [groups][2][queries of a tile]: max (log2), sum
     float* out;                         // [B][qL][H*128]
     int64_t maxlen;
-    int B, qL, G, Hkv, M, Mq;           // M = B*qL*G, Mq = qL*G
+    int B, qL, G, Hkv, M, Mq, half;     // Mq = qL*G
     int tile, tiles, groups, join;      // queries of a tile, tiles of a sequence's queries for a kv head; workgroups; queries that one joins
+    int rows16;
 };
-struct Q4Prep {
-    const float *q, *k, *v, *inv_freq;
-    int64_t qsb, qsl, ksb, ksl, vsb, vsl;
-    int half, rows16;
-};
+// query `in` of a sequence for kv head hk: token in / G, head hk*G + in % G
+__device__ __forceinline__ const float* query_at(const Q4Args& a, int b, int hk, int in) {
+    const int l = in / a.G;
+    return a.q + b * a.qsb + l * a.qsl + (int64_t)(hk * a.G + in - l * a.G) * kS;
+}
 
 // ---- 1. ----
+// Sixteen lanes to a row of k or v, dims 8 * (lane % 16) .. to a lane: k turned and its codes chosen in 64 bits, v in fp32; the row written
+__device__ __forceinline__ void write_row(const Q4Args& a, const float* src, bool is_k, int b, int hk, int64_t row, int j, const double2* turn) {
+    uint8_t* dst = (is_k ? a.ck : a.cv) + (((int64_t)b * a.Hkv + hk) * a.maxlen + row) * kQ4Row;
+    float x[8];
+    load8(src + 8 * j, x);
+    if (is_k) {
+        double y[8];
+        turn_row64(src, x, j, turn, a.half, y);
+        store_q4(dst, quantise8(y), j);
+    } else {
+        store_q4(dst, quantise8(x), j);
+    }
+}
+// .. of a query: turned in fp32
+__device__ __forceinline__ QueryRow turned_query(const float* src, int j, const double2* turn, int half, bool live) {
+    float x[8];
+    load8(src + 8 * j, x);
+    if (live) turn_row32(src, j, turn, half, x);
+    return query_row(x, live);
+}
+
 // A workgroup per token and 16 of its H + 2*Hkv rows of 128, sixteen lanes to a row
-__global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a, Q4Prep p) {
+__global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a) {
     __shared__ double2 turn[64];
-    const int bl = blockIdx.x / p.rows16, group = blockIdx.x - bl * p.rows16, b = bl / a.qL, l = bl - b * a.qL;
+    const int bl = blockIdx.x / a.rows16, group = blockIdx.x - bl * a.rows16, b = bl / a.qL, l = bl - b * a.qL;
     const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), j = threadIdx.x & 15;
-    const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv, none = row >= H + 2 * a.Hkv;
-    const int hk = is_k ? row - H : row - H - a.Hkv;
-    const float* src = is_q ? p.q + b * p.qsb + l * p.qsl + (int64_t)row * kS : is_k ? p.k + b * p.ksb + l * p.ksl + (int64_t)hk * kS : p.v + b * p.vsb + l * p.vsl + (int64_t)hk * kS;
-    // (the row is on its way while the length is fetched and the angles are formed, also where the token turns out to be padding)
-    double x[8] = {};
-    if (!none) load8(src + 8 * j, x);
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
     const bool live = l < n;
-    if (live && (int)threadIdx.x < p.half) turn[threadIdx.x] = turn64(p.inv_freq[threadIdx.x], len + l);
+    if (live && (int)threadIdx.x < a.half) turn[threadIdx.x] = turn64(a.inv_freq[threadIdx.x], len + l);
     __syncthreads();
-    if (none || (!live && !is_q)) return;
-    if (live && (is_q || is_k)) turn_row64(src, j, turn, p.half, x);
-    if (!is_q) {
-        store_q4((is_k ? a.k : a.v) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kQ4Row, quantise8(x), j);
-        return;
+    if (row < H) {
+        const int64_t m = (int64_t)(row / a.G) * a.M + (int64_t)bl * a.G + row % a.G;
+        const QueryRow r = turned_query(a.q + b * a.qsb + l * a.qsl + (int64_t)row * kS, j, turn, a.half, live);
+        *reinterpret_cast<uint4*>(a.qh + m * kS + 8 * j) = r.hi;
+        *reinterpret_cast<uint4*>(a.ql + m * kS + 8 * j) = r.lo;
+        if (j == 0) a.cq[m] = r.c;
+    } else if (live && row < H + 2 * a.Hkv) {
+        const bool is_k = row < H + a.Hkv;
+        const int hk = is_k ? row - H : row - H - a.Hkv;
+        write_row(a, is_k ? a.k + b * a.ksb + l * a.ksl + (int64_t)hk * kS : a.v + b * a.vsb + l * a.vsl + (int64_t)hk * kS, is_k, b, hk, len + l, j, turn);
     }
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = (float)x[e];
-    const int64_t m = (int64_t)(row / a.G) * a.M + (int64_t)bl * a.G + row % a.G;
-    const QueryRow r = query_row(y, live);
-    *reinterpret_cast<uint4*>(a.qh + m * kS + 8 * j) = r.hi;
-    *reinterpret_cast<uint4*>(a.ql + m * kS + 8 * j) = r.lo;
-    if (j == 0) a.cq[m] = r.c;
 }
 
 // ---- 2. rows for a tile of queries ----
@@ -126,24 +141,51 @@ struct Q4Regs {
 };
 __device__ __forceinline__ constexpr int first_code(int y) { return y == 0 ? 0 : y == 1 ? 4 : y == 2 ? 1 : 5; }  // of byte y; the other is 2 more
 
-// the queries' operands, in LDS: the four waves share them, and leave registers for a fourth wave on a SIMD
+// A tile's rotated queries as operands in LDS (the four waves share them, and leave registers for a fourth wave on a SIMD), with their factors
 template <int RT>
-struct Q4QueryOps {
-    const uint4* mine;
-    __device__ __forceinline__ void load(const Q4Args& a, uint4* lds, int hk, int m0, int m_end, int lane) {
-        const int wave = threadIdx.x >> 6;  // a step to a wave
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            const int64_t at = ((int64_t)hk * a.M + min(m0 + 16 * rt + (lane & 15), m_end - 1)) * kS + 32 * (lane >> 4) + 8 * wave;
-            lds[(rt * 8 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.qh + at);
-            lds[(rt * 8 + 4 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.ql + at);
-        }
-        mine = lds + lane;
-        __syncthreads();
-    }
-    __device__ __forceinline__ v8h hi(int rt, int step) const { return as_v8h(mine[(rt * 8 + step) * 64]); }
-    __device__ __forceinline__ v8h lo(int rt, int step) const { return as_v8h(mine[(rt * 8 + 4 + step) * 64]); }
+struct Q4FewIn {
+    uint4 q[RT * 8 * 64];
+    double2 turn[16 * RT][64];  // of the sequence's tokens
 };
+template <int RT>
+__device__ __forceinline__ void q4_take(const Q4Args& a, Q4FewIn<RT>& sm, float* factors, int b, int hk, int lane) {
+    const int wave = threadIdx.x >> 6;  // a step to a wave
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int64_t m = (int64_t)hk * a.M + (int64_t)b * a.Mq + min(16 * rt + (lane & 15), a.Mq - 1), at = m * kS + 32 * (lane >> 4) + 8 * wave;
+        sm.q[(rt * 8 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.qh + at);
+        sm.q[(rt * 8 + 4 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.ql + at);
+        if (wave == 0 && lane < 16) factors[16 * rt + lane] = a.cq[m];
+    }
+    __syncthreads();
+}
+// The same from q itself, and the sequence's new rows of k and v written (a launch less).  All of it by the workgroup, sixteen lanes to a row, 16 rows at a time.
+// Loads that wait for each other: where many workgroups keep the memory busy the launch is the better way (32 sequences of up to 4096 rows 88 us with
+// it, 109 without; two of up to 200 14.9 and 10.7).
+template <int RT>
+__device__ __forceinline__ void q4_begin(const Q4Args& a, Q4FewIn<RT>& sm, float* factors, int b, int hk, int len, int n) {
+    const int thread = (int)unseen(threadIdx.x), i = thread >> 4, j = thread & 15;
+#pragma unroll 1
+    for (int e = thread; e < n * 64; e += 256)
+        if ((e & 63) < a.half) sm.turn[e >> 6][e & 63] = turn64(a.inv_freq[e & 63], len + (e >> 6));
+    __syncthreads();
+#pragma unroll 1
+    for (int rt = 0; rt < RT; rt++) {
+        const int in = min(16 * rt + i, a.Mq - 1), l = in / a.G;
+        const QueryRow r = turned_query(query_at(a, b, hk, in), j, sm.turn[min(l, max(n - 1, 0))], a.half, l < n);
+        const int at = rt * 8 * 64 + (j & 3) * 64 + 16 * (j >> 2) + i;  // dims 32*g + 8*step .. of query i
+        sm.q[at] = r.hi;
+        sm.q[at + 4 * 64] = r.lo;
+        if (j == 0) factors[16 * rt + i] = r.c;
+    }
+#pragma unroll 1
+    for (int r = i; r < 2 * n; r += 16) {  // (k and v of a row in turn)
+        const int l = r >> 1;
+        const bool is_k = (r & 1) == 0;
+        write_row(a, is_k ? a.k + b * a.ksb + l * a.ksl + (int64_t)hk * kS : a.v + b * a.vsb + l * a.vsl + (int64_t)hk * kS, is_k, b, hk, len + l, j, sm.turn[l]);
+    }
+    __syncthreads();
+}
 
 // Units of 128 rows are numbered through: sequence after sequence, in each kv head after kv head, in each tile after tile.  Behind the units of a tile
 // there are kStart more without rows, for what it costs to begin with queries and to bring the waves' sums together, so that workgroups with short
@@ -212,34 +254,42 @@ __device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane, bool by
 }
 __device__ __forceinline__ int share_of(int all, int groups) { return (all + groups - 1) / groups; }
 
-__device__ __forceinline__ void q4_leave(const Q4Args& a, int hk, int m, int d, float4 o, float sum, bool live) {
+__device__ __forceinline__ void q4_leave(const Q4Args& a, int b, int hk, int in, int d, float4 o, float sum, bool live) {
     const float f = live ? 1.0f / sum : 0.0f;
-    const int bl = m / a.G;
-    *reinterpret_cast<float4*>(a.out + ((int64_t)bl * a.G * a.Hkv + (int64_t)hk * a.G + (m - bl * a.G)) * kS + d) =
+    const int l = in / a.G;
+    *reinterpret_cast<float4*>(a.out + (((int64_t)b * a.qL + l) * a.G * a.Hkv + (int64_t)hk * a.G + (in - l * a.G)) * kS + d) =
         live ? make_float4(o.x * f, o.y * f, o.z * f, o.w * f) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 constexpr int kQ4MeetRow = 132;  // floats (16 queries' rows on different banks)
+template <int RT>
 struct Q4MeetSmem {
-    float m[4][32], l[4][32], sum[16];
+    float m[4][32], l[4][32], sum[16], factors[16 * RT];
     union {
         float o[4][16][kQ4MeetRow];
-        uint4 q[16 * 64];
+        Q4FewIn<RT> in;
     };
 };
 
 // Few queries to a workgroup (16 * RT).  The four waves take 32 rows each of every 128; operands come straight from memory, the next rows asked
 // for when these are used up; the waves' sums meet in LDS.
-template <int RT>
+template <int RT, bool WHOLE>
 __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) {
-    __shared__ Q4MeetSmem sm;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    __shared__ Q4MeetSmem<RT> sm;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Codes codes;
-    int share = 0;
-    const UnitPlace start = place_of(a, lane, true, [&](int all) { share = share_of(all, a.groups); return (int)min((int64_t)blockIdx.x * share, (int64_t)INT_MAX); });
-    if (start.b < 0) return;
-    const int first = (int)blockIdx.x * share, last = min(start.all, first + share);
-    int b = start.b, before = start.before;
+    int b, before, first, last;
+    if constexpr (WHOLE) {  // a kv head of a sequence to a workgroup
+        b = blockIdx.x / a.Hkv, before = 0;
+        const int units = units_of(a, b).head;
+        first = (blockIdx.x - b * a.Hkv) * units, last = first + units;
+    } else {
+        int share = 0;
+        const UnitPlace start = place_of(a, threadIdx.x & 63, true, [&](int all) { share = share_of(all, a.groups); return (int)min((int64_t)blockIdx.x * share, (int64_t)INT_MAX); });
+        if (start.b < 0) return;
+        b = start.b, before = start.before;
+        first = (int)blockIdx.x * share, last = min(start.all, first + share);
+    }
     UnitsOf its = units_of(a, b);
 #pragma unroll 1
     for (int at = first; at < last;) {
@@ -248,30 +298,31 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
             its = units_of(a, ++b);
         }
         const int hk = (at - before) / its.head;
-        int tile, units, u0;
+        int tile, units, u0;  // (one tile)
         tile_of(its, at - before - hk * its.head, tile, units, u0);
         const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
         at += u1 - u0;
         if (u0 >= real) continue;
+        const int lane = (int)unseen(threadIdx.x & 63), i = lane & 15, g = lane >> 4;
         int len, n;
         own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-        const int m0 = b * a.Mq + tile * 16 * RT, m_end = min((b + 1) * a.Mq, m0 + 16 * RT);
-        // rows that the tile's last live query sees
-        const int seen_by_last = min(n, (m_end - 1 - b * a.Mq) / a.G + 1), rows = tile * 16 * RT < n * a.G ? len + seen_by_last : 0;
+        const int rows = n > 0 ? len + n : 0;
         const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kQ4Row;
-        const uint8_t *K = a.k + plane, *V = a.v + plane;
+        const uint8_t *K = a.ck + plane, *V = a.cv + plane;
         Q4Regs x;
         const int j0 = 4 * u0 + wave, j1 = min(4 * u1, (rows + 31) / 32);
+        if constexpr (WHOLE) q4_begin<RT>(a, sm.in, sm.factors, b, hk, len, n);
         if (j0 < j1) x.load_k(q4_rows(K, 32 * j0, rows), i, g), x.load_v(q4_rows(V, 32 * j0, rows), i, g);
-        Q4QueryOps<RT> q;
-        q.load(a, sm.q, hk, m0, m_end, lane);
+        if constexpr (!WHOLE) q4_take<RT>(a, sm.in, sm.factors, b, hk, lane);
         Queries<RT> s;
-        s.start(a.cq + (int64_t)hk * a.M + m0, m0, m_end, i);
         bool live[RT];
         int see_min = INT_MAX;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            const int l = (min(m0 + 16 * rt + i, m_end - 1) - b * a.Mq) / a.G;
+            const int l = min(16 * rt + i, a.Mq - 1) / a.G;
+            s.c[rt] = sm.factors[16 * rt + i], s.m[rt] = -INFINITY, s.l[rt] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 8; c++) s.o[rt][c] = v4f{0.f, 0.f, 0.f, 0.f};
             live[rt] = l < n;
             s.see[rt] = live[rt] ? len + l + 1 : INT_MAX;  // (what padding sees is thrown away)
             see_min = min(see_min, s.see[rt]);
@@ -280,6 +331,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
         for (int j = j0; j < j1; j += 4) {
             const int t = 32 * j;
             const bool masked = __any(t + 32 > see_min);
+            const uint4* q = sm.in.q + unseen(lane);  // (read here and now: kept from one time to the next, operands take registers)
             v4f sc[RT][2];
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -288,7 +340,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
                 const v8h k0 = x.k_op(codes, 0, step), k1 = x.k_op(codes, 1, step);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
-                    const v8h hi = q.hi(rt, step), lo = q.lo(rt, step);
+                    const v8h hi = as_v8h(q[(rt * 8 + step) * 64]), lo = as_v8h(q[(rt * 8 + 4 + step) * 64]);
                     sc[rt][0] = mfma(k0, hi, sc[rt][0]);
                     sc[rt][1] = mfma(k1, hi, sc[rt][1]);
                     sc[rt][0] = mfma(k0, lo, sc[rt][0]);
@@ -360,15 +412,15 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const int e = threadIdx.x + 256 * u, query = e >> 5, d = 4 * (e & 31), m = m0 + 16 * rt + query;
-                if (m < m_end) {
+                const int e = lane + 64 * wave + 256 * u, query = e >> 5, d = 4 * (e & 31), in = 16 * rt + query;
+                if (in < a.Mq) {
                     float4 r = *reinterpret_cast<const float4*>(&sm.o[0][query][d]);
 #pragma unroll
                     for (int w = 1; w < 4; w++) {
                         const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][query][d]);
                         r.x += y.x, r.y += y.y, r.z += y.z, r.w += y.w;
                     }
-                    if (whole) q4_leave(a, hk, m, d, r, sm.sum[query], sm.sum[query] != -1.0f);
+                    if (whole) q4_leave(a, b, hk, in, d, r, sm.sum[query], sm.sum[query] != -1.0f);
                     else *reinterpret_cast<float4*>(a.rec_out + (record + 16 * rt + query) * kS + d) = r;
                 }
             }
@@ -458,33 +510,32 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
         if (u0 >= real) continue;
         int len, n;
         own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-        const int m0 = b * a.Mq + tile * 64 * RT, m_end = min((b + 1) * a.Mq, m0 + 64 * RT);
-        const int seen_by_last = min(n, (m_end - 1 - b * a.Mq) / a.G + 1), rows = tile * 64 * RT < n * a.G ? len + seen_by_last : 0;
+        const int in0 = tile * 64 * RT, in_end = min(a.Mq, in0 + 64 * RT);
+        // rows that the tile's last live query sees
+        const int rows = in0 < n * a.G ? len + min(n, (in_end - 1) / a.G + 1) : 0;
         const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kQ4Row;
-        const uint8_t *K = a.k + plane, *V = a.v + plane;
+        const uint8_t *K = a.ck + plane, *V = a.cv + plane;
         const int j0 = 2 * u0, j1 = min(2 * u1, (rows + 63) / 64);
         Q4TileRegs x;
         auto load = [&](int j) { x.load(q4_rows<64>(K, 64 * j, rows), q4_rows<64>(V, 64 * j, rows), wave, i, g); };
         if (j0 < j1) load(j0);
         v8h qh[RT][4], ql[RT][4];
         Queries<RT> s;
-        const int mw = m0 + 16 * RT * wave;
         bool live[RT];
         int see_min = INT_MAX;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            const int m = min(mw + 16 * rt + i, m_end - 1), l = (m - b * a.Mq) / a.G;
-            const int64_t from = ((int64_t)hk * a.M + m) * kS + 32 * g;
+            const int in = min(in0 + 16 * (RT * wave + rt) + i, in_end - 1), l = in / a.G;
+            live[rt] = l < n;
+            const int64_t m = (int64_t)hk * a.M + (int64_t)b * a.Mq + in, from = m * kS + 32 * g;
 #pragma unroll
             for (int step = 0; step < 4; step++) {
                 qh[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + from + 8 * step));
                 ql[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + from + 8 * step));
             }
-            s.c[rt] = a.cq[(int64_t)hk * a.M + m];
-            s.m[rt] = -INFINITY, s.l[rt] = 0.0f;
+            s.c[rt] = a.cq[m], s.m[rt] = -INFINITY, s.l[rt] = 0.0f;
 #pragma unroll
             for (int c = 0; c < 8; c++) s.o[rt][c] = v4f{0.f, 0.f, 0.f, 0.f};
-            live[rt] = l < n;
             s.see[rt] = live[rt] ? len + l + 1 : INT_MAX;  // (what padding sees is thrown away)
             see_min = min(see_min, s.see[rt]);
         }
@@ -555,8 +606,8 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
         for (int rt = 0; rt < RT; rt++) {
             s.l[rt] += __shfl_xor(s.l[rt], 16, 64);
             s.l[rt] += __shfl_xor(s.l[rt], 32, 64);
-            const int in = 16 * RT * wave + 16 * rt + i, m = m0 + in;
-            if (m >= m_end) continue;
+            const int in = 16 * (RT * wave + rt) + i;
+            if (in0 + in >= in_end) continue;
             if (!whole && g == 0) a.rec_stat[record + in] = make_float2(s.m[rt], s.l[rt]);
 #pragma unroll
             for (int v = 0; v < 4; v++)
@@ -564,7 +615,7 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
                 for (int h = 0; h < 2; h++) {
                     const float4 o = make_float4(s.o[rt][4 * h][v], s.o[rt][4 * h + 1][v], s.o[rt][4 * h + 2][v], s.o[rt][4 * h + 3][v]);
                     const int d = 8 * (4 * g + v) + 4 * h;
-                    if (whole) q4_leave(a, hk, m, d, o, s.l[rt], live[rt]);
+                    if (whole) q4_leave(a, b, hk, in0 + in, d, o, s.l[rt], live[rt]);
                     else *reinterpret_cast<float4*>(a.rec_out + (record + in) * kS + d) = o;
                 }
         }
@@ -636,7 +687,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
         }
     }
     const int in = tile * a.tile + query;
-    if (query < in0 + queries) q4_leave(a, hk, b * a.Mq + in, d, o, L, in / a.G < n);
+    if (query < in0 + queries) q4_leave(a, b, hk, in, d, o, L, in / a.G < n);
 }
 
 struct Q4Plan {
@@ -650,7 +701,12 @@ static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t max
     p.rt = !p.many && Mq > 16 ? 2 : 1;
     p.tile = (p.many ? 64 : 16) * p.rt;
     p.tiles = (int)((Mq + p.tile - 1) / p.tile);
-    const int64_t most = B * Hkv * p.tiles * ((maxlen + kUnit - 1) / kUnit + kStart), held = p.many || p.rt == 2 ? 512 : 1024;  // (workgroups that the chip holds)
+    const int64_t items = B * Hkv * p.tiles;
+    if (!p.many && maxlen <= 3 * kUnit) {
+        p.groups = (int)items;
+        return p;
+    }
+    const int64_t most = items * ((maxlen + kUnit - 1) / kUnit + kStart), held = p.many || p.rt == 2 ? 512 : 1024;  // (workgroups that the chip holds)
     p.groups = (int)(most < held ? most : held);
     const int64_t queries = B * Hkv * Mq;  // (workgroups enough to fill the chip, then queries to each)
     p.join = queries >= 8192 ? 8 : queries >= 4096 ? 4 : queries >= 2048 ? 2 : 1;
@@ -667,26 +723,30 @@ static Q4Layout layout_q4(const Q4Plan& plan, int64_t rows) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    const size_t records = (size_t)plan.groups * 2 * plan.tile;
-    w.qh = take((size_t)rows * kS * 2);
-    w.ql = take((size_t)rows * kS * 2);
-    w.cq = take((size_t)rows * 4);
+    const size_t records = plan.join > 0 ? (size_t)plan.groups * 2 * plan.tile : 0, held = plan.join > 0 ? rows : 0;
+    w.qh = take(held * kS * 2);
+    w.ql = take(held * kS * 2);
+    w.cq = take(held * 4);
     w.stat = take(records * 8);
     w.rec = take(records * kS * 4);
-    w.total = at;
+    w.total = at > 0 ? at : 256;  // (0 stands for sizes that are refused)
     return w;
 }
 
-static int q4_launch(const Q4Args& a, const Q4Prep& p, const Q4Plan& plan, hipStream_t st) {
-    q4_prep_kernel<<<(unsigned)((int64_t)a.B * a.qL * p.rows16), 256, 0, st>>>(a, p);
+static int q4_launch(const Q4Args& a, const Q4Plan& plan, hipStream_t st) {
+    if (plan.join > 0) q4_prep_kernel<<<(unsigned)((int64_t)a.B * a.qL * a.rows16), 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
     const unsigned groups = (unsigned)plan.groups;
     if (plan.many) q4_many_kernel<1><<<groups, 256, 0, st>>>(a);
-    else if (plan.rt == 2) q4_few_kernel<2><<<groups, 256, 0, st>>>(a);
-    else q4_few_kernel<1><<<groups, 256, 0, st>>>(a);
+    else if (plan.join == 0 && plan.rt == 2) q4_few_kernel<2, true><<<groups, 256, 0, st>>>(a);
+    else if (plan.join == 0) q4_few_kernel<1, true><<<groups, 256, 0, st>>>(a);
+    else if (plan.rt == 2) q4_few_kernel<2, false><<<groups, 256, 0, st>>>(a);
+    else q4_few_kernel<1, false><<<groups, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
-    const int64_t parts = ((plan.tile < a.Mq ? plan.tile : a.Mq) + plan.join - 1) / plan.join;
-    q4_join_kernel<<<(unsigned)((int64_t)a.B * a.Hkv * plan.tiles * parts), 256, 0, st>>>(a);
+    if (plan.join > 0) {
+        const int64_t parts = ((plan.tile < a.Mq ? plan.tile : a.Mq) + plan.join - 1) / plan.join;
+        q4_join_kernel<<<(unsigned)((int64_t)a.B * a.Hkv * plan.tiles * parts), 256, 0, st>>>(a);
+    }
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }
@@ -728,18 +788,19 @@ extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int6
     if (workspace_bytes < w.total) return fail(LLMOPS_EWORKSPACE, "attention_rope_q4 needs %zu workspace bytes, got %zu", w.total, workspace_bytes);
     char* ws = reinterpret_cast<char*>(workspace);
     Q4Args a{};
+    a.q = q, a.k = k, a.v = v, a.inv_freq = inv_freq;
+    a.qsb = q_stride_b, a.qsl = q_stride_l, a.ksb = k_stride_b, a.ksl = k_stride_l, a.vsb = v_stride_b, a.vsl = v_stride_l;
     a.qh = reinterpret_cast<_Float16*>(ws + w.qh), a.ql = reinterpret_cast<_Float16*>(ws + w.ql), a.cq = reinterpret_cast<float*>(ws + w.cq);
     a.rec_out = reinterpret_cast<float*>(ws + w.rec), a.rec_stat = reinterpret_cast<float2*>(ws + w.stat);
-    a.k = reinterpret_cast<uint8_t*>(kv_cache) + 2 * layer_id * (int64_t)plane, a.v = a.k + (int64_t)plane;
+    a.ck = reinterpret_cast<uint8_t*>(kv_cache) + 2 * layer_id * (int64_t)plane, a.cv = a.ck + (int64_t)plane;
     a.lengths = lengths, a.q_lens = q_lens, a.out = out, a.maxlen = maxlen;
-    a.B = (int)B, a.qL = (int)qL, a.G = (int)G, a.Hkv = (int)Hkv, a.Mq = (int)(qL * G), a.M = (int)(B * qL * G);
+    a.B = (int)B, a.qL = (int)qL, a.G = (int)G, a.Hkv = (int)Hkv, a.Mq = (int)(qL * G), a.M = (int)(B * qL * G), a.half = (int)half, a.rows16 = (int)rows16;
     a.tile = plan.tile, a.tiles = plan.tiles, a.groups = plan.groups, a.join = plan.join;
     // (a workgroup reads its q, k and v while others may have written their rows and results)
     const Extent q_at(q, B, (Wide)q_stride_b * 4, qL, (Wide)q_stride_l * 4, heads), k_at(k, B, (Wide)k_stride_b * 4, qL, (Wide)k_stride_l * 4, kv_heads),
-        v_at(v, B, (Wide)v_stride_b * 4, qL, (Wide)v_stride_l * 4, kv_heads), out_at(out, (Wide)B * qL * heads), written(a.k, 2 * plane);
+        v_at(v, B, (Wide)v_stride_b * 4, qL, (Wide)v_stride_l * 4, kv_heads), out_at(out, (Wide)B * qL * heads), written(a.ck, 2 * plane);
     LLMOPS_REQUIRE(apart(written, q_at) && apart(written, k_at) && apart(written, v_at));
     LLMOPS_REQUIRE(apart(out_at, q_at) && apart(out_at, k_at) && apart(out_at, v_at) && apart(out_at, written));
-    const Q4Prep p{q, k, v, inv_freq, q_stride_b, q_stride_l, k_stride_b, k_stride_l, v_stride_b, v_stride_l, (int)half, (int)rows16};
     hipStream_t st = as_stream(stream);
-    return q4_launch(a, p, plan, st);
+    return q4_launch(a, plan, st);
 }

@@ -29,10 +29,16 @@ __global__ __launch_bounds__(256) void q4_write_turned_kernel(WriteArgs a) {
     const bool is_k = row < a.Hkv;
     const int hk = is_k ? row : row - a.Hkv;
     const T* src = is_k ? (const T*)a.k + b * a.ksb + l * a.ksl + hk * a.ksh : (const T*)a.v + b * a.vsb + l * a.vsl + hk * a.vsh;
-    double x[8];
+    uint8_t* dst = (is_k ? a.ck : a.cv) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kQ4Row;
+    float x[8];
     load8(src + 8 * j, x);
-    if (is_k) turn_row64(src, j, turn, a.half, x);
-    store_q4((is_k ? a.ck : a.cv) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kQ4Row, quantise8(x), j);
+    if (is_k) {
+        double y[8];
+        turn_row64(src, x, j, turn, a.half, y);
+        store_q4(dst, quantise8(y), j);
+    } else {
+        store_q4(dst, quantise8(x), j);
+    }
 }
 
 // Rows that need no turning, in fp32: a workgroup per 16 tokens and one of the 2*Hkv rows of each.  Rows that all sequences are given

@@ -69,16 +69,34 @@ __device__ __forceinline__ uint2 quantise8(const R (&x)[8]) {
     const int step = ((int)(hi - lo) + 14) / 15;  // (lo is no -0: zeros of either sign are stored alike)
     const float s = (float)step, half = 0.5f * s, inv = step > 0 ? 1.0f / s : 0.0f;
     uint32_t word = 0;
+    bool near = sizeof(R) == 4;
+    if constexpr (sizeof(R) == 8) {
+        // in fp32, which is off by less than 2^-12 here, unless a value is nearer than 2^-11 to a border (in one of some thousand rows)
+        const float scale = ldexpf(1.0f, 11 - e);
+        float nearest = 1.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        // a first guess, put right by the borders on either side of it, which are exact: lo + (c - 1/2) s and lo + (c + 1/2) s
-        const R t = scaled(x[i], 11 - e);
-        const float c = fminf(fmaxf(rintf(((float)t - lo) * inv), 0.0f), 15.0f), level = fmaf(c, s, lo);
-        const bool odd = (int)c & 1;
-        const R above = (R)(level + half), below = (R)(level - half);
-        int code = (int)c + ((t > above || (t == above && odd)) ? 1 : 0) - ((t < below || (t == below && odd)) ? 1 : 0);
-        code = step > 0 ? min(max(code, 0), 15) : 0;
-        word |= (uint32_t)code << (4 * (i >> 1) + 16 * (i & 1));
+        for (int i = 0; i < 8; i++) {
+            const float t = (float)x[i] * scale, c = fminf(fmaxf(rintf((t - lo) * inv), 0.0f), 15.0f), off = t - fmaf(c, s, lo);
+            nearest = fminf(nearest, fabsf(fabsf(off) - half));
+            const int code = min(max((int)c + (off > half ? 1 : 0) - (off < -half ? 1 : 0), 0), 15);
+            word |= (uint32_t)code << (4 * (i >> 1) + 16 * (i & 1));
+        }
+        near = nearest < 0x1p-11f;
+        if (step == 0) near = false, word = 0;
+    }
+    if (__any(near)) {
+        word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            // a first guess, put right by the borders on either side of it, which are exact: lo + (c - 1/2) s and lo + (c + 1/2) s
+            const R t = scaled(x[i], 11 - e);
+            const float c = fminf(fmaxf(rintf(((float)t - lo) * inv), 0.0f), 15.0f), level = fmaf(c, s, lo);
+            const bool odd = (int)c & 1;
+            const R above = (R)(level + half), below = (R)(level - half);
+            int code = (int)c + ((t > above || (t == above && odd)) ? 1 : 0) - ((t < below || (t == below && odd)) ? 1 : 0);
+            code = step > 0 ? min(max(code, 0), 15) : 0;
+            word |= (uint32_t)code << (4 * (i >> 1) + 16 * (i & 1));
+        }
     }
     const uint32_t d = f32_to_f16_bits(ldexpf(s, e - 11)), m = f32_to_f16_bits(ldexpf(lo, e - 11));
     return spoilt ? make_uint2(0u, 0x7e000000u) : make_uint2(word, d | m << 16);
@@ -96,23 +114,45 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, R (&x)[8]) {
     }
 }
 
-// dims 8 j .. of a row turned, in 64 bits: pairs (at, at + half), the dims behind them as they are.  x: the row's own values of these dims
+// dims 8 j .. of a row turned: pairs (at, at + half), the dims behind them as they are.  x: the row's own values of these dims.  In 64 bits ..
 template <typename T>
-__device__ __forceinline__ void turn_row64(const T* __restrict__ row, int j, const double2* turn, int half, double (&x)[8]) {
+__device__ __forceinline__ void turn_row64(const T* __restrict__ row, const float (&x)[8], int j, const double2* turn, int half, double (&out)[8]) {
     if (half == 64) {
-        double y[8];
+        float y[8];
         load8(row + (8 * j ^ 64), y);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const double2 t = turn[(8 * j & 63) + e];
-            x[e] = j < 8 ? t.x * x[e] - t.y * y[e] : t.x * x[e] + t.y * y[e];
+            out[e] = fma(t.x, (double)x[e], (j < 8 ? -t.y : t.y) * (double)y[e]);
         }
     } else {
+        const int first = 8 * (int)unseen(j);  // (so that no loop keeps these addresses in registers)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const int at = 8 * j + e;
-            if (at < half) x[e] = turn[at].x * x[e] - turn[at].y * (double)(float)row[at + half];
-            else if (at < 2 * half) x[e] = turn[at - half].x * x[e] + turn[at - half].y * (double)(float)row[at - half];
+            const int at = first + e;
+            out[e] = x[e];
+            if (at < half) out[e] = fma(turn[at].x, (double)x[e], -turn[at].y * (double)(float)row[at + half]);
+            else if (at < 2 * half) out[e] = fma(turn[at - half].x, (double)x[e], turn[at - half].y * (double)(float)row[at - half]);
+        }
+    }
+}
+// .. and in fp32
+__device__ __forceinline__ void turn_row32(const float* __restrict__ row, int j, const double2* turn, int half, float (&x)[8]) {
+    if (half == 64) {
+        float y[8];
+        load8(row + (8 * j ^ 64), y);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double2 t = turn[(8 * j & 63) + e];
+            x[e] = fmaf((float)t.x, x[e], (j < 8 ? -(float)t.y : (float)t.y) * y[e]);
+        }
+    } else {
+        const int first = 8 * (int)unseen(j);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int at = first + e;
+            if (at < half) x[e] = fmaf((float)turn[at].x, x[e], -(float)turn[at].y * row[at + half]);
+            else if (at < 2 * half) x[e] = fmaf((float)turn[at - half].x, x[e], (float)turn[at - half].y * row[at - half]);
         }
     }
 }

@@ -27,7 +27,8 @@ struct Q4Args {
     uint8_t *ck, *cv;                   // the layer's planes [B][Hkv][maxlen][80]
     const int32_t *lengths, *q_lens;    // [B]; q_lens may be null
     float* rec_out;                     // [groups][2][queries of a tile][128]
-    float2* rec_stat;                   // [groups][2][queries of a tile]: max (log2), sum
+    float2* rec_stat;                   // [groups][2][queries of a tile]: max (log2), sum (-1: padding)
+    int2* parts;                        // [B][Hkv][tiles]: the first and the last workgroup that have rows of a tile
     float* out;                         // [B][qL][H*128]
     int64_t maxlen;
     int B, qL, G, Hkv, M, Mq, half;     // Mq = qL*G
@@ -42,24 +43,27 @@ __device__ __forceinline__ const float* query_at(const Q4Args& a, int b, int hk,
 
 // ---- 1. ----
 // Sixteen lanes to a row of k or v, dims 8 * (lane % 16) .. to a lane: k turned and its codes chosen in 64 bits, v in fp32; the row written
-__device__ __forceinline__ void write_row(const Q4Args& a, const float* src, bool is_k, int b, int hk, int64_t row, int j, const double2* turn) {
+__device__ __forceinline__ void write_row(const Q4Args& a, const RowPair& p, const float* src, bool is_k, int b, int hk, int64_t row, int j, const double2* turn) {
     uint8_t* dst = (is_k ? a.ck : a.cv) + (((int64_t)b * a.Hkv + hk) * a.maxlen + row) * kQ4Row;
-    float x[8];
-    load8(src + 8 * j, x);
     if (is_k) {
-        double y[8];
-        turn_row64(src, x, j, turn, a.half, y);
-        store_q4(dst, quantise8(y), j);
-    } else {
+        double x[8];
+        turn_row(p, src, j, turn, a.half, x);
         store_q4(dst, quantise8(x), j);
+    } else {
+        store_q4(dst, quantise8(p.x), j);
     }
 }
 // .. of a query: turned in fp32
-__device__ __forceinline__ QueryRow turned_query(const float* src, int j, const double2* turn, int half, bool live) {
+__device__ __forceinline__ QueryRow turned_query(const RowPair& p, const float* src, int j, const double2* turn, int half, bool live) {
     float x[8];
-    load8(src + 8 * j, x);
-    if (live) turn_row32(src, j, turn, half, x);
+    if (live) turn_row(p, src, j, turn, half, x);
+    else
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = 0.0f;
     return query_row(x, live);
+}
+__device__ __forceinline__ const float* new_row_at(const Q4Args& a, bool is_k, int b, int hk, int l) {
+    return is_k ? a.k + b * a.ksb + l * a.ksl + (int64_t)hk * kS : a.v + b * a.vsb + l * a.vsl + (int64_t)hk * kS;
 }
 
 // A workgroup per token and 16 of its H + 2*Hkv rows of 128, sixteen lanes to a row
@@ -67,21 +71,25 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a) {
     __shared__ double2 turn[64];
     const int bl = blockIdx.x / a.rows16, group = blockIdx.x - bl * a.rows16, b = bl / a.qL, l = bl - b * a.qL;
     const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), j = threadIdx.x & 15;
+    const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv, none = row >= H + 2 * a.Hkv;
+    const int hk = is_k ? row - H : row - H - a.Hkv;
+    const float* src = is_q ? a.q + b * a.qsb + l * a.qsl + (int64_t)row * kS : new_row_at(a, is_k, b, hk, l);
+    // (the row is on its way while the length is fetched and the angles are formed, also where the token turns out to be padding)
+    RowPair p = {};
+    if (!none) p.load(src, j);
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
     const bool live = l < n;
     if (live && (int)threadIdx.x < a.half) turn[threadIdx.x] = turn64(a.inv_freq[threadIdx.x], len + l);
     __syncthreads();
-    if (row < H) {
+    if (is_q) {
         const int64_t m = (int64_t)(row / a.G) * a.M + (int64_t)bl * a.G + row % a.G;
-        const QueryRow r = turned_query(a.q + b * a.qsb + l * a.qsl + (int64_t)row * kS, j, turn, a.half, live);
+        const QueryRow r = turned_query(p, src, j, turn, a.half, live);
         *reinterpret_cast<uint4*>(a.qh + m * kS + 8 * j) = r.hi;
         *reinterpret_cast<uint4*>(a.ql + m * kS + 8 * j) = r.lo;
         if (j == 0) a.cq[m] = r.c;
-    } else if (live && row < H + 2 * a.Hkv) {
-        const bool is_k = row < H + a.Hkv;
-        const int hk = is_k ? row - H : row - H - a.Hkv;
-        write_row(a, is_k ? a.k + b * a.ksb + l * a.ksl + (int64_t)hk * kS : a.v + b * a.vsb + l * a.vsl + (int64_t)hk * kS, is_k, b, hk, len + l, j, turn);
+    } else if (live && !none) {
+        write_row(a, p, src, is_k, b, hk, len + l, j, turn);
     }
 }
 
@@ -163,26 +171,27 @@ __device__ __forceinline__ void q4_take(const Q4Args& a, Q4FewIn<RT>& sm, float*
 // Loads that wait for each other: where many workgroups keep the memory busy the launch is the better way (32 sequences of up to 4096 rows 88 us with
 // it, 109 without; two of up to 200 14.9 and 10.7).
 template <int RT>
-__device__ __forceinline__ void q4_begin(const Q4Args& a, Q4FewIn<RT>& sm, float* factors, int b, int hk, int len, int n) {
+__device__ __forceinline__ void q4_begin(const Q4Args& a, Q4FewIn<RT>& sm, float* factors, int b, int hk, int len, int n, const RowPair (&q)[RT], const RowPair& first_new) {
     const int thread = (int)unseen(threadIdx.x), i = thread >> 4, j = thread & 15;
 #pragma unroll 1
     for (int e = thread; e < n * 64; e += 256)
         if ((e & 63) < a.half) sm.turn[e >> 6][e & 63] = turn64(a.inv_freq[e & 63], len + (e >> 6));
     __syncthreads();
-#pragma unroll 1
+#pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int in = min(16 * rt + i, a.Mq - 1), l = in / a.G;
-        const QueryRow r = turned_query(query_at(a, b, hk, in), j, sm.turn[min(l, max(n - 1, 0))], a.half, l < n);
+        const QueryRow r = turned_query(q[rt], query_at(a, b, hk, in), j, sm.turn[min(l, max(n - 1, 0))], a.half, l < n);
         const int at = rt * 8 * 64 + (j & 3) * 64 + 16 * (j >> 2) + i;  // dims 32*g + 8*step .. of query i
         sm.q[at] = r.hi;
         sm.q[at + 4 * 64] = r.lo;
         if (j == 0) factors[16 * rt + i] = r.c;
     }
+    RowPair p = first_new;
 #pragma unroll 1
     for (int r = i; r < 2 * n; r += 16) {  // (k and v of a row in turn)
-        const int l = r >> 1;
-        const bool is_k = (r & 1) == 0;
-        write_row(a, is_k ? a.k + b * a.ksb + l * a.ksl + (int64_t)hk * kS : a.v + b * a.vsb + l * a.vsl + (int64_t)hk * kS, is_k, b, hk, len + l, j, sm.turn[l]);
+        const float* src = new_row_at(a, (r & 1) == 0, b, hk, r >> 1);
+        if (r != i) p.load(src, j);
+        write_row(a, p, src, (r & 1) == 0, b, hk, len + (r >> 1), j, sm.turn[r >> 1]);
     }
     __syncthreads();
 }
@@ -218,12 +227,12 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
     }
     return v;
 }
-// Every wave for itself: all units, and the sequence that has unit `wanted(all)`, or that is `wanted(all)` where by_unit is false; the units before it.
+// Every wave for itself: all units, the share of a workgroup, and the sequence that has the first unit of this one's (-1: none is left), with the units
+// before that sequence
 struct UnitPlace {
-    int all, b, before;
+    int all, share, b, before;
 };
-template <typename F>
-__device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane, bool by_unit, F wanted) {
+__device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane) {
     int all = 0, its = 0, upto = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -231,9 +240,9 @@ __device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane, bool by
         upto = all + wave_scan(its, lane);
         all = __builtin_amdgcn_readlane(upto, 63);
     }
-    UnitPlace p{all, -1, 0};
-    const int want = wanted(all);
-    if (by_unit && want >= all) return p;
+    UnitPlace p{all, (all + a.groups - 1) / a.groups, -1, 0};
+    const int64_t want = (int64_t)blockIdx.x * p.share;
+    if (want >= all) return p;
     int before = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -241,7 +250,7 @@ __device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane, bool by
             its = b0 + lane < a.B ? units_of(a, b0 + lane).head * a.Hkv : 0;
             upto = before + wave_scan(its, lane);
         }
-        const uint64_t hit = by_unit ? __ballot(upto > want) : want >= b0 && want < b0 + 64 ? 1ull << (want - b0) : 0;
+        const uint64_t hit = __ballot(upto > want);
         if (hit != 0) {
             const int at = __builtin_ctzll(hit);
             p.b = b0 + at;
@@ -252,7 +261,6 @@ __device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane, bool by
     }
     return p;
 }
-__device__ __forceinline__ int share_of(int all, int groups) { return (all + groups - 1) / groups; }
 
 __device__ __forceinline__ void q4_leave(const Q4Args& a, int b, int hk, int in, int d, float4 o, float sum, bool live) {
     const float f = live ? 1.0f / sum : 0.0f;
@@ -274,21 +282,27 @@ struct Q4MeetSmem {
 // Few queries to a workgroup (16 * RT).  The four waves take 32 rows each of every 128; operands come straight from memory, the next rows asked
 // for when these are used up; the waves' sums meet in LDS.
 template <int RT, bool WHOLE>
-__global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) {
+__global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(Q4Args a) {
     __shared__ Q4MeetSmem<RT> sm;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Codes codes;
-    int b, before, first, last;
+    int b, before, first, last, share = 1;
     if constexpr (WHOLE) {  // a kv head of a sequence to a workgroup
         b = blockIdx.x / a.Hkv, before = 0;
         const int units = units_of(a, b).head;
         first = (blockIdx.x - b * a.Hkv) * units, last = first + units;
     } else {
-        int share = 0;
-        const UnitPlace start = place_of(a, threadIdx.x & 63, true, [&](int all) { share = share_of(all, a.groups); return (int)min((int64_t)blockIdx.x * share, (int64_t)INT_MAX); });
+        const UnitPlace start = place_of(a, threadIdx.x & 63);
         if (start.b < 0) return;
-        b = start.b, before = start.before;
+        b = start.b, before = start.before, share = start.share;
         first = (int)blockIdx.x * share, last = min(start.all, first + share);
+    }
+    RowPair q_rows[WHOLE ? RT : 1], new_row;
+    if constexpr (WHOLE) {  // (asked for with the length)
+        const int r = threadIdx.x >> 4, j = threadIdx.x & 15, hk = blockIdx.x - b * a.Hkv;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) q_rows[rt].load(query_at(a, b, hk, min(16 * rt + r, a.Mq - 1)), j);
+        if (r < 2 * a.qL) new_row.load(new_row_at(a, (r & 1) == 0, b, hk, r >> 1), j);
     }
     UnitsOf its = units_of(a, b);
 #pragma unroll 1
@@ -301,6 +315,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
         int tile, units, u0;  // (one tile)
         tile_of(its, at - before - hk * its.head, tile, units, u0);
         const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
+        if (!WHOLE && u0 == 0 && threadIdx.x == 0)
+            a.parts[((int64_t)b * a.Hkv + hk) * a.tiles + tile] = make_int2(blockIdx.x, blockIdx.x + (at + real - 1 - (int)blockIdx.x * share) / share);
         at += u1 - u0;
         if (u0 >= real) continue;
         const int lane = (int)unseen(threadIdx.x & 63), i = lane & 15, g = lane >> 4;
@@ -311,8 +327,13 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
         const uint8_t *K = a.ck + plane, *V = a.cv + plane;
         Q4Regs x;
         const int j0 = 4 * u0 + wave, j1 = min(4 * u1, (rows + 31) / 32);
-        if constexpr (WHOLE) q4_begin<RT>(a, sm.in, sm.factors, b, hk, len, n);
-        if (j0 < j1) x.load_k(q4_rows(K, 32 * j0, rows), i, g), x.load_v(q4_rows(V, 32 * j0, rows), i, g);
+        // (rows that were there before this call are asked for before the queries are turned, new ones when they are written)
+        const bool old = !WHOLE || 32 * j0 + 32 <= len;
+        if (j0 < j1 && old) x.load_k(q4_rows(K, 32 * j0, rows), i, g), x.load_v(q4_rows(V, 32 * j0, rows), i, g);
+        if constexpr (WHOLE) {
+            q4_begin<RT>(a, sm.in, sm.factors, b, hk, len, n, q_rows, new_row);
+            if (j0 < j1 && !old) x.load_k(q4_rows(K, 32 * j0, rows), i, g), x.load_v(q4_rows(V, 32 * j0, rows), i, g);
+        }
         if constexpr (!WHOLE) q4_take<RT>(a, sm.in, sm.factors, b, hk, lane);
         Queries<RT> s;
         bool live[RT];
@@ -407,7 +428,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 4 : 2) void q4_few_kernel(Q4Args a) 
                     L += sm.l[w][16 * rt + i] * (mw == M ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
                 }
                 sm.sum[i] = live[rt] ? L : -1.0f;
-                if (!whole) a.rec_stat[record + 16 * rt + i] = make_float2(M, L);
+                if (!whole) a.rec_stat[record + 16 * rt + i] = make_float2(M, sm.sum[i]);
             }
             __syncthreads();
 #pragma unroll
@@ -490,10 +511,9 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
     __shared__ Q4TileSmem sm;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const Codes codes;
-    int share = 0;
-    const UnitPlace start = place_of(a, lane, true, [&](int all) { share = share_of(all, a.groups); return (int)min((int64_t)blockIdx.x * share, (int64_t)INT_MAX); });
+    const UnitPlace start = place_of(a, lane);
     if (start.b < 0) return;
-    const int first = (int)blockIdx.x * share, last = min(start.all, first + share);
+    const int share = start.share, first = (int)blockIdx.x * share, last = min(start.all, first + share);
     int b = start.b, before = start.before;
     UnitsOf its = units_of(a, b);
 #pragma unroll 1
@@ -506,6 +526,8 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
         int tile, units, u0;
         tile_of(its, at - before - hk * its.head, tile, units, u0);
         const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
+        if (u0 == 0 && threadIdx.x == 0)
+            a.parts[((int64_t)b * a.Hkv + hk) * a.tiles + tile] = make_int2(blockIdx.x, blockIdx.x + (at + real - 1 - (int)blockIdx.x * share) / share);
         at += u1 - u0;
         if (u0 >= real) continue;
         int len, n;
@@ -608,7 +630,7 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
             s.l[rt] += __shfl_xor(s.l[rt], 32, 64);
             const int in = 16 * (RT * wave + rt) + i;
             if (in0 + in >= in_end) continue;
-            if (!whole && g == 0) a.rec_stat[record + in] = make_float2(s.m[rt], s.l[rt]);
+            if (!whole && g == 0) a.rec_stat[record + in] = make_float2(s.m[rt], live[rt] ? s.l[rt] : -1.0f);
 #pragma unroll
             for (int v = 0; v < 4; v++)
 #pragma unroll
@@ -629,14 +651,10 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
     __shared__ float4 part[8][32];
     const int parts = (min(a.tile, a.Mq) + a.join - 1) / a.join, item = blockIdx.x / parts, in0 = a.join * (blockIdx.x - item * parts);
     const int each = a.Hkv * a.tiles, b = item / each, hk = (item - b * each) / a.tiles, tile = item % a.tiles;
-    const UnitPlace p = place_of(a, threadIdx.x & 63, false, [&](int) { return b; });
-    const UnitsOf its = units_of(a, b);
-    if (tile >= its.live) return;  // (zeros, which one workgroup has written)
-    const int share = share_of(p.all, a.groups), at = p.before + hk * its.head + tile * its.tile, w0 = at / share, w1 = (at + its.tile - kStart - 1) / share;
+    const int2 of = a.parts[item];
+    const int w0 = of.x, w1 = of.y;
     const int queries = min(a.join, min(a.tile, a.Mq - tile * a.tile) - in0);
     if (w0 == w1 || queries <= 0) return;
-    int len, n;
-    own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
     const int halves = 8 / a.join;
     const int half = threadIdx.x >> 5, turn = half & (halves - 1), query = in0 + half / halves, d = 4 * (threadIdx.x & 31);
     float M = -INFINITY, L = 0.0f;
@@ -648,7 +666,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
             float4 x[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const int64_t wg = min(w + halves * u, w1), record = (wg * 2 + (wg * share <= at)) * a.tile + query;
+                const int64_t wg = min(w + halves * u, w1), record = (wg * 2 + (wg == w0)) * a.tile + query;
                 st[u] = a.rec_stat[record];
                 x[u] = *reinterpret_cast<const float4*>(a.rec_out + record * kS + d);
             }
@@ -687,7 +705,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
         }
     }
     const int in = tile * a.tile + query;
-    if (query < in0 + queries) q4_leave(a, b, hk, in, d, o, L, in / a.G < n);
+    if (query < in0 + queries) q4_leave(a, b, hk, in, d, o, L, !(L < 0.0f));
 }
 
 struct Q4Plan {
@@ -713,9 +731,9 @@ static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t max
     return p;
 }
 struct Q4Layout {
-    size_t qh, ql, cq, stat, rec, total;
+    size_t qh, ql, cq, parts, stat, rec, total;
 };
-static Q4Layout layout_q4(const Q4Plan& plan, int64_t rows) {
+static Q4Layout layout_q4(const Q4Plan& plan, int64_t rows, int64_t items) {
     Q4Layout w{};
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -727,6 +745,7 @@ static Q4Layout layout_q4(const Q4Plan& plan, int64_t rows) {
     w.qh = take(held * kS * 2);
     w.ql = take(held * kS * 2);
     w.cq = take(held * 4);
+    w.parts = take(plan.join > 0 ? items * 8 : 0);
     w.stat = take(records * 8);
     w.rec = take(records * kS * 4);
     w.total = at > 0 ? at : 256;  // (0 stands for sizes that are refused)
@@ -763,7 +782,8 @@ static bool q4_sizes_fit(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t 
 
 extern "C" size_t llmops_attention_q4_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t maxlen) {
     if (S != kS || !q4_sizes_fit(B, qL, H, Hkv, maxlen)) return 0;
-    return layout_q4(plan_q4(B, qL, H, Hkv, maxlen), B * qL * H).total;
+    const Q4Plan plan = plan_q4(B, qL, H, Hkv, maxlen);
+    return layout_q4(plan, B * qL * H, B * Hkv * plan.tiles).total;
 }
 
 extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b, int64_t k_stride_l,
@@ -784,14 +804,14 @@ extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int6
     const Wide heads = (Wide)H * kS * 4, kv_heads = (Wide)Hkv * kS * 4, plane = (Wide)B * Hkv * maxlen * kQ4Row;
     LLMOPS_REQUIRE((Wide)planes * plane < ((Wide)1 << 62));
     const Q4Plan plan = plan_q4(B, qL, H, Hkv, maxlen);
-    const Q4Layout w = layout_q4(plan, B * qL * H);
+    const Q4Layout w = layout_q4(plan, B * qL * H, B * Hkv * plan.tiles);
     if (workspace_bytes < w.total) return fail(LLMOPS_EWORKSPACE, "attention_rope_q4 needs %zu workspace bytes, got %zu", w.total, workspace_bytes);
     char* ws = reinterpret_cast<char*>(workspace);
     Q4Args a{};
     a.q = q, a.k = k, a.v = v, a.inv_freq = inv_freq;
     a.qsb = q_stride_b, a.qsl = q_stride_l, a.ksb = k_stride_b, a.ksl = k_stride_l, a.vsb = v_stride_b, a.vsl = v_stride_l;
     a.qh = reinterpret_cast<_Float16*>(ws + w.qh), a.ql = reinterpret_cast<_Float16*>(ws + w.ql), a.cq = reinterpret_cast<float*>(ws + w.cq);
-    a.rec_out = reinterpret_cast<float*>(ws + w.rec), a.rec_stat = reinterpret_cast<float2*>(ws + w.stat);
+    a.rec_out = reinterpret_cast<float*>(ws + w.rec), a.rec_stat = reinterpret_cast<float2*>(ws + w.stat), a.parts = reinterpret_cast<int2*>(ws + w.parts);
     a.ck = reinterpret_cast<uint8_t*>(kv_cache) + 2 * layer_id * (int64_t)plane, a.cv = a.ck + (int64_t)plane;
     a.lengths = lengths, a.q_lens = q_lens, a.out = out, a.maxlen = maxlen;
     a.B = (int)B, a.qL = (int)qL, a.G = (int)G, a.Hkv = (int)Hkv, a.Mq = (int)(qL * G), a.M = (int)(B * qL * G), a.half = (int)half, a.rows16 = (int)rows16;

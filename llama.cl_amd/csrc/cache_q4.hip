@@ -30,13 +30,15 @@ __global__ __launch_bounds__(256) void q4_write_turned_kernel(WriteArgs a) {
     const int hk = is_k ? row : row - a.Hkv;
     const T* src = is_k ? (const T*)a.k + b * a.ksb + l * a.ksl + hk * a.ksh : (const T*)a.v + b * a.vsb + l * a.vsl + hk * a.vsh;
     uint8_t* dst = (is_k ? a.ck : a.cv) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kQ4Row;
-    float x[8];
-    load8(src + 8 * j, x);
     if (is_k) {
-        double y[8];
-        turn_row64(src, x, j, turn, a.half, y);
-        store_q4(dst, quantise8(y), j);
+        RowPair p;
+        p.load(src, j);
+        double x[8];
+        turn_row(p, src, j, turn, a.half, x);
+        store_q4(dst, quantise8(x), j);
     } else {
+        float x[8];
+        load8(src + 8 * j, x);
         store_q4(dst, quantise8(x), j);
     }
 }
@@ -48,14 +50,17 @@ __global__ __launch_bounds__(256) void q4_write_kernel(WriteArgs a) {
     const int tiles = (a.qL + 15) / 16, plane_row = blockIdx.x % (2 * a.Hkv), rest = blockIdx.x / (2 * a.Hkv), tile = rest % tiles, b0 = rest / tiles;
     const bool is_k = plane_row < a.Hkv;
     const int hk = is_k ? plane_row : plane_row - a.Hkv, l = tile * 16 + (threadIdx.x >> 4), j = threadIdx.x & 15;
-    if (l >= a.qL) return;  // (all sixteen lanes of a row)
-    const T* src = is_k ? (const T*)a.k + b0 * a.ksb + l * a.ksl + hk * a.ksh : (const T*)a.v + b0 * a.vsb + l * a.vsl + hk * a.vsh;
+    const int b_end = a.shared ? a.B : b0 + 1, lane = threadIdx.x & 63;
+    // (all sixteen lanes of a row behind the last)
+    const T* src = is_k ? (const T*)a.k + b0 * a.ksb + min(l, a.qL - 1) * a.ksl + hk * a.ksh : (const T*)a.v + b0 * a.vsb + min(l, a.qL - 1) * a.vsl + hk * a.vsh;
     float x[8];
     load8(src + 8 * j, x);
+    int lens = 0, ns = 0;  // of 64 sequences, one to a lane
+    if (b0 + lane < b_end) own_extent(a.lengths, a.q_lens, b0 + lane, a.qL, a.maxlen, lens, ns);
     const uint2 q = quantise8(x);
-    for (int b = b0; b < (a.shared ? a.B : b0 + 1); b++) {
-        int len, n;
-        own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+    for (int b = b0; b < b_end; b++) {
+        if (b > b0 && (b & 63) == 0 && b + lane < b_end) own_extent(a.lengths, a.q_lens, b + lane, a.qL, a.maxlen, lens, ns);
+        const int len = __builtin_amdgcn_readlane(lens, (b - b0) & 63), n = __builtin_amdgcn_readlane(ns, (b - b0) & 63);
         if (l < n) store_q4((is_k ? a.ck : a.cv) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kQ4Row, q, j);
     }
 }

@@ -114,45 +114,32 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, R (&x)[8]) {
     }
 }
 
-// dims 8 j .. of a row turned: pairs (at, at + half), the dims behind them as they are.  x: the row's own values of these dims.  In 64 bits ..
-template <typename T>
-__device__ __forceinline__ void turn_row64(const T* __restrict__ row, const float (&x)[8], int j, const double2* turn, int half, double (&out)[8]) {
-    if (half == 64) {
-        float y[8];
+// A lane's eight values of a row, dims 8 j .., and those that they turn with where all dims turn (asked for together)
+struct RowPair {
+    float x[8], y[8];
+    template <typename T>
+    __device__ __forceinline__ void load(const T* __restrict__ row, int j) {
+        load8(row + 8 * j, x);
         load8(row + (8 * j ^ 64), y);
+    }
+};
+// .. turned: pairs (at, at + half), the dims behind them as they are.  R double or float
+template <typename R, typename T>
+__device__ __forceinline__ void turn_row(const RowPair& p, const T* __restrict__ row, int j, const double2* turn, int half, R (&out)[8]) {
+    if (half == 64) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const double2 t = turn[(8 * j & 63) + e];
-            out[e] = fma(t.x, (double)x[e], (j < 8 ? -t.y : t.y) * (double)y[e]);
+            out[e] = fma((R)t.x, (R)p.x[e], (j < 8 ? -(R)t.y : (R)t.y) * (R)p.y[e]);
         }
     } else {
         const int first = 8 * (int)unseen(j);  // (so that no loop keeps these addresses in registers)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int at = first + e;
-            out[e] = x[e];
-            if (at < half) out[e] = fma(turn[at].x, (double)x[e], -turn[at].y * (double)(float)row[at + half]);
-            else if (at < 2 * half) out[e] = fma(turn[at - half].x, (double)x[e], turn[at - half].y * (double)(float)row[at - half]);
-        }
-    }
-}
-// .. and in fp32
-__device__ __forceinline__ void turn_row32(const float* __restrict__ row, int j, const double2* turn, int half, float (&x)[8]) {
-    if (half == 64) {
-        float y[8];
-        load8(row + (8 * j ^ 64), y);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const double2 t = turn[(8 * j & 63) + e];
-            x[e] = fmaf((float)t.x, x[e], (j < 8 ? -(float)t.y : (float)t.y) * y[e]);
-        }
-    } else {
-        const int first = 8 * (int)unseen(j);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int at = first + e;
-            if (at < half) x[e] = fmaf((float)turn[at].x, x[e], -(float)turn[at].y * row[at + half]);
-            else if (at < 2 * half) x[e] = fmaf((float)turn[at - half].x, x[e], (float)turn[at - half].y * row[at - half]);
+            out[e] = p.x[e];
+            if (at < half) out[e] = fma((R)turn[at].x, (R)p.x[e], -(R)turn[at].y * (R)(float)row[at + half]);
+            else if (at < 2 * half) out[e] = fma((R)turn[at - half].x, (R)p.x[e], (R)turn[at - half].y * (R)(float)row[at - half]);
         }
     }
 }

@@ -43,25 +43,30 @@ __global__ __launch_bounds__(256) void q4_write_turned_kernel(WriteArgs a) {
     }
 }
 
-// Rows that need no turning, in fp32: a workgroup per 16 tokens and one of the 2*Hkv rows of each.  Rows that all sequences are given
-// (a system prompt) are quantised once.
+// Rows that need no turning, in fp32: a workgroup per 16 tokens and one of the 2*Hkv rows of each.  Rows that all sequences are given (a system
+// prompt) are quantised once.  The rows meet in LDS and are stored 16 bytes at a time, 1280 bytes on end: word by word, as the lanes have them, 2048 rows of 32
+// heads for eight sequences took 42 us, of which the stores' partial lines were most.
 template <typename T>
 __global__ __launch_bounds__(256) void q4_write_kernel(WriteArgs a) {
+    __shared__ uint4 rows[16 * kQ4Row / 16];
     const int tiles = (a.qL + 15) / 16, plane_row = blockIdx.x % (2 * a.Hkv), rest = blockIdx.x / (2 * a.Hkv), tile = rest % tiles, b0 = rest / tiles;
     const bool is_k = plane_row < a.Hkv;
-    const int hk = is_k ? plane_row : plane_row - a.Hkv, l = tile * 16 + (threadIdx.x >> 4), j = threadIdx.x & 15;
-    const int b_end = a.shared ? a.B : b0 + 1, lane = threadIdx.x & 63;
-    // (all sixteen lanes of a row behind the last)
-    const T* src = is_k ? (const T*)a.k + b0 * a.ksb + min(l, a.qL - 1) * a.ksl + hk * a.ksh : (const T*)a.v + b0 * a.vsb + min(l, a.qL - 1) * a.vsl + hk * a.vsh;
+    const int hk = is_k ? plane_row : plane_row - a.Hkv, row = threadIdx.x >> 4, j = threadIdx.x & 15, from = min(tile * 16 + row, a.qL - 1);
+    const T* src = is_k ? (const T*)a.k + b0 * a.ksb + from * a.ksl + hk * a.ksh : (const T*)a.v + b0 * a.vsb + from * a.vsl + hk * a.vsh;
     float x[8];
     load8(src + 8 * j, x);
-    int lens = 0, ns = 0;  // of 64 sequences, one to a lane
-    if (b0 + lane < b_end) own_extent(a.lengths, a.q_lens, b0 + lane, a.qL, a.maxlen, lens, ns);
-    const uint2 q = quantise8(x);
-    for (int b = b0; b < b_end; b++) {
-        if (b > b0 && (b & 63) == 0 && b + lane < b_end) own_extent(a.lengths, a.q_lens, b + lane, a.qL, a.maxlen, lens, ns);
-        const int len = __builtin_amdgcn_readlane(lens, (b - b0) & 63), n = __builtin_amdgcn_readlane(ns, (b - b0) & 63);
-        if (l < n) store_q4((is_k ? a.ck : a.cv) + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + l) * kQ4Row, q, j);
+    store_q4(reinterpret_cast<uint8_t*>(rows) + row * kQ4Row, quantise8(x), j);
+    __syncthreads();
+    // (three sequences at a time, 80 lanes to each)
+    const int piece = threadIdx.x % 80, l = tile * 16 + piece / 5, b_end = a.shared ? a.B : b0 + 1;
+    if (threadIdx.x >= 240) return;
+    const uint4 mine = rows[piece];
+    uint8_t* plane = is_k ? a.ck : a.cv;
+#pragma unroll 4
+    for (int b = b0 + (int)threadIdx.x / 80; b < b_end; b += 3) {
+        int len, n;
+        own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
+        if (l < n) *reinterpret_cast<uint4*>(plane + (((int64_t)b * a.Hkv + hk) * a.maxlen + len + tile * 16) * kQ4Row + 16 * piece) = mine;
     }
 }
 

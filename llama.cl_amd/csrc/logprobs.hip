@@ -50,6 +50,7 @@ __device__ __forceinline__ int is_ahead(Held a, Held b) { return a.key > b.key |
 // how many of `held` (n, and up to three that are nothing behind them) are before one of them
 __device__ __forceinline__ int how_many_ahead(const Held* held, int n, Held one) {
     int before = 0;
+#pragma unroll 4
     for (int t = 0; t < n; t += 4) {
         const uint4 x = *reinterpret_cast<const uint4*>(held + t), y = *reinterpret_cast<const uint4*>(held + t + 2);
         before += is_ahead({x.x, (int)x.y}, one) + is_ahead({x.z, (int)x.w}, one) + is_ahead({y.x, (int)y.y}, one) + is_ahead({y.z, (int)y.w}, one);
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
         const uint32_t key = rank_key(own);
         uint32_t bound = 0;
 #pragma unroll 1
-        for (int bit = 31; bit >= 0; bit--) {
+        for (int bit = 31; bit >= 12; bit--) {  // (a bound need not be the nearest: the lower bits leave a few more and take as long as the others)
             const uint32_t more = bound | 1u << bit;
             if ((int)__builtin_popcountll(__ballot(key >= more)) >= a.top) bound = more;
         }
@@ -127,14 +128,22 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
     auto at = [&](int e) { return base + 1024 * (e >> 2) + (e & 3); };
     if (a.top > 0) {
         const uint32_t bound = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
-        if (rank_key(own) >= bound) {
+        // (one arrival for a wave, its lanes in order)
+        const float least = bound <= 0x007fffffu ? -INFINITY : of_key(bound);  // (keys up to that of minus infinity)
+        int its = 0;
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const uint32_t key = rank_key(x[e]);
-                if (key >= bound) {
-                    const int slot = atomicAdd(&count, 1);
-                    if (slot < kHeld) held[slot] = {key, at(e)};
-                }
+        for (int e = 0; e < E; e++) its += (int)__builtin_popcountll(__ballot(something(x[e]) >= least));
+        int to = 0;
+        if (lane == 0 && its > 0) to = atomicAdd(&count, its);
+        to = __builtin_amdgcn_readfirstlane(to);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const bool taken = something(x[e]) >= least;
+            const uint64_t all = __ballot(taken);
+            if (all != 0) {
+                const int slot = to + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+                if (taken && slot < kHeld) held[slot] = {rank_key(x[e]), at(e)};
+                to += (int)__builtin_popcountll(all);
             }
         }
     }
@@ -224,24 +233,25 @@ __global__ __launch_bounds__(256) void logprob_rows_kernel(LogprobArgs a) {
     const int64_t n = (int64_t)a.runs * a.top;
     const Held* from = a.best + (int64_t)row * n;
     int kept = 0;
+    const bool sums_wave = threadIdx.x >= 192;
     for (int64_t c0 = 0; c0 < n; c0 += 512) {
         const int more = (int)min((int64_t)512, n - c0), m = more + kept;
         for (int c = threadIdx.x; c < more + 4; c += 256) held[kept + c] = c < more ? from[c0 + c] : nothing_held();
         if ((int)threadIdx.x < kept) held[threadIdx.x] = best[threadIdx.x];
         __syncthreads();
-        for (int c = threadIdx.x; c < m; c += 256) {
-            const int before = how_many_ahead(held, m, held[c]);
-            if (before < a.top) best[before] = held[c];
+        if (!sums_wave) {
+            for (int c = threadIdx.x; c < m; c += 192) {
+                const int before = how_many_ahead(held, m, held[c]);
+                if (before < a.top) best[before] = held[c];
+            }
+        } else if (c0 == 0) {  // (beside the others' comparisons)
+            RowSums s;
+            row_answers(a, row, threadIdx.x & 63, s);
+            if (threadIdx.x == 192) sums = s;
         }
         kept = min(m, a.top);
         __syncthreads();
     }
-    if (threadIdx.x < 64) {
-        RowSums s;
-        row_answers(a, row, threadIdx.x, s);
-        if (threadIdx.x == 0) sums = s;
-    }
-    __syncthreads();
     if ((int)threadIdx.x < a.top) {
         a.top_tokens[(int64_t)row * a.top + threadIdx.x] = best[threadIdx.x].at;
         a.top_logprobs[(int64_t)row * a.top + threadIdx.x] = logprob_of(sums, of_key(best[threadIdx.x].key));

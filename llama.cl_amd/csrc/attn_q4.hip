@@ -32,8 +32,9 @@ struct Q4Args {
     float* out;                         // [B][qL][H*128]
     int64_t maxlen;
     int B, qL, G, Hkv, M, Mq, half;     // Mq = qL*G
-    int tile, tiles, groups, join;      // queries of a tile, tiles of a sequence's queries for a kv head; workgroups; queries that one joins
-    int rows16;
+    int tile, tiles, groups, turns;     // queries of a tile, tiles of a sequence's queries for a kv head; workgroups, to a compute unit
+    int join;                           // queries that a workgroup joins
+    int row_groups;                     // workgroups to a token that rotate its rows
 };
 // query `in` of a sequence for kv head hk: token in / G, head hk*G + in % G
 __device__ __forceinline__ const float* query_at(const Q4Args& a, int b, int hk, int in) {
@@ -69,7 +70,7 @@ __device__ __forceinline__ const float* new_row_at(const Q4Args& a, bool is_k, i
 // A workgroup per token and 16 of its H + 2*Hkv rows of 128, sixteen lanes to a row
 __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a) {
     __shared__ double2 turn[64];
-    const int bl = blockIdx.x / a.rows16, group = blockIdx.x - bl * a.rows16, b = bl / a.qL, l = bl - b * a.qL;
+    const int bl = blockIdx.x / a.row_groups, group = blockIdx.x - bl * a.row_groups, b = bl / a.qL, l = bl - b * a.qL;
     const int H = a.G * a.Hkv, row = group * 16 + (threadIdx.x >> 4), j = threadIdx.x & 15;
     const bool is_q = row < H, is_k = !is_q && row < H + a.Hkv, none = row >= H + 2 * a.Hkv;
     const int hk = is_k ? row - H : row - H - a.Hkv;
@@ -79,16 +80,16 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a) {
     if (!none) p.load(src, j);
     int len, n;
     own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-    const bool live = l < n;
-    if (live && (int)threadIdx.x < a.half) turn[threadIdx.x] = turn64(a.inv_freq[threadIdx.x], len + l);
+    if (l >= n) return;
+    if ((int)threadIdx.x < a.half) turn[threadIdx.x] = turn64(a.inv_freq[threadIdx.x], len + l);
     __syncthreads();
     if (is_q) {
         const int64_t m = (int64_t)(row / a.G) * a.M + (int64_t)bl * a.G + row % a.G;
-        const QueryRow r = turned_query(p, src, j, turn, a.half, live);
+        const QueryRow r = turned_query(p, src, j, turn, a.half, true);
         *reinterpret_cast<uint4*>(a.qh + m * kS + 8 * j) = r.hi;
         *reinterpret_cast<uint4*>(a.ql + m * kS + 8 * j) = r.lo;
         if (j == 0) a.cq[m] = r.c;
-    } else if (live && !none) {
+    } else if (!none) {
         write_row(a, p, src, is_k, b, hk, len + l, j, turn);
     }
 }
@@ -156,14 +157,14 @@ struct Q4FewIn {
     double2 turn[16 * RT][64];  // of the sequence's tokens
 };
 template <int RT>
-__device__ __forceinline__ void q4_take(const Q4Args& a, Q4FewIn<RT>& sm, float* factors, int b, int hk, int lane) {
+__device__ __forceinline__ void q4_take(const Q4Args& a, Q4FewIn<RT>& sm, float* factors, int b, int hk, int n, int lane) {
     const int wave = threadIdx.x >> 6;  // a step to a wave
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int64_t m = (int64_t)hk * a.M + (int64_t)b * a.Mq + min(16 * rt + (lane & 15), a.Mq - 1), at = m * kS + 32 * (lane >> 4) + 8 * wave;
         sm.q[(rt * 8 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.qh + at);
         sm.q[(rt * 8 + 4 + wave) * 64 + lane] = *reinterpret_cast<const uint4*>(a.ql + at);
-        if (wave == 0 && lane < 16) factors[16 * rt + lane] = a.cq[m];
+        if (wave == 0 && lane < 16) factors[16 * rt + lane] = min(16 * rt + lane, a.Mq - 1) / a.G < n ? a.cq[m] : 0.0f;  // (padding's queries hold anything)
     }
     __syncthreads();
 }
@@ -227,10 +228,22 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
     }
     return v;
 }
-// Every wave for itself: all units, the share of a workgroup, and the sequence that has the first unit of this one's (-1: none is left), with the units
-// before that sequence
+// Units first .. last-1 of a workgroup's, out of `all`.  Where the chip is full, a.turns workgroups to a compute unit, those that come first have the
+// waves that are served first when several wait: with equal shares they were done in half the time of those that come last.  So shares fall from 1.25
+// to 0.75 of the mean (32 sequences of up to 4096 rows 86.2 us with equal shares, 86.3 / 84.2 / 87.4 with 0.15 / 0.25 / 0.35; 64 with grouped heads 88.2, 85.3 / 83.6 /
+// 85.4; 16 of 5 tokens 39.8, 37.5 / 37.1 / 37.0; 4 turns 86.4, 86.3 / 83.8 / 85.6).
+constexpr int kSlope = 25;  // hundredths
+__device__ __forceinline__ int64_t share_at(const Q4Args& a, int w, int64_t all) {
+    // (few units: one to a workgroup, or as many to each, until there are none.  None may be left out between two that have rows of a tile)
+    if (a.turns == 1 || all < 4 * (int64_t)a.groups) return min(all, (all + a.groups - 1) / a.groups * w);
+    const int each = a.groups / a.turns, turn = w / each, in = w - turn * each;
+    // shares of turn 0, 1, ..: 100 + kSlope * (1 - 2 turn / (turns - 1)), in all 100 * turns
+    const int64_t steps = a.turns - 1, before = turn * (100 + kSlope) * steps - kSlope * (int64_t)turn * (turn - 1), its = (100 + kSlope) * steps - 2 * kSlope * turn;
+    return all * (before * each + its * in) / (100 * steps * a.groups);
+}
+// Every wave for itself: a workgroup's units, and the sequence that has the first of them (-1: it has none), with the units before that sequence
 struct UnitPlace {
-    int all, share, b, before;
+    int first, last, b, before;
 };
 __device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane) {
     int all = 0, its = 0, upto = 0;
@@ -240,9 +253,8 @@ __device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane) {
         upto = all + wave_scan(its, lane);
         all = __builtin_amdgcn_readlane(upto, 63);
     }
-    UnitPlace p{all, (all + a.groups - 1) / a.groups, -1, 0};
-    const int64_t want = (int64_t)blockIdx.x * p.share;
-    if (want >= all) return p;
+    UnitPlace p{(int)share_at(a, blockIdx.x, all), (int)share_at(a, blockIdx.x + 1, all), -1, 0};
+    if (p.first >= p.last) return p;
     int before = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -250,7 +262,7 @@ __device__ __forceinline__ UnitPlace place_of(const Q4Args& a, int lane) {
             its = b0 + lane < a.B ? units_of(a, b0 + lane).head * a.Hkv : 0;
             upto = before + wave_scan(its, lane);
         }
-        const uint64_t hit = __ballot(upto > want);
+        const uint64_t hit = __ballot(upto > p.first);
         if (hit != 0) {
             const int at = __builtin_ctzll(hit);
             p.b = b0 + at;
@@ -286,7 +298,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
     __shared__ Q4MeetSmem<RT> sm;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Codes codes;
-    int b, before, first, last, share = 1;
+    int b, before, first, last;
     if constexpr (WHOLE) {  // a kv head of a sequence to a workgroup
         b = blockIdx.x / a.Hkv, before = 0;
         const int units = units_of(a, b).head;
@@ -294,8 +306,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
     } else {
         const UnitPlace start = place_of(a, threadIdx.x & 63);
         if (start.b < 0) return;
-        b = start.b, before = start.before, share = start.share;
-        first = (int)blockIdx.x * share, last = min(start.all, first + share);
+        b = start.b, before = start.before, first = start.first, last = start.last;
     }
     RowPair q_rows[WHOLE ? RT : 1], new_row;
     if constexpr (WHOLE) {  // (asked for with the length)
@@ -315,8 +326,11 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
         int tile, units, u0;  // (one tile)
         tile_of(its, at - before - hk * its.head, tile, units, u0);
         const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
-        if (!WHOLE && u0 == 0 && threadIdx.x == 0)
-            a.parts[((int64_t)b * a.Hkv + hk) * a.tiles + tile] = make_int2(blockIdx.x, blockIdx.x + (at + real - 1 - (int)blockIdx.x * share) / share);
+        if (!WHOLE && (u0 == 0 || u1 >= real) && threadIdx.x == 0) {
+            int2* parts = a.parts + ((int64_t)b * a.Hkv + hk) * a.tiles + tile;
+            if (u0 == 0) parts->x = blockIdx.x;
+            if (u0 < real && u1 >= real) parts->y = blockIdx.x;
+        }
         at += u1 - u0;
         if (u0 >= real) continue;
         const int lane = (int)unseen(threadIdx.x & 63), i = lane & 15, g = lane >> 4;
@@ -334,7 +348,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
             q4_begin<RT>(a, sm.in, sm.factors, b, hk, len, n, q_rows, new_row);
             if (j0 < j1 && !old) x.load_k(q4_rows(K, 32 * j0, rows), i, g), x.load_v(q4_rows(V, 32 * j0, rows), i, g);
         }
-        if constexpr (!WHOLE) q4_take<RT>(a, sm.in, sm.factors, b, hk, lane);
+        if constexpr (!WHOLE) q4_take<RT>(a, sm.in, sm.factors, b, hk, n, lane);
         Queries<RT> s;
         bool live[RT];
         int see_min = INT_MAX;
@@ -369,7 +383,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (j + 4 < j1) x.load_k(q4_rows(K, t + 128, rows), i, g);
+            x.load_k(q4_rows(K, t + 128, rows), i, g);  // (behind the last rows too, where nothing is read: with a branch around them all loads would be waited for)
             uint32_t hidden = 0;
             if (masked) x.hide_nan(hidden);
             Weights w[RT];
@@ -396,7 +410,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (j + 4 < j1) x.load_v(q4_rows(V, t + 128, rows), i, g);
+            x.load_v(q4_rows(V, t + 128, rows), i, g);
         }
         // the four waves' sums
 #pragma unroll
@@ -513,7 +527,7 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
     const Codes codes;
     const UnitPlace start = place_of(a, lane);
     if (start.b < 0) return;
-    const int share = start.share, first = (int)blockIdx.x * share, last = min(start.all, first + share);
+    const int first = start.first, last = start.last;
     int b = start.b, before = start.before;
     UnitsOf its = units_of(a, b);
 #pragma unroll 1
@@ -526,8 +540,11 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
         int tile, units, u0;
         tile_of(its, at - before - hk * its.head, tile, units, u0);
         const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
-        if (u0 == 0 && threadIdx.x == 0)
-            a.parts[((int64_t)b * a.Hkv + hk) * a.tiles + tile] = make_int2(blockIdx.x, blockIdx.x + (at + real - 1 - (int)blockIdx.x * share) / share);
+        if ((u0 == 0 || u1 >= real) && threadIdx.x == 0) {
+            int2* parts = a.parts + ((int64_t)b * a.Hkv + hk) * a.tiles + tile;
+            if (u0 == 0) parts->x = blockIdx.x;
+            if (u0 < real && u1 >= real) parts->y = blockIdx.x;
+        }
         at += u1 - u0;
         if (u0 >= real) continue;
         int len, n;
@@ -555,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
                 qh[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + from + 8 * step));
                 ql[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + from + 8 * step));
             }
-            s.c[rt] = a.cq[m], s.m[rt] = -INFINITY, s.l[rt] = 0.0f;
+            s.c[rt] = live[rt] ? a.cq[m] : 0.0f, s.m[rt] = -INFINITY, s.l[rt] = 0.0f;
 #pragma unroll
             for (int c = 0; c < 8; c++) s.o[rt][c] = v4f{0.f, 0.f, 0.f, 0.f};
             s.see[rt] = live[rt] ? len + l + 1 : INT_MAX;  // (what padding sees is thrown away)
@@ -710,7 +727,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
 
 struct Q4Plan {
     bool many;
-    int rt, tile, tiles, groups, join;
+    int rt, tile, tiles, groups, turns, join;
 };
 static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t maxlen) {
     Q4Plan p{};
@@ -726,6 +743,7 @@ static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t max
     }
     const int64_t most = items * ((maxlen + kUnit - 1) / kUnit + kStart), held = p.many || p.rt == 2 ? 512 : 1024;  // (workgroups that the chip holds)
     p.groups = (int)(most < held ? most : held);
+    p.turns = most < held ? 1 : (int)(held / 256);
     const int64_t queries = B * Hkv * Mq;  // (workgroups enough to fill the chip, then queries to each)
     p.join = queries >= 8192 ? 8 : queries >= 4096 ? 4 : queries >= 2048 ? 2 : 1;
     return p;
@@ -753,7 +771,8 @@ static Q4Layout layout_q4(const Q4Plan& plan, int64_t rows, int64_t items) {
 }
 
 static int q4_launch(const Q4Args& a, const Q4Plan& plan, hipStream_t st) {
-    if (plan.join > 0) q4_prep_kernel<<<(unsigned)((int64_t)a.B * a.qL * a.rows16), 256, 0, st>>>(a);
+    const unsigned prep = (unsigned)((int64_t)a.B * a.qL * a.row_groups);
+    if (plan.join > 0) q4_prep_kernel<<<prep, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
     const unsigned groups = (unsigned)plan.groups;
     if (plan.many) q4_many_kernel<1><<<groups, 256, 0, st>>>(a);
@@ -799,8 +818,8 @@ extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int6
     LLMOPS_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(kv_cache, 16) && aligned(workspace, 256));
     LLMOPS_REQUIRE(aligned(inv_freq, 4) && aligned(lengths, 4) && aligned(q_lens, 4));
     LLMOPS_REQUIRE(q_stride_b % 4 == 0 && q_stride_l % 4 == 0 && k_stride_b % 4 == 0 && k_stride_l % 4 == 0 && v_stride_b % 4 == 0 && v_stride_l % 4 == 0);
-    const int64_t G = H / Hkv, rows16 = (H + 2 * Hkv + 15) / 16;
-    LLMOPS_REQUIRE((Wide)B * qL * rows16 < ((Wide)1 << 24));
+    const int64_t G = H / Hkv;
+    LLMOPS_REQUIRE((Wide)B * qL * ((H + 2 * Hkv + 15) / 16) < ((Wide)1 << 24));
     const Wide heads = (Wide)H * kS * 4, kv_heads = (Wide)Hkv * kS * 4, plane = (Wide)B * Hkv * maxlen * kQ4Row;
     LLMOPS_REQUIRE((Wide)planes * plane < ((Wide)1 << 62));
     const Q4Plan plan = plan_q4(B, qL, H, Hkv, maxlen);
@@ -814,8 +833,8 @@ extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int6
     a.rec_out = reinterpret_cast<float*>(ws + w.rec), a.rec_stat = reinterpret_cast<float2*>(ws + w.stat), a.parts = reinterpret_cast<int2*>(ws + w.parts);
     a.ck = reinterpret_cast<uint8_t*>(kv_cache) + 2 * layer_id * (int64_t)plane, a.cv = a.ck + (int64_t)plane;
     a.lengths = lengths, a.q_lens = q_lens, a.out = out, a.maxlen = maxlen;
-    a.B = (int)B, a.qL = (int)qL, a.G = (int)G, a.Hkv = (int)Hkv, a.Mq = (int)(qL * G), a.M = (int)(B * qL * G), a.half = (int)half, a.rows16 = (int)rows16;
-    a.tile = plan.tile, a.tiles = plan.tiles, a.groups = plan.groups, a.join = plan.join;
+    a.B = (int)B, a.qL = (int)qL, a.G = (int)G, a.Hkv = (int)Hkv, a.Mq = (int)(qL * G), a.M = (int)(B * qL * G), a.half = (int)half, a.row_groups = (int)((H + 2 * Hkv + 15) / 16);
+    a.tile = plan.tile, a.tiles = plan.tiles, a.groups = plan.groups, a.turns = plan.turns, a.join = plan.join;
     // (a workgroup reads its q, k and v while others may have written their rows and results)
     const Extent q_at(q, B, (Wide)q_stride_b * 4, qL, (Wide)q_stride_l * 4, heads), k_at(k, B, (Wide)k_stride_b * 4, qL, (Wide)k_stride_l * 4, kv_heads),
         v_at(v, B, (Wide)v_stride_b * 4, qL, (Wide)v_stride_l * 4, kv_heads), out_at(out, (Wide)B * qL * heads), written(a.ck, 2 * plane);

@@ -49,9 +49,9 @@ __device__ __forceinline__ void write_row(const Q4Args& a, const RowPair& p, con
     if (is_k) {
         double x[8];
         turn_row(p, src, j, turn, a.half, x);
-        store_q4(dst, quantise8(x), j);
+        store_q4(dst, quantise8<true>(x), j);
     } else {
-        store_q4(dst, quantise8(p.x), j);
+        store_q4(dst, quantise8<true>(p.x), j);
     }
 }
 // .. of a query: turned in fp32

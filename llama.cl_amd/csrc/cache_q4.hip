@@ -35,11 +35,11 @@ __global__ __launch_bounds__(256) void q4_write_turned_kernel(WriteArgs a) {
         p.load(src, j);
         double x[8];
         turn_row(p, src, j, turn, a.half, x);
-        store_q4(dst, quantise8(x), j);
+        store_q4(dst, quantise8<true>(x), j);
     } else {
         float x[8];
         load8(src + 8 * j, x);
-        store_q4(dst, quantise8(x), j);
+        store_q4(dst, quantise8<sizeof(T) == 4>(x), j);
     }
 }
 
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void q4_write_kernel(WriteArgs a) {
     const T* src = is_k ? (const T*)a.k + b0 * a.ksb + from * a.ksl + hk * a.ksh : (const T*)a.v + b0 * a.vsb + from * a.vsl + hk * a.vsh;
     float x[8];
     load8(src + 8 * j, x);
-    store_q4(reinterpret_cast<uint8_t*>(rows) + row * kQ4Row, quantise8(x), j);
+    store_q4(reinterpret_cast<uint8_t*>(rows) + row * kQ4Row, quantise8<sizeof(T) == 4>(x), j);
     __syncthreads();
     // (three sequences at a time, 80 lanes to each)
     const int piece = threadIdx.x % 80, l = tile * 16 + piece / 5, b_end = a.shared ? a.B : b0 + 1;

@@ -47,7 +47,8 @@ __device__ __forceinline__ double scaled(double x, int e) { return ldexp(x, e); 
 
 // Sixteen lanes to a row, eight values to a lane (dims 8 * (lane % 16) ..), R float or double: the lane's word of codes, and d | m << 16 of its
 // group (the same in its four lanes)
-template <typename R>
+// GUESS: not for values that are halves, or whole numbers of any other unit, which lie on borders all the time
+template <bool GUESS, typename R>
 __device__ __forceinline__ uint2 quantise8(const R (&x)[8]) {
     R top = x[0], low = x[0];
     bool fine = true;
@@ -69,20 +70,18 @@ __device__ __forceinline__ uint2 quantise8(const R (&x)[8]) {
     const int step = ((int)(hi - lo) + 14) / 15;  // (lo is no -0: zeros of either sign are stored alike)
     const float s = (float)step, half = 0.5f * s, inv = step > 0 ? 1.0f / s : 0.0f;
     uint32_t word = 0;
-    bool near = sizeof(R) == 4;
-    if constexpr (sizeof(R) == 8) {
-        // in fp32, which is off by less than 2^-12 here, unless a value is nearer than 2^-11 to a border (in one of some thousand rows)
+    bool near = true;
+    if constexpr (GUESS) {
+        // in fp32, which is off by less than 2^-12 of a unit here, unless a value is nearer than 2^-11 to a border (in one of some hundred rows)
         const float scale = ldexpf(1.0f, 11 - e);
-        float nearest = 1.0f;
+        float farthest = -1.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float t = (float)x[i] * scale, c = fminf(fmaxf(rintf((t - lo) * inv), 0.0f), 15.0f), off = t - fmaf(c, s, lo);
-            nearest = fminf(nearest, fabsf(fabsf(off) - half));
-            const int code = min(max((int)c + (off > half ? 1 : 0) - (off < -half ? 1 : 0), 0), 15);
-            word |= (uint32_t)code << (4 * (i >> 1) + 16 * (i & 1));
+            const float t = (float)x[i] * scale, c = rintf(fminf(fmaxf((t - lo) * inv, 0.0f), 15.0f));
+            farthest = fmaxf(farthest, fabsf(t - fmaf(c, s, lo)));
+            word |= (uint32_t)c << (4 * (i >> 1) + 16 * (i & 1));
         }
-        near = nearest < 0x1p-11f;
-        if (step == 0) near = false, word = 0;
+        near = farthest > half - 0x1p-11f && step > 0;
     }
     if (__any(near)) {
         word = 0;

@@ -25,7 +25,7 @@ __all__ = [
     "attention_rope", "attention_rope2", "attention_rope2_records", "attention_records_supported", "AttentionRecords", "rope_embed", "softmax", "rmsnorm", "iadd", "imul", "itrans", "clone",
     "rmsnorm_out", "silu_mul", "empty", "ones", "embedding", "embedding_q8c_quant_w", "embedding_q8c", "tensor_pool", "set_default_group_k", "reserve_workspace", "reset_workspaces",
     "group_k_of", "attention_rope_prefix", "lora_add", "verify_drafts",
-    "cache_write_q4", "cache_read_q4", "attention_rope_q4", "token_logprobs",
+    "cache_write_q4", "cache_read_q4", "attention_rope_q4", "token_logprobs", "Q4_ROW_BYTES",
 ]
 
 # Callers of the reference read ``tensor.item_size`` (chatllama/main.py:171-173, ops/perf_ops.py:242; bound at
@@ -677,12 +677,12 @@ def verify_drafts(logits, drafts, uniforms, draft_probs=None, temperature=None, 
     return tokens, accepted
 
 
-_Q4_ROW = 80  # bytes of a row of 128 values
+Q4_ROW_BYTES = 80  # a row of 128 values
 
 
 def _q4_cache(t):
     _require(isinstance(t, torch.Tensor) and t.is_cuda, "kv_cache is on the HIP device (llmops has no CPU path)")
-    _require(t.dtype == torch.int8 and t.dim() == 5 and t.shape[4] == _Q4_ROW and t.is_contiguous(), "kv_cache.is<int8_t>({planes, B, Hkv, maxlen, 80})")
+    _require(t.dtype == torch.int8 and t.dim() == 5 and t.shape[4] == Q4_ROW_BYTES and t.is_contiguous(), "kv_cache.is<int8_t>({planes, B, Hkv, maxlen, 80})")
     return t.shape[:4]
 
 

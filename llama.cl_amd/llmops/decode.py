@@ -14,13 +14,14 @@ A decode step (one token, batch 1) has fixed shapes and no host-side decisions, 
 captured once as a HIP graph and replayed (``capture_decode``).
 
 Several requests in step (``forward_requests``, ``step_requests``; no counterpart in the reference): sequences that share a prefix and
-differ in length, with low-rank adapters of their own, each bringing drafted tokens that the step checks.
+differ in length, with low-rank adapters of their own, each bringing drafted tokens that the step checks; their caches in full width or in 4
+bits, and what texts are worth to the model (``score_requests``).
 """
 import numpy as np
 import torch
 
 import llmops
-from llmops.opset import KVCache, LoraAdapters, PrefixCache, llmop_embedding_q8c, llmop_fc_q4a, llmop_rmsnorm
+from llmops.opset import KVCache, LoraAdapters, PrefixCache, Q4Cache, llmop_embedding_q8c, llmop_fc_q4a, llmop_rmsnorm
 
 LLAMA_7B = dict(layer_num=32, head_num=32, head_size=128, hidden_size=4096, intermediate_size=11008,
                 vocab_size=55296, rms_norm_eps=1e-5, rope_base=10000.0)
@@ -248,8 +249,17 @@ class LlamaDecoder:
         self.forward(input_ids, kv.cache, kv.slots, kv.position_id)
         return kv.cache
 
-    def request_cache(self, batch_size, max_kv_len, prefix=None, dtype=None):
-        """A ``PrefixCache`` for this model behind a prefix that ``read_prefix`` has made (all of its rows)."""
+    def request_cache(self, batch_size, max_kv_len, prefix=None, dtype=None, bits=None):
+        """A ``PrefixCache`` for this model behind a prefix that ``read_prefix`` has made (all of its rows).  ``bits=4``: a ``Q4Cache``, in which every
+        sequence begins with the prefix and has ``max_kv_len`` rows behind it."""
+        if bits is not None:
+            if bits != 4 or dtype is not None:
+                raise ValueError("a cache in 4 bits, or one of a dtype")
+            rows = 0 if prefix is None else prefix.shape[3]
+            cache = Q4Cache(self.configs, batch_size, rows + max_kv_len, self.device)
+            if rows:
+                cache.begin(prefix)
+            return cache
         return PrefixCache(self.configs, batch_size, max_kv_len, prefix, 0 if prefix is None else prefix.shape[3], self.device, dtype)
 
     def set_adapters(self, layers, dtype=torch.float16):
@@ -306,7 +316,7 @@ class LlamaDecoder:
 
         hidden = hidden_states
         (q, k, v), _ = project(("q_proj", "k_proj", "v_proj"), ops["input_layernorm"], "qkv_proj", H)
-        attn = llmops.attention_rope_prefix(q, k, v, self.inv_freq, cache.prefix, cache.prefix_len, cache.cache, cache.lengths, i, q_lens=q_lens)
+        attn = cache.attend(q, k, v, self.inv_freq, i, q_lens=q_lens)
         hidden = llmops.fc_Q4A(attn, ops["o_proj"].weight, H, residual=hidden_states)
         add("o_proj", hidden, attn)
         norm = ops["post_attention_layernorm"]
@@ -326,12 +336,23 @@ class LlamaDecoder:
         add("down_proj", out, act)
         return out
 
-    def step_requests(self, tokens, cache, uniforms, drafts=None, draft_probs=None, draft_lens=None, temperature=None, adapters=None):
+    def score_requests(self, input_ids, cache, q_lens=None, adapters=None, top=0):
+        """What texts are worth to the model: ``forward_requests`` for the same arguments, then ``llmops.token_logprobs`` of each token behind the
+        first against the logits of the one before it.  Returns its (logprobs [B, qL-1], entropy [B, qL-1], top_tokens, top_logprobs [B, qL-1,
+        top]); tokens behind a text's end (``q_lens``) have log probability 0.  exp(-sum / count) of the log probabilities is the perplexity."""
+        logits = self.forward_requests(input_ids, cache, q_lens, adapters)
+        behind = input_ids[:, 1:]
+        if q_lens is not None:
+            behind = behind.masked_fill(torch.arange(1, input_ids.shape[1], device=behind.device) >= q_lens[:, None], -1)
+        return llmops.token_logprobs(logits[:, :-1], behind, top)
+
+    def step_requests(self, tokens, cache, uniforms, drafts=None, draft_probs=None, draft_lens=None, temperature=None, adapters=None, top=None):
         """One step of several requests: each sequence's last token (``tokens`` int64 [B], not yet in the cache) and its K drafted ones
         (``drafts`` int64 [B, K]; None: none) go through the model, the drafts are checked and the token behind those accepted is drawn
         (``llmops.verify_drafts`` for the other arguments), and the rows of what was accepted are kept in the cache.  Drafts that no longer
         fit the cache are not checked; a sequence without a row left for its token answers -1.  Returns its (tokens
-        [B, K+1], accepted [B]): ``tokens`` of the next step is ``result.gather(1, accepted[:, None].long())[:, 0]``."""
+        [B, K+1], accepted [B]): ``tokens`` of the next step is ``result.gather(1, accepted[:, None].long())[:, 0]``.  With ``top`` also
+        ``llmops.token_logprobs`` of these tokens (of the model's distributions, whatever the temperature)."""
         B = tokens.shape[0]
         if drafts is None:
             drafts = torch.empty((B, 0), dtype=torch.int64, device=tokens.device)
@@ -344,7 +365,7 @@ class LlamaDecoder:
         result, accepted = llmops.verify_drafts(logits, drafts, uniforms, draft_probs=draft_probs, temperature=temperature, draft_lens=q_lens - 1)
         result.masked_fill_((room <= 0)[:, None], -1)
         cache.keep(accepted + 1)
-        return result, accepted
+        return (result, accepted) if top is None else (result, accepted, llmops.token_logprobs(logits, result, top))
 
     def capture_decode(self, kv_cache, slot, position_id, stream=None):
         """Capture one decode step (batch 1, one token) as a HIP graph that serves every position: the token id,

@@ -160,6 +160,51 @@ class PrefixCache:
             raise ValueError("length outside the cache")
         self.lengths[sequence] = length
 
+    def attend(self, q, k, v, inv_freq, layer_id, q_lens=None):
+        return llmops.attention_rope_prefix(q, k, v, inv_freq, self.prefix, self.prefix_len, self.cache, self.lengths, layer_id, q_lens=q_lens)
+
+
+class Q4Cache(PrefixCache):
+    """KV cache of a batch in 4 bits (``llmops.attention_rope_q4``): 80 bytes for a token and head where fp32 takes 512 and fp16 256, on the device
+    int8 [2*layers, batch, heads, max_kv_len, 80].  Each sequence has rows of its own from the first on; ``begin`` gives all of them
+    the same first rows, of a cache in full width (a system prompt that was read once), which ``forget`` keeps."""
+
+    def __init__(self, configs, batch_size, max_kv_len, device="cuda"):
+        if configs["head_size"] != 128:
+            raise ValueError("a cache in 4 bits holds heads of 128")
+        self.prefix, self.prefix_len, self.begun = None, 0, 0
+        self.cache = torch.zeros(configs["layer_num"] * 2, batch_size, configs["head_num"], max_kv_len, llmops.Q4_ROW_BYTES, dtype=torch.int8, device=device)
+        self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        self.max_kv_len = max_kv_len
+
+    def begin(self, full, rows=None):
+        """The first ``rows`` rows (None: all) of a cache in full width, [2*layers, 1, heads, rows, 128] in fp32 or fp16 with k rotated
+        (``LlamaDecoder.read_prefix``), become every sequence's beginning; what sequences had is forgotten."""
+        rows = full.shape[3] if rows is None else int(rows)
+        planes, batch = self.cache.shape[:2]
+        if full.dim() != 5 or full.shape[:3] != (planes, 1, self.cache.shape[2]) or full.shape[4] != 128 or not 0 <= rows <= min(full.shape[3], self.max_kv_len):
+            raise ValueError("a cache of one sequence of the same layers and heads, and rows that both have")
+        self.lengths.zero_()
+        for i in range(planes // 2 if rows else 0):
+            k, v = (full[2 * i + j, :, :, :rows].transpose(1, 2).expand(batch, -1, -1, -1) for j in (0, 1))
+            llmops.cache_write_q4(k, v, self.cache, self.lengths, i)
+        self.begun = rows
+        self.lengths.fill_(rows)
+
+    def read(self, rows=None, starts=None, dtype=torch.float16):
+        """What rows stand for, in full width: [2*layers, batch, heads, rows, 128] (of one sequence: the form that ``PrefixCache`` and ``begin`` take)"""
+        return llmops.cache_read_q4(self.cache, self.max_kv_len if rows is None else rows, starts=starts, dtype=dtype)
+
+    def size(self):
+        return self.cache.numel()
+
+    def forget(self, sequence, length=0):
+        """a sequence ends (or goes back to its first ``length`` rows behind its beginning)"""
+        super().forget(sequence, self.begun + length)
+
+    def attend(self, q, k, v, inv_freq, layer_id, q_lens=None):
+        return llmops.attention_rope_q4(q, k, v, inv_freq, self.cache, self.lengths, layer_id, q_lens=q_lens)
+
 
 class LoraAdapters:
     """Low-rank adapters of one projection, by number: y + scale * (x A^T) B^T (``llmops.lora_add``).  ``adapters``: a list of

@@ -65,6 +65,42 @@ def test_against_the_formula(B, L, H, Hkv, maxlen):
     _check(q, k, v, cache, lengths, q_lens)
 
 
+@pytest.mark.parametrize("B,L,H,Hkv,maxlen", [(64, 1, 32, 8, 3000), (130, 1, 8, 8, 1000), (40, 3, 16, 16, 1500), (70, 40, 8, 4, 700), (9, 150, 16, 8, 1200), (33, 20, 8, 8, 2500)])
+def test_the_chip_full_of_workgroups(B, L, H, Hkv, maxlen):
+    """shares that differ, sequences past 64: against the formula in 64 bits on the device, over what the cache is read back as; tolerance as in q4_reference.py"""
+    g = torch.Generator().manual_seed(B)
+    q, k, v = (x.cuda() for x in _random(g, B, L, H, Hkv))
+    cache = torch.stack([_filled(g, 2, 1, Hkv, maxlen)[:, 0] for _ in range(4)], 1).repeat(1, -(-B // 4), 1, 1, 1)[:, :B].contiguous().cuda()
+    lengths = torch.randint(0, maxlen - L + 1, (B,), generator=g, dtype=torch.int32).cuda()
+    q_lens = torch.randint(0, L + 1, (B,), generator=g, dtype=torch.int32).cuda() if L > 1 else None
+    f, e, G = _inv_freq().cuda(), 2.0 ** -24, H // Hkv
+    written = cache.clone()
+    llmops.cache_write_q4(k, v, written, lengths, 0, inv_freq=f, q_lens=q_lens)
+    out = llmops.attention_rope_q4(q, k, v, f, cache, lengths, 0, q_lens=q_lens).reshape(B, L, H, 128)
+    assert torch.equal(cache, written)
+    full = llmops.cache_read_q4(cache, maxlen)
+    for b in range(B):
+        n, t = int(lengths[b]), L if q_lens is None else int(q_lens[b])
+        assert not out[b, t:].any()
+        if not t:
+            continue
+        K, V = (full[i, b, :, :n + t].double() for i in (0, 1))
+        angle = (n + torch.arange(t, device="cuda")).double()[:, None] * f.double()
+        lo, hi = q[b, :t].double().reshape(t, H, 128).chunk(2, dim=-1)
+        x = torch.cat((lo * angle.cos()[:, None] - hi * angle.sin()[:, None], hi * angle.cos()[:, None] + lo * angle.sin()[:, None]), -1)
+        x = x.reshape(t, Hkv, G, 128).permute(1, 0, 2, 3).reshape(Hkv, t * G, 128).contiguous()
+        s = torch.matmul(x, K.transpose(1, 2).contiguous()) / math.sqrt(128)
+        seen = (torch.arange(n + t, device="cuda") <= n + torch.arange(t, device="cuda")[:, None]).repeat_interleave(G, 0)
+        want = torch.matmul(torch.softmax(s.masked_fill(~seen, -math.inf), -1), V)
+        products = torch.matmul(x.abs(), K.abs().transpose(1, 2).contiguous()).amax(-1)
+        largest = x.abs().amax(-1) * K.abs().sum(-1).amax(-1)[:, None]
+        score = (12 * products + 4 * largest) * e / math.sqrt(128) + 3 * e * s.abs().amax(-1)
+        rows = n + t
+        tol = V.abs().amax((1, 2))[:, None] * (2 * score + (4 + 16 + 2 * (rows / 128 + 12)) * e + rows * 2.0 ** -28) + 2.0 ** -36
+        got = out[b, :t].reshape(t, Hkv, G, 128).permute(1, 0, 2, 3).reshape(Hkv, t * G, 128)
+        assert ((got - want).abs().amax(-1) <= tol).all(), b
+
+
 @pytest.mark.parametrize("L", [1, 3, 40])
 def test_empty_full_and_almost(L):
     g = torch.Generator().manual_seed(L)

@@ -1,0 +1,141 @@
+"""A cache in 4 bits through LlamaDecoder: turns, steps with drafted tokens, a beginning in common, scores.  End to end two evaluations drift by the 8-bit
+rounding of activations (test_decode_gpu.py says why): logits are compared at its 5e-2 against the same model whose attention is
+evaluated plainly over what the cache stands for; what must be the same bits is compared as such."""
+import math
+
+import pytest
+import torch
+
+import llmops
+from conftest import max_rel_err
+from llmops.decode import LlamaDecoder
+from llmops.opset import Q4Cache
+
+pytestmark = pytest.mark.gpu
+
+CFG = dict(layer_num=2, head_num=2, head_size=128, hidden_size=256, intermediate_size=512, vocab_size=320, rms_norm_eps=1e-5, rope_base=10000.0)
+
+
+def _ids(seed, *shape):
+    return torch.randint(0, CFG["vocab_size"], shape, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+class PlainCache(Q4Cache):
+    """the same cache, attention evaluated in 64 bits over what it stands for"""
+
+    def attend(self, q, k, v, inv_freq, layer_id, q_lens=None):
+        llmops.cache_write_q4(k, v, self.cache, self.lengths, layer_id, inv_freq=inv_freq, q_lens=q_lens)
+        K, V = self.read(dtype=torch.float32)[2 * layer_id:2 * layer_id + 2].double()
+        B, L, width = q.shape
+        row = self.lengths[:, None] + torch.arange(L, device="cuda")
+        angle = row[..., None].double() * inv_freq.double()
+        lo, hi = q.double().reshape(B, L, -1, 128).chunk(2, dim=-1)
+        cos, sin = angle.cos()[:, :, None], angle.sin()[:, :, None]
+        x = torch.cat((lo * cos - hi * sin, hi * cos + lo * sin), dim=-1).transpose(1, 2).contiguous()
+        s = torch.matmul(x, K.transpose(2, 3).contiguous()) / math.sqrt(128)
+        s = s.masked_fill((torch.arange(self.max_kv_len, device="cuda") > row[..., None])[:, None], -math.inf)
+        out = torch.matmul(torch.softmax(s, dim=-1), V).transpose(1, 2).reshape(B, L, width)
+        live = torch.arange(L, device="cuda") < (q_lens[:, None] if q_lens is not None else L)
+        return torch.where(live[..., None], out, 0.0).float()
+
+
+@pytest.mark.parametrize("plan", ["fused", "reference"])
+@pytest.mark.parametrize("P", [0, 21])
+def test_turns_and_tokens(plan, P):
+    model = LlamaDecoder(CFG, seed=3, plan=plan)
+    prefix = model.read_prefix(_ids(1, 1, P), torch.float16) if P else None
+    cache = model.request_cache(3, 60, prefix, bits=4)
+    assert isinstance(cache, Q4Cache) and cache.lengths.tolist() == [P] * 3 and cache.size() == 4 * 3 * 2 * (60 + P) * 80
+    plain = PlainCache(CFG, 3, 60 + P)
+    if P:
+        plain.begin(prefix)
+    n = torch.tensor([40, 2, 17], dtype=torch.int32).cuda()
+    for step in range(5):
+        ids, lens = (_ids(2, 3, 40), n) if step == 0 else (_ids(10 + step, 3, 1), None)
+        a, b = model.forward_requests(ids, cache, lens), model.forward_requests(ids, plain, lens)
+        for s in range(3):
+            t = int(n[s]) if step == 0 else 1
+            assert max_rel_err(a[s, :t].cpu().numpy(), b[s, :t].cpu().numpy()) <= 5e-2
+        plain.cache.copy_(cache.cache)  # (codes that flip would drift apart)
+        cache.keep(lens if lens is not None else 1), plain.keep(lens if lens is not None else 1)
+    assert cache.lengths.tolist() == [P + 44, P + 6, P + 21]
+
+
+def test_a_beginning_in_common():
+    model = LlamaDecoder(CFG, seed=5)
+    prefix = model.read_prefix(_ids(1, 1, 30))
+    cache = model.request_cache(3, 10, prefix, bits=4)
+    held = cache.read(30, dtype=torch.float32)
+    assert torch.equal(held[:, :1].expand(-1, 3, -1, -1, -1), held)
+    # within a step of every group of 32: a fifteenth of its range, and two units of the group's largest value's 1016th
+    off, groups = (held[:, :1] - prefix).abs().unflatten(-1, (4, 32)), prefix.unflatten(-1, (4, 32))
+    step = (groups.amax(-1) - groups.amin(-1)) / 15 + groups.abs().amax(-1) / 508
+    assert (off.amax(-1) <= step).all()
+    model.forward_requests(_ids(2, 3, 4), cache)
+    cache.keep(4)
+    cache.forget(1)
+    cache.forget(2, 3)
+    assert cache.lengths.tolist() == [34, 30, 33] and torch.equal(cache.read(30, dtype=torch.float32), held)
+    # what was read back serves as a prefix in full width
+    full = model.request_cache(2, 8, cache.read(30)[:, :1].contiguous())
+    x = _ids(3, 2, 5)
+    a = model.forward_requests(x, full)
+    cache.begin(cache.read(30)[:, :1].contiguous())
+    b = model.forward_requests(torch.cat((x, x[:1])), cache)
+    # (its own five rows are in 4 bits, of 35)
+    assert max_rel_err(b[:2].cpu().numpy(), a.cpu().numpy()) <= 0.2
+    for bad in (lambda: cache.begin(prefix[:2]), lambda: cache.begin(prefix, 31), lambda: cache.begin(prefix[..., :64]), lambda: model.request_cache(1, 8, bits=3),
+                lambda: model.request_cache(1, 8, dtype=torch.float16, bits=4), lambda: Q4Cache(dict(CFG, head_size=64), 1, 8), lambda: cache.forget(0, 11)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.parametrize("K", [0, 3])
+def test_steps_with_drafts_captured(K):
+    """one graph serves following steps, with alternatives beside the tokens: the same as step by step"""
+    model = LlamaDecoder(CFG, seed=6)
+    prefix = model.read_prefix(_ids(1, 1, 9))
+    caches = [model.request_cache(3, 16, prefix, bits=4) for _ in range(2)]
+    tokens, uniforms = _ids(2, 3), torch.rand(3, K + 1, generator=torch.Generator().manual_seed(1)).cuda()
+    drafts = _ids(3, 3, K)
+
+    def step(cache):
+        return model.step_requests(tokens, cache, uniforms, drafts if K else None, top=4)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(caches[0])  # (workspaces of this stream)
+        caches[0].lengths.fill_(9)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            result, accepted, (logprobs, entropy, top, top_logprobs) = step(caches[0])
+    caches[0].lengths.fill_(9)
+    for i in range(6):
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        r, n, scores = step(caches[1])
+        assert torch.equal(r, result) and torch.equal(n, accepted) and torch.equal(caches[0].lengths, caches[1].lengths)
+        assert all(torch.equal(a, b) for a, b in zip((logprobs, entropy, top, top_logprobs), scores))
+        assert logprobs.shape == (3, K + 1) and top.shape == (3, K + 1, 4) and (logprobs[result < 0] == 0).all() and (logprobs[result >= 0] < 0).all()
+        tokens.copy_(r.gather(1, n[:, None].long())[:, 0].clamp(min=0))
+        drafts.copy_(_ids(20 + i, 3, K)), uniforms.copy_(torch.rand(3, K + 1, generator=torch.Generator().manual_seed(50 + i)))
+    assert (caches[0].lengths <= 25).all()
+
+
+@pytest.mark.parametrize("bits", [None, 4])
+def test_scores(bits):
+    model = LlamaDecoder(CFG, seed=7)
+    ids, n = _ids(4, 3, 30), torch.tensor([30, 11, 1], dtype=torch.int32).cuda()
+    caches = [model.request_cache(3, 32, bits=bits) for _ in range(2)]
+    lp, ent, top, top_lp = model.score_requests(ids, caches[0], n, top=5)
+    logits = model.forward_requests(ids, caches[1], n).double()
+    want = torch.log_softmax(logits[:, :-1], dim=-1)
+    live = torch.arange(1, 30, device="cuda") < n[:, None]
+    assert lp.shape == ent.shape == (3, 29) and top.shape == top_lp.shape == (3, 29, 5)
+    # (tolerances: test_token_logprobs_gpu.py; logits here are within 20 of their top, 42 + 2 * 20 roundings)
+    assert (lp - torch.where(live, want.gather(-1, ids[:, 1:, None])[..., 0], 0.0)).abs().max() <= 100 * 2.0 ** -24
+    assert (top_lp - want.gather(-1, top)).abs().max() <= 100 * 2.0 ** -24
+    assert torch.equal(top[..., 0], logits[:, :-1].argmax(-1))
+    assert model.score_requests(ids, caches[0])[2].shape == (3, 29, 0)

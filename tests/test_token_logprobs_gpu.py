@@ -48,7 +48,7 @@ def _near(got, want, tol):
     got = got.cpu().double().numpy()
     plain = np.isfinite(want)
     assert np.array_equal(got[~plain], want[~plain], equal_nan=True)
-    off = np.abs(got - want)[plain]
+    off = np.abs(got[plain] - want[plain])
     room = (np.broadcast_to(tol, want.shape) + np.abs(np.where(plain, want, 0.0)) * E + 1e-45)[plain]
     assert (off <= room).all(), (off.max(), (off / room).max())
 

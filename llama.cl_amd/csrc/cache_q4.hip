@@ -117,9 +117,11 @@ extern "C" int llmops_cache_write_q4(const void* k, int64_t k_stride_b, int64_t 
     a.ck = reinterpret_cast<uint8_t*>(kv_cache) + 2 * layer_id * (int64_t)plane, a.cv = a.ck + (int64_t)plane;
     // (a workgroup reads its rows while others have written theirs)
     const Extent written(a.ck, 2 * plane);
-    for (int64_t h = 0; h < Hkv; h++) {
-        const Extent kh(reinterpret_cast<const char*>(k) + h * k_stride_h * e, B, (Wide)k_stride_b * e, qL, (Wide)k_stride_l * e, kS * e),
-            vh(reinterpret_cast<const char*>(v) + h * v_stride_h * e, B, (Wide)v_stride_b * e, qL, (Wide)v_stride_l * e, kS * e);
+    const bool dense = k_stride_h == kS && v_stride_h == kS;  // (a token's heads one behind the other: looked at together)
+    for (int64_t h = 0; h < (dense ? 1 : Hkv); h++) {
+        const Wide width = (Wide)(dense ? Hkv : 1) * kS * e;
+        const Extent kh(reinterpret_cast<const char*>(k) + h * k_stride_h * e, B, (Wide)k_stride_b * e, qL, (Wide)k_stride_l * e, width),
+            vh(reinterpret_cast<const char*>(v) + h * v_stride_h * e, B, (Wide)v_stride_b * e, qL, (Wide)v_stride_l * e, width);
         LLMOPS_REQUIRE(apart(written, kh) && apart(written, vh));
     }
     a.lengths = lengths, a.q_lens = q_lens, a.maxlen = maxlen;

@@ -171,27 +171,33 @@ __device__ __forceinline__ void q4_take(const Q4Args& a, Q4FewIn<RT>& sm, float*
 // The same from q itself, and the sequence's new rows of k and v written (a launch less).  All of it by the workgroup, sixteen lanes to a row, 16 rows at a time.
 // Loads that wait for each other: where many workgroups keep the memory busy the launch is the better way (32 sequences of up to 4096 rows 88 us with
 // it, 109 without; two of up to 200 14.9 and 10.7).
+// What it needs of memory is asked for with the length (q, first_new: a row of k or v, f); queries from the first sixteen lanes on, new rows from the last, so
+// that one query and its row are turned by different waves at a time.
+struct Q4Asked {
+    RowPair first_new;
+    float f;
+};
 template <int RT>
-__device__ __forceinline__ void q4_begin(const Q4Args& a, Q4FewIn<RT>& sm, float* factors, int b, int hk, int len, int n, const RowPair (&q)[RT], const RowPair& first_new) {
+__device__ __forceinline__ void q4_begin(const Q4Args& a, Q4FewIn<RT>& sm, float* factors, int b, int hk, int len, int n, const RowPair (&q)[RT], const Q4Asked& asked) {
     const int thread = (int)unseen(threadIdx.x), i = thread >> 4, j = thread & 15;
+    if ((thread & 63) < a.half)
 #pragma unroll 1
-    for (int e = thread; e < n * 64; e += 256)
-        if ((e & 63) < a.half) sm.turn[e >> 6][e & 63] = turn64(a.inv_freq[e & 63], len + (e >> 6));
+        for (int l = thread >> 6; l < n; l += 4) sm.turn[l][thread & 63] = turn64(asked.f, len + l);
     __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const int in = min(16 * rt + i, a.Mq - 1), l = in / a.G;
-        const QueryRow r = turned_query(q[rt], query_at(a, b, hk, in), j, sm.turn[min(l, max(n - 1, 0))], a.half, l < n);
-        const int at = rt * 8 * 64 + (j & 3) * 64 + 16 * (j >> 2) + i;  // dims 32*g + 8*step .. of query i
+        const int in = 16 * rt + i, at = rt * 8 * 64 + (j & 3) * 64 + 16 * (j >> 2) + i;  // dims 32*g + 8*step .. of query i
+        QueryRow r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0), 0.0f};
+        if (in < a.Mq) r = turned_query(q[rt], query_at(a, b, hk, in), j, sm.turn[min(in / a.G, max(n - 1, 0))], a.half, in / a.G < n);
         sm.q[at] = r.hi;
         sm.q[at + 4 * 64] = r.lo;
         if (j == 0) factors[16 * rt + i] = r.c;
     }
-    RowPair p = first_new;
+    RowPair p = asked.first_new;
 #pragma unroll 1
-    for (int r = i; r < 2 * n; r += 16) {  // (k and v of a row in turn)
+    for (int r = 15 - i; r < 2 * n; r += 16) {  // (k and v of a row in turn)
         const float* src = new_row_at(a, (r & 1) == 0, b, hk, r >> 1);
-        if (r != i) p.load(src, j);
+        if (r >= 16) p.load(src, j);
         write_row(a, p, src, (r & 1) == 0, b, hk, len + (r >> 1), j, sm.turn[r >> 1]);
     }
     __syncthreads();
@@ -308,12 +314,14 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
         if (start.b < 0) return;
         b = start.b, before = start.before, first = start.first, last = start.last;
     }
-    RowPair q_rows[WHOLE ? RT : 1], new_row;
+    RowPair q_rows[WHOLE ? RT : 1];
+    Q4Asked asked;
     if constexpr (WHOLE) {  // (asked for with the length)
-        const int r = threadIdx.x >> 4, j = threadIdx.x & 15, hk = blockIdx.x - b * a.Hkv;
+        const int i = threadIdx.x >> 4, r = 15 - i, j = threadIdx.x & 15, hk = blockIdx.x - b * a.Hkv;
+        asked.f = a.inv_freq[min((int)threadIdx.x & 63, a.half - 1)];
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) q_rows[rt].load(query_at(a, b, hk, min(16 * rt + r, a.Mq - 1)), j);
-        if (r < 2 * a.qL) new_row.load(new_row_at(a, (r & 1) == 0, b, hk, r >> 1), j);
+        for (int rt = 0; rt < RT; rt++) q_rows[rt].load(query_at(a, b, hk, min(16 * rt + i, a.Mq - 1)), j);
+        if (r < 2 * a.qL) asked.first_new.load(new_row_at(a, (r & 1) == 0, b, hk, r >> 1), j);
     }
     UnitsOf its = units_of(a, b);
 #pragma unroll 1
@@ -345,7 +353,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
         const bool old = !WHOLE || 32 * j0 + 32 <= len;
         if (j0 < j1 && old) x.load_k(q4_rows(K, 32 * j0, rows), i, g), x.load_v(q4_rows(V, 32 * j0, rows), i, g);
         if constexpr (WHOLE) {
-            q4_begin<RT>(a, sm.in, sm.factors, b, hk, len, n, q_rows, new_row);
+            q4_begin<RT>(a, sm.in, sm.factors, b, hk, len, n, q_rows, asked);
             if (j0 < j1 && !old) x.load_k(q4_rows(K, 32 * j0, rows), i, g), x.load_v(q4_rows(V, 32 * j0, rows), i, g);
         }
         if constexpr (!WHOLE) q4_take<RT>(a, sm.in, sm.factors, b, hk, n, lane);

@@ -170,7 +170,7 @@ __device__ __forceinline__ void q4_take(const Q4Args& a, Q4FewIn<RT>& sm, float*
 }
 // The same from q itself, and the sequence's new rows of k and v written (a launch less).  All of it by the workgroup, sixteen lanes to a row, 16 rows at a time.
 // Loads that wait for each other: where many workgroups keep the memory busy the launch is the better way (32 sequences of up to 4096 rows 88 us with
-// it, 109 without; two of up to 200 14.9 and 10.7).
+// it, 109 without; two of up to 200 14.9 and 9.7).
 // What it needs of memory is asked for with the length (q, first_new: a row of k or v, f); queries from the first sixteen lanes on, new rows from the last, so
 // that one query and its row are turned by different waves at a time.
 struct Q4Asked {
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
     }
 }
 
-// Many queries (64 * RT to a workgroup, 16 * RT to a wave).  All waves multiply the same 64 rows, whose values the workgroup forms once and leaves in LDS in the
+// Many queries (64 to a workgroup, 16 to a wave).  All waves multiply the same 64 rows, whose values the workgroup forms once and leaves in LDS in the
 // order of the operands (a read is 16 bytes to a lane, in lane order); two buffers: while a tile is multiplied the next one's values are formed and the one
 // behind it is on its way from memory.
 struct Q4TileSmem {
@@ -528,7 +528,6 @@ struct Q4TileRegs {
     }
 };
 
-template <int RT>
 __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
     __shared__ Q4TileSmem sm;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
@@ -557,7 +556,7 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
         if (u0 >= real) continue;
         int len, n;
         own_extent(a.lengths, a.q_lens, b, a.qL, a.maxlen, len, n);
-        const int in0 = tile * 64 * RT, in_end = min(a.Mq, in0 + 64 * RT);
+        const int in0 = tile * 64, in_end = min(a.Mq, in0 + 64);
         // rows that the tile's last live query sees
         const int rows = in0 < n * a.G ? len + min(n, (in_end - 1) / a.G + 1) : 0;
         const int64_t plane = ((int64_t)b * a.Hkv + hk) * a.maxlen * kQ4Row;
@@ -566,26 +565,20 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
         Q4TileRegs x;
         auto load = [&](int j) { x.load(q4_rows<64>(K, 64 * j, rows), q4_rows<64>(V, 64 * j, rows), wave, i, g); };
         if (j0 < j1) load(j0);
-        v8h qh[RT][4], ql[RT][4];
-        Queries<RT> s;
-        bool live[RT];
-        int see_min = INT_MAX;
+        v8h qh[4], ql[4];
+        Queries<1> s;
+        const int mine = min(in0 + 16 * wave + i, in_end - 1), l = mine / a.G;
+        const bool live = l < n;
+        const int64_t m = (int64_t)hk * a.M + (int64_t)b * a.Mq + mine, from = m * kS + 32 * g;
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            const int in = min(in0 + 16 * (RT * wave + rt) + i, in_end - 1), l = in / a.G;
-            live[rt] = l < n;
-            const int64_t m = (int64_t)hk * a.M + (int64_t)b * a.Mq + in, from = m * kS + 32 * g;
-#pragma unroll
-            for (int step = 0; step < 4; step++) {
-                qh[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + from + 8 * step));
-                ql[rt][step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + from + 8 * step));
-            }
-            s.c[rt] = live[rt] ? a.cq[m] : 0.0f, s.m[rt] = -INFINITY, s.l[rt] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < 8; c++) s.o[rt][c] = v4f{0.f, 0.f, 0.f, 0.f};
-            s.see[rt] = live[rt] ? len + l + 1 : INT_MAX;  // (what padding sees is thrown away)
-            see_min = min(see_min, s.see[rt]);
+        for (int step = 0; step < 4; step++) {
+            qh[step] = as_v8h(*reinterpret_cast<const uint4*>(a.qh + from + 8 * step));
+            ql[step] = as_v8h(*reinterpret_cast<const uint4*>(a.ql + from + 8 * step));
         }
+        s.c[0] = live ? a.cq[m] : 0.0f, s.m[0] = -INFINITY, s.l[0] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; c++) s.o[0][c] = v4f{0.f, 0.f, 0.f, 0.f};
+        s.see[0] = live ? len + l + 1 : INT_MAX;  // (what padding sees is thrown away)
         if (j0 < j1) {
             x.write(codes, sm, 0, wave, lane, 64 * j0 + 64 > len);
             load(min(j0 + 1, j1 - 1));
@@ -597,75 +590,62 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
             x.write(codes, sm, buf ^ 1, wave, lane, t + 128 > len);  // (behind the last tile that one again: nobody reads it)
             load(min(j + 2, j1 - 1));
             __builtin_amdgcn_sched_barrier(0);  // (asked for now: behind the scores' products they come late)
-            const bool masked = __any(t + 64 > see_min);
-            v4f sc[RT][4];
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = sc[rt][2] = sc[rt][3] = v4f{0.f, 0.f, 0.f, 0.f};
+            const bool masked = __any(t + 64 > s.see[0]);
+            v4f sc[4];
+            sc[0] = sc[1] = sc[2] = sc[3] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int step = 0; step < 4; step++) {
                 v8h k[4];
 #pragma unroll
                 for (int tt = 0; tt < 4; tt++) k[tt] = as_v8h(sm.k[buf][4 * tt + step][lane]);
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
+                for (int tt = 0; tt < 4; tt++) sc[tt] = mfma(k[tt], qh[step], sc[tt]);
 #pragma unroll
-                    for (int tt = 0; tt < 4; tt++) sc[rt][tt] = mfma(k[tt], qh[rt][step], sc[rt][tt]);
+                for (int tt = 0; tt < 4; tt++) sc[tt] = mfma(k[tt], ql[step], sc[tt]);
+            }
+            Weights w[2];
+            if (t + 64 > len) {
 #pragma unroll
-                    for (int tt = 0; tt < 4; tt++) sc[rt][tt] = mfma(k[tt], ql[rt][step], sc[rt][tt]);
+                for (int tt = 0; tt < 4; tt++) {
+                    const uint32_t bad = __builtin_amdgcn_readfirstlane(sm.bad[buf][tt]);
+                    if (bad != 0)
+#pragma unroll
+                        for (int v = 0; v < 4; v++)
+                            if (bad >> (4 * g + v) & 1) sc[tt][v] = NAN;
                 }
             }
-            Weights w[RT][2];
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                if (t + 64 > len) {
-#pragma unroll
-                    for (int tt = 0; tt < 4; tt++) {
-                        const uint32_t bad = __builtin_amdgcn_readfirstlane(sm.bad[buf][tt]);
-                        if (bad != 0)
-#pragma unroll
-                            for (int v = 0; v < 4; v++)
-                                if (bad >> (4 * g + v) & 1) sc[rt][tt][v] = NAN;
-                    }
-                }
-                weigh<true>(s, rt, sc[rt], t, g, masked);
-                w[rt][0] = weights_of<__half>({sc[rt][0], sc[rt][1]});
-                w[rt][1] = weights_of<__half>({sc[rt][2], sc[rt][3]});
-            }
+            weigh<true>(s, 0, sc, t, g, masked);
+            w[0] = weights_of<__half>({sc[0], sc[1]});
+            w[1] = weights_of<__half>({sc[2], sc[3]});
 #pragma unroll
             for (int c0 = 0; c0 < 16; c0 += 4) {
                 v8h h[4];
 #pragma unroll
                 for (int c = 0; c < 4; c++) h[c] = as_v8h(sm.v[buf][c0 + c][lane]);
+                const Weights& x2 = w[c0 >> 3];
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    const Weights& x2 = w[rt][c0 >> 3];
+                for (int c = 0; c < 4; c++) s.o[0][(c0 & 7) + c] = mfma(h[c], x2.hi, s.o[0][(c0 & 7) + c]);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) s.o[rt][(c0 & 7) + c] = mfma(h[c], x2.hi, s.o[rt][(c0 & 7) + c]);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) s.o[rt][(c0 & 7) + c] = mfma(h[c], x2.lo, s.o[rt][(c0 & 7) + c]);
-                }
+                for (int c = 0; c < 4; c++) s.o[0][(c0 & 7) + c] = mfma(h[c], x2.lo, s.o[0][(c0 & 7) + c]);
             }
             __syncthreads();
         }
         const bool whole = u0 == 0 && u1 >= real;
-        const int64_t record = ((int64_t)blockIdx.x * 2 + (u0 == 0)) * (64 * RT);
+        const int64_t record = ((int64_t)blockIdx.x * 2 + (u0 == 0)) * 64;
+        s.l[0] += __shfl_xor(s.l[0], 16, 64);
+        s.l[0] += __shfl_xor(s.l[0], 32, 64);
+        const int in = 16 * wave + i;
+        if (in0 + in >= in_end) continue;
+        if (!whole && g == 0) a.rec_stat[record + in] = make_float2(s.m[0], live ? s.l[0] : -1.0f);
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            s.l[rt] += __shfl_xor(s.l[rt], 16, 64);
-            s.l[rt] += __shfl_xor(s.l[rt], 32, 64);
-            const int in = 16 * (RT * wave + rt) + i;
-            if (in0 + in >= in_end) continue;
-            if (!whole && g == 0) a.rec_stat[record + in] = make_float2(s.m[rt], live[rt] ? s.l[rt] : -1.0f);
+        for (int v = 0; v < 4; v++)
 #pragma unroll
-            for (int v = 0; v < 4; v++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float4 o = make_float4(s.o[rt][4 * h][v], s.o[rt][4 * h + 1][v], s.o[rt][4 * h + 2][v], s.o[rt][4 * h + 3][v]);
-                    const int d = 8 * (4 * g + v) + 4 * h;
-                    if (whole) q4_leave(a, b, hk, in0 + in, d, o, s.l[rt], live[rt]);
-                    else *reinterpret_cast<float4*>(a.rec_out + (record + in) * kS + d) = o;
-                }
-        }
+            for (int h = 0; h < 2; h++) {
+                const float4 o = make_float4(s.o[0][4 * h][v], s.o[0][4 * h + 1][v], s.o[0][4 * h + 2][v], s.o[0][4 * h + 3][v]);
+                const int d = 8 * (4 * g + v) + 4 * h;
+                if (whole) q4_leave(a, b, hk, in0 + in, d, o, s.l[0], live);
+                else *reinterpret_cast<float4*>(a.rec_out + (record + in) * kS + d) = o;
+            }
     }
 }
 
@@ -741,11 +721,15 @@ static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t max
     Q4Plan p{};
     const int64_t Mq = qL * (H / Hkv);
     p.many = Mq > 32;
-    p.rt = !p.many && Mq > 16 ? 2 : 1;
-    p.tile = (p.many ? 64 : 16) * p.rt;
+    p.rt = !p.many && Mq > 16 ? 2 : 1;  // (of the few)
+    p.tile = p.many ? 64 : 16 * p.rt;
     p.tiles = (int)((Mq + p.tile - 1) / p.tile);
     const int64_t items = B * Hkv * p.tiles;
-    if (!p.many && maxlen <= 3 * kUnit) {
+    // One launch where a workgroup can have all rows of a kv head in the time of the two others' launches, or the chip is busy with one to each anyway;
+    // not where so many queries and new rows wait for memory at once (us with three launches and with one: 2 sequences of 32 kv heads and 300 rows 14.8 and 9.8,
+    // 1000 rows 16.5 and 14.3; 2 of 8 kv heads and 1500 rows 14.9 and 16.5; 16 of 32 and 500 rows 22.6 and 14.7, 1500 rows 30.5 and 24.4;
+    // 16 of 32 and 5 tokens, up to 2200 rows, 37.8 and 33.2; 32 of 32 and 1500 rows 44.4 and 44.3; 64 of 32 and 300 rows 35.1 and 39.1)
+    if (!p.many && items <= 1024 && maxlen <= (items >= 256 ? 16 : 8) * kUnit) {
         p.groups = (int)items;
         return p;
     }
@@ -783,7 +767,7 @@ static int q4_launch(const Q4Args& a, const Q4Plan& plan, hipStream_t st) {
     if (plan.join > 0) q4_prep_kernel<<<prep, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
     const unsigned groups = (unsigned)plan.groups;
-    if (plan.many) q4_many_kernel<1><<<groups, 256, 0, st>>>(a);
+    if (plan.many) q4_many_kernel<<<groups, 256, 0, st>>>(a);
     else if (plan.join == 0 && plan.rt == 2) q4_few_kernel<2, true><<<groups, 256, 0, st>>>(a);
     else if (plan.join == 0) q4_few_kernel<1, true><<<groups, 256, 0, st>>>(a);
     else if (plan.rt == 2) q4_few_kernel<2, false><<<groups, 256, 0, st>>>(a);

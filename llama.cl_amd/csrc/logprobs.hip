@@ -9,8 +9,9 @@
 //
 // The likeliest of a run: the `top`-th largest of the 64 lanes' own maxima is found in each wave bit by bit (a comparison and a count of lanes for each
 // bit, most of it on the scalar unit), and no logit below the largest of the four waves' can be among them; that leaves some 3 * top logits, of which each
-// counts how many others are before it.  Rows of equal logits leave more; where that is more than there is room for, the same search goes over all
-// logits and then over the numbers of those that are equal to the last.
+// counts how many others are before it.  Where that bound is minus infinity (few tokens are allowed) they are all logits above it, and the run's first ones
+// that are not.  Rows of equal logits leave more; where that is more than there is room for, the same search goes over all logits and then over the
+// numbers of those that are equal to the last.
 // fp32 sums over a thread's logits and a workgroup's threads; runs are joined, and logarithms taken, in 64 bits.
 #include <limits.h>
 
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
     if (a.top > 0) {
         const uint32_t bound = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
         // (one arrival for a wave, its lanes in order)
-        const float least = bound <= 0x007fffffu ? -INFINITY : of_key(bound);  // (keys up to that of minus infinity)
+        const float least = of_key(max(bound, 0x00800000u));  // (something: at least the lowest finite logit)
         int its = 0;
 #pragma unroll
         for (int e = 0; e < E; e++) its += (int)__builtin_popcountll(__ballot(something(x[e]) >= least));
@@ -145,6 +146,16 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
                 if (taken && slot < kHeld) held[slot] = {rank_key(x[e]), at(e)};
                 to += (int)__builtin_popcountll(all);
             }
+        }
+        // Few tokens allowed: fewer than `top` in each wave, so that there may be fewer than `top` of them, and tokens that are nothing follow, which are
+        // equal.  Their first ones are among the run's first 2 * top tokens, of which fewer than `top` are something if they are needed.
+        if (bound < 0x00800000u && 4 * (int)threadIdx.x < 2 * a.top) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (!(something(x[e]) >= least)) {  // (behind the row's end too: what a run leaves are `top` tokens, and those are behind all that are there)
+                    const int slot = atomicAdd(&count, 1);
+                    if (slot < kHeld) held[slot] = {rank_key(x[e]), at(e)};
+                }
         }
     }
     __syncthreads();

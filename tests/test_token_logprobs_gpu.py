@@ -114,6 +114,22 @@ def test_infinities_and_nan():
         _check(rows, torch.full_like(tokens, 6), 64)
 
 
+@pytest.mark.parametrize("V", [70, 2048, 8195, 24000])
+def test_few_tokens_are_allowed(V):
+    g = torch.Generator().manual_seed(V)
+    few = [n for n in (1, 5, 19, 20, 21, 63, 64, 65, 130, 300, 3000) if n <= V]
+    rows = torch.full((4 * len(few), 1, V), -math.inf)
+    for i, n in enumerate(few):
+        x = torch.randn(n, generator=g)
+        rows[4 * i, 0, torch.randperm(V, generator=g)[:n]] = x
+        rows[4 * i + 1, 0, :n] = x
+        rows[4 * i + 2, 0, V - n:] = x
+        rows[4 * i + 3, 0, (torch.arange(n) * 4 % V)] = 1.0  # (equal ones)
+    tokens = torch.randint(0, V, (len(rows), 1), generator=g)
+    for top in (1, 20, 64):
+        _check(rows, tokens, top)
+
+
 @pytest.mark.parametrize("spread", [1e-3, 30.0, 1000.0])
 def test_flat_and_steep(spread):
     logits, tokens = _case(6, 2, 4000, 5, spread)

@@ -46,7 +46,8 @@ def sources():
 # requests in step, but for prefix_apart_kernel<float, 2, false, false> (9 registers, 40 bytes of scratch a lane).
 NO_SPILL = ["fc_gemv_fused_kernelILi128ELi1E", "attn_prefill_kernel", "fc_gemm_tile_kernel", "prefix_brief_kernel", "prefix_sweep_kernel",
             "prefix_apart_kernelI6__half", "prefix_apart_kernelIfLi1E", "prefix_apart_kernelIfLi2ELb1E", "lora_down_kernel", "lora_up_kernel",
-            "verify_rows_kernel", "verify_next_kernel"]
+            "verify_rows_kernel", "verify_next_kernel", "q4_write_turned_kernel", "q4_write_kernel", "q4_read_kernel", "q4_prep_kernel", "q4_few_kernel",
+            "q4_many_kernel", "q4_join_kernel", "logprob_runs_kernel", "logprob_rows_kernel"]
 
 
 def check_spills(remarks):

@@ -832,6 +832,9 @@ extern "C" int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int6
         v_at(v, B, (Wide)v_stride_b * 4, qL, (Wide)v_stride_l * 4, kv_heads), out_at(out, (Wide)B * qL * heads), written(a.ck, 2 * plane);
     LLMOPS_REQUIRE(apart(written, q_at) && apart(written, k_at) && apart(written, v_at));
     LLMOPS_REQUIRE(apart(out_at, q_at) && apart(out_at, k_at) && apart(out_at, v_at) && apart(out_at, written));
+    const Extent lengths_at(lengths, (Wide)B * 4), q_lens_at(q_lens, q_lens != nullptr ? (Wide)B * 4 : 0), inv_freq_at(inv_freq, (Wide)half * 4);
+    LLMOPS_REQUIRE(apart(written, lengths_at) && apart(written, q_lens_at) && apart(written, inv_freq_at));
+    LLMOPS_REQUIRE(apart(out_at, lengths_at) && apart(out_at, q_lens_at) && apart(out_at, inv_freq_at));
     hipStream_t st = as_stream(stream);
     return q4_launch(a, plan, st);
 }

@@ -124,6 +124,8 @@ extern "C" int llmops_cache_write_q4(const void* k, int64_t k_stride_b, int64_t 
             vh(reinterpret_cast<const char*>(v) + h * v_stride_h * e, B, (Wide)v_stride_b * e, qL, (Wide)v_stride_l * e, width);
         LLMOPS_REQUIRE(apart(written, kh) && apart(written, vh));
     }
+    const Extent lengths_at(lengths, (Wide)B * 4), q_lens_at(q_lens, q_lens != nullptr ? (Wide)B * 4 : 0), inv_freq_at(inv_freq, inv_freq != nullptr ? (Wide)half * 4 : 0);
+    LLMOPS_REQUIRE(apart(written, lengths_at) && apart(written, q_lens_at) && apart(written, inv_freq_at));
     a.lengths = lengths, a.q_lens = q_lens, a.maxlen = maxlen;
     a.B = (int)B, a.qL = (int)qL, a.Hkv = (int)Hkv, a.half = (int)half, a.groups = (int)((2 * Hkv + 15) / 16);
     a.shared = B > 1 && k_stride_b == 0 && v_stride_b == 0;

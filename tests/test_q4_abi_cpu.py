@@ -39,6 +39,7 @@ def _write(lib, **kw):
     (dict(half=0), b"half"), (dict(layer=1), b"layer_id"), (dict(layer=-1), b"layer_id"), (dict(k=ctypes.c_void_p(4104)), b"aligned(k, 16)"),
     (dict(kv=ctypes.c_void_p(4104)), b"aligned"), (dict(kl=1026), b"k_stride_l"), (dict(dt=1, vh=132), b"v_stride_h"), (dict(kv=P), b"apart(written, kh)"),
     (dict(k=ctypes.c_void_p(1 << 30), kv=ctypes.c_void_p((1 << 30) - 2 * 2 * 8 * 64 * 80 + 16)), b"apart(written"), (dict(B=1 << 20, qL=1 << 20, maxlen=1), b"most"),
+    (dict(lengths=ctypes.c_void_p((1 << 40) + 400)), b"apart(written, lengths_at)"), (dict(q_lens=FAR), b"apart(written, q_lens_at)"), (dict(f=FAR), b"apart(written, inv_freq_at)"),
 ])
 def test_cache_write_refuses(lib, kw, what):
     _refused(lib, _write(lib, **kw), what)
@@ -74,6 +75,9 @@ def _attend(lib, **kw):
     (dict(maxlen=(1 << 24) + 1), b"q4_sizes_fit"), (dict(B=1 << 20), b"q4_sizes_fit"), (dict(B=1 << 12, maxlen=1 << 24), b"q4_sizes_fit"), (dict(half=65), b"half"), (dict(half=0), b"half"),
     (dict(layer=1), b"layer_id"), (dict(layer=-1), b"layer_id"), (dict(q=ctypes.c_void_p(4104)), b"aligned(q, 16)"), (dict(ws=ctypes.c_void_p((1 << 35) + 16)), b"aligned(workspace, 256)"),
     (dict(kl=1026), b"k_stride_l"), (dict(kv=P), b"apart(written, q_at)"), (dict(out=P), b"apart(out_at, q_at)"), (dict(out=FAR), b"apart(out_at, written)"),
+    (dict(lengths=FAR), b"apart(written, lengths_at)"), (dict(q_lens=FAR), b"apart(written, q_lens_at)"), (dict(f=FAR), b"apart(written, inv_freq_at)"),
+    (dict(lengths=ctypes.c_void_p(1 << 30)), b"apart(out_at, lengths_at)"), (dict(q_lens=ctypes.c_void_p(1 << 30)), b"apart(out_at, q_lens_at)"),
+    (dict(f=ctypes.c_void_p((1 << 30) + 256)), b"apart(out_at, inv_freq_at)"),
 ])
 def test_attention_refuses(lib, kw, what):
     _refused(lib, _attend(lib, **kw), what)

@@ -48,15 +48,16 @@ struct Held {
     int32_t at;
 };
 __device__ __forceinline__ int is_ahead(Held a, Held b) { return a.key > b.key || (a.key == b.key && a.at < b.at) ? 1 : 0; }
-// how many of `held` (n, and up to three that are nothing behind them) are before one of them
+// how many of `held` (n, and up to three that are nothing behind them) are before one of them; four neighbouring lanes count a quarter each
 __device__ __forceinline__ int how_many_ahead(const Held* held, int n, Held one) {
     int before = 0;
-#pragma unroll 4
-    for (int t = 0; t < n; t += 4) {
+#pragma unroll 2
+    for (int t = 4 * (threadIdx.x & 3); t < n; t += 16) {
         const uint4 x = *reinterpret_cast<const uint4*>(held + t), y = *reinterpret_cast<const uint4*>(held + t + 2);
         before += is_ahead({x.x, (int)x.y}, one) + is_ahead({x.z, (int)x.w}, one) + is_ahead({y.x, (int)y.y}, one) + is_ahead({y.z, (int)y.w}, one);
     }
-    return before;
+    before += __shfl_xor(before, 1, 64);
+    return before + __shfl_xor(before, 2, 64);
 }
 __device__ __forceinline__ Held nothing_held() { return {0u, INT_MAX}; }
 
@@ -133,13 +134,15 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
         const float least = of_key(max(bound, 0x00800000u));  // (something: at least the lowest finite logit)
         int its = 0;
 #pragma unroll
-        for (int e = 0; e < E; e++) its += (int)__builtin_popcountll(__ballot(something(x[e]) >= least));
+        for (int e = 0; e < E; e++) its += (int)__builtin_popcountll(__ballot(x[e] >= least));
         int to = 0;
         if (lane == 0 && its > 0) to = atomicAdd(&count, its);
         to = __builtin_amdgcn_readfirstlane(to);
+        float again = least;  // (the comparisons made again: 32 of their results kept take more scalar registers than there are)
+        asm volatile("" : "+v"(again));
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const bool taken = something(x[e]) >= least;
+            const bool taken = x[e] >= again;
             const uint64_t all = __ballot(taken);
             if (all != 0) {
                 const int slot = to + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
         if (bound < 0x00800000u && 4 * (int)threadIdx.x < 2 * a.top) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (!(something(x[e]) >= least)) {  // (behind the row's end too: what a run leaves are `top` tokens, and those are behind all that are there)
+                if (!(x[e] >= least)) {  // (behind the row's end too: what a run leaves are `top` tokens, and those are behind all that are there)
                     const int slot = atomicAdd(&count, 1);
                     if (slot < kHeld) held[slot] = {rank_key(x[e]), at(e)};
                 }
@@ -188,9 +191,9 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
     if (threadIdx.x < 4) held[n + threadIdx.x] = nothing_held();
     __syncthreads();
     const int64_t to = ((int64_t)row * a.runs + run) * a.top;
-    for (int c = threadIdx.x; c < n; c += 256) {
+    for (int c = (int)threadIdx.x >> 2; c < n; c += 64) {
         const int before = how_many_ahead(held, n, held[c]);
-        if (before < a.top) a.best[to + before] = held[c];
+        if (before < a.top && (threadIdx.x & 3) == 0) a.best[to + before] = held[c];
     }
 }
 
@@ -237,28 +240,28 @@ __global__ __launch_bounds__(256) void logprob_sums_kernel(LogprobArgs a, int ro
 }
 
 // a workgroup to a row: one wave its sums, all its likeliest tokens, those of 512 / top runs after the other
-__global__ __launch_bounds__(256) void logprob_rows_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(1024) void logprob_rows_kernel(LogprobArgs a) {
     __shared__ __align__(16) Held held[512 + kMostTop + 4], best[kMostTop];
     __shared__ RowSums sums;
-    const int row = blockIdx.x;
+    const int row = blockIdx.x, threads = blockDim.x;
     const int64_t n = (int64_t)a.runs * a.top;
     const Held* from = a.best + (int64_t)row * n;
     int kept = 0;
-    const bool sums_wave = threadIdx.x >= 192;
+    const bool sums_wave = threadIdx.x >= threads - 64;
     for (int64_t c0 = 0; c0 < n; c0 += 512) {
         const int more = (int)min((int64_t)512, n - c0), m = more + kept;
-        for (int c = threadIdx.x; c < more + 4; c += 256) held[kept + c] = c < more ? from[c0 + c] : nothing_held();
+        for (int c = threadIdx.x; c < more + 4; c += threads) held[kept + c] = c < more ? from[c0 + c] : nothing_held();
         if ((int)threadIdx.x < kept) held[threadIdx.x] = best[threadIdx.x];
         __syncthreads();
         if (!sums_wave) {
-            for (int c = threadIdx.x; c < m; c += 192) {
+            for (int c = (int)threadIdx.x >> 2; c < m; c += (threads - 64) / 4) {
                 const int before = how_many_ahead(held, m, held[c]);
-                if (before < a.top) best[before] = held[c];
+                if (before < a.top && (threadIdx.x & 3) == 0) best[before] = held[c];
             }
         } else if (c0 == 0) {  // (beside the others' comparisons)
             RowSums s;
             row_answers(a, row, threadIdx.x & 63, s);
-            if (threadIdx.x == 192) sums = s;
+            if (threadIdx.x == threads - 64) sums = s;
         }
         kept = min(m, a.top);
         __syncthreads();
@@ -329,7 +332,8 @@ extern "C" int llmops_token_logprobs(const float* logits, int64_t stride_b, int6
     if (logprob_each(V) == 8) logprob_runs_kernel<8><<<grid, 256, 0, st>>>(a);
     else logprob_runs_kernel<32><<<grid, 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
-    if (top > 0) logprob_rows_kernel<<<(unsigned)(B * L), 256, 0, st>>>(a);
+    // (us in workgroups of 256, 512 and 1024: 2100 rows with 20 tokens of runs to compare 51 and 58, 160 rows with 140 19.5, 18.5 and 18.2, 32 rows with 320 28.2, 19.5 and 17.3)
+    if (top > 0) logprob_rows_kernel<<<(unsigned)(B * L), w.runs * top <= 96 ? 256 : 1024, 0, st>>>(a);
     else logprob_sums_kernel<<<(unsigned)((B * L + 3) / 4), 256, 0, st>>>(a, (int)(B * L));
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;

@@ -49,9 +49,9 @@ __device__ __forceinline__ void write_row(const Q4Args& a, const RowPair& p, con
     if (is_k) {
         double x[8];
         turn_row(p, src, j, turn, a.half, x);
-        store_q4(dst, quantise8<true>(x), j);
+        store_q4(dst, quantise8(x), j);
     } else {
-        store_q4(dst, quantise8<true>(p.x), j);
+        store_q4(dst, quantise8(p.x), j);
     }
 }
 // .. of a query: turned in fp32
@@ -67,7 +67,10 @@ __device__ __forceinline__ const float* new_row_at(const Q4Args& a, bool is_k, i
     return is_k ? a.k + b * a.ksb + l * a.ksl + (int64_t)hk * kS : a.v + b * a.vsb + l * a.vsl + (int64_t)hk * kS;
 }
 
-// A workgroup per token and 16 of its H + 2*Hkv rows of 128, sixteen lanes to a row
+// A workgroup per token and 16 of its H + 2*Hkv rows of 128, sixteen lanes to a row.  By itself and not in the workgroups of step 2: many of these share a
+// query and each would turn it again (4 turns of 300 tokens: step 2 takes 62 us as it is, 73 with that).
+// Latency with few tokens (32 of 96 rows 5.0 us: the length, the row and the frequency in one round trip, the sincos in 64 bits, the codes), memory with many
+// (1200 tokens, 29 MB in from the memory side, 26 out, 18 us; two or three rows one behind the other to sixteen lanes: the same).
 __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a) {
     __shared__ double2 turn[64];
     const int bl = blockIdx.x / a.row_groups, group = blockIdx.x - bl * a.row_groups, b = bl / a.qL, l = bl - b * a.qL;
@@ -299,6 +302,10 @@ struct Q4MeetSmem {
 
 // Few queries to a workgroup (16 * RT).  The four waves take 32 rows each of every 128; operands come straight from memory, the next rows asked
 // for when these are used up; the waves' sums meet in LDS.
+// Memory bounds it: a row's 80 bytes of K are read in 16-byte pieces by the lanes that multiply them, V's in words.  32 sequences of up to 4096 rows, 32 heads: 335 MB
+// in 74 us, 4.5 TB/s (a kernel that only reads them, in one order: 51 us; this one with its products taken out: 65); the vector ALU is busy half of
+// the time, mostly with making halves of codes.  100001 rows of 8 heads: 128 MB in 23 us, with 6 us of joining behind.  Not faster: copies to LDS by the DMA
+// engine, one or two stages ahead (87 us for the call, 87 and 93); waves' priorities by turn (91 to 97); more workgroups than the chip holds (87).
 template <int RT, bool WHOLE>
 __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(Q4Args a) {
     __shared__ Q4MeetSmem<RT> sm;
@@ -475,6 +482,10 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
 // Many queries (64 to a workgroup, 16 to a wave).  All waves multiply the same 64 rows, whose values the workgroup forms once and leaves in LDS in the
 // order of the operands (a read is 16 bytes to a lane, in lane order); two buffers: while a tile is multiplied the next one's values are formed and the one
 // behind it is on its way from memory.
+// Instructions bound it, and what two waves to a SIMD leave uncovered: 4 turns of 300 tokens behind up to 1777 rows, 32 heads, 61 us, of which the vector ALU is
+// busy 21, the matrix cores 12 and LDS reads, 32 KB to a wave and tile of 64 rows, 12; waves wait for data 28 % of the time and for a turn to issue 36 %.  Not faster: 128 queries to four
+// waves (fewer workgroups than places, twice the registers), 128 to eight waves (the call 104 us instead of 86; 2048 tokens of one sequence, 194 instead of 211),
+// one buffer and three workgroups to a compute unit (85 instead of 83).
 struct Q4TileSmem {
     uint4 k[2][16][64], v[2][16][64];
     uint32_t bad[2][4];  // of 16 rows each: V rows that hold NaN, among those that are new
@@ -650,7 +661,9 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
 }
 
 // ---- 3. what several workgroups have of a query ----
-// A workgroup to a.join (1, 2, 4, 8) queries of a tile, 8 / a.join half waves to a query, each to as many records from the other, 16 bytes to a lane
+// A workgroup to a.join (1, 2, 4, 8) queries of a tile, 8 / a.join half waves to a query, each to as many records from the other, 16 bytes to a lane.  Latency: 5 us
+// with one or two records to a query, 6.2 with 128, 9.7 with 38400 queries (20 MB of records, 20 MB out).  Joined by the last workgroup to arrive
+// instead, records written through to memory: 32 sequences 90 us instead of 89, 64 with grouped heads 87.5 and 89.4, one of 100001 rows 41 and 32.
 __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
     __shared__ float stat[8][2];
     __shared__ float4 part[8][32];
@@ -720,6 +733,7 @@ struct Q4Plan {
 static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t maxlen) {
     Q4Plan p{};
     const int64_t Mq = qL * (H / Hkv);
+    // (us with few and with many: 16 sequences of 20 queries to a kv head 59 and 66, of 30 62 and 72; 2 of 20 28 and 32.  Above 32 queries the few would read rows twice)
     p.many = Mq > 32;
     p.rt = !p.many && Mq > 16 ? 2 : 1;  // (of the few)
     p.tile = p.many ? 64 : 16 * p.rt;

@@ -47,8 +47,7 @@ __device__ __forceinline__ double scaled(double x, int e) { return ldexp(x, e); 
 
 // Sixteen lanes to a row, eight values to a lane (dims 8 * (lane % 16) ..), R float or double: the lane's word of codes, and d | m << 16 of its
 // group (the same in its four lanes)
-// GUESS: not for values that are halves, or whole numbers of any other unit, which lie on borders all the time
-template <bool GUESS, typename R>
+template <typename R>
 __device__ __forceinline__ uint2 quantise8(const R (&x)[8]) {
     R top = x[0], low = x[0];
     bool fine = true;
@@ -68,12 +67,21 @@ __device__ __forceinline__ uint2 quantise8(const R (&x)[8]) {
     e = spoilt ? 0 : max(e, 11 - 24);
     const float lo = (float)rint(scaled(low, 11 - e)) + 0.0f, hi = (float)rint(scaled(top, 11 - e));
     const int step = ((int)(hi - lo) + 14) / 15;  // (lo is no -0: zeros of either sign are stored alike)
-    const float s = (float)step, half = 0.5f * s, inv = step > 0 ? 1.0f / s : 0.0f;
+    const float s = (float)step, half = 0.5f * s, inv = step > 0 ? 1.0f / s : 0.0f, scale = ldexpf(1.0f, 11 - e);
     uint32_t word = 0;
-    bool near = true;
-    if constexpr (GUESS) {
+    if constexpr (sizeof(R) == 4) {
+        // The code or one less, from (x / u - lo) / s less 2^-10 (fp32 is off by less than 2^-12 there), then put right by the border above it,
+        // lo + (code + 1/2) s, which is exact, as is the sign of what x / u is away from it; on the border itself odd codes go up
+        const float slope = scale * inv, from = fmaf(-lo, inv, -0x1p-10f), border = lo + half;
+        const int most_code = step > 0 ? 15 : 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float c = rintf(fmaf(x[i], slope, from)), past = fmaf(x[i], scale, -fmaf(c, s, border)), odd = __builtin_amdgcn_fractf(0.5f * c);
+            const int code = (int)c + (fmaf(odd, 0x1p-99f, past) > 0.0f ? 1 : 0);
+            word |= (uint32_t)min(code, most_code) << (4 * (i >> 1) + 16 * (i & 1));
+        }
+    } else {
         // in fp32, which is off by less than 2^-12 of a unit here, unless a value is nearer than 2^-11 to a border (in one of some hundred rows)
-        const float scale = ldexpf(1.0f, 11 - e);
         float farthest = -1.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -81,20 +89,19 @@ __device__ __forceinline__ uint2 quantise8(const R (&x)[8]) {
             farthest = fmaxf(farthest, fabsf(t - fmaf(c, s, lo)));
             word |= (uint32_t)c << (4 * (i >> 1) + 16 * (i & 1));
         }
-        near = farthest > half - 0x1p-11f && step > 0;
-    }
-    if (__any(near)) {
-        word = 0;
+        if (__any(farthest > half - 0x1p-11f && step > 0)) {
+            word = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // a first guess, put right by the borders on either side of it, which are exact: lo + (c - 1/2) s and lo + (c + 1/2) s
-            const R t = scaled(x[i], 11 - e);
-            const float c = fminf(fmaxf(rintf(((float)t - lo) * inv), 0.0f), 15.0f), level = fmaf(c, s, lo);
-            const bool odd = (int)c & 1;
-            const R above = (R)(level + half), below = (R)(level - half);
-            int code = (int)c + ((t > above || (t == above && odd)) ? 1 : 0) - ((t < below || (t == below && odd)) ? 1 : 0);
-            code = step > 0 ? min(max(code, 0), 15) : 0;
-            word |= (uint32_t)code << (4 * (i >> 1) + 16 * (i & 1));
+            for (int i = 0; i < 8; i++) {
+                // a first guess, put right by the borders on either side of it, which are exact: lo + (c - 1/2) s and lo + (c + 1/2) s
+                const R t = scaled(x[i], 11 - e);
+                const float c = fminf(fmaxf(rintf(((float)t - lo) * inv), 0.0f), 15.0f), level = fmaf(c, s, lo);
+                const bool odd = (int)c & 1;
+                const R above = (R)(level + half), below = (R)(level - half);
+                int code = (int)c + ((t > above || (t == above && odd)) ? 1 : 0) - ((t < below || (t == below && odd)) ? 1 : 0);
+                code = step > 0 ? min(max(code, 0), 15) : 0;
+                word |= (uint32_t)code << (4 * (i >> 1) + 16 * (i & 1));
+            }
         }
     }
     const uint32_t d = f32_to_f16_bits(ldexpf(s, e - 11)), m = f32_to_f16_bits(ldexpf(lo, e - 11));

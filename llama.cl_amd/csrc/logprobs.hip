@@ -74,6 +74,9 @@ __device__ __forceinline__ int count_all(int* sums, F is) {
     return all;
 }
 
+// 32 logits to a thread: with fewer the reductions and the search weigh more, with more the registers of six workgroups to a compute unit do not suffice.
+// 2100 rows of 32003: 269 MB in 45 us, 6.0 TB/s.  With tokens to be found and all workgroups at work at once loads come first and arithmetic behind: 160 rows of
+// 55296, 35 MB, 15 us, of which memory takes 7 and the vector ALU, with 20 instructions a logit, 5.
 template <int E>
 __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
     __shared__ float red[3][4];

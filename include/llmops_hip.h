@@ -356,7 +356,7 @@ int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, int64_t V, c
  * 2*layer_id+1 (v).  k and v are of `dtype` (LLMOPS_F32, _F16), head h of token l of sequence b at + b*stride_b + l*stride_l + h*stride_h elements
  * (multiples of 16 bytes; 0 where rows are the same), unchanged.  With inv_freq [half] k is rotated by its row's number first, as
  * llmops_rope_embed with angles, rotation and codes in 64 bits; NULL: k comes rotated.  lengths, q_lens, and tokens that do not fit: as llmops_attention_rope_prefix.
- * The caller adds to lengths[b] what is to be kept.  kv_cache 16-byte aligned; k or v over the two planes are refused. */
+ * The caller adds to lengths[b] what is to be kept.  kv_cache 16-byte aligned; k, v, lengths, q_lens or inv_freq over the two planes are refused. */
 int llmops_cache_write_q4(const void* k, int64_t k_stride_b, int64_t k_stride_l, int64_t k_stride_h, const void* v, int64_t v_stride_b,
                           int64_t v_stride_l, int64_t v_stride_h, int dtype, int64_t B, int64_t qL, int64_t Hkv, int64_t S, const float* inv_freq,
                           int64_t half, void* kv_cache, int64_t planes, int64_t maxlen, const int32_t* lengths, const int32_t* q_lens, int layer_id,
@@ -369,8 +369,9 @@ int llmops_cache_read_q4(const void* kv_cache, int64_t planes, int64_t B, int64_
                          void* out, int dtype, llmops_stream_t stream);
 
 /* llmops_attention_rope_prefix without a prefix, over a cache in 4 bits: the new tokens' k (rotated) and v go to the cache as llmops_cache_write_q4 writes them,
- * and out is the softmax over what rows 0 .. lengths[b] + l of the cache stand for, the call's own among them.  Arguments, padding and refusals as there.
- * Rows are shared out among workgroups by the lengths on the device: a cache's capacity costs nothing but its memory.
+ * and out is the softmax over what rows 0 .. lengths[b] + l of the cache stand for, the call's own among them.  Arguments, padding and refusals as there; lengths,
+ * q_lens or inv_freq over out or the two planes are refused too.  Rows are shared out among workgroups by the lengths on the device: a cache's capacity costs its
+ * memory and little else (up to 2048 rows each kv head of a sequence may be one workgroup's).
  * Arithmetic: products of halves with fp32 sums, the cache's values exact, queries and weights in two halves (22 bits of a query beside its
  * head's largest value): results agree with fp32 evaluation to about 1e-6 of the largest output, and 2^-36 beside it, and are the same bits in every call.
  * B*qL*H < 2^24, and times ceil(maxlen/128) < 2^31. */
@@ -386,6 +387,7 @@ int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int64_t q_strid
  *   `top` likeliest tokens in the order of their logits, equal ones in the order of their numbers (top 0 .. 64, at most V; 0: both may be NULL).
  * Logits that are NaN or minus infinity weigh nothing (log p is minus infinity), equal plus infinities share the row; a row without any other
  * logit gives NaN.  fp32 sums; right to about 1e-6.
+ * Rows in which more than some hundred logits are equal and among the likeliest take up to ten times as long (minus infinity does not count).
  * B*L < 2^24, V <= 2^27, B*L*ceil(V/8192) < 2^24.  Outputs that lie over each other or over inputs are refused. */
 size_t llmops_token_logprobs_workspace_bytes(int64_t B, int64_t L, int64_t V, int64_t top);
 int llmops_token_logprobs(const float* logits, int64_t stride_b, int64_t stride_l, int64_t B, int64_t L, int64_t V, const int64_t* tokens,

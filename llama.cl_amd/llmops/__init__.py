@@ -795,6 +795,8 @@ def token_logprobs(logits, tokens, top=0):
     lib = _lib.load()
     logprobs, entropy, top_logprobs = (torch.empty(s, dtype=torch.float32, device=logits.device) for s in ((B, L), (B, L), (B, L, max(top, 0))))
     top_tokens = torch.empty((B, L, max(top, 0)), dtype=torch.int64, device=logits.device)
+    if B > 0 and L == 0 and 0 <= top <= min(V, 64):  # (a text of one token has none behind it)
+        return logprobs, entropy, top_tokens, top_logprobs
     ws = torch.empty(max(lib.llmops_token_logprobs_workspace_bytes(B, L, V, top), 1), dtype=torch.uint8, device=logits.device)
     _on_device(logits.device, lib.llmops_token_logprobs, zp, zb, zl, B, L, V, _ptr(tokens), tokens.stride(0) if B > 1 else 0, tokens.stride(1) if L > 1 else 0,
                top, _ptr(logprobs), _ptr(entropy), _ptr(top_tokens) if top > 0 else None, _ptr(top_logprobs) if top > 0 else None, _ptr(ws), ws.numel())

@@ -139,3 +139,4 @@ def test_scores(bits):
     assert (top_lp - want.gather(-1, top)).abs().max() <= 100 * 2.0 ** -24
     assert torch.equal(top[..., 0], logits[:, :-1].argmax(-1))
     assert model.score_requests(ids, caches[0])[2].shape == (3, 29, 0)
+    assert model.score_requests(_ids(5, 3, 1), caches[0], top=2)[3].shape == (3, 0, 2)

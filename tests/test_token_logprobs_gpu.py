@@ -146,6 +146,14 @@ def test_a_text_against_the_logits_before_each_token():
     _check(wide[:, ::3, 7:1010].transpose(0, 1), ids[:, ::3].T, 0)
 
 
+def test_a_text_of_one_token_has_none_behind_it():
+    logits, tokens = (x.cuda() for x in _case(3, 1, 50, 2))
+    lp, ent, ids, lps = llmops.token_logprobs(logits[:, :-1], tokens[:, 1:], 4)
+    assert lp.shape == ent.shape == (3, 0) and ids.shape == lps.shape == (3, 0, 4)
+    with pytest.raises(RuntimeError):
+        llmops.token_logprobs(logits[:, :-1], tokens[:, 1:], 51)
+
+
 def test_offsets_past_32_bits():
     V = 1 << 20
     logits = torch.zeros(2100, V, device="cuda")  # 8.8 GB

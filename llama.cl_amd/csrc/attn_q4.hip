@@ -304,7 +304,8 @@ struct Q4MeetSmem {
 // for when these are used up; the waves' sums meet in LDS.
 // Memory bounds it: a row's 80 bytes of K are read in 16-byte pieces by the lanes that multiply them, V's in words.  32 sequences of up to 4096 rows, 32 heads: 335 MB
 // in 74 us, 4.5 TB/s (a kernel that only reads them, in one order: 51 us; this one with its products taken out: 65); the vector ALU is busy half of
-// the time, mostly with making halves of codes.  100001 rows of 8 heads: 128 MB in 23 us, with 6 us of joining behind.  Not faster: copies to LDS by the DMA
+// the time, mostly with making halves of codes.  One sequence of 50000 rows, 8 kv heads: 64 MB
+// in 23 us, three or four times 128 rows to a workgroup, so that beginning and end are as long as the stream.  Not faster: copies to LDS by the DMA
 // engine, one or two stages ahead (87 us for the call, 87 and 93); waves' priorities by turn (91 to 97); more workgroups than the chip holds (87).
 template <int RT, bool WHOLE>
 __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(Q4Args a) {
@@ -663,7 +664,7 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
 // ---- 3. what several workgroups have of a query ----
 // A workgroup to a.join (1, 2, 4, 8) queries of a tile, 8 / a.join half waves to a query, each to as many records from the other, 16 bytes to a lane.  Latency: 5 us
 // with one or two records to a query, 6.2 with 128, 9.7 with 38400 queries (20 MB of records, 20 MB out).  Joined by the last workgroup to arrive
-// instead, records written through to memory: 32 sequences 90 us instead of 89, 64 with grouped heads 87.5 and 89.4, one of 100001 rows 41 and 32.
+// instead, records written through to memory: 32 sequences 90 us instead of 89, 64 with grouped heads 87.5 and 89.4, one of 50000 rows 41 and 32.
 __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
     __shared__ float stat[8][2];
     __shared__ float4 part[8][32];

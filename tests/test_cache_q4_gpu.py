@@ -136,6 +136,23 @@ def test_strides_and_shared_rows():
         _same(dev, want)
 
 
+@pytest.mark.parametrize("B", [12, 13, 40])
+def test_rows_that_many_sequences_share(B):
+    g = torch.Generator().manual_seed(B)
+    L, Hkv, maxlen = 50, 3, 70
+    k, v, own = (torch.randn(n, L, Hkv, 128, generator=g).half() for n in (1, 1, B))
+    lengths = torch.randint(-2, maxlen + 3, (B,), generator=g, dtype=torch.int32)
+    q_lens = torch.randint(-1, L + 2, (B,), generator=g, dtype=torch.int32)
+    kd, vd, ownd = k.cuda().expand(B, -1, -1, -1), v.cuda().expand(B, -1, -1, -1), own.cuda()
+    for lens in (None, q_lens):
+        for values, on in ((v.expand(B, -1, -1, -1), vd), (own, ownd)):  # (both in common; k alone)
+            want = np.full((2, B, Hkv, maxlen, 80), 3, np.int8)
+            ref.write(want, k.expand(B, -1, -1, -1).numpy(), values.numpy(), 0, lengths, lens, None)
+            dev = torch.full((2, B, Hkv, maxlen, 80), 3, dtype=torch.int8, device="cuda")
+            llmops.cache_write_q4(kd, on, dev, lengths.cuda(), 0, q_lens=None if lens is None else lens.cuda())
+            _same(dev, want)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 @pytest.mark.parametrize("planes,B,Hkv,maxlen,rows", [(2, 1, 1, 1, 1), (4, 3, 5, 33, 33), (2, 2, 32, 200, 7), (2, 67, 3, 20, 41)])
 def test_read_back(planes, B, Hkv, maxlen, rows, dtype):

@@ -339,11 +339,13 @@ class LlamaDecoder:
     def score_requests(self, input_ids, cache, q_lens=None, adapters=None, top=0):
         """What texts are worth to the model: ``forward_requests`` for the same arguments, then ``llmops.token_logprobs`` of each token behind the
         first against the logits of the one before it.  Returns its (logprobs [B, qL-1], entropy [B, qL-1], top_tokens, top_logprobs [B, qL-1,
-        top]); tokens behind a text's end (``q_lens``) have log probability 0.  exp(-sum / count) of the log probabilities is the perplexity."""
+        top]); tokens behind a text's end (``q_lens``), and those behind one that no longer fits the cache, have log probability 0.  exp(-sum / count)
+        of the log probabilities is the perplexity."""
         logits = self.forward_requests(input_ids, cache, q_lens, adapters)
-        behind = input_ids[:, 1:]
+        at = torch.arange(1, input_ids.shape[1], device=input_ids.device)
+        behind = input_ids[:, 1:].masked_fill(at > (cache.max_kv_len - cache.lengths)[:, None], -1)
         if q_lens is not None:
-            behind = behind.masked_fill(torch.arange(1, input_ids.shape[1], device=behind.device) >= q_lens[:, None], -1)
+            behind = behind.masked_fill(at >= q_lens[:, None], -1)
         return llmops.token_logprobs(logits[:, :-1], behind, top)
 
     def step_requests(self, tokens, cache, uniforms, drafts=None, draft_probs=None, draft_lens=None, temperature=None, adapters=None, top=None):
@@ -364,8 +366,9 @@ class LlamaDecoder:
         logits = self.forward_requests(ids, cache, q_lens, adapters)
         result, accepted = llmops.verify_drafts(logits, drafts, uniforms, draft_probs=draft_probs, temperature=temperature, draft_lens=q_lens - 1)
         result.masked_fill_((room <= 0)[:, None], -1)
+        answers = (result, accepted) if top is None else (result, accepted, llmops.token_logprobs(logits, result, top))
         cache.keep(accepted + 1)
-        return (result, accepted) if top is None else (result, accepted, llmops.token_logprobs(logits, result, top))
+        return answers
 
     def capture_decode(self, kv_cache, slot, position_id, stream=None):
         """Capture one decode step (batch 1, one token) as a HIP graph that serves every position: the token id,

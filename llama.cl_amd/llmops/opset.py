@@ -184,6 +184,8 @@ class Q4Cache(PrefixCache):
         planes, batch = self.cache.shape[:2]
         if full.dim() != 5 or full.shape[:3] != (planes, 1, self.cache.shape[2]) or full.shape[4] != 128 or not 0 <= rows <= min(full.shape[3], self.max_kv_len):
             raise ValueError("a cache of one sequence of the same layers and heads, and rows that both have")
+        if full.dtype not in (torch.float32, torch.float16) or full.device != self.cache.device:
+            raise ValueError("a cache in fp32 or fp16 on the same device")
         self.lengths.zero_()
         for i in range(planes // 2 if rows else 0):
             k, v = (full[2 * i + j, :, :, :rows].transpose(1, 2).expand(batch, -1, -1, -1) for j in (0, 1))
@@ -200,6 +202,8 @@ class Q4Cache(PrefixCache):
 
     def forget(self, sequence, length=0):
         """a sequence ends (or goes back to its first ``length`` rows behind its beginning)"""
+        if length < 0:
+            raise ValueError("length outside the cache")
         super().forget(sequence, self.begun + length)
 
     def attend(self, q, k, v, inv_freq, layer_id, q_lens=None):

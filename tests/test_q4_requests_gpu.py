@@ -140,3 +140,39 @@ def test_scores(bits):
     assert torch.equal(top[..., 0], logits[:, :-1].argmax(-1))
     assert model.score_requests(ids, caches[0])[2].shape == (3, 29, 0)
     assert model.score_requests(_ids(5, 3, 1), caches[0], top=2)[3].shape == (3, 0, 2)
+
+
+@pytest.mark.parametrize("bits", [None, 4])
+def test_texts_that_do_not_fit(bits):
+    model = LlamaDecoder(CFG, seed=8)
+    ids = _ids(6, 3, 20)
+    cache, wide = model.request_cache(3, 24, bits=bits), model.request_cache(3, 60, bits=bits)
+    for c in (cache, wide):
+        c.lengths.copy_(torch.tensor([0, 12, 24], dtype=torch.int32))
+    lp, want = model.score_requests(ids, cache)[0], model.score_requests(ids, wide)[0]
+    assert (lp[0] < 0).all() and (lp[0] - want[0]).abs().max() <= 5e-2 * want.abs().max()
+    # rows 12 .. 23 are left for 12 tokens, the last of which says what the next one is worth
+    # (caches of two capacities may add in different orders: codes of activations may flip, as above)
+    assert (lp[1, :12] < 0).all() and (lp[1, 12:] == 0).all() and (lp[1, :12] - want[1, :12]).abs().max() <= 5e-2 * want.abs().max()
+    assert (lp[2] == 0).all()
+
+
+def test_what_is_refused_changes_nothing():
+    model = LlamaDecoder(CFG, seed=9)
+    prefix = model.read_prefix(_ids(1, 1, 5), torch.float16)
+    cache = model.request_cache(2, 20, prefix, bits=4)
+    tokens, uniforms = _ids(2, 2), torch.full((2, 1), 0.5, device="cuda")
+    for top in (65, -1, CFG["vocab_size"] + 1):
+        with pytest.raises(RuntimeError):
+            model.step_requests(tokens, cache, uniforms, top=top)
+    for length in (-1, 21):
+        with pytest.raises(ValueError):
+            cache.forget(0, length)
+    for full in (prefix.bfloat16(), prefix.cpu(), prefix[:2], prefix[0], prefix.expand(-1, 2, -1, -1, -1)):
+        with pytest.raises(ValueError):
+            cache.begin(full)
+    with pytest.raises(ValueError):
+        cache.begin(prefix, 6)
+    assert cache.lengths.tolist() == [5, 5] and cache.begun == 5
+    cache.forget(1, 3)
+    assert cache.lengths.tolist() == [5, 8]

@@ -4,8 +4,8 @@
 //   entropy = - sum p_i log p_i = log S - (sum exp(z - M) (z - M)) / S,
 //   the likeliest `top` tokens in the order of their logits, equal ones in the order of their numbers.
 //
-//   1. logprob_runs_kernel   a run of a row to a workgroup, whose logits stay in registers: maximum, both sums, its likeliest tokens
-//   2. logprob_rows_kernel   joins a row's runs
+//   1. logprob_runs_kernel   a run of a row (up to 8192 logits) to a workgroup, whose logits stay in registers: maximum, both sums, its likeliest tokens
+//   2. logprob_rows_kernel or logprob_sums_kernel   joins a row's runs, if it has several
 //
 // The likeliest of a run: the `top`-th largest of the 64 lanes' own maxima is found in each wave bit by bit (a comparison and a count of lanes for each
 // bit, most of it on the scalar unit), and no logit below the largest of the four waves' can be among them; that leaves some 3 * top logits, of which each
@@ -74,21 +74,50 @@ __device__ __forceinline__ int count_all(int* sums, F is) {
     return all;
 }
 
+// A row's top, the logarithm of its sum, its entropy
+struct RowSums {
+    float M;
+    double log_s, entropy;
+};
+__device__ __forceinline__ RowSums row_sums_of(float M, double S, double T) {
+    const double log_s = M == -INFINITY ? NAN : log(S);
+    return {M, log_s, log_s - T / S};
+}
+__device__ __forceinline__ float logprob_of(const RowSums& s, float v) { return (float)((v == s.M ? 0.0 : (double)v - (double)s.M) - s.log_s); }
+// .. its token
+struct RowToken {
+    bool real = false;
+    float its = 0.0f;
+    __device__ __forceinline__ RowToken() {}
+    __device__ __forceinline__ RowToken(const LogprobArgs& a, int row) {
+        const int b = row / a.L, l = row - b * a.L;
+        const int64_t token = a.tokens[b * a.tsb + l * a.tsl];
+        real = token >= 0 && token < a.V;
+        its = real ? something(a.logits[b * a.lsb + l * a.lsl + token]) : 0.0f;
+    }
+    __device__ __forceinline__ void answer(const LogprobArgs& a, int row, const RowSums& s) const {
+        a.logprobs[row] = real ? logprob_of(s, its) : 0.0f, a.entropy[row] = (float)s.entropy;
+    }
+};
+
 // 32 logits to a thread: with fewer the reductions and the search weigh more, with more the registers of six workgroups to a compute unit do not suffice.
 // 2100 rows of 32003: 269 MB in 45 us, 6.0 TB/s.  With tokens to be found and all workgroups at work at once loads come first and arithmetic behind: 160 rows of
 // 55296, 35 MB, 15 us, of which memory takes 7 and the vector ALU, with 20 instructions a logit, 5.
-template <int E>
+template <int E, bool WHOLE>
 __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
     __shared__ float red[3][4];
     __shared__ int sums[4], count;
     __shared__ uint32_t bounds[4];
+    __shared__ RowSums row_of;
     __shared__ __align__(16) Held held[kHeld + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = blockIdx.x / a.runs, run = blockIdx.x - row * a.runs, b = row / a.L, l = row - b * a.L;
+    const int row = WHOLE ? blockIdx.x : blockIdx.x / a.runs, run = WHOLE ? 0 : blockIdx.x - row * a.runs, b = row / a.L, l = row - b * a.L;
     const float* z = a.logits + b * a.lsb + l * a.lsl;
     const buffer_rsrc r = make_rsrc(z, (uint32_t)a.V * 4u);
     const int base = run * 256 * E + 4 * threadIdx.x;
     float x[E];
+    RowToken token;
+    if (WHOLE && threadIdx.x == 192) token = RowToken(a, row);
 #pragma unroll
     for (int u = 0; u < E / 4; u++) {
         const float4 y = buf_ldf4(r, (uint32_t)(base + 1024 * u) * 4u, 0);
@@ -165,7 +194,16 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0) a.stat[(int64_t)row * a.runs + run] = make_float4(M, red[1][0] + red[1][1] + red[1][2] + red[1][3], red[2][0] + red[2][1] + red[2][2] + red[2][3], 0.0f);
+    const bool sums_thread = threadIdx.x == (WHOLE ? 192 : 0);  // (of a whole row: beside the other waves' comparisons)
+    if (sums_thread) {
+        const float all = red[1][0] + red[1][1] + red[1][2] + red[1][3], weighed = red[2][0] + red[2][1] + red[2][2] + red[2][3];
+        if constexpr (WHOLE) {
+            row_of = row_sums_of(M, all, weighed);
+            token.answer(a, row, row_of);
+        } else {
+            a.stat[(int64_t)row * a.runs + run] = make_float4(M, all, weighed, 0.0f);
+        }
+    }
     if (a.top == 0) return;
     if (count > kHeld) {  // (the same in all threads)
         uint32_t last = 0;
@@ -193,18 +231,16 @@ __global__ __launch_bounds__(256) void logprob_runs_kernel(LogprobArgs a) {
     const int n = count;
     if (threadIdx.x < 4) held[n + threadIdx.x] = nothing_held();
     __syncthreads();
-    const int64_t to = ((int64_t)row * a.runs + run) * a.top;
+    const int64_t to = (WHOLE ? (int64_t)row : (int64_t)row * a.runs + run) * a.top;
     for (int c = (int)threadIdx.x >> 2; c < n; c += 64) {
         const int before = how_many_ahead(held, n, held[c]);
-        if (before < a.top && (threadIdx.x & 3) == 0) a.best[to + before] = held[c];
+        if (before >= a.top || (threadIdx.x & 3) != 0) continue;
+        if constexpr (WHOLE) a.top_tokens[to + before] = held[c].at, a.top_logprobs[to + before] = logprob_of(row_of, of_key(held[c].key));
+        else a.best[to + before] = held[c];
     }
 }
 
-// A row's runs, in one wave: its top, its logarithm of the sum and its entropy
-struct RowSums {
-    float M;
-    double log_s, entropy;
-};
+// A row's runs, in one wave
 __device__ __forceinline__ RowSums row_sums(const LogprobArgs& a, int row, int lane) {
     const float4* stat = a.stat + (int64_t)row * a.runs;
     float4 s = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
@@ -222,17 +258,12 @@ __device__ __forceinline__ RowSums row_sums(const LogprobArgs& a, int row, int l
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) S += __shfl_xor(S, o, 64), T += __shfl_xor(T, o, 64);
-    const double log_s = M == -INFINITY ? NAN : log(S);
-    return {M, log_s, log_s - T / S};
+    return row_sums_of(M, S, T);
 }
-__device__ __forceinline__ float logprob_of(const RowSums& s, float v) { return (float)((v == s.M ? 0.0 : (double)v - (double)s.M) - s.log_s); }
 __device__ __forceinline__ void row_answers(const LogprobArgs& a, int row, int lane, RowSums& s) {
-    const int b = row / a.L, l = row - b * a.L;
-    const int64_t token = a.tokens[b * a.tsb + l * a.tsl];
-    const bool real = token >= 0 && token < a.V;
-    const float its = real ? something(a.logits[b * a.lsb + l * a.lsl + token]) : 0.0f;
+    const RowToken token(a, row);
     s = row_sums(a, row, lane);
-    if (lane == 0) a.logprobs[row] = real ? logprob_of(s, its) : 0.0f, a.entropy[row] = (float)s.entropy;
+    if (lane == 0) token.answer(a, row, s);
 }
 
 // without likeliest tokens: a wave to a row
@@ -331,9 +362,15 @@ extern "C" int llmops_token_logprobs(const float* logits, int64_t stride_b, int6
     a.stat = reinterpret_cast<float4*>(ws + w.stat), a.best = reinterpret_cast<Held*>(ws + w.best);
     a.logprobs = logprobs, a.entropy = entropy, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
     hipStream_t st = as_stream(stream);
-    const unsigned grid = (unsigned)(B * L * w.runs);
-    if (logprob_each(V) == 8) logprob_runs_kernel<8><<<grid, 256, 0, st>>>(a);
-    else logprob_runs_kernel<32><<<grid, 256, 0, st>>>(a);
+    // One launch where a run is a whole row (us with two launches and with one, 5 likeliest: a row of 1500 7.6 and 5.1, 32 of 6000 10.1 and 6.8, 2100 of 6000 23.5 and 17.8;
+    // a row of 9000 to 32768 to a workgroup of 1024 threads: 240 rows 10.9 to 13.8 and 9.7 to 10.7, with 20 likeliest 13.5 and 14.2, 960 rows 28 and 40)
+    if (w.runs == 1) {
+        if (V <= 2048) logprob_runs_kernel<8, true><<<(unsigned)(B * L), 256, 0, st>>>(a);
+        else logprob_runs_kernel<32, true><<<(unsigned)(B * L), 256, 0, st>>>(a);
+        LLMOPS_LAUNCH_CHECK();
+        return LLMOPS_OK;
+    }
+    logprob_runs_kernel<32, false><<<(unsigned)(B * L * w.runs), 256, 0, st>>>(a);
     LLMOPS_LAUNCH_CHECK();
     // (us in workgroups of 256, 512 and 1024: 2100 rows with 20 tokens of runs to compare 51 and 58, 160 rows with 140 19.5, 18.5 and 18.2, 32 rows with 320 28.2, 19.5 and 17.3)
     if (top > 0) logprob_rows_kernel<<<(unsigned)(B * L), w.runs * top <= 96 ? 256 : 1024, 0, st>>>(a);

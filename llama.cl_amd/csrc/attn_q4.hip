@@ -743,8 +743,12 @@ static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t max
     // One launch where a workgroup can have all rows of a kv head in the time of the two others' launches, or the chip is busy with one to each anyway;
     // not where so many queries and new rows wait for memory at once (us with three launches and with one: 2 sequences of 32 kv heads and 300 rows 14.8 and 9.8,
     // 1000 rows 16.5 and 14.3; 2 of 8 kv heads and 1500 rows 14.9 and 16.5; 16 of 32 and 500 rows 22.6 and 14.7, 1500 rows 30.5 and 24.4;
-    // 16 of 32 and 5 tokens, up to 2200 rows, 37.8 and 33.2; 32 of 32 and 1500 rows 44.4 and 44.3; 64 of 32 and 300 rows 35.1 and 39.1)
-    if (!p.many && items <= 1024 && maxlen <= (items >= 256 ? 16 : 8) * kUnit) {
+    // 16 of 32 and 5 tokens, up to 2200 rows, 37.8 and 33.2; 32 of 32 and 1500 rows 44.4 and 44.3; 64 of 32 and 300 rows 35.1 and 39.1).
+    // With more than 16 queries to a kv head a workgroup takes longer for its rows, and two fit a compute unit: (4 of 32 kv heads and 20 tokens, 300 rows 20.5 and 17.0, 700
+    // rows 24.4 and 22.9; 2 of 32 and 30 tokens, 1000 rows 23.6 and 27.1, 1 and 32 tokens, 100 rows 15.0 and 17.6; 1 of 8 and 8 tokens of 4 heads each, 400 rows 16.3 and 14.1, 1000
+    // 16.5 and 17.6; 40 of 8 and 8 tokens, 900 rows 34.3 and 30.7, 1500 37.5 and 41.0; 10 of 32 and 20 tokens, 900 rows 33.9 and 27.4; 20 of 32, 2000 rows 71.9 and 60.5)
+    const int one_launch = p.rt == 1 ? (items >= 256 ? 16 : 8) : items >= 512 ? 16 : items >= 256 ? 8 : qL <= 24 ? 4 : 0;  // units
+    if (!p.many && items <= 1024 && maxlen <= one_launch * kUnit) {
         p.groups = (int)items;
         return p;
     }

@@ -53,7 +53,8 @@ def _random(g, B, L, H, Hkv):
     (1, 1, 1, 1, 1), (1, 1, 32, 32, 2), (2, 1, 32, 32, 200), (3, 1, 8, 2, 1000), (1, 1, 8, 1, 5000), (5, 1, 16, 4, 129), (70, 1, 4, 2, 300), (130, 1, 2, 1, 40),
     (2, 5, 8, 8, 700), (3, 4, 16, 4, 140), (2, 3, 32, 2, 333), (4, 16, 4, 4, 64), (2, 17, 4, 4, 500), (1, 33, 8, 2, 257), (1, 7, 40, 1, 150), (2, 64, 4, 4, 400),
     (1, 300, 4, 1, 500), (3, 130, 2, 2, 131), (1, 257, 3, 3, 1300), (66, 20, 2, 2, 60),
-    (2, 1, 4, 4, 1024), (2, 1, 4, 4, 1025), (3, 6, 8, 2, 900), (2, 8, 16, 4, 1024)])
+    (2, 1, 4, 4, 1024), (2, 1, 4, 4, 1025), (3, 6, 8, 2, 900), (2, 8, 16, 4, 1024),
+    (1, 20, 4, 4, 512), (2, 24, 4, 4, 513), (1, 25, 2, 2, 400), (3, 5, 16, 4, 510)])
 def test_against_the_formula(B, L, H, Hkv, maxlen):
     g = torch.Generator().manual_seed(B * L + maxlen)
     q, k, v = _random(g, B, L, H, Hkv)
@@ -67,7 +68,8 @@ def test_against_the_formula(B, L, H, Hkv, maxlen):
 
 
 @pytest.mark.parametrize("B,L,H,Hkv,maxlen", [(64, 1, 32, 8, 3000), (130, 1, 8, 8, 1000), (40, 3, 16, 16, 1500), (70, 40, 8, 4, 700), (9, 150, 16, 8, 1200), (33, 20, 8, 8, 2500),
-                                              (16, 1, 32, 16, 2048), (17, 1, 16, 16, 2049), (32, 30, 8, 8, 2000), (33, 1, 32, 32, 300), (9, 5, 32, 32, 1500)])
+                                              (16, 1, 32, 16, 2048), (17, 1, 16, 16, 2049), (32, 30, 8, 8, 2000), (33, 1, 32, 32, 300), (9, 5, 32, 32, 1500),
+                                              (32, 30, 8, 8, 1000), (64, 20, 8, 8, 2000), (33, 8, 32, 8, 1024)])
 def test_the_chip_full_of_workgroups(B, L, H, Hkv, maxlen):
     """shares that differ, sequences past 64: against the formula in 64 bits on the device, over what the cache is read back as; tolerance as in q4_reference.py"""
     g = torch.Generator().manual_seed(B)

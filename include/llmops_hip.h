@@ -433,10 +433,10 @@ int llmops_imul(float* a, const float* b, int64_t rows, int64_t inner, int b_is_
 int llmops_itrans_silu(float* a, int64_t n, llmops_stream_t stream);
 /* embedding_q8c_quant_w (ops/op_embedding.hpp:51-78): w fp32 [V,E] -> q int8 [V,E], scales [V] */
 int llmops_embedding_q8c_quant_w(const float* w, int64_t V, int64_t E, int8_t* q, float* scales, llmops_stream_t stream);
-/* embedding_q8c (ops/op_embedding.hpp:108-137): out[i,:] = scales[ids[i]] * q[ids[i],:]; ids int64 */
+/* embedding_q8c (ops/op_embedding.hpp:108-137): out[i,:] = scales[ids[i]] * q[ids[i],:]; ids int64, zeros for one outside 0..V-1 */
 int llmops_embedding_q8c(float* out, const int64_t* ids, int64_t n, const int8_t* q, const float* scales,
                          int64_t V, int64_t E, llmops_stream_t stream);
-/* embedding (ops/op_embedding.hpp:24-49): out[i,:] = w[ids[i],:]; ids int64 */
+/* embedding (ops/op_embedding.hpp:24-49): out[i,:] = w[ids[i],:]; ids int64, zeros for one outside 0..V-1 */
 int llmops_embedding(float* out, const int64_t* ids, int64_t n, const float* w, int64_t V, int64_t E, llmops_stream_t stream);
 
 #ifdef __cplusplus

@@ -121,24 +121,27 @@ __global__ __launch_bounds__(256) void emb_quant_kernel(const float* __restrict_
     }
 }
 
-// embedding_q8c (ops/op_embedding.hpp:81-137): out[i,:] = scales[id] * q[id,:]
+// embedding_q8c (ops/op_embedding.hpp:81-137): out[i,:] = scales[id] * q[id,:].  Ids outside the table (texts of different
+// lengths are padded with -1) give zeros: they come from device memory, where nobody has looked at them.
 __global__ void emb_q8c_kernel(float* __restrict__ out, const int64_t* __restrict__ ids, const int8_t* __restrict__ q,
-                               const float* __restrict__ scales, int64_t E) {
+                               const float* __restrict__ scales, int64_t V, int64_t E) {
     const int64_t id = ids[blockIdx.x];
-    const float s = scales[id];
-    for (int64_t e = threadIdx.x; e < E; e += blockDim.x) out[(int64_t)blockIdx.x * E + e] = s * (float)q[id * E + e];
+    const bool real = id >= 0 && id < V;
+    const float s = real ? scales[id] : 0.0f;
+    for (int64_t e = threadIdx.x; e < E; e += blockDim.x) out[(int64_t)blockIdx.x * E + e] = real ? s * (float)q[id * E + e] : 0.0f;
 }
 
 // The same with E a multiple of 4 and 4-byte aligned rows: four codes per thread, blockIdx.y walks the row, so a
 // single token's row is one round of independent loads instead of a loop in one workgroup.
 __global__ __launch_bounds__(256) void emb_q8c_vec_kernel(float* __restrict__ out, const int64_t* __restrict__ ids,
                                                           const int8_t* __restrict__ q, const float* __restrict__ scales,
-                                                          int64_t E) {
+                                                          int64_t V, int64_t E) {
     const int64_t e = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
     if (e >= E) return;
     const int64_t id = ids[blockIdx.x];
-    const float s = scales[id];
-    const uint32_t c = *reinterpret_cast<const uint32_t*>(q + id * E + e);
+    const bool real = id >= 0 && id < V;
+    const float s = real ? scales[id] : 0.0f;
+    const uint32_t c = real ? *reinterpret_cast<const uint32_t*>(q + id * E + e) : 0u;
     float4 v;
     v.x = s * (float)(int8_t)(c & 0xFFu);
     v.y = s * (float)(int8_t)((c >> 8) & 0xFFu);
@@ -147,10 +150,11 @@ __global__ __launch_bounds__(256) void emb_q8c_vec_kernel(float* __restrict__ ou
     *reinterpret_cast<float4*>(out + (int64_t)blockIdx.x * E + e) = v;
 }
 
-// embedding (ops/op_embedding.hpp:24-49): out[i,:] = w[ids[i],:]
-__global__ void emb_kernel(float* __restrict__ out, const int64_t* __restrict__ ids, const float* __restrict__ w, int64_t E) {
+// embedding (ops/op_embedding.hpp:24-49): out[i,:] = w[ids[i],:], zeros for ids outside the table
+__global__ void emb_kernel(float* __restrict__ out, const int64_t* __restrict__ ids, const float* __restrict__ w, int64_t V, int64_t E) {
     const int64_t id = ids[blockIdx.x];
-    for (int64_t e = threadIdx.x; e < E; e += blockDim.x) out[(int64_t)blockIdx.x * E + e] = w[id * E + e];
+    const bool real = id >= 0 && id < V;
+    for (int64_t e = threadIdx.x; e < E; e += blockDim.x) out[(int64_t)blockIdx.x * E + e] = real ? w[id * E + e] : 0.0f;
 }
 
 }  // namespace llmops
@@ -262,22 +266,20 @@ extern "C" int llmops_embedding_q8c_quant_w(const float* w, int64_t V, int64_t E
 
 extern "C" int llmops_embedding_q8c(float* out, const int64_t* ids, int64_t n, const int8_t* q, const float* scales,
                                     int64_t V, int64_t E, llmops_stream_t stream) {
-    (void)V;
-    LLMOPS_REQUIRE(out != nullptr && ids != nullptr && q != nullptr && scales != nullptr && n > 0 && E > 0);
+    LLMOPS_REQUIRE(out != nullptr && ids != nullptr && q != nullptr && scales != nullptr && n > 0 && V > 0 && E > 0);
     LLMOPS_REQUIRE(n < ((int64_t)1 << 31));
     if ((E % 4) == 0 && aligned(q, 4) && aligned(out, 16) && (E + 1023) / 1024 < 65536)
-        emb_q8c_vec_kernel<<<dim3((unsigned)n, (unsigned)((E + 1023) / 1024)), 256, 0, as_stream(stream)>>>(out, ids, q, scales, E);
+        emb_q8c_vec_kernel<<<dim3((unsigned)n, (unsigned)((E + 1023) / 1024)), 256, 0, as_stream(stream)>>>(out, ids, q, scales, V, E);
     else
-        emb_q8c_kernel<<<(unsigned)n, 256, 0, as_stream(stream)>>>(out, ids, q, scales, E);
+        emb_q8c_kernel<<<(unsigned)n, 256, 0, as_stream(stream)>>>(out, ids, q, scales, V, E);
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }
 
 extern "C" int llmops_embedding(float* out, const int64_t* ids, int64_t n, const float* w, int64_t V, int64_t E,
                                 llmops_stream_t stream) {
-    (void)V;
-    LLMOPS_REQUIRE(out != nullptr && ids != nullptr && w != nullptr && n > 0 && E > 0 && n < ((int64_t)1 << 31));
-    emb_kernel<<<(unsigned)n, 256, 0, as_stream(stream)>>>(out, ids, w, E);
+    LLMOPS_REQUIRE(out != nullptr && ids != nullptr && w != nullptr && n > 0 && V > 0 && E > 0 && n < ((int64_t)1 << 31));
+    emb_kernel<<<(unsigned)n, 256, 0, as_stream(stream)>>>(out, ids, w, V, E);
     LLMOPS_LAUNCH_CHECK();
     return LLMOPS_OK;
 }

@@ -279,7 +279,8 @@ class LlamaDecoder:
 
     def forward_requests(self, input_ids, cache, q_lens=None, adapters=None):
         """Like ``forward`` for sequences that share ``cache``'s prefix: input_ids int64 [B, qL], the tokens behind those that each
-        sequence has kept (``cache.keep``).  q_lens int32 [B]: how many of the qL each brings; logits of the others mean nothing.
+        sequence has kept (``cache.keep``).  q_lens int32 [B]: how many of the qL each brings; the others may be any ids (-1 too), and their logits
+        mean nothing.
         adapters int32 [B]: each sequence's number for ``set_adapters``, -1 for none.  All of it is read on the device: a captured call
         serves following steps.  A sequence must have room for its tokens in the cache.  Returns logits fp32 [B, qL, vocab]."""
         hidden_states = self.embed_tokens(input_ids)

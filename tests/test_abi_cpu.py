@@ -286,3 +286,11 @@ def test_attention_planner_pieces_of_the_tiled_kernel(heads, tokens, past, piece
         kv = past + tokens
         assert lib.llmops_test_attn_plan(1, tokens, heads, kv, past, half, ctypes.byref(k), ctypes.byref(r), ctypes.byref(n)) == 0
         assert k.value == 3 and several in (None, n.value > 1) and r.value % 64 == 0 and (n.value - 1) * r.value < kv <= n.value * r.value
+
+
+def test_a_table_without_rows_is_refused(lib):
+    p = ctypes.c_void_p(4096)
+    lib.llmops_last_error.restype = ctypes.c_char_p
+    i64 = ctypes.c_int64
+    assert lib.llmops_embedding_q8c(p, p, i64(1), p, p, i64(0), i64(64), None) == 1 and b"V > 0" in lib.llmops_last_error()
+    assert lib.llmops_embedding(p, p, i64(1), p, i64(0), i64(64), None) == 1 and b"V > 0" in lib.llmops_last_error()

@@ -691,3 +691,23 @@ def test_decode_attention_with_more_than_65535_heads_in_all(ops, orc):
     assert np.abs(host(tk)[sel] - k_ref).max() <= 1e-5
     assert np.abs(host(tc)[:, sel] - cache_ref).max() <= 1e-5
     assert torch.isfinite(tq).all()
+
+
+@pytest.mark.parametrize("E", [4096, 5000, 30])
+def test_embedding_ids_outside_the_table(ops, orc, E):
+    """ids that no row belongs to (padding) give zeros and leave the others as they are, in every kernel of the lookup"""
+    V, outside = 12, np.array([-1, -100, 12, 13, 1 << 40, -(1 << 62), np.iinfo(np.int64).max, np.iinfo(np.int64).min])
+    rng = np.random.default_rng(E)
+    w = rng.standard_normal((V, E)).astype(np.float32)
+    real = rng.integers(0, V, size=len(outside))
+    real[:2] = 0, V - 1
+    ids = np.stack((real, outside), axis=1).reshape(1, -1).astype(np.int64)
+    q, s = orc.embedding_q8c_quant_w(w)
+    for n in (ids.shape[1], 1, 2):
+        out = dev(np.full((1, n, E), 7.0, np.float32))
+        ops.embedding_q8c(out, dev(ids[:, :n]), dev(q), dev(s))
+        got = host(out)
+        assert np.array_equal(got[:, ::2], orc.embedding_q8c(ids[:, :n:2], q, s)) and not got[:, 1::2].any()
+        ops.embedding(out, dev(ids[:, :n]), dev(w))
+        got = host(out)
+        assert np.array_equal(got[:, ::2], w[ids[:, :n:2]]) and not got[:, 1::2].any()

@@ -176,3 +176,21 @@ def test_what_is_refused_changes_nothing():
     assert cache.lengths.tolist() == [5, 5] and cache.begun == 5
     cache.forget(1, 3)
     assert cache.lengths.tolist() == [5, 8]
+
+
+@pytest.mark.parametrize("plan", ["fused", "reference"])
+@pytest.mark.parametrize("bits", [None, 4])
+def test_texts_padded_with_anything(bits, plan):
+    """what lies behind a text's end has no effect on it: ids that are no tokens give the bits that tokens give"""
+    model = LlamaDecoder(CFG, seed=10, plan=plan)
+    n = torch.tensor([20, 7, 1], dtype=torch.int32).cuda()
+    ids = _ids(7, 3, 20)
+    behind = torch.arange(20, device="cuda") >= n[:, None]
+    want = model.score_requests(ids, model.request_cache(3, 32, bits=bits), n, top=3)
+    for pad in (-1, -100, CFG["vocab_size"], 1 << 40):
+        got = model.score_requests(ids.masked_fill(behind, pad), model.request_cache(3, 32, bits=bits), n, top=3)
+        live = ~behind[:, 1:]
+        assert torch.equal(got[0], want[0])
+        assert all(torch.equal(a[live], b[live]) for a, b in zip(got[1:], want[1:]))
+        logits = model.forward_requests(ids.masked_fill(behind, pad), model.request_cache(3, 32, bits=bits), n)
+        assert logits.isfinite().all()

@@ -286,7 +286,7 @@ PyObject* call_write_q4(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     int64_t layer = 0;
     if (n != 7 || !THPVariable_CheckExact(args[0]) || !THPVariable_CheckExact(args[1]) || !q4_cache(args[2]) || !whole(args[4], layer) ||
-        !(args[5] == Py_None || plain(args[5], at::kFloat, 1)) || !direct())
+        !(args[5] == Py_None || (plain(args[5], at::kFloat, 1) && THPVariable_Unpack(args[5]).numel() > 0)) || !direct())
         return not_ordinary();
     const at::Tensor &c = THPVariable_Unpack(args[2]), &first = THPVariable_Unpack(args[0]);
     const int64_t B = c.size(1), Hkv = c.size(2), S = 128;

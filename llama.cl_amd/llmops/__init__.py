@@ -715,6 +715,7 @@ def cache_write_q4(k, v, kv_cache, lengths, layer_id, inv_freq=None, q_lens=None
     _q4_lengths(kv_cache, lengths, q_lens)
     if inv_freq is not None:
         _dev(inv_freq, torch.float32, 1, "inv_freq")
+        _require(inv_freq.shape[0] > 0, "inv_freq.size(0) > 0")  # (its address would be the null that stands for none)
     _here(kv_cache, k=k, v=v, lengths=lengths, inv_freq=inv_freq, q_lens=q_lens)
     _on_device(kv_cache.device, _lib.load().llmops_cache_write_q4, *at, _LORA_TYPES[k.dtype], B, k.shape[1], Hkv, 128,
                _ptr(inv_freq) if inv_freq is not None else None, inv_freq.shape[0] if inv_freq is not None else 0, _ptr(kv_cache), planes, maxlen, _ptr(lengths),

@@ -236,3 +236,17 @@ def test_refusals():
     for kw in (dict(kv_cache=cache.float()), dict(rows=-1), dict(dtype=torch.bfloat16), dict(starts=lengths[:1]), dict(starts=lengths.long())):
         with pytest.raises(RuntimeError):
             llmops.cache_read_q4(**{**dict(kv_cache=cache, rows=3), **kw})
+
+
+def test_frequencies_of_no_dims_are_refused():
+    """no frequencies are None: an empty tensor of them does not stand for rows that come rotated"""
+    cache, lengths, k = torch.full((2, 1, 4, 8, 80), 3, dtype=torch.int8, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"), torch.ones(1, 3, 512, device="cuda")
+    native = llmops._lib.host()
+    for host in (native, llmops._lib._PythonCalls()):
+        llmops._lib._host = host
+        try:
+            with pytest.raises(RuntimeError, match="inv_freq"):
+                llmops.cache_write_q4(k, k, cache, lengths, 0, inv_freq=torch.zeros(0, device="cuda"))
+        finally:
+            llmops._lib._host = native
+    assert (cache == 3).all()

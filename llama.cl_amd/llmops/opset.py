@@ -186,10 +186,16 @@ class Q4Cache(PrefixCache):
             raise ValueError("a cache of one sequence of the same layers and heads, and rows that both have")
         if full.dtype not in (torch.float32, torch.float16) or full.device != self.cache.device:
             raise ValueError("a cache in fp32 or fp16 on the same device")
-        self.lengths.zero_()
+        # what cache_write_q4 would refuse is refused before anything changes: its calls write layer after layer
+        e = full.element_size()
+        if rows and (full.stride(4) != 1 or full.data_ptr() % 16 or any(full.shape[d] > 1 and full.stride(d) * e % 16 for d in (0, 2, 3))):
+            raise ValueError("a cache with dense rows, each at 16 bytes")
+        if full.untyped_storage().data_ptr() == self.cache.untyped_storage().data_ptr():
+            raise ValueError("a cache in memory of its own")
+        at = torch.zeros_like(self.lengths)
         for i in range(planes // 2 if rows else 0):
             k, v = (full[2 * i + j, :, :, :rows].transpose(1, 2).expand(batch, -1, -1, -1) for j in (0, 1))
-            llmops.cache_write_q4(k, v, self.cache, self.lengths, i)
+            llmops.cache_write_q4(k, v, self.cache, at, i)
         self.begun = rows
         self.lengths.fill_(rows)
 

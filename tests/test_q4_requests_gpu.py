@@ -194,3 +194,34 @@ def test_texts_padded_with_anything(bits, plan):
         assert all(torch.equal(a[live], b[live]) for a, b in zip(got[1:], want[1:]))
         logits = model.forward_requests(ids.masked_fill(behind, pad), model.request_cache(3, 32, bits=bits), n)
         assert logits.isfinite().all()
+
+
+def test_a_beginning_that_is_refused_changes_nothing():
+    model = LlamaDecoder(CFG, seed=11)
+    prefix = model.read_prefix(_ids(1, 1, 6))
+    cache = model.request_cache(2, 20, prefix, bits=4)
+    cache.keep(3)
+    held = cache.cache.clone()
+    wide = torch.zeros(4, 1, 2, 6, 256, device="cuda")
+    flat = torch.zeros(prefix.numel() + 8192, device="cuda")
+    strides = prefix.stride()
+    inside = cache.cache.view(torch.float32).flatten()
+    for full in (wide[..., ::2],                                                        # rows that are not dense
+                 wide[..., 1:129],                                                      # an address between 16 bytes
+                 flat[2:2 + prefix.numel()].view(prefix.shape),                         # ..
+                 flat.as_strided(prefix.shape, (strides[0] + 2,) + strides[1:]),        # only later layers are
+                 flat.as_strided(prefix.shape, strides[:2] + (strides[2] + 1,) + strides[3:]), flat.as_strided(prefix.shape, strides[:3] + (130, 1)),
+                 flat.half().as_strided(prefix.shape, strides[:3] + (132, 1)),
+                 inside.as_strided(prefix.shape, (0, 0, 0, 128, 1), inside.numel() - 6 * 128)):   # the cache's own memory
+        with pytest.raises(ValueError):
+            cache.begin(full)
+        assert cache.begun == 6 and cache.lengths.tolist() == [9, 9] and torch.equal(cache.cache, held)
+    # strides of dims of one element, and rows that lie apart, are none of the refused
+    roomy = torch.zeros(4, 3, 2, 9, 128, device="cuda")[:, 1:2]
+    roomy[:, :, :, :6] = prefix
+    cache.begin(roomy, 6)
+    assert torch.equal(cache.cache[..., :6, :], held[..., :6, :]) and cache.lengths.tolist() == [6, 6]
+    cache.begin(prefix.as_strided(prefix.shape, (strides[0], 1) + strides[2:]), 6)
+    assert torch.equal(cache.cache[..., :6, :], held[..., :6, :])
+    cache.begin(prefix, 0)
+    assert cache.begun == 0 and cache.lengths.tolist() == [0, 0]

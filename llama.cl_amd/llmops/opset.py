@@ -167,7 +167,7 @@ class PrefixCache:
 class Q4Cache(PrefixCache):
     """KV cache of a batch in 4 bits (``llmops.attention_rope_q4``): 80 bytes for a token and head where fp32 takes 512 and fp16 256, on the device
     int8 [2*layers, batch, heads, max_kv_len, 80].  Each sequence has rows of its own from the first on; ``begin`` gives all of them
-    the same first rows, of a cache in full width (a system prompt that was read once), which ``forget`` keeps."""
+    the same first rows, of a cache in full width (a system prompt that was read once), which ``forget`` and ``keep`` leave."""
 
     def __init__(self, configs, batch_size, max_kv_len, device="cuda"):
         if configs["head_size"] != 128:
@@ -175,6 +175,8 @@ class Q4Cache(PrefixCache):
         self.prefix, self.prefix_len, self.begun = None, 0, 0
         self.cache = torch.zeros(configs["layer_num"] * 2, batch_size, configs["head_num"], max_kv_len, llmops.Q4_ROW_BYTES, dtype=torch.int8, device=device)
         self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        # what lengths are held to, on the device: a captured step holds them to the beginning that there is when it is replayed
+        self.least, self.most = (torch.full((), n, dtype=torch.int32, device=device) for n in (0, max_kv_len))
         self.max_kv_len = max_kv_len
 
     def begin(self, full, rows=None):
@@ -197,6 +199,7 @@ class Q4Cache(PrefixCache):
             k, v = (full[2 * i + j, :, :, :rows].transpose(1, 2).expand(batch, -1, -1, -1) for j in (0, 1))
             llmops.cache_write_q4(k, v, self.cache, at, i)
         self.begun = rows
+        self.least.fill_(rows)
         self.lengths.fill_(rows)
 
     def read(self, rows=None, starts=None, dtype=torch.float16):
@@ -205,6 +208,10 @@ class Q4Cache(PrefixCache):
 
     def size(self):
         return self.cache.numel()
+
+    def keep(self, tokens):
+        """as in ``PrefixCache``; a negative number takes rows back, of a sequence's own: its beginning stays"""
+        self.lengths.add_(tokens).clamp_(self.least, self.most)
 
     def forget(self, sequence, length=0):
         """a sequence ends (or goes back to its first ``length`` rows behind its beginning)"""

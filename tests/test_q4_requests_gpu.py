@@ -225,3 +225,39 @@ def test_a_beginning_that_is_refused_changes_nothing():
     assert torch.equal(cache.cache[..., :6, :], held[..., :6, :])
     cache.begin(prefix, 0)
     assert cache.begun == 0 and cache.lengths.tolist() == [0, 0]
+
+
+def test_tokens_taken_back_end_at_the_beginning():
+    model = LlamaDecoder(CFG, seed=12)
+    prefix = model.read_prefix(_ids(1, 1, 9))
+    cache = model.request_cache(3, 16, prefix, bits=4)
+    tokens = torch.tensor([5, 0, 16], dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            cache.keep(tokens)
+
+    def replay():
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+
+    cache.keep(tokens)
+    assert cache.lengths.tolist() == [14, 9, 25]
+    cache.keep(-7)
+    assert cache.lengths.tolist() == [9, 9, 18]
+    cache.keep(torch.tensor([-1, 3, -100], dtype=torch.int32, device="cuda"))
+    assert cache.lengths.tolist() == [9, 12, 9]
+    cache.keep(40)
+    assert cache.lengths.tolist() == [25, 25, 25]
+    # a captured step, behind other beginnings than the one that it was captured with
+    for rows in (9, 4, 0, 7):
+        cache.begin(prefix, rows)
+        replay()
+        assert cache.lengths.tolist() == [rows + 5, rows, rows + 16]
+        tokens.neg_(), replay()
+        assert cache.lengths.tolist() == [rows] * 3
+        tokens.neg_()
+    assert cache.begun == 7

@@ -374,7 +374,7 @@ int llmops_cache_read_q4(const void* kv_cache, int64_t planes, int64_t B, int64_
  * memory and little else (up to 2048 rows each kv head of a sequence may be one workgroup's).
  * Arithmetic: products of halves with fp32 sums, the cache's values exact, queries and weights in two halves (22 bits of a query beside its
  * head's largest value): results agree with fp32 evaluation to about 1e-6 of the largest output, and 2^-36 beside it, and are the same bits in every call.
- * B*qL*H < 2^24, and times ceil(maxlen/128) < 2^31. */
+ * B*qL*H < 2^24, maxlen <= 2^24, and B*Hkv*ceil(qL*(H/Hkv)/64) * (ceil(maxlen/128) + 1) < 2^31. */
 size_t llmops_attention_q4_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t maxlen);
 int llmops_attention_rope_q4(const float* q, int64_t q_stride_b, int64_t q_stride_l, const float* k, int64_t k_stride_b, int64_t k_stride_l,
                              const float* v, int64_t v_stride_b, int64_t v_stride_l, int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S,

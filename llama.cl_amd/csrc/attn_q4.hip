@@ -341,7 +341,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
         const int hk = (at - before) / its.head;
         int tile, units, u0;  // (one tile)
         tile_of(its, at - before - hk * its.head, tile, units, u0);
-        const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
+        const int u1 = min(units, u0 + (last - at)), real = units > kStart ? units - kStart : units;
         if (!WHOLE && (u0 == 0 || u1 >= real) && threadIdx.x == 0) {
             int2* parts = a.parts + ((int64_t)b * a.Hkv + hk) * a.tiles + tile;
             if (u0 == 0) parts->x = blockIdx.x;
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(256, 2) void q4_many_kernel(Q4Args a) {
         const int hk = (at - before) / its.head;
         int tile, units, u0;
         tile_of(its, at - before - hk * its.head, tile, units, u0);
-        const int u1 = min(units, u0 + last - at), real = units > kStart ? units - kStart : units;
+        const int u1 = min(units, u0 + (last - at)), real = units > kStart ? units - kStart : units;
         if ((u0 == 0 || u1 >= real) && threadIdx.x == 0) {
             int2* parts = a.parts + ((int64_t)b * a.Hkv + hk) * a.tiles + tile;
             if (u0 == 0) parts->x = blockIdx.x;
@@ -806,8 +806,10 @@ using namespace llmops;
 
 static bool q4_sizes_fit(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t maxlen) {
     const int64_t most = (int64_t)1 << 24;  // (a launch has fewer than 2^32 threads)
-    return B > 0 && qL > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && maxlen > 0 && B < most && qL < most && H < most && maxlen <= most && B * qL < most &&
-           B * qL * H < most && (Wide)B * H * qL * ((maxlen + kUnit - 1) / kUnit + kStart) < ((Wide)1 << 31);
+    if (!(B > 0 && qL > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && maxlen > 0 && B < most && qL < most && H < most && maxlen <= most && B * qL < most && B * qL * H < most)) return false;
+    // (units are numbered in 32 bits; of fewer than 64 queries there is one tile)
+    const int64_t tiles = (qL * (H / Hkv) + 63) / 64, units = (maxlen + kUnit - 1) / kUnit + kStart;
+    return (Wide)B * Hkv * tiles * units < ((Wide)1 << 31);
 }
 
 extern "C" size_t llmops_attention_q4_workspace_bytes(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t S, int64_t maxlen) {

@@ -269,3 +269,19 @@ def test_refusals():
             llmops.attention_rope_q4(**{**a, **kw})
     with pytest.raises(RuntimeError):  # rows that lie in the cache
         llmops.attention_rope_q4(**{**a, "k": cache.view(torch.float32).flatten().as_strided((2, 3, 512), (512, 0, 1))})
+
+
+def test_a_capacity_of_two_million_rows():
+    """a prompt of a few thousand tokens over a cache of 2^21 rows: as over a small one, bit for bit (work is shared out by the lengths)"""
+    g = torch.Generator().manual_seed(12)
+    L, H = 4096, 32
+    q, k, v = (x.cuda() for x in _random(g, 1, L, H, 1))
+    lengths, f = torch.tensor([10], dtype=torch.int32, device="cuda"), _inv_freq().cuda()
+    part = _filled(g, 2, 1, 1, L + 10).cuda()
+    cache = torch.zeros(2, 1, 1, 1 << 21, 80, dtype=torch.int8, device="cuda")
+    cache[..., :L + 10, :] = part
+    a, b = (llmops.attention_rope_q4(q, k, v, f, c, lengths, 0) for c in (cache, part))
+    assert torch.equal(a, b) and torch.equal(cache[..., :L + 10, :], part) and not cache[..., L + 10:, :].any()
+    lengths.fill_((1 << 21) - L)
+    out = llmops.attention_rope_q4(q[:, :5], k[:, :5], v[:, :5], f, cache, lengths, 0)
+    assert out.isfinite().all()

@@ -125,3 +125,16 @@ def test_python_functions_refuse_host_tensors():
                  lambda: llmops.attention_rope_q4(k, k, k, torch.ones(64), cache, lengths, 0), lambda: llmops.token_logprobs(torch.zeros(1, 1, 5), torch.zeros(1, 1, dtype=torch.int64))):
         with pytest.raises(RuntimeError, match="no CPU path|HIP device"):
             call()
+
+
+@pytest.mark.parametrize("B,qL,H,Hkv,maxlen,fits", [
+    (1, 100000, 32, 32, 100000, True), (1, 100000, 32, 8, 1 << 20, True),                       # long prompts: tiles of 64 queries count
+    (1, 4096, 32, 32, 16383 * 128, True), (1, 4096, 32, 1, 1 << 21, True),
+    (1 << 14, 1, 1, 1, 131070 * 128, True), (1 << 14, 1, 1, 1, 131070 * 128 + 1, False),        # 2^31 units less 2^14, and 2^31
+    (1 << 12, 64, 4, 4, 131070 * 128, True), (1 << 12, 65, 4, 4, 65535 * 128, False), (1 << 12, 65, 4, 4, 65534 * 128, True),
+    (1 << 23, 1, 1, 1, 254 * 128, True), (1 << 23, 1, 1, 1, 255 * 128, False), (1, 1 << 19, 32, 32, 1, False), (1, (1 << 19) - 1, 32, 32, 1, True)])
+def test_attention_sizes_that_fit(lib, B, qL, H, Hkv, maxlen, fits):
+    need = lib.llmops_attention_q4_workspace_bytes(B, qL, H, Hkv, 128, maxlen)
+    assert (need > 0) == fits
+    far = dict(B=B, qL=qL, H=H, Hkv=Hkv, maxlen=maxlen, out=ctypes.c_void_p(1 << 55), kv=ctypes.c_void_p(1 << 56), qb=0, ql=0, kb=0, kl=0, vb=0, vl=0)
+    _refused(lib, _attend(lib, bytes=0, **far), *((b"workspace bytes", 2) if fits else (b"q4_sizes_fit",)))

@@ -15,7 +15,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef unsigned short v2us __attribute__((ext_vector_type(2)));
 
 constexpr int kS = 128;
-constexpr float kLift = 14.0f;  // weights are exp2(.. + kLift)
+constexpr float kLift = 14.0f, kLifted = 16384.0f;  // weights are exp2(.. + kLift)
 
 // rows that sequence b has and new tokens that it brings; what does not fit the cache counts as padding
 __device__ __forceinline__ void own_extent(const int32_t* __restrict__ lengths, const int32_t* __restrict__ q_lens, int b, int qL, int64_t maxlen,
@@ -101,9 +101,11 @@ __device__ __forceinline__ float over_groups(float v) {
 }
 
 // scores (before the factor, which is positive) to weights: the running maximum, the sum, and what the sums so far shrink by.
-// sc[tt]: rows t + 16*tt + 4*g + v.  FAR: also scores so far from 0 that their products with the factor may not be left unrounded beside the
-// rounded maximum (from 2^31 on the weight of the maximum itself would be infinite)
-template <bool FAR = false, int RT, int N>
+// sc[tt]: rows t + 16*tt + 4*g + v.  With the lift in exp2's argument that is rounded between 8 and 16 for all weights that count, and they are off by
+// 2^-22 of themselves in the mean.  NEAR: lifted by a product of their own (an instruction for each), right to exp2's own unit beside the largest;
+// also scores so far from 0 that their products with the factor may not be left unrounded beside the rounded maximum (from 2^31 on the weight of
+// the maximum itself would be infinite)
+template <bool NEAR = false, int RT, int N>
 __device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[N], int t, int g, bool masked) {
     if (masked) {
 #pragma unroll
@@ -122,23 +124,24 @@ __device__ __forceinline__ void weigh(Queries<RT>& s, int rt, v4f (&sc)[N], int 
 #pragma unroll
         for (int c = 0; c < 8; c++) s.o[rt][c] *= shrink;
     }
-    if (FAR && __any(fabsf(s.m[rt]) > 0x1p20f && s.m[rt] != -INFINITY)) {
+    if (NEAR && __any(fabsf(s.m[rt]) > 0x1p20f && s.m[rt] != -INFINITY)) {
 #pragma unroll
         for (int tt = 0; tt < N; tt++)
 #pragma unroll
             for (int v = 0; v < 4; v++) {
                 const float x = sc[tt][v] * s.c[rt];
-                sc[tt][v] = __builtin_amdgcn_exp2f(s.m[rt] == -INFINITY ? x : (x - s.m[rt]) + kLift);
+                sc[tt][v] = __builtin_amdgcn_exp2f(s.m[rt] == -INFINITY ? x : x - s.m[rt]) * kLifted;
                 s.l[rt] += sc[tt][v];
             }
         return;
     }
-    const float base = s.m[rt] == -INFINITY ? 0.0f : kLift - s.m[rt];  // (nothing seen yet: every weight is exp2(-inf) = 0)
+    const float base = s.m[rt] == -INFINITY ? 0.0f : NEAR ? -s.m[rt] : kLift - s.m[rt];  // (nothing seen yet: every weight is exp2(-inf) = 0)
 #pragma unroll
     for (int tt = 0; tt < N; tt++)
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            sc[tt][v] = __builtin_amdgcn_exp2f(fmaf(sc[tt][v], s.c[rt], base));
+            const float w = __builtin_amdgcn_exp2f(fmaf(sc[tt][v], s.c[rt], base));
+            sc[tt][v] = NEAR ? w * kLifted : w;
             s.l[rt] += sc[tt][v];
         }
 }

@@ -285,3 +285,36 @@ def test_a_capacity_of_two_million_rows():
     lengths.fill_((1 << 21) - L)
     out = llmops.attention_rope_q4(q[:, :5], k[:, :5], v[:, :5], f, cache, lengths, 0)
     assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("B,L,H,Hkv,maxlen", [(40, 1, 4, 4, 100), (40, 1, 4, 4, 3000), (6, 1, 24, 1, 100), (6, 1, 24, 1, 5000), (6, 1, 40, 1, 100), (3, 4, 64, 1, 600)])
+def test_weights_near_the_largest_keep_their_bits(B, L, H, Hkv, maxlen):
+    """Rows whose scores lie within half a unit (of log2) of each other; out is their weights' ratios to the largest, times 15/16.  Nothing turns, and scores are
+    exact.  With e = 2^-24, roots of mean squares: a weight's two halves 1.75 e (a remainder below 2^-10 of it, cut to 11 bits), exp2 of at most one unit 1.15 e, the sum of
+    its two products and the product with 1 / sum 0.6 e; the largest one's 0.6, 0.6 and 0.5 e; the factor's 1.5 e of half a unit 0.5 e: 2.5 e in all, and a fifth for the sample.
+    (An argument of exp2 that is rounded between 8 and 16 would alone be off by 16 e / sqrt(12) log 2 = 3.2 e, here and at the largest.)"""
+    g = torch.Generator().manual_seed(B + H)
+    rows, e = 64, 2.0 ** -24
+    k, v = torch.zeros(B, rows, Hkv, 128), torch.zeros(B, rows, Hkv, 128)
+    k[..., 0] = torch.randint(-15, 16, (B, rows, Hkv), generator=g) / 8
+    k[..., 1] = torch.randint(-7, 8, (B, rows, Hkv), generator=g) / 64
+    v[:, torch.arange(rows), :, torch.arange(rows)] = 15 / 16
+    cache, f = torch.zeros(2, B, Hkv, maxlen, 80, dtype=torch.int8, device="cuda"), torch.zeros(64, device="cuda")
+    none = torch.zeros(B, dtype=torch.int32, device="cuda")
+    llmops.cache_write_q4(k.cuda(), v.cuda(), cache, none, 0, inv_freq=f)
+    K, V = llmops.cache_read_q4(cache, rows).double()
+    assert torch.equal(V.cpu().float(), v.transpose(1, 2))
+    q = torch.zeros(B, L, H, 128)
+    q[..., :2] = torch.randint(1024, 2048, (B, L, H, 1), generator=g) / 1024
+    first = rows - L
+    new = [x[:, first:].flatten(2).cuda() for x in (k, v)]
+    out = llmops.attention_rope_q4(q.flatten(2).cuda(), *new, f, cache, none + first, 0).double().unflatten(-1, (Hkv, H // Hkv, 128))
+    off = []
+    for l in range(L):
+        n = first + l + 1
+        s = torch.matmul(q[:, l].double().cuda().reshape(B, Hkv, -1, 128), K[:, :, :n].transpose(2, 3).contiguous()) / math.sqrt(128)
+        near = s - s.amax(-1, keepdim=True)
+        got = out[:, l, ..., :n] / out[:, l, ..., :n].gather(-1, s.argmax(-1, keepdim=True))
+        off.append((got / near.exp() - 1)[(near > -0.5 * math.log(2)) & (near < 0)])
+    off = torch.cat(off)
+    assert len(off) > 2000 and float(off.square().mean().sqrt()) <= 3 * e

@@ -188,3 +188,27 @@ def test_refusals():
               (logits[..., ::2], tokens, 0), (logits.cpu(), tokens, 0), (logits, tokens.cpu(), 0), (logits[0], tokens, 0), (logits[:0], tokens[:0], 0)):
         with pytest.raises(RuntimeError):
             llmops.token_logprobs(*a)
+
+
+def test_rows_further_apart_than_32_bits():
+    """strides that take later rows past 2^31 elements from the first, for rows of many runs and of one"""
+    far = torch.zeros(2100, 1 << 20, device="cuda")  # 8.8 GB
+    far[2050, 777] = 5.0
+    far[2091, 4000] = 3.0
+    for logits, V in ((far[None, ::41], 1 << 20), (far[None, ::41, :5000], 5000), (far[::41, None, :20001], 20001)):
+        shape = logits.shape[:2]
+        tokens = torch.full(shape, 777, device="cuda")
+        for top in (0, 2):
+            lp, ent, ids, lps = llmops.token_logprobs(logits, tokens, top)
+            lp, ent, ids, lps = lp.flatten(), ent.flatten(), ids.reshape(52, top), lps.reshape(52, top)
+            for row, z in ((49, 0.0), (50, 5.0), (51, 0.0)):  # (logits of 777; the last row has 3 elsewhere)
+                highest = (0.0, 5.0, 3.0)[row - 49]
+                log_s = math.log(V - 1 + math.exp(highest))
+                # p * distance from the top: at most that distance
+                assert abs(float(lp[row]) - (z - log_s)) <= (2 * highest + 42 + 14) * E
+                p = math.exp(highest - log_s)
+                want = log_s - p * highest
+                assert abs(float(ent[row]) - want) <= (2 * highest + 42 + 14 + highest * (2 * highest + 43) + highest * (2 * highest + 42)) * E
+            if top:
+                assert ids[49].tolist() == [0, 1] and ids[50].tolist() == [777, 0] and ids[51].tolist() == [4000, 0]
+                assert abs(float(lps[50, 0] - lp[50])) == 0.0

@@ -318,3 +318,27 @@ def test_weights_near_the_largest_keep_their_bits(B, L, H, Hkv, maxlen):
         off.append((got / near.exp() - 1)[(near > -0.5 * math.log(2)) & (near < 0)])
     off = torch.cat(off)
     assert len(off) > 2000 and float(off.square().mean().sqrt()) <= 3 * e
+
+
+@pytest.mark.parametrize("L,H,Hkv,maxlen", [(1, 16, 4, 500), (1, 16, 4, 3000), (5, 4, 4, 700), (20, 4, 4, 300), (24, 4, 4, 4000), (40, 8, 4, 700), (70, 4, 2, 3000)])
+def test_rows_behind_a_sequence_may_hold_anything(L, H, Hkv, maxlen):
+    """the same bits whatever the rest of the capacity, and the rows that the call writes, held before: NaN, infinities, any bytes.  In one launch and three"""
+    g = torch.Generator().manual_seed(L + maxlen)
+    B, f = 5, _inv_freq().cuda()
+    q, k, v = (x.cuda() for x in _random(g, B, L, H, Hkv))
+    cache = _filled(g, 2, B, Hkv, maxlen)
+    lengths, q_lens = torch.tensor([0, 31, 128, maxlen // 2 + 1, maxlen - L], dtype=torch.int32), torch.tensor([L, 1, L, max(L - 3, 0), L], dtype=torch.int32)
+    held = torch.arange(maxlen) < lengths[:, None]
+    written = (torch.arange(maxlen) < (lengths + q_lens)[:, None])[None, :, None, :, None].expand(2, -1, Hkv, -1, 80)
+    fill = [torch.zeros_like(cache), torch.randint(-128, 128, cache.shape, generator=g, dtype=torch.int8)]
+    for bad in (math.nan, math.inf, -math.inf, 65504.0):
+        fill.append(torch.randint(-128, 128, cache.shape, generator=g, dtype=torch.int8))
+        fill[-1][..., 64:] = torch.full((8,), bad, dtype=torch.float16).view(torch.int8)
+    got = []
+    for other in fill:
+        dev = torch.where(held[None, :, None, :, None], cache, other).cuda()
+        out = llmops.attention_rope_q4(q, k, v, f, dev, lengths.cuda(), 0, q_lens=q_lens.cuda())
+        got.append((out, dev.cpu()))
+        assert out.isfinite().all() and torch.equal(got[-1][1][~written], other[~written])  # (what is behind stays as it is)
+    for out, dev in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(dev[written], got[0][1][written])

@@ -250,3 +250,18 @@ def test_frequencies_of_no_dims_are_refused():
         finally:
             llmops._lib._host = native
     assert (cache == 3).all()
+
+
+@pytest.mark.parametrize("offset,spread", [(0.0, 1.0), (1000.0, 0.5), (-60000.0, 100.0), (3.0, 1e-3), (1e-4, 1e-6), (2.0 ** -14, 2.0 ** -20), (0.0, 2.0 ** -22), (-7.0, 0.0)])
+def test_how_far_a_value_may_be_off(offset, spread):
+    """With u the group's unit: levels lie s <= range / (15 u) + 1 units apart, and the ends half a unit inside at most, so that a value is off by at most (range / 15 + u) / 2;
+    u is at most a 1016th of the largest magnitude, or 2^-24.  A group whose values have much in common is off by the second part."""
+    g = torch.Generator().manual_seed(13)
+    x = offset + spread * torch.randn(300, 128, generator=g)
+    back = llmops.cache_read_q4(_write_one(x), 300, dtype=torch.float32)[0, 0, 0].cpu().double().reshape(300, 4, 32)
+    t = x.double().reshape(300, 4, 32)
+    span, most = t.amax(-1) - t.amin(-1), t.abs().amax(-1)
+    off = (back - t).abs().amax(-1)
+    assert (off <= span / 30 + torch.clamp(most / 2032, min=2.0 ** -25)).all()
+    if offset == 1000.0:  # (a thirtieth of the range alone is no bound)
+        assert float((off / span).max()) > 0.1

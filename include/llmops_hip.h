@@ -356,7 +356,9 @@ int llmops_verify_drafts(const float* logits, int64_t B, int64_t K, int64_t V, c
  * 2*layer_id+1 (v).  k and v are of `dtype` (LLMOPS_F32, _F16), head h of token l of sequence b at + b*stride_b + l*stride_l + h*stride_h elements
  * (multiples of 16 bytes; 0 where rows are the same), unchanged.  With inv_freq [half] k is rotated by its row's number first, as
  * llmops_rope_embed with angles, rotation and codes in 64 bits; NULL: k comes rotated.  lengths, q_lens, and tokens that do not fit: as llmops_attention_rope_prefix.
- * The caller adds to lengths[b] what is to be kept.  kv_cache 16-byte aligned; k, v, lengths, q_lens or inv_freq over the two planes are refused. */
+ * The caller adds to lengths[b] what is to be kept.  kv_cache 16-byte aligned; k, v, lengths, q_lens or inv_freq over the two planes are refused.
+ * maxlen <= 2^24; B*qL*ceil(Hkv/8) < 2^24 with inv_freq, 2*Hkv*ceil(qL/16) < 2^24 without (times B, unless all sequences are given the
+ * same rows), and B*qL*Hkv < 2^39. */
 int llmops_cache_write_q4(const void* k, int64_t k_stride_b, int64_t k_stride_l, int64_t k_stride_h, const void* v, int64_t v_stride_b,
                           int64_t v_stride_l, int64_t v_stride_h, int dtype, int64_t B, int64_t qL, int64_t Hkv, int64_t S, const float* inv_freq,
                           int64_t half, void* kv_cache, int64_t planes, int64_t maxlen, const int32_t* lengths, const int32_t* q_lens, int layer_id,
@@ -364,7 +366,7 @@ int llmops_cache_write_q4(const void* k, int64_t k_stride_b, int64_t k_stride_l,
 
 /* The values that rows starts[b] .. starts[b] + rows - 1 (starts int32 [B] on the device, NULL: from 0) of every plane, sequence and head of a cache in
  * 4 bits stand for -> out [planes,B,Hkv,rows,S] of `dtype` (LLMOPS_F32, _F16: exact in both).  Rows outside the cache give 0.  An out over the cache or
- * starts is refused.  planes*B*Hkv*rows below 2^28. */
+ * starts is refused.  planes*B*Hkv*rows at most 2^28 - 16, rows and maxlen at most 2^24. */
 int llmops_cache_read_q4(const void* kv_cache, int64_t planes, int64_t B, int64_t Hkv, int64_t maxlen, int64_t S, const int32_t* starts, int64_t rows,
                          void* out, int dtype, llmops_stream_t stream);
 

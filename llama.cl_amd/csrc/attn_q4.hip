@@ -70,7 +70,7 @@ __device__ __forceinline__ const float* new_row_at(const Q4Args& a, bool is_k, i
 // A workgroup per token and 16 of its H + 2*Hkv rows of 128, sixteen lanes to a row.  By itself and not in the workgroups of step 2: many of these share a
 // query and each would turn it again (4 turns of 300 tokens: step 2 takes 62 us as it is, 73 with that).
 // Latency with few tokens (32 of 96 rows 5.0 us: the length, the row and the frequency in one round trip, the sincos in 64 bits, the codes), memory with many
-// (1200 tokens, 29 MB in from the memory side, 26 out, 18 us; two or three rows one behind the other to sixteen lanes: the same).
+// (1200 tokens, 59 MB in, padding's rows among them, and 21 out, 18 us, 4.4 TB/s; two or three rows one behind the other to sixteen lanes: the same).
 __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Args a) {
     __shared__ double2 turn[64];
     const int bl = blockIdx.x / a.row_groups, group = blockIdx.x - bl * a.row_groups, b = bl / a.qL, l = bl - b * a.qL;
@@ -743,10 +743,12 @@ static Q4Plan plan_q4(int64_t B, int64_t qL, int64_t H, int64_t Hkv, int64_t max
     // One launch where a workgroup can have all rows of a kv head in the time of the two others' launches, or the chip is busy with one to each anyway;
     // not where so many queries and new rows wait for memory at once (us with three launches and with one: 2 sequences of 32 kv heads and 300 rows 14.8 and 9.8,
     // 1000 rows 16.5 and 14.3; 2 of 8 kv heads and 1500 rows 14.9 and 16.5; 16 of 32 and 500 rows 22.6 and 14.7, 1500 rows 30.5 and 24.4;
-    // 16 of 32 and 5 tokens, up to 2200 rows, 37.8 and 33.2; 32 of 32 and 1500 rows 44.4 and 44.3; 64 of 32 and 300 rows 35.1 and 39.1).
+    // 16 of 32 and 1 token, up to 2200 rows, 36.0 and 31.6, 5 tokens 37.8 and 33.2; 24 of 32 and 2200 rows 45.1 and 45.6; 40 of 8 and 2200 rows 32.3 and 33.6, 100 of 8 52.2 and 58.5;
+    // 32 of 32 and 1500 rows 44.4 and 44.3; 64 of 32 and 300 rows 35.1 and 39.1).  Above 2048 rows some numbers of sequences gain and others lose: those stay with three.
     // With more than 16 queries to a kv head a workgroup takes longer for its rows, and two fit a compute unit: (4 of 32 kv heads and 20 tokens, 300 rows 20.5 and 17.0, 700
     // rows 24.4 and 22.9; 2 of 32 and 30 tokens, 1000 rows 23.6 and 27.1, 1 and 32 tokens, 100 rows 15.0 and 17.6; 1 of 8 and 8 tokens of 4 heads each, 400 rows 16.3 and 14.1, 1000
     // 16.5 and 17.6; 40 of 8 and 8 tokens, 900 rows 34.3 and 30.7, 1500 37.5 and 41.0; 10 of 32 and 20 tokens, 900 rows 33.9 and 27.4; 20 of 32, 2000 rows 71.9 and 60.5)
+    // (there by tokens, not queries: new rows and angles are by token, and a workgroup has those of its kv head all to itself)
     const int one_launch = p.rt == 1 ? (items >= 256 ? 16 : 8) : items >= 512 ? 16 : items >= 256 ? 8 : qL <= 24 ? 4 : 0;  // units
     if (!p.many && items <= 1024 && maxlen <= one_launch * kUnit) {
         p.groups = (int)items;

@@ -363,7 +363,8 @@ extern "C" int llmops_token_logprobs(const float* logits, int64_t stride_b, int6
     a.logprobs = logprobs, a.entropy = entropy, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
     hipStream_t st = as_stream(stream);
     // One launch where a run is a whole row (us with two launches and with one, 5 likeliest: a row of 1500 7.6 and 5.1, 32 of 6000 10.1 and 6.8, 2100 of 6000 23.5 and 17.8;
-    // a row of 9000 to 32768 to a workgroup of 1024 threads: 240 rows 10.9 to 13.8 and 9.7 to 10.7, with 20 likeliest 13.5 and 14.2, 960 rows 28 and 40)
+    // longer rows, of 9000 to 32768, to a workgroup of 1024 threads gain with 240 rows and 5 likeliest, 10.9 to 13.8 and 9.7 to 10.7, and lose with 20, 13.5 and 14.2, and with
+    // 960 rows, 28 and 40: they stay with two)
     if (w.runs == 1) {
         if (V <= 2048) logprob_runs_kernel<8, true><<<(unsigned)(B * L), 256, 0, st>>>(a);
         else logprob_runs_kernel<32, true><<<(unsigned)(B * L), 256, 0, st>>>(a);

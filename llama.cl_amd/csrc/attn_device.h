@@ -12,7 +12,6 @@ namespace llmops {
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef unsigned short v2us __attribute__((ext_vector_type(2)));
 
 constexpr int kS = 128;
 constexpr float kLift = 14.0f, kLifted = 16384.0f;  // weights are exp2(.. + kLift)
@@ -25,30 +24,17 @@ __device__ __forceinline__ void own_extent(const int32_t* __restrict__ lengths, 
     n = (int)max((int64_t)0, min((int64_t)want, maxlen - len));
 }
 
-// cos and sin of inv_freq * pos: the product is exact in 64 bits, and so reduced to [-pi, pi] there (in fp32 it is off by 1.2e-4 at position
-// 4000, by up to 0.5 at 2^23); what its rounding to fp32 leaves out is put back to first order, 2^-24 being all that it can be
-__device__ __forceinline__ void turn_of(float f, int pos, float& c, float& s) {
-    const double angle = (double)f * (double)pos, whole = rint(angle * 0.15915494309189535);
-    const double rest = fma(-whole, 2.4492935982947064e-16, fma(-whole, 6.283185307179586, angle));  // 2 pi in two parts
-    const float hi = (float)rest, lo = (float)(rest - (double)hi);
-    float s0, c0;
-    sincosf(hi, &s0, &c0);
-    c = fmaf(-lo, s0, c0);
-    s = fmaf(lo, c0, s0);
-}
-
-// 8 * N values of a rotated query as halves, in their order, and its factor.  top: the largest magnitude of all of the query's; bad: it holds an infinity or NaN
-template <int N>
-__device__ __forceinline__ float halves_of(const float (&x)[8 * N], float top, bool bad, bool live, v8h (&hi)[N], v8h (&lo)[N]) {
+// eight values of a rotated query as halves, in their order, and its factor.  top: the largest magnitude of all of the query's; bad: it holds an infinity or NaN
+__device__ __forceinline__ float halves_of(const float (&x)[8], float top, bool bad, bool live, v8h& hi, v8h& lo) {
     const bool use = live && !bad && top > 0.0f;
     // (2^123 at most: the factor stays a normal number.  It would lose its bits below 2^-126, and at 0 make NaN of a masked score's -inf)
     const int e2 = use ? min(123, 13 - ilogbf(top)) : 0;
 #pragma unroll
-    for (int e = 0; e < 8 * N; e++) {
+    for (int e = 0; e < 8; e++) {
         const float y = use ? ldexpf(x[e], e2) : 0.0f;
         const _Float16 h = (_Float16)y;
-        hi[e >> 3][e & 7] = h;
-        lo[e >> 3][e & 7] = (_Float16)(y - (float)h);
+        hi[e] = h;
+        lo[e] = (_Float16)(y - (float)h);
     }
     // (a query that holds an infinity or NaN has no score that is a number)
     return live && bad ? NAN : ldexpf(1.44269504f * 0.08838834764831845f, -e2);
@@ -65,9 +51,9 @@ __device__ __forceinline__ QueryRow query_row(const float (&x)[8], bool live) {
     float bad = fine ? 0.0f : 1.0f;
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64)), bad = fmaxf(bad, __shfl_xor(bad, o, 64));
-    v8h h[1], l[1];
+    v8h h, l;
     const float c = halves_of(x, top, bad != 0.0f, live, h, l);
-    return {__builtin_bit_cast(uint4, h[0]), __builtin_bit_cast(uint4, l[0]), c};
+    return {__builtin_bit_cast(uint4, h), __builtin_bit_cast(uint4, l), c};
 }
 
 __device__ __forceinline__ v8h as_v8h(uint4 u) { return *reinterpret_cast<const v8h*>(&u); }
@@ -174,21 +160,4 @@ __device__ __forceinline__ uint32_t unseen(uint32_t x) {
 __device__ __forceinline__ uint4 ask16(buffer_rsrc r, uint32_t lane_at, uint32_t at) {
     return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_at + at, 0, 0));
 }
-__device__ __forceinline__ uint2 ask8(buffer_rsrc r, uint32_t lane_at, uint32_t at) {
-    return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_at + at, 0, 0));
-}
-
-// Item `at` of groups * each: the items of a group, which read the same rows, follow each other on one XCD (consecutive workgroups go to
-// the eight in turn), so that its L2 serves all but the first
-__device__ __forceinline__ void item_of(unsigned at, unsigned groups, unsigned each, int& group, int& sub) {
-    const unsigned whole = groups & ~7u;
-    if (at < whole * each) {
-        const unsigned eight = at / (8 * each), in = at - eight * 8 * each;
-        group = (int)(eight * 8 + (in & 7)), sub = (int)(in >> 3);
-    } else {
-        const unsigned in = at - whole * each;
-        group = (int)(whole + in / each), sub = (int)(in % each);
-    }
-}
-
 }  // namespace llmops

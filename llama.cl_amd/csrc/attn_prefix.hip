@@ -30,6 +30,8 @@
 
 namespace llmops {
 
+typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+
 struct PrefixArgs {
     _Float16 *qh, *ql;                  // [Hkv][M][128]
     float* cq;                          // [Hkv][M]: score = cq * (q' . k), in units of log2
@@ -47,6 +49,18 @@ struct PrefixArgs {
 };
 
 // ---- 1. rotation, cache rows, operands ----
+// cos and sin of inv_freq * pos: the product is exact in 64 bits, and so reduced to [-pi, pi] there (in fp32 it is off by 1.2e-4 at position
+// 4000, by up to 0.5 at 2^23); what its rounding to fp32 leaves out is put back to first order, 2^-24 being all that it can be
+__device__ __forceinline__ void turn_of(float f, int pos, float& c, float& s) {
+    const double angle = (double)f * (double)pos, whole = rint(angle * 0.15915494309189535);
+    const double rest = fma(-whole, 2.4492935982947064e-16, fma(-whole, 6.283185307179586, angle));  // 2 pi in two parts
+    const float hi = (float)rest, lo = (float)(rest - (double)hi);
+    float s0, c0;
+    sincosf(hi, &s0, &c0);
+    c = fmaf(-lo, s0, c0);
+    s = fmaf(lo, c0, s0);
+}
+
 __device__ __forceinline__ void store_row4(float* dst, const float* v) { *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void store_row4(__half* dst, const float* v) {
     const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
@@ -360,6 +374,10 @@ struct MeetSmem {
         } in;
     };
 };
+
+__device__ __forceinline__ uint2 ask8(buffer_rsrc r, uint32_t lane_at, uint32_t at) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_at + at, 0, 0));
+}
 
 template <typename T>
 struct RowRegs;
@@ -824,6 +842,19 @@ __device__ __forceinline__ void many_queries(const PrefixArgs& a, int hk, int m0
             for (int v = 0; v < 4; v++)
                 leave(a, hk, m, piece, 64 * h + 16 * g + 4 * v, make_float4(s.o[rt][4 * h][v], s.o[rt][4 * h + 1][v], s.o[rt][4 * h + 2][v], s.o[rt][4 * h + 3][v]),
                       s.l[rt], see[rt] > 0);
+    }
+}
+
+// Item `at` of groups * each: the items of a group, which read the same rows, follow each other on one XCD (consecutive workgroups go to
+// the eight in turn), so that its L2 serves all but the first
+__device__ __forceinline__ void item_of(unsigned at, unsigned groups, unsigned each, int& group, int& sub) {
+    const unsigned whole = groups & ~7u;
+    if (at < whole * each) {
+        const unsigned eight = at / (8 * each), in = at - eight * 8 * each;
+        group = (int)(eight * 8 + (in & 7)), sub = (int)(in >> 3);
+    } else {
+        const unsigned in = at - whole * each;
+        group = (int)(whole + in / each), sub = (int)(in % each);
     }
 }
 

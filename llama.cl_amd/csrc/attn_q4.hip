@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256, RT == 1 && !WHOLE ? 4 : 2) void q4_few_kernel(
 // order of the operands (a read is 16 bytes to a lane, in lane order); two buffers: while a tile is multiplied the next one's values are formed and the one
 // behind it is on its way from memory.
 // Instructions bound it, and what two waves to a SIMD leave uncovered: 4 turns of 300 tokens behind up to 1777 rows, 32 heads, 61 us, of which the vector ALU is
-// busy 21, the matrix cores 12 and LDS reads, 32 KB to a wave and tile of 64 rows, 12; waves wait for data 28 % of the time and for a turn to issue 36 %.  Not faster: 128 queries to four
+// busy 22, the matrix cores 12 and LDS reads, 32 KB to a wave and tile of 64 rows, 12; waves wait for data 28 % of the time and for a turn to issue 36 %.  Not faster: 128 queries to four
 // waves (fewer workgroups than places, twice the registers), 128 to eight waves (the call 104 us instead of 86; 2048 tokens of one sequence, 194 instead of 211),
 // one buffer and three workgroups to a compute unit (85 instead of 83).
 struct Q4TileSmem {

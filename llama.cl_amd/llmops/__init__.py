@@ -904,6 +904,7 @@ def embedding_q8c(output, input, weight, scales):
     _dev(output, torch.float32, None, "output")
     ids = _ids(input)
     V, E = weight.shape
+    _require(scales.shape[0] == V, "scales.size(0) == weight.size(0)")
     _require(tuple(output.shape) == tuple(input.shape) + (E,), "infer_shape() == output.shape()")
     _lib.check(_lib.load().llmops_embedding_q8c(_ptr(output), _ptr(ids), ids.numel(), _ptr(weight), _ptr(scales), V, E,
                                                _stream(output)))

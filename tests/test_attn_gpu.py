@@ -711,3 +711,10 @@ def test_embedding_ids_outside_the_table(ops, orc, E):
         ops.embedding(out, dev(ids[:, :n]), dev(w))
         got = host(out)
         assert np.array_equal(got[:, ::2], w[ids[:, :n:2]]) and not got[:, 1::2].any()
+
+
+def test_embedding_scales_of_another_table_are_refused(ops):
+    q, ids, out = dev(np.zeros((12, 64), np.int8)), dev(np.zeros((1, 2), np.int64)), ops.empty(1, 2, 64)
+    for rows in (0, 1, 11, 13):
+        with pytest.raises(RuntimeError):
+            ops.embedding_q8c(out, ids, q, dev(np.zeros(rows, np.float32)))

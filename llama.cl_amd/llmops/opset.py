@@ -190,7 +190,7 @@ class Q4Cache(PrefixCache):
             raise ValueError("a cache in fp32 or fp16 on the same device")
         # what cache_write_q4 would refuse is refused before anything changes: its calls write layer after layer
         e = full.element_size()
-        if rows and (full.stride(4) != 1 or full.data_ptr() % 16 or any(full.shape[d] > 1 and full.stride(d) * e % 16 for d in (0, 2, 3))):
+        if rows and (full.stride(4) != 1 or full.data_ptr() % 16 or any(n > 1 and full.stride(d) * e % 16 for d, n in ((0, planes), (2, full.shape[2]), (3, rows)))):
             raise ValueError("a cache with dense rows, each at 16 bytes")
         if full.untyped_storage().data_ptr() == self.cache.untyped_storage().data_ptr():
             raise ValueError("a cache in memory of its own")

@@ -223,6 +223,8 @@ def test_a_beginning_that_is_refused_changes_nothing():
     assert torch.equal(cache.cache[..., :6, :], held[..., :6, :]) and cache.lengths.tolist() == [6, 6]
     cache.begin(prefix.as_strided(prefix.shape, (strides[0], 1) + strides[2:]), 6)
     assert torch.equal(cache.cache[..., :6, :], held[..., :6, :])
+    cache.begin(flat.as_strided(prefix.shape, strides[:3] + (130, 1)), 1)
+    assert cache.begun == 1 and cache.lengths.tolist() == [1, 1] and not cache.read(1).any()
     cache.begin(prefix, 0)
     assert cache.begun == 0 and cache.lengths.tolist() == [0, 0]
 
